@@ -452,6 +452,47 @@ int grm_hip_fuse_residual(const void* h_online, const void* retrieved, const flo
                           const void* ln_weight, const void* ln_bias, void* out, int64_t rows,
                           int64_t routes, int64_t hidden_size, int dtype, float eps, void* stream);
 
+/*
+ * Short causal depthwise convolution.  No counterpart in the reference.
+ *   pre_t = bias + sum_w weight[:, w] x_{t - width + 1 + w};  out_t = silu ? silu(pre_t) : pre_t
+ * x:         [batch, seq_len, channels]; rows of `channels` packed elements, x_batch_stride and
+ *            x_token_stride elements apart, so a slice of a wider projection is read in place.
+ * weight:    [channels, width], bias [channels] or NULL, both in weight_dtype: x's dtype or float32.
+ * state:     [batch, width - 1, channels] in x's dtype, the rows before token 0; NULL: zeros.
+ * lengths:   NULL, or int64 [batch] (device), clamped to [0, seq_len]: tokens from lengths[b] on are
+ *            not read and their rows of out are zeros.
+ * out:       [batch, seq_len, channels], contiguous.
+ * state_out: [batch, width - 1, channels], the last width - 1 rows of (state, x) before the
+ *            length.  Required; may not overlap state.
+ * Float32 arithmetic.  Limits: width 2 to 4, channels >= 1.
+ */
+int grm_hip_short_conv_fwd(const void* x, const void* weight, const void* bias, const void* state,
+                           const int64_t* lengths, void* out, void* state_out, int64_t batch, int64_t seq_len,
+                           int64_t channels, int64_t width, int64_t x_batch_stride, int64_t x_token_stride, int dtype,
+                           int weight_dtype, int silu, void* stream);
+
+/*
+ * Gradients of grm_hip_short_conv_fwd.  grad_out [batch, seq_len, channels] and grad_state_out
+ * [batch, width - 1, channels] are contiguous, either may be NULL (zeros).  grad_x is contiguous;
+ * grad_bias and grad_state may be NULL.  The weights' sums are taken in a fixed order (no atomics).
+ * Workspace: grm_hip_short_conv_bwd_workspace() bytes.
+ */
+int64_t grm_hip_short_conv_bwd_workspace(int64_t batch, int64_t seq_len, int64_t channels, int64_t width, int dtype);
+int grm_hip_short_conv_bwd(const void* x, const void* weight, const void* bias, const void* state,
+                           const int64_t* lengths, const void* grad_out, const void* grad_state_out, void* grad_x,
+                           void* grad_weight, void* grad_bias, void* grad_state, void* workspace,
+                           int64_t workspace_bytes, int64_t batch, int64_t seq_len, int64_t channels, int64_t width,
+                           int64_t x_batch_stride, int64_t x_token_stride, int dtype, int weight_dtype, int silu,
+                           void* stream);
+
+/*
+ * One token of grm_hip_short_conv_fwd: x and out [batch, channels], state_out the state moved by
+ * that token.  state_out may be state itself (updated in place), but not overlap it otherwise.
+ */
+int grm_hip_short_conv_step(const void* x, const void* weight, const void* bias, const void* state, void* out,
+                            void* state_out, int64_t batch, int64_t channels, int64_t width, int64_t x_batch_stride,
+                            int dtype, int weight_dtype, int silu, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

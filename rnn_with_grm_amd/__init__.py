@@ -17,6 +17,10 @@ from .cuda_ops import (  # noqa: F401
     cuda_fuse_residual,
     cuda_gather_apply,
     cuda_segment_scan,
+    cuda_selective_scan,
+    cuda_selective_step,
+    cuda_short_conv,
+    cuda_short_conv_step,
     cuda_topk_route,
     get_grm_cuda_runtime_status,
     is_grm_cpp_extension_available,
@@ -34,6 +38,10 @@ __all__ = [
     "cuda_fuse_residual",
     "cuda_gather_apply",
     "cuda_segment_scan",
+    "cuda_selective_scan",
+    "cuda_selective_step",
+    "cuda_short_conv",
+    "cuda_short_conv_step",
     "cuda_topk_route",
     "get_grm_cuda_runtime_status",
     "is_grm_cpp_extension_available",

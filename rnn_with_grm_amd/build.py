@@ -30,8 +30,8 @@ LIB_EXT = PKG_DIR / "grm_cuda_ext.so"
 OFFLOAD_ARCH = "gfx950"
 HIP_SOURCES = ["grm_capi.hip", "chunk_scan.hip", "chunk_scan_wide.hip", "chunk_scan_vsplit.hip", "chunk_scan_par.hip",
                "chunk_bwd.hip", "chunk_bwd_f32.hip", "gather_apply.hip", "retrieve.hip", "retrieve_window.hip",
-               "route_fuse.hip", "route_select.hip", "layer_glue.hip"]
-EXT_SOURCE = "grm_torch_ops.cpp"
+               "route_fuse.hip", "route_select.hip", "layer_glue.hip", "short_conv.hip"]
+EXT_SOURCES = ["grm_torch_ops.cpp", "grm_selective_ops.cpp"]
 
 # Packed fp32 instructions are kept out of every kernel (the flag is for the
 # device pass; the host pass warns that it does not know it, harmlessly).
@@ -106,21 +106,25 @@ def build_torch_extension(force: bool = True, verbose: bool = False) -> Path:
     from torch.utils import cpp_extension
 
     BUILD_DIR.mkdir(exist_ok=True)
-    src = CSRC / EXT_SOURCE
-    if not force and not _stale(LIB_EXT, [src, LIB_HIP] + _headers()):
+    if not force and not _stale(LIB_EXT, [CSRC / s for s in EXT_SOURCES] + [LIB_HIP] + _headers()):
         return LIB_EXT
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     incs = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], str(INCLUDE), f"{rocm}/include"]
     torch_lib = cpp_extension.library_paths()[0]
-    obj = BUILD_DIR / "grm_torch_ops.o"
     cxx = os.environ.get("CXX", "g++")
-    _run([cxx, "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-          f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=grm_cuda_ext",
-          "-DTORCH_API_INCLUDE_EXTENSION_H", *[f"-I{i}" for i in incs], "-c", str(src), "-o", str(obj)],
-         verbose)
+    objs, todo = [], []
+    for name in EXT_SOURCES:
+        src, obj = CSRC / name, BUILD_DIR / (Path(name).stem + ".o")
+        objs.append(str(obj))
+        if force or _stale(obj, [src] + _headers()):
+            todo.append([cxx, "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+                         f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=grm_cuda_ext",
+                         "-DTORCH_API_INCLUDE_EXTENSION_H", *[f"-I{i}" for i in incs], "-c", str(src), "-o", str(obj)])
+    with ThreadPoolExecutor(max_workers=len(EXT_SOURCES)) as pool:
+        list(pool.map(lambda c: _run(c, verbose), todo))
     tmp = LIB_EXT.with_suffix(".so.tmp")
-    _run([cxx, "-shared", "-o", str(tmp), str(obj), f"-L{PKG_DIR}", "-lgrm_hip", f"-L{torch_lib}",
+    _run([cxx, "-shared", "-o", str(tmp), *objs, f"-L{PKG_DIR}", "-lgrm_hip", f"-L{torch_lib}",
           "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python",
           "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"], verbose)
     os.replace(tmp, LIB_EXT)

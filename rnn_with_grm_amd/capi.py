@@ -58,6 +58,11 @@ SIGNATURES = {
     "grm_hip_topk_route": (_C, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _C, _I, ctypes.c_float, ctypes.c_float, _P]),
     "grm_hip_segment_route": (_C, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _C, _I, _I, _I, _I, ctypes.c_float,
                                    ctypes.c_float, _P]),
+    "grm_hip_short_conv_fwd": (_C, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _C, _C, _C, _P]),
+    "grm_hip_short_conv_bwd_workspace": (_I, [_I, _I, _I, _I, _C]),
+    "grm_hip_short_conv_bwd": (_C, [_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _C,
+                                    _C, _C, _P]),
+    "grm_hip_short_conv_step": (_C, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _C, _C, _C, _P]),
     "grm_hip_fuse_residual": (_C, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _C, ctypes.c_float, _P]),
 }
 

@@ -16,7 +16,9 @@ Deliberate differences:
     64-token chunk as ``aux``; the backward reads it instead of re-running the
     scan (the schema allows it, bindings.cpp:6-7; the reference's aux is empty).
   * New entry points: ``cuda_segment_scan``, ``cuda_topk_route``,
-    ``cuda_segment_route``, ``cuda_gather_apply`` and ``cuda_fuse_residual``.
+    ``cuda_segment_route``, ``cuda_gather_apply`` and ``cuda_fuse_residual``; the
+    selective state scan and its short convolution (``cuda_selective_scan``,
+    ``cuda_selective_step``, ``cuda_short_conv``, ``cuda_short_conv_step``).
 """
 
 from __future__ import annotations
@@ -40,7 +42,8 @@ SCHEMA_OPS = (
 EXTRA_OPS = ("segment_scan_forward", "topk_route", "fuse_residual", "gather_apply", "segment_route",
              "retrieve_fuse", "project_split", "residual_layer_norm", "gather_apply_backward_queries",
              "gather_apply_backward_tokens", "apply_query_backward_queries", "archive_cast", "project_gemm",
-             "linear_residual_layer_norm", "segment_retrieve_fuse")
+             "linear_residual_layer_norm", "segment_retrieve_fuse", "selective_scan_forward", "selective_scan_backward",
+             "selective_step", "short_conv_forward", "short_conv_backward", "short_conv_step")
 
 # Environment variables of the reference (cuda_ops.py:26-32): one per op and a global one.
 GLOBAL_POLICY_ENV = "GRM_CUDA_KERNEL_POLICY"
@@ -830,6 +833,270 @@ def cuda_linear_residual_layer_norm(x: Tensor, weight: Tensor, bias: Optional[Te
     return torch.nn.functional.layer_norm(y + residual, (y.size(-1),), ln_weight, ln_bias, eps)
 
 
+# ---------------------------------------------------------------------------
+# Selective state scan and its short causal convolution.  The reference has neither; the scan is the
+# linear memory above with a decay and a write strength that each token chooses per head.
+
+def _wants_grad(*tensors: Optional[Tensor]) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _live_tokens(lengths: Optional[Tensor], batch: int, seq_len: int, device) -> Optional[Tensor]:
+    """[B, T] bool, the tokens before each sequence's length; None without lengths."""
+    if lengths is None:
+        return None
+    if lengths.shape != (batch,) or lengths.dtype not in (torch.int32, torch.int64):
+        raise ValueError("lengths must be int32 or int64 [batch]")
+    return torch.arange(seq_len, device=device) < lengths.clamp(0, seq_len)[:, None]
+
+
+def _silu_flag(activation: Optional[str]) -> bool:
+    if activation not in (None, "silu"):
+        raise ValueError(f"activation must be None or 'silu', got {activation!r}")
+    return activation == "silu"
+
+
+def _torch_short_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor], state: Optional[Tensor],
+                      lengths: Optional[Tensor], silu: bool) -> Tuple[Tensor, Tensor]:
+    if x.ndim != 3 or weight.ndim != 2 or weight.size(0) != x.size(2):
+        raise ValueError("short_conv: x must be [batch, seq_len, channels] and weight [channels, width]")
+    B, T, C = x.shape
+    W = weight.size(1)
+    if C < 1 or not 2 <= W <= 4:
+        raise ValueError(f"short_conv: needs channels >= 1 and width 2, 3 or 4, got width {W}")
+    if weight.dtype not in (x.dtype, torch.float32):
+        raise ValueError("short_conv: weight must have x's type or be float32")
+    if bias is not None and (bias.shape != (C,) or bias.dtype != weight.dtype):
+        raise ValueError("short_conv: bias must be [channels] in weight's type")
+    if state is not None and (state.shape != (B, W - 1, C) or state.dtype != x.dtype):
+        raise ValueError("short_conv: state must be [batch, width - 1, channels] in x's type")
+    live = _live_tokens(lengths, B, T, x.device)
+    cdt = torch.float64 if x.dtype == torch.float64 else torch.float32
+    xf, wf = x.to(cdt), weight.to(cdt)
+    if live is not None:
+        xf = xf.masked_fill(~live[..., None], 0.0)
+    before = xf.new_zeros(B, W - 1, C) if state is None else state.to(cdt)
+    full = torch.cat([before, xf], 1)
+    pre = sum(full[:, w:w + T] * wf[:, w] for w in range(W))
+    if bias is not None:
+        pre = pre + bias.to(cdt)
+    out = torch.nn.functional.silu(pre) if silu else pre
+    if live is None:
+        return out.to(x.dtype), full[:, T:].to(x.dtype)
+    rows = lengths.clamp(0, T).long()[:, None] + torch.arange(W - 1, device=x.device)
+    last = full.gather(1, rows[..., None].expand(B, W - 1, C))
+    return out.masked_fill(~live[..., None], 0.0).to(x.dtype), last.to(x.dtype)
+
+
+class _ShortConvFn(torch.autograd.Function):
+    """The convolution's inputs are all that its backward needs: it forms the sums before the
+    activation again, as cheap as reading them back."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, state, lengths, silu: bool):
+        ctx.silu = silu
+        ctx.save_for_backward(x, weight, bias, state, lengths)
+        ctx.set_materialize_grads(False)
+        return torch.ops.grm_cuda.short_conv_forward(x, weight, bias, state, lengths, silu)
+
+    @staticmethod
+    def backward(ctx, grad_out, grad_state_out):
+        x, weight, bias, state, lengths = ctx.saved_tensors
+        dx, dw, db, ds = torch.ops.grm_cuda.short_conv_backward(grad_out, grad_state_out, x, weight, bias, state,
+                                                                lengths, ctx.silu)
+        return dx, dw, None if bias is None else db, None if state is None else ds, None, None
+
+
+def cuda_short_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, state: Optional[Tensor] = None, *,
+                    activation: Optional[str] = None, lengths: Optional[Tensor] = None, enabled: bool = True,
+                    debug_fallback: bool = False) -> Tuple[Tensor, Tensor]:
+    """Causal depthwise convolution over the last ``width`` (2 to 4) tokens of every channel:
+    ``out_t = act(bias + sum_w weight[:, w] x_{t - width + 1 + w})``, ``activation`` None or "silu".
+
+    x [B, T, C] (float32, float16 or bfloat16; rows of C packed elements, e.g. a slice of a wider
+    projection, are read in place), weight [C, width] and bias [C] in x's type or float32, state
+    [B, width - 1, C] the rows before token 0 (None: zeros), lengths [B] the tokens of each sequence
+    of a padded batch (clamped to [0, T]; the rows behind are not read and come out as zeros).
+    Returns (out [B, T, C], state_out [B, width - 1, C]: the rows that the next call starts from).
+    Differentiable in x, weight, bias and state."""
+    silu = _silu_flag(activation)
+    if x.is_cuda and _run_native("short_conv", x.device, enabled=enabled, debug_fallback=debug_fallback):
+        if _wants_grad(x, weight, bias, state):
+            return _ShortConvFn.apply(x, weight, bias, state, lengths, silu)
+        return torch.ops.grm_cuda.short_conv_forward(x, weight, bias, state, lengths, silu)
+    return _torch_short_conv(x, weight, bias, state, lengths, silu)
+
+
+def _check_out(out: Optional[Tensor], like: Tensor, name: str, grad: bool) -> None:
+    if out is None:
+        return
+    if grad:
+        raise ValueError(f"{name} cannot be given where gradients are wanted")
+    if out.shape != like.shape or out.dtype != like.dtype or not out.is_contiguous():
+        raise ValueError(f"{name} must be contiguous and match its input in shape and type")
+
+
+def cuda_short_conv_step(x: Tensor, state: Tensor, weight: Tensor, bias: Optional[Tensor] = None, *,
+                         activation: Optional[str] = None, state_out: Optional[Tensor] = None,
+                         enabled: bool = True, debug_fallback: bool = False) -> Tuple[Tensor, Tensor]:
+    """One token of ``cuda_short_conv``: x [B, C], state [B, width - 1, C].  Returns (out [B, C], the
+    state moved by this token).  ``state_out`` takes that state; with ``state_out=state`` it is
+    updated in place, as a serving loop or a captured graph keeps it."""
+    silu = _silu_flag(activation)
+    grad = _wants_grad(x, state, weight, bias)
+    if state_out is not None:
+        _check_out(state_out, state, "state_out", grad)
+    if not grad and x.is_cuda and _run_native("short_conv", x.device, enabled=enabled,
+                                              debug_fallback=debug_fallback):
+        if state_out is None:
+            state_out = torch.empty_like(state, memory_format=torch.contiguous_format)
+        return torch.ops.grm_cuda.short_conv_step(x, state, weight, bias, silu, state_out), state_out
+    if x.ndim != 2:
+        raise ValueError("short_conv_step: x must be [batch, channels]")
+    out, moved = cuda_short_conv(x[:, None], weight, bias, state, activation=activation, enabled=enabled,
+                                 debug_fallback=debug_fallback)
+    return out[:, 0], moved if state_out is None else state_out.copy_(moved)
+
+
+def _check_selective(keys: Tensor, values: Tensor, queries: Tensor, steps: Tensor, rates: Tensor,
+                     memory: Optional[Tensor], skip: Optional[Tensor], step_bias: Optional[Tensor]) -> None:
+    if keys.ndim != 4 or values.ndim != 4 or steps.ndim != 3:
+        raise ValueError("selective_scan: keys and queries must be [batch, seq_len, groups, key_dim], values "
+                         "[batch, seq_len, heads, value_dim] and steps [batch, seq_len, heads]")
+    B, T, H, P = values.shape
+    G, N = keys.shape[2:]
+    if queries.shape != keys.shape or keys.shape[:2] != (B, T) or steps.shape != (B, T, H):
+        raise ValueError("selective_scan: keys, queries, values and steps must agree in batch, length and heads")
+    if G < 1 or H < 1 or P < 1 or H % G != 0 or not 1 <= N <= 128:
+        raise ValueError("selective_scan: heads must be a multiple of groups and key_dim in [1, 128]")
+    if not keys.dtype == values.dtype == queries.dtype or steps.dtype not in (values.dtype, torch.float32):
+        raise ValueError("selective_scan: keys, values and queries must share a type, steps have it or float32")
+    for name, t in (("rates", rates), ("skip", skip), ("step_bias", step_bias)):
+        if t is not None and t.shape != (H,):
+            raise ValueError(f"selective_scan: {name} must be [heads]")
+    if memory is not None and memory.shape != (B, H, P, N):
+        raise ValueError("selective_scan: memory must be [batch, heads, value_dim, key_dim]")
+
+
+def _torch_selective_scan(keys: Tensor, values: Tensor, queries: Tensor, steps: Tensor, rates: Tensor,
+                          memory: Optional[Tensor], skip: Optional[Tensor], step_bias: Optional[Tensor],
+                          lengths: Optional[Tensor], softplus: bool) -> Tuple[Tensor, Tensor]:
+    """Closed form of 64 tokens at a time in float32 (float64 for float64 inputs); log decays are
+    summed in float64, whose differences stay exact where a chunk's sum is large."""
+    _check_selective(keys, values, queries, steps, rates, memory, skip, step_bias)
+    B, T, H, P = values.shape
+    G, N = keys.shape[2:]
+    cdt = torch.float64 if values.dtype == torch.float64 else torch.float32
+    state = values.new_zeros(B, H, P, N, dtype=cdt) if memory is None else memory.to(cdt)
+    d = steps.to(cdt) if step_bias is None else steps.to(cdt) + step_bias.to(cdt)
+    if softplus:
+        d = torch.nn.functional.softplus(d)
+    x, k, q = values.to(cdt), keys.to(cdt), queries.to(cdt)
+    live = _live_tokens(lengths, B, T, values.device)
+    if live is not None:
+        d = d.masked_fill(~live[..., None], 0.0)
+        x, k, q = (t.masked_fill(~live[..., None, None], 0.0) for t in (x, k, q))
+    xh = x.transpose(1, 2)                                            # [B, H, T, P]
+    kh, qh = (t.transpose(1, 2).repeat_interleave(H // G, 1) for t in (k, q))
+    dh = d.transpose(1, 2)                                            # [B, H, T]
+    outs = []
+    for t0 in range(0, T, 64):
+        part = slice(t0, min(t0 + 64, T))
+        xc, kc, qc, dc = xh[:, :, part], kh[:, :, part], qh[:, :, part], dh[:, :, part]
+        n = xc.size(2)
+        cum = (dc.double() * rates.double()[:, None]).cumsum(-1)
+        lower = torch.ones(n, n, dtype=torch.bool, device=x.device).tril()
+        decay = torch.exp((cum[..., :, None] - cum[..., None, :]).masked_fill(~lower, -math.inf)).to(cdt)
+        within = torch.matmul(torch.matmul(qc, kc.transpose(-1, -2)) * decay * dc[..., None, :], xc)
+        outs.append(within + torch.exp(cum).to(cdt)[..., None] * torch.matmul(qc, state.transpose(-1, -2)))
+        tail = torch.exp(cum[..., -1:] - cum).to(cdt) * dc
+        state = (torch.exp(cum[..., -1]).to(cdt)[..., None, None] * state +
+                 torch.matmul((xc * tail[..., None]).transpose(-1, -2), kc))
+    hidden = torch.cat(outs, 2).transpose(1, 2) if outs else x.new_zeros(B, 0, H, P)
+    if skip is not None:
+        hidden = hidden + skip.to(cdt)[:, None] * x
+    return hidden.to(values.dtype), state
+
+
+class _SelectiveScanFn(torch.autograd.Function):
+    """The scan; where gradients are wanted the forward also keeps the float32 state at the start of
+    every chunk of the backward, which then runs all chunks side by side."""
+
+    @staticmethod
+    def forward(ctx, keys, values, queries, steps, rates, memory, skip, step_bias, lengths, softplus: bool):
+        hidden, memory_out, states = torch.ops.grm_cuda.selective_scan_forward(
+            keys, values, queries, steps, rates, memory, skip, step_bias, lengths, softplus, True)
+        ctx.softplus = softplus
+        ctx.save_for_backward(keys, values, queries, steps, rates, memory, skip, step_bias, lengths, states)
+        ctx.set_materialize_grads(False)
+        return hidden, memory_out
+
+    @staticmethod
+    def backward(ctx, grad_hidden, grad_memory_out):
+        keys, values, queries, steps, rates, memory, skip, step_bias, lengths, states = ctx.saved_tensors
+        dk, dv, dq, ds, dr, dm, dskip, dbias = torch.ops.grm_cuda.selective_scan_backward(
+            grad_hidden, grad_memory_out, keys, values, queries, steps, rates, skip, step_bias, lengths, states,
+            ctx.softplus)
+        return (dk, dv, dq, ds, dr, None if memory is None else dm, None if skip is None else dskip,
+                None if step_bias is None else dbias, None, None)
+
+
+def _f32(t: Optional[Tensor]) -> Optional[Tensor]:
+    return t if t is None or t.dtype == torch.float32 else t.float()
+
+
+def cuda_selective_scan(keys: Tensor, values: Tensor, queries: Tensor, steps: Tensor, rates: Tensor,
+                        memory: Optional[Tensor] = None, *, skip: Optional[Tensor] = None,
+                        step_bias: Optional[Tensor] = None, softplus: bool = False, lengths: Optional[Tensor] = None,
+                        enabled: bool = True, debug_fallback: bool = False) -> Tuple[Tensor, Tensor]:
+    """Linear memory whose decay and write strength are chosen by every token and head.  With
+    ``d_t = softplus(steps_t + step_bias)`` (without ``softplus``: ``steps_t + step_bias``),
+    ``M_t = exp(d_t rates) M_{t-1} + d_t v_t k_t^T`` and ``h_t = M_t q_t + skip v_t``.
+
+    keys, queries [B, T, G, N] (a group's row is shared by H / G heads), values [B, T, H, P] in one
+    type (float32, float16 or bfloat16), steps [B, T, H] in that type or float32, rates, skip and
+    step_bias [H] (used in float32; rates are negative for a decaying state), memory [B, H, P, N] the state
+    before token 0 (used in float32; None: zeros), lengths [B] the tokens of each sequence of a padded
+    batch (clamped to [0, T]; the tokens behind are not read, leave the state alone and come out as
+    zeros).  The last two dimensions of keys, values and queries are packed; a slice of a wider row is read in
+    place.  Returns (hidden [B, T, H, P], memory_out [B, H, P, N] float32).  Differentiable in all
+    but lengths.  Limits: N <= 128."""
+    if values.is_cuda and _run_native("selective_scan", values.device, enabled=enabled,
+                                      debug_fallback=debug_fallback):
+        args = (keys, values, queries, steps, _f32(rates), _f32(memory), _f32(skip), _f32(step_bias), lengths,
+                bool(softplus))
+        if _wants_grad(keys, values, queries, steps, rates, memory, skip, step_bias):
+            return _SelectiveScanFn.apply(*args)
+        return torch.ops.grm_cuda.selective_scan_forward(*args, False)[:2]
+    return _torch_selective_scan(keys, values, queries, steps, rates, memory, skip, step_bias, lengths, softplus)
+
+
+def cuda_selective_step(keys: Tensor, values: Tensor, queries: Tensor, steps: Tensor, rates: Tensor, memory: Tensor,
+                        *, skip: Optional[Tensor] = None, step_bias: Optional[Tensor] = None, softplus: bool = False,
+                        memory_out: Optional[Tensor] = None, enabled: bool = True,
+                        debug_fallback: bool = False) -> Tuple[Tensor, Tensor]:
+    """One token of ``cuda_selective_scan``: keys, queries [B, G, N], values [B, H, P], steps [B, H],
+    memory [B, H, P, N] float32.  Returns (hidden [B, H, P], the state moved by this token).
+    ``memory_out`` takes that state; with ``memory_out=memory`` it is updated in place, as a serving
+    loop or a captured graph keeps it."""
+    grad = _wants_grad(keys, values, queries, steps, rates, memory, skip, step_bias)
+    if memory_out is not None:
+        _check_out(memory_out, memory, "memory_out", grad)
+    if not grad and values.is_cuda and _run_native("selective_scan", values.device, enabled=enabled,
+                                                   debug_fallback=debug_fallback):
+        if memory_out is None:
+            memory_out = torch.empty_like(memory, memory_format=torch.contiguous_format)
+        return torch.ops.grm_cuda.selective_step(keys, values, queries, steps, _f32(rates), memory, _f32(skip),
+                                                 _f32(step_bias), bool(softplus), memory_out), memory_out
+    if values.ndim != 3 or keys.ndim != 3 or queries.ndim != 3 or steps.ndim != 2:
+        raise ValueError("selective_step: keys and queries must be [batch, groups, key_dim], values "
+                         "[batch, heads, value_dim] and steps [batch, heads]")
+    hidden, moved = cuda_selective_scan(keys[:, None], values[:, None], queries[:, None], steps[:, None], rates, memory,
+                                        skip=skip, step_bias=step_bias, softplus=softplus, enabled=enabled,
+                                        debug_fallback=debug_fallback)
+    return hidden[:, 0], moved if memory_out is None else memory_out.copy_(moved)
+
+
 __all__ = [
     "GrmExtensionUnavailable",
     "cuda_apply_query",
@@ -845,6 +1112,10 @@ __all__ = [
     "cuda_segment_retrieve_fuse",
     "cuda_segment_route",
     "cuda_segment_scan",
+    "cuda_selective_scan",
+    "cuda_selective_step",
+    "cuda_short_conv",
+    "cuda_short_conv_step",
     "cuda_topk_route",
     "extension_load_error",
     "extension_module",
