@@ -493,6 +493,65 @@ int grm_hip_short_conv_step(const void* x, const void* weight, const void* bias,
                             void* state_out, int64_t batch, int64_t channels, int64_t width, int64_t x_batch_stride,
                             int dtype, int weight_dtype, int silu, void* stream);
 
+/*
+ * Selective state scan: linear memory whose decay and write strength every token and head
+ * chooses.  No counterpart in the reference (its decay is one constant).
+ *   d_t = softplus(steps_t + step_bias)   (softplus = 0: steps_t + step_bias)
+ *   M_t = exp(d_t rates) M_{t-1} + d_t v_t k_t^T,   h_t = M_t q_t + skip v_t
+ * keys, queries [batch, seq_len, groups, key_dim]: a group's row serves heads / groups heads;
+ * values [batch, seq_len, heads, value_dim]; steps [batch, seq_len, heads].  The last two
+ * dimensions (of steps: the last) are packed, the strides are elements between sequences and between tokens, so slices
+ * of a wider row are read in place.  dtype is that of keys, values, queries and hidden; steps have it
+ * or are float32.  rates, skip (or NULL) and step_bias (or NULL): float32 [heads].
+ * lengths: NULL, or int64 [batch] (device), clamped to [0, seq_len]: the tokens from lengths[b] on
+ * are not read, leave the state alone, and their rows of every output are zeros.
+ * memory: float32 [batch, heads, value_dim, key_dim], 16-byte aligned, the state before token 0;
+ * NULL: zeros.
+ * bfloat16 inputs run bf16 MFMA (the float32 state kept whole in its updates, rounded once to bf16 where a
+ * query reads it, as are the weights between tokens of a chunk); float16 and float32 inputs run float32 MFMA.
+ * Limits: key_dim <= 128, heads a multiple of groups, token strides and rows below 2^21 elements.
+ */
+typedef struct grm_hip_selective_args {
+  const void* keys;
+  const void* values;
+  const void* queries;
+  const void* steps;
+  const float* rates;
+  const float* skip;
+  const float* step_bias;
+  const int64_t* lengths;
+  const float* memory;
+  int64_t batch, seq_len, heads, value_dim, groups, key_dim;
+  int64_t keys_batch_stride, keys_token_stride;
+  int64_t values_batch_stride, values_token_stride;
+  int64_t queries_batch_stride, queries_token_stride;
+  int64_t steps_batch_stride, steps_token_stride;
+  int dtype, steps_dtype, softplus;
+} grm_hip_selective_args;
+
+/*
+ * hidden:     [batch, seq_len, heads, value_dim], contiguous.
+ * memory_out: float32 [batch, heads, value_dim, key_dim], the state after each sequence's last
+ *             token; may not overlap memory.
+ * states:     NULL, or float32 [batch, ceil(seq_len / block), heads, value_dim, key_dim], block =
+ *             grm_hip_selective_scan_block(dtype): the state before every block of tokens, which the
+ *             backward reads (blocks behind a sequence's length are left as they were).
+ * workspace:  grm_hip_selective_scan_workspace() bytes, 16-byte aligned (0: none): the sums of
+ *             sequences' time parts, scanned side by side where sequences and heads are few.
+ */
+int64_t grm_hip_selective_scan_block(int dtype);
+int64_t grm_hip_selective_scan_workspace(int64_t batch, int64_t seq_len, int64_t heads, int64_t value_dim,
+                                         int64_t key_dim, int dtype);
+int grm_hip_selective_scan_fwd(const grm_hip_selective_args* args, void* hidden, float* memory_out, float* states,
+                               void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * One token of grm_hip_selective_scan_fwd (seq_len = 1, no lengths): hidden [batch, heads,
+ * value_dim], memory_out the state moved by the token.  memory_out may be memory itself (updated in
+ * place), but not overlap it otherwise.
+ */
+int grm_hip_selective_step(const grm_hip_selective_args* args, void* hidden, float* memory_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -66,6 +66,27 @@ SIGNATURES = {
     "grm_hip_fuse_residual": (_C, [_P, _P, _P, _P, _P, _P, _I, _I, _I, _C, ctypes.c_float, _P]),
 }
 
+
+
+class SelectiveArgs(ctypes.Structure):
+    """grm_hip_selective_args of include/grm_hip.h."""
+
+    _fields_ = ([(n, _P) for n in ("keys", "values", "queries", "steps", "rates", "skip", "step_bias", "lengths",
+                                   "memory")] +
+                [(n, _I) for n in ("batch", "seq_len", "heads", "value_dim", "groups", "key_dim",
+                                   "keys_batch_stride", "keys_token_stride", "values_batch_stride",
+                                   "values_token_stride", "queries_batch_stride", "queries_token_stride",
+                                   "steps_batch_stride", "steps_token_stride")] +
+                [(n, _C) for n in ("dtype", "steps_dtype", "softplus")])
+
+
+SIGNATURES.update({
+    "grm_hip_selective_scan_block": (_I, [_C]),
+    "grm_hip_selective_scan_workspace": (_I, [_I, _I, _I, _I, _I, _C]),
+    "grm_hip_selective_scan_fwd": (_C, [ctypes.POINTER(SelectiveArgs), _P, _P, _P, _P, _I, _P]),
+    "grm_hip_selective_step": (_C, [ctypes.POINTER(SelectiveArgs), _P, _P, _P]),
+})
+
 _lib: Optional[ctypes.CDLL] = None
 
 

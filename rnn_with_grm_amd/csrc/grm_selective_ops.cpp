@@ -184,6 +184,129 @@ Tensor short_conv_step(const Tensor& x, const Tensor& state, const Tensor& weigh
   return out;
 }
 
+// ---------------------------------------------------------------------------
+// Selective scan.
+
+bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
+// The checked inputs of a call and what keeps their memory alive.
+struct Scan {
+  int64_t B, T, H, P, G, N;
+  grm_hip_selective_args args;
+  Tensor keys, values, queries, steps, rates, skip, bias, lengths, memory;
+};
+
+Tensor f32_state(const Tensor& t) {
+  Tensor m = t.contiguous();
+  return aligned16(m) ? m : m.clone();
+}
+
+// `step`: one token, without the length's dimension.
+Scan check_scan(const Tensor& keys, const Tensor& values, const Tensor& queries, const Tensor& steps,
+                const Tensor& rates, const OptTensor& memory, const OptTensor& skip, const OptTensor& step_bias,
+                const OptTensor& lengths, bool softplus, bool step, const char* op) {
+  const int64_t lead = step ? 1 : 2;
+  TORCH_CHECK_VALUE(keys.dim() == lead + 2 && queries.dim() == lead + 2 && values.dim() == lead + 2 &&
+                        steps.dim() == lead + 1,
+                    op, step ? ": keys and queries must be [batch, groups, key_dim], values [batch, heads, value_dim] and "
+                               "steps [batch, heads]"
+                             : ": keys and queries must be [batch, seq_len, groups, key_dim], values [batch, seq_len, "
+                               "heads, value_dim] and steps [batch, seq_len, heads]");
+  Scan s{};
+  s.B = values.size(0); s.T = step ? 1 : values.size(1); s.H = values.size(-2); s.P = values.size(-1);
+  s.G = keys.size(-2); s.N = keys.size(-1);
+  TORCH_CHECK_VALUE(queries.sizes() == keys.sizes() && keys.size(0) == s.B && steps.size(0) == s.B &&
+                        steps.size(-1) == s.H && (step || (keys.size(1) == s.T && steps.size(1) == s.T)),
+                    op, ": keys, queries, values and steps must agree in batch, length and heads");
+  TORCH_CHECK_VALUE(s.G >= 1 && s.H >= 1 && s.P >= 1 && s.H % s.G == 0 && s.N >= 1 && s.N <= 128, op,
+                    ": heads must be a multiple of groups and key_dim in [1, 128]");
+  const int dt = dtype_code(values, op, "values"), sdt = dtype_code(steps, op, "steps");
+  TORCH_CHECK_VALUE(keys.scalar_type() == values.scalar_type() && queries.scalar_type() == values.scalar_type() &&
+                        (sdt == dt || sdt == GRM_HIP_F32),
+                    op, ": keys, values and queries must share a type, steps have it or float32");
+  check_device(keys, values, op, "keys");
+  check_device(queries, values, op, "queries");
+  check_device(steps, values, op, "steps");
+  auto per_head = [&](const Tensor& t, const char* name) {
+    check_device(t, values, op, name);
+    TORCH_CHECK_VALUE(t.dim() == 1 && t.size(0) == s.H && t.scalar_type() == at::kFloat, op, ": ", name,
+                      " must be float32 [heads]");
+    return t.contiguous();
+  };
+  s.rates = per_head(rates, "rates");
+  if (has(skip)) s.skip = per_head(*skip, "skip");
+  if (has(step_bias)) s.bias = per_head(*step_bias, "step_bias");
+  if (has(memory)) {
+    check_device(*memory, values, op, "memory");
+    TORCH_CHECK_VALUE(memory->sizes() == at::IntArrayRef({s.B, s.H, s.P, s.N}) && memory->scalar_type() == at::kFloat,
+                      op, ": memory must be float32 [batch, heads, value_dim, key_dim]");
+    s.memory = f32_state(*memory);
+  }
+  s.keys = packed_rows(keys, 2);
+  s.values = packed_rows(values, 2);
+  s.queries = packed_rows(queries, 2);
+  s.steps = packed_rows(steps, 1);
+  grm_hip_selective_args& a = s.args;
+  a.keys = s.keys.data_ptr(); a.values = s.values.data_ptr(); a.queries = s.queries.data_ptr();
+  a.steps = s.steps.data_ptr();
+  a.rates = s.rates.data_ptr<float>();
+  a.skip = s.skip.defined() ? s.skip.data_ptr<float>() : nullptr;
+  a.step_bias = s.bias.defined() ? s.bias.data_ptr<float>() : nullptr;
+  a.lengths = lengths_ptr(lengths, s.B, values, op, s.lengths);
+  a.memory = s.memory.defined() ? s.memory.data_ptr<float>() : nullptr;
+  a.batch = s.B; a.seq_len = s.T; a.heads = s.H; a.value_dim = s.P; a.groups = s.G; a.key_dim = s.N;
+  auto strides = [&](const Tensor& t, int64_t width, int64_t* batch, int64_t* token) {
+    *batch = stride_of(t, 0, s.T * width);
+    *token = step ? width : stride_of(t, 1, width);
+  };
+  strides(s.keys, s.G * s.N, &a.keys_batch_stride, &a.keys_token_stride);
+  strides(s.values, s.H * s.P, &a.values_batch_stride, &a.values_token_stride);
+  strides(s.queries, s.G * s.N, &a.queries_batch_stride, &a.queries_token_stride);
+  strides(s.steps, s.H, &a.steps_batch_stride, &a.steps_token_stride);
+  a.dtype = dt; a.steps_dtype = sdt; a.softplus = softplus;
+  return s;
+}
+
+Tensor bytes(int64_t n, const Tensor& like) {
+  return at::empty({std::max<int64_t>(n, 16)}, like.options().dtype(at::kByte));
+}
+
+std::tuple<Tensor, Tensor, Tensor> selective_scan_forward(const Tensor& keys, const Tensor& values,
+                                                          const Tensor& queries, const Tensor& steps,
+                                                          const Tensor& rates, const OptTensor& memory,
+                                                          const OptTensor& skip, const OptTensor& step_bias,
+                                                          const OptTensor& lengths, bool softplus, bool save) {
+  const char* op = "selective_scan";
+  c10::OptionalDeviceGuard guard(values.device());
+  const Scan s = check_scan(keys, values, queries, steps, rates, memory, skip, step_bias, lengths, softplus, false, op);
+  const auto f32 = values.options().dtype(at::kFloat);
+  Tensor hidden = at::empty({s.B, s.T, s.H, s.P}, values.options());
+  Tensor memory_out = at::empty({s.B, s.H, s.P, s.N}, f32);
+  const int64_t block = grm_hip_selective_scan_block(s.args.dtype);
+  Tensor states = save ? at::empty({s.B, (s.T + block - 1) / block, s.H, s.P, s.N}, f32) : at::empty({0}, f32);
+  const int64_t wsb = grm_hip_selective_scan_workspace(s.B, s.T, s.H, s.P, s.N, s.args.dtype);
+  Tensor ws = bytes(wsb, values);
+  check_rc(grm_hip_selective_scan_fwd(&s.args, hidden.data_ptr(), memory_out.data_ptr<float>(),
+                                      save ? states.data_ptr<float>() : nullptr, ws.data_ptr(), wsb, stream_of(values)),
+           op);
+  return {hidden, memory_out, states};
+}
+
+Tensor selective_step(const Tensor& keys, const Tensor& values, const Tensor& queries, const Tensor& steps,
+                      const Tensor& rates, const Tensor& memory, const OptTensor& skip, const OptTensor& step_bias,
+                      bool softplus, Tensor& memory_out) {
+  const char* op = "selective_step";
+  c10::OptionalDeviceGuard guard(values.device());
+  const Scan s = check_scan(keys, values, queries, steps, rates, memory, skip, step_bias, c10::nullopt, softplus, true, op);
+  check_device(memory_out, values, op, "memory_out");
+  TORCH_CHECK_VALUE(memory_out.sizes() == memory.sizes() && memory_out.scalar_type() == at::kFloat &&
+                        memory_out.is_contiguous() && aligned16(memory_out),
+                    op, ": memory_out must be contiguous, 16-byte aligned and match memory");
+  Tensor hidden = at::empty({s.B, s.H, s.P}, values.options());
+  check_rc(grm_hip_selective_step(&s.args, hidden.data_ptr(), memory_out.data_ptr<float>(), stream_of(values)), op);
+  return hidden;
+}
+
 }  // namespace
 }  // namespace grm_selective
 
@@ -191,10 +314,14 @@ TORCH_LIBRARY_FRAGMENT(grm_cuda, m) {
   m.def("short_conv_forward(Tensor x, Tensor weight, Tensor? bias, Tensor? state, Tensor? lengths, bool silu) -> (Tensor out, Tensor state_out)");
   m.def("short_conv_backward(Tensor? grad_out, Tensor? grad_state_out, Tensor x, Tensor weight, Tensor? bias, Tensor? state, Tensor? lengths, bool silu) -> (Tensor grad_x, Tensor grad_weight, Tensor grad_bias, Tensor grad_state)");
   m.def("short_conv_step(Tensor x, Tensor state, Tensor weight, Tensor? bias, bool silu, Tensor(a!) state_out) -> Tensor");
+  m.def("selective_scan_forward(Tensor keys, Tensor values, Tensor queries, Tensor steps, Tensor rates, Tensor? memory, Tensor? skip, Tensor? step_bias, Tensor? lengths, bool softplus, bool save) -> (Tensor hidden, Tensor memory_out, Tensor states)");
+  m.def("selective_step(Tensor keys, Tensor values, Tensor queries, Tensor steps, Tensor rates, Tensor memory, Tensor? skip, Tensor? step_bias, bool softplus, Tensor(a!) memory_out) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(grm_cuda, CUDA, m) {
   m.impl("short_conv_forward", grm_selective::short_conv_forward);
   m.impl("short_conv_backward", grm_selective::short_conv_backward);
   m.impl("short_conv_step", grm_selective::short_conv_step);
+  m.impl("selective_scan_forward", grm_selective::selective_scan_forward);
+  m.impl("selective_step", grm_selective::selective_step);
 }

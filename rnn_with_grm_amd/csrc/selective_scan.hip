@@ -1,0 +1,592 @@
+// Selective state scan (forward) and its single-token form, gfx950.
+//
+//   d_t = softplus(steps_t + bias),  M_t = exp(d_t A) M_{t-1} + d_t v_t k_t^T,  h_t = M_t q_t + D v_t
+//
+// per head, state M of [P value rows, N key columns], keys and queries shared by the heads of a
+// group.  Over a chunk of L tokens from state M, with c_i the summed log decays:
+//   h_i = e^{c_i} M q_i + sum_{j<=i} e^{c_i - c_j} d_j (q_i . k_j) v_j + D v_i
+//   M'  = e^{c_L} M + sum_j e^{c_L - c_j} d_j v_j k_j^T
+//
+// One workgroup walks one (sequence, head, 64 value rows) chunk by chunk, so the inputs are read
+// and the outputs written once, and no state but the last one reaches memory (under autograd: one
+// per 128 tokens).  Eight waves in two roles with one barrier a chunk: waves 0-3 form the chunk's outputs from a copy of the state in
+// LDS (16 tokens each, every product but the last kept in registers as the next one's operand);
+// waves 4-7 hold the state in float32 accumulators (16 rows each), move it over the same
+// chunk and leave the copy for the next.  The next chunk's rows are in registers meanwhile.
+// Where heads are too few to fill 256 CUs, sequences are cut in time: a first launch sums each part's own
+// writes, and each part of the second starts from the combination of the parts before it.
+#include <stdint.h>
+
+#include "selective.h"
+
+namespace grmhip {
+namespace {
+
+constexpr int kWalkThreads = 512;
+constexpr int kPassThreads = 256;
+constexpr int kMaxParts = 32;
+
+template <class M, int NP>
+struct WalkLds {
+  using S = SelShape<M>;
+  static constexpr int NS = NP + S::PAD;                        // key, query and state row stride
+  static constexpr int STAGE = S::L * (2 * NS + S::XS);         // keys, queries, values of a chunk
+  static constexpr int COPY = kSelRows * NS;
+  static constexpr int SCAL = 6 * S::L;                         // hi, lo, d, tail weight, decay; total
+  static constexpr size_t bytes = (2 * STAGE + 2 * COPY) * sizeof(typename ET<M>::raw) + 2 * SCAL * sizeof(float);
+  static_assert(bytes <= 160 * 1024, "one CU's LDS");
+};
+
+struct WalkPlace {
+  int b, h, g, pt, part;
+};
+
+__device__ __forceinline__ WalkPlace walk_place(const SelArgs& a, uint32_t v) {
+  WalkPlace w;
+  w.pt = static_cast<int>(v % a.PT);
+  v /= a.PT;
+  w.h = static_cast<int>(v % a.H);
+  v /= a.H;
+  w.part = static_cast<int>(v % a.parts);
+  w.b = static_cast<int>(v / a.parts);
+  w.g = w.h / (a.H / a.G);
+  return w;
+}
+
+// A part's starting state: the given one and the sums of the parts before (REV: behind) it, decayed.
+template <int NT, bool REV>
+__device__ __forceinline__ void part_start(f32x4 (&acc)[NT], const SelArgs& a, const WalkPlace& w, int p0) {
+  const int64_t head = static_cast<int64_t>(w.b) * a.H + w.h, one = static_cast<int64_t>(a.P) * a.N;
+  const int64_t all = static_cast<int64_t>(a.B) * a.H;
+  double log = 0.0;
+  const int end = REV ? a.parts : -1;
+  for (int q = REV ? w.part + 1 : w.part - 1; q != end; q += REV ? 1 : -1) {
+    state_add<NT>(acc, a.part_state + (q * all + head) * one, p0, a.P, a.N, exp2_d(log));
+    log += a.part_log[q * all + head];
+  }
+  if (a.memory != nullptr) state_add<NT>(acc, a.memory + head * one, p0, a.P, a.N, exp2_d(log));
+}
+
+template <class E, class M, int NP>
+__global__ __launch_bounds__(kWalkThreads, 1) void selective_walk_kernel(SelArgs a) {
+  using S = SelShape<M>;
+  using Lds = WalkLds<M, NP>;
+  using raw = typename ET<M>::raw;
+  using eraw = typename ET<E>::raw;
+  constexpr int L = S::L, NS = Lds::NS, XS = S::XS, NT = NP / 16, NK = NP / 32, NIT = L / 16, PPW = NIT;
+  extern __shared__ __align__(16) unsigned char smem[];
+  raw* stage = reinterpret_cast<raw*>(smem);
+  raw* copy = stage + 2 * Lds::STAGE;
+  float* scal = reinterpret_cast<float*>(copy + 2 * Lds::COPY);
+
+  const WalkPlace w = walk_place(a, xcd_order(blockIdx.x, gridDim.x));
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, g = lane >> 4, n16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int p0 = w.pt * kSelRows, pw = a.P - p0;
+  const int64_t len = sel_length(a, w.b);
+  const int64_t t_first = w.part * a.part_tokens, t_last = min_i64(t_first + a.part_tokens, a.T);
+  const int64_t live = max_i64(0, min_i64(len, t_last) - t_first);
+  const int chunks = static_cast<int>((live + L - 1) / L);
+  const float rate = a.rates[w.h], skip = a.skip == nullptr ? 0.f : a.skip[w.h];
+  const bool vec = a.vec != 0;
+
+  TileLoad<E, M, L, NP, kWalkThreads> kr, qr;
+  TileLoad<E, M, L, kSelRows, kWalkThreads> xr;
+  auto load = [&](int c) {
+    const int64_t t = t_first + static_cast<int64_t>(c) * L, rows = len - t;
+    kr.load(a.keys, w.b * a.kb + t * a.kt + static_cast<int64_t>(w.g) * a.N, a.kt, rows, a.N, vec, tid);
+    qr.load(a.queries, w.b * a.qb + t * a.qt + static_cast<int64_t>(w.g) * a.N, a.qt, rows, a.N, vec, tid);
+    xr.load(a.values, w.b * a.vb + t * a.vt + static_cast<int64_t>(w.h) * a.P + p0, a.vt, rows, pw, vec, tid);
+  };
+  auto put = [&](int c) {
+    raw* s = stage + (c & 1) * Lds::STAGE;
+    kr.store(s, NS, tid);
+    qr.store(s + L * NS, NS, tid);
+    xr.store(s + 2 * L * NS, XS, tid);
+  };
+  auto scalars = [&](int c) {
+    const TokenScalars s = token_scalars<E, L>(a, w.b, w.h, t_first + static_cast<int64_t>(c) * L + lane, len, rate);
+    float* o = scal + (c & 1) * Lds::SCAL;
+    if (lane < L) {
+      const float hi = static_cast<float>(s.cum);
+      o[lane] = hi;
+      o[L + lane] = static_cast<float>(s.cum - hi);
+      o[2 * L + lane] = s.d;
+      o[3 * L + lane] = s.d * exp2_d(s.total - s.cum);
+      o[4 * L + lane] = exp2_d(s.cum);
+    }
+    if (lane == 0) o[5 * L] = exp2_d(s.total);
+  };
+
+  f32x4 acc[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int sp = p0 + 16 * (wave & 3);  // a state wave's first row
+  auto copy_out = [&](int c) {
+    raw* s = copy + (c & 1) * Lds::COPY + (16 * (wave & 3) + n16) * NS + 4 * g;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) store4_raw<M>(s + nt * 16, acc[nt]);
+  };
+  if (chunks > 0) load(0);
+  if (wave >= 4) {
+    part_start<NT, false>(acc, a, w, sp);
+    copy_out(0);
+  }
+  if (chunks > 0) {
+    put(0);
+    if (wave == 0) scalars(0);
+  }
+  __syncthreads();
+
+  eraw* hid = static_cast<eraw*>(a.hidden) + (static_cast<int64_t>(w.b) * a.T * a.H + w.h) * a.P + p0;
+  const int64_t hstride = static_cast<int64_t>(a.H) * a.P;
+  const bool hvec = vec && (a.P & 3) == 0;
+  for (int c = 0; c < chunks; ++c) {
+    if (c + 1 < chunks) load(c + 1);
+    const raw* ks = stage + (c & 1) * Lds::STAGE;
+    const raw *qs = ks + L * NS, *xs = qs + L * NS;
+    const float* sc = scal + (c & 1) * Lds::SCAL;
+    if (wave < 4) {
+      const int it = wave % NIT, pt0 = wave / NIT * PPW, i = it * 16 + n16;
+      const raw* cp = copy + (c & 1) * Lds::COPY;
+      f32x4 y[PPW];
+      Frag8<M> qf[NK];
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) qf[kk] = row_frag<M>(qs, NS, it * 16, kk * 32);
+#pragma unroll
+      for (int p = 0; p < PPW; ++p) {
+        y[p] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) y[p] = mfma8(row_frag<M>(cp, NS, (pt0 + p) * 16, kk * 32), qf[kk], y[p]);
+        const float e = sc[4 * L + i];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[p][r] *= e;
+      }
+      const float hi_i = sc[i], lo_i = sc[L + i];
+      for (int jp = 0; jp <= it; jp += 2) {
+        f32x4 m[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int jt = jp + u;
+          m[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+          if (jt <= it) {
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) m[u] = mfma8(row_frag<M>(ks, NS, jt * 16, kk * 32), qf[kk], m[u]);
+            const int j0 = jt * 16 + 4 * g;
+            const f32x4 hj = *reinterpret_cast<const f32x4*>(sc + j0), lj = *reinterpret_cast<const f32x4*>(sc + L + j0),
+                        dj = *reinterpret_cast<const f32x4*>(sc + 2 * L + j0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              m[u][r] = j0 + r <= i ? m[u][r] * dj[r] * exp2_f((hi_i - hj[r]) + (lo_i - lj[r])) : 0.f;
+          }
+        }
+        // One rounding of the weights to 16 bits, as far from them as the output's own rounding is
+        // from it; the values they meet are exact.
+        const Frag8<M> mf = pair_frag<M>(m[0], m[1]);
+#pragma unroll
+        for (int p = 0; p < PPW; ++p) y[p] = mfma8(col_frag<M>(xs, XS, jp * 16, (pt0 + p) * 16), mf, y[p]);
+      }
+      const int64_t t = t_first + static_cast<int64_t>(c) * L + i;
+      if (t < t_last) {
+        eraw* o = hid + t * hstride;
+        const bool on = t < len;
+#pragma unroll
+        for (int p = 0; p < PPW; ++p) {
+          const int col = (pt0 + p) * 16 + 4 * g;
+          const f32x4 x = lds_row4<M>(xs + i * XS + col);
+          f32x4 v;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = on ? fmaf(skip, x[r], y[p][r]) : 0.f;
+          if (hvec) {
+            if (col < pw) store4_raw<E>(o + col, v);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              if (col + r < pw) o[col + r] = ET<E>::from_f(v[r]);
+            }
+          }
+        }
+      }
+      if (wave == 0 && c + 1 < chunks) scalars(c + 1);
+    } else {
+      if (a.states != nullptr && c * L % S::LB == 0) {
+        const int64_t blk = (t_first + static_cast<int64_t>(c) * L) / S::LB;
+        state_store<NT>(acc, a.states + ((w.b * a.nsave + blk) * a.H + w.h) * a.P * a.N, sp, a.P, a.N);
+      }
+      state_update<M, L, NT>(acc, ks, NS, xs, XS, 16 * (wave & 3), sc + 3 * L, sc[5 * L]);
+      if (c + 1 < chunks) copy_out(c + 1);
+    }
+    if (c + 1 < chunks) put(c + 1);
+    __syncthreads();
+  }
+  if (wave >= 4 && w.part == a.parts - 1)
+    state_store<NT>(acc, a.memory_out + (static_cast<int64_t>(w.b) * a.H + w.h) * a.P * a.N, sp, a.P, a.N);
+  // Tokens behind the length (the walk's last chunk has written its own).
+  const int64_t t_fill = t_first + static_cast<int64_t>(chunks) * L;
+  const int cols = pw < kSelRows ? pw : kSelRows;
+  for (int64_t t = t_fill + wave; t < t_last; t += kWalkThreads / 64) {
+    if (lane < cols) hid[t * hstride + lane] = ET<E>::from_f(0.f);
+  }
+}
+
+// The state's walk alone.  Forward: from zero over a part, leaving the part's sum and log decay.  REV
+// (the backward's adjoint): `keys` are the queries and `values` the output's gradient,
+//   G_{before} = e^{c_L} G + sum_i e^{c_i} dy_i q_i^T,
+// from the gradient of the final state back to the first, G kept at the end of every backward chunk.
+template <class E, class M, int NP, bool REV, bool LOCAL>
+__global__ __launch_bounds__(kPassThreads) void selective_pass_kernel(SelArgs a) {
+  using S = SelShape<M>;
+  using raw = typename ET<M>::raw;
+  constexpr int L = S::L, NS = NP + S::PAD, XS = S::XS, NT = NP / 16, STAGE = L * (NS + XS), SCAL = L + 4;
+  extern __shared__ __align__(16) unsigned char smem[];
+  raw* stage = reinterpret_cast<raw*>(smem);
+  float* scal = reinterpret_cast<float*>(stage + 2 * STAGE);
+
+  const WalkPlace w = walk_place(a, xcd_order(blockIdx.x, gridDim.x));
+  // Parts whose sums nothing asks for: the last one of a forward walk, the first of a reverse one.
+  if (LOCAL && w.part == (REV ? 0 : a.parts - 1)) return;
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int p0 = w.pt * kSelRows, pw = a.P - p0, sp = p0 + 16 * wave;
+  const int64_t len = sel_length(a, w.b);
+  const int64_t t_first = w.part * a.part_tokens, t_last = min_i64(t_first + a.part_tokens, a.T);
+  const int chunks = static_cast<int>((max_i64(0, min_i64(len, t_last) - t_first) + L - 1) / L);
+  const float rate = a.rates[w.h];
+  const bool vec = a.vec != 0;
+  auto chunk_of = [&](int i) { return REV ? chunks - 1 - i : i; };
+
+  TileLoad<E, M, L, NP, kPassThreads> kr;
+  TileLoad<E, M, L, kSelRows, kPassThreads> xr;
+  auto load = [&](int i) {
+    const int64_t t = t_first + static_cast<int64_t>(chunk_of(i)) * L, rows = len - t;
+    kr.load(a.keys, w.b * a.kb + t * a.kt + static_cast<int64_t>(w.g) * a.N, a.kt, rows, a.N, vec, tid);
+    xr.load(a.values, w.b * a.vb + t * a.vt + static_cast<int64_t>(w.h) * a.P + p0, a.vt, rows, pw, vec, tid);
+  };
+  double log = 0.0;
+  auto put = [&](int i) {
+    raw* s = stage + (i & 1) * STAGE;
+    kr.store(s, NS, tid);
+    xr.store(s + L * NS, XS, tid);
+    if (wave == 0) {
+      const TokenScalars t =
+          token_scalars<E, L>(a, w.b, w.h, t_first + static_cast<int64_t>(chunk_of(i)) * L + lane, len, rate);
+      float* o = scal + (i & 1) * SCAL;
+      if (lane < L)
+        o[lane] = REV ? exp2_d(t.cum) : t.d * exp2_d(t.total - t.cum);
+      if (lane == 0) o[L] = exp2_d(t.total);
+      log += t.total;
+    }
+  };
+  f32x4 acc[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (chunks > 0) load(0);
+  if (!LOCAL) part_start<NT, REV>(acc, a, w, sp);
+  if (chunks > 0) put(0);
+  __syncthreads();
+  for (int i = 0; i < chunks; ++i) {
+    if (i + 1 < chunks) load(i + 1);
+    const raw* ks = stage + (i & 1) * STAGE;
+    const float* sc = scal + (i & 1) * SCAL;
+    if (REV && !LOCAL) {
+      const int64_t t = t_first + static_cast<int64_t>(chunk_of(i)) * L;
+      if (i == 0 || (t + L) % S::LB == 0)
+        state_store<NT>(acc, a.states + ((w.b * a.nsave + t / S::LB) * a.H + w.h) * a.P * a.N, sp, a.P, a.N);
+    }
+    state_update<M, L, NT>(acc, ks, NS, ks + L * NS, XS, 16 * wave, sc, sc[L]);
+    if (i + 1 < chunks) put(i + 1);
+    __syncthreads();
+  }
+  const int64_t head = static_cast<int64_t>(w.b) * a.H + w.h, one = static_cast<int64_t>(a.P) * a.N;
+  if (LOCAL) {
+    const int64_t slot = static_cast<int64_t>(w.part) * a.B * a.H + head;
+    state_store<NT>(acc, a.part_state + slot * one, sp, a.P, a.N);
+    if (tid == 0 && w.pt == 0) a.part_log[slot] = log;
+  } else if (w.part == 0) {
+    state_store<NT>(acc, a.memory_out + head * one, sp, a.P, a.N);
+  }
+}
+
+// One token: a row of the state lies on LPR lanes (4 columns each), a wave moves 64 / LPR rows at a
+// time, each element read and written by one thread (so memory_out may be memory).
+template <class E, int LPR>
+__global__ __launch_bounds__(256) void selective_step_kernel(SelArgs a) {
+  using raw = typename ET<E>::raw;
+  constexpr int RPW = 64 / LPR, U = 4;  // rows a wave moves at once, and in how many loads
+  const int lane = lane_id(), wave = static_cast<int>(threadIdx.x) >> 6;
+  const int head = static_cast<int>(blockIdx.x), b = head / a.H, h = head - b * a.H, gi = h / (a.H / a.G);
+  const int col = lane % LPR * 4;
+  const bool whole = (a.N & 3) == 0;
+  float k[4], q[4];
+  const raw* kp = static_cast<const raw*>(a.keys) + b * a.kb + static_cast<int64_t>(gi) * a.N;
+  const raw* qp = static_cast<const raw*>(a.queries) + b * a.qb + static_cast<int64_t>(gi) * a.N;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const bool in = col + r < a.N;
+    k[r] = in ? ET<E>::to_f(kp[col + r]) : 0.f;
+    q[r] = in ? ET<E>::to_f(qp[col + r]) : 0.f;
+  }
+  const float d = step_size(a, raw_step<E>(a, b, 0, h));
+  const float keep = __expf(d * a.rates[h]), skip = a.skip == nullptr ? 0.f : a.skip[h];
+  const raw* xp = static_cast<const raw*>(a.values) + b * a.vb + static_cast<int64_t>(h) * a.P;
+  const float* mp = a.memory + static_cast<int64_t>(head) * a.P * a.N;
+  float* op = a.memory_out + static_cast<int64_t>(head) * a.P * a.N;
+  raw* hp = static_cast<raw*>(a.hidden) + static_cast<int64_t>(head) * a.P;
+  const int stride = static_cast<int>(gridDim.y) * 4 * RPW * U;
+  for (int p0 = (static_cast<int>(blockIdx.y) * 4 + wave) * RPW * U; p0 < a.P; p0 += stride) {
+    float4 m[U];
+    float x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int p = p0 + u * RPW + lane / LPR;
+      m[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      x[u] = p < a.P ? ET<E>::to_f(xp[p]) : 0.f;
+      if (p < a.P && col < a.N) {
+        const float* s = mp + static_cast<int64_t>(p) * a.N + col;
+        if (whole) {
+          m[u] = *reinterpret_cast<const float4*>(s);
+        } else {
+          m[u].x = s[0];
+          if (col + 1 < a.N) m[u].y = s[1];
+          if (col + 2 < a.N) m[u].z = s[2];
+          if (col + 3 < a.N) m[u].w = s[3];
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int p = p0 + u * RPW + lane / LPR;
+      const float dx = d * x[u];
+      m[u].x = fmaf(dx, k[0], keep * m[u].x);
+      m[u].y = fmaf(dx, k[1], keep * m[u].y);
+      m[u].z = fmaf(dx, k[2], keep * m[u].z);
+      m[u].w = fmaf(dx, k[3], keep * m[u].w);
+      float y = fmaf(m[u].x, q[0], fmaf(m[u].y, q[1], fmaf(m[u].z, q[2], m[u].w * q[3])));
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) y += __shfl_xor(y, o);
+      if (p < a.P && col < a.N) {
+        float* s = op + static_cast<int64_t>(p) * a.N + col;
+        if (whole) {
+          *reinterpret_cast<float4*>(s) = m[u];
+        } else {
+          s[0] = m[u].x;
+          if (col + 1 < a.N) s[1] = m[u].y;
+          if (col + 2 < a.N) s[2] = m[u].z;
+          if (col + 3 < a.N) s[3] = m[u].w;
+        }
+      }
+      if (p < a.P && lane % LPR == 0) hp[p] = ET<E>::from_f(fmaf(skip, x[u], y));
+    }
+  }
+}
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// f(E, M, NP): one of the compiled forms.
+template <class F>
+void with_form(int dtype, int64_t N, F f) {
+  auto by_width = [&](auto e, auto m) {
+    if (N <= 32) f(e, m, std::integral_constant<int, 32>{});
+    else if (N <= 64) f(e, m, std::integral_constant<int, 64>{});
+    else f(e, m, std::integral_constant<int, 128>{});
+  };
+  if (dtype == GRM_HIP_BF16) by_width(BF16{}, BF16{});
+  else if (dtype == GRM_HIP_F16) by_width(F16{}, F32{});
+  else by_width(F32{}, F32{});
+}
+
+int set_lds(const void* kernel, size_t bytes, const char* what) {
+  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (e != hipSuccess) {
+    set_error("%s: %s", what, hipGetErrorString(e));
+    return static_cast<int>(e);
+  }
+  return GRM_HIP_OK;
+}
+
+uint32_t walk_blocks(const SelArgs& a) { return static_cast<uint32_t>(a.B) * a.H * a.PT * a.parts; }
+
+}  // namespace
+
+int64_t sel_block(int dtype) { return dtype == GRM_HIP_BF16 ? SelShape<BF16>::LB : SelShape<F32>::LB; }
+
+// Enough parts for a workgroup on each of 256 CUs, of at least four backward chunks each: a part costs a
+// second reading of its keys and values.
+int sel_parts(int64_t seqs, int64_t T, int dtype, int64_t* part_tokens) {
+  const int64_t block = sel_block(dtype), blocks = T > 0 ? sel_ceil(T, block) : 1;
+  int64_t parts = 256 / (seqs > 0 ? seqs : 1);
+  if (parts > blocks / 4) parts = blocks / 4;
+  if (parts > kMaxParts) parts = kMaxParts;
+  if (parts < 1) parts = 1;
+  const int64_t per = sel_ceil(blocks, parts);
+  *part_tokens = per * block;
+  return static_cast<int>(sel_ceil(blocks, per));
+}
+
+int sel_check(const grm_hip_selective_args* u, const char* what) {
+  auto bad = [&](const char* why) {
+    set_error("%s: %s", what, why);
+    return GRM_HIP_EINVAL;
+  };
+  if (u == nullptr) return bad("no arguments");
+  if (u->batch < 0 || u->seq_len < 0 || u->heads < 1 || u->value_dim < 1 || u->groups < 1 || u->key_dim < 1)
+    return bad("batch and seq_len must be >= 0, the other sizes >= 1");
+  if (u->heads % u->groups != 0) return bad("heads must be a multiple of groups");
+  if (u->dtype < 0 || u->dtype > 2 || (u->steps_dtype != u->dtype && u->steps_dtype != GRM_HIP_F32)) {
+    set_error("%s: keys, values and queries must be float32, float16 or bfloat16, steps the same or float32", what);
+    return GRM_HIP_EUNSUPPORTED;
+  }
+  if (u->key_dim > 128) {
+    set_error("%s: key_dim must be <= 128, got %lld", what, static_cast<long long>(u->key_dim));
+    return GRM_HIP_EUNSUPPORTED;
+  }
+  const int64_t most = int64_t{1} << 21;
+  if (u->keys_token_stride < 0 || u->keys_token_stride > most || u->values_token_stride < 0 ||
+      u->values_token_stride > most || u->queries_token_stride < 0 || u->queries_token_stride > most ||
+      u->heads * sel_ceil(u->value_dim, kSelRows) * u->batch > (1 << 24) || u->heads * u->value_dim > most ||
+      u->groups * u->key_dim > most) {
+    set_error("%s: token strides and row widths must be below 2^21 elements and batch * heads * value tiles below 2^24", what);
+    return GRM_HIP_EUNSUPPORTED;
+  }
+  if (u->batch > 0 && u->rates == nullptr) return bad("rates are required");
+  if (u->batch > 0 && u->seq_len > 0 &&
+      (u->keys == nullptr || u->values == nullptr || u->queries == nullptr || u->steps == nullptr))
+    return bad("keys, values, queries and steps are required");
+  if (!aligned(u->memory)) return bad("memory must be 16-byte aligned");
+  return GRM_HIP_OK;
+}
+
+SelArgs sel_args(const grm_hip_selective_args* u) {
+  SelArgs a{};
+  a.keys = u->keys; a.values = u->values; a.queries = u->queries; a.steps = u->steps;
+  a.rates = u->rates; a.skip = u->skip; a.bias = u->step_bias; a.lengths = u->lengths; a.memory = u->memory;
+  a.kb = u->keys_batch_stride; a.kt = u->keys_token_stride;
+  a.vb = u->values_batch_stride; a.vt = u->values_token_stride;
+  a.qb = u->queries_batch_stride; a.qt = u->queries_token_stride;
+  a.sb = u->steps_batch_stride; a.st = u->steps_token_stride;
+  a.T = u->seq_len;
+  a.B = static_cast<int>(u->batch); a.H = static_cast<int>(u->heads); a.P = static_cast<int>(u->value_dim);
+  a.G = static_cast<int>(u->groups); a.N = static_cast<int>(u->key_dim);
+  a.PT = static_cast<int>(sel_ceil(u->value_dim, kSelRows));
+  a.parts = 1;
+  a.steps_f32 = u->steps_dtype == GRM_HIP_F32;
+  a.softplus = u->softplus;
+  // Whole 16-byte loads where every row of 8-element units allows them.
+  a.vec = u->value_dim % 8 == 0 && u->key_dim % 8 == 0 && aligned(u->keys) && aligned(u->values) &&
+          aligned(u->queries) && (u->keys_batch_stride | u->keys_token_stride | u->values_batch_stride |
+                                  u->values_token_stride | u->queries_batch_stride | u->queries_token_stride) % 8 == 0;
+  return a;
+}
+
+int launch_state_pass(const SelArgs& a, int dtype, bool reverse, bool local, hipStream_t stream, const char* what) {
+  int rc = GRM_HIP_OK;
+  with_form(dtype, a.N, [&](auto e, auto m, auto np) {
+    using E = decltype(e);
+    using M = decltype(m);
+    constexpr int NP = decltype(np)::value;
+    using S = SelShape<M>;
+    constexpr size_t lds = 2 * S::L * (NP + S::PAD + S::XS) * sizeof(typename ET<M>::raw) + 2 * (S::L + 4) * sizeof(float);
+    auto go = [&](auto kernel) {
+      if ((rc = set_lds(reinterpret_cast<const void*>(kernel), lds, what)) != GRM_HIP_OK) return;
+      kernel<<<dim3(walk_blocks(a)), dim3(kPassThreads), lds, stream>>>(a);
+      rc = check_launch(what);
+    };
+    if (reverse && local) go(selective_pass_kernel<E, M, NP, true, true>);
+    else if (reverse) go(selective_pass_kernel<E, M, NP, true, false>);
+    else go(selective_pass_kernel<E, M, NP, false, true>);
+  });
+  return rc;
+}
+
+}  // namespace grmhip
+
+using namespace grmhip;
+
+extern "C" int64_t grm_hip_selective_scan_block(int dtype) { return dtype < 0 || dtype > 2 ? 0 : sel_block(dtype); }
+
+extern "C" int64_t grm_hip_selective_scan_workspace(int64_t batch, int64_t seq_len, int64_t heads, int64_t value_dim,
+                                                    int64_t key_dim, int dtype) {
+  if (batch <= 0 || seq_len < 0 || heads <= 0 || value_dim <= 0 || key_dim <= 0 || dtype < 0 || dtype > 2) return 0;
+  int64_t per = 0;
+  const int64_t parts = sel_parts(batch * heads * sel_ceil(value_dim, kSelRows), seq_len, dtype, &per);
+  return parts == 1 ? 0 : sel_ceil(parts * batch * heads * 8, 16) * 16 + parts * batch * heads * value_dim * key_dim * 4;
+}
+
+extern "C" int grm_hip_selective_scan_fwd(const grm_hip_selective_args* u, void* hidden, float* memory_out,
+                                          float* states, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "selective_scan";
+  if (int rc = sel_check(u, what)) return rc;
+  if (u->batch == 0) return GRM_HIP_OK;
+  const int64_t state_bytes = u->batch * u->heads * u->value_dim * u->key_dim * 4;
+  if (memory_out == nullptr || (u->seq_len > 0 && hidden == nullptr) || !aligned(memory_out) || !aligned(states)) {
+    set_error("%s: hidden and memory_out are required, memory_out and states 16-byte aligned", what);
+    return GRM_HIP_EINVAL;
+  }
+  if (ranges_overlap(u->memory, state_bytes, memory_out, state_bytes)) {
+    set_error("%s: memory_out may not overlap memory", what);
+    return GRM_HIP_EINVAL;
+  }
+  SelArgs a = sel_args(u);
+  a.hidden = hidden; a.memory_out = memory_out; a.states = states;
+  a.vec = a.vec && aligned(hidden);
+  a.nsave = sel_ceil(u->seq_len, sel_block(u->dtype));
+  a.parts = sel_parts(static_cast<int64_t>(a.B) * a.H * a.PT, a.T, u->dtype, &a.part_tokens);
+  if (a.parts > 1) {
+    if (workspace == nullptr || !aligned(workspace) ||
+        workspace_bytes < grm_hip_selective_scan_workspace(u->batch, u->seq_len, u->heads, u->value_dim, u->key_dim, u->dtype)) {
+      set_error("%s: workspace missing, misaligned or too small", what);
+      return GRM_HIP_EINVAL;
+    }
+    a.part_log = static_cast<double*>(workspace);
+    a.part_state = reinterpret_cast<float*>(static_cast<char*>(workspace) + sel_ceil(int64_t{a.parts} * a.B * a.H * 8, 16) * 16);
+    if (int rc = launch_state_pass(a, u->dtype, false, true, static_cast<hipStream_t>(stream), what)) return rc;
+  }
+  int rc = GRM_HIP_OK;
+  with_form(u->dtype, a.N, [&](auto e, auto m, auto np) {
+    using E = decltype(e);
+    using M = decltype(m);
+    constexpr int NP = decltype(np)::value;
+    auto kernel = selective_walk_kernel<E, M, NP>;
+    if ((rc = set_lds(reinterpret_cast<const void*>(kernel), WalkLds<M, NP>::bytes, what)) != GRM_HIP_OK) return;
+    kernel<<<dim3(walk_blocks(a)), dim3(kWalkThreads), WalkLds<M, NP>::bytes, static_cast<hipStream_t>(stream)>>>(a);
+    rc = check_launch(what);
+  });
+  return rc;
+}
+
+extern "C" int grm_hip_selective_step(const grm_hip_selective_args* u, void* hidden, float* memory_out, void* stream) {
+  const char* what = "selective_step";
+  if (int rc = sel_check(u, what)) return rc;
+  if (u->seq_len != 1 || u->lengths != nullptr) {
+    set_error("%s: seq_len must be 1, without lengths", what);
+    return GRM_HIP_EINVAL;
+  }
+  if (u->batch == 0) return GRM_HIP_OK;
+  if (u->memory == nullptr || hidden == nullptr || memory_out == nullptr || !aligned(memory_out)) {
+    set_error("%s: memory, hidden and memory_out are required, memory_out 16-byte aligned", what);
+    return GRM_HIP_EINVAL;
+  }
+  const int64_t state_bytes = u->batch * u->heads * u->value_dim * u->key_dim * 4;
+  if (memory_out != u->memory && ranges_overlap(u->memory, state_bytes, memory_out, state_bytes)) {
+    set_error("%s: memory_out must be memory itself or not overlap it", what);
+    return GRM_HIP_EINVAL;
+  }
+  SelArgs a = sel_args(u);
+  a.hidden = hidden; a.memory_out = memory_out;
+  auto go = [&](auto e, auto lpr) {
+    constexpr int LPR = decltype(lpr)::value, rows = 4 * (64 / LPR) * 4;  // of a workgroup at a time
+    selective_step_kernel<decltype(e), LPR>
+        <<<dim3(static_cast<uint32_t>(a.B) * a.H, static_cast<uint32_t>(sel_ceil(a.P, rows))), dim3(256), 0,
+           static_cast<hipStream_t>(stream)>>>(a);
+  };
+  auto by_width = [&](auto e) {
+    if (a.N <= 16) go(e, std::integral_constant<int, 4>{});
+    else if (a.N <= 32) go(e, std::integral_constant<int, 8>{});
+    else if (a.N <= 64) go(e, std::integral_constant<int, 16>{});
+    else go(e, std::integral_constant<int, 32>{});
+  };
+  if (u->dtype == GRM_HIP_F32) by_width(F32{});
+  else if (u->dtype == GRM_HIP_F16) by_width(F16{});
+  else by_width(BF16{});
+  return check_launch(what);
+}
