@@ -546,6 +546,21 @@ int grm_hip_selective_scan_fwd(const grm_hip_selective_args* args, void* hidden,
                                void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
+ * Gradients of grm_hip_selective_scan_fwd.  states is what the forward left for the same arguments;
+ * grad_hidden [batch, seq_len, heads, value_dim] is contiguous in dtype, grad_memory_out float32 or
+ * NULL (zeros).  grad_keys, grad_values, grad_queries (dtype) and grad_steps (steps_dtype) are
+ * contiguous, the others float32; grad_skip and grad_step_bias may be NULL.  Rows behind a
+ * sequence's length get zeros.  The sums over heads, tokens and sequences are taken in a fixed order (no atomics).
+ * Workspace: grm_hip_selective_scan_bwd_workspace() bytes, 16-byte aligned.
+ */
+int64_t grm_hip_selective_scan_bwd_workspace(int64_t batch, int64_t seq_len, int64_t heads, int64_t value_dim,
+                                             int64_t groups, int64_t key_dim, int dtype);
+int grm_hip_selective_scan_bwd(const grm_hip_selective_args* args, const float* states, const void* grad_hidden,
+                               const float* grad_memory_out, void* grad_keys, void* grad_values, void* grad_queries,
+                               void* grad_steps, float* grad_rates, float* grad_memory, float* grad_skip,
+                               float* grad_step_bias, void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * One token of grm_hip_selective_scan_fwd (seq_len = 1, no lengths): hidden [batch, heads,
  * value_dim], memory_out the state moved by the token.  memory_out may be memory itself (updated in
  * place), but not overlap it otherwise.

@@ -84,6 +84,8 @@ SIGNATURES.update({
     "grm_hip_selective_scan_block": (_I, [_C]),
     "grm_hip_selective_scan_workspace": (_I, [_I, _I, _I, _I, _I, _C]),
     "grm_hip_selective_scan_fwd": (_C, [ctypes.POINTER(SelectiveArgs), _P, _P, _P, _P, _I, _P]),
+    "grm_hip_selective_scan_bwd_workspace": (_I, [_I, _I, _I, _I, _I, _I, _C]),
+    "grm_hip_selective_scan_bwd": (_C, [ctypes.POINTER(SelectiveArgs)] + [_P] * 12 + [_I, _P]),
     "grm_hip_selective_step": (_C, [ctypes.POINTER(SelectiveArgs), _P, _P, _P]),
 })
 

@@ -292,6 +292,51 @@ std::tuple<Tensor, Tensor, Tensor> selective_scan_forward(const Tensor& keys, co
   return {hidden, memory_out, states};
 }
 
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> selective_scan_backward(
+    const OptTensor& grad_hidden, const OptTensor& grad_memory_out, const Tensor& keys, const Tensor& values,
+    const Tensor& queries, const Tensor& steps, const Tensor& rates, const OptTensor& skip, const OptTensor& step_bias,
+    const OptTensor& lengths, const Tensor& states, bool softplus) {
+  const char* op = "selective_scan backward";
+  c10::OptionalDeviceGuard guard(values.device());
+  const Scan s =
+      check_scan(keys, values, queries, steps, rates, c10::nullopt, skip, step_bias, lengths, softplus, false, op);
+  const auto f32 = values.options().dtype(at::kFloat);
+  const int64_t block = grm_hip_selective_scan_block(s.args.dtype);
+  check_device(states, values, op, "states");
+  TORCH_CHECK_VALUE(states.sizes() == at::IntArrayRef({s.B, (s.T + block - 1) / block, s.H, s.P, s.N}) &&
+                        states.scalar_type() == at::kFloat,
+                    op, ": states must be what the forward kept");
+  Tensor dy, dm, st = f32_state(states);
+  if (has(grad_hidden)) {
+    check_device(*grad_hidden, values, op, "grad_hidden");
+    TORCH_CHECK_VALUE(grad_hidden->sizes() == values.sizes() && grad_hidden->scalar_type() == values.scalar_type(), op,
+                      ": grad_hidden must match values");
+    dy = grad_hidden->contiguous();
+  } else {
+    dy = at::zeros(values.sizes(), values.options());
+  }
+  if (has(grad_memory_out)) {
+    check_device(*grad_memory_out, values, op, "grad_memory_out");
+    TORCH_CHECK_VALUE(grad_memory_out->sizes() == at::IntArrayRef({s.B, s.H, s.P, s.N}) &&
+                          grad_memory_out->scalar_type() == at::kFloat,
+                      op, ": grad_memory_out must be float32 [batch, heads, value_dim, key_dim]");
+    dm = f32_state(*grad_memory_out);
+  }
+  Tensor gk = at::empty(keys.sizes(), values.options()), gv = at::empty(values.sizes(), values.options()),
+         gq = at::empty(keys.sizes(), values.options()), gst = at::empty(steps.sizes(), steps.options());
+  Tensor gr = at::empty({s.H}, f32), gm = at::empty({s.B, s.H, s.P, s.N}, f32), gsk = at::empty({s.H}, f32),
+         gb = at::empty({s.H}, f32);
+  const int64_t wsb = grm_hip_selective_scan_bwd_workspace(s.B, s.T, s.H, s.P, s.G, s.N, s.args.dtype);
+  Tensor ws = bytes(wsb, values);
+  check_rc(grm_hip_selective_scan_bwd(&s.args, st.data_ptr<float>(), dy.data_ptr(),
+                                      dm.defined() ? dm.data_ptr<float>() : nullptr, gk.data_ptr(), gv.data_ptr(),
+                                      gq.data_ptr(), gst.data_ptr(), gr.data_ptr<float>(), gm.data_ptr<float>(),
+                                      gsk.data_ptr<float>(), gb.data_ptr<float>(), ws.data_ptr(), wsb,
+                                      stream_of(values)),
+           op);
+  return {gk, gv, gq, gst, gr, gm, gsk, gb};
+}
+
 Tensor selective_step(const Tensor& keys, const Tensor& values, const Tensor& queries, const Tensor& steps,
                       const Tensor& rates, const Tensor& memory, const OptTensor& skip, const OptTensor& step_bias,
                       bool softplus, Tensor& memory_out) {
@@ -315,6 +360,7 @@ TORCH_LIBRARY_FRAGMENT(grm_cuda, m) {
   m.def("short_conv_backward(Tensor? grad_out, Tensor? grad_state_out, Tensor x, Tensor weight, Tensor? bias, Tensor? state, Tensor? lengths, bool silu) -> (Tensor grad_x, Tensor grad_weight, Tensor grad_bias, Tensor grad_state)");
   m.def("short_conv_step(Tensor x, Tensor state, Tensor weight, Tensor? bias, bool silu, Tensor(a!) state_out) -> Tensor");
   m.def("selective_scan_forward(Tensor keys, Tensor values, Tensor queries, Tensor steps, Tensor rates, Tensor? memory, Tensor? skip, Tensor? step_bias, Tensor? lengths, bool softplus, bool save) -> (Tensor hidden, Tensor memory_out, Tensor states)");
+  m.def("selective_scan_backward(Tensor? grad_hidden, Tensor? grad_memory_out, Tensor keys, Tensor values, Tensor queries, Tensor steps, Tensor rates, Tensor? skip, Tensor? step_bias, Tensor? lengths, Tensor states, bool softplus) -> (Tensor grad_keys, Tensor grad_values, Tensor grad_queries, Tensor grad_steps, Tensor grad_rates, Tensor grad_memory, Tensor grad_skip, Tensor grad_step_bias)");
   m.def("selective_step(Tensor keys, Tensor values, Tensor queries, Tensor steps, Tensor rates, Tensor memory, Tensor? skip, Tensor? step_bias, bool softplus, Tensor(a!) memory_out) -> Tensor");
 }
 
@@ -323,5 +369,6 @@ TORCH_LIBRARY_IMPL(grm_cuda, CUDA, m) {
   m.impl("short_conv_backward", grm_selective::short_conv_backward);
   m.impl("short_conv_step", grm_selective::short_conv_step);
   m.impl("selective_scan_forward", grm_selective::selective_scan_forward);
+  m.impl("selective_scan_backward", grm_selective::selective_scan_backward);
   m.impl("selective_step", grm_selective::selective_step);
 }

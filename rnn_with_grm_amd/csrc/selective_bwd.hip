@@ -1,0 +1,675 @@
+// Gradients of the selective state scan, gfx950.
+//
+// Over a block of L tokens from state S at its start, with the adjoint G of the state at its end,
+// c_i the summed log decays, E_ij = e^{c_i - c_j} (j <= i), K_ij = q_i . k_j and W_ij = dy_i . x_j:
+//   dx_j = d_j (sum_i E_ij K_ij dy_i + e^{c_L - c_j} G k_j) + D dy_j
+//   dq_i = sum_j E_ij d_j W_ij k_j + e^{c_i} S^T dy_i          summed over the heads of a group
+//   dk_j = sum_i E_ij d_j W_ij q_i + d_j e^{c_L - c_j} G^T x_j  likewise
+//   G'   = e^{c_L} G + sum_i e^{c_i} dy_i q_i^T                 the adjoint at the block's start
+// and for the step sizes, with Q_ij = E_ij d_j K_ij W_ij (j < i), t1_i = e^{c_i} q_i . S^T dy_i and
+// t2_j = e^{c_L - c_j} k_j . G^T x_j,
+//   dc_i = sum_j Q_ij - sum_j Q_ji + t1_i - d_i t2_i
+//   dl_t = sum_{s >= t} dc_s + sum_j d_j t2_j + e^{c_L} <G, S>     (l_t = d_t A, the log decay)
+//   dd_t = A dl_t + sum_i E_it K_it W_it + t2_t,   dA = sum_t d_t dl_t,   dD = sum_t W_tt
+//
+// Three steps.  The forward has left S before every block; the reverse walk (selective_pass_kernel)
+// leaves G behind every block; then all blocks run side by side, one workgroup for a block and some
+// of a group's heads, whose dk and dq it sums in registers (K is formed once for all of them).  Where more
+// than one workgroup shares a group, their sums are added in a fixed order by a last kernel: no
+// atomics, the same bits on every run.
+//
+// The step sizes' gradient is a difference of large sums, so its terms stay float32: K and W are sums
+// of exact products, and S and G enter t1 and t2 as two bfloat16 parts (16 bits and more; 2^-17).
+// dx, dk and dq are rounded to 16 bits in the end; their weights E K and E d W are rounded once to bfloat16,
+// as is G where it meets k.
+#include <stdint.h>
+
+#include "selective.h"
+
+namespace grmhip {
+namespace {
+
+constexpr int kGradThreads = 512;
+
+struct GradArgs {
+  SelArgs s;              // the forward's inputs; states: S before every block
+  const void* dy;         // [B, T, H, P]
+  const float* adj;       // [B, nsave, H, P, N]: G behind every block
+  void* dx;               // [B, T, H, P]
+  void* dk;               // [B, T, G, N]
+  void* dq;               // [B, T, G, N]
+  void* dsteps;           // [B, T, H]
+  float* rows_part;       // [splits][2][B, T, G, N] or null: dk and dq of each share of the heads
+  float* steps_part;      // [PT][B, T, H] or null
+  float* head_part;       // [B * nsave][H * PT][3]
+  int splits;
+};
+
+template <class M, int NP>
+struct GradLds {
+  using S = SelShape<M>;
+  static constexpr int LB = S::LB, NS = NP + S::PAD, XS = S::XS;
+  static constexpr int SPARTS = S::kHalf ? 2 : 1;             // parts of S and G in LDS
+  static constexpr int STATE = kSelRows * NS;
+  static constexpr int TILES = LB * (2 * NS + 2 * XS) + SPARTS * STATE;
+  static constexpr int TOK = LB / 16;                          // token tiles
+  static constexpr int CS = 8 / TOK;                           // waves that share one, a share of the columns each
+  // hi, lo, d, e^c, e^{c_L - c}; column sums, diagonal, W_jj; t1, t2 per share; row sums per tile; <G, S>
+  static constexpr int SCAL = 5 * LB + 3 * LB + 2 * CS * LB + TOK * LB + 16;
+  static constexpr size_t bytes = TILES * sizeof(typename ET<M>::raw) + SCAL * sizeof(float);
+  static_assert(bytes <= 160 * 1024, "one CU's LDS");
+};
+
+template <int ROT>
+__device__ __forceinline__ float row_rot(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + ROT, 0xf, 0xf, true));
+}
+// Sum over the 16 lanes of a row, in all of them.
+__device__ __forceinline__ float row_sum(float x) {
+  x += row_rot<8>(x);
+  x += row_rot<4>(x);
+  x += row_rot<2>(x);
+  x += row_rot<1>(x);
+  return x;
+}
+// Sum over the four lane groups.
+__device__ __forceinline__ float group_sum(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+// Fragment of 16 rows, reduction along the row in the tokens' slot order (4g + s, 16 + 4g + s).
+template <class M>
+__device__ __forceinline__ Frag8<M> row_frag_t(const typename ET<M>::raw* tile, int stride, int row, int col) {
+  const int lane = lane_id();
+  const typename ET<M>::raw* p = tile + (row + (lane & 15)) * stride + col + 4 * (lane >> 4);
+  return lds_frag_4x2<M>(p, p + 16);
+}
+
+template <class E>
+__device__ __forceinline__ void store_row4(typename ET<E>::raw* p, int left, bool vec, f32x4 v) {
+  if (vec) {
+    if (left > 0) store4_raw<E>(p, v);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (r < left) p[r] = ET<E>::from_f(v[r]);
+    }
+  }
+}
+
+template <class E, class M, int NP>
+__global__ __launch_bounds__(kGradThreads, 1) void selective_grad_kernel(GradArgs a) {
+  using S = SelShape<M>;
+  using Lds = GradLds<M, NP>;
+  using raw = typename ET<M>::raw;
+  using eraw = typename ET<E>::raw;
+  constexpr int LB = S::LB, NS = Lds::NS, XS = S::XS, TOK = Lds::TOK, CS = Lds::CS, SP = Lds::SPARTS;
+  constexpr int NK = NP / 32, NT = NP / 16 / CS, PW = kSelRows / 16 / CS, PL = (LB + 63) / 64;
+  constexpr int SU = kSelRows * NP / 4 / kGradThreads;  // float4 of a state per thread
+  static_assert(SU >= 1 && SU * kGradThreads * 4 == kSelRows * NP, "states split evenly");
+  extern __shared__ __align__(16) unsigned char smem[];
+  raw* kt = reinterpret_cast<raw*>(smem);
+  raw* qt = kt + LB * NS;
+  raw* xt = qt + LB * NS;
+  raw* yt = xt + LB * XS;
+  raw* st = yt + LB * XS;
+  float* hi = reinterpret_cast<float*>(st + SP * Lds::STATE);
+  float *lo = hi + LB, *dd = lo + LB, *ec = dd + LB, *et = ec + LB, *col = et + LB, *diag = col + LB, *wjj = diag + LB,
+        *t1 = wjj + LB, *t2 = t1 + CS * LB, *rows = t2 + CS * LB, *gs = rows + TOK * LB;
+
+  const SelArgs& f = a.s;
+  uint32_t v = xcd_order(blockIdx.x, gridDim.x);
+  const int split = static_cast<int>(v % a.splits);
+  v /= a.splits;
+  const int gi = static_cast<int>(v % f.G);
+  v /= f.G;
+  const int blk = static_cast<int>(v % f.nsave), b = static_cast<int>(v / f.nsave);
+  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, g = lane >> 4, n16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int tile = wave % TOK, cs = wave / TOK, tok = tile * 16 + n16;  // this lane's token in both orders
+  const int64_t len = sel_length(f, b), t0 = static_cast<int64_t>(blk) * LB, live = len - t0;
+  const bool vec = f.vec != 0, nvec = vec && (f.N & 3) == 0, pvec = vec && (f.P & 3) == 0;
+  const int heads = f.H / f.G * f.PT;  // (head, value tile) pairs of the group
+  const int h_lo = static_cast<int>(static_cast<int64_t>(heads) * split / a.splits),
+            h_hi = static_cast<int>(static_cast<int64_t>(heads) * (split + 1) / a.splits);
+
+  f32x4 dk[NT], dq[NT], score[TOK];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) dk[i] = dq[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (live > 0) {
+    TileLoad<E, M, LB, NP, kGradThreads> r;
+    r.load(f.keys, b * f.kb + t0 * f.kt + static_cast<int64_t>(gi) * f.N, f.kt, live, f.N, vec, tid);
+    r.store(kt, NS, tid);
+    r.load(f.queries, b * f.qb + t0 * f.qt + static_cast<int64_t>(gi) * f.N, f.qt, live, f.N, vec, tid);
+    r.store(qt, NS, tid);
+    __syncthreads();
+    // K: rows i of every tile from this wave's on, columns j of this wave's tile.
+    Frag8<M> kf[NK];
+#pragma unroll
+    for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<M>(kt, NS, tile * 16, kk * 32);
+#pragma unroll
+    for (int it = 0; it < TOK; ++it) {
+      score[it] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (it >= tile) {
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) score[it] = mfma8(row_frag<M>(qt, NS, it * 16, kk * 32), kf[kk], score[it]);
+      }
+    }
+  }
+
+  for (int hp = h_lo; hp < h_hi; ++hp) {
+    const int h = gi * (f.H / f.G) + hp / f.PT, pt = hp % f.PT, p0 = pt * kSelRows, pw = f.P - p0;
+    const int64_t row0 = (static_cast<int64_t>(b) * f.T + t0) * f.H + h;
+    const int64_t hs = static_cast<int64_t>(f.H);
+    eraw* dxp = static_cast<eraw*>(a.dx) + row0 * f.P + p0;
+    float* hpart = a.head_part + ((static_cast<int64_t>(b) * f.nsave + blk) * f.H * f.PT + h * f.PT + pt) * 3;
+    auto put_step = [&](int64_t t, float x) {
+      const int64_t at = row0 + t * hs;
+      if (a.steps_part != nullptr) a.steps_part[static_cast<int64_t>(pt) * f.B * f.T * f.H + at] = x;
+      else st_state<E>(a.dsteps, at, f.steps_f32 != 0, x);
+    };
+    const int in_block = static_cast<int>(min_i64(LB, f.T - t0));
+    if (live <= 0) {  // behind the sequence's length: zeros
+      const int cols = pw < kSelRows ? pw : kSelRows;
+      for (int t = wave; t < in_block; t += 8) {
+        if (lane < cols) dxp[t * hs * f.P + lane] = ET<E>::from_f(0.f);
+        if (lane == 0) put_step(t, 0.f);
+      }
+      if (tid < 3) hpart[tid] = 0.f;
+      continue;
+    }
+    const float rate = f.rates[h], skip = f.skip == nullptr ? 0.f : f.skip[h];
+
+    // The head's rows, the state and the adjoint.
+    TileLoad<E, M, LB, kSelRows, kGradThreads> xr, yr;
+    xr.load(f.values, b * f.vb + t0 * f.vt + static_cast<int64_t>(h) * f.P + p0, f.vt, live, pw, vec, tid);
+    yr.load(a.dy, row0 * f.P + p0, hs * f.P, live, pw, vec, tid);
+    const int64_t sat = ((static_cast<int64_t>(b) * f.nsave + blk) * f.H + h) * f.P * f.N;
+    f32x4 gr[SU], sr[SU];
+    auto load_state = [&](const float* base, f32x4 (&r)[SU]) {
+#pragma unroll
+      for (int i = 0; i < SU; ++i) {
+        const int u = tid + i * kGradThreads, p = p0 + u / (NP / 4), n = u % (NP / 4) * 4;
+        r[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (p < f.P && n < f.N) {
+          const float* q = base + sat + static_cast<int64_t>(p) * f.N + n;
+          if ((f.N & 3) == 0) {
+            const float4 w = *reinterpret_cast<const float4*>(q);
+            r[i] = f32x4{w.x, w.y, w.z, w.w};
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[i][e] = n + e < f.N ? q[e] : 0.f;
+          }
+        }
+      }
+    };
+    auto put_state = [&](const f32x4 (&r)[SU]) {
+#pragma unroll
+      for (int i = 0; i < SU; ++i) {
+        const int u = tid + i * kGradThreads;
+        raw* q = st + u / (NP / 4) * NS + u % (NP / 4) * 4;
+        f32x4 rest = r[i];
+#pragma unroll
+        for (int s = 0; s < SP; ++s) {
+          store4_raw<M>(q + s * Lds::STATE, rest);
+          if (s + 1 < SP) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) rest[e] -= ET<M>::to_f(ET<M>::from_f(rest[e]));
+          }
+        }
+      }
+    };
+    load_state(f.states, sr);
+    load_state(a.adj, gr);
+    // Token scalars, PL tokens a lane, by the first wave.
+    double cum[PL], total = 0.0;
+    float dt[PL];
+    if (wave == 0) {
+#pragma unroll
+      for (int k = 0; k < PL; ++k) {
+        const int64_t t = t0 + lane * PL + k;
+        dt[k] = t < len ? step_size(f, raw_step<E>(f, b, t, h)) : 0.f;
+        double l = static_cast<double>(dt[k]) * static_cast<double>(rate);
+        l = l < -200.0 ? -200.0 : l;
+        total += l * 1.4426950408889634;
+        cum[k] = total;
+      }
+      double scan = total;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const double up = __shfl_up(scan, o);
+        if (lane >= o) scan += up;
+      }
+      const double before = scan - total;
+      total = __shfl(scan, 63);
+#pragma unroll
+      for (int k = 0; k < PL; ++k) {
+        cum[k] += before;
+        const int t = lane * PL + k;
+        const float top = static_cast<float>(cum[k]);
+        hi[t] = top;
+        lo[t] = static_cast<float>(cum[k] - top);
+        dd[t] = dt[k];
+        ec[t] = exp2_d(cum[k]);
+        et[t] = exp2_d(total - cum[k]);
+      }
+    }
+    xr.store(xt, XS, tid);
+    yr.store(yt, XS, tid);
+    put_state(sr);
+    float dot = 0.f;
+#pragma unroll
+    for (int i = 0; i < SU; ++i) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) dot = fmaf(gr[i][e], sr[i][e], dot);
+    }
+    dot = group_sum(row_sum(dot));
+    if (lane == 0) gs[wave] = dot;
+    __syncthreads();
+
+    // Columns j of this wave's tile: dx and dk from the rows i >= j.
+    f32x4 dx[PW];
+#pragma unroll
+    for (int p = 0; p < PW; ++p) dx[p] = f32x4{0.f, 0.f, 0.f, 0.f};
+    Frag8<M> xf[2], yf[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      xf[k] = row_frag_t<M>(xt, XS, tile * 16, k * 32);
+      yf[k] = row_frag_t<M>(yt, XS, tile * 16, k * 32);
+    }
+    const float hj = hi[tok], lj = lo[tok], dj = dd[tok];
+    float colsum = 0.f, on_diag = 0.f, w_diag = 0.f;
+#pragma unroll
+    for (int ip = 0; ip < TOK; ip += 2) {
+      if (ip + 1 < tile) continue;
+      f32x4 ek[2], ew[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int it = ip + u;
+        ek[u] = ew[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (it < tile) continue;
+        f32x4 w = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) w = mfma8(row_frag_t<M>(yt, XS, it * 16, k * 32), xf[k], w);
+        const int i0 = it * 16 + 4 * g;
+        const f32x4 hv = *reinterpret_cast<const f32x4*>(hi + i0), lv = *reinterpret_cast<const f32x4*>(lo + i0);
+        f32x4 q;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const bool in = i0 + r >= tok;
+          const float e = exp2_f((hv[r] - hj) + (lv[r] - lj));
+          ek[u][r] = in ? e * score[it][r] : 0.f;
+          ew[u][r] = in ? e * dj * w[r] : 0.f;
+          const float ekw = in ? ek[u][r] * w[r] : 0.f;
+          colsum += ekw;
+          const bool same = i0 + r == tok;
+          on_diag += same ? ekw : 0.f;
+          w_diag += same ? w[r] : 0.f;
+          q[r] = row_sum(same ? 0.f : ekw * dj);
+        }
+        if (cs == 0 && n16 == 0) *reinterpret_cast<f32x4*>(rows + tile * LB + i0) = q;
+      }
+      const Frag8<M> ekf = pair_frag<M>(ek[0], ek[1]), ewf = pair_frag<M>(ew[0], ew[1]);
+#pragma unroll
+      for (int p = 0; p < PW; ++p) dx[p] = mfma8(col_frag<M>(yt, XS, ip * 16, (cs * PW + p) * 16), ekf, dx[p]);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) dk[nt] = mfma8(col_frag<M>(qt, NS, ip * 16, (cs * NT + nt) * 16), ewf, dk[nt]);
+    }
+    colsum = group_sum(colsum);
+    on_diag = group_sum(on_diag);
+    w_diag = group_sum(w_diag);
+    if (cs == 0 && g == 0) {
+      col[tok] = colsum;
+      diag[tok] = on_diag;
+      wjj[tok] = w_diag;
+    }
+    // Rows i of this wave's tile: dq from the columns j <= i, and from the state.
+    const float e_i = ec[tok];
+#pragma unroll
+    for (int jp = 0; jp < TOK; jp += 2) {
+      if (jp > tile) continue;
+      f32x4 ew[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int jt = jp + u;
+        ew[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (jt > tile) continue;
+        f32x4 w = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) w = mfma8(row_frag_t<M>(xt, XS, jt * 16, k * 32), yf[k], w);
+        const int j0 = jt * 16 + 4 * g;
+        const f32x4 hv = *reinterpret_cast<const f32x4*>(hi + j0), lv = *reinterpret_cast<const f32x4*>(lo + j0),
+                    dv = *reinterpret_cast<const f32x4*>(dd + j0);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) ew[u][r] = j0 + r <= tok ? exp2_f((hj - hv[r]) + (lj - lv[r])) * dv[r] * w[r] : 0.f;
+      }
+      const Frag8<M> ewf = pair_frag<M>(ew[0], ew[1]);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) dq[nt] = mfma8(col_frag<M>(kt, NS, jp * 16, (cs * NT + nt) * 16), ewf, dq[nt]);
+    }
+    float dot1 = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      f32x4 r = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = SP - 1; s >= 0; --s) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) r = mfma8(col_frag<M>(st + s * Lds::STATE, NS, k * 32, (cs * NT + nt) * 16), yf[k], r);
+      }
+      const f32x4 qv = lds_row4<M>(qt + tok * NS + (cs * NT + nt) * 16 + 4 * g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        dot1 = fmaf(qv[e], r[e], dot1);
+        dq[nt][e] = fmaf(e_i, r[e], dq[nt][e]);
+      }
+    }
+    dot1 = group_sum(dot1);
+    if (g == 0) t1[cs * LB + tok] = e_i * dot1;
+    __syncthreads();
+    put_state(gr);
+    __syncthreads();
+    // Columns j again: dk and dx from the adjoint.
+    const float e_t = et[tok];
+    float dot2 = 0.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      f32x4 r = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = SP - 1; s >= 0; --s) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) r = mfma8(col_frag<M>(st + s * Lds::STATE, NS, k * 32, (cs * NT + nt) * 16), xf[k], r);
+      }
+      const f32x4 kv = lds_row4<M>(kt + tok * NS + (cs * NT + nt) * 16 + 4 * g);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        dot2 = fmaf(kv[e], r[e], dot2);
+        dk[nt][e] = fmaf(dj * e_t, r[e], dk[nt][e]);
+      }
+    }
+    dot2 = group_sum(dot2);
+    if (g == 0) t2[cs * LB + tok] = e_t * dot2;
+    {
+      Frag8<M> kf[NK];
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<M>(kt, NS, tile * 16, kk * 32);
+#pragma unroll
+      for (int p = 0; p < PW; ++p) {
+        f32x4 u = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) u = mfma8(row_frag<M>(st, NS, (cs * PW + p) * 16, kk * 32), kf[kk], u);
+        const int c = (cs * PW + p) * 16 + 4 * g;
+        const f32x4 yv = lds_row4<M>(yt + tok * XS + c);
+        f32x4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = tok < live ? fmaf(dj, fmaf(e_t, u[e], dx[p][e]), skip * yv[e]) : 0.f;
+        if (tok < in_block) store_row4<E>(dxp + static_cast<int64_t>(tok) * hs * f.P + c, pw - c, pvec, o);
+      }
+    }
+    __syncthreads();
+    // The step sizes, by the wave that holds their scalars.
+    if (wave == 0) {
+      float dc[PL], direct[PL], back = 0.f, tail = 0.f, dskip = 0.f;
+#pragma unroll
+      for (int k = PL - 1; k >= 0; --k) {
+        const int t = lane * PL + k;
+        float s1 = 0.f, s2 = 0.f, rs = 0.f;
+#pragma unroll
+        for (int c = 0; c < CS; ++c) { s1 += t1[c * LB + t]; s2 += t2[c * LB + t]; }
+#pragma unroll
+        for (int j = 0; j < TOK; ++j) rs += j * 16 <= t ? rows[j * LB + t] : 0.f;
+        direct[k] = col[t] + s2;
+        back += (rs - dt[k] * (col[t] - diag[t])) + (s1 - dt[k] * s2);
+        dc[k] = back;  // over this lane's tokens from k on
+        tail += dt[k] * s2;
+        dskip += wjj[t];
+      }
+      float behind = back;  // inclusive suffix sum over the lanes
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const float up = __shfl_down(behind, o);
+        if (lane + o < 64) behind += up;
+      }
+      behind -= back;
+      tail = group_sum(row_sum(tail));
+      float gdot = 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) gdot += gs[k];
+      const float end = fmaf(exp2_d(total), gdot, tail);
+      float da = 0.f, db = 0.f;
+#pragma unroll
+      for (int k = 0; k < PL; ++k) {
+        const int64_t t = lane * PL + k;
+        const float dl = dc[k] + behind + end;
+        float dz = fmaf(rate, dl, direct[k]);
+        if (f.softplus && t < live) {
+          const float z = raw_step<E>(f, b, t0 + t, h);
+          dz *= z > 20.f ? 1.f : 1.f / (1.f + __expf(-z));
+        }
+        dz = t < live ? dz : 0.f;
+        da = fmaf(dt[k], dl, da);
+        db += dz;
+        if (t < in_block) put_step(t, dz);
+      }
+      da = group_sum(row_sum(da));
+      db = group_sum(row_sum(db));
+      dskip = group_sum(row_sum(dskip));
+      if (lane < 3) hpart[lane] = lane == 0 ? da : lane == 1 ? dskip : db;
+    }
+    __syncthreads();
+  }
+
+  // dk and dq of this workgroup's heads.
+  const int64_t all = static_cast<int64_t>(f.B) * f.T * f.G * f.N;
+  const int64_t at = (static_cast<int64_t>(b) * f.T + t0 + tok) * f.G * f.N + static_cast<int64_t>(gi) * f.N;
+  if (t0 + tok < f.T) {
+    const bool on = tok < live;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int c = (cs * NT + nt) * 16 + 4 * g;
+      const f32x4 none = {0.f, 0.f, 0.f, 0.f}, ko = on ? dk[nt] : none, qo = on ? dq[nt] : none;
+      if (a.rows_part != nullptr) {
+        float* p = a.rows_part + static_cast<int64_t>(split) * 2 * all + at + c;
+        store_row4<F32>(p, f.N - c, (f.N & 3) == 0, ko);
+        store_row4<F32>(p + all, f.N - c, (f.N & 3) == 0, qo);
+      } else {
+        store_row4<E>(static_cast<eraw*>(a.dk) + at + c, f.N - c, nvec, ko);
+        store_row4<E>(static_cast<eraw*>(a.dq) + at + c, f.N - c, nvec, qo);
+      }
+    }
+  }
+}
+
+// out[i] = sum of `parts` rows of n floats, in order.
+template <class E>
+__global__ __launch_bounds__(256) void selective_sum_kernel(const float* part, int64_t stride, int parts, void* out, int64_t n,
+                                                            int out_f32) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += step) {
+    float s = part[i];
+    for (int p = 1; p < parts; ++p) s += part[p * stride + i];
+    st_state<E>(out, i, out_f32 != 0, s);
+  }
+}
+
+// dA, dD and the step bias's gradient of a head: the blocks' sums, in a fixed order.
+__global__ __launch_bounds__(256) void selective_head_kernel(const float* part, int64_t blocks, int H, int PT, float* da,
+                                                             float* dskip, float* dbias) {
+  __shared__ float sums[3][4];
+  const int h = static_cast<int>(blockIdx.x), tid = static_cast<int>(threadIdx.x);
+  float s[3] = {0.f, 0.f, 0.f};
+  for (int64_t i = tid; i < blocks * PT; i += 256) {
+    const float* p = part + ((i / PT) * H * PT + static_cast<int64_t>(h) * PT + i % PT) * 3;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) s[k] += p[k];
+  }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const float x = group_sum(row_sum(s[k]));
+    if ((tid & 63) == 0) sums[k][tid >> 6] = x;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    float* out[3] = {da, dskip, dbias};
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      if (out[k] != nullptr) out[k][h] = (sums[k][0] + sums[k][1]) + (sums[k][2] + sums[k][3]);
+    }
+  }
+}
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <class F>
+void with_form(int dtype, int64_t N, F f) {
+  auto by_width = [&](auto e, auto m) {
+    if (N <= 32) f(e, m, std::integral_constant<int, 32>{});
+    else if (N <= 64) f(e, m, std::integral_constant<int, 64>{});
+    else f(e, m, std::integral_constant<int, 128>{});
+  };
+  if (dtype == GRM_HIP_BF16) by_width(BF16{}, BF16{});
+  else if (dtype == GRM_HIP_F16) by_width(F16{}, F32{});
+  else by_width(F32{}, F32{});
+}
+
+// Workspace: the adjoint behind every block, its walk's parts, and the shares' sums.
+struct BwdPlan {
+  int64_t nsave, part_tokens, wgs;
+  int parts, splits, PT;
+  int64_t adj, part_state, part_log, rows, steps, heads, bytes;  // byte offsets
+};
+
+BwdPlan bwd_plan(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G, int64_t N, int dtype) {
+  BwdPlan p{};
+  auto up = [](int64_t n) { return sel_ceil(n, 256) * 256; };
+  p.PT = static_cast<int>(sel_ceil(P, kSelRows));
+  p.nsave = sel_ceil(T, sel_block(dtype));
+  p.parts = sel_parts(B * H * p.PT, T, dtype, &p.part_tokens);
+  // A workgroup for each of 256 CUs; the heads of a group are shared no further, since every share adds
+  // its own K and a float32 copy of dk and dq.
+  p.wgs = B * p.nsave * G;
+  const int64_t heads = H / G * p.PT;
+  int64_t splits = p.wgs > 0 ? sel_ceil(256, p.wgs) : 1;
+  if (splits > heads) splits = heads;
+  p.splits = static_cast<int>(splits);
+  const int64_t state = H * P * N * 4;
+  int64_t at = 0;
+  p.adj = at; at += up(B * p.nsave * state);
+  p.part_state = at; at += p.parts > 1 ? up(p.parts * B * state) : 0;
+  p.part_log = at; at += p.parts > 1 ? up(p.parts * B * H * 8) : 0;
+  p.rows = at; at += p.splits > 1 ? up(p.splits * 2 * B * T * G * N * 4) : 0;
+  p.steps = at; at += p.PT > 1 ? up(p.PT * B * T * H * 4) : 0;
+  p.heads = at; at += up(B * p.nsave * H * p.PT * 12);
+  p.bytes = at;
+  return p;
+}
+
+}  // namespace
+}  // namespace grmhip
+
+using namespace grmhip;
+
+extern "C" int64_t grm_hip_selective_scan_bwd_workspace(int64_t batch, int64_t seq_len, int64_t heads, int64_t value_dim,
+                                                        int64_t groups, int64_t key_dim, int dtype) {
+  if (batch <= 0 || seq_len < 0 || heads <= 0 || value_dim <= 0 || groups <= 0 || heads % groups != 0 || key_dim <= 0 ||
+      dtype < 0 || dtype > 2)
+    return 0;
+  return bwd_plan(batch, seq_len, heads, value_dim, groups, key_dim, dtype).bytes;
+}
+
+extern "C" int grm_hip_selective_scan_bwd(const grm_hip_selective_args* u, const float* states, const void* grad_hidden,
+                                          const float* grad_memory_out, void* grad_keys, void* grad_values,
+                                          void* grad_queries, void* grad_steps, float* grad_rates, float* grad_memory,
+                                          float* grad_skip, float* grad_step_bias, void* workspace,
+                                          int64_t workspace_bytes, void* stream) {
+  const char* what = "selective_scan backward";
+  if (int rc = sel_check(u, what)) return rc;
+  if (grad_rates == nullptr || (u->batch > 0 && grad_memory == nullptr) || !aligned(states) || !aligned(grad_memory_out) ||
+      !aligned(grad_memory) ||
+      (u->batch > 0 && u->seq_len > 0 &&
+       (states == nullptr || grad_hidden == nullptr || grad_keys == nullptr || grad_values == nullptr ||
+        grad_queries == nullptr || grad_steps == nullptr))) {
+    set_error("%s: every gradient but those of skip and step_bias is required, states 16-byte aligned", what);
+    return GRM_HIP_EINVAL;
+  }
+  const BwdPlan p = bwd_plan(u->batch > 0 ? u->batch : 0, u->seq_len, u->heads, u->value_dim, u->groups, u->key_dim, u->dtype);
+  if (u->batch > 0 && (workspace == nullptr || !aligned(workspace) || workspace_bytes < p.bytes)) {
+    set_error("%s: workspace missing, misaligned or too small", what);
+    return GRM_HIP_EINVAL;
+  }
+  if (p.wgs * p.splits > INT32_MAX) {
+    set_error("%s: too many blocks for one launch", what);
+    return GRM_HIP_EUNSUPPORTED;
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  const int64_t rows = u->heads * u->value_dim;
+  if (u->batch > 0) {
+    // The adjoint's walk, from the gradient of the final state to that of the first.
+    SelArgs r = sel_args(u);
+    r.vec = r.vec && aligned(grad_hidden);
+    r.keys = u->queries; r.kb = u->queries_batch_stride; r.kt = u->queries_token_stride;
+    r.values = grad_hidden; r.vb = u->seq_len * rows; r.vt = rows;
+    r.memory = grad_memory_out; r.memory_out = grad_memory;
+    r.states = reinterpret_cast<float*>(ws + p.adj); r.nsave = p.nsave;
+    r.parts = p.parts; r.part_tokens = p.part_tokens;
+    r.part_state = reinterpret_cast<float*>(ws + p.part_state);
+    r.part_log = reinterpret_cast<double*>(ws + p.part_log);
+    if (p.parts > 1) {
+      if (int rc = launch_state_pass(r, u->dtype, true, true, s, what)) return rc;
+    }
+    if (int rc = launch_state_pass(r, u->dtype, true, false, s, what)) return rc;
+  }
+  int rc = GRM_HIP_OK;
+  if (p.wgs > 0) {
+    GradArgs a{};
+    a.s = sel_args(u);
+    a.s.states = const_cast<float*>(states);
+    a.s.nsave = p.nsave;
+    a.s.vec = a.s.vec && aligned(grad_hidden) && aligned(grad_keys) && aligned(grad_values) && aligned(grad_queries);
+    a.dy = grad_hidden; a.adj = reinterpret_cast<const float*>(ws + p.adj);
+    a.dx = grad_values; a.dk = grad_keys; a.dq = grad_queries; a.dsteps = grad_steps;
+    a.rows_part = p.splits > 1 ? reinterpret_cast<float*>(ws + p.rows) : nullptr;
+    a.steps_part = p.PT > 1 ? reinterpret_cast<float*>(ws + p.steps) : nullptr;
+    a.head_part = reinterpret_cast<float*>(ws + p.heads);
+    a.splits = p.splits;
+    with_form(u->dtype, u->key_dim, [&](auto e, auto m, auto np) {
+      using E = decltype(e);
+      using M = decltype(m);
+      constexpr int NP = decltype(np)::value;
+      auto kernel = selective_grad_kernel<E, M, NP>;
+      constexpr size_t lds = GradLds<M, NP>::bytes;
+      const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
+      if (err != hipSuccess) {
+        set_error("%s: %s", what, hipGetErrorString(err));
+        rc = static_cast<int>(err);
+        return;
+      }
+      kernel<<<dim3(static_cast<uint32_t>(p.wgs * p.splits)), dim3(kGradThreads), lds, s>>>(a);
+      if ((rc = check_launch(what)) != GRM_HIP_OK) return;
+      auto sum = [&](const float* part, int64_t stride, int parts, void* out, int64_t n, int f32) {
+        const int64_t blocks = sel_ceil(n, 256);
+        selective_sum_kernel<E><<<dim3(static_cast<uint32_t>(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s>>>(
+            part, stride, parts, out, n, f32);
+        rc = check_launch(what);
+      };
+      if (a.rows_part != nullptr) {
+        const int64_t n = u->batch * u->seq_len * u->groups * u->key_dim;
+        sum(a.rows_part, 2 * n, p.splits, grad_keys, n, 0);
+        if (rc != GRM_HIP_OK) return;
+        sum(a.rows_part + n, 2 * n, p.splits, grad_queries, n, 0);
+        if (rc != GRM_HIP_OK) return;
+      }
+      if (a.steps_part != nullptr) {
+        const int64_t n = u->batch * u->seq_len * u->heads;
+        sum(a.steps_part, n, p.PT, grad_steps, n, u->steps_dtype == GRM_HIP_F32);
+      }
+    });
+    if (rc != GRM_HIP_OK) return rc;
+  }
+  selective_head_kernel<<<dim3(static_cast<uint32_t>(u->heads)), dim3(256), 0, s>>>(
+      reinterpret_cast<const float*>(ws + p.heads), u->batch * p.nsave, static_cast<int>(u->heads), p.PT, grad_rates, grad_skip,
+      grad_step_bias);
+  return check_launch(what);
+}

@@ -48,7 +48,8 @@ def selective_scan(keys, values, queries, steps, rates, memory, skip, step_bias,
             if softplus:
                 d = torch.logaddexp(d, torch.zeros_like(d))
             k, q = (v[b, t].repeat_interleave(H // G, 0) for v in (keys, queries))
-            M = torch.exp(d * rates)[:, None, None] * M + (d[:, None] * values[b, t])[..., None] * k[:, None]
+            rate = rates if rates.ndim == 1 else rates[b, t]  # [B, T, H]: one a token, whose gradients are apart
+            M = torch.exp(d * rate)[:, None, None] * M + (d[:, None] * values[b, t])[..., None] * k[:, None]
             h = (M * q[:, None]).sum(-1)
             rows.append(h if skip is None else h + skip[:, None] * values[b, t])
         hidden.append(torch.stack(rows) if rows else 1.0 * values[b])
