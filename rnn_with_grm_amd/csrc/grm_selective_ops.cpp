@@ -59,9 +59,9 @@ Tensor packed_rows(const Tensor& t, int64_t inner) {
     if (t.size(d) != 1 && t.stride(d) != want) return t.contiguous();
     want *= t.size(d);
   }
-  for (int64_t d = 0; d < t.dim() - inner; ++d) {  // byte offsets inside a tile of tokens stay below 2^31
-    if (t.size(d) != 1 && d > 0 && t.stride(d) > (int64_t{1} << 21)) return t.contiguous();
-  }
+  // Rows of a sequence lie one behind the other, near enough for 32-bit offsets inside a tile of tokens.
+  const int64_t d = t.dim() - inner - 1;
+  if (d > 0 && t.size(d) != 1 && (t.stride(d) < want || t.stride(d) > (int64_t{1} << 21))) return t.contiguous();
   return t;
 }
 

@@ -1,7 +1,6 @@
 // Pieces shared by the selective scan's kernels (selective_scan.hip, selective_bwd.hip).
 //
-// Tiles and fragments.  Token tiles lie in LDS row-major, one row a token, rows padded by 16
-// bytes so that 16 rows fall on distinct banks.  Two orders of the reduction slots are used:
+// Tiles and fragments.  Tiles lie in LDS row-major (a row is a token, or a value row of a state).  Two orders of the reduction slots are used:
 // along a row (key or value dimensions) slot s of lane group g is element 8g + s; along a column
 // (tokens) slots 0-3 are tokens 4g + s and slots 4-7 tokens 16 + 4g + s - 4 of a 32-token step,
 // which is how two 16x16 accumulators sit in the registers, so that a product feeds the next one
@@ -28,8 +27,6 @@ struct SelShape {
   static constexpr bool kHalf = sizeof(typename ET<M>::raw) == 2;
   static constexpr int L = kHalf ? 64 : 32;       // tokens of a walk's chunk
   static constexpr int LB = kHalf ? 128 : 64;     // tokens of a backward chunk (states are kept this often)
-  static constexpr int PAD = kHalf ? 8 : 4;       // 16 bytes
-  static constexpr int XS = kSelRows + PAD;       // value row stride
   static constexpr int PARTS = kHalf ? 3 : 1;     // bfloat16 parts that hold a float32 (24 bits)
 };
 
@@ -73,15 +70,58 @@ __device__ __forceinline__ int64_t sel_length(const SelArgs& a, int b) {
   return a.lengths == nullptr ? a.T : max_i64(0, min_i64(a.lengths[b], a.T));
 }
 
+// A token's entry of steps as it lies in memory (16 bits in the low half), 0 where not `live`.  Nothing is
+// done to it here, so that a load ahead of time is waited for where it is used.
+template <class E>
+__device__ __forceinline__ uint32_t load_step(const SelArgs& a, int b, int64_t t, int h, bool live) {
+  const int64_t at = b * a.sb + t * a.st + h;
+  uint32_t v = 0;
+  if (a.steps_f32 || std::is_same_v<E, F32>) {
+    if (live) v = static_cast<const uint32_t*>(a.steps)[at];
+  } else {
+    if (live) v = static_cast<const uint16_t*>(a.steps)[at];
+  }
+  return v;
+}
+template <class E>
+__device__ __forceinline__ float step_value(const SelArgs& a, uint32_t v) {
+  if constexpr (std::is_same_v<E, F32>) return __uint_as_float(v);
+  else return a.steps_f32 ? __uint_as_float(v) : ET<E>::to_f(static_cast<uint16_t>(v));
+}
 // steps + bias of a token, before softplus.
 template <class E>
 __device__ __forceinline__ float raw_step(const SelArgs& a, int b, int64_t t, int h) {
-  const float z = ld_state<E>(a.steps, b * a.sb + t * a.st + h, a.steps_f32 != 0);
+  const float z = step_value<E>(a, load_step<E>(a, b, t, h, true));
   return a.bias == nullptr ? z : z + a.bias[h];
 }
 
 __device__ __forceinline__ float step_size(const SelArgs& a, float z) {
   return !a.softplus || z > 20.f ? z : log1pf(__expf(z));
+}
+
+// x of the lane that a DPP control names, 0 where it names none or the row mask leaves this row out.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double dpp_f64(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(b), CTRL, ROWS, 0xf, false);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(b >> 32), CTRL, ROWS, 0xf, false);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+// Inclusive prefix sum over the wave: inside rows of 16 lanes, then from row to row.
+__device__ __forceinline__ double wave_prefix(double x) {
+  x += dpp_f64<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+  x += dpp_f64<0x112, 0xf>(x);
+  x += dpp_f64<0x114, 0xf>(x);
+  x += dpp_f64<0x118, 0xf>(x);
+  x += dpp_f64<0x142, 0xa>(x);  // lane 15 of rows 0 and 2 to the next row
+  x += dpp_f64<0x143, 0xc>(x);  // lane 31 to rows 2 and 3
+  return x;
+}
+__device__ __forceinline__ double lane_value(double x, int lane) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(b), lane);
+  const uint32_t hi = __builtin_amdgcn_readlane(static_cast<int>(b >> 32), lane);
+  return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
 
 // One wave's scan over a chunk's log decays, lane = token.  In log2 units and float64: a chunk's
@@ -93,35 +133,54 @@ struct TokenScalars {
   double total;   // of the whole chunk
 };
 
-template <class E, int L>
-__device__ __forceinline__ TokenScalars token_scalars(const SelArgs& a, int b, int h, int64_t t, int64_t n, float rate) {
-  const int lane = lane_id();
+template <int L>
+__device__ __forceinline__ TokenScalars token_scalars(const SelArgs& a, float z, bool live, float rate) {
   TokenScalars s;
-  s.d = lane < L && t < n ? step_size(a, raw_step<E>(a, b, t, h)) : 0.f;
+  s.d = lane_id() < L && live ? step_size(a, z) : 0.f;
   double l = static_cast<double>(s.d) * static_cast<double>(rate);
   l = l < -200.0 ? -200.0 : l;
   l *= 1.4426950408889634;  // log2(e)
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const double up = __shfl_up(l, o);
-    if (lane >= o) l += up;
-  }
-  s.cum = l;
-  s.total = __shfl(l, L - 1);
+  s.cum = wave_prefix(l);
+  s.total = lane_value(s.cum, L - 1);
   return s;
 }
 
+// LDS tiles with rows of W elements, padded against bank conflicts (64 banks of 4 bytes).  Measured with
+// SQ_LDS_BANK_CONFLICT, clocks per read of one wave:
+//                                     rows 4 banks apart   8 banks apart
+//   transpose read (8 rows x 32 bytes)        4                  2
+//   16 bytes of each of 16 rows               8                  4
+//   8 bytes of each of 16 rows                2                  4
+// COLS: 8 banks apart modulo 64, for tiles read by columns (and rows in 16 bytes); else 4, for tiles
+// read by rows in 8 bytes.  (XORed granules without padding are as good for the transpose reads, but
+// their addresses differ from lane to lane, so that the two halves of a fragment are no constant
+// distance apart: slower.)  Float32 tiles: 4 banks apart.
+template <class M, int W, bool COLS>
+struct SelTile {
+  static constexpr bool kHalf = SelShape<M>::kHalf;
+  static constexpr int STRIDE = W + (!kHalf ? 4 : COLS ? 16 : 8);
+  __device__ __forceinline__ static int at(int row, int col) { return row * STRIDE + col; }
+};
+
 // Fragment of 16 rows (row + lane % 16), reduction along the row from `col`.
-template <class M>
-__device__ __forceinline__ Frag8<M> row_frag(const typename ET<M>::raw* tile, int stride, int row, int col) {
+template <class T, class M>
+__device__ __forceinline__ Frag8<M> row_frag(const typename ET<M>::raw* tile, int row, int col) {
   const int lane = lane_id();
-  const typename ET<M>::raw* p = tile + (row + (lane & 15)) * stride + col + 8 * (lane >> 4);
-  return lds_frag_4x2<M>(p, p + 4);
+  const typename ET<M>::raw* p = tile + T::at(row + (lane & 15), col + 8 * (lane >> 4));
+  if constexpr (sizeof(typename ET<M>::raw) == 2) return __builtin_bit_cast(Frag8<M>, *reinterpret_cast<const uint4*>(p));
+  else return lds_frag_4x2<M>(p, p + 4);
+}
+
+// The same with the reduction in the tokens' slot order (4g + s, 16 + 4g + s).
+template <class T, class M>
+__device__ __forceinline__ Frag8<M> row_frag_t(const typename ET<M>::raw* tile, int row, int col) {
+  const int lane = lane_id(), r = row + (lane & 15), c = col + 4 * (lane >> 4);
+  return lds_frag_4x2<M>(tile + T::at(r, c), tile + T::at(r, c + 16));
 }
 
 // Fragment of 16 columns (col + lane % 16), reduction over 32 tokens from row `t0`.
-template <class M>
-__device__ __forceinline__ Frag8<M> col_frag(const typename ET<M>::raw* tile, int stride, int t0, int col) {
+template <class T, class M>
+__device__ __forceinline__ Frag8<M> col_frag(const typename ET<M>::raw* tile, int t0, int col) {
   const int lane = lane_id(), g = lane >> 4, n = lane & 15;
   Frag8<M> f;
   if constexpr (sizeof(typename ET<M>::raw) == 2) {
@@ -129,20 +188,21 @@ __device__ __forceinline__ Frag8<M> col_frag(const typename ET<M>::raw* tile, in
     // passes &X[r0 + (s >> 2)][c0 + 4 (s & 3)].
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    const typename ET<M>::raw* p = tile + (t0 + 4 * g + (n >> 2)) * stride + col + 4 * (n & 3);
+    const typename ET<M>::raw* p = tile + T::at(t0 + 4 * g + (n >> 2), col + 4 * (n & 3));
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 16 * stride));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 16 * T::STRIDE));
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       f.e[e] = static_cast<uint16_t>(lo[e]);
       f.e[4 + e] = static_cast<uint16_t>(hi[e]);
     }
   } else {
-    const float* p = tile + (t0 + 4 * g) * stride + col + n;
+    constexpr int S = T::STRIDE;
+    const float* p = tile + (t0 + 4 * g) * S + col + n;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      f.e[e] = p[e * stride];
-      f.e[4 + e] = p[(16 + e) * stride];
+      f.e[e] = p[e * S];
+      f.e[4 + e] = p[(16 + e) * S];
     }
   }
   return f;
@@ -177,35 +237,82 @@ __device__ __forceinline__ void split_frag(const float (&v)[8], Frag8<M> (&out)[
 }
 
 // Rows [0, ROWS) x [0, COLS) of a tile from global memory into registers (8 elements a unit, units dealt to
-// THREADS threads), then into LDS as M.  Rows from `rows` on and columns from `cols` on are zeros.
-template <class E, class M, int ROWS, int COLS, int THREADS>
+// THREADS threads), then into LDS as M.  Rows from `rows` on and columns from `cols` on are zeros: they
+// lie outside the buffer resource or are sent there, so no load stands behind a branch and all stay in
+// flight until the tile is stored.
+// VEC: every row's units are whole 16-byte accesses.
+template <class E, class T, class M, bool VEC, int ROWS, int COLS, int THREADS>
 struct TileLoad {
-  static constexpr int UPR = COLS / 8, UNITS = ROWS * UPR, PER = (UNITS + THREADS - 1) / THREADS;
-  U8<E> r[PER];
-  __device__ __forceinline__ void load(const void* base, int64_t at, int64_t stride, int64_t rows, int cols, bool vec,
-                                       int tid) {
-    const typename ET<E>::raw* p = static_cast<const typename ET<E>::raw*>(base) + at;
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  static constexpr int ES = static_cast<int>(sizeof(typename ET<E>::raw));
+  static constexpr int UPR = COLS / 8, UNITS = ROWS * UPR, PER = (UNITS + THREADS - 1) / THREADS, W = ES / 2;
+  static constexpr int DROW = THREADS / UPR;  // rows between a thread's units
+  static_assert(THREADS % UPR == 0 && (UNITS % THREADS == 0 || PER == 1), "a thread's units share a column");
+  u32x4 r[PER][W];
+  int off;          // byte offset of this thread's first unit, out of range where its column is
+  int at;           // element in the LDS tile
+  int step, width;  // bytes from row to row, columns
+
+  // stride in elements, at least cols.
+  __device__ __forceinline__ void init(int64_t stride, int cols, int tid) {
+    step = static_cast<int>(stride) * ES;
+    width = cols;
+    const int row = tid / UPR, col = tid % UPR * 8;
+    off = col < cols && tid < UNITS ? row * step + col * ES : kBufOOB;
+    at = T::at(row, col);
+  }
+  // base: the first row's first element.
+  __device__ __forceinline__ void load(const typename ET<E>::raw* base, int64_t rows, int tid) {
+    const int n = static_cast<int>(max_i64(0, min_i64(rows, ROWS)));
+    const __amdgpu_buffer_rsrc_t rsrc =
+        make_rsrc(base, n > 0 ? static_cast<uint32_t>((n - 1) * step + width * ES) : 0u);
+    if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int u = tid + i * THREADS, row = u / UPR, col = u % UPR * 8;
-      r[i] = load_u8<E>(p + row * stride, col, cols, u < UNITS && row < rows, vec);
+      for (int i = 0; i < PER; ++i) {
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+          r[i][w] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + 16 * w, i * DROW * step, 0);
+      }
+    } else {
+      const int col = tid % UPR * 8;
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const int row = tid / UPR + i * DROW;
+        const bool in = tid < UNITS && row < n;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if constexpr (ES == 4) {
+              const int c = col + 4 * w + k;
+              r[i][w][k] = __builtin_amdgcn_raw_buffer_load_b32(rsrc, in && c < width ? row * step + c * 4 : kBufOOB, 0, 0);
+            } else {
+              const int c = col + 2 * k;
+              const uint32_t lo = static_cast<uint16_t>(
+                  __builtin_amdgcn_raw_buffer_load_b16(rsrc, in && c < width ? row * step + c * 2 : kBufOOB, 0, 0));
+              const uint32_t hi = static_cast<uint16_t>(
+                  __builtin_amdgcn_raw_buffer_load_b16(rsrc, in && c + 1 < width ? row * step + c * 2 + 2 : kBufOOB, 0, 0));
+              r[i][w][k] = lo | hi << 16;
+            }
+          }
+        }
+      }
     }
   }
-  __device__ __forceinline__ void store(typename ET<M>::raw* tile, int stride, int tid) const {
+  __device__ __forceinline__ void store(typename ET<M>::raw* tile, int tid) const {
+    if (UNITS < THREADS && tid >= UNITS) return;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int u = tid + i * THREADS, row = u / UPR, col = u % UPR * 8;
-      if (u < UNITS) {
-        typename ET<M>::raw* p = tile + row * stride + col;
-        if constexpr (sizeof(typename ET<M>::raw) == 2) {
-          *reinterpret_cast<uint4*>(p) = __builtin_bit_cast(uint4, r[i]);
-        } else {
-          float4 lo, hi;
-          lo.x = ET<E>::to_f(r[i].e[0]); lo.y = ET<E>::to_f(r[i].e[1]); lo.z = ET<E>::to_f(r[i].e[2]); lo.w = ET<E>::to_f(r[i].e[3]);
-          hi.x = ET<E>::to_f(r[i].e[4]); hi.y = ET<E>::to_f(r[i].e[5]); hi.z = ET<E>::to_f(r[i].e[6]); hi.w = ET<E>::to_f(r[i].e[7]);
-          reinterpret_cast<float4*>(p)[0] = lo;
-          reinterpret_cast<float4*>(p)[1] = hi;
-        }
+      typename ET<M>::raw* p = tile + at + i * DROW * T::STRIDE;
+      if constexpr (ES == sizeof(typename ET<M>::raw)) {
+#pragma unroll
+        for (int w = 0; w < W; ++w) reinterpret_cast<u32x4*>(p)[w] = r[i][w];
+      } else {
+        const U8<E> e = __builtin_bit_cast(U8<E>, r[i][0]);
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+          reinterpret_cast<float4*>(p)[w] = make_float4(ET<E>::to_f(e.e[4 * w]), ET<E>::to_f(e.e[4 * w + 1]),
+                                                        ET<E>::to_f(e.e[4 * w + 2]), ET<E>::to_f(e.e[4 * w + 3]));
       }
     }
   }
@@ -257,43 +364,52 @@ __device__ __forceinline__ void state_store(const f32x4 (&acc)[NT], float* s, in
   }
 }
 
-// acc = decay acc + sum_t weight_t x_t[p] k_t^T over a chunk's L tokens: x the value tile (this wave's 16 rows from
-// column `xc`), k the key tile.  weight_t x_t is a float32 number, kept whole as three bfloat16 parts:
-// the state is carried over thousands of tokens, where a rounding to fewer bits would add up.
-template <class M, int L, int NT>
-__device__ __forceinline__ void state_update(f32x4 (&acc)[NT], const typename ET<M>::raw* k, int ks,
-                                             const typename ET<M>::raw* x, int xs, int xc, const float* weight,
-                                             float decay) {
-  constexpr int PARTS = SelShape<M>::PARTS;
-  const int g = lane_id() >> 4;
+// The state's update acc = decay acc + sum_t weight_t x_t[p] k_t^T, 32 tokens at a time.  weight_t x_t is a float32
+// number, kept whole as three bfloat16 parts: the state is carried over thousands of tokens, where a
+// rounding to fewer bits would add up.
+template <class M>
+__device__ __forceinline__ void weigh_frag(const Frag8<M>& x, f32x4 w0, f32x4 w1, Frag8<M> (&part)[SelShape<M>::PARTS]) {
+  float v[8];
 #pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) acc[nt][r] *= decay;
+  for (int e = 0; e < 4; ++e) {
+    v[e] = ET<M>::to_f(x.e[e]) * w0[e];
+    v[4 + e] = ET<M>::to_f(x.e[4 + e]) * w1[e];
   }
+  split_frag<M, SelShape<M>::PARTS>(v, part);
+}
+template <class M, int NT>
+__device__ __forceinline__ void update_step(f32x4 (&acc)[NT], const Frag8<M> (&kf)[NT],
+                                            const Frag8<M> (&part)[SelShape<M>::PARTS]) {
 #pragma unroll
-  for (int t0 = 0; t0 < L; t0 += 32) {
-    const Frag8<M> xf = col_frag<M>(x, xs, t0, xc);
-    const f32x4 w0 = *reinterpret_cast<const f32x4*>(weight + t0 + 4 * g);
-    const f32x4 w1 = *reinterpret_cast<const f32x4*>(weight + t0 + 16 + 4 * g);
-    float v[8];
+  for (int p = SelShape<M>::PARTS - 1; p >= 0; --p) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[e] = ET<M>::to_f(xf.e[e]) * w0[e];
-      v[4 + e] = ET<M>::to_f(xf.e[4 + e]) * w1[e];
-    }
-    Frag8<M> part[PARTS];
-    split_frag<M, PARTS>(v, part);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const Frag8<M> kf = col_frag<M>(k, ks, t0, nt * 16);
-#pragma unroll
-      for (int p = PARTS - 1; p >= 0; --p) acc[nt] = mfma8(kf, part[p], acc[nt]);
-    }
+    for (int nt = 0; nt < NT; ++nt) acc[nt] = mfma8(kf[nt], part[p], acc[nt]);
   }
 }
+template <class T, class M, int NT>
+__device__ __forceinline__ void key_frags(Frag8<M> (&kf)[NT], const typename ET<M>::raw* k, int t0) {
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) kf[nt] = col_frag<T, M>(k, t0, nt * 16);
+}
+// Keeps what stands before it before it: reads issued ahead stay ahead.
+__device__ __forceinline__ void hold_order() { __builtin_amdgcn_sched_barrier(0); }
 
-// Host side.
+// Host side: f(E, M, NP, VEC) with one of the compiled forms.
+template <class F>
+void sel_with_form(int dtype, int64_t N, bool vec, F f) {
+  auto by_vec = [&](auto e, auto m, auto np) {
+    if (vec) f(e, m, np, std::true_type{});
+    else f(e, m, np, std::false_type{});
+  };
+  auto by_width = [&](auto e, auto m) {
+    if (N <= 32) by_vec(e, m, std::integral_constant<int, 32>{});
+    else if (N <= 64) by_vec(e, m, std::integral_constant<int, 64>{});
+    else by_vec(e, m, std::integral_constant<int, 128>{});
+  };
+  if (dtype == GRM_HIP_BF16) by_width(BF16{}, BF16{});
+  else if (dtype == GRM_HIP_F16) by_width(F16{}, F32{});
+  else by_width(F32{}, F32{});
+}
 inline int64_t sel_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 int sel_check(const struct grm_hip_selective_args* u, const char* what);
 SelArgs sel_args(const struct grm_hip_selective_args* u);

@@ -48,7 +48,7 @@ struct GradArgs {
 template <class M, int NP>
 struct GradLds {
   using S = SelShape<M>;
-  static constexpr int LB = S::LB, NS = NP + S::PAD, XS = S::XS;
+  static constexpr int LB = S::LB, NS = SelTile<M, NP, true>::STRIDE, XS = SelTile<M, kSelRows, true>::STRIDE;
   static constexpr int SPARTS = S::kHalf ? 2 : 1;             // parts of S and G in LDS
   static constexpr int STATE = kSelRows * NS;
   static constexpr int TILES = LB * (2 * NS + 2 * XS) + SPARTS * STATE;
@@ -78,14 +78,6 @@ __device__ __forceinline__ float group_sum(float x) {
   return x + __shfl_xor(x, 32);
 }
 
-// Fragment of 16 rows, reduction along the row in the tokens' slot order (4g + s, 16 + 4g + s).
-template <class M>
-__device__ __forceinline__ Frag8<M> row_frag_t(const typename ET<M>::raw* tile, int stride, int row, int col) {
-  const int lane = lane_id();
-  const typename ET<M>::raw* p = tile + (row + (lane & 15)) * stride + col + 4 * (lane >> 4);
-  return lds_frag_4x2<M>(p, p + 16);
-}
-
 template <class E>
 __device__ __forceinline__ void store_row4(typename ET<E>::raw* p, int left, bool vec, f32x4 v) {
   if (vec) {
@@ -98,13 +90,15 @@ __device__ __forceinline__ void store_row4(typename ET<E>::raw* p, int left, boo
   }
 }
 
-template <class E, class M, int NP>
-__global__ __launch_bounds__(kGradThreads, 1) void selective_grad_kernel(GradArgs a) {
+template <class E, class M, int NP, bool VEC>
+__global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void selective_grad_kernel(GradArgs a) {
   using S = SelShape<M>;
   using Lds = GradLds<M, NP>;
   using raw = typename ET<M>::raw;
   using eraw = typename ET<E>::raw;
-  constexpr int LB = S::LB, NS = Lds::NS, XS = S::XS, TOK = Lds::TOK, CS = Lds::CS, SP = Lds::SPARTS;
+  using KT = SelTile<M, NP, true>;        // keys, queries, state rows
+  using XT = SelTile<M, kSelRows, true>;  // values and their gradients
+  constexpr int LB = S::LB, NS = Lds::NS, XS = Lds::XS, TOK = Lds::TOK, CS = Lds::CS, SP = Lds::SPARTS;
   constexpr int NK = NP / 32, NT = NP / 16 / CS, PW = kSelRows / 16 / CS, PL = (LB + 63) / 64;
   constexpr int SU = kSelRows * NP / 4 / kGradThreads;  // float4 of a state per thread
   static_assert(SU >= 1 && SU * kGradThreads * 4 == kSelRows * NP, "states split evenly");
@@ -129,7 +123,7 @@ __global__ __launch_bounds__(kGradThreads, 1) void selective_grad_kernel(GradArg
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int tile = wave % TOK, cs = wave / TOK, tok = tile * 16 + n16;  // this lane's token in both orders
   const int64_t len = sel_length(f, b), t0 = static_cast<int64_t>(blk) * LB, live = len - t0;
-  const bool vec = f.vec != 0, nvec = vec && (f.N & 3) == 0, pvec = vec && (f.P & 3) == 0;
+  const bool nvec = VEC && (f.N & 3) == 0, pvec = VEC && (f.P & 3) == 0;
   const int heads = f.H / f.G * f.PT;  // (head, value tile) pairs of the group
   const int h_lo = static_cast<int>(static_cast<int64_t>(heads) * split / a.splits),
             h_hi = static_cast<int>(static_cast<int64_t>(heads) * (split + 1) / a.splits);
@@ -138,22 +132,24 @@ __global__ __launch_bounds__(kGradThreads, 1) void selective_grad_kernel(GradArg
 #pragma unroll
   for (int i = 0; i < NT; ++i) dk[i] = dq[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (live > 0) {
-    TileLoad<E, M, LB, NP, kGradThreads> r;
-    r.load(f.keys, b * f.kb + t0 * f.kt + static_cast<int64_t>(gi) * f.N, f.kt, live, f.N, vec, tid);
-    r.store(kt, NS, tid);
-    r.load(f.queries, b * f.qb + t0 * f.qt + static_cast<int64_t>(gi) * f.N, f.qt, live, f.N, vec, tid);
-    r.store(qt, NS, tid);
+    TileLoad<E, KT, M, VEC, LB, NP, kGradThreads> r;
+    r.init(f.kt, f.N, tid);
+    r.load(static_cast<const eraw*>(f.keys) + b * f.kb + t0 * f.kt + gi * f.N, live, tid);
+    r.store(kt, tid);
+    r.init(f.qt, f.N, tid);
+    r.load(static_cast<const eraw*>(f.queries) + b * f.qb + t0 * f.qt + gi * f.N, live, tid);
+    r.store(qt, tid);
     __syncthreads();
     // K: rows i of every tile from this wave's on, columns j of this wave's tile.
     Frag8<M> kf[NK];
 #pragma unroll
-    for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<M>(kt, NS, tile * 16, kk * 32);
+    for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<KT, M>(kt, tile * 16, kk * 32);
 #pragma unroll
     for (int it = 0; it < TOK; ++it) {
       score[it] = f32x4{0.f, 0.f, 0.f, 0.f};
       if (it >= tile) {
 #pragma unroll
-        for (int kk = 0; kk < NK; ++kk) score[it] = mfma8(row_frag<M>(qt, NS, it * 16, kk * 32), kf[kk], score[it]);
+        for (int kk = 0; kk < NK; ++kk) score[it] = mfma8(row_frag<KT, M>(qt, it * 16, kk * 32), kf[kk], score[it]);
       }
     }
   }
@@ -182,9 +178,11 @@ __global__ __launch_bounds__(kGradThreads, 1) void selective_grad_kernel(GradArg
     const float rate = f.rates[h], skip = f.skip == nullptr ? 0.f : f.skip[h];
 
     // The head's rows, the state and the adjoint.
-    TileLoad<E, M, LB, kSelRows, kGradThreads> xr, yr;
-    xr.load(f.values, b * f.vb + t0 * f.vt + static_cast<int64_t>(h) * f.P + p0, f.vt, live, pw, vec, tid);
-    yr.load(a.dy, row0 * f.P + p0, hs * f.P, live, pw, vec, tid);
+    TileLoad<E, XT, M, VEC, LB, kSelRows, kGradThreads> xr, yr;
+    xr.init(f.vt, pw < kSelRows ? pw : kSelRows, tid);
+    xr.load(static_cast<const eraw*>(f.values) + b * f.vb + t0 * f.vt + h * f.P + p0, live, tid);
+    yr.init(hs * f.P, pw < kSelRows ? pw : kSelRows, tid);
+    yr.load(static_cast<const eraw*>(a.dy) + row0 * f.P + p0, live, tid);
     const int64_t sat = ((static_cast<int64_t>(b) * f.nsave + blk) * f.H + h) * f.P * f.N;
     f32x4 gr[SU], sr[SU];
     auto load_state = [&](const float* base, f32x4 (&r)[SU]) {
@@ -208,7 +206,7 @@ __global__ __launch_bounds__(kGradThreads, 1) void selective_grad_kernel(GradArg
 #pragma unroll
       for (int i = 0; i < SU; ++i) {
         const int u = tid + i * kGradThreads;
-        raw* q = st + u / (NP / 4) * NS + u % (NP / 4) * 4;
+        raw* q = st + KT::at(u / (NP / 4), u % (NP / 4) * 4);
         f32x4 rest = r[i];
 #pragma unroll
         for (int s = 0; s < SP; ++s) {
@@ -235,14 +233,8 @@ __global__ __launch_bounds__(kGradThreads, 1) void selective_grad_kernel(GradArg
         total += l * 1.4426950408889634;
         cum[k] = total;
       }
-      double scan = total;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const double up = __shfl_up(scan, o);
-        if (lane >= o) scan += up;
-      }
-      const double before = scan - total;
-      total = __shfl(scan, 63);
+      const double scan = wave_prefix(total), before = scan - total;
+      total = lane_value(scan, 63);
 #pragma unroll
       for (int k = 0; k < PL; ++k) {
         cum[k] += before;
@@ -255,8 +247,8 @@ __global__ __launch_bounds__(kGradThreads, 1) void selective_grad_kernel(GradArg
         et[t] = exp2_d(total - cum[k]);
       }
     }
-    xr.store(xt, XS, tid);
-    yr.store(yt, XS, tid);
+    xr.store(xt, tid);
+    yr.store(yt, tid);
     put_state(sr);
     float dot = 0.f;
 #pragma unroll
@@ -275,8 +267,8 @@ __global__ __launch_bounds__(kGradThreads, 1) void selective_grad_kernel(GradArg
     Frag8<M> xf[2], yf[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      xf[k] = row_frag_t<M>(xt, XS, tile * 16, k * 32);
-      yf[k] = row_frag_t<M>(yt, XS, tile * 16, k * 32);
+      xf[k] = row_frag_t<XT, M>(xt, tile * 16, k * 32);
+      yf[k] = row_frag_t<XT, M>(yt, tile * 16, k * 32);
     }
     const float hj = hi[tok], lj = lo[tok], dj = dd[tok];
     float colsum = 0.f, on_diag = 0.f, w_diag = 0.f;
@@ -291,7 +283,7 @@ __global__ __launch_bounds__(kGradThreads, 1) void selective_grad_kernel(GradArg
         if (it < tile) continue;
         f32x4 w = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < 2; ++k) w = mfma8(row_frag_t<M>(yt, XS, it * 16, k * 32), xf[k], w);
+        for (int k = 0; k < 2; ++k) w = mfma8(row_frag_t<XT, M>(yt, it * 16, k * 32), xf[k], w);
         const int i0 = it * 16 + 4 * g;
         const f32x4 hv = *reinterpret_cast<const f32x4*>(hi + i0), lv = *reinterpret_cast<const f32x4*>(lo + i0);
         f32x4 q;
@@ -312,9 +304,9 @@ __global__ __launch_bounds__(kGradThreads, 1) void selective_grad_kernel(GradArg
       }
       const Frag8<M> ekf = pair_frag<M>(ek[0], ek[1]), ewf = pair_frag<M>(ew[0], ew[1]);
 #pragma unroll
-      for (int p = 0; p < PW; ++p) dx[p] = mfma8(col_frag<M>(yt, XS, ip * 16, (cs * PW + p) * 16), ekf, dx[p]);
+      for (int p = 0; p < PW; ++p) dx[p] = mfma8(col_frag<XT, M>(yt, ip * 16, (cs * PW + p) * 16), ekf, dx[p]);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) dk[nt] = mfma8(col_frag<M>(qt, NS, ip * 16, (cs * NT + nt) * 16), ewf, dk[nt]);
+      for (int nt = 0; nt < NT; ++nt) dk[nt] = mfma8(col_frag<KT, M>(qt, ip * 16, (cs * NT + nt) * 16), ewf, dk[nt]);
     }
     colsum = group_sum(colsum);
     on_diag = group_sum(on_diag);
@@ -337,7 +329,7 @@ __global__ __launch_bounds__(kGradThreads, 1) void selective_grad_kernel(GradArg
         if (jt > tile) continue;
         f32x4 w = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < 2; ++k) w = mfma8(row_frag_t<M>(xt, XS, jt * 16, k * 32), yf[k], w);
+        for (int k = 0; k < 2; ++k) w = mfma8(row_frag_t<XT, M>(xt, jt * 16, k * 32), yf[k], w);
         const int j0 = jt * 16 + 4 * g;
         const f32x4 hv = *reinterpret_cast<const f32x4*>(hi + j0), lv = *reinterpret_cast<const f32x4*>(lo + j0),
                     dv = *reinterpret_cast<const f32x4*>(dd + j0);
@@ -346,7 +338,7 @@ __global__ __launch_bounds__(kGradThreads, 1) void selective_grad_kernel(GradArg
       }
       const Frag8<M> ewf = pair_frag<M>(ew[0], ew[1]);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) dq[nt] = mfma8(col_frag<M>(kt, NS, jp * 16, (cs * NT + nt) * 16), ewf, dq[nt]);
+      for (int nt = 0; nt < NT; ++nt) dq[nt] = mfma8(col_frag<KT, M>(kt, jp * 16, (cs * NT + nt) * 16), ewf, dq[nt]);
     }
     float dot1 = 0.f;
 #pragma unroll
@@ -355,9 +347,9 @@ __global__ __launch_bounds__(kGradThreads, 1) void selective_grad_kernel(GradArg
 #pragma unroll
       for (int s = SP - 1; s >= 0; --s) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) r = mfma8(col_frag<M>(st + s * Lds::STATE, NS, k * 32, (cs * NT + nt) * 16), yf[k], r);
+        for (int k = 0; k < 2; ++k) r = mfma8(col_frag<KT, M>(st + s * Lds::STATE, k * 32, (cs * NT + nt) * 16), yf[k], r);
       }
-      const f32x4 qv = lds_row4<M>(qt + tok * NS + (cs * NT + nt) * 16 + 4 * g);
+      const f32x4 qv = lds_row4<M>(qt + KT::at(tok, (cs * NT + nt) * 16 + 4 * g));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         dot1 = fmaf(qv[e], r[e], dot1);
@@ -378,9 +370,9 @@ __global__ __launch_bounds__(kGradThreads, 1) void selective_grad_kernel(GradArg
 #pragma unroll
       for (int s = SP - 1; s >= 0; --s) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) r = mfma8(col_frag<M>(st + s * Lds::STATE, NS, k * 32, (cs * NT + nt) * 16), xf[k], r);
+        for (int k = 0; k < 2; ++k) r = mfma8(col_frag<KT, M>(st + s * Lds::STATE, k * 32, (cs * NT + nt) * 16), xf[k], r);
       }
-      const f32x4 kv = lds_row4<M>(kt + tok * NS + (cs * NT + nt) * 16 + 4 * g);
+      const f32x4 kv = lds_row4<M>(kt + KT::at(tok, (cs * NT + nt) * 16 + 4 * g));
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         dot2 = fmaf(kv[e], r[e], dot2);
@@ -392,14 +384,14 @@ __global__ __launch_bounds__(kGradThreads, 1) void selective_grad_kernel(GradArg
     {
       Frag8<M> kf[NK];
 #pragma unroll
-      for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<M>(kt, NS, tile * 16, kk * 32);
+      for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<KT, M>(kt, tile * 16, kk * 32);
 #pragma unroll
       for (int p = 0; p < PW; ++p) {
         f32x4 u = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int kk = 0; kk < NK; ++kk) u = mfma8(row_frag<M>(st, NS, (cs * PW + p) * 16, kk * 32), kf[kk], u);
+        for (int kk = 0; kk < NK; ++kk) u = mfma8(row_frag<KT, M>(st, (cs * PW + p) * 16, kk * 32), kf[kk], u);
         const int c = (cs * PW + p) * 16 + 4 * g;
-        const f32x4 yv = lds_row4<M>(yt + tok * XS + c);
+        const f32x4 yv = lds_row4<M>(yt + XT::at(tok, c));
         f32x4 o;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = tok < live ? fmaf(dj, fmaf(e_t, u[e], dx[p][e]), skip * yv[e]) : 0.f;
@@ -520,18 +512,6 @@ __global__ __launch_bounds__(256) void selective_head_kernel(const float* part, 
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-template <class F>
-void with_form(int dtype, int64_t N, F f) {
-  auto by_width = [&](auto e, auto m) {
-    if (N <= 32) f(e, m, std::integral_constant<int, 32>{});
-    else if (N <= 64) f(e, m, std::integral_constant<int, 64>{});
-    else f(e, m, std::integral_constant<int, 128>{});
-  };
-  if (dtype == GRM_HIP_BF16) by_width(BF16{}, BF16{});
-  else if (dtype == GRM_HIP_F16) by_width(F16{}, F32{});
-  else by_width(F32{}, F32{});
-}
-
 // Workspace: the adjoint behind every block, its walk's parts, and the shares' sums.
 struct BwdPlan {
   int64_t nsave, part_tokens, wgs;
@@ -633,11 +613,11 @@ extern "C" int grm_hip_selective_scan_bwd(const grm_hip_selective_args* u, const
     a.steps_part = p.PT > 1 ? reinterpret_cast<float*>(ws + p.steps) : nullptr;
     a.head_part = reinterpret_cast<float*>(ws + p.heads);
     a.splits = p.splits;
-    with_form(u->dtype, u->key_dim, [&](auto e, auto m, auto np) {
+    sel_with_form(u->dtype, u->key_dim, a.s.vec != 0, [&](auto e, auto m, auto np, auto vec) {
       using E = decltype(e);
       using M = decltype(m);
       constexpr int NP = decltype(np)::value;
-      auto kernel = selective_grad_kernel<E, M, NP>;
+      auto kernel = selective_grad_kernel<E, M, NP, decltype(vec)::value>;
       constexpr size_t lds = GradLds<M, NP>::bytes;
       const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));

@@ -9,10 +9,11 @@
 //
 // One workgroup walks one (sequence, head, 64 value rows) chunk by chunk, so the inputs are read
 // and the outputs written once, and no state but the last one reaches memory (under autograd: one
-// per 128 tokens).  Eight waves in two roles with one barrier a chunk: waves 0-3 form the chunk's outputs from a copy of the state in
-// LDS (16 tokens each, every product but the last kept in registers as the next one's operand);
-// waves 4-7 hold the state in float32 accumulators (16 rows each), move it over the same
-// chunk and leave the copy for the next.  The next chunk's rows are in registers meanwhile.
+// per 128 tokens).  Eight waves in two roles with one barrier a chunk.  In the step of chunk c
+//   waves 0-3  bring chunk c + 2 from memory into the third of three LDS stages, and form the weights
+//              between the tokens of chunk c + 1, e^{c_i - c_j} d_j (q_i . k_j), into one of two LDS tiles;
+//   waves 4-7  hold the state in float32 accumulators, 16 value rows each, which are the operand of the
+//              queries' product as they stand; they write the chunk's outputs and move the state.
 // Where heads are too few to fill 256 CUs, sequences are cut in time: a first launch sums each part's own
 // writes, and each part of the second starts from the combination of the parts before it.
 #include <stdint.h>
@@ -29,11 +30,16 @@ constexpr int kMaxParts = 32;
 template <class M, int NP>
 struct WalkLds {
   using S = SelShape<M>;
-  static constexpr int NS = NP + S::PAD;                        // key, query and state row stride
-  static constexpr int STAGE = S::L * (2 * NS + S::XS);         // keys, queries, values of a chunk
-  static constexpr int COPY = kSelRows * NS;
-  static constexpr int SCAL = 6 * S::L;                         // hi, lo, d, tail weight, decay; total
-  static constexpr size_t bytes = (2 * STAGE + 2 * COPY) * sizeof(typename ET<M>::raw) + 2 * SCAL * sizeof(float);
+  using KT = SelTile<M, NP, true>;         // keys: columns
+  using QT = SelTile<M, NP, false>;        // queries: rows in 8-byte pieces
+  using XT = SelTile<M, kSelRows, true>;   // values: columns
+  using MT = SelTile<M, S::L, false>;      // weights between tokens: rows in 8-byte pieces
+  static constexpr int Q0 = S::L * KT::STRIDE, X0 = Q0 + S::L * QT::STRIDE;
+  static constexpr int STAGES = 3, STAGE = X0 + S::L * XT::STRIDE;  // a chunk's tiles
+  static constexpr int MIX = S::L * MT::STRIDE;
+  static constexpr int SCAL = 6 * S::L;                             // hi, lo, d, tail weight, decay; total
+  static constexpr size_t bytes =
+      (STAGES * STAGE + 2 * MIX) * sizeof(typename ET<M>::raw) + STAGES * SCAL * sizeof(float);
   static_assert(bytes <= 160 * 1024, "one CU's LDS");
 };
 
@@ -67,17 +73,21 @@ __device__ __forceinline__ void part_start(f32x4 (&acc)[NT], const SelArgs& a, c
   if (a.memory != nullptr) state_add<NT>(acc, a.memory + head * one, p0, a.P, a.N, exp2_d(log));
 }
 
-template <class E, class M, int NP>
-__global__ __launch_bounds__(kWalkThreads, 1) void selective_walk_kernel(SelArgs a) {
+template <class E, class M, int NP, bool VEC>
+__global__ __launch_bounds__(kWalkThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void selective_walk_kernel(SelArgs a) {
   using S = SelShape<M>;
   using Lds = WalkLds<M, NP>;
   using raw = typename ET<M>::raw;
   using eraw = typename ET<E>::raw;
-  constexpr int L = S::L, NS = Lds::NS, XS = S::XS, NT = NP / 16, NK = NP / 32, NIT = L / 16, PPW = NIT;
+  using KT = typename Lds::KT;
+  using QT = typename Lds::QT;
+  using XT = typename Lds::XT;
+  using MT = typename Lds::MT;
+  constexpr int L = S::L, NT = NP / 16, NK = NP / 32, NIT = L / 16, NS32 = L / 32;
   extern __shared__ __align__(16) unsigned char smem[];
   raw* stage = reinterpret_cast<raw*>(smem);
-  raw* copy = stage + 2 * Lds::STAGE;
-  float* scal = reinterpret_cast<float*>(copy + 2 * Lds::COPY);
+  raw* mix = stage + Lds::STAGES * Lds::STAGE;
+  float* scal = reinterpret_cast<float*>(mix + 2 * Lds::MIX);
 
   const WalkPlace w = walk_place(a, xcd_order(blockIdx.x, gridDim.x));
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, g = lane >> 4, n16 = lane & 15;
@@ -85,146 +95,232 @@ __global__ __launch_bounds__(kWalkThreads, 1) void selective_walk_kernel(SelArgs
   const int p0 = w.pt * kSelRows, pw = a.P - p0;
   const int64_t len = sel_length(a, w.b);
   const int64_t t_first = w.part * a.part_tokens, t_last = min_i64(t_first + a.part_tokens, a.T);
-  const int64_t live = max_i64(0, min_i64(len, t_last) - t_first);
-  const int chunks = static_cast<int>((live + L - 1) / L);
-  const float rate = a.rates[w.h], skip = a.skip == nullptr ? 0.f : a.skip[w.h];
-  const bool vec = a.vec != 0;
-
-  TileLoad<E, M, L, NP, kWalkThreads> kr, qr;
-  TileLoad<E, M, L, kSelRows, kWalkThreads> xr;
-  auto load = [&](int c) {
-    const int64_t t = t_first + static_cast<int64_t>(c) * L, rows = len - t;
-    kr.load(a.keys, w.b * a.kb + t * a.kt + static_cast<int64_t>(w.g) * a.N, a.kt, rows, a.N, vec, tid);
-    qr.load(a.queries, w.b * a.qb + t * a.qt + static_cast<int64_t>(w.g) * a.N, a.qt, rows, a.N, vec, tid);
-    xr.load(a.values, w.b * a.vb + t * a.vt + static_cast<int64_t>(w.h) * a.P + p0, a.vt, rows, pw, vec, tid);
-  };
-  auto put = [&](int c) {
-    raw* s = stage + (c & 1) * Lds::STAGE;
-    kr.store(s, NS, tid);
-    qr.store(s + L * NS, NS, tid);
-    xr.store(s + 2 * L * NS, XS, tid);
-  };
-  auto scalars = [&](int c) {
-    const TokenScalars s = token_scalars<E, L>(a, w.b, w.h, t_first + static_cast<int64_t>(c) * L + lane, len, rate);
-    float* o = scal + (c & 1) * Lds::SCAL;
-    if (lane < L) {
-      const float hi = static_cast<float>(s.cum);
-      o[lane] = hi;
-      o[L + lane] = static_cast<float>(s.cum - hi);
-      o[2 * L + lane] = s.d;
-      o[3 * L + lane] = s.d * exp2_d(s.total - s.cum);
-      o[4 * L + lane] = exp2_d(s.cum);
-    }
-    if (lane == 0) o[5 * L] = exp2_d(s.total);
-  };
-
-  f32x4 acc[NT];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int sp = p0 + 16 * (wave & 3);  // a state wave's first row
-  auto copy_out = [&](int c) {
-    raw* s = copy + (c & 1) * Lds::COPY + (16 * (wave & 3) + n16) * NS + 4 * g;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) store4_raw<M>(s + nt * 16, acc[nt]);
-  };
-  if (chunks > 0) load(0);
-  if (wave >= 4) {
-    part_start<NT, false>(acc, a, w, sp);
-    copy_out(0);
-  }
-  if (chunks > 0) {
-    put(0);
-    if (wave == 0) scalars(0);
-  }
-  __syncthreads();
-
-  eraw* hid = static_cast<eraw*>(a.hidden) + (static_cast<int64_t>(w.b) * a.T * a.H + w.h) * a.P + p0;
+  const int live = static_cast<int>(max_i64(0, min_i64(len, t_last) - t_first));  // tokens of this walk
+  const int chunks = (live + L - 1) / L;
+  eraw* hid = static_cast<eraw*>(a.hidden) + ((w.b * a.T + t_first) * a.H + w.h) * a.P + p0;
   const int64_t hstride = static_cast<int64_t>(a.H) * a.P;
-  const bool hvec = vec && (a.P & 3) == 0;
-  for (int c = 0; c < chunks; ++c) {
-    if (c + 1 < chunks) load(c + 1);
-    const raw* ks = stage + (c & 1) * Lds::STAGE;
-    const raw *qs = ks + L * NS, *xs = qs + L * NS;
-    const float* sc = scal + (c & 1) * Lds::SCAL;
-    if (wave < 4) {
-      const int it = wave % NIT, pt0 = wave / NIT * PPW, i = it * 16 + n16;
-      const raw* cp = copy + (c & 1) * Lds::COPY;
-      f32x4 y[PPW];
-      Frag8<M> qf[NK];
-#pragma unroll
-      for (int kk = 0; kk < NK; ++kk) qf[kk] = row_frag<M>(qs, NS, it * 16, kk * 32);
-#pragma unroll
-      for (int p = 0; p < PPW; ++p) {
-        y[p] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int kk = 0; kk < NK; ++kk) y[p] = mfma8(row_frag<M>(cp, NS, (pt0 + p) * 16, kk * 32), qf[kk], y[p]);
-        const float e = sc[4 * L + i];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) y[p][r] *= e;
-      }
-      const float hi_i = sc[i], lo_i = sc[L + i];
-      for (int jp = 0; jp <= it; jp += 2) {
-        f32x4 m[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int jt = jp + u;
-          m[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-          if (jt <= it) {
-#pragma unroll
-            for (int kk = 0; kk < NK; ++kk) m[u] = mfma8(row_frag<M>(ks, NS, jt * 16, kk * 32), qf[kk], m[u]);
-            const int j0 = jt * 16 + 4 * g;
-            const f32x4 hj = *reinterpret_cast<const f32x4*>(sc + j0), lj = *reinterpret_cast<const f32x4*>(sc + L + j0),
-                        dj = *reinterpret_cast<const f32x4*>(sc + 2 * L + j0);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              m[u][r] = j0 + r <= i ? m[u][r] * dj[r] * exp2_f((hi_i - hj[r]) + (lo_i - lj[r])) : 0.f;
-          }
+
+  if (wave < 4) {
+    const float rate = a.rates[w.h], bias = a.bias == nullptr ? 0.f : a.bias[w.h];
+    const eraw* kp = static_cast<const eraw*>(a.keys) + w.b * a.kb + t_first * a.kt + w.g * a.N;
+    const eraw* qp = static_cast<const eraw*>(a.queries) + w.b * a.qb + t_first * a.qt + w.g * a.N;
+    const eraw* xp = static_cast<const eraw*>(a.values) + w.b * a.vb + t_first * a.vt + w.h * a.P + p0;
+    TileLoad<E, KT, M, VEC, L, NP, kWalkThreads / 2> kr;
+    TileLoad<E, QT, M, VEC, L, NP, kWalkThreads / 2> qr;
+    TileLoad<E, XT, M, VEC, L, kSelRows, kWalkThreads / 2> xr;
+    kr.init(a.kt, a.N, tid);
+    qr.init(a.qt, a.N, tid);
+    xr.init(a.vt, pw < kSelRows ? pw : kSelRows, tid);
+    uint32_t z = 0;  // the loaded chunk's steps
+    constexpr int kStepWave = 3;
+    int at = 0;      // tokens before the next chunk to load
+    auto load = [&]() {
+      kr.load(kp + at * a.kt, live - at, tid);
+      qr.load(qp + at * a.qt, live - at, tid);
+      xr.load(xp + at * a.vt, live - at, tid);
+      if (wave == kStepWave) z = load_step<E>(a, w.b, t_first + at + lane, w.h, lane < L && at + lane < live);
+      at += L;
+    };
+    auto put = [&](int slot) {
+      raw* s = stage + slot * Lds::STAGE;
+      kr.store(s, tid);
+      qr.store(s + Lds::Q0, tid);
+      xr.store(s + Lds::X0, tid);
+      if (wave == kStepWave) {
+        const TokenScalars s = token_scalars<L>(a, step_value<E>(a, z) + bias, at - L + lane < live, rate);
+        float* o = scal + slot * Lds::SCAL;
+        if (lane < L) {
+          const float hi = static_cast<float>(s.cum);
+          o[lane] = hi;
+          o[L + lane] = static_cast<float>(s.cum - hi);
+          o[2 * L + lane] = s.d;
+          o[3 * L + lane] = s.d * exp2_d(s.total - s.cum);
+          o[4 * L + lane] = exp2_d(s.cum);
         }
-        // One rounding of the weights to 16 bits, as far from them as the output's own rounding is
-        // from it; the values they meet are exact.
-        const Frag8<M> mf = pair_frag<M>(m[0], m[1]);
-#pragma unroll
-        for (int p = 0; p < PPW; ++p) y[p] = mfma8(col_frag<M>(xs, XS, jp * 16, (pt0 + p) * 16), mf, y[p]);
+        if (lane == 0) o[5 * L] = exp2_d(s.total);
       }
-      const int64_t t = t_first + static_cast<int64_t>(c) * L + i;
-      if (t < t_last) {
-        eraw* o = hid + t * hstride;
-        const bool on = t < len;
+    };
+    // 16-bit types: waves 0 to 2 form a 32 x 32 block of the weights each, its fragments read once for two tiles;
+    // float32: waves 0 to 2 one tile each.  The last wave has the step sizes.
+    auto weights = [&](int slot, int c) {
+      if (wave == 3) return;
+      const raw *ks = stage + slot * Lds::STAGE, *qs = ks + Lds::Q0;
+      const float* sc = scal + slot * Lds::SCAL;
+      raw* m = mix + (c & 1) * Lds::MIX;
+      constexpr int NB = NIT / 2;  // tiles of a block each way
+      const int it0 = NB * (wave == 1 ? 0 : 1), jt0 = NB * (wave == 2 ? 1 : 0);
+      Frag8<M> kf[NB][NK], qf[NB][NK];
 #pragma unroll
-        for (int p = 0; p < PPW; ++p) {
-          const int col = (pt0 + p) * 16 + 4 * g;
-          const f32x4 x = lds_row4<M>(xs + i * XS + col);
-          f32x4 v;
+      for (int kk = 0; kk < NK; ++kk) {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = on ? fmaf(skip, x[r], y[p][r]) : 0.f;
-          if (hvec) {
-            if (col < pw) store4_raw<E>(o + col, v);
-          } else {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              if (col + r < pw) o[col + r] = ET<E>::from_f(v[r]);
-            }
-          }
+        for (int u = 0; u < NB; ++u) {
+          kf[u][kk] = row_frag<KT, M>(ks, (jt0 + u) * 16, kk * 32);
+          qf[u][kk] = row_frag<QT, M>(qs, (it0 + u) * 16, kk * 32);
         }
       }
-      if (wave == 0 && c + 1 < chunks) scalars(c + 1);
-    } else {
+      hold_order();
+#pragma unroll
+      for (int u = 0; u < NB; ++u) {
+#pragma unroll
+        for (int v = 0; v < NB; ++v) {
+          const int it = it0 + u, jt = jt0 + v;
+          if (jt > it) continue;
+          f32x4 d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int kk = 0; kk < NK; ++kk) d = mfma8(kf[v][kk], qf[u][kk], d);
+          const int j0 = jt * 16 + 4 * g, i = it * 16 + n16;
+          const f32x4 hj = *reinterpret_cast<const f32x4*>(sc + j0), lj = *reinterpret_cast<const f32x4*>(sc + L + j0),
+                      dj = *reinterpret_cast<const f32x4*>(sc + 2 * L + j0);
+          const float hi_i = sc[i], lo_i = sc[L + i];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) d[r] = j0 + r <= i ? d[r] * dj[r] * exp2_f((hi_i - hj[r]) + (lo_i - lj[r])) : 0.f;
+          // One rounding of the weights to 16 bits, as far from them as the output's own rounding is
+          // from it; the values they meet are exact.
+          store4_raw<M>(m + MT::at(i, j0), d);
+        }
+      }
+    };
+    // The tiles behind the diagonal that share a 32-token step with it stay zero.
+    for (int u = tid; u < 2 * Lds::MIX; u += kWalkThreads / 2) mix[u] = 0;
+    if (chunks > 0) {
+      load();
+      put(0);
+      if (chunks > 1) load();
+    }
+    __syncthreads();
+    if (chunks > 0) weights(0, 0);
+    if (chunks > 1) put(1);
+    __syncthreads();
+    int s1 = 1, s2 = 2;  // stages of chunks c + 1 and c + 2
+    for (int c = 0; c < chunks; ++c) {
+      if (c + 2 < chunks) load();
+      if (c + 1 < chunks) weights(s1, c + 1);
+      if (c + 2 < chunks) put(s2);
+      __syncthreads();
+      s1 = s2;
+      s2 = s2 == 2 ? 0 : s2 + 1;
+    }
+  } else {
+    const int rw = 16 * (wave & 3), sp = p0 + rw;  // this wave's first row
+    const float skip = a.skip == nullptr ? 0.f : a.skip[w.h];
+    f32x4 acc[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    part_start<NT, false>(acc, a, w, sp);
+    const int col = rw + 4 * g;  // this lane's first value column, of four
+    const bool hvec = VEC && (a.P & 3) == 0;
+    __syncthreads();
+    __syncthreads();
+    int s0 = 0;  // stage of chunk c
+    Frag8<M> qf[NK][NIT];
+    auto ask_queries = [&](int slot) {
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) {
+#pragma unroll
+        for (int it = 0; it < NIT; ++it) qf[kk][it] = row_frag_t<QT, M>(stage + slot * Lds::STAGE + Lds::Q0, it * 16, kk * 32);
+      }
+    };
+    if (chunks > 0) ask_queries(0);
+    for (int c = 0; c < chunks; ++c) {
+      const raw* ks = stage + s0 * Lds::STAGE;
+      const raw* xs = ks + Lds::X0;
+      const float* sc = scal + s0 * Lds::SCAL;
+      const raw* m = mix + (c & 1) * Lds::MIX;
       if (a.states != nullptr && c * L % S::LB == 0) {
         const int64_t blk = (t_first + static_cast<int64_t>(c) * L) / S::LB;
         state_store<NT>(acc, a.states + ((w.b * a.nsave + blk) * a.H + w.h) * a.P * a.N, sp, a.P, a.N);
       }
-      state_update<M, L, NT>(acc, ks, NS, xs, XS, 16 * (wave & 3), sc + 3 * L, sc[5 * L]);
-      if (c + 1 < chunks) copy_out(c + 1);
+      // Reads are issued a phase ahead of the products that want them: the weights and the first keys with
+      // the state's product, the next chunk's queries with the last of the update.
+      Frag8<M> xf[NS32], sf[NK], mf[NS32][NIT], kf[NT];
+      f32x4 xv[NIT];
+      float e[NIT];
+#pragma unroll
+      for (int it = 0; it < NIT; ++it) e[it] = sc[4 * L + it * 16 + n16];
+#pragma unroll
+      for (int s = 0; s < NS32; ++s) {
+        xf[s] = col_frag<XT, M>(xs, 32 * s, rw);
+#pragma unroll
+        for (int it = 2 * s; it < NIT; ++it) mf[s][it] = row_frag_t<MT, M>(m, it * 16, 32 * s);
+      }
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) sf[kk] = pair_frag<M>(acc[2 * kk], acc[2 * kk + 1]);
+      hold_order();
+      f32x4 y[NIT];
+#pragma unroll
+      for (int it = 0; it < NIT; ++it) y[it] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) {
+#pragma unroll
+        for (int it = 0; it < NIT; ++it) y[it] = mfma8(sf[kk], qf[kk][it], y[it]);
+      }
+      key_frags<KT, M, NT>(kf, ks, 0);
+#pragma unroll
+      for (int it = 0; it < NIT; ++it) xv[it] = lds_row4<M>(xs + XT::at(it * 16 + n16, col));
+      f32x4 w0 = *reinterpret_cast<const f32x4*>(sc + 3 * L + 4 * g), w1 = *reinterpret_cast<const f32x4*>(sc + 3 * L + 16 + 4 * g);
+      const float decay = sc[5 * L];
+      hold_order();
+#pragma unroll
+      for (int it = 0; it < NIT; ++it) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y[it][r] *= e[it];
+      }
+#pragma unroll
+      for (int s = 0; s < NS32; ++s) {
+#pragma unroll
+        for (int it = 2 * s; it < NIT; ++it) y[it] = mfma8(xf[s], mf[s][it], y[it]);
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[nt][r] *= decay;
+      }
+      Frag8<M> part[S::PARTS];
+      weigh_frag<M>(xf[0], w0, w1, part);
+#pragma unroll
+      for (int it = 0; it < NIT; ++it) {
+        const int t = c * L + it * 16 + n16;
+        f32x4 v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = t < live ? fmaf(skip, xv[it][r], y[it][r]) : 0.f;
+        if (t_first + t < t_last) {
+          eraw* o = hid + t * hstride + col;
+          if (hvec) {
+            if (col < pw) store4_raw<E>(o, v);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              if (col + r < pw) o[r] = ET<E>::from_f(v[r]);
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int s = 0; s < NS32; ++s) {
+        Frag8<M> kn[NT];
+        if (s + 1 < NS32) {
+          key_frags<KT, M, NT>(kn, ks, 32 * (s + 1));
+          w0 = *reinterpret_cast<const f32x4*>(sc + 3 * L + 32 * (s + 1) + 4 * g);
+          w1 = *reinterpret_cast<const f32x4*>(sc + 3 * L + 32 * (s + 1) + 16 + 4 * g);
+        }
+        if (s + 1 == NS32 && c + 1 < chunks) ask_queries(s0 == 2 ? 0 : s0 + 1);
+        hold_order();
+        update_step<M, NT>(acc, kf, part);
+        if (s + 1 < NS32) {
+          weigh_frag<M>(xf[s + 1 < NS32 ? s + 1 : 0], w0, w1, part);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) kf[nt] = kn[nt];
+        }
+      }
+      __syncthreads();
+      s0 = s0 == 2 ? 0 : s0 + 1;
     }
-    if (c + 1 < chunks) put(c + 1);
-    __syncthreads();
+    if (w.part == a.parts - 1)
+      state_store<NT>(acc, a.memory_out + (static_cast<int64_t>(w.b) * a.H + w.h) * a.P * a.N, sp, a.P, a.N);
   }
-  if (wave >= 4 && w.part == a.parts - 1)
-    state_store<NT>(acc, a.memory_out + (static_cast<int64_t>(w.b) * a.H + w.h) * a.P * a.N, sp, a.P, a.N);
   // Tokens behind the length (the walk's last chunk has written its own).
-  const int64_t t_fill = t_first + static_cast<int64_t>(chunks) * L;
   const int cols = pw < kSelRows ? pw : kSelRows;
-  for (int64_t t = t_fill + wave; t < t_last; t += kWalkThreads / 64) {
+  for (int64_t t = chunks * L + wave; t < t_last - t_first; t += kWalkThreads / 64) {
     if (lane < cols) hid[t * hstride + lane] = ET<E>::from_f(0.f);
   }
 }
@@ -233,11 +329,14 @@ __global__ __launch_bounds__(kWalkThreads, 1) void selective_walk_kernel(SelArgs
 // (the backward's adjoint): `keys` are the queries and `values` the output's gradient,
 //   G_{before} = e^{c_L} G + sum_i e^{c_i} dy_i q_i^T,
 // from the gradient of the final state back to the first, G kept at the end of every backward chunk.
-template <class E, class M, int NP, bool REV, bool LOCAL>
-__global__ __launch_bounds__(kPassThreads) void selective_pass_kernel(SelArgs a) {
+template <class E, class M, int NP, bool VEC, bool REV, bool LOCAL>
+__global__ __launch_bounds__(kPassThreads) __attribute__((amdgpu_waves_per_eu(1, 2))) void selective_pass_kernel(SelArgs a) {
   using S = SelShape<M>;
   using raw = typename ET<M>::raw;
-  constexpr int L = S::L, NS = NP + S::PAD, XS = S::XS, NT = NP / 16, STAGE = L * (NS + XS), SCAL = L + 4;
+  using eraw = typename ET<E>::raw;
+  using KT = SelTile<M, NP, true>;
+  using XT = SelTile<M, kSelRows, true>;
+  constexpr int L = S::L, NT = NP / 16, X0 = L * KT::STRIDE, STAGE = X0 + L * XT::STRIDE, SCAL = L + 4;
   extern __shared__ __align__(16) unsigned char smem[];
   raw* stage = reinterpret_cast<raw*>(smem);
   float* scal = reinterpret_cast<float*>(stage + 2 * STAGE);
@@ -251,25 +350,33 @@ __global__ __launch_bounds__(kPassThreads) void selective_pass_kernel(SelArgs a)
   const int64_t len = sel_length(a, w.b);
   const int64_t t_first = w.part * a.part_tokens, t_last = min_i64(t_first + a.part_tokens, a.T);
   const int chunks = static_cast<int>((max_i64(0, min_i64(len, t_last) - t_first) + L - 1) / L);
-  const float rate = a.rates[w.h];
-  const bool vec = a.vec != 0;
+  const float rate = a.rates[w.h], bias = a.bias == nullptr ? 0.f : a.bias[w.h];
   auto chunk_of = [&](int i) { return REV ? chunks - 1 - i : i; };
 
-  TileLoad<E, M, L, NP, kPassThreads> kr;
-  TileLoad<E, M, L, kSelRows, kPassThreads> xr;
+  TileLoad<E, KT, M, VEC, L, NP, kPassThreads> kr;
+  TileLoad<E, XT, M, VEC, L, kSelRows, kPassThreads> xr;
+  kr.init(a.kt, a.N, tid);
+  xr.init(a.vt, pw < kSelRows ? pw : kSelRows, tid);
+  const eraw* kp = static_cast<const eraw*>(a.keys) + w.b * a.kb + w.g * a.N;
+  const eraw* xp = static_cast<const eraw*>(a.values) + w.b * a.vb + w.h * a.P + p0;
   auto load = [&](int i) {
     const int64_t t = t_first + static_cast<int64_t>(chunk_of(i)) * L, rows = len - t;
-    kr.load(a.keys, w.b * a.kb + t * a.kt + static_cast<int64_t>(w.g) * a.N, a.kt, rows, a.N, vec, tid);
-    xr.load(a.values, w.b * a.vb + t * a.vt + static_cast<int64_t>(w.h) * a.P + p0, a.vt, rows, pw, vec, tid);
+    kr.load(kp + t * a.kt, rows, tid);
+    xr.load(xp + t * a.vt, rows, tid);
   };
   double log = 0.0;
+  uint32_t z = 0;  // wave 0: the next chunk's steps
+  auto ask_step = [&](int i) {
+    const int64_t t = t_first + static_cast<int64_t>(chunk_of(i)) * L + lane;
+    z = load_step<E>(a, w.b, t, w.h, lane < L && t < len);
+  };
   auto put = [&](int i) {
     raw* s = stage + (i & 1) * STAGE;
-    kr.store(s, NS, tid);
-    xr.store(s + L * NS, XS, tid);
+    kr.store(s, tid);
+    xr.store(s + X0, tid);
     if (wave == 0) {
       const TokenScalars t =
-          token_scalars<E, L>(a, w.b, w.h, t_first + static_cast<int64_t>(chunk_of(i)) * L + lane, len, rate);
+          token_scalars<L>(a, step_value<E>(a, z) + bias, t_first + static_cast<int64_t>(chunk_of(i)) * L + lane < len, rate);
       float* o = scal + (i & 1) * SCAL;
       if (lane < L)
         o[lane] = REV ? exp2_d(t.cum) : t.d * exp2_d(t.total - t.cum);
@@ -280,12 +387,18 @@ __global__ __launch_bounds__(kPassThreads) void selective_pass_kernel(SelArgs a)
   f32x4 acc[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (chunks > 0) load(0);
+  if (chunks > 0) {
+    load(0);
+    if (wave == 0) ask_step(0);
+  }
   if (!LOCAL) part_start<NT, REV>(acc, a, w, sp);
   if (chunks > 0) put(0);
   __syncthreads();
   for (int i = 0; i < chunks; ++i) {
-    if (i + 1 < chunks) load(i + 1);
+    if (i + 1 < chunks) {
+      load(i + 1);
+      if (wave == 0) ask_step(i + 1);
+    }
     const raw* ks = stage + (i & 1) * STAGE;
     const float* sc = scal + (i & 1) * SCAL;
     if (REV && !LOCAL) {
@@ -293,7 +406,23 @@ __global__ __launch_bounds__(kPassThreads) void selective_pass_kernel(SelArgs a)
       if (i == 0 || (t + L) % S::LB == 0)
         state_store<NT>(acc, a.states + ((w.b * a.nsave + t / S::LB) * a.H + w.h) * a.P * a.N, sp, a.P, a.N);
     }
-    state_update<M, L, NT>(acc, ks, NS, ks + L * NS, XS, 16 * wave, sc, sc[L]);
+    Frag8<M> xf[L / 32];
+#pragma unroll
+    for (int s = 0; s < L / 32; ++s) xf[s] = col_frag<XT, M>(ks + X0, 32 * s, 16 * wave);
+    const float decay = sc[L];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[nt][r] *= decay;
+    }
+#pragma unroll
+    for (int s = 0; s < L / 32; ++s) {
+      Frag8<M> kf[NT], part[S::PARTS];
+      key_frags<KT, M, NT>(kf, ks, 32 * s);
+      weigh_frag<M>(xf[s], *reinterpret_cast<const f32x4*>(sc + 32 * s + 4 * (lane >> 4)),
+                    *reinterpret_cast<const f32x4*>(sc + 32 * s + 16 + 4 * (lane >> 4)), part);
+      update_step<M, NT>(acc, kf, part);
+    }
     if (i + 1 < chunks) put(i + 1);
     __syncthreads();
   }
@@ -382,19 +511,6 @@ __global__ __launch_bounds__(256) void selective_step_kernel(SelArgs a) {
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// f(E, M, NP): one of the compiled forms.
-template <class F>
-void with_form(int dtype, int64_t N, F f) {
-  auto by_width = [&](auto e, auto m) {
-    if (N <= 32) f(e, m, std::integral_constant<int, 32>{});
-    else if (N <= 64) f(e, m, std::integral_constant<int, 64>{});
-    else f(e, m, std::integral_constant<int, 128>{});
-  };
-  if (dtype == GRM_HIP_BF16) by_width(BF16{}, BF16{});
-  else if (dtype == GRM_HIP_F16) by_width(F16{}, F32{});
-  else by_width(F32{}, F32{});
-}
-
 int set_lds(const void* kernel, size_t bytes, const char* what) {
   const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
   if (e != hipSuccess) {
@@ -441,6 +557,10 @@ int sel_check(const grm_hip_selective_args* u, const char* what) {
     return GRM_HIP_EUNSUPPORTED;
   }
   const int64_t most = int64_t{1} << 21;
+  if (u->seq_len > (1 << 30)) {
+    set_error("%s: seq_len must be at most 2^30", what);
+    return GRM_HIP_EUNSUPPORTED;
+  }
   if (u->keys_token_stride < 0 || u->keys_token_stride > most || u->values_token_stride < 0 ||
       u->values_token_stride > most || u->queries_token_stride < 0 || u->queries_token_stride > most ||
       u->heads * sel_ceil(u->value_dim, kSelRows) * u->batch > (1 << 24) || u->heads * u->value_dim > most ||
@@ -448,6 +568,9 @@ int sel_check(const grm_hip_selective_args* u, const char* what) {
     set_error("%s: token strides and row widths must be below 2^21 elements and batch * heads * value tiles below 2^24", what);
     return GRM_HIP_EUNSUPPORTED;
   }
+  if (u->seq_len > 1 && (u->keys_token_stride < u->groups * u->key_dim || u->queries_token_stride < u->groups * u->key_dim ||
+                         u->values_token_stride < u->heads * u->value_dim))
+    return bad("token strides must not be below a row's width");
   if (u->batch > 0 && u->rates == nullptr) return bad("rates are required");
   if (u->batch > 0 && u->seq_len > 0 &&
       (u->keys == nullptr || u->values == nullptr || u->queries == nullptr || u->steps == nullptr))
@@ -480,20 +603,21 @@ SelArgs sel_args(const grm_hip_selective_args* u) {
 
 int launch_state_pass(const SelArgs& a, int dtype, bool reverse, bool local, hipStream_t stream, const char* what) {
   int rc = GRM_HIP_OK;
-  with_form(dtype, a.N, [&](auto e, auto m, auto np) {
+  sel_with_form(dtype, a.N, a.vec != 0, [&](auto e, auto m, auto np, auto vec) {
+    constexpr bool VEC = decltype(vec)::value;
     using E = decltype(e);
     using M = decltype(m);
     constexpr int NP = decltype(np)::value;
     using S = SelShape<M>;
-    constexpr size_t lds = 2 * S::L * (NP + S::PAD + S::XS) * sizeof(typename ET<M>::raw) + 2 * (S::L + 4) * sizeof(float);
+    constexpr size_t lds = 2 * S::L * (SelTile<M, NP, true>::STRIDE + SelTile<M, kSelRows, true>::STRIDE) * sizeof(typename ET<M>::raw) + 2 * (S::L + 4) * sizeof(float);
     auto go = [&](auto kernel) {
       if ((rc = set_lds(reinterpret_cast<const void*>(kernel), lds, what)) != GRM_HIP_OK) return;
       kernel<<<dim3(walk_blocks(a)), dim3(kPassThreads), lds, stream>>>(a);
       rc = check_launch(what);
     };
-    if (reverse && local) go(selective_pass_kernel<E, M, NP, true, true>);
-    else if (reverse) go(selective_pass_kernel<E, M, NP, true, false>);
-    else go(selective_pass_kernel<E, M, NP, false, true>);
+    if (reverse && local) go(selective_pass_kernel<E, M, NP, VEC, true, true>);
+    else if (reverse) go(selective_pass_kernel<E, M, NP, VEC, true, false>);
+    else go(selective_pass_kernel<E, M, NP, VEC, false, true>);
   });
   return rc;
 }
@@ -542,11 +666,11 @@ extern "C" int grm_hip_selective_scan_fwd(const grm_hip_selective_args* u, void*
     if (int rc = launch_state_pass(a, u->dtype, false, true, static_cast<hipStream_t>(stream), what)) return rc;
   }
   int rc = GRM_HIP_OK;
-  with_form(u->dtype, a.N, [&](auto e, auto m, auto np) {
+  sel_with_form(u->dtype, a.N, a.vec != 0, [&](auto e, auto m, auto np, auto vec) {
     using E = decltype(e);
     using M = decltype(m);
     constexpr int NP = decltype(np)::value;
-    auto kernel = selective_walk_kernel<E, M, NP>;
+    auto kernel = selective_walk_kernel<E, M, NP, decltype(vec)::value>;
     if ((rc = set_lds(reinterpret_cast<const void*>(kernel), WalkLds<M, NP>::bytes, what)) != GRM_HIP_OK) return;
     kernel<<<dim3(walk_blocks(a)), dim3(kWalkThreads), WalkLds<M, NP>::bytes, static_cast<hipStream_t>(stream)>>>(a);
     rc = check_launch(what);
