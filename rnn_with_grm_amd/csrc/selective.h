@@ -164,8 +164,7 @@ struct SelTile {
 
 // Fragment of 16 rows (row + lane % 16), reduction along the row from `col`.
 template <class T, class M>
-__device__ __forceinline__ Frag8<M> row_frag(const typename ET<M>::raw* tile, int row, int col) {
-  const int lane = lane_id();
+__device__ __forceinline__ Frag8<M> row_frag(const typename ET<M>::raw* tile, int row, int col, int lane = lane_id()) {
   const typename ET<M>::raw* p = tile + T::at(row + (lane & 15), col + 8 * (lane >> 4));
   if constexpr (sizeof(typename ET<M>::raw) == 2) return __builtin_bit_cast(Frag8<M>, *reinterpret_cast<const uint4*>(p));
   else return lds_frag_4x2<M>(p, p + 4);
@@ -173,15 +172,15 @@ __device__ __forceinline__ Frag8<M> row_frag(const typename ET<M>::raw* tile, in
 
 // The same with the reduction in the tokens' slot order (4g + s, 16 + 4g + s).
 template <class T, class M>
-__device__ __forceinline__ Frag8<M> row_frag_t(const typename ET<M>::raw* tile, int row, int col) {
-  const int lane = lane_id(), r = row + (lane & 15), c = col + 4 * (lane >> 4);
+__device__ __forceinline__ Frag8<M> row_frag_t(const typename ET<M>::raw* tile, int row, int col, int lane = lane_id()) {
+  const int r = row + (lane & 15), c = col + 4 * (lane >> 4);
   return lds_frag_4x2<M>(tile + T::at(r, c), tile + T::at(r, c + 16));
 }
 
 // Fragment of 16 columns (col + lane % 16), reduction over 32 tokens from row `t0`.
 template <class T, class M>
-__device__ __forceinline__ Frag8<M> col_frag(const typename ET<M>::raw* tile, int t0, int col) {
-  const int lane = lane_id(), g = lane >> 4, n = lane & 15;
+__device__ __forceinline__ Frag8<M> col_frag(const typename ET<M>::raw* tile, int t0, int col, int lane = lane_id()) {
+  const int g = lane >> 4, n = lane & 15;
   Frag8<M> f;
   if constexpr (sizeof(typename ET<M>::raw) == 2) {
     // The transpose read hands lane i of a 16-lane block X[r0 + e][c0 + i], e = 0..3, when lane s

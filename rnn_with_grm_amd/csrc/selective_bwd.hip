@@ -155,6 +155,11 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
   }
 
   for (int hp = h_lo; hp < h_hi; ++hp) {
+    // The lane's number anew for every head, so that the hundreds of LDS addresses made from it are not kept in
+    // registers from head to head.
+    int lane = lane_id();
+    asm volatile("" : "+v"(lane));
+    const int g = lane >> 4, n16 = lane & 15, tok = tile * 16 + n16;
     const int h = gi * (f.H / f.G) + hp / f.PT, pt = hp % f.PT, p0 = pt * kSelRows, pw = f.P - p0;
     const int64_t row0 = (static_cast<int64_t>(b) * f.T + t0) * f.H + h;
     const int64_t hs = static_cast<int64_t>(f.H);
@@ -261,14 +266,15 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
     __syncthreads();
 
     // Columns j of this wave's tile: dx and dk from the rows i >= j.
+    hold_order();
     f32x4 dx[PW];
 #pragma unroll
     for (int p = 0; p < PW; ++p) dx[p] = f32x4{0.f, 0.f, 0.f, 0.f};
     Frag8<M> xf[2], yf[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      xf[k] = row_frag_t<XT, M>(xt, tile * 16, k * 32);
-      yf[k] = row_frag_t<XT, M>(yt, tile * 16, k * 32);
+      xf[k] = row_frag_t<XT, M>(xt, tile * 16, k * 32, lane);
+      yf[k] = row_frag_t<XT, M>(yt, tile * 16, k * 32, lane);
     }
     const float hj = hi[tok], lj = lo[tok], dj = dd[tok];
     float colsum = 0.f, on_diag = 0.f, w_diag = 0.f;
@@ -283,7 +289,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
         if (it < tile) continue;
         f32x4 w = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < 2; ++k) w = mfma8(row_frag_t<XT, M>(yt, it * 16, k * 32), xf[k], w);
+        for (int k = 0; k < 2; ++k) w = mfma8(row_frag_t<XT, M>(yt, it * 16, k * 32, lane), xf[k], w);
         const int i0 = it * 16 + 4 * g;
         const f32x4 hv = *reinterpret_cast<const f32x4*>(hi + i0), lv = *reinterpret_cast<const f32x4*>(lo + i0);
         f32x4 q;
@@ -304,9 +310,10 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       }
       const Frag8<M> ekf = pair_frag<M>(ek[0], ek[1]), ewf = pair_frag<M>(ew[0], ew[1]);
 #pragma unroll
-      for (int p = 0; p < PW; ++p) dx[p] = mfma8(col_frag<XT, M>(yt, ip * 16, (cs * PW + p) * 16), ekf, dx[p]);
+      for (int p = 0; p < PW; ++p) dx[p] = mfma8(col_frag<XT, M>(yt, ip * 16, (cs * PW + p) * 16, lane), ekf, dx[p]);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) dk[nt] = mfma8(col_frag<KT, M>(qt, ip * 16, (cs * NT + nt) * 16), ewf, dk[nt]);
+      for (int nt = 0; nt < NT; ++nt) dk[nt] = mfma8(col_frag<KT, M>(qt, ip * 16, (cs * NT + nt) * 16, lane), ewf, dk[nt]);
+      hold_order();
     }
     colsum = group_sum(colsum);
     on_diag = group_sum(on_diag);
@@ -316,6 +323,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       diag[tok] = on_diag;
       wjj[tok] = w_diag;
     }
+    hold_order();
     // Rows i of this wave's tile: dq from the columns j <= i, and from the state.
     const float e_i = ec[tok];
 #pragma unroll
@@ -329,7 +337,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
         if (jt > tile) continue;
         f32x4 w = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < 2; ++k) w = mfma8(row_frag_t<XT, M>(xt, jt * 16, k * 32), yf[k], w);
+        for (int k = 0; k < 2; ++k) w = mfma8(row_frag_t<XT, M>(xt, jt * 16, k * 32, lane), yf[k], w);
         const int j0 = jt * 16 + 4 * g;
         const f32x4 hv = *reinterpret_cast<const f32x4*>(hi + j0), lv = *reinterpret_cast<const f32x4*>(lo + j0),
                     dv = *reinterpret_cast<const f32x4*>(dd + j0);
@@ -338,8 +346,10 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       }
       const Frag8<M> ewf = pair_frag<M>(ew[0], ew[1]);
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) dq[nt] = mfma8(col_frag<KT, M>(kt, jp * 16, (cs * NT + nt) * 16), ewf, dq[nt]);
+      for (int nt = 0; nt < NT; ++nt) dq[nt] = mfma8(col_frag<KT, M>(kt, jp * 16, (cs * NT + nt) * 16, lane), ewf, dq[nt]);
+      hold_order();
     }
+    hold_order();
     float dot1 = 0.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -347,7 +357,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
       for (int s = SP - 1; s >= 0; --s) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) r = mfma8(col_frag<KT, M>(st + s * Lds::STATE, k * 32, (cs * NT + nt) * 16), yf[k], r);
+        for (int k = 0; k < 2; ++k) r = mfma8(col_frag<KT, M>(st + s * Lds::STATE, k * 32, (cs * NT + nt) * 16, lane), yf[k], r);
       }
       const f32x4 qv = lds_row4<M>(qt + KT::at(tok, (cs * NT + nt) * 16 + 4 * g));
 #pragma unroll
@@ -355,6 +365,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
         dot1 = fmaf(qv[e], r[e], dot1);
         dq[nt][e] = fmaf(e_i, r[e], dq[nt][e]);
       }
+      if (nt & 1) hold_order();
     }
     dot1 = group_sum(dot1);
     if (g == 0) t1[cs * LB + tok] = e_i * dot1;
@@ -370,7 +381,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
       for (int s = SP - 1; s >= 0; --s) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) r = mfma8(col_frag<KT, M>(st + s * Lds::STATE, k * 32, (cs * NT + nt) * 16), xf[k], r);
+        for (int k = 0; k < 2; ++k) r = mfma8(col_frag<KT, M>(st + s * Lds::STATE, k * 32, (cs * NT + nt) * 16, lane), xf[k], r);
       }
       const f32x4 kv = lds_row4<M>(kt + KT::at(tok, (cs * NT + nt) * 16 + 4 * g));
 #pragma unroll
@@ -378,18 +389,19 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
         dot2 = fmaf(kv[e], r[e], dot2);
         dk[nt][e] = fmaf(dj * e_t, r[e], dk[nt][e]);
       }
+      if (nt & 1) hold_order();
     }
     dot2 = group_sum(dot2);
     if (g == 0) t2[cs * LB + tok] = e_t * dot2;
     {
       Frag8<M> kf[NK];
 #pragma unroll
-      for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<KT, M>(kt, tile * 16, kk * 32);
+      for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<KT, M>(kt, tile * 16, kk * 32, lane);
 #pragma unroll
       for (int p = 0; p < PW; ++p) {
         f32x4 u = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int kk = 0; kk < NK; ++kk) u = mfma8(row_frag<KT, M>(st, (cs * PW + p) * 16, kk * 32), kf[kk], u);
+        for (int kk = 0; kk < NK; ++kk) u = mfma8(row_frag<KT, M>(st, (cs * PW + p) * 16, kk * 32, lane), kf[kk], u);
         const int c = (cs * PW + p) * 16 + 4 * g;
         const f32x4 yv = lds_row4<M>(yt + XT::at(tok, c));
         f32x4 o;
