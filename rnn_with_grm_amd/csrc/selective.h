@@ -177,9 +177,9 @@ __device__ __forceinline__ Frag8<M> row_frag_t(const typename ET<M>::raw* tile, 
   return lds_frag_4x2<M>(tile + T::at(r, c), tile + T::at(r, c + 16));
 }
 
-// Fragment of 16 columns (col + lane % 16), reduction over 32 tokens from row `t0`.
+// Fragment of 16 columns (col + lane % 16), reduction over the 16 tokens from row `t0` and the 16 from row `t1`.
 template <class T, class M>
-__device__ __forceinline__ Frag8<M> col_frag(const typename ET<M>::raw* tile, int t0, int col, int lane = lane_id()) {
+__device__ __forceinline__ Frag8<M> col_frag2(const typename ET<M>::raw* tile, int t0, int t1, int col, int lane = lane_id()) {
   const int g = lane >> 4, n = lane & 15;
   Frag8<M> f;
   if constexpr (sizeof(typename ET<M>::raw) == 2) {
@@ -187,9 +187,9 @@ __device__ __forceinline__ Frag8<M> col_frag(const typename ET<M>::raw* tile, in
     // passes &X[r0 + (s >> 2)][c0 + 4 (s & 3)].
     typedef short s16x4 __attribute__((ext_vector_type(4)));
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    const typename ET<M>::raw* p = tile + T::at(t0 + 4 * g + (n >> 2), col + 4 * (n & 3));
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + 16 * T::STRIDE));
+    const typename ET<M>::raw* p = tile + T::at(4 * g + (n >> 2), col + 4 * (n & 3));
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + t0 * T::STRIDE));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + t1 * T::STRIDE));
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       f.e[e] = static_cast<uint16_t>(lo[e]);
@@ -197,14 +197,18 @@ __device__ __forceinline__ Frag8<M> col_frag(const typename ET<M>::raw* tile, in
     }
   } else {
     constexpr int S = T::STRIDE;
-    const float* p = tile + (t0 + 4 * g) * S + col + n;
+    const float* p = tile + 4 * g * S + col + n;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      f.e[e] = p[e * S];
-      f.e[4 + e] = p[(16 + e) * S];
+      f.e[e] = p[(t0 + e) * S];
+      f.e[4 + e] = p[(t1 + e) * S];
     }
   }
   return f;
+}
+template <class T, class M>
+__device__ __forceinline__ Frag8<M> col_frag(const typename ET<M>::raw* tile, int t0, int col, int lane = lane_id()) {
+  return col_frag2<T, M>(tile, t0, t0 + 16, col, lane);
 }
 
 // Two accumulators (tokens 0-15 and 16-31 of a step) as one fragment.

@@ -48,15 +48,18 @@ struct GradArgs {
 template <class M, int NP>
 struct GradLds {
   using S = SelShape<M>;
-  static constexpr int LB = S::LB, NS = SelTile<M, NP, true>::STRIDE, XS = SelTile<M, kSelRows, true>::STRIDE;
+  using KT = SelTile<M, NP, true>;          // keys, queries, states: columns, and rows in 16-byte pieces
+  using XT = SelTile<M, kSelRows, false>;   // values and their gradients: rows in 8-byte pieces
+  static constexpr int LB = S::LB;
   static constexpr int SPARTS = S::kHalf ? 2 : 1;             // parts of S and G in LDS
-  static constexpr int STATE = kSelRows * NS;
-  static constexpr int TILES = LB * (2 * NS + 2 * XS) + SPARTS * STATE;
+  static constexpr int STATE = kSelRows * KT::STRIDE;
+  static constexpr int TILES = LB * (2 * KT::STRIDE + 2 * XT::STRIDE) + SPARTS * STATE;
   static constexpr int TOK = LB / 16;                          // token tiles
   static constexpr int CS = 8 / TOK;                           // waves that share one, a share of the columns each
-  // hi, lo, d, e^c, e^{c_L - c}; column sums, diagonal, W_jj; t1, t2 per share; row sums per tile; <G, S>
-  static constexpr int SCAL = 5 * LB + 3 * LB + 2 * CS * LB + TOK * LB + 16;
-  static constexpr size_t bytes = TILES * sizeof(typename ET<M>::raw) + SCAL * sizeof(float);
+  // A head's numbers by token: hi, lo, d, e^c, e^{c_L - c}, decays inside a tile (two); column and row sums;
+  // t1, t2 per share; then sums of W_jj and <G, S> per wave.
+  static constexpr int SCAL = (9 + 2 * CS) * LB + 16;
+  static constexpr size_t bytes = TILES * sizeof(typename ET<M>::raw) + 2 * SCAL * sizeof(float);
   static_assert(bytes <= 160 * 1024, "one CU's LDS");
 };
 
@@ -71,6 +74,14 @@ __device__ __forceinline__ float row_sum(float x) {
   x += row_rot<2>(x);
   x += row_rot<1>(x);
   return x;
+}
+// x of the lane ROT further in the row, 0 past its end.
+template <int ROT>
+__device__ __forceinline__ float dpp_shl(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x100 + ROT, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float lane_f32(float x, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
 }
 // Sum over the four lane groups.
 __device__ __forceinline__ float group_sum(float x) {
@@ -90,27 +101,68 @@ __device__ __forceinline__ void store_row4(typename ET<E>::raw* p, int left, boo
   }
 }
 
+// A 64 x NP float32 state by 512 threads: from memory into registers (zeros outside [rows, N]), then into LDS as
+// bfloat16 parts or as it is.
+template <class M, int NP>
+struct StateLoad {
+  using KT = SelTile<M, NP, true>;
+  static constexpr int PER = kSelRows * NP / 4 / kGradThreads, PARTS = GradLds<M, NP>::SPARTS;
+  static constexpr int DROW = kGradThreads * 4 / NP;
+  static_assert(PER >= 1 && PER * kGradThreads * 4 == kSelRows * NP, "states split evenly");
+  f32x4 r[PER];
+  __device__ __forceinline__ void load(const float* base, int rows, int N, int tid) {
+    const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(base, static_cast<uint32_t>((rows < kSelRows ? rows : kSelRows) * N * 4));
+    const int row = tid / (NP / 4), n = tid % (NP / 4) * 4;
+    if ((N & 3) == 0) {
+      const int off = n < N ? (row * N + n) * 4 : kBufOOB;
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        r[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, i * DROW * N * 4, 0));
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          r[i][e] = buf_load1<F32>(rsrc, n + e < N ? ((row + i * DROW) * N + n + e) * 4 : kBufOOB);
+      }
+    }
+  }
+  __device__ __forceinline__ void store(typename ET<M>::raw* tile, int tid) const {
+    typename ET<M>::raw* q = tile + KT::at(tid / (NP / 4), tid % (NP / 4) * 4);
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      f32x4 rest = r[i];
+#pragma unroll
+      for (int s = 0; s < PARTS; ++s) {
+        store4_raw<M>(q + i * DROW * KT::STRIDE + s * GradLds<M, NP>::STATE, rest);
+        if (s + 1 < PARTS) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) rest[e] -= ET<M>::to_f(ET<M>::from_f(rest[e]));
+        }
+      }
+    }
+  }
+};
+
 template <class E, class M, int NP, bool VEC>
 __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void selective_grad_kernel(GradArgs a) {
   using S = SelShape<M>;
   using Lds = GradLds<M, NP>;
   using raw = typename ET<M>::raw;
   using eraw = typename ET<E>::raw;
-  using KT = SelTile<M, NP, true>;        // keys, queries, state rows
-  using XT = SelTile<M, kSelRows, true>;  // values and their gradients
-  constexpr int LB = S::LB, NS = Lds::NS, XS = Lds::XS, TOK = Lds::TOK, CS = Lds::CS, SP = Lds::SPARTS;
+  using KT = typename Lds::KT;
+  using XT = typename Lds::XT;
+  constexpr int LB = S::LB, TOK = Lds::TOK, CS = Lds::CS, SP = Lds::SPARTS;
   constexpr int NK = NP / 32, NT = NP / 16 / CS, PW = kSelRows / 16 / CS, PL = (LB + 63) / 64;
-  constexpr int SU = kSelRows * NP / 4 / kGradThreads;  // float4 of a state per thread
-  static_assert(SU >= 1 && SU * kGradThreads * 4 == kSelRows * NP, "states split evenly");
   extern __shared__ __align__(16) unsigned char smem[];
   raw* kt = reinterpret_cast<raw*>(smem);
-  raw* qt = kt + LB * NS;
-  raw* xt = qt + LB * NS;
-  raw* yt = xt + LB * XS;
-  raw* st = yt + LB * XS;
-  float* hi = reinterpret_cast<float*>(st + SP * Lds::STATE);
-  float *lo = hi + LB, *dd = lo + LB, *ec = dd + LB, *et = ec + LB, *col = et + LB, *diag = col + LB, *wjj = diag + LB,
-        *t1 = wjj + LB, *t2 = t1 + CS * LB, *rows = t2 + CS * LB, *gs = rows + TOK * LB;
+  raw* qt = kt + LB * KT::STRIDE;
+  raw* xt = qt + LB * KT::STRIDE;
+  raw* yt = xt + LB * XT::STRIDE;
+  raw* st = yt + LB * XT::STRIDE;
+  float* scal = reinterpret_cast<float*>(st + SP * Lds::STATE);
+  constexpr int HI = 0, LO = LB, DD = 2 * LB, EC = 3 * LB, EE = 4 * LB, RB = 5 * LB, TD = 6 * LB, COL = 7 * LB, ROW = 8 * LB,
+                T1 = 9 * LB, T2 = T1 + CS * LB, WJ = T2 + CS * LB, GS = WJ + 8;
 
   const SelArgs& f = a.s;
   uint32_t v = xcd_order(blockIdx.x, gridDim.x);
@@ -119,354 +171,404 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
   const int gi = static_cast<int>(v % f.G);
   v /= f.G;
   const int blk = static_cast<int>(v % f.nsave), b = static_cast<int>(v / f.nsave);
-  const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, g = lane >> 4, n16 = lane & 15;
+  const int tid = static_cast<int>(threadIdx.x);
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int tile = wave % TOK, cs = wave / TOK, tok = tile * 16 + n16;  // this lane's token in both orders
-  const int64_t len = sel_length(f, b), t0 = static_cast<int64_t>(blk) * LB, live = len - t0;
+  const int tile = wave % TOK, cs = wave / TOK;
+  const int64_t t0 = static_cast<int64_t>(blk) * LB;
+  const int live = static_cast<int>(max_i64(0, min_i64(sel_length(f, b) - t0, LB)));
+  const int in_block = static_cast<int>(min_i64(LB, f.T - t0));
   const bool nvec = VEC && (f.N & 3) == 0, pvec = VEC && (f.P & 3) == 0;
   const int heads = f.H / f.G * f.PT;  // (head, value tile) pairs of the group
   const int h_lo = static_cast<int>(static_cast<int64_t>(heads) * split / a.splits),
             h_hi = static_cast<int>(static_cast<int64_t>(heads) * (split + 1) / a.splits);
+  const int64_t row_b = static_cast<int64_t>(b) * f.T + t0;  // the block's first token
+  auto head_of = [&](int hp) { return gi * (f.H / f.G) + hp / f.PT; };
+  auto put_step = [&](int hp, int t, float x) {
+    const int64_t at = (row_b + t) * f.H + head_of(hp);
+    if (a.steps_part != nullptr) a.steps_part[static_cast<int64_t>(hp % f.PT) * f.B * f.T * f.H + at] = x;
+    else st_state<E>(a.dsteps, at, f.steps_f32 != 0, x);
+  };
+  auto head_sums = [&](int hp) {
+    return a.head_part + ((static_cast<int64_t>(b) * f.nsave + blk) * f.H * f.PT + head_of(hp) * f.PT + hp % f.PT) * 3;
+  };
 
-  f32x4 dk[NT], dq[NT], score[TOK];
+  f32x4 dk[NT], dq[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) dk[i] = dq[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (live > 0) {
-    TileLoad<E, KT, M, VEC, LB, NP, kGradThreads> r;
-    r.init(f.kt, f.N, tid);
-    r.load(static_cast<const eraw*>(f.keys) + b * f.kb + t0 * f.kt + gi * f.N, live, tid);
-    r.store(kt, tid);
-    r.init(f.qt, f.N, tid);
-    r.load(static_cast<const eraw*>(f.queries) + b * f.qb + t0 * f.qt + gi * f.N, live, tid);
-    r.store(qt, tid);
-    __syncthreads();
-    // K: rows i of every tile from this wave's on, columns j of this wave's tile.
-    Frag8<M> kf[NK];
-#pragma unroll
-    for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<KT, M>(kt, tile * 16, kk * 32);
-#pragma unroll
-    for (int it = 0; it < TOK; ++it) {
-      score[it] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (it >= tile) {
-#pragma unroll
-        for (int kk = 0; kk < NK; ++kk) score[it] = mfma8(row_frag<KT, M>(qt, it * 16, kk * 32), kf[kk], score[it]);
-      }
-    }
-  }
-
-  for (int hp = h_lo; hp < h_hi; ++hp) {
-    // The lane's number anew for every head, so that the hundreds of LDS addresses made from it are not kept in
-    // registers from head to head.
-    int lane = lane_id();
-    asm volatile("" : "+v"(lane));
-    const int g = lane >> 4, n16 = lane & 15, tok = tile * 16 + n16;
-    const int h = gi * (f.H / f.G) + hp / f.PT, pt = hp % f.PT, p0 = pt * kSelRows, pw = f.P - p0;
-    const int64_t row0 = (static_cast<int64_t>(b) * f.T + t0) * f.H + h;
-    const int64_t hs = static_cast<int64_t>(f.H);
-    eraw* dxp = static_cast<eraw*>(a.dx) + row0 * f.P + p0;
-    float* hpart = a.head_part + ((static_cast<int64_t>(b) * f.nsave + blk) * f.H * f.PT + h * f.PT + pt) * 3;
-    auto put_step = [&](int64_t t, float x) {
-      const int64_t at = row0 + t * hs;
-      if (a.steps_part != nullptr) a.steps_part[static_cast<int64_t>(pt) * f.B * f.T * f.H + at] = x;
-      else st_state<E>(a.dsteps, at, f.steps_f32 != 0, x);
-    };
-    const int in_block = static_cast<int>(min_i64(LB, f.T - t0));
-    if (live <= 0) {  // behind the sequence's length: zeros
-      const int cols = pw < kSelRows ? pw : kSelRows;
+  if (live == 0) {  // behind the sequence's length: zeros
+    for (int hp = h_lo; hp < h_hi; ++hp) {
+      const int p0 = hp % f.PT * kSelRows, cols = f.P - p0 < kSelRows ? f.P - p0 : kSelRows, lane = lane_id();
+      eraw* dxp = static_cast<eraw*>(a.dx) + (row_b * f.H + head_of(hp)) * f.P + p0;
       for (int t = wave; t < in_block; t += 8) {
-        if (lane < cols) dxp[t * hs * f.P + lane] = ET<E>::from_f(0.f);
-        if (lane == 0) put_step(t, 0.f);
+        if (lane < cols) dxp[static_cast<int64_t>(t) * f.H * f.P + lane] = ET<E>::from_f(0.f);
+        if (lane == 0) put_step(hp, t, 0.f);
       }
-      if (tid < 3) hpart[tid] = 0.f;
-      continue;
+      if (tid < 3) head_sums(hp)[tid] = 0.f;
     }
-    const float rate = f.rates[h], skip = f.skip == nullptr ? 0.f : f.skip[h];
-
-    // The head's rows, the state and the adjoint.
+  } else {
+    constexpr int kStepWave = 7;  // the wave with the fewest tiles in the first of the two triangles
     TileLoad<E, XT, M, VEC, LB, kSelRows, kGradThreads> xr, yr;
-    xr.init(f.vt, pw < kSelRows ? pw : kSelRows, tid);
-    xr.load(static_cast<const eraw*>(f.values) + b * f.vb + t0 * f.vt + h * f.P + p0, live, tid);
-    yr.init(hs * f.P, pw < kSelRows ? pw : kSelRows, tid);
-    yr.load(static_cast<const eraw*>(a.dy) + row0 * f.P + p0, live, tid);
-    const int64_t sat = ((static_cast<int64_t>(b) * f.nsave + blk) * f.H + h) * f.P * f.N;
-    f32x4 gr[SU], sr[SU];
-    auto load_state = [&](const float* base, f32x4 (&r)[SU]) {
-#pragma unroll
-      for (int i = 0; i < SU; ++i) {
-        const int u = tid + i * kGradThreads, p = p0 + u / (NP / 4), n = u % (NP / 4) * 4;
-        r[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (p < f.P && n < f.N) {
-          const float* q = base + sat + static_cast<int64_t>(p) * f.N + n;
-          if ((f.N & 3) == 0) {
-            const float4 w = *reinterpret_cast<const float4*>(q);
-            r[i] = f32x4{w.x, w.y, w.z, w.w};
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) r[i][e] = n + e < f.N ? q[e] : 0.f;
-          }
-        }
-      }
+    auto ask_rows = [&](int hp) {
+      const int h = head_of(hp), p0 = hp % f.PT * kSelRows, cols = f.P - p0 < kSelRows ? f.P - p0 : kSelRows;
+      xr.init(f.vt, cols, tid);
+      xr.load(static_cast<const eraw*>(f.values) + b * f.vb + t0 * f.vt + h * f.P + p0, live, tid);
+      yr.init(static_cast<int64_t>(f.H) * f.P, cols, tid);
+      yr.load(static_cast<const eraw*>(a.dy) + (row_b * f.H + h) * f.P + p0, live, tid);
     };
-    auto put_state = [&](const f32x4 (&r)[SU]) {
-#pragma unroll
-      for (int i = 0; i < SU; ++i) {
-        const int u = tid + i * kGradThreads;
-        raw* q = st + KT::at(u / (NP / 4), u % (NP / 4) * 4);
-        f32x4 rest = r[i];
-#pragma unroll
-        for (int s = 0; s < SP; ++s) {
-          store4_raw<M>(q + s * Lds::STATE, rest);
-          if (s + 1 < SP) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) rest[e] -= ET<M>::to_f(ET<M>::from_f(rest[e]));
-          }
-        }
-      }
+    // The step wave: a head's token scalars, PL tokens a lane, one head ahead of the others; what its end needs
+    // of them stays in registers.
+    struct Steps {
+      float d[PL], slope[PL];
+      double total;
     };
-    load_state(f.states, sr);
-    load_state(a.adj, gr);
-    // Token scalars, PL tokens a lane, by the first wave.
-    double cum[PL], total = 0.0;
-    float dt[PL];
-    if (wave == 0) {
+    uint32_t zr[PL];
+    auto ask_steps = [&](int hp) {
 #pragma unroll
       for (int k = 0; k < PL; ++k) {
-        const int64_t t = t0 + lane * PL + k;
-        dt[k] = t < len ? step_size(f, raw_step<E>(f, b, t, h)) : 0.f;
-        double l = static_cast<double>(dt[k]) * static_cast<double>(rate);
+        const int t = lane_id() * PL + k;
+        zr[k] = load_step<E>(f, b, t0 + t, head_of(hp), t < live);
+      }
+    };
+    auto begin_head = [&](int hp, Steps& s) {
+      const int lane = lane_id(), h = head_of(hp);
+      const float rate = f.rates[h], bias = f.bias == nullptr ? 0.f : f.bias[h];
+      float* o = scal + (hp & 1) * Lds::SCAL;
+      double cum[PL], sum = 0.0;
+#pragma unroll
+      for (int k = 0; k < PL; ++k) {
+        const float z = step_value<E>(f, zr[k]) + bias;
+        const bool on = lane * PL + k < live;
+        s.d[k] = on ? step_size(f, z) : 0.f;
+        s.slope[k] = !on ? 0.f : !f.softplus || z > 20.f ? 1.f : __builtin_amdgcn_rcpf(1.f + __expf(-z));
+        double l = static_cast<double>(s.d[k]) * static_cast<double>(rate);
         l = l < -200.0 ? -200.0 : l;
-        total += l * 1.4426950408889634;
-        cum[k] = total;
+        sum += l * 1.4426950408889634;
+        cum[k] = sum;
       }
-      const double scan = wave_prefix(total), before = scan - total;
-      total = lane_value(scan, 63);
+      const double scan = wave_prefix(sum), before = scan - sum;
+      s.total = lane_value(scan, LB / PL - 1);
+#pragma unroll
+      for (int k = 0; k < PL; ++k) cum[k] += before;
+      // The sums before this token's tile and through its end.
+      constexpr int LPT = 16 / PL;  // lanes of a tile
+      const int first = lane / LPT * LPT;
+      const double tile_end = __shfl(cum[PL - 1], first + LPT - 1), up = __shfl(cum[PL - 1], first > 0 ? first - 1 : 0);
+      const double tile_start = first > 0 ? up : 0.0;
 #pragma unroll
       for (int k = 0; k < PL; ++k) {
-        cum[k] += before;
         const int t = lane * PL + k;
-        const float top = static_cast<float>(cum[k]);
-        hi[t] = top;
-        lo[t] = static_cast<float>(cum[k] - top);
-        dd[t] = dt[k];
-        ec[t] = exp2_d(cum[k]);
-        et[t] = exp2_d(total - cum[k]);
-      }
-    }
-    xr.store(xt, tid);
-    yr.store(yt, tid);
-    put_state(sr);
-    float dot = 0.f;
-#pragma unroll
-    for (int i = 0; i < SU; ++i) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) dot = fmaf(gr[i][e], sr[i][e], dot);
-    }
-    dot = group_sum(row_sum(dot));
-    if (lane == 0) gs[wave] = dot;
-    __syncthreads();
-
-    // Columns j of this wave's tile: dx and dk from the rows i >= j.
-    hold_order();
-    f32x4 dx[PW];
-#pragma unroll
-    for (int p = 0; p < PW; ++p) dx[p] = f32x4{0.f, 0.f, 0.f, 0.f};
-    Frag8<M> xf[2], yf[2];
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      xf[k] = row_frag_t<XT, M>(xt, tile * 16, k * 32, lane);
-      yf[k] = row_frag_t<XT, M>(yt, tile * 16, k * 32, lane);
-    }
-    const float hj = hi[tok], lj = lo[tok], dj = dd[tok];
-    float colsum = 0.f, on_diag = 0.f, w_diag = 0.f;
-#pragma unroll
-    for (int ip = 0; ip < TOK; ip += 2) {
-      if (ip + 1 < tile) continue;
-      f32x4 ek[2], ew[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int it = ip + u;
-        ek[u] = ew[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (it < tile) continue;
-        f32x4 w = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < 2; ++k) w = mfma8(row_frag_t<XT, M>(yt, it * 16, k * 32, lane), xf[k], w);
-        const int i0 = it * 16 + 4 * g;
-        const f32x4 hv = *reinterpret_cast<const f32x4*>(hi + i0), lv = *reinterpret_cast<const f32x4*>(lo + i0);
-        f32x4 q;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const bool in = i0 + r >= tok;
-          const float e = exp2_f((hv[r] - hj) + (lv[r] - lj));
-          ek[u][r] = in ? e * score[it][r] : 0.f;
-          ew[u][r] = in ? e * dj * w[r] : 0.f;
-          const float ekw = in ? ek[u][r] * w[r] : 0.f;
-          colsum += ekw;
-          const bool same = i0 + r == tok;
-          on_diag += same ? ekw : 0.f;
-          w_diag += same ? w[r] : 0.f;
-          q[r] = row_sum(same ? 0.f : ekw * dj);
+        if (t < LB) {
+          const float top = static_cast<float>(cum[k]);
+          o[HI + t] = top;
+          o[LO + t] = static_cast<float>(cum[k] - top);
+          o[DD + t] = s.d[k];
+          o[EC + t] = exp2_d(cum[k]);
+          o[EE + t] = exp2_d(s.total - cum[k]);
+          o[RB + t] = exp2_d(cum[k] - tile_start);
+          o[TD + t] = s.d[k] * exp2_d(tile_end - cum[k]);
         }
-        if (cs == 0 && n16 == 0) *reinterpret_cast<f32x4*>(rows + tile * LB + i0) = q;
       }
-      const Frag8<M> ekf = pair_frag<M>(ek[0], ek[1]), ewf = pair_frag<M>(ew[0], ew[1]);
-#pragma unroll
-      for (int p = 0; p < PW; ++p) dx[p] = mfma8(col_frag<XT, M>(yt, ip * 16, (cs * PW + p) * 16, lane), ekf, dx[p]);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) dk[nt] = mfma8(col_frag<KT, M>(qt, ip * 16, (cs * NT + nt) * 16, lane), ewf, dk[nt]);
-      hold_order();
-    }
-    colsum = group_sum(colsum);
-    on_diag = group_sum(on_diag);
-    w_diag = group_sum(w_diag);
-    if (cs == 0 && g == 0) {
-      col[tok] = colsum;
-      diag[tok] = on_diag;
-      wjj[tok] = w_diag;
-    }
-    hold_order();
-    // Rows i of this wave's tile: dq from the columns j <= i, and from the state.
-    const float e_i = ec[tok];
-#pragma unroll
-    for (int jp = 0; jp < TOK; jp += 2) {
-      if (jp > tile) continue;
-      f32x4 ew[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int jt = jp + u;
-        ew[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (jt > tile) continue;
-        f32x4 w = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < 2; ++k) w = mfma8(row_frag_t<XT, M>(xt, jt * 16, k * 32, lane), yf[k], w);
-        const int j0 = jt * 16 + 4 * g;
-        const f32x4 hv = *reinterpret_cast<const f32x4*>(hi + j0), lv = *reinterpret_cast<const f32x4*>(lo + j0),
-                    dv = *reinterpret_cast<const f32x4*>(dd + j0);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) ew[u][r] = j0 + r <= tok ? exp2_f((hj - hv[r]) + (lj - lv[r])) * dv[r] * w[r] : 0.f;
-      }
-      const Frag8<M> ewf = pair_frag<M>(ew[0], ew[1]);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) dq[nt] = mfma8(col_frag<KT, M>(kt, jp * 16, (cs * NT + nt) * 16, lane), ewf, dq[nt]);
-      hold_order();
-    }
-    hold_order();
-    float dot1 = 0.f;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      f32x4 r = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = SP - 1; s >= 0; --s) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) r = mfma8(col_frag<KT, M>(st + s * Lds::STATE, k * 32, (cs * NT + nt) * 16, lane), yf[k], r);
-      }
-      const f32x4 qv = lds_row4<M>(qt + KT::at(tok, (cs * NT + nt) * 16 + 4 * g));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        dot1 = fmaf(qv[e], r[e], dot1);
-        dq[nt][e] = fmaf(e_i, r[e], dq[nt][e]);
-      }
-      if (nt & 1) hold_order();
-    }
-    dot1 = group_sum(dot1);
-    if (g == 0) t1[cs * LB + tok] = e_i * dot1;
-    __syncthreads();
-    put_state(gr);
-    __syncthreads();
-    // Columns j again: dk and dx from the adjoint.
-    const float e_t = et[tok];
-    float dot2 = 0.f;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      f32x4 r = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = SP - 1; s >= 0; --s) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k) r = mfma8(col_frag<KT, M>(st + s * Lds::STATE, k * 32, (cs * NT + nt) * 16, lane), xf[k], r);
-      }
-      const f32x4 kv = lds_row4<M>(kt + KT::at(tok, (cs * NT + nt) * 16 + 4 * g));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        dot2 = fmaf(kv[e], r[e], dot2);
-        dk[nt][e] = fmaf(dj * e_t, r[e], dk[nt][e]);
-      }
-      if (nt & 1) hold_order();
-    }
-    dot2 = group_sum(dot2);
-    if (g == 0) t2[cs * LB + tok] = e_t * dot2;
-    {
-      Frag8<M> kf[NK];
-#pragma unroll
-      for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<KT, M>(kt, tile * 16, kk * 32, lane);
-#pragma unroll
-      for (int p = 0; p < PW; ++p) {
-        f32x4 u = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int kk = 0; kk < NK; ++kk) u = mfma8(row_frag<KT, M>(st, (cs * PW + p) * 16, kk * 32, lane), kf[kk], u);
-        const int c = (cs * PW + p) * 16 + 4 * g;
-        const f32x4 yv = lds_row4<M>(yt + XT::at(tok, c));
-        f32x4 o;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = tok < live ? fmaf(dj, fmaf(e_t, u[e], dx[p][e]), skip * yv[e]) : 0.f;
-        if (tok < in_block) store_row4<E>(dxp + static_cast<int64_t>(tok) * hs * f.P + c, pw - c, pvec, o);
-      }
-    }
-    __syncthreads();
-    // The step sizes, by the wave that holds their scalars.
-    if (wave == 0) {
-      float dc[PL], direct[PL], back = 0.f, tail = 0.f, dskip = 0.f;
+    };
+    // The step sizes' gradient of a head whose products are all in LDS.
+    auto end_head = [&](int hp, const Steps& s) {
+      const int lane = lane_id();
+      const float rate = f.rates[head_of(hp)];
+      const float* o = scal + (hp & 1) * Lds::SCAL;
+      float dc[PL], direct[PL], back = 0.f, tail = 0.f;
 #pragma unroll
       for (int k = PL - 1; k >= 0; --k) {
-        const int t = lane * PL + k;
-        float s1 = 0.f, s2 = 0.f, rs = 0.f;
+        const int t = lane * PL + k;  // (lanes past the block read other numbers of it, and are left out below)
+        float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-        for (int c = 0; c < CS; ++c) { s1 += t1[c * LB + t]; s2 += t2[c * LB + t]; }
-#pragma unroll
-        for (int j = 0; j < TOK; ++j) rs += j * 16 <= t ? rows[j * LB + t] : 0.f;
-        direct[k] = col[t] + s2;
-        back += (rs - dt[k] * (col[t] - diag[t])) + (s1 - dt[k] * s2);
+        for (int c = 0; c < CS; ++c) { s1 += o[T1 + c * LB + t]; s2 += o[T2 + c * LB + t]; }
+        const float cols = o[COL + t];
+        direct[k] = cols + s2;
+        back += (o[ROW + t] - s.d[k] * cols) + (s1 - s.d[k] * s2);
         dc[k] = back;  // over this lane's tokens from k on
-        tail += dt[k] * s2;
-        dskip += wjj[t];
+        tail += s.d[k] * s2;
       }
-      float behind = back;  // inclusive suffix sum over the lanes
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const float up = __shfl_down(behind, o);
-        if (lane + o < 64) behind += up;
-      }
+      static_assert(LB == 64 * PL, "a lane for every PL tokens");
+      // Sums over the lanes behind: inside rows of 16, then the rows behind.
+      float behind = back;
+      behind += dpp_shl<1>(behind);
+      behind += dpp_shl<2>(behind);
+      behind += dpp_shl<4>(behind);
+      behind += dpp_shl<8>(behind);
+      const float r1 = lane_f32(behind, 16), r2 = lane_f32(behind, 32), r3 = lane_f32(behind, 48);
+      behind += lane < 16 ? (r1 + r2) + r3 : lane < 32 ? r2 + r3 : lane < 48 ? r3 : 0.f;
       behind -= back;
       tail = group_sum(row_sum(tail));
-      float gdot = 0.f;
+      float gdot = 0.f, dskip = 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) gdot += gs[k];
-      const float end = fmaf(exp2_d(total), gdot, tail);
+      for (int k = 0; k < 8; ++k) {
+        gdot += o[GS + k];
+        dskip += o[WJ + k];
+      }
+      const float end = fmaf(exp2_d(s.total), gdot, tail);
       float da = 0.f, db = 0.f;
 #pragma unroll
       for (int k = 0; k < PL; ++k) {
-        const int64_t t = lane * PL + k;
+        const int t = lane * PL + k;
         const float dl = dc[k] + behind + end;
-        float dz = fmaf(rate, dl, direct[k]);
-        if (f.softplus && t < live) {
-          const float z = raw_step<E>(f, b, t0 + t, h);
-          dz *= z > 20.f ? 1.f : 1.f / (1.f + __expf(-z));
-        }
-        dz = t < live ? dz : 0.f;
-        da = fmaf(dt[k], dl, da);
+        const float dz = t < live ? fmaf(rate, dl, direct[k]) * s.slope[k] : 0.f;
+        da = fmaf(s.d[k], dl, da);
         db += dz;
-        if (t < in_block) put_step(t, dz);
+        if (t < in_block) put_step(hp, t, dz);
       }
       da = group_sum(row_sum(da));
       db = group_sum(row_sum(db));
-      dskip = group_sum(row_sum(dskip));
-      if (lane < 3) hpart[lane] = lane == 0 ? da : lane == 1 ? dskip : db;
+      if (lane < 3) head_sums(hp)[lane] = lane == 0 ? da : lane == 1 ? dskip : db;
+    };
+
+    Steps now{}, old{};
+    ask_rows(h_lo);
+    if (wave == kStepWave) ask_steps(h_lo);
+    {
+      TileLoad<E, KT, M, VEC, LB, NP, kGradThreads> r;
+      r.init(f.kt, f.N, tid);
+      r.load(static_cast<const eraw*>(f.keys) + b * f.kb + t0 * f.kt + gi * f.N, live, tid);
+      r.store(kt, tid);
+      r.init(f.qt, f.N, tid);
+      r.load(static_cast<const eraw*>(f.queries) + b * f.qb + t0 * f.qt + gi * f.N, live, tid);
+      r.store(qt, tid);
+    }
+    if (wave == kStepWave) {
+      begin_head(h_lo, now);
+      if (h_lo + 1 < h_hi) ask_steps(h_lo + 1);
     }
     __syncthreads();
+    // K: columns j of this wave's tile, rows i of the tiles from its own on (d tiles further).
+    f32x4 score[TOK];
+    {
+      Frag8<M> kf[NK];
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<KT, M>(kt, tile * 16, kk * 32);
+#pragma unroll
+      for (int d = 0; d < TOK; ++d) {
+        score[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (tile + d < TOK) {
+#pragma unroll
+          for (int kk = 0; kk < NK; ++kk) score[d] = mfma8(row_frag<KT, M>(qt, (tile + d) * 16, kk * 32), kf[kk], score[d]);
+        }
+      }
+    }
+
+    for (int hp = h_lo; hp < h_hi; ++hp) {
+      // The lane's number anew for every head, so that the hundreds of LDS addresses made from it are not kept in
+      // registers from head to head.
+      int lane = lane_id();
+      asm volatile("" : "+v"(lane));
+      const int g = lane >> 4, n16 = lane & 15, tok = tile * 16 + n16;  // this lane's token in both orders
+      const int h = head_of(hp), p0 = hp % f.PT * kSelRows, pw = f.P - p0;
+      const float skip = f.skip == nullptr ? 0.f : f.skip[h];
+      const int64_t sat = (((static_cast<int64_t>(b) * f.nsave + blk) * f.H + h) * f.P + p0) * f.N;
+      float* sc = scal + (hp & 1) * Lds::SCAL;
+      xr.store(xt, tid);
+      yr.store(yt, tid);
+      StateLoad<M, NP> sr, gr;
+      sr.load(f.states + sat, pw, f.N, tid);
+      __syncthreads();
+
+      // Columns j of this wave's tile: dx and dk from the rows i >= j, two tiles of rows at a time.
+      f32x4 dx[PW];
+#pragma unroll
+      for (int p = 0; p < PW; ++p) dx[p] = f32x4{0.f, 0.f, 0.f, 0.f};
+      Frag8<M> xf[2], yf[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        xf[k] = row_frag_t<XT, M>(xt, tile * 16, k * 32, lane);
+        yf[k] = row_frag_t<XT, M>(yt, tile * 16, k * 32, lane);
+      }
+      const float hj = sc[HI + tok], lj = sc[LO + tok], dj = sc[DD + tok];
+      float colsum = 0.f, w_diag = 0.f;
+#pragma unroll
+      for (int dp = 0; dp < TOK; dp += 2) {
+        if (tile + dp >= TOK) continue;
+        // The second tile past the block is the first again, with weights of zero.
+        const int i0 = tile + dp, i1 = i0 + 1 < TOK ? i0 + 1 : i0;
+        f32x4 ek[2], ew[2], w[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          w[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < 2; ++k) w[u] = mfma8(row_frag_t<XT, M>(yt, (u ? i1 : i0) * 16, k * 32, lane), xf[k], w[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int it = u ? i1 : i0, ti = it * 16 + 4 * g;
+          if (dp + u == 0) {  // the tile on the diagonal
+            const f32x4 hv = *reinterpret_cast<const f32x4*>(sc + HI + ti), lv = *reinterpret_cast<const f32x4*>(sc + LO + ti);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const bool in = ti + r >= tok;
+              const float e = exp2_f(in ? (hv[r] - hj) + (lv[r] - lj) : -INFINITY), wr = in ? w[u][r] : 0.f;
+              ek[u][r] = e * (in ? score[0][r] : 0.f);
+              ew[u][r] = e * dj * wr;
+              colsum = fmaf(ek[u][r], wr, colsum);
+              w_diag += ti + r == tok ? wr : 0.f;
+            }
+          } else {
+            // e^{c_i - c_j} through the end of the tile before i's: one exponential a lane, one product a pair.
+            const f32x4 rv = *reinterpret_cast<const f32x4*>(sc + RB + ti);
+            const bool on = u == 0 || i1 != i0;
+            const float c = on ? exp2_f((sc[HI + it * 16 - 1] - hj) + (sc[LO + it * 16 - 1] - lj)) : 0.f, cd = c * dj;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              ek[u][r] = rv[r] * c * score[dp + u][r];
+              ew[u][r] = rv[r] * cd * w[u][r];
+              colsum = fmaf(ek[u][r], w[u][r], colsum);
+            }
+          }
+        }
+        const Frag8<M> ekf = pair_frag<M>(ek[0], ek[1]), ewf = pair_frag<M>(ew[0], ew[1]);
+#pragma unroll
+        for (int p = 0; p < PW; ++p) dx[p] = mfma8(col_frag2<XT, M>(yt, i0 * 16, i1 * 16, (cs * PW + p) * 16, lane), ekf, dx[p]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          dk[nt] = mfma8(col_frag2<KT, M>(qt, i0 * 16, i1 * 16, (cs * NT + nt) * 16, lane), ewf, dk[nt]);
+        hold_order();
+      }
+      colsum = group_sum(colsum);
+      w_diag = group_sum(row_sum(w_diag));
+      if (cs == 0 && g == 0) sc[COL + tok] = colsum;
+      if (lane == 0) sc[WJ + wave] = cs == 0 ? w_diag : 0.f;
+
+      // Rows i of this wave's tile: dq from the columns j <= i, and the rows' sums.
+      const float e_i = sc[EC + tok];
+      float rowsum = 0.f;
+      Frag8<M> qf[NK];
+#pragma unroll
+      for (int kk = 0; kk < NK; ++kk) qf[kk] = row_frag<KT, M>(qt, tile * 16, kk * 32, lane);
+#pragma unroll 1
+      for (int dp = 0; dp <= tile; dp += 2) {
+        const int j0 = tile - dp, j1 = j0 > 0 ? j0 - 1 : 0;
+        f32x4 ew[2], w[2], k2[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          w[u] = k2[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int k = 0; k < 2; ++k) w[u] = mfma8(row_frag_t<XT, M>(xt, (u ? j1 : j0) * 16, k * 32, lane), yf[k], w[u]);
+#pragma unroll
+          for (int kk = 0; kk < NK; ++kk) k2[u] = mfma8(row_frag<KT, M>(kt, (u ? j1 : j0) * 16, kk * 32, lane), qf[kk], k2[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int jt = u ? j1 : j0, tj = jt * 16 + 4 * g;
+          // On the diagonal pair by pair; else through the end of j's tile, one exponential a lane.
+          const f32x4 hv = *reinterpret_cast<const f32x4*>(sc + HI + tj), lv = *reinterpret_cast<const f32x4*>(sc + LO + tj),
+                      dv = *reinterpret_cast<const f32x4*>(sc + (jt == tile ? DD : TD) + tj);
+          const bool on = u == 0 || j0 > 0;
+          const float c = on ? exp2_f((hj - sc[HI + jt * 16 + 15]) + (lj - sc[LO + jt * 16 + 15])) : 0.f;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const bool in = tj + r <= tok;
+            const float e = jt == tile ? exp2_f(in ? (hj - hv[r]) + (lj - lv[r]) : -INFINITY) : c;
+            ew[u][r] = on && in ? e * dv[r] * w[u][r] : 0.f;
+            rowsum += on && in ? ew[u][r] * k2[u][r] : 0.f;
+          }
+        }
+        const Frag8<M> ewf = pair_frag<M>(ew[0], ew[1]);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          dq[nt] = mfma8(col_frag2<KT, M>(kt, j0 * 16, j1 * 16, (cs * NT + nt) * 16, lane), ewf, dq[nt]);
+      }
+      rowsum = group_sum(rowsum);
+      if (cs == 0 && g == 0) sc[ROW + tok] = rowsum;
+      // The step wave has waited least so far: the head before ends here, and the next one begins.
+      if (wave == kStepWave) {
+        if (hp > h_lo) end_head(hp - 1, old);
+        old = now;
+        if (hp + 1 < h_hi) {
+          begin_head(hp + 1, now);
+          if (hp + 2 < h_hi) ask_steps(hp + 2);
+        }
+      }
+      sr.store(st, tid);
+      gr.load(a.adj + sat, pw, f.N, tid);
+      __syncthreads();
+
+      // From the state: dq.
+      if (hp + 1 < h_hi) ask_rows(hp + 1);
+      float dot1 = 0.f;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        f32x4 r = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = SP - 1; s >= 0; --s) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) r = mfma8(col_frag<KT, M>(st + s * Lds::STATE, k * 32, (cs * NT + nt) * 16, lane), yf[k], r);
+        }
+        const f32x4 qv = lds_row4<M>(qt + KT::at(tok, (cs * NT + nt) * 16 + 4 * g));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          dot1 = fmaf(qv[e], r[e], dot1);
+          dq[nt][e] = fmaf(e_i, r[e], dq[nt][e]);
+        }
+        if (nt & 1) hold_order();
+      }
+      dot1 = group_sum(dot1);
+      if (g == 0) sc[T1 + cs * LB + tok] = e_i * dot1;
+      float dot = 0.f;
+#pragma unroll
+      for (int i = 0; i < StateLoad<M, NP>::PER; ++i) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) dot = fmaf(gr.r[i][e], sr.r[i][e], dot);
+      }
+      dot = group_sum(row_sum(dot));
+      if (lane == 0) sc[GS + wave] = dot;
+      __syncthreads();
+      gr.store(st, tid);
+      __syncthreads();
+
+      // From the adjoint: dk and dx.
+      const float e_t = sc[EE + tok];
+      float dot2 = 0.f;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        f32x4 r = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = SP - 1; s >= 0; --s) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) r = mfma8(col_frag<KT, M>(st + s * Lds::STATE, k * 32, (cs * NT + nt) * 16, lane), xf[k], r);
+        }
+        const f32x4 kv = lds_row4<M>(kt + KT::at(tok, (cs * NT + nt) * 16 + 4 * g));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          dot2 = fmaf(kv[e], r[e], dot2);
+          dk[nt][e] = fmaf(dj * e_t, r[e], dk[nt][e]);
+        }
+        if (nt & 1) hold_order();
+      }
+      dot2 = group_sum(dot2);
+      if (g == 0) sc[T2 + cs * LB + tok] = e_t * dot2;
+      {
+        eraw* dxp = static_cast<eraw*>(a.dx) + ((row_b + tok) * f.H + h) * f.P + p0;
+        Frag8<M> kf[NK];
+#pragma unroll
+        for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<KT, M>(kt, tile * 16, kk * 32, lane);
+#pragma unroll
+        for (int p = 0; p < PW; ++p) {
+          f32x4 u = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int kk = 0; kk < NK; ++kk) u = mfma8(row_frag<KT, M>(st, (cs * PW + p) * 16, kk * 32, lane), kf[kk], u);
+          const int c = (cs * PW + p) * 16 + 4 * g;
+          const f32x4 yv = lds_row4<M>(yt + XT::at(tok, c));
+          f32x4 o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = tok < live ? fmaf(dj, fmaf(e_t, u[e], dx[p][e]), skip * yv[e]) : 0.f;
+          if (tok < in_block) store_row4<E>(dxp + c, pw - c, pvec, o);
+        }
+      }
+      __syncthreads();
+    }
+    if (wave == kStepWave) end_head(h_hi - 1, old);
   }
 
   // dk and dq of this workgroup's heads.
+  const int lane = lane_id(), g = lane >> 4, tok = tile * 16 + (lane & 15);
   const int64_t all = static_cast<int64_t>(f.B) * f.T * f.G * f.N;
-  const int64_t at = (static_cast<int64_t>(b) * f.T + t0 + tok) * f.G * f.N + static_cast<int64_t>(gi) * f.N;
-  if (t0 + tok < f.T) {
+  const int64_t at = (row_b + tok) * f.G * f.N + static_cast<int64_t>(gi) * f.N;
+  if (tok < in_block) {
     const bool on = tok < live;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {

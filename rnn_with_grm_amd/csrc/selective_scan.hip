@@ -173,7 +173,13 @@ __global__ __launch_bounds__(kWalkThreads) __attribute__((amdgpu_waves_per_eu(2,
                       dj = *reinterpret_cast<const f32x4*>(sc + 2 * L + j0);
           const float hi_i = sc[i], lo_i = sc[L + i];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) d[r] = j0 + r <= i ? d[r] * dj[r] * exp2_f((hi_i - hj[r]) + (lo_i - lj[r])) : 0.f;
+          for (int r = 0; r < 4; ++r) {
+            // Above the diagonal both factors are zeros: a select of their product would become a branch round
+            // the exponential.
+            const bool in = j0 + r <= i;
+            const float x = (hi_i - hj[r]) + (lo_i - lj[r]);
+            d[r] = (in ? d[r] * dj[r] : 0.f) * exp2_f(in ? x : -INFINITY);
+          }
           // One rounding of the weights to 16 bits, as far from them as the output's own rounding is
           // from it; the values they meet are exact.
           store4_raw<M>(m + MT::at(i, j0), d);
