@@ -12,11 +12,12 @@
 //   dl_t = sum_{s >= t} dc_s + sum_j d_j t2_j + e^{c_L} <G, S>     (l_t = d_t A, the log decay)
 //   dd_t = A dl_t + sum_i E_it K_it W_it + t2_t,   dA = sum_t d_t dl_t,   dD = sum_t W_tt
 //
-// Three steps.  The forward has left S before every block; the reverse walk (selective_pass_kernel)
-// leaves G behind every block; then all blocks run side by side, one workgroup for a block and some
-// of a group's heads, whose dk and dq it sums in registers (K is formed once for all of them).  Where more
-// than one workgroup shares a group, their sums are added in a fixed order by a last kernel: no
-// atomics, the same bits on every run.
+// Steps.  The forward has left S before every block; the reverse walk (selective_pass_kernel)
+// leaves G behind every block, and selective_token_kernel every token's decays; then all blocks run side by
+// side, one workgroup for a block and some of a group's heads, whose dk and dq it sums in registers.  It leaves dc
+// and du . x by token, of which selective_steps_kernel makes the step sizes' gradients, one wave a head and block.
+// Where more than one workgroup shares a group, their sums are added in a fixed order by a last
+// kernel: no atomics, the same bits on every run.
 //
 // The step sizes' gradient is a difference of large sums, so its terms stay float32: K and W are sums
 // of exact products, and S and G enter t1 and t2 as two bfloat16 parts (16 bits and more; 2^-17).
@@ -31,17 +32,24 @@ namespace {
 
 constexpr int kGradThreads = 512;
 
+// A head's numbers by token, planes of LB in `tokens`: log2 decay from the block's start through the token in two
+// floats, step size, e^c, e^{c_L - c}, and decays inside 16-token tiles: from the end of the tile before
+// through the token, and from the token through its tile's end times the step size.
+enum { HI, LO, DD, EC, EE, RB, TD, kPlanes };
+
 struct GradArgs {
   SelArgs s;              // the forward's inputs; states: S before every block
   const void* dy;         // [B, T, H, P]
   const float* adj;       // [B, nsave, H, P, N]: G behind every block
+  float* tokens;          // [B, nsave, H, kPlanes, LB]
+  float* diffs;           // [B, nsave, H * PT, shares, LB, 2]: dc and du . x of each token
+  float* dots;            // [B, nsave, H * PT, 8, 2]: <G, S> and sum W_jj, then [.., 8]: sum d_j t2_j, a part a wave
   void* dx;               // [B, T, H, P]
   void* dk;               // [B, T, G, N]
   void* dq;               // [B, T, G, N]
   void* dsteps;           // [B, T, H]
   float* rows_part;       // [splits][2][B, T, G, N] or null: dk and dq of each share of the heads
-  float* steps_part;      // [PT][B, T, H] or null
-  float* head_part;       // [B * nsave][H * PT][3]
+  float* head_part;       // [B * nsave, H, 3]: dA, dD and the step bias's gradient
   int splits;
 };
 
@@ -56,10 +64,7 @@ struct GradLds {
   static constexpr int TILES = LB * (2 * KT::STRIDE + 2 * XT::STRIDE) + SPARTS * STATE;
   static constexpr int TOK = LB / 16;                          // token tiles
   static constexpr int CS = 8 / TOK;                           // waves that share one, a share of the columns each
-  // A head's numbers by token: hi, lo, d, e^c, e^{c_L - c}, decays inside a tile (two); column and row sums;
-  // t1, t2 per share; then sums of W_jj and <G, S> per wave.
-  static constexpr int SCAL = (9 + 2 * CS) * LB + 16;
-  static constexpr size_t bytes = TILES * sizeof(typename ET<M>::raw) + 2 * SCAL * sizeof(float);
+  static constexpr size_t bytes = TILES * sizeof(typename ET<M>::raw) + kPlanes * LB * sizeof(float);
   static_assert(bytes <= 160 * 1024, "one CU's LDS");
 };
 
@@ -144,6 +149,139 @@ struct StateLoad {
   }
 };
 
+// One wave a head and block: every token's decays (PL tokens a lane).
+template <class E, int LB>
+__global__ __launch_bounds__(256) void selective_token_kernel(GradArgs a) {
+  constexpr int PL = LB / 64;
+  const SelArgs& f = a.s;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (id >= static_cast<int64_t>(f.B) * f.nsave * f.H) return;
+  const int h = static_cast<int>(id % f.H), lane = lane_id();
+  const int64_t blk = id / f.H % f.nsave, t0 = blk * LB;
+  const int b = static_cast<int>(id / f.H / f.nsave);
+  const int64_t len = sel_length(f, b);
+  if (t0 >= len) return;
+  const float rate = f.rates[h];
+  float d[PL];
+  double cum[PL], sum = 0.0;
+#pragma unroll
+  for (int k = 0; k < PL; ++k) {
+    const int64_t t = t0 + lane * PL + k;
+    d[k] = t < len ? step_size(f, raw_step<E>(f, b, t, h)) : 0.f;
+    double l = static_cast<double>(d[k]) * static_cast<double>(rate);
+    l = l < -200.0 ? -200.0 : l;
+    sum += l * 1.4426950408889634;
+    cum[k] = sum;
+  }
+  const double scan = wave_prefix(sum), before = scan - sum, total = lane_value(scan, 63);
+#pragma unroll
+  for (int k = 0; k < PL; ++k) cum[k] += before;
+  constexpr int LPT = 16 / PL;  // lanes of a tile
+  const int first = lane / LPT * LPT;
+  const double tile_end = __shfl(cum[PL - 1], first + LPT - 1), up = __shfl(cum[PL - 1], first > 0 ? first - 1 : 0);
+  const double tile_start = first > 0 ? up : 0.0;
+  float* o = a.tokens + id * kPlanes * LB + lane * PL;
+#pragma unroll
+  for (int k = 0; k < PL; ++k) {
+    const float top = static_cast<float>(cum[k]);
+    o[HI * LB + k] = top;
+    o[LO * LB + k] = static_cast<float>(cum[k] - top);
+    o[DD * LB + k] = d[k];
+    o[EC * LB + k] = exp2_d(cum[k]);
+    o[EE * LB + k] = exp2_d(total - cum[k]);
+    o[RB * LB + k] = exp2_d(cum[k] - tile_start);
+    o[TD * LB + k] = d[k] * exp2_d(tile_end - cum[k]);
+  }
+}
+
+// One wave a head and block: the step sizes' gradients from dc, du . x and the states' product,
+//   dl_t = sum_{s >= t} dc_s + end,  dd_t = A dl_t + du_t . x_t,  end = sum_j d_j t2_j + e^{c_L} <G, S>.
+template <class E, int LB, int CS>
+__global__ __launch_bounds__(256) void selective_steps_kernel(GradArgs a) {
+  constexpr int PL = LB / 64;
+  const SelArgs& f = a.s;
+  const int64_t id = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (id >= static_cast<int64_t>(f.B) * f.nsave * f.H) return;
+  const int h = static_cast<int>(id % f.H), lane = lane_id();
+  const int64_t blk = id / f.H % f.nsave, t0 = blk * LB;
+  const int b = static_cast<int>(id / f.H / f.nsave);
+  const int64_t len = sel_length(f, b);
+  float da = 0.f, db = 0.f, dskip = 0.f, dz[PL];
+#pragma unroll
+  for (int k = 0; k < PL; ++k) dz[k] = 0.f;
+  if (t0 < len) {
+    const float* tk = a.tokens + id * kPlanes * LB + lane * PL;
+    float dc[PL], direct[PL], d[PL], gdot = 0.f, tail = 0.f;
+#pragma unroll
+    for (int k = 0; k < PL; ++k) {
+      d[k] = tk[DD * LB + k];
+      dc[k] = direct[k] = 0.f;
+    }
+    for (int pt = 0; pt < f.PT; ++pt) {
+      const int64_t hp = id * f.PT + pt;
+#pragma unroll
+      for (int c = 0; c < CS; ++c) {
+#pragma unroll
+        for (int k = 0; k < PL; ++k) {
+          const float2 v = *reinterpret_cast<const float2*>(a.diffs + ((hp * CS + c) * LB + lane * PL + k) * 2);
+          dc[k] += v.x;
+          direct[k] += v.y;
+        }
+      }
+      const float2 v = *reinterpret_cast<const float2*>(a.dots + (hp * 8 + (lane & 7)) * 2);
+      gdot += lane < 8 ? v.x : 0.f;
+      dskip += lane < 8 ? v.y : 0.f;
+      // d_j t2_j: the tokens' sums that the workgroups left beside.
+      const float* t2 = a.dots + static_cast<int64_t>(f.B) * f.nsave * f.H * f.PT * 16 + hp * 8;
+      tail += lane < 8 ? t2[lane] : 0.f;
+    }
+    const float total = lane_f32(tk[HI * LB + PL - 1], 63), rest = lane_f32(tk[LO * LB + PL - 1], 63);
+    gdot = group_sum(row_sum(gdot));
+    dskip = group_sum(row_sum(dskip));
+    tail = group_sum(row_sum(tail));
+    const float end = fmaf(exp2_f(total) * exp2_f(rest), gdot, tail);
+    float back = 0.f;
+#pragma unroll
+    for (int k = PL - 1; k >= 0; --k) {
+      back += dc[k];
+      dc[k] = back;  // over this lane's tokens from k on
+    }
+    // Sums over the lanes behind: inside rows of 16, then the rows behind.
+    float behind = back;
+    behind += dpp_shl<1>(behind);
+    behind += dpp_shl<2>(behind);
+    behind += dpp_shl<4>(behind);
+    behind += dpp_shl<8>(behind);
+    const float r1 = lane_f32(behind, 16), r2 = lane_f32(behind, 32), r3 = lane_f32(behind, 48);
+    behind += lane < 16 ? (r1 + r2) + r3 : lane < 32 ? r2 + r3 : lane < 48 ? r3 : 0.f;
+    behind -= back;
+    const float rate = f.rates[h];
+#pragma unroll
+    for (int k = 0; k < PL; ++k) {
+      const int64_t t = t0 + lane * PL + k;
+      const float dl = dc[k] + behind + end;
+      if (t < len) {
+        float slope = 1.f;
+        if (f.softplus) {
+          const float z = raw_step<E>(f, b, t, h);
+          slope = z > 20.f ? 1.f : __builtin_amdgcn_rcpf(1.f + __expf(-z));
+        }
+        dz[k] = fmaf(rate, dl, direct[k]) * slope;
+        da = fmaf(d[k], dl, da);
+        db += dz[k];
+      }
+    }
+    da = group_sum(row_sum(da));
+    db = group_sum(row_sum(db));
+  }
+#pragma unroll
+  for (int k = 0; k < PL; ++k) {
+    const int64_t t = t0 + lane * PL + k;
+    if (t < f.T) st_state<E>(a.dsteps, (b * f.T + t) * f.H + h, f.steps_f32 != 0, dz[k]);
+  }
+  if (lane < 3) a.head_part[id * 3 + lane] = lane == 0 ? da : lane == 1 ? dskip : db;
+}
+
 template <class E, class M, int NP, bool VEC>
 __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void selective_grad_kernel(GradArgs a) {
   using S = SelShape<M>;
@@ -153,16 +291,15 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
   using KT = typename Lds::KT;
   using XT = typename Lds::XT;
   constexpr int LB = S::LB, TOK = Lds::TOK, CS = Lds::CS, SP = Lds::SPARTS;
-  constexpr int NK = NP / 32, NT = NP / 16 / CS, PW = kSelRows / 16 / CS, PL = (LB + 63) / 64;
+  constexpr int NK = NP / 32, NT = NP / 16 / CS, PW = kSelRows / 16 / CS;
+  constexpr int NPL = (kPlanes * LB + kGradThreads - 1) / kGradThreads;
   extern __shared__ __align__(16) unsigned char smem[];
   raw* kt = reinterpret_cast<raw*>(smem);
   raw* qt = kt + LB * KT::STRIDE;
   raw* xt = qt + LB * KT::STRIDE;
   raw* yt = xt + LB * XT::STRIDE;
   raw* st = yt + LB * XT::STRIDE;
-  float* scal = reinterpret_cast<float*>(st + SP * Lds::STATE);
-  constexpr int HI = 0, LO = LB, DD = 2 * LB, EC = 3 * LB, EE = 4 * LB, RB = 5 * LB, TD = 6 * LB, COL = 7 * LB, ROW = 8 * LB,
-                T1 = 9 * LB, T2 = T1 + CS * LB, WJ = T2 + CS * LB, GS = WJ + 8;
+  float* sc = reinterpret_cast<float*>(st + SP * Lds::STATE);
 
   const SelArgs& f = a.s;
   uint32_t v = xcd_order(blockIdx.x, gridDim.x);
@@ -182,147 +319,35 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
   const int h_lo = static_cast<int>(static_cast<int64_t>(heads) * split / a.splits),
             h_hi = static_cast<int>(static_cast<int64_t>(heads) * (split + 1) / a.splits);
   const int64_t row_b = static_cast<int64_t>(b) * f.T + t0;  // the block's first token
-  auto head_of = [&](int hp) { return gi * (f.H / f.G) + hp / f.PT; };
-  auto put_step = [&](int hp, int t, float x) {
-    const int64_t at = (row_b + t) * f.H + head_of(hp);
-    if (a.steps_part != nullptr) a.steps_part[static_cast<int64_t>(hp % f.PT) * f.B * f.T * f.H + at] = x;
-    else st_state<E>(a.dsteps, at, f.steps_f32 != 0, x);
-  };
-  auto head_sums = [&](int hp) {
-    return a.head_part + ((static_cast<int64_t>(b) * f.nsave + blk) * f.H * f.PT + head_of(hp) * f.PT + hp % f.PT) * 3;
-  };
+  const int64_t blocks = static_cast<int64_t>(b) * f.nsave + blk;
+  int h = gi * (f.H / f.G) + h_lo / f.PT, pt = h_lo % f.PT;  // the head and its value tile
 
   f32x4 dk[NT], dq[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) dk[i] = dq[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   if (live == 0) {  // behind the sequence's length: zeros
     for (int hp = h_lo; hp < h_hi; ++hp) {
-      const int p0 = hp % f.PT * kSelRows, cols = f.P - p0 < kSelRows ? f.P - p0 : kSelRows, lane = lane_id();
-      eraw* dxp = static_cast<eraw*>(a.dx) + (row_b * f.H + head_of(hp)) * f.P + p0;
+      const int p0 = pt * kSelRows, cols = f.P - p0 < kSelRows ? f.P - p0 : kSelRows, lane = lane_id();
+      eraw* dxp = static_cast<eraw*>(a.dx) + (row_b * f.H + h) * f.P + p0;
       for (int t = wave; t < in_block; t += 8) {
         if (lane < cols) dxp[static_cast<int64_t>(t) * f.H * f.P + lane] = ET<E>::from_f(0.f);
-        if (lane == 0) put_step(hp, t, 0.f);
       }
-      if (tid < 3) head_sums(hp)[tid] = 0.f;
+      if (++pt == f.PT) pt = 0, ++h;
     }
   } else {
-    constexpr int kStepWave = 7;  // the wave with the fewest tiles in the first of the two triangles
     TileLoad<E, XT, M, VEC, LB, kSelRows, kGradThreads> xr, yr;
-    auto ask_rows = [&](int hp) {
-      const int h = head_of(hp), p0 = hp % f.PT * kSelRows, cols = f.P - p0 < kSelRows ? f.P - p0 : kSelRows;
+    float pr[NPL];
+    auto ask_rows = [&](int hn, int pn) {
+      const int p0 = pn * kSelRows, cols = f.P - p0 < kSelRows ? f.P - p0 : kSelRows;
       xr.init(f.vt, cols, tid);
-      xr.load(static_cast<const eraw*>(f.values) + b * f.vb + t0 * f.vt + h * f.P + p0, live, tid);
+      xr.load(static_cast<const eraw*>(f.values) + b * f.vb + t0 * f.vt + hn * f.P + p0, live, tid);
       yr.init(static_cast<int64_t>(f.H) * f.P, cols, tid);
-      yr.load(static_cast<const eraw*>(a.dy) + (row_b * f.H + h) * f.P + p0, live, tid);
+      yr.load(static_cast<const eraw*>(a.dy) + (row_b * f.H + hn) * f.P + p0, live, tid);
+      const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(a.tokens + (blocks * f.H + hn) * kPlanes * LB, kPlanes * LB * 4);
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) pr[i] = buf_load1<F32>(rsrc, (tid + i * kGradThreads) * 4);
     };
-    // The step wave: a head's token scalars, PL tokens a lane, one head ahead of the others; what its end needs
-    // of them stays in registers.
-    struct Steps {
-      float d[PL], slope[PL];
-      double total;
-    };
-    uint32_t zr[PL];
-    auto ask_steps = [&](int hp) {
-#pragma unroll
-      for (int k = 0; k < PL; ++k) {
-        const int t = lane_id() * PL + k;
-        zr[k] = load_step<E>(f, b, t0 + t, head_of(hp), t < live);
-      }
-    };
-    auto begin_head = [&](int hp, Steps& s) {
-      const int lane = lane_id(), h = head_of(hp);
-      const float rate = f.rates[h], bias = f.bias == nullptr ? 0.f : f.bias[h];
-      float* o = scal + (hp & 1) * Lds::SCAL;
-      double cum[PL], sum = 0.0;
-#pragma unroll
-      for (int k = 0; k < PL; ++k) {
-        const float z = step_value<E>(f, zr[k]) + bias;
-        const bool on = lane * PL + k < live;
-        s.d[k] = on ? step_size(f, z) : 0.f;
-        s.slope[k] = !on ? 0.f : !f.softplus || z > 20.f ? 1.f : __builtin_amdgcn_rcpf(1.f + __expf(-z));
-        double l = static_cast<double>(s.d[k]) * static_cast<double>(rate);
-        l = l < -200.0 ? -200.0 : l;
-        sum += l * 1.4426950408889634;
-        cum[k] = sum;
-      }
-      const double scan = wave_prefix(sum), before = scan - sum;
-      s.total = lane_value(scan, LB / PL - 1);
-#pragma unroll
-      for (int k = 0; k < PL; ++k) cum[k] += before;
-      // The sums before this token's tile and through its end.
-      constexpr int LPT = 16 / PL;  // lanes of a tile
-      const int first = lane / LPT * LPT;
-      const double tile_end = __shfl(cum[PL - 1], first + LPT - 1), up = __shfl(cum[PL - 1], first > 0 ? first - 1 : 0);
-      const double tile_start = first > 0 ? up : 0.0;
-#pragma unroll
-      for (int k = 0; k < PL; ++k) {
-        const int t = lane * PL + k;
-        if (t < LB) {
-          const float top = static_cast<float>(cum[k]);
-          o[HI + t] = top;
-          o[LO + t] = static_cast<float>(cum[k] - top);
-          o[DD + t] = s.d[k];
-          o[EC + t] = exp2_d(cum[k]);
-          o[EE + t] = exp2_d(s.total - cum[k]);
-          o[RB + t] = exp2_d(cum[k] - tile_start);
-          o[TD + t] = s.d[k] * exp2_d(tile_end - cum[k]);
-        }
-      }
-    };
-    // The step sizes' gradient of a head whose products are all in LDS.
-    auto end_head = [&](int hp, const Steps& s) {
-      const int lane = lane_id();
-      const float rate = f.rates[head_of(hp)];
-      const float* o = scal + (hp & 1) * Lds::SCAL;
-      float dc[PL], direct[PL], back = 0.f, tail = 0.f;
-#pragma unroll
-      for (int k = PL - 1; k >= 0; --k) {
-        const int t = lane * PL + k;  // (lanes past the block read other numbers of it, and are left out below)
-        float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-        for (int c = 0; c < CS; ++c) { s1 += o[T1 + c * LB + t]; s2 += o[T2 + c * LB + t]; }
-        const float cols = o[COL + t];
-        direct[k] = cols + s2;
-        back += (o[ROW + t] - s.d[k] * cols) + (s1 - s.d[k] * s2);
-        dc[k] = back;  // over this lane's tokens from k on
-        tail += s.d[k] * s2;
-      }
-      static_assert(LB == 64 * PL, "a lane for every PL tokens");
-      // Sums over the lanes behind: inside rows of 16, then the rows behind.
-      float behind = back;
-      behind += dpp_shl<1>(behind);
-      behind += dpp_shl<2>(behind);
-      behind += dpp_shl<4>(behind);
-      behind += dpp_shl<8>(behind);
-      const float r1 = lane_f32(behind, 16), r2 = lane_f32(behind, 32), r3 = lane_f32(behind, 48);
-      behind += lane < 16 ? (r1 + r2) + r3 : lane < 32 ? r2 + r3 : lane < 48 ? r3 : 0.f;
-      behind -= back;
-      tail = group_sum(row_sum(tail));
-      float gdot = 0.f, dskip = 0.f;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        gdot += o[GS + k];
-        dskip += o[WJ + k];
-      }
-      const float end = fmaf(exp2_d(s.total), gdot, tail);
-      float da = 0.f, db = 0.f;
-#pragma unroll
-      for (int k = 0; k < PL; ++k) {
-        const int t = lane * PL + k;
-        const float dl = dc[k] + behind + end;
-        const float dz = t < live ? fmaf(rate, dl, direct[k]) * s.slope[k] : 0.f;
-        da = fmaf(s.d[k], dl, da);
-        db += dz;
-        if (t < in_block) put_step(hp, t, dz);
-      }
-      da = group_sum(row_sum(da));
-      db = group_sum(row_sum(db));
-      if (lane < 3) head_sums(hp)[lane] = lane == 0 ? da : lane == 1 ? dskip : db;
-    };
-
-    Steps now{}, old{};
-    ask_rows(h_lo);
-    if (wave == kStepWave) ask_steps(h_lo);
+    ask_rows(h, pt);
     {
       TileLoad<E, KT, M, VEC, LB, NP, kGradThreads> r;
       r.init(f.kt, f.N, tid);
@@ -332,26 +357,6 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       r.load(static_cast<const eraw*>(f.queries) + b * f.qb + t0 * f.qt + gi * f.N, live, tid);
       r.store(qt, tid);
     }
-    if (wave == kStepWave) {
-      begin_head(h_lo, now);
-      if (h_lo + 1 < h_hi) ask_steps(h_lo + 1);
-    }
-    __syncthreads();
-    // K: columns j of this wave's tile, rows i of the tiles from its own on (d tiles further).
-    f32x4 score[TOK];
-    {
-      Frag8<M> kf[NK];
-#pragma unroll
-      for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<KT, M>(kt, tile * 16, kk * 32);
-#pragma unroll
-      for (int d = 0; d < TOK; ++d) {
-        score[d] = f32x4{0.f, 0.f, 0.f, 0.f};
-        if (tile + d < TOK) {
-#pragma unroll
-          for (int kk = 0; kk < NK; ++kk) score[d] = mfma8(row_frag<KT, M>(qt, (tile + d) * 16, kk * 32), kf[kk], score[d]);
-        }
-      }
-    }
 
     for (int hp = h_lo; hp < h_hi; ++hp) {
       // The lane's number anew for every head, so that the hundreds of LDS addresses made from it are not kept in
@@ -359,12 +364,16 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       int lane = lane_id();
       asm volatile("" : "+v"(lane));
       const int g = lane >> 4, n16 = lane & 15, tok = tile * 16 + n16;  // this lane's token in both orders
-      const int h = head_of(hp), p0 = hp % f.PT * kSelRows, pw = f.P - p0;
+      const int p0 = pt * kSelRows, pw = f.P - p0;
       const float skip = f.skip == nullptr ? 0.f : f.skip[h];
-      const int64_t sat = (((static_cast<int64_t>(b) * f.nsave + blk) * f.H + h) * f.P + p0) * f.N;
-      float* sc = scal + (hp & 1) * Lds::SCAL;
+      const int64_t sat = ((blocks * f.H + h) * f.P + p0) * f.N;
+      const int64_t pair = (blocks * f.H + h) * f.PT + pt;
       xr.store(xt, tid);
       yr.store(yt, tid);
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) {
+        if (kPlanes * LB % kGradThreads == 0 || tid + i * kGradThreads < kPlanes * LB) sc[tid + i * kGradThreads] = pr[i];
+      }
       StateLoad<M, NP> sr, gr;
       sr.load(f.states + sat, pw, f.N, tid);
       __syncthreads();
@@ -373,51 +382,48 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       f32x4 dx[PW];
 #pragma unroll
       for (int p = 0; p < PW; ++p) dx[p] = f32x4{0.f, 0.f, 0.f, 0.f};
-      Frag8<M> xf[2], yf[2];
+      Frag8<M> xf[2], yf[2], kf[NK];
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         xf[k] = row_frag_t<XT, M>(xt, tile * 16, k * 32, lane);
         yf[k] = row_frag_t<XT, M>(yt, tile * 16, k * 32, lane);
       }
-      const float hj = sc[HI + tok], lj = sc[LO + tok], dj = sc[DD + tok];
-      float colsum = 0.f, w_diag = 0.f;
 #pragma unroll
-      for (int dp = 0; dp < TOK; dp += 2) {
-        if (tile + dp >= TOK) continue;
+      for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<KT, M>(kt, tile * 16, kk * 32, lane);
+      const float hj = sc[HI * LB + tok], lj = sc[LO * LB + tok], dj = sc[DD * LB + tok];
+      float colsum = 0.f, w_diag = 0.f;
+#pragma unroll 1
+      for (int dp = 0; dp < TOK - tile; dp += 2) {
         // The second tile past the block is the first again, with weights of zero.
         const int i0 = tile + dp, i1 = i0 + 1 < TOK ? i0 + 1 : i0;
-        f32x4 ek[2], ew[2], w[2];
+        f32x4 ek[2], ew[2], w[2], k2[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          w[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+          w[u] = k2[u] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int k = 0; k < 2; ++k) w[u] = mfma8(row_frag_t<XT, M>(yt, (u ? i1 : i0) * 16, k * 32, lane), xf[k], w[u]);
+#pragma unroll
+          for (int kk = 0; kk < NK; ++kk) k2[u] = mfma8(row_frag<KT, M>(qt, (u ? i1 : i0) * 16, kk * 32, lane), kf[kk], k2[u]);
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int it = u ? i1 : i0, ti = it * 16 + 4 * g;
-          if (dp + u == 0) {  // the tile on the diagonal
-            const f32x4 hv = *reinterpret_cast<const f32x4*>(sc + HI + ti), lv = *reinterpret_cast<const f32x4*>(sc + LO + ti);
+          // On the diagonal pair by pair; else e^{c_i - c_j} through the end of the tile before i's: one
+          // exponential a lane, one product a pair.
+          const bool own = it == tile, on = u == 0 || i1 != i0;
+          const f32x4 hv = *reinterpret_cast<const f32x4*>(sc + HI * LB + ti), lv = *reinterpret_cast<const f32x4*>(sc + LO * LB + ti),
+                      rv = *reinterpret_cast<const f32x4*>(sc + RB * LB + ti);
+          const int before = it > 0 ? it * 16 - 1 : 0;
+          const float c = on ? exp2_f((sc[HI * LB + before] - hj) + (sc[LO * LB + before] - lj)) : 0.f;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const bool in = ti + r >= tok;
-              const float e = exp2_f(in ? (hv[r] - hj) + (lv[r] - lj) : -INFINITY), wr = in ? w[u][r] : 0.f;
-              ek[u][r] = e * (in ? score[0][r] : 0.f);
-              ew[u][r] = e * dj * wr;
-              colsum = fmaf(ek[u][r], wr, colsum);
-              w_diag += ti + r == tok ? wr : 0.f;
-            }
-          } else {
-            // e^{c_i - c_j} through the end of the tile before i's: one exponential a lane, one product a pair.
-            const f32x4 rv = *reinterpret_cast<const f32x4*>(sc + RB + ti);
-            const bool on = u == 0 || i1 != i0;
-            const float c = on ? exp2_f((sc[HI + it * 16 - 1] - hj) + (sc[LO + it * 16 - 1] - lj)) : 0.f, cd = c * dj;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              ek[u][r] = rv[r] * c * score[dp + u][r];
-              ew[u][r] = rv[r] * cd * w[u][r];
-              colsum = fmaf(ek[u][r], w[u][r], colsum);
-            }
+          for (int r = 0; r < 4; ++r) {
+            const bool in = on && ti + r >= tok;
+            const float e = own ? exp2_f(in ? (hv[r] - hj) + (lv[r] - lj) : -INFINITY) : rv[r] * c;
+            const float wr = in ? w[u][r] : 0.f;
+            ek[u][r] = in ? e * k2[u][r] : 0.f;
+            ew[u][r] = in ? e * dj * wr : 0.f;
+            colsum = fmaf(ek[u][r], wr, colsum);
+            w_diag += ti + r == tok ? wr : 0.f;
           }
         }
         const Frag8<M> ekf = pair_frag<M>(ek[0], ek[1]), ewf = pair_frag<M>(ew[0], ew[1]);
@@ -426,15 +432,10 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
           dk[nt] = mfma8(col_frag2<KT, M>(qt, i0 * 16, i1 * 16, (cs * NT + nt) * 16, lane), ewf, dk[nt]);
-        hold_order();
       }
-      colsum = group_sum(colsum);
-      w_diag = group_sum(row_sum(w_diag));
-      if (cs == 0 && g == 0) sc[COL + tok] = colsum;
-      if (lane == 0) sc[WJ + wave] = cs == 0 ? w_diag : 0.f;
 
       // Rows i of this wave's tile: dq from the columns j <= i, and the rows' sums.
-      const float e_i = sc[EC + tok];
+      const float e_i = sc[EC * LB + tok];
       float rowsum = 0.f;
       Frag8<M> qf[NK];
 #pragma unroll
@@ -455,16 +456,16 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
         for (int u = 0; u < 2; ++u) {
           const int jt = u ? j1 : j0, tj = jt * 16 + 4 * g;
           // On the diagonal pair by pair; else through the end of j's tile, one exponential a lane.
-          const f32x4 hv = *reinterpret_cast<const f32x4*>(sc + HI + tj), lv = *reinterpret_cast<const f32x4*>(sc + LO + tj),
-                      dv = *reinterpret_cast<const f32x4*>(sc + (jt == tile ? DD : TD) + tj);
-          const bool on = u == 0 || j0 > 0;
-          const float c = on ? exp2_f((hj - sc[HI + jt * 16 + 15]) + (lj - sc[LO + jt * 16 + 15])) : 0.f;
+          const bool own = jt == tile, on = u == 0 || j0 > 0;
+          const f32x4 hv = *reinterpret_cast<const f32x4*>(sc + HI * LB + tj), lv = *reinterpret_cast<const f32x4*>(sc + LO * LB + tj),
+                      dv = *reinterpret_cast<const f32x4*>(sc + (own ? DD : TD) * LB + tj);
+          const float c = on ? exp2_f((hj - sc[HI * LB + jt * 16 + 15]) + (lj - sc[LO * LB + jt * 16 + 15])) : 0.f;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const bool in = tj + r <= tok;
-            const float e = jt == tile ? exp2_f(in ? (hj - hv[r]) + (lj - lv[r]) : -INFINITY) : c;
-            ew[u][r] = on && in ? e * dv[r] * w[u][r] : 0.f;
-            rowsum += on && in ? ew[u][r] * k2[u][r] : 0.f;
+            const bool in = on && tj + r <= tok;
+            const float e = own ? exp2_f(in ? (hj - hv[r]) + (lj - lv[r]) : -INFINITY) : c;
+            ew[u][r] = in ? e * dv[r] * w[u][r] : 0.f;
+            rowsum = fmaf(ew[u][r], in ? k2[u][r] : 0.f, rowsum);
           }
         }
         const Frag8<M> ewf = pair_frag<M>(ew[0], ew[1]);
@@ -472,23 +473,11 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
         for (int nt = 0; nt < NT; ++nt)
           dq[nt] = mfma8(col_frag2<KT, M>(kt, j0 * 16, j1 * 16, (cs * NT + nt) * 16, lane), ewf, dq[nt]);
       }
-      rowsum = group_sum(rowsum);
-      if (cs == 0 && g == 0) sc[ROW + tok] = rowsum;
-      // The step wave has waited least so far: the head before ends here, and the next one begins.
-      if (wave == kStepWave) {
-        if (hp > h_lo) end_head(hp - 1, old);
-        old = now;
-        if (hp + 1 < h_hi) {
-          begin_head(hp + 1, now);
-          if (hp + 2 < h_hi) ask_steps(hp + 2);
-        }
-      }
       sr.store(st, tid);
       gr.load(a.adj + sat, pw, f.N, tid);
       __syncthreads();
 
       // From the state: dq.
-      if (hp + 1 < h_hi) ask_rows(hp + 1);
       float dot1 = 0.f;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -506,8 +495,6 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
         }
         if (nt & 1) hold_order();
       }
-      dot1 = group_sum(dot1);
-      if (g == 0) sc[T1 + cs * LB + tok] = e_i * dot1;
       float dot = 0.f;
 #pragma unroll
       for (int i = 0; i < StateLoad<M, NP>::PER; ++i) {
@@ -515,13 +502,15 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
         for (int e = 0; e < 4; ++e) dot = fmaf(gr.r[i][e], sr.r[i][e], dot);
       }
       dot = group_sum(row_sum(dot));
-      if (lane == 0) sc[GS + wave] = dot;
       __syncthreads();
       gr.store(st, tid);
+      const bool wrap = pt + 1 == f.PT;
+      const int hn = h + (wrap ? 1 : 0), pn = wrap ? 0 : pt + 1;
+      if (hp + 1 < h_hi) ask_rows(hn, pn);
       __syncthreads();
 
       // From the adjoint: dk and dx.
-      const float e_t = sc[EE + tok];
+      const float e_t = sc[EE * LB + tok];
       float dot2 = 0.f;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -539,11 +528,8 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
         }
         if (nt & 1) hold_order();
       }
-      dot2 = group_sum(dot2);
-      if (g == 0) sc[T2 + cs * LB + tok] = e_t * dot2;
       {
         eraw* dxp = static_cast<eraw*>(a.dx) + ((row_b + tok) * f.H + h) * f.P + p0;
-        Frag8<M> kf[NK];
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<KT, M>(kt, tile * 16, kk * 32, lane);
 #pragma unroll
@@ -559,9 +545,21 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
           if (tok < in_block) store_row4<E>(dxp + c, pw - c, pvec, o);
         }
       }
+      // What the step sizes' gradients want of this wave's tokens.
+      const float s1 = e_i * group_sum(dot1), s2 = e_t * group_sum(dot2);
+      const float cols = cs == 0 ? group_sum(colsum) : 0.f, rws = cs == 0 ? group_sum(rowsum) : 0.f;
+      if (g == 0)
+        *reinterpret_cast<float2*>(a.diffs + ((pair * CS + cs) * LB + tok) * 2) =
+            make_float2((rws - dj * cols) + (s1 - dj * s2), cols + s2);
+      const float tail = row_sum(dj * s2), wsum = group_sum(row_sum(w_diag));
+      if (lane == 0) {
+        *reinterpret_cast<float2*>(a.dots + (pair * 8 + wave) * 2) = make_float2(dot, cs == 0 ? wsum : 0.f);
+        a.dots[static_cast<int64_t>(f.B) * f.nsave * f.H * f.PT * 16 + pair * 8 + wave] = tail;
+      }
       __syncthreads();
+      h = hn;
+      pt = pn;
     }
-    if (wave == kStepWave) end_head(h_hi - 1, old);
   }
 
   // dk and dq of this workgroup's heads.
@@ -586,26 +584,28 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
   }
 }
 
-// out[i] = sum of `parts` rows of n floats, in order.
+// The first blocks: dk and dq as the sums of their shares, in order (n elements each, `parts` shares of both).  The
+// last H blocks: dA, dD and the step bias's gradient of a head, its blocks' sums in a fixed order.
 template <class E>
-__global__ __launch_bounds__(256) void selective_sum_kernel(const float* part, int64_t stride, int parts, void* out, int64_t n,
-                                                            int out_f32) {
-  const int64_t step = static_cast<int64_t>(gridDim.x) * 256;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += step) {
-    float s = part[i];
-    for (int p = 1; p < parts; ++p) s += part[p * stride + i];
-    st_state<E>(out, i, out_f32 != 0, s);
+__global__ __launch_bounds__(256) void selective_sum_kernel(const float* part, int parts, void* dk, void* dq, int64_t n,
+                                                            const float* heads, int64_t blocks, int H, float* da, float* dskip,
+                                                            float* dbias) {
+  const int tid = static_cast<int>(threadIdx.x), row_blocks = static_cast<int>(gridDim.x) - H;
+  if (static_cast<int>(blockIdx.x) < row_blocks) {
+    const int64_t step = static_cast<int64_t>(row_blocks) * 256;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + tid; i < 2 * n; i += step) {
+      float s = part[i];
+      for (int p = 1; p < parts; ++p) s += part[p * 2 * n + i];
+      if (i < n) st_state<E>(dk, i, false, s);
+      else st_state<E>(dq, i - n, false, s);
+    }
+    return;
   }
-}
-
-// dA, dD and the step bias's gradient of a head: the blocks' sums, in a fixed order.
-__global__ __launch_bounds__(256) void selective_head_kernel(const float* part, int64_t blocks, int H, int PT, float* da,
-                                                             float* dskip, float* dbias) {
   __shared__ float sums[3][4];
-  const int h = static_cast<int>(blockIdx.x), tid = static_cast<int>(threadIdx.x);
+  const int h = static_cast<int>(blockIdx.x) - row_blocks;
   float s[3] = {0.f, 0.f, 0.f};
-  for (int64_t i = tid; i < blocks * PT; i += 256) {
-    const float* p = part + ((i / PT) * H * PT + static_cast<int64_t>(h) * PT + i % PT) * 3;
+  for (int64_t i = tid; i < blocks; i += 256) {
+    const float* p = heads + (i * H + h) * 3;
 #pragma unroll
     for (int k = 0; k < 3; ++k) s[k] += p[k];
   }
@@ -626,34 +626,37 @@ __global__ __launch_bounds__(256) void selective_head_kernel(const float* part, 
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// Workspace: the adjoint behind every block, its walk's parts, and the shares' sums.
+// Workspace: the adjoint behind every block, its walk's parts, the tokens' numbers and the shares' sums.
 struct BwdPlan {
   int64_t nsave, part_tokens, wgs;
   int parts, splits, PT;
-  int64_t adj, part_state, part_log, rows, steps, heads, bytes;  // byte offsets
+  int64_t adj, part_state, part_log, tokens, diffs, dots, rows, heads, bytes;  // byte offsets
 };
 
 BwdPlan bwd_plan(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G, int64_t N, int dtype) {
   BwdPlan p{};
   auto up = [](int64_t n) { return sel_ceil(n, 256) * 256; };
+  const int64_t LB = sel_block(dtype), CS = 128 / LB;
   p.PT = static_cast<int>(sel_ceil(P, kSelRows));
-  p.nsave = sel_ceil(T, sel_block(dtype));
+  p.nsave = sel_ceil(T, LB);
   p.parts = sel_parts(B * H * p.PT, T, dtype, &p.part_tokens);
-  // A workgroup for each of 256 CUs; the heads of a group are shared no further, since every share adds
-  // its own K and a float32 copy of dk and dq.
+  // A workgroup for each of 256 CUs; the heads of a group are shared no further, since every share reads
+  // the keys and queries and writes a float32 copy of dk and dq.
   p.wgs = B * p.nsave * G;
   const int64_t heads = H / G * p.PT;
   int64_t splits = p.wgs > 0 ? sel_ceil(256, p.wgs) : 1;
   if (splits > heads) splits = heads;
   p.splits = static_cast<int>(splits);
-  const int64_t state = H * P * N * 4;
+  const int64_t state = H * P * N * 4, pairs = B * p.nsave * H * p.PT;
   int64_t at = 0;
   p.adj = at; at += up(B * p.nsave * state);
   p.part_state = at; at += p.parts > 1 ? up(p.parts * B * state) : 0;
   p.part_log = at; at += p.parts > 1 ? up(p.parts * B * H * 8) : 0;
+  p.tokens = at; at += up(B * p.nsave * H * kPlanes * LB * 4);
+  p.diffs = at; at += up(pairs * CS * LB * 8);
+  p.dots = at; at += up(pairs * 24 * 4);
   p.rows = at; at += p.splits > 1 ? up(p.splits * 2 * B * T * G * N * 4) : 0;
-  p.steps = at; at += p.PT > 1 ? up(p.PT * B * T * H * 4) : 0;
-  p.heads = at; at += up(B * p.nsave * H * p.PT * 12);
+  p.heads = at; at += up(B * p.nsave * H * 12);
   p.bytes = at;
   return p;
 }
@@ -723,47 +726,45 @@ extern "C" int grm_hip_selective_scan_bwd(const grm_hip_selective_args* u, const
     a.s.vec = a.s.vec && aligned(grad_hidden) && aligned(grad_keys) && aligned(grad_values) && aligned(grad_queries);
     a.dy = grad_hidden; a.adj = reinterpret_cast<const float*>(ws + p.adj);
     a.dx = grad_values; a.dk = grad_keys; a.dq = grad_queries; a.dsteps = grad_steps;
+    a.tokens = reinterpret_cast<float*>(ws + p.tokens);
+    a.diffs = reinterpret_cast<float*>(ws + p.diffs);
+    a.dots = reinterpret_cast<float*>(ws + p.dots);
     a.rows_part = p.splits > 1 ? reinterpret_cast<float*>(ws + p.rows) : nullptr;
-    a.steps_part = p.PT > 1 ? reinterpret_cast<float*>(ws + p.steps) : nullptr;
     a.head_part = reinterpret_cast<float*>(ws + p.heads);
     a.splits = p.splits;
+    const dim3 waves(static_cast<uint32_t>(sel_ceil(u->batch * p.nsave * u->heads, 4)));
     sel_with_form(u->dtype, u->key_dim, a.s.vec != 0, [&](auto e, auto m, auto np, auto vec) {
       using E = decltype(e);
       using M = decltype(m);
       constexpr int NP = decltype(np)::value;
+      using Lds = GradLds<M, NP>;
       auto kernel = selective_grad_kernel<E, M, NP, decltype(vec)::value>;
-      constexpr size_t lds = GradLds<M, NP>::bytes;
       const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Lds::bytes));
       if (err != hipSuccess) {
         set_error("%s: %s", what, hipGetErrorString(err));
         rc = static_cast<int>(err);
         return;
       }
-      kernel<<<dim3(static_cast<uint32_t>(p.wgs * p.splits)), dim3(kGradThreads), lds, s>>>(a);
+      selective_token_kernel<E, Lds::LB><<<waves, dim3(256), 0, s>>>(a);
       if ((rc = check_launch(what)) != GRM_HIP_OK) return;
-      auto sum = [&](const float* part, int64_t stride, int parts, void* out, int64_t n, int f32) {
-        const int64_t blocks = sel_ceil(n, 256);
-        selective_sum_kernel<E><<<dim3(static_cast<uint32_t>(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s>>>(
-            part, stride, parts, out, n, f32);
-        rc = check_launch(what);
-      };
-      if (a.rows_part != nullptr) {
-        const int64_t n = u->batch * u->seq_len * u->groups * u->key_dim;
-        sum(a.rows_part, 2 * n, p.splits, grad_keys, n, 0);
-        if (rc != GRM_HIP_OK) return;
-        sum(a.rows_part + n, 2 * n, p.splits, grad_queries, n, 0);
-        if (rc != GRM_HIP_OK) return;
-      }
-      if (a.steps_part != nullptr) {
-        const int64_t n = u->batch * u->seq_len * u->heads;
-        sum(a.steps_part, n, p.PT, grad_steps, n, u->steps_dtype == GRM_HIP_F32);
-      }
+      kernel<<<dim3(static_cast<uint32_t>(p.wgs * p.splits)), dim3(kGradThreads), Lds::bytes, s>>>(a);
+      if ((rc = check_launch(what)) != GRM_HIP_OK) return;
+      selective_steps_kernel<E, Lds::LB, Lds::CS><<<waves, dim3(256), 0, s>>>(a);
+      rc = check_launch(what);
     });
     if (rc != GRM_HIP_OK) return rc;
   }
-  selective_head_kernel<<<dim3(static_cast<uint32_t>(u->heads)), dim3(256), 0, s>>>(
-      reinterpret_cast<const float*>(ws + p.heads), u->batch * p.nsave, static_cast<int>(u->heads), p.PT, grad_rates, grad_skip,
-      grad_step_bias);
+  const int64_t n = p.splits > 1 ? u->batch * u->seq_len * u->groups * u->key_dim : 0, blocks = sel_ceil(2 * n, 256);
+  const dim3 grid(static_cast<uint32_t>((blocks < 4096 ? blocks : 4096) + u->heads));
+  auto sum = [&](auto e) {
+    selective_sum_kernel<decltype(e)><<<grid, dim3(256), 0, s>>>(
+        reinterpret_cast<const float*>(ws + p.rows), p.splits, grad_keys, grad_queries, n,
+        reinterpret_cast<const float*>(ws + p.heads), u->batch * p.nsave, static_cast<int>(u->heads), grad_rates, grad_skip,
+        grad_step_bias);
+  };
+  if (u->dtype == GRM_HIP_F32) sum(F32{});
+  else if (u->dtype == GRM_HIP_F16) sum(F16{});
+  else sum(BF16{});
   return check_launch(what);
 }
