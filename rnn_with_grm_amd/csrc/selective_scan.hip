@@ -24,7 +24,7 @@ namespace grmhip {
 namespace {
 
 constexpr int kWalkThreads = 512;
-constexpr int kPassThreads = 256;
+constexpr int kPassThreads = 512;
 constexpr int kMaxParts = 32;
 
 template <class M, int NP>
@@ -335,8 +335,10 @@ __global__ __launch_bounds__(kWalkThreads) __attribute__((amdgpu_waves_per_eu(2,
 // (the backward's adjoint): `keys` are the queries and `values` the output's gradient,
 //   G_{before} = e^{c_L} G + sum_i e^{c_i} dy_i q_i^T,
 // from the gradient of the final state back to the first, G kept at the end of every backward chunk.
+// Waves 0-3 bring the chunks, one in LDS and one on its way; waves 4-7 hold 16 rows of the state each.  (One
+// role for all waves measured 120 us where this takes LATER: a state's stores then stand between a load and its use.)
 template <class E, class M, int NP, bool VEC, bool REV, bool LOCAL>
-__global__ __launch_bounds__(kPassThreads) __attribute__((amdgpu_waves_per_eu(1, 2))) void selective_pass_kernel(SelArgs a) {
+__global__ __launch_bounds__(kPassThreads) __attribute__((amdgpu_waves_per_eu(2, 4))) void selective_pass_kernel(SelArgs a) {
   using S = SelShape<M>;
   using raw = typename ET<M>::raw;
   using eraw = typename ET<E>::raw;
@@ -352,93 +354,90 @@ __global__ __launch_bounds__(kPassThreads) __attribute__((amdgpu_waves_per_eu(1,
   if (LOCAL && w.part == (REV ? 0 : a.parts - 1)) return;
   const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int p0 = w.pt * kSelRows, pw = a.P - p0, sp = p0 + 16 * wave;
-  const int64_t len = sel_length(a, w.b);
+  const int p0 = w.pt * kSelRows, pw = a.P - p0;
   const int64_t t_first = w.part * a.part_tokens, t_last = min_i64(t_first + a.part_tokens, a.T);
-  const int chunks = static_cast<int>((max_i64(0, min_i64(len, t_last) - t_first) + L - 1) / L);
-  const float rate = a.rates[w.h], bias = a.bias == nullptr ? 0.f : a.bias[w.h];
-  auto chunk_of = [&](int i) { return REV ? chunks - 1 - i : i; };
-
-  TileLoad<E, KT, M, VEC, L, NP, kPassThreads> kr;
-  TileLoad<E, XT, M, VEC, L, kSelRows, kPassThreads> xr;
-  kr.init(a.kt, a.N, tid);
-  xr.init(a.vt, pw < kSelRows ? pw : kSelRows, tid);
-  const eraw* kp = static_cast<const eraw*>(a.keys) + w.b * a.kb + w.g * a.N;
-  const eraw* xp = static_cast<const eraw*>(a.values) + w.b * a.vb + w.h * a.P + p0;
-  auto load = [&](int i) {
-    const int64_t t = t_first + static_cast<int64_t>(chunk_of(i)) * L, rows = len - t;
-    kr.load(kp + t * a.kt, rows, tid);
-    xr.load(xp + t * a.vt, rows, tid);
-  };
-  double log = 0.0;
-  uint32_t z = 0;  // wave 0: the next chunk's steps
-  auto ask_step = [&](int i) {
-    const int64_t t = t_first + static_cast<int64_t>(chunk_of(i)) * L + lane;
-    z = load_step<E>(a, w.b, t, w.h, lane < L && t < len);
-  };
-  auto put = [&](int i) {
-    raw* s = stage + (i & 1) * STAGE;
-    kr.store(s, tid);
-    xr.store(s + X0, tid);
-    if (wave == 0) {
-      const TokenScalars t =
-          token_scalars<L>(a, step_value<E>(a, z) + bias, t_first + static_cast<int64_t>(chunk_of(i)) * L + lane < len, rate);
-      float* o = scal + (i & 1) * SCAL;
-      if (lane < L)
-        o[lane] = REV ? exp2_d(t.cum) : t.d * exp2_d(t.total - t.cum);
-      if (lane == 0) o[L] = exp2_d(t.total);
-      log += t.total;
-    }
-  };
-  f32x4 acc[NT];
-#pragma unroll
-  for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  if (chunks > 0) {
-    load(0);
-    if (wave == 0) ask_step(0);
-  }
-  if (!LOCAL) part_start<NT, REV>(acc, a, w, sp);
-  if (chunks > 0) put(0);
-  __syncthreads();
-  for (int i = 0; i < chunks; ++i) {
-    if (i + 1 < chunks) {
-      load(i + 1);
-      if (wave == 0) ask_step(i + 1);
-    }
-    const raw* ks = stage + (i & 1) * STAGE;
-    const float* sc = scal + (i & 1) * SCAL;
-    if (REV && !LOCAL) {
-      const int64_t t = t_first + static_cast<int64_t>(chunk_of(i)) * L;
-      if (i == 0 || (t + L) % S::LB == 0)
-        state_store<NT>(acc, a.states + ((w.b * a.nsave + t / S::LB) * a.H + w.h) * a.P * a.N, sp, a.P, a.N);
-    }
-    Frag8<M> xf[L / 32];
-#pragma unroll
-    for (int s = 0; s < L / 32; ++s) xf[s] = col_frag<XT, M>(ks + X0, 32 * s, 16 * wave);
-    const float decay = sc[L];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) acc[nt][r] *= decay;
-    }
-#pragma unroll
-    for (int s = 0; s < L / 32; ++s) {
-      Frag8<M> kf[NT], part[S::PARTS];
-      key_frags<KT, M, NT>(kf, ks, 32 * s);
-      weigh_frag<M>(xf[s], *reinterpret_cast<const f32x4*>(sc + 32 * s + 4 * (lane >> 4)),
-                    *reinterpret_cast<const f32x4*>(sc + 32 * s + 16 + 4 * (lane >> 4)), part);
-      update_step<M, NT>(acc, kf, part);
-    }
-    if (i + 1 < chunks) put(i + 1);
-    __syncthreads();
-  }
+  const int live = static_cast<int>(max_i64(0, min_i64(sel_length(a, w.b), t_last) - t_first));
+  const int chunks = (live + L - 1) / L;
   const int64_t head = static_cast<int64_t>(w.b) * a.H + w.h, one = static_cast<int64_t>(a.P) * a.N;
-  if (LOCAL) {
-    const int64_t slot = static_cast<int64_t>(w.part) * a.B * a.H + head;
-    state_store<NT>(acc, a.part_state + slot * one, sp, a.P, a.N);
-    if (tid == 0 && w.pt == 0) a.part_log[slot] = log;
-  } else if (w.part == 0) {
-    state_store<NT>(acc, a.memory_out + head * one, sp, a.P, a.N);
+  const int64_t slot = static_cast<int64_t>(w.part) * a.B * a.H + head;
+  auto chunk_of = [&](int i) { return REV ? chunks - 1 - i : i; };
+  if (wave < 4) {
+    constexpr int kStepWave = 3;
+    const float rate = a.rates[w.h], bias = a.bias == nullptr ? 0.f : a.bias[w.h];
+    TileLoad<E, KT, M, VEC, L, NP, kPassThreads / 2> kr;
+    TileLoad<E, XT, M, VEC, L, kSelRows, kPassThreads / 2> xr;
+    kr.init(a.kt, a.N, tid);
+    xr.init(a.vt, pw < kSelRows ? pw : kSelRows, tid);
+    const eraw* kp = static_cast<const eraw*>(a.keys) + w.b * a.kb + t_first * a.kt + w.g * a.N;
+    const eraw* xp = static_cast<const eraw*>(a.values) + w.b * a.vb + t_first * a.vt + w.h * a.P + p0;
+    uint32_t z = 0;  // the chunk's steps
+    double log = 0.0;
+    auto load = [&](int i) {
+      const int t = chunk_of(i) * L;
+      kr.load(kp + t * a.kt, live - t, tid);
+      xr.load(xp + t * a.vt, live - t, tid);
+      if (wave == kStepWave) z = load_step<E>(a, w.b, t_first + t + lane, w.h, lane < L && t + lane < live);
+    };
+    auto put = [&](int i) {
+      raw* s = stage + (i & 1) * STAGE;
+      kr.store(s, tid);
+      xr.store(s + X0, tid);
+      if (wave == kStepWave) {
+        const TokenScalars t = token_scalars<L>(a, step_value<E>(a, z) + bias, chunk_of(i) * L + lane < live, rate);
+        float* o = scal + (i & 1) * SCAL;
+        if (lane < L) o[lane] = REV ? exp2_d(t.cum) : t.d * exp2_d(t.total - t.cum);
+        if (lane == 0) o[L] = exp2_d(t.total);
+        log += t.total;
+      }
+    };
+    if (chunks > 0) {
+      load(0);
+      put(0);
+      if (chunks > 1) load(1);
+    }
+    __syncthreads();
+    for (int i = 0; i < chunks; ++i) {
+      if (i + 1 < chunks) put(i + 1);
+      if (i + 2 < chunks) load(i + 2);
+      __syncthreads();
+    }
+    if (LOCAL && wave == kStepWave && lane == 0 && w.pt == 0) a.part_log[slot] = log;
+  } else {
+    const int rw = 16 * (wave & 3), sp = p0 + rw, g = lane >> 4;
+    f32x4 acc[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (!LOCAL) part_start<NT, REV>(acc, a, w, sp);
+    __syncthreads();
+    for (int i = 0; i < chunks; ++i) {
+      const raw* ks = stage + (i & 1) * STAGE;
+      const float* sc = scal + (i & 1) * SCAL;
+      Frag8<M> xf[L / 32], kf[NT], part[S::PARTS];
+#pragma unroll
+      for (int s = 0; s < L / 32; ++s) xf[s] = col_frag<XT, M>(ks + X0, 32 * s, rw);
+      key_frags<KT, M, NT>(kf, ks, 0);
+      if (REV && !LOCAL) {
+        const int64_t t = t_first + static_cast<int64_t>(chunk_of(i)) * L;
+        if (i == 0 || (t + L) % S::LB == 0)
+          state_store<NT>(acc, a.states + ((w.b * a.nsave + t / S::LB) * a.H + w.h) * a.P * a.N, sp, a.P, a.N);
+      }
+      const float decay = sc[L];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[nt][r] *= decay;
+      }
+#pragma unroll
+      for (int s = 0; s < L / 32; ++s) {
+        weigh_frag<M>(xf[s], *reinterpret_cast<const f32x4*>(sc + 32 * s + 4 * g),
+                      *reinterpret_cast<const f32x4*>(sc + 32 * s + 16 + 4 * g), part);
+        update_step<M, NT>(acc, kf, part);
+        if (s + 1 < L / 32) key_frags<KT, M, NT>(kf, ks, 32 * (s + 1));
+      }
+      __syncthreads();
+    }
+    if (LOCAL) state_store<NT>(acc, a.part_state + slot * one, sp, a.P, a.N);
+    else if (w.part == 0) state_store<NT>(acc, a.memory_out + head * one, sp, a.P, a.N);
   }
 }
 
