@@ -337,7 +337,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
   } else {
     TileLoad<E, XT, M, VEC, LB, kSelRows, kGradThreads> xr, yr;
     float pr[NPL];
-    auto ask_rows = [&](int hn, int pn) {
+    auto ask_rows = [&](int hn, int pn, int tid) {
       const int p0 = pn * kSelRows, cols = f.P - p0 < kSelRows ? f.P - p0 : kSelRows;
       xr.init(f.vt, cols, tid);
       xr.load(static_cast<const eraw*>(f.values) + b * f.vb + t0 * f.vt + hn * f.P + p0, live, tid);
@@ -347,7 +347,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
       for (int i = 0; i < NPL; ++i) pr[i] = buf_load1<F32>(rsrc, (tid + i * kGradThreads) * 4);
     };
-    ask_rows(h, pt);
+    ask_rows(h, pt, tid);
     {
       TileLoad<E, KT, M, VEC, LB, NP, kGradThreads> r;
       r.init(f.kt, f.N, tid);
@@ -363,11 +363,13 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       // registers from head to head.
       int lane = lane_id();
       asm volatile("" : "+v"(lane));
+      const int tid = wave * 64 + lane;
       const int g = lane >> 4, n16 = lane & 15, tok = tile * 16 + n16;  // this lane's token in both orders
       const int p0 = pt * kSelRows, pw = f.P - p0;
       const float skip = f.skip == nullptr ? 0.f : f.skip[h];
       const int64_t sat = ((blocks * f.H + h) * f.P + p0) * f.N;
       const int64_t pair = (blocks * f.H + h) * f.PT + pt;
+      xr.at = yr.at = XT::at(tid / (kSelRows / 8), tid % (kSelRows / 8) * 8);
       xr.store(xt, tid);
       yr.store(yt, tid);
 #pragma unroll
@@ -392,8 +394,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<KT, M>(kt, tile * 16, kk * 32, lane);
       const float hj = sc[HI * LB + tok], lj = sc[LO * LB + tok], dj = sc[DD * LB + tok];
       float colsum = 0.f, w_diag = 0.f;
-#pragma unroll 1
-      for (int dp = 0; dp < TOK - tile; dp += 2) {
+      auto columns = [&](int dp, auto diag) {
         // The second tile past the block is the first again, with weights of zero.
         const int i0 = tile + dp, i1 = i0 + 1 < TOK ? i0 + 1 : i0;
         f32x4 ek[2], ew[2], w[2], k2[2];
@@ -408,22 +409,28 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int it = u ? i1 : i0, ti = it * 16 + 4 * g;
-          // On the diagonal pair by pair; else e^{c_i - c_j} through the end of the tile before i's: one
-          // exponential a lane, one product a pair.
-          const bool own = it == tile, on = u == 0 || i1 != i0;
-          const f32x4 hv = *reinterpret_cast<const f32x4*>(sc + HI * LB + ti), lv = *reinterpret_cast<const f32x4*>(sc + LO * LB + ti),
-                      rv = *reinterpret_cast<const f32x4*>(sc + RB * LB + ti);
-          const int before = it > 0 ? it * 16 - 1 : 0;
-          const float c = on ? exp2_f((sc[HI * LB + before] - hj) + (sc[LO * LB + before] - lj)) : 0.f;
+          if (decltype(diag)::value && u == 0) {  // on the diagonal, pair by pair
+            const f32x4 hv = *reinterpret_cast<const f32x4*>(sc + HI * LB + ti), lv = *reinterpret_cast<const f32x4*>(sc + LO * LB + ti);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const bool in = on && ti + r >= tok;
-            const float e = own ? exp2_f(in ? (hv[r] - hj) + (lv[r] - lj) : -INFINITY) : rv[r] * c;
-            const float wr = in ? w[u][r] : 0.f;
-            ek[u][r] = in ? e * k2[u][r] : 0.f;
-            ew[u][r] = in ? e * dj * wr : 0.f;
-            colsum = fmaf(ek[u][r], wr, colsum);
-            w_diag += ti + r == tok ? wr : 0.f;
+            for (int r = 0; r < 4; ++r) {
+              const bool in = ti + r >= tok;
+              const float e = exp2_f(in ? (hv[r] - hj) + (lv[r] - lj) : -INFINITY), wr = in ? w[u][r] : 0.f;
+              ek[u][r] = e * (in ? k2[u][r] : 0.f);
+              ew[u][r] = e * dj * wr;
+              colsum = fmaf(ek[u][r], wr, colsum);
+              w_diag += ti + r == tok ? wr : 0.f;
+            }
+          } else {  // e^{c_i - c_j} through the end of the tile before i's: one exponential a lane, one product a pair
+            const bool on = u == 0 || i1 != i0;
+            const f32x4 rv = *reinterpret_cast<const f32x4*>(sc + RB * LB + ti);
+            const int before = on ? it * 16 - 1 : 0;
+            const float c = on ? exp2_f((sc[HI * LB + before] - hj) + (sc[LO * LB + before] - lj)) : 0.f, cd = c * dj;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              ek[u][r] = rv[r] * c * k2[u][r];
+              ew[u][r] = rv[r] * cd * w[u][r];
+              colsum = fmaf(ek[u][r], w[u][r], colsum);
+            }
           }
         }
         const Frag8<M> ekf = pair_frag<M>(ek[0], ek[1]), ewf = pair_frag<M>(ew[0], ew[1]);
@@ -432,7 +439,10 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
           dk[nt] = mfma8(col_frag2<KT, M>(qt, i0 * 16, i1 * 16, (cs * NT + nt) * 16, lane), ewf, dk[nt]);
-      }
+      };
+      columns(0, std::true_type{});
+#pragma unroll 1
+      for (int dp = 2; dp < TOK - tile; dp += 2) columns(dp, std::false_type{});
 
       // Rows i of this wave's tile: dq from the columns j <= i, and the rows' sums.
       const float e_i = sc[EC * LB + tok];
@@ -440,8 +450,8 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       Frag8<M> qf[NK];
 #pragma unroll
       for (int kk = 0; kk < NK; ++kk) qf[kk] = row_frag<KT, M>(qt, tile * 16, kk * 32, lane);
-#pragma unroll 1
-      for (int dp = 0; dp <= tile; dp += 2) {
+      gr.load(a.adj + sat, pw, f.N, tid);
+      auto rows = [&](int dp, auto diag) {
         const int j0 = tile - dp, j1 = j0 > 0 ? j0 - 1 : 0;
         f32x4 ew[2], w[2], k2[2];
 #pragma unroll
@@ -455,26 +465,35 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int jt = u ? j1 : j0, tj = jt * 16 + 4 * g;
-          // On the diagonal pair by pair; else through the end of j's tile, one exponential a lane.
-          const bool own = jt == tile, on = u == 0 || j0 > 0;
-          const f32x4 hv = *reinterpret_cast<const f32x4*>(sc + HI * LB + tj), lv = *reinterpret_cast<const f32x4*>(sc + LO * LB + tj),
-                      dv = *reinterpret_cast<const f32x4*>(sc + (own ? DD : TD) * LB + tj);
-          const float c = on ? exp2_f((hj - sc[HI * LB + jt * 16 + 15]) + (lj - sc[LO * LB + jt * 16 + 15])) : 0.f;
+          if (decltype(diag)::value && u == 0) {
+            const f32x4 hv = *reinterpret_cast<const f32x4*>(sc + HI * LB + tj), lv = *reinterpret_cast<const f32x4*>(sc + LO * LB + tj),
+                        dv = *reinterpret_cast<const f32x4*>(sc + DD * LB + tj);
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const bool in = on && tj + r <= tok;
-            const float e = own ? exp2_f(in ? (hj - hv[r]) + (lj - lv[r]) : -INFINITY) : c;
-            ew[u][r] = in ? e * dv[r] * w[u][r] : 0.f;
-            rowsum = fmaf(ew[u][r], in ? k2[u][r] : 0.f, rowsum);
+            for (int r = 0; r < 4; ++r) {
+              const bool in = tj + r <= tok;
+              ew[u][r] = exp2_f(in ? (hj - hv[r]) + (lj - lv[r]) : -INFINITY) * (in ? dv[r] * w[u][r] : 0.f);
+              rowsum = fmaf(ew[u][r], in ? k2[u][r] : 0.f, rowsum);
+            }
+          } else {  // through the end of j's tile
+            const bool on = u == 0 || j0 > 0;
+            const f32x4 dv = *reinterpret_cast<const f32x4*>(sc + TD * LB + tj);
+            const float c = on ? exp2_f((hj - sc[HI * LB + jt * 16 + 15]) + (lj - sc[LO * LB + jt * 16 + 15])) : 0.f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              ew[u][r] = c * dv[r] * w[u][r];
+              rowsum = fmaf(ew[u][r], k2[u][r], rowsum);
+            }
           }
         }
         const Frag8<M> ewf = pair_frag<M>(ew[0], ew[1]);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
           dq[nt] = mfma8(col_frag2<KT, M>(kt, j0 * 16, j1 * 16, (cs * NT + nt) * 16, lane), ewf, dq[nt]);
-      }
+      };
+      rows(0, std::true_type{});
+#pragma unroll 1
+      for (int dp = 2; dp <= tile; dp += 2) rows(dp, std::false_type{});
       sr.store(st, tid);
-      gr.load(a.adj + sat, pw, f.N, tid);
       __syncthreads();
 
       // From the state: dq.
@@ -506,7 +525,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       gr.store(st, tid);
       const bool wrap = pt + 1 == f.PT;
       const int hn = h + (wrap ? 1 : 0), pn = wrap ? 0 : pt + 1;
-      if (hp + 1 < h_hi) ask_rows(hn, pn);
+      if (hp + 1 < h_hi) ask_rows(hn, pn, tid);
       __syncthreads();
 
       // From the adjoint: dk and dx.
@@ -529,7 +548,10 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
         if (nt & 1) hold_order();
       }
       {
-        eraw* dxp = static_cast<eraw*>(a.dx) + ((row_b + tok) * f.H + h) * f.P + p0;
+        // (Buffer stores: with no branch round them the compiler knows how many stand behind the next head's loads.)
+        const int64_t wide = static_cast<int64_t>(f.H) * f.P;
+        const __amdgpu_buffer_rsrc_t dxr = make_rsrc(static_cast<eraw*>(a.dx) + row_b * wide + h * f.P + p0, 0x7fffff00u);
+        const int dx_at = tok * static_cast<int>(wide);
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<KT, M>(kt, tile * 16, kk * 32, lane);
 #pragma unroll
@@ -542,20 +564,21 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
           f32x4 o;
 #pragma unroll
           for (int e = 0; e < 4; ++e) o[e] = tok < live ? fmaf(dj, fmaf(e_t, u[e], dx[p][e]), skip * yv[e]) : 0.f;
-          if (tok < in_block) store_row4<E>(dxp + c, pw - c, pvec, o);
+          out4<E>(dxr, dx_at + c, tok < in_block ? pw - c : 0, pvec, o);
         }
       }
       // What the step sizes' gradients want of this wave's tokens.
       const float s1 = e_i * group_sum(dot1), s2 = e_t * group_sum(dot2);
       const float cols = cs == 0 ? group_sum(colsum) : 0.f, rws = cs == 0 ? group_sum(rowsum) : 0.f;
-      if (g == 0)
-        *reinterpret_cast<float2*>(a.diffs + ((pair * CS + cs) * LB + tok) * 2) =
-            make_float2((rws - dj * cols) + (s1 - dj * s2), cols + s2);
+      const __amdgpu_buffer_rsrc_t dfr = make_rsrc(a.diffs + (pair * CS + cs) * LB * 2, LB * 8);
+      buf_store1<F32>(dfr, g == 0 ? tok * 8 : kBufOOB, (rws - dj * cols) + (s1 - dj * s2));
+      buf_store1<F32>(dfr, g == 0 ? tok * 8 + 4 : kBufOOB, cols + s2);
       const float tail = row_sum(dj * s2), wsum = group_sum(row_sum(w_diag));
-      if (lane == 0) {
-        *reinterpret_cast<float2*>(a.dots + (pair * 8 + wave) * 2) = make_float2(dot, cs == 0 ? wsum : 0.f);
-        a.dots[static_cast<int64_t>(f.B) * f.nsave * f.H * f.PT * 16 + pair * 8 + wave] = tail;
-      }
+      const __amdgpu_buffer_rsrc_t dtr = make_rsrc(a.dots + (pair * 8 + wave) * 2, 8),
+                                   tlr = make_rsrc(a.dots + static_cast<int64_t>(f.B) * f.nsave * f.H * f.PT * 16 + pair * 8 + wave, 4);
+      buf_store1<F32>(dtr, lane == 0 ? 0 : kBufOOB, dot);
+      buf_store1<F32>(dtr, lane == 0 ? 4 : kBufOOB, cs == 0 ? wsum : 0.f);
+      buf_store1<F32>(tlr, lane == 0 ? 0 : kBufOOB, tail);
       __syncthreads();
       h = hn;
       pt = pn;
