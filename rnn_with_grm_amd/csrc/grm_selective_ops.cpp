@@ -165,8 +165,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> short_conv_backward(const OptTensor& 
           dstate.defined() ? dstate : at::empty({0}, x.options())};
 }
 
-Tensor short_conv_step(const Tensor& x, const Tensor& state, const Tensor& weight, const OptTensor& bias, bool silu,
-                       Tensor& state_out) {
+Tensor short_conv_step_out(const Tensor& x, const Tensor& state, const Tensor& weight, const OptTensor& bias, bool silu,
+                           Tensor& state_out) {
   const char* op = "short_conv_step";
   const Conv c = check_conv(x, weight, bias, state, true, op);
   check_device(state_out, x, op, "state_out");
@@ -182,6 +182,12 @@ Tensor short_conv_step(const Tensor& x, const Tensor& state, const Tensor& weigh
                                    silu, stream_of(x)),
            op);
   return out;
+}
+
+std::tuple<Tensor, Tensor> short_conv_step(const Tensor& x, const Tensor& state, const Tensor& weight,
+                                           const OptTensor& bias, bool silu) {
+  Tensor moved = at::empty(state.sizes(), state.options());
+  return {short_conv_step_out(x, state, weight, bias, silu, moved), moved};
 }
 
 // ---------------------------------------------------------------------------
@@ -337,7 +343,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> selec
   return {gk, gv, gq, gst, gr, gm, gsk, gb};
 }
 
-Tensor selective_step(const Tensor& keys, const Tensor& values, const Tensor& queries, const Tensor& steps,
+Tensor selective_step_out(const Tensor& keys, const Tensor& values, const Tensor& queries, const Tensor& steps,
                       const Tensor& rates, const Tensor& memory, const OptTensor& skip, const OptTensor& step_bias,
                       bool softplus, Tensor& memory_out) {
   const char* op = "selective_step";
@@ -352,23 +358,34 @@ Tensor selective_step(const Tensor& keys, const Tensor& values, const Tensor& qu
   return hidden;
 }
 
+std::tuple<Tensor, Tensor> selective_step(const Tensor& keys, const Tensor& values, const Tensor& queries,
+                                          const Tensor& steps, const Tensor& rates, const Tensor& memory,
+                                          const OptTensor& skip, const OptTensor& step_bias, bool softplus) {
+  Tensor moved = at::empty(memory.sizes(), memory.options());
+  return {selective_step_out(keys, values, queries, steps, rates, memory, skip, step_bias, softplus, moved), moved};
+}
+
 }  // namespace
 }  // namespace grm_selective
 
 TORCH_LIBRARY_FRAGMENT(grm_cuda, m) {
   m.def("short_conv_forward(Tensor x, Tensor weight, Tensor? bias, Tensor? state, Tensor? lengths, bool silu) -> (Tensor out, Tensor state_out)");
   m.def("short_conv_backward(Tensor? grad_out, Tensor? grad_state_out, Tensor x, Tensor weight, Tensor? bias, Tensor? state, Tensor? lengths, bool silu) -> (Tensor grad_x, Tensor grad_weight, Tensor grad_bias, Tensor grad_state)");
-  m.def("short_conv_step(Tensor x, Tensor state, Tensor weight, Tensor? bias, bool silu, Tensor(a!) state_out) -> Tensor");
+  m.def("short_conv_step(Tensor x, Tensor state, Tensor weight, Tensor? bias, bool silu) -> (Tensor out, Tensor state_out)");
+  m.def("short_conv_step_out(Tensor x, Tensor state, Tensor weight, Tensor? bias, bool silu, Tensor(a!) state_out) -> Tensor");
   m.def("selective_scan_forward(Tensor keys, Tensor values, Tensor queries, Tensor steps, Tensor rates, Tensor? memory, Tensor? skip, Tensor? step_bias, Tensor? lengths, bool softplus, bool save) -> (Tensor hidden, Tensor memory_out, Tensor states)");
   m.def("selective_scan_backward(Tensor? grad_hidden, Tensor? grad_memory_out, Tensor keys, Tensor values, Tensor queries, Tensor steps, Tensor rates, Tensor? skip, Tensor? step_bias, Tensor? lengths, Tensor states, bool softplus) -> (Tensor grad_keys, Tensor grad_values, Tensor grad_queries, Tensor grad_steps, Tensor grad_rates, Tensor grad_memory, Tensor grad_skip, Tensor grad_step_bias)");
-  m.def("selective_step(Tensor keys, Tensor values, Tensor queries, Tensor steps, Tensor rates, Tensor memory, Tensor? skip, Tensor? step_bias, bool softplus, Tensor(a!) memory_out) -> Tensor");
+  m.def("selective_step(Tensor keys, Tensor values, Tensor queries, Tensor steps, Tensor rates, Tensor memory, Tensor? skip, Tensor? step_bias, bool softplus) -> (Tensor hidden, Tensor memory_out)");
+  m.def("selective_step_out(Tensor keys, Tensor values, Tensor queries, Tensor steps, Tensor rates, Tensor memory, Tensor? skip, Tensor? step_bias, bool softplus, Tensor(a!) memory_out) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(grm_cuda, CUDA, m) {
   m.impl("short_conv_forward", grm_selective::short_conv_forward);
   m.impl("short_conv_backward", grm_selective::short_conv_backward);
   m.impl("short_conv_step", grm_selective::short_conv_step);
+  m.impl("short_conv_step_out", grm_selective::short_conv_step_out);
   m.impl("selective_scan_forward", grm_selective::selective_scan_forward);
   m.impl("selective_scan_backward", grm_selective::selective_scan_backward);
   m.impl("selective_step", grm_selective::selective_step);
+  m.impl("selective_step_out", grm_selective::selective_step_out);
 }

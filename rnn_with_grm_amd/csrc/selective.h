@@ -49,6 +49,7 @@ struct SelArgs {
   int64_t T, nsave, part_tokens;
   int B, H, P, G, N, PT, parts;
   int steps_f32, softplus, vec;
+  int stream;  // outputs are stored past the caches
 };
 
 __device__ __forceinline__ float exp2_f(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -397,6 +398,13 @@ __device__ __forceinline__ void key_frags(Frag8<M> (&kf)[NT], const typename ET<
 // Keeps what stands before it before it: reads issued ahead stay ahead.
 __device__ __forceinline__ void hold_order() { __builtin_amdgcn_sched_barrier(0); }
 
+// A 16- or 8-byte store, past the caches where `stream`.
+template <class T>
+__device__ __forceinline__ void store_as(T* p, T v, bool stream) {
+  if (stream) __builtin_nontemporal_store(v, p);
+  else *p = v;
+}
+
 // Host side: f(E, M, NP, VEC) with one of the compiled forms.
 template <class F>
 void sel_with_form(int dtype, int64_t N, bool vec, F f) {
@@ -414,6 +422,9 @@ void sel_with_form(int dtype, int64_t N, bool vec, F f) {
   else by_width(F32{}, F32{});
 }
 inline int64_t sel_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
+// More than the eight 4 MB L2 caches hold is stored past them: what would be written back at the kernel's end leaves
+// during it (STREAMLATER).
+inline int sel_streams(int64_t bytes) { return bytes > (int64_t{32} << 20); }
 int sel_check(const struct grm_hip_selective_args* u, const char* what);
 SelArgs sel_args(const struct grm_hip_selective_args* u);
 // Tokens of a backward chunk, and time parts of a walk: part_tokens set to a multiple of it.

@@ -292,7 +292,14 @@ __global__ __launch_bounds__(kWalkThreads) __attribute__((amdgpu_waves_per_eu(2,
         if (t_first + t < t_last) {
           eraw* o = hid + t * hstride + col;
           if (hvec) {
-            if (col < pw) store4_raw<E>(o, v);
+            if (col < pw) {
+              if constexpr (sizeof(eraw) == 2) {
+                typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+                store_as(reinterpret_cast<u32x2*>(o), u32x2{pack2<E>(v[0], v[1]), pack2<E>(v[2], v[3])}, a.stream != 0);
+              } else {
+                store_as(reinterpret_cast<f32x4*>(o), v, a.stream != 0);
+              }
+            }
           } else {
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
@@ -501,7 +508,7 @@ __global__ __launch_bounds__(256) void selective_step_kernel(SelArgs a) {
       if (p < a.P && col < a.N) {
         float* s = op + static_cast<int64_t>(p) * a.N + col;
         if (whole) {
-          *reinterpret_cast<float4*>(s) = m[u];
+          store_as(reinterpret_cast<f32x4*>(s), f32x4{m[u].x, m[u].y, m[u].z, m[u].w}, a.stream != 0);
         } else {
           s[0] = m[u].x;
           if (col + 1 < a.N) s[1] = m[u].y;
@@ -657,6 +664,7 @@ extern "C" int grm_hip_selective_scan_fwd(const grm_hip_selective_args* u, void*
   }
   SelArgs a = sel_args(u);
   a.hidden = hidden; a.memory_out = memory_out; a.states = states;
+  a.stream = sel_streams(u->batch * u->seq_len * u->heads * u->value_dim * (u->dtype == GRM_HIP_F32 ? 4 : 2));
   a.vec = a.vec && aligned(hidden);
   a.nsave = sel_ceil(u->seq_len, sel_block(u->dtype));
   a.parts = sel_parts(static_cast<int64_t>(a.B) * a.H * a.PT, a.T, u->dtype, &a.part_tokens);
@@ -702,6 +710,7 @@ extern "C" int grm_hip_selective_step(const grm_hip_selective_args* u, void* hid
   }
   SelArgs a = sel_args(u);
   a.hidden = hidden; a.memory_out = memory_out;
+  a.stream = sel_streams(state_bytes);
   auto go = [&](auto e, auto lpr) {
     constexpr int LPR = decltype(lpr)::value, rows = 4 * (64 / LPR) * 4;  // of a workgroup at a time
     selective_step_kernel<decltype(e), LPR>

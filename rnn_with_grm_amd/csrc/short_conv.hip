@@ -15,6 +15,8 @@
 // float32, rounded once on output.  All three are bound by HBM.
 #include <stdint.h>
 
+#include <utility>
+
 #include "f32_tiles.h"
 #include "grm_hip.h"
 #include "grm_hip_common.h"
@@ -41,37 +43,63 @@ struct ConvArgs {
   int64_t xb, xt;        // elements between sequences and between tokens of x
   int64_t B, T, C;
   int64_t runs;          // runs of a sequence
-  int run;               // tokens of one
+  int64_t run;           // tokens of one
   int w_f32;             // weight and bias are float32 whatever x is
-  int silu;
+  int stream;            // outputs are stored past the caches
 };
 
-// V consecutive elements as floats.
+// V consecutive elements as they lie in memory.
+template <class E, int V>
+struct RawRow {
+  typename ET<E>::raw e[V];
+};
+template <class E, int V>
+__device__ __forceinline__ void widen(const RawRow<E, V>& r, float (&v)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = ET<E>::to_f(r.e[i]);
+}
+// The access that a row is read or written in: 16 or 8 bytes, or one element.
+template <class E, int V>
+using Access = std::conditional_t<V * sizeof(typename ET<E>::raw) == 16, uint32_t __attribute__((ext_vector_type(4))),
+                                  std::conditional_t<V * sizeof(typename ET<E>::raw) == 8, uint32_t __attribute__((ext_vector_type(2))),
+                                                     typename ET<E>::raw>>;
+template <class E, int V>
+__device__ __forceinline__ RawRow<E, V> raw_row(const typename ET<E>::raw* p) {
+  return __builtin_bit_cast(RawRow<E, V>, *reinterpret_cast<const Access<E, V>*>(p));
+}
+// The row at p, or zeros: a load that nothing is done to, so that it is waited for where it is used.
+template <class E, int V>
+__device__ __forceinline__ RawRow<E, V> raw_row_if(const typename ET<E>::raw* p, bool in) {
+  Access<E, V> u = {};
+  if (in) u = *reinterpret_cast<const Access<E, V>*>(p);
+  return __builtin_bit_cast(RawRow<E, V>, u);
+}
 template <class E, int V>
 __device__ __forceinline__ void ld_row(const typename ET<E>::raw* p, float (&v)[V]) {
-  if constexpr (V == 1) {
-    v[0] = ET<E>::to_f(p[0]);
-  } else if constexpr (sizeof(typename ET<E>::raw) == 4) {
-    const float4 u = *reinterpret_cast<const float4*>(p);
-    v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
-  } else {
-    const U8<E> u = __builtin_bit_cast(U8<E>, *reinterpret_cast<const uint4*>(p));
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = ET<E>::to_f(u.e[i]);
-  }
+  widen<E, V>(raw_row<E, V>(p), v);
 }
 
+// `stream`: past the caches (see streams()).
 template <class E, int V>
-__device__ __forceinline__ void st_row(typename ET<E>::raw* p, const float (&v)[V]) {
-  if constexpr (V == 1) {
-    p[0] = ET<E>::from_f(v[0]);
-  } else if constexpr (sizeof(typename ET<E>::raw) == 4) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  } else {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack2<E>(v[0], v[1]), pack2<E>(v[2], v[3]), pack2<E>(v[4], v[5]),
-                                              pack2<E>(v[6], v[7]));
-  }
+__device__ __forceinline__ void st_row(typename ET<E>::raw* p, const float (&v)[V], bool stream = false) {
+  RawRow<E, V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.e[i] = ET<E>::from_f(v[i]);
+  const Access<E, V> q = __builtin_bit_cast(Access<E, V>, r);
+  if (stream) __builtin_nontemporal_store(q, reinterpret_cast<Access<E, V>*>(p));
+  else *reinterpret_cast<Access<E, V>*>(p) = q;
 }
+
+// f(0), ..., f(U - 1) with constants, so that a window's slots are registers by name.
+template <int U, class F, int... I>
+__device__ __forceinline__ void unrolled(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int U, class F>
+__device__ __forceinline__ void unrolled(F f) { unrolled<U>(f, std::make_integer_sequence<int, U>{}); }
+
+// Steps taken at once: a multiple of the window, so that its rows need not move.
+template <int W> constexpr int kSteps = W == 3 ? 3 : 4;
 
 template <int V>
 __device__ __forceinline__ void zero(float (&v)[V]) {
@@ -85,15 +113,29 @@ __device__ __forceinline__ int64_t length_of(const ConvArgs& a, int64_t b) {
   return a.lengths == nullptr ? a.T : max_i64(0, min_i64(a.lengths[b], a.T));
 }
 
-// weight[c .. c + V)[0 .. W) and bias of a thread's channels.
-template <class E, int V, int W>
-__device__ __forceinline__ void ld_weight(const ConvArgs& a, int64_t c, float (&w)[W][V], float (&b)[V]) {
+// weight[c .. c + V)[0 .. W) and bias of a thread's channels: V W consecutive elements, in 16-byte accesses where
+// rows are read so.
+template <class D, int V, int W>
+__device__ __forceinline__ void ld_weight_as(const ConvArgs& a, int64_t c, float (&w)[W][V], float (&b)[V]) {
+  using raw = typename ET<D>::raw;
+  const raw *wp = static_cast<const raw*>(a.weight) + c * W, *bp = static_cast<const raw*>(a.bias) + c;
+  constexpr int Q = V == 1 ? 1 : V * static_cast<int>(sizeof(raw)) < 16 ? V : 16 / static_cast<int>(sizeof(raw));  // of an access
+  RawRow<D, Q> r[V * W / Q], rb[V / Q];
+#pragma unroll
+  for (int i = 0; i < V * W / Q; ++i) r[i] = raw_row<D, Q>(wp + i * Q);
+#pragma unroll
+  for (int i = 0; i < V / Q; ++i) rb[i] = raw_row_if<D, Q>(bp + i * Q, a.bias != nullptr);
 #pragma unroll
   for (int i = 0; i < V; ++i) {
 #pragma unroll
-    for (int j = 0; j < W; ++j) w[j][i] = ld_state<E>(a.weight, (c + i) * W + j, a.w_f32 != 0);
-    b[i] = a.bias == nullptr ? 0.f : ld_state<E>(a.bias, c + i, a.w_f32 != 0);
+    for (int j = 0; j < W; ++j) w[j][i] = ET<D>::to_f(r[(i * W + j) / Q].e[(i * W + j) % Q]);
+    b[i] = ET<D>::to_f(rb[i / Q].e[i % Q]);
   }
+}
+template <class E, int V, int W>
+__device__ __forceinline__ void ld_weight(const ConvArgs& a, int64_t c, float (&w)[W][V], float (&b)[V]) {
+  if (a.w_f32) ld_weight_as<F32, V, W>(a, c, w, b);
+  else ld_weight_as<E, V, W>(a, c, w, b);
 }
 
 // Row t of a sequence, t >= -(W - 1): the state below 0, zeros from `n` on.
@@ -111,7 +153,7 @@ __device__ __forceinline__ void ld_x(const ConvArgs& a, int64_t b, int64_t t, in
 
 // Threads 0 .. B * runs * CV walk runs of tokens; B * (W - 1) * CV more copy the state that
 // the call leaves.
-template <class E, int V, int W>
+template <class E, int V, int W, bool SILU>
 __global__ __launch_bounds__(kThreads) void conv_fwd_kernel(ConvArgs a) {
   using raw = typename ET<E>::raw;
   const uint32_t cv = static_cast<uint32_t>(a.C / V), runs = static_cast<uint32_t>(a.runs);
@@ -129,51 +171,37 @@ __global__ __launch_bounds__(kThreads) void conv_fwd_kernel(ConvArgs a) {
   }
   const int64_t c = id % cv * V, run = id / cv % runs, b = id / cv / runs;
   const int64_t n = length_of(a, b), t0 = run * a.run, t1 = min_i64(t0 + a.run, a.T);
+  // The window's slot of a token is its number in the run, modulo W.
   float w[W][V], bias[V], win[W][V];
   ld_weight<E, V, W>(a, c, w, bias);
 #pragma unroll
   for (int j = 1; j < W; ++j) ld_x<E, V, W>(a, b, t0 - W + j, n, c, win[j]);
   const raw* xp = static_cast<const raw*>(a.x) + b * a.xb + c;
   raw* op = static_cast<raw*>(a.out) + b * a.T * a.C + c;
-  auto step = [&](int64_t t, const float (&x)[V]) {
+  constexpr int U = kSteps<W>;
+  for (int64_t tb = t0; tb < t1; tb += U) {
+    RawRow<E, V> x[U];
 #pragma unroll
-    for (int j = 0; j + 1 < W; ++j) {
+    for (int u = 0; u < U; ++u) x[u] = raw_row_if<E, V>(xp + (tb + u) * a.xt, tb + u < n);
+    unrolled<U>([&](auto uc) {
+      constexpr int u = decltype(uc)::value;
+      widen<E, V>(x[u], win[u % W]);
+      float y[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) win[j][i] = win[j + 1][i];
-    }
-    float y[V];
+      for (int i = 0; i < V; ++i) {
+        float p = bias[i];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      win[W - 1][i] = x[i];
-      float p = bias[i];
-#pragma unroll
-      for (int j = 0; j < W; ++j) p = fmaf(w[j][i], win[j][i], p);
-      y[i] = a.silu ? p * sigmoid_f(p) : p;
-    }
-    st_row<E, V>(op + t * a.C, y);
-  };
-  constexpr int U = 4;  // rows in flight
-  int64_t t = t0;
-  const int64_t live = min_i64(t1, n);
-  for (; t + U <= live; t += U) {
-    float x[U][V];
-#pragma unroll
-    for (int u = 0; u < U; ++u) ld_row<E, V>(xp + (t + u) * a.xt, x[u]);
-#pragma unroll
-    for (int u = 0; u < U; ++u) step(t + u, x[u]);
+        for (int j = 0; j < W; ++j) p = fmaf(w[j][i], win[(u + 1 + j) % W][i], p);
+        y[i] = SILU ? p * sigmoid_f(p) : p;
+        if (tb + u >= n) y[i] = 0.f;
+      }
+      if (tb + u < t1) st_row<E, V>(op + (tb + u) * a.C, y, a.stream != 0);
+    });
   }
-  for (; t < live; ++t) {
-    float x[V];
-    ld_row<E, V>(xp + t * a.xt, x);
-    step(t, x);
-  }
-  float none[V];
-  zero<V>(none);
-  for (; t < t1; ++t) st_row<E, V>(op + t * a.C, none);
 }
 
 // Lane = channels, wave = every fourth run from its workgroup's part of all B * runs.
-template <class E, int V, int W>
+template <class E, int V, int W, bool SILU>
 __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(ConvArgs a) {
   using raw = typename ET<E>::raw;
   __shared__ float sums[3][64 * V * (W + 1)];
@@ -198,46 +226,59 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(ConvArgs a) {
         ld_x<E, V, W>(a, b, t0 - W + j, n, c, win[j]);
         zero<V>(g[j]);
       }
-      // Step t: the window moves to x_t, g_t = dy_t act'(pre_t), and row s = t - W + 1 of
-      // dx (below 0: of dstate, by the first run only) has all of its terms.
-      const int64_t first = run == 0 ? -(W - 1) : t0;
-      for (int64_t t = t0; t < t1 + W - 1; ++t) {
-        float x[V], dy[V];
-        ld_x<E, V, W>(a, b, t, n, c, x);
-        if (a.dy != nullptr && t < n) ld_row<E, V>(dyp + t * a.C, dy);
-        else zero<V>(dy);
-        const int64_t s = t - W + 1;
-        float dx[V];
-        const int64_t at = s - (n - (W - 1));  // row of the state left behind that is x_s
-        if (a.dstate_out != nullptr && at >= 0 && at < W - 1)
-          ld_row<E, V>(static_cast<const raw*>(a.dstate_out) + (b * (W - 1) + at) * a.C + c, dx);
-        else zero<V>(dx);
+      // Step t: x_t and g_t = dy_t act'(pre_t) take their slots, and row s = t - W + 1 of dx (below 0: of
+      // dstate, by the first run only) has all of its terms.  The rows of U steps are in flight together.
+      const int64_t first = run == 0 ? -(W - 1) : t0, end = t1 + W - 1;
+      const raw* xp = static_cast<const raw*>(a.x) + b * a.xb + c;
+      constexpr int U = kSteps<W>;
+      for (int64_t tb = t0; tb < end; tb += U) {
+        RawRow<E, V> xr[U], yr[U];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-#pragma unroll
-          for (int j = 0; j + 1 < W; ++j) { win[j][i] = win[j + 1][i]; g[j][i] = g[j + 1][i]; }
-          win[W - 1][i] = x[i];
-          float d = dy[i];
-          if (a.silu) {
-            float p = bias[i];
-#pragma unroll
-            for (int j = 0; j < W; ++j) p = fmaf(w[j][i], win[j][i], p);
-            const float sg = sigmoid_f(p);
-            d *= sg * fmaf(p, 1.f - sg, 1.f);
-          }
-          g[W - 1][i] = t < n ? d : 0.f;
-          if (t < t1) {
-            db[i] += g[W - 1][i];
-#pragma unroll
-            for (int j = 0; j < W; ++j) dw[j][i] = fmaf(g[W - 1][i], win[j][i], dw[j][i]);
-          }
-#pragma unroll
-          for (int j = 0; j < W; ++j) dx[i] = fmaf(w[j][i], g[W - 1 - j][i], dx[i]);
-          if (s >= n) dx[i] = 0.f;
+        for (int u = 0; u < U; ++u) {
+          const bool in = tb + u < n;
+          xr[u] = raw_row_if<E, V>(xp + (tb + u) * a.xt, in);
+          yr[u] = raw_row_if<E, V>(dyp + (tb + u) * a.C, in && a.dy != nullptr);
         }
-        if (s < first) continue;
-        if (s >= 0) st_row<E, V>(static_cast<raw*>(a.dx) + (b * a.T + s) * a.C + c, dx);
-        else if (a.dstate != nullptr) st_row<E, V>(static_cast<raw*>(a.dstate) + (b * (W - 1) + s + W - 1) * a.C + c, dx);
+        auto steps = [&](auto inner) {  // inner: all of these tokens are the run's own and away from both ends
+          constexpr bool INNER = decltype(inner)::value;
+          unrolled<U>([&](auto uc) {
+            constexpr int u = decltype(uc)::value;
+            const int64_t t = tb + u, s = t - W + 1;
+            if (!INNER && t >= end) return;
+            float dx[V];
+            zero<V>(dx);
+            const int64_t at = s - (n - (W - 1));  // row of the state left behind that is x_s
+            if (!INNER && a.dstate_out != nullptr && at >= 0 && at < W - 1)
+              ld_row<E, V>(static_cast<const raw*>(a.dstate_out) + (b * (W - 1) + at) * a.C + c, dx);
+            float (&xv)[V] = win[u % W], (&gv)[V] = g[u % W];
+            widen<E, V>(xr[u], xv);
+            widen<E, V>(yr[u], gv);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              if constexpr (SILU) {
+                float p = bias[i];
+#pragma unroll
+                for (int j = 0; j < W; ++j) p = fmaf(w[j][i], win[(u + 1 + j) % W][i], p);
+                const float sg = sigmoid_f(p);
+                gv[i] *= sg * fmaf(p, 1.f - sg, 1.f);
+              }
+              if (!INNER && t >= n) gv[i] = 0.f;
+              const float gw = INNER || t < t1 ? gv[i] : 0.f;  // the rows past the run are another one's
+              db[i] += gw;
+#pragma unroll
+              for (int j = 0; j < W; ++j) {
+                dw[j][i] = fmaf(gw, win[(u + 1 + j) % W][i], dw[j][i]);
+                dx[i] = fmaf(w[j][i], g[(u + W - j) % W][i], dx[i]);
+              }
+              if (!INNER && s >= n) dx[i] = 0.f;
+            }
+            if (!INNER && s < first) return;
+            if (INNER || s >= 0) st_row<E, V>(static_cast<raw*>(a.dx) + (b * a.T + s) * a.C + c, dx, a.stream != 0);
+            else if (a.dstate != nullptr) st_row<E, V>(static_cast<raw*>(a.dstate) + (b * (W - 1) + s + W - 1) * a.C + c, dx);
+          });
+        };
+        if (tb - W + 1 >= (first > 0 ? first : 0) && tb + U <= (n < t1 ? n : t1)) steps(std::true_type{});
+        else steps(std::false_type{});
       }
     }
   }
@@ -263,21 +304,23 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(ConvArgs a) {
   }
 }
 
-// Sums of the workgroups' parts: 64 elements per workgroup, four waves a quarter of the parts each.
+// Sums of the workgroups' parts: 64 elements per workgroup, eight waves an eighth of the parts each.
 template <class E, int W>
-__global__ __launch_bounds__(kThreads) void conv_weight_kernel(const float* partial, void* dweight, void* dbias,
-                                                               int64_t C, int parts, int w_f32) {
-  __shared__ float sums[3][64];
+__global__ __launch_bounds__(512) void conv_weight_kernel(const float* partial, void* dweight, void* dbias, int64_t C,
+                                                          int parts, int w_f32) {
+  __shared__ float sums[7][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t e = static_cast<int64_t>(blockIdx.x) * 64 + lane, total = C * (W + 1);
   float s = 0.f;
   if (e < total) {
-    for (int p = wave; p < parts; p += 4) s += partial[static_cast<int64_t>(p) * total + e];
+#pragma unroll 4
+    for (int p = wave; p < parts; p += 8) s += partial[static_cast<int64_t>(p) * total + e];
   }
   if (wave > 0) sums[wave - 1][lane] = s;
   __syncthreads();
   if (wave > 0 || e >= total) return;
-  s += sums[0][lane] + sums[1][lane] + sums[2][lane];
+#pragma unroll
+  for (int i = 0; i < 7; ++i) s += sums[i][lane];
   const int64_t c = e / (W + 1);
   const int j = static_cast<int>(e % (W + 1));
   if (j < W) st_state<E>(dweight, c * W + j, w_f32 != 0, s);
@@ -286,7 +329,7 @@ __global__ __launch_bounds__(kThreads) void conv_weight_kernel(const float* part
 
 // One token: every thread reads its channels of the state before it writes them, so the state
 // may be updated in place.
-template <class E, int V, int W>
+template <class E, int V, int W, bool SILU>
 __global__ __launch_bounds__(kThreads) void conv_step_kernel(ConvArgs a) {
   using raw = typename ET<E>::raw;
   const uint32_t cv = static_cast<uint32_t>(a.C / V), id = blockIdx.x * kThreads + threadIdx.x;
@@ -301,7 +344,7 @@ __global__ __launch_bounds__(kThreads) void conv_step_kernel(ConvArgs a) {
     float p = bias[i];
 #pragma unroll
     for (int j = 0; j < W; ++j) p = fmaf(w[j][i], win[j][i], p);
-    y[i] = a.silu ? p * sigmoid_f(p) : p;
+    y[i] = SILU ? p * sigmoid_f(p) : p;
   }
   st_row<E, V>(static_cast<raw*>(a.out) + b * a.C + c, y);
 #pragma unroll
@@ -333,19 +376,23 @@ int check_conv(const ConvArgs& a, int64_t width, int dtype, int w_dtype, const c
 bool whole_rows(const ConvArgs& a, int dtype) {
   const int64_t v = dtype == GRM_HIP_F32 ? 4 : 8;
   return a.C % v == 0 && a.xb % v == 0 && a.xt % v == 0 && aligned(a.x) && aligned(a.state) && aligned(a.out) &&
-         aligned(a.state_out) && aligned(a.dy) && aligned(a.dstate_out) && aligned(a.dx) && aligned(a.dstate);
+         aligned(a.state_out) && aligned(a.weight) && aligned(a.bias) && aligned(a.dy) && aligned(a.dstate_out) && aligned(a.dx) && aligned(a.dstate);
 }
 
-// f(E, V, W): one of the compiled forms.
-template <class F>
-void with_form(int dtype, bool vec, int64_t width, F f) {
+// f(E, V, W, SILU): one of the compiled forms, V = 1 or (vec) 16 bytes of elements, at most MOST of them.
+template <int MOST, class F>
+void with_form(int dtype, bool vec, int64_t width, bool silu, F f) {
+  auto by_silu = [&](auto e, auto v, auto w) {
+    if (silu) f(e, v, w, std::true_type{});
+    else f(e, v, w, std::false_type{});
+  };
   auto by_width = [&](auto e, auto v) {
-    if (width == 2) f(e, v, std::integral_constant<int, 2>{});
-    else if (width == 3) f(e, v, std::integral_constant<int, 3>{});
-    else f(e, v, std::integral_constant<int, 4>{});
+    if (width == 2) by_silu(e, v, std::integral_constant<int, 2>{});
+    else if (width == 3) by_silu(e, v, std::integral_constant<int, 3>{});
+    else by_silu(e, v, std::integral_constant<int, 4>{});
   };
   auto by_vec = [&](auto e) {
-    constexpr int V = sizeof(typename ET<decltype(e)>::raw) == 4 ? 4 : 8;
+    constexpr int V = sizeof(typename ET<decltype(e)>::raw) == 4 || MOST == 4 ? 4 : 8;
     if (vec) by_width(e, std::integral_constant<int, V>{});
     else by_width(e, std::integral_constant<int, 1>{});
   };
@@ -356,14 +403,21 @@ void with_form(int dtype, bool vec, int64_t width, F f) {
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Workgroups that share the backward's sums: enough for four waves on every SIMD of 256 CUs over the
-// channel blocks, and no more than there are sets of four runs.
-constexpr int kBwdRun = 32;
-int64_t bwd_parts(int64_t B, int64_t T, int64_t C, int dtype, bool vec) {
-  const int64_t v = !vec ? 1 : dtype == GRM_HIP_F32 ? 4 : 8;
-  const int64_t blocks = ceil_div(C, 64 * v), runs = B * ceil_div(T > 0 ? T : 1, kBwdRun);
-  const int64_t want = ceil_div(1024, blocks), most = ceil_div(runs, 4);
-  return want < most ? want : (most > 0 ? most : 1);
+// Rows of more than the eight 4 MB L2 caches hold are stored past them: what would be written back at the kernel's end
+// leaves during it (8 x 2048 tokens of 2304 bf16 channels 38.5 -> 31.7 us; 4 MB outputs the same either way).
+int streams(int64_t elements, int dtype) { return elements * (dtype == GRM_HIP_F32 ? 4 : 2) > (int64_t{32} << 20); }
+
+// The backward's runs: about one for each of the 2048 waves that fit the chip at once (two a SIMD), of 16 tokens
+// at least (three rows of each run's 19 or more are formed twice).  A thread has four channels: with eight, its
+// sums and windows leave two waves a SIMD (8 x 2048 tokens of 2304 bf16 channels: 96 us, with four 68).
+int64_t bwd_run(int64_t B, int64_t T, int64_t C, bool vec) {
+  const int64_t run = ceil_div(B * T * ceil_div(C, 64 * (vec ? 4 : 1)), 2048);
+  return run < 16 ? 16 : run < T ? run : (T > 16 ? T : 16);
+}
+// Workgroups that share the sums, four runs at a time.
+int64_t bwd_parts(int64_t B, int64_t T, int64_t run) {
+  const int64_t sets = ceil_div(B * ceil_div(T > 0 ? T : 1, run), 4);
+  return sets < 1024 ? sets : 1024;
 }
 
 }  // namespace
@@ -378,7 +432,7 @@ extern "C" int grm_hip_short_conv_fwd(const void* x, const void* weight, const v
   ConvArgs a{};
   a.x = x; a.weight = weight; a.bias = bias; a.state = state; a.lengths = lengths; a.out = out;
   a.state_out = state_out; a.xb = x_batch_stride; a.xt = x_token_stride; a.B = batch; a.T = seq_len; a.C = channels;
-  a.w_f32 = weight_dtype == GRM_HIP_F32; a.silu = silu;
+  a.w_f32 = weight_dtype == GRM_HIP_F32;
   if (int rc = check_conv(a, width, dtype, weight_dtype, "short_conv")) return rc;
   if (batch == 0) return GRM_HIP_OK;
   if (weight == nullptr || state_out == nullptr || (seq_len > 0 && (x == nullptr || out == nullptr))) {
@@ -391,6 +445,7 @@ extern "C" int grm_hip_short_conv_fwd(const void* x, const void* weight, const v
     return GRM_HIP_EINVAL;
   }
   const bool vec = whole_rows(a, dtype);
+  a.stream = streams(batch * a.T * channels, dtype);
   const int64_t cv = vec ? channels / (dtype == GRM_HIP_F32 ? 4 : 8) : channels;
   // Runs of 16 tokens read 3 rows of 19 twice; where that leaves fewer than four waves a SIMD
   // (2^18 threads), runs of 4 give the CUs more to have in flight.
@@ -401,8 +456,8 @@ extern "C" int grm_hip_short_conv_fwd(const void* x, const void* weight, const v
     set_error("short_conv: too many elements for one launch");
     return GRM_HIP_EUNSUPPORTED;
   }
-  with_form(dtype, vec, width, [&](auto e, auto v, auto w) {
-    conv_fwd_kernel<decltype(e), decltype(v)::value, decltype(w)::value>
+  with_form<8>(dtype, vec, width, silu != 0, [&](auto e, auto v, auto w, auto act) {
+    conv_fwd_kernel<decltype(e), decltype(v)::value, decltype(w)::value, decltype(act)::value>
         <<<dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0, static_cast<hipStream_t>(stream)>>>(a);
   });
   return check_launch("short_conv");
@@ -411,7 +466,8 @@ extern "C" int grm_hip_short_conv_fwd(const void* x, const void* weight, const v
 extern "C" int64_t grm_hip_short_conv_bwd_workspace(int64_t batch, int64_t seq_len, int64_t channels, int64_t width,
                                                     int dtype) {
   if (batch <= 0 || seq_len < 0 || channels <= 0 || width < 2 || width > 4 || dtype < 0 || dtype > 2) return 0;
-  const int64_t a = bwd_parts(batch, seq_len, channels, dtype, true), b = bwd_parts(batch, seq_len, channels, dtype, false);
+  const int64_t a = bwd_parts(batch, seq_len, bwd_run(batch, seq_len, channels, true)),
+                b = bwd_parts(batch, seq_len, bwd_run(batch, seq_len, channels, false));
   return (a > b ? a : b) * channels * (width + 1) * 4;
 }
 
@@ -425,7 +481,7 @@ extern "C" int grm_hip_short_conv_bwd(const void* x, const void* weight, const v
   a.x = x; a.weight = weight; a.bias = bias; a.state = state; a.lengths = lengths; a.dy = grad_out;
   a.dstate_out = grad_state_out; a.dx = grad_x; a.dstate = grad_state; a.partial = static_cast<float*>(workspace);
   a.xb = x_batch_stride; a.xt = x_token_stride; a.B = batch; a.T = seq_len; a.C = channels;
-  a.w_f32 = weight_dtype == GRM_HIP_F32; a.silu = silu;
+  a.w_f32 = weight_dtype == GRM_HIP_F32;
   if (int rc = check_conv(a, width, dtype, weight_dtype, "short_conv backward")) return rc;
   if (weight == nullptr || grad_weight == nullptr || (batch > 0 && seq_len > 0 && (x == nullptr || grad_x == nullptr))) {
     set_error("short_conv backward: x, weight, grad_x and grad_weight are required");
@@ -437,26 +493,27 @@ extern "C" int grm_hip_short_conv_bwd(const void* x, const void* weight, const v
     return GRM_HIP_EINVAL;
   }
   const bool vec = whole_rows(a, dtype);
-  const int64_t v = !vec ? 1 : dtype == GRM_HIP_F32 ? 4 : 8;
-  const int64_t parts = batch > 0 ? bwd_parts(batch, seq_len, channels, dtype, vec) : 0;
-  a.run = kBwdRun;
-  a.runs = ceil_div(seq_len > 0 ? seq_len : 1, kBwdRun);
+  a.stream = streams(batch * a.T * channels, dtype);
+  const int64_t v = vec ? 4 : 1;
+  a.run = bwd_run(batch, seq_len, channels, vec);
+  a.runs = ceil_div(seq_len > 0 ? seq_len : 1, a.run);
+  const int64_t parts = batch > 0 ? bwd_parts(batch, seq_len, a.run) : 0;
   const int64_t blocks = ceil_div(channels, 64 * v), weight_blocks = ceil_div(channels * (width + 1), 64);
-  if (weight_blocks > kMaxBlocks) {
-    set_error("short_conv backward: too many channels for one launch");
+  if (weight_blocks > kMaxBlocks || blocks > kMaxBlocks) {
+    set_error("short_conv backward: too many elements for one launch");
     return GRM_HIP_EUNSUPPORTED;
   }
   int rc = GRM_HIP_OK;
-  with_form(dtype, vec, width, [&](auto e, auto vv, auto w) {
+  with_form<4>(dtype, vec, width, silu != 0, [&](auto e, auto vv, auto w, auto act) {
     using E = decltype(e);
     constexpr int W = decltype(w)::value;
     if (parts > 0) {
-      conv_bwd_kernel<E, decltype(vv)::value, W>
+      conv_bwd_kernel<E, decltype(vv)::value, W, decltype(act)::value>
           <<<dim3(static_cast<uint32_t>(blocks), static_cast<uint32_t>(parts)), dim3(kThreads), 0,
              static_cast<hipStream_t>(stream)>>>(a);
       if ((rc = check_launch("short_conv backward")) != GRM_HIP_OK) return;
     }
-    conv_weight_kernel<E, W><<<dim3(static_cast<uint32_t>(weight_blocks)), dim3(kThreads), 0,
+    conv_weight_kernel<E, W><<<dim3(static_cast<uint32_t>(weight_blocks)), dim3(512), 0,
                                static_cast<hipStream_t>(stream)>>>(a.partial, grad_weight, grad_bias, channels,
                                                                    static_cast<int>(parts), a.w_f32);
     rc = check_launch("short_conv backward, weights");
@@ -470,7 +527,7 @@ extern "C" int grm_hip_short_conv_step(const void* x, const void* weight, const 
   ConvArgs a{};
   a.x = x; a.weight = weight; a.bias = bias; a.state = state; a.out = out; a.state_out = state_out;
   a.xb = x_batch_stride; a.xt = 0; a.B = batch; a.T = 1; a.C = channels;
-  a.w_f32 = weight_dtype == GRM_HIP_F32; a.silu = silu;
+  a.w_f32 = weight_dtype == GRM_HIP_F32;
   if (int rc = check_conv(a, width, dtype, weight_dtype, "short_conv_step")) return rc;
   if (batch == 0) return GRM_HIP_OK;
   if (x == nullptr || weight == nullptr || state == nullptr || out == nullptr || state_out == nullptr) {
@@ -483,14 +540,15 @@ extern "C" int grm_hip_short_conv_step(const void* x, const void* weight, const 
     return GRM_HIP_EINVAL;
   }
   const bool vec = whole_rows(a, dtype);
+  a.stream = streams(batch * a.T * channels, dtype);
   const int64_t cv = vec ? channels / (dtype == GRM_HIP_F32 ? 4 : 8) : channels;
   const int64_t blocks = ceil_div(batch * cv, kThreads);
   if (blocks > kMaxBlocks) {
     set_error("short_conv_step: too many elements for one launch");
     return GRM_HIP_EUNSUPPORTED;
   }
-  with_form(dtype, vec, width, [&](auto e, auto v, auto w) {
-    conv_step_kernel<decltype(e), decltype(v)::value, decltype(w)::value>
+  with_form<8>(dtype, vec, width, silu != 0, [&](auto e, auto v, auto w, auto act) {
+    conv_step_kernel<decltype(e), decltype(v)::value, decltype(w)::value, decltype(act)::value>
         <<<dim3(static_cast<uint32_t>(blocks)), dim3(kThreads), 0, static_cast<hipStream_t>(stream)>>>(a);
   });
   return check_launch("short_conv_step");

@@ -43,7 +43,8 @@ EXTRA_OPS = ("segment_scan_forward", "topk_route", "fuse_residual", "gather_appl
              "retrieve_fuse", "project_split", "residual_layer_norm", "gather_apply_backward_queries",
              "gather_apply_backward_tokens", "apply_query_backward_queries", "archive_cast", "project_gemm",
              "linear_residual_layer_norm", "segment_retrieve_fuse", "selective_scan_forward", "selective_scan_backward",
-             "selective_step", "short_conv_forward", "short_conv_backward", "short_conv_step")
+             "selective_step", "selective_step_out", "short_conv_forward", "short_conv_backward", "short_conv_step",
+             "short_conv_step_out")
 
 # Environment variables of the reference (cuda_ops.py:26-32): one per op and a global one.
 GLOBAL_POLICY_ENV = "GRM_CUDA_KERNEL_POLICY"
@@ -949,8 +950,8 @@ def cuda_short_conv_step(x: Tensor, state: Tensor, weight: Tensor, bias: Optiona
     if not grad and x.is_cuda and _run_native("short_conv", x.device, enabled=enabled,
                                               debug_fallback=debug_fallback):
         if state_out is None:
-            state_out = torch.empty_like(state, memory_format=torch.contiguous_format)
-        return torch.ops.grm_cuda.short_conv_step(x, state, weight, bias, silu, state_out), state_out
+            return torch.ops.grm_cuda.short_conv_step(x, state, weight, bias, silu)
+        return torch.ops.grm_cuda.short_conv_step_out(x, state, weight, bias, silu, state_out), state_out
     if x.ndim != 2:
         raise ValueError("short_conv_step: x must be [batch, channels]")
     out, moved = cuda_short_conv(x[:, None], weight, bias, state, activation=activation, enabled=enabled,
@@ -1084,10 +1085,10 @@ def cuda_selective_step(keys: Tensor, values: Tensor, queries: Tensor, steps: Te
         _check_out(memory_out, memory, "memory_out", grad)
     if not grad and values.is_cuda and _run_native("selective_scan", values.device, enabled=enabled,
                                                    debug_fallback=debug_fallback):
+        args = (keys, values, queries, steps, _f32(rates), memory, _f32(skip), _f32(step_bias), bool(softplus))
         if memory_out is None:
-            memory_out = torch.empty_like(memory, memory_format=torch.contiguous_format)
-        return torch.ops.grm_cuda.selective_step(keys, values, queries, steps, _f32(rates), memory, _f32(skip),
-                                                 _f32(step_bias), bool(softplus), memory_out), memory_out
+            return torch.ops.grm_cuda.selective_step(*args)
+        return torch.ops.grm_cuda.selective_step_out(*args, memory_out), memory_out
     if values.ndim != 3 or keys.ndim != 3 or queries.ndim != 3 or steps.ndim != 2:
         raise ValueError("selective_step: keys and queries must be [batch, groups, key_dim], values "
                          "[batch, heads, value_dim] and steps [batch, heads]")
