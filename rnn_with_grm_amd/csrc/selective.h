@@ -303,6 +303,21 @@ struct TileLoad {
       }
     }
   }
+  // Whether any element is an infinity or a NaN (all bits of its exponent are set).
+  __device__ __forceinline__ bool odd() const {
+    constexpr uint32_t X = std::is_same_v<E, F32> ? 0x7f800000u : std::is_same_v<E, BF16> ? 0x7f807f80u : 0x7c007c00u;
+    constexpr uint32_t ONE = std::is_same_v<E, F32> ? 0x00800000u : std::is_same_v<E, BF16> ? 0x00800080u : 0x04000400u;
+    uint32_t any = 0;  // one more in a full exponent carries into the sign
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) any |= (r[i][w][k] & X) + ONE;
+      }
+    }
+    return (any & (std::is_same_v<E, F32> ? 0x80000000u : 0x80008000u)) != 0;
+  }
   __device__ __forceinline__ void store(typename ET<M>::raw* tile, int tid) const {
     if (UNITS < THREADS && tid >= UNITS) return;
 #pragma unroll

@@ -37,7 +37,7 @@ struct WalkLds {
   static constexpr int Q0 = S::L * KT::STRIDE, X0 = Q0 + S::L * QT::STRIDE;
   static constexpr int STAGES = 3, STAGE = X0 + S::L * XT::STRIDE;  // a chunk's tiles
   static constexpr int MIX = S::L * MT::STRIDE;
-  static constexpr int SCAL = 6 * S::L;                             // hi, lo, d, tail weight, decay; total
+  static constexpr int SCAL = 5 * S::L + 8;  // hi, lo, d, tail weight, decay; total; whether a value is infinite or NaN, by wave
   static constexpr size_t bytes =
       (STAGES * STAGE + 2 * MIX) * sizeof(typename ET<M>::raw) + STAGES * SCAL * sizeof(float);
   static_assert(bytes <= 160 * 1024, "one CU's LDS");
@@ -126,6 +126,8 @@ __global__ __launch_bounds__(kWalkThreads) __attribute__((amdgpu_waves_per_eu(2,
       kr.store(s, tid);
       qr.store(s + Lds::Q0, tid);
       xr.store(s + Lds::X0, tid);
+      const bool odd = __any(xr.odd());
+      if (lane == 0) scal[slot * Lds::SCAL + 5 * L + 4 + wave] = odd ? 1.f : 0.f;
       if (wave == kStepWave) {
         const TokenScalars s = token_scalars<L>(a, step_value<E>(a, z) + bias, at - L + lane < live, rate);
         float* o = scal + slot * Lds::SCAL;
@@ -243,6 +245,7 @@ __global__ __launch_bounds__(kWalkThreads) __attribute__((amdgpu_waves_per_eu(2,
       float e[NIT];
 #pragma unroll
       for (int it = 0; it < NIT; ++it) e[it] = sc[4 * L + it * 16 + n16];
+      const f32x4 flags = *reinterpret_cast<const f32x4*>(sc + 5 * L + 4);
 #pragma unroll
       for (int s = 0; s < NS32; ++s) {
         xf[s] = col_frag<XT, M>(xs, 32 * s, rw);
@@ -275,6 +278,38 @@ __global__ __launch_bounds__(kWalkThreads) __attribute__((amdgpu_waves_per_eu(2,
       for (int s = 0; s < NS32; ++s) {
 #pragma unroll
         for (int it = 2 * s; it < NIT; ++it) y[it] = mfma8(xf[s], mf[s][it], y[it]);
+      }
+      if (__builtin_expect(__any(flags[0] + flags[1] + flags[2] + flags[3] != 0.f), 0)) {
+        // A weight of zero does not keep an infinity or a NaN out of a product: all outputs again, one token i at a
+        // time, with the values of the tokens behind it taken out.  (The lane's number anew: what is made of it here
+        // is not to be kept in registers for the case.)
+        int ln = lane_id();
+        asm volatile("" : "+v"(ln));
+#pragma unroll
+        for (int it = 0; it < NIT; ++it) {
+          f32x4 from = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int kk = 0; kk < NK; ++kk)
+            from = mfma8(pair_frag<M>(acc[2 * kk], acc[2 * kk + 1]), row_frag_t<QT, M>(ks + Lds::Q0, it * 16, kk * 32, ln), from);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) from[r] *= e[it];
+#pragma unroll 1
+          for (int k = 0; k < 16; ++k) {
+            f32x4 one = from;
+#pragma unroll
+            for (int s = 0; 2 * s <= it; ++s) {
+              Frag8<M> x = xf[s];
+#pragma unroll
+              for (int u = 0; u < 8; ++u) {
+                const int t = 32 * s + 4 * (ln >> 4) + (u < 4 ? u : 12 + u);
+                x.e[u] = t <= it * 16 + k ? x.e[u] : static_cast<raw>(0);
+              }
+              one = mfma8(x, mf[s][it], one);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[it][r] = (ln & 15) == k ? one[r] : y[it][r];
+          }
+        }
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {

@@ -407,11 +407,11 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // leaves during it (8 x 2048 tokens of 2304 bf16 channels 38.5 -> 31.7 us; 4 MB outputs the same either way).
 int streams(int64_t elements, int dtype) { return elements * (dtype == GRM_HIP_F32 ? 4 : 2) > (int64_t{32} << 20); }
 
-// The backward's runs: about one for each of the 2048 waves that fit the chip at once (two a SIMD), of 16 tokens
+// The backward's runs: about 3000, one and a half for each of the waves that fit the chip at once (104 us in the case below; 2000: 115, 4000: 109), of 16 tokens
 // at least (three rows of each run's 19 or more are formed twice).  A thread has four channels: with eight, its
-// sums and windows leave two waves a SIMD (8 x 2048 tokens of 2304 bf16 channels: 96 us, with four 68).
+// sums and windows leave two waves a SIMD (8 x 2048 tokens of 2304 bf16 channels: 96 us, with four 62).
 int64_t bwd_run(int64_t B, int64_t T, int64_t C, bool vec) {
-  const int64_t run = ceil_div(B * T * ceil_div(C, 64 * (vec ? 4 : 1)), 2048);
+  const int64_t run = ceil_div(B * T * ceil_div(C, 64 * (vec ? 4 : 1)), 3000);
   return run < 16 ? 16 : run < T ? run : (T > 16 ? T : 16);
 }
 // Workgroups that share the sums, four runs at a time.

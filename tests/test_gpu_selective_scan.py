@@ -175,3 +175,38 @@ def test_refusals(dev):
     both = torch.zeros(3, 4, 16, 16, device=dev)
     with pytest.raises(RuntimeError):  # the new state half over the old one
         step(*args[:-1], both[:2], memory_out=both[1:])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_infinities_and_nan_reach_no_earlier_token(dev, dtype):
+    """A value that is no number changes its own row of the state from its token on, and nothing else."""
+    x = inputs(dev, 1, 150, 2, 32, 1, 32, dtype, seed=21)
+    clean, clean_memory = run(x)
+    x["values"] = x["values"].clone()
+    x["values"][0, 20, 1, 5] = float("inf")
+    x["values"][0, 77, 0, 9] = float("nan")
+    hidden, memory = run(x)
+    same = torch.ones_like(hidden, dtype=torch.bool)
+    same[0, 20:, 1, 5] = False
+    same[0, 77:, 0, 9] = False
+    assert torch.equal(hidden[same], clean[same])
+    assert not torch.isfinite(hidden[0, 20, 1, 5]) and torch.isnan(hidden[0, 77:, 0, 9]).all()
+    rows = torch.ones_like(memory, dtype=torch.bool)
+    rows[0, 1, 5] = rows[0, 0, 9] = False
+    assert torch.equal(memory[rows], clean_memory[rows])
+
+
+@pytest.mark.parametrize("which", ["keys", "queries", "steps"])
+def test_an_odd_key_query_or_step_reaches_no_earlier_token(dev, which):
+    x = inputs(dev, 1, 150, 2, 32, 2, 32, torch.bfloat16, seed=22)
+    clean, _ = run(x)
+    x[which] = x[which].clone()
+    if which == "steps":
+        x[which][0, 70, 1] = float("nan")
+    else:
+        x[which][0, 70, 1, 3] = float("nan")
+    hidden, _ = run(x)
+    assert torch.equal(hidden[0, :70], clean[0, :70]) and torch.equal(hidden[0, :, 0], clean[0, :, 0])
+    assert torch.isnan(hidden[0, 70, 1]).all()
+    if which == "queries":
+        assert torch.equal(hidden[0, 71:], clean[0, 71:])
