@@ -6,13 +6,17 @@
 // with x_{-W+1 .. -1} the state's rows (zeros without one), W = 2 .. 4.  The state that a
 // call leaves is the last W - 1 rows of (state, x) before the sequence's length.
 //
-// Every element of x is wanted by W outputs of its own channel only, so a thread owns 16
-// bytes of channels and walks a run of tokens with the last rows in registers: each row is
-// read from HBM once, the W - 1 rows before a run a second time, from L2.  Nothing is kept
-// for the backward pass: it forms pre again from x, as cheap as reading it back.  The gradient of the weights is summed in registers
-// over a thread's runs, over a workgroup's four waves in LDS, and over the workgroups by a
-// second kernel in a fixed order (no atomics: the same sums on every run).  All arithmetic is
-// float32, rounded once on output.  All three are bound by HBM.
+// Every element of x is wanted by W outputs of its own channel only, so a thread owns 16 bytes of
+// channels (backward four channels, whose sums and windows then fit its registers) and walks a run of
+// tokens with the last rows in registers: each row is read from HBM once, the W - 1 rows before a run
+// a second time, from L2.  Nothing is kept for the backward pass: it forms pre again from x, as cheap
+// as reading it back.  The gradient of the weights is summed in registers over a thread's runs, over a
+// workgroup's four waves in LDS, and over the workgroups by a second kernel in a fixed order (no
+// atomics: the same sums on every run).  All arithmetic is float32, rounded once on output.
+//
+// HBM bounds the prompts, the launch bounds single tokens: 8 x 2048 tokens x 2304 bf16 channels 33 us
+// (151 MB, 4.6 TB/s), with all gradients 104 us (forward 33, backward 66, its weights' sums 5), one
+// token of 64 sequences 8 us.
 #include <stdint.h>
 
 #include <utility>
@@ -108,6 +112,15 @@ __device__ __forceinline__ void zero(float (&v)[V]) {
 }
 
 __device__ __forceinline__ float sigmoid_f(float p) { return __builtin_amdgcn_rcpf(1.f + __expf(-p)); }
+// silu(p) or p, in float32.  Kept whole: fused with the rounding to float16 in one form and not in another, the same
+// row would differ by a step of float16 between a prompt's aligned and unaligned rows and its single tokens.
+template <bool SILU>
+__device__ __forceinline__ float activate(float p) {
+  if constexpr (!SILU) return p;
+  float y = p * sigmoid_f(p);
+  asm("" : "+v"(y));
+  return y;
+}
 
 __device__ __forceinline__ int64_t length_of(const ConvArgs& a, int64_t b) {
   return a.lengths == nullptr ? a.T : max_i64(0, min_i64(a.lengths[b], a.T));
@@ -192,7 +205,7 @@ __global__ __launch_bounds__(kThreads) void conv_fwd_kernel(ConvArgs a) {
         float p = bias[i];
 #pragma unroll
         for (int j = 0; j < W; ++j) p = fmaf(w[j][i], win[(u + 1 + j) % W][i], p);
-        y[i] = SILU ? p * sigmoid_f(p) : p;
+        y[i] = activate<SILU>(p);
         if (tb + u >= n) y[i] = 0.f;
       }
       if (tb + u < t1) st_row<E, V>(op + (tb + u) * a.C, y, a.stream != 0);
@@ -344,7 +357,7 @@ __global__ __launch_bounds__(kThreads) void conv_step_kernel(ConvArgs a) {
     float p = bias[i];
 #pragma unroll
     for (int j = 0; j < W; ++j) p = fmaf(w[j][i], win[j][i], p);
-    y[i] = SILU ? p * sigmoid_f(p) : p;
+    y[i] = activate<SILU>(p);
   }
   st_row<E, V>(static_cast<raw*>(a.out) + b * a.C + c, y);
 #pragma unroll
@@ -371,8 +384,8 @@ int check_conv(const ConvArgs& a, int64_t width, int dtype, int w_dtype, const c
   return GRM_HIP_OK;
 }
 
-// Whole 16-byte accesses where every row allows them: 2304 channels of 8 x 2048 bf16 tokens take
-// a tenth of the time that single elements take.
+// Whole 16-byte accesses where every row allows them: 2304 channels of 8 x 2048 bf16 tokens take 30 us so, and
+// 49 us element by element.
 bool whole_rows(const ConvArgs& a, int dtype) {
   const int64_t v = dtype == GRM_HIP_F32 ? 4 : 8;
   return a.C % v == 0 && a.xb % v == 0 && a.xt % v == 0 && aligned(a.x) && aligned(a.state) && aligned(a.out) &&
@@ -407,9 +420,10 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // leaves during it (8 x 2048 tokens of 2304 bf16 channels 38.5 -> 31.7 us; 4 MB outputs the same either way).
 int streams(int64_t elements, int dtype) { return elements * (dtype == GRM_HIP_F32 ? 4 : 2) > (int64_t{32} << 20); }
 
-// The backward's runs: about 3000, one and a half for each of the waves that fit the chip at once (104 us in the case below; 2000: 115, 4000: 109), of 16 tokens
-// at least (three rows of each run's 19 or more are formed twice).  A thread has four channels: with eight, its
-// sums and windows leave two waves a SIMD (8 x 2048 tokens of 2304 bf16 channels: 96 us, with four 62).
+// The backward's runs: about 3000, one and a half for each of the waves that fit the chip at once (8 x 2048 tokens of
+// 2304 bf16 channels, forward and backward: 104 us; 2000 runs: 115, 4000: 109), of 16 tokens at least (three rows of each
+// run's 19 or more are formed twice).  A thread has four channels: with eight, its sums and windows leave two waves a
+// SIMD (the backward kernel 96 us, with four 62).
 int64_t bwd_run(int64_t B, int64_t T, int64_t C, bool vec) {
   const int64_t run = ceil_div(B * T * ceil_div(C, 64 * (vec ? 4 : 1)), 3000);
   return run < 16 ? 16 : run < T ? run : (T > 16 ? T : 16);

@@ -140,7 +140,8 @@ BAD = [
     (dict(dtype=3), capi.EUNSUPPORTED), (dict(steps_dtype=capi.F16), capi.EUNSUPPORTED), (dict(keys=None), capi.EINVAL),
     (dict(rates=None), capi.EINVAL), (dict(memory=FAKE + 4), capi.EINVAL), (dict(keys_token_stride=63), capi.EINVAL),
     (dict(values_token_stride=1 << 22), capi.EUNSUPPORTED), (dict(seq_len=1 << 31), capi.EUNSUPPORTED),
-    (dict(batch=1 << 24), capi.EUNSUPPORTED),
+    (dict(batch=1 << 24), capi.EUNSUPPORTED), (dict(batch=1 << 62), capi.EUNSUPPORTED),
+    (dict(heads=1 << 62, groups=1), capi.EUNSUPPORTED), (dict(value_dim=1 << 62), capi.EUNSUPPORTED),
 ]
 
 
