@@ -551,6 +551,8 @@ int grm_hip_selective_scan_fwd(const grm_hip_selective_args* args, void* hidden,
  * NULL (zeros).  grad_keys, grad_values, grad_queries (dtype) and grad_steps (steps_dtype) are
  * contiguous, the others float32; grad_skip and grad_step_bias may be NULL.  Rows behind a
  * sequence's length get zeros.  The sums over heads, tokens and sequences are taken in a fixed order (no atomics).
+ * An infinity or a NaN in the inputs or gradients may reach every gradient of its block of grm_hip_selective_scan_block()
+ * tokens, and those behind and before it.
  * Workspace: grm_hip_selective_scan_bwd_workspace() bytes, 16-byte aligned.
  */
 int64_t grm_hip_selective_scan_bwd_workspace(int64_t batch, int64_t seq_len, int64_t heads, int64_t value_dim,
