@@ -6,21 +6,19 @@
 //   dq_i = sum_j E_ij d_j W_ij k_j + e^{c_i} S^T dy_i          summed over the heads of a group
 //   dk_j = sum_i E_ij d_j W_ij q_i + d_j e^{c_L - c_j} G^T x_j  likewise
 //   G'   = e^{c_L} G + sum_i e^{c_i} dy_i q_i^T                 the adjoint at the block's start
-// and for the step sizes, with Q_ij = E_ij d_j K_ij W_ij (j < i), t1_i = e^{c_i} q_i . S^T dy_i and
-// t2_j = e^{c_L - c_j} k_j . G^T x_j,
-//   dc_i = sum_j Q_ij - sum_j Q_ji + t1_i - d_i t2_i
-//   dl_t = sum_{s >= t} dc_s + sum_j d_j t2_j + e^{c_L} <G, S>     (l_t = d_t A, the log decay)
+// and for the step sizes, with Q_ij = E_ij d_j K_ij W_ij, t1_i = e^{c_i} q_i . S^T dy_i and t2_j = e^{c_L - c_j} k_j . G^T x_j,
+//   dl_t = sum_{j < t <= i} Q_ij + sum_{i >= t} t1_i + sum_{j < t} d_j t2_j + e^{c_L} <G, S>   (l_t = d_t A, the log decay)
 //   dd_t = A dl_t + sum_i E_it K_it W_it + t2_t,   dA = sum_t d_t dl_t,   dD = sum_t W_tt
 //
 // Steps.  The forward has left S before every block; the reverse walk (selective_pass_kernel)
 // leaves G behind every block, and selective_token_kernel every token's decays; then all blocks run side by
-// side, one workgroup for a block and some of a group's heads, whose dk and dq it sums in registers.  It leaves dc
-// and du . x by token, of which selective_steps_kernel makes the step sizes' gradients, one wave a head and block.
+// side, one workgroup for a block and some of a group's heads, whose dk and dq it sums in registers.  It leaves the
+// sums of Q, t1 and t2 by token, of which selective_steps_kernel makes the step sizes' gradients, one wave a head and block.
 // Where more than one workgroup shares a group, their sums are added in a fixed order by a last
 // kernel: no atomics, the same bits on every run.
 //
-// The step sizes' gradient is a difference of large sums, so its terms stay float32: K and W are sums
-// of exact products, and S and G enter t1 and t2 as two bfloat16 parts (16 bits and more; 2^-17).
+// The step sizes' gradients stay float32: K and W are sums of exact products, and S and G enter t1 and t2 as two
+// bfloat16 parts (16 bits and more; 2^-17).  dl_t is summed without taking large sums off each other (see there).
 // dx, dk and dq are rounded to 16 bits in the end; their weights E K and E d W are rounded once to bfloat16,
 // as is G where it meets k.
 #include <stdint.h>
@@ -36,14 +34,17 @@ constexpr int kGradThreads = 512;
 // floats, step size, e^c, e^{c_L - c}, and decays inside 16-token tiles: from the end of the tile before
 // through the token, and from the token through its tile's end times the step size.
 enum { HI, LO, DD, EC, EE, RB, TD, kPlanes };
+// A head's sums by token that the step sizes' gradients are made of: its row of Q in earlier 16-token tiles, its row less
+// its column inside its own tile, its column in later tiles, t1, d t2, and du . x.
+enum { ROW, TILE, COL, T1, T2, DUX, kSums };
 
 struct GradArgs {
   SelArgs s;              // the forward's inputs; states: S before every block
   const void* dy;         // [B, T, H, P]
   const float* adj;       // [B, nsave, H, P, N]: G behind every block
   float* tokens;          // [B, nsave, H, kPlanes, LB]
-  float* diffs;           // [B, nsave, H * PT, shares, LB, 2]: dc and du . x of each token
-  float* dots;            // [B, nsave, H * PT, 8, 2]: <G, S> and sum W_jj, then [.., 8]: sum d_j t2_j, a part a wave
+  float* diffs;           // [B, nsave, H * PT, shares, kSums, LB]
+  float* dots;            // [B, nsave, H * PT, 8, 2]: <G, S> and sum W_jj, a part a wave
   void* dx;               // [B, T, H, P]
   void* dk;               // [B, T, G, N]
   void* dq;               // [B, T, G, N]
@@ -84,6 +85,11 @@ __device__ __forceinline__ float row_sum(float x) {
 template <int ROT>
 __device__ __forceinline__ float dpp_shl(float x) {
   return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x100 + ROT, 0xf, 0xf, true));
+}
+// x of the lane ROT before in the row, 0 past its start.
+template <int ROT>
+__device__ __forceinline__ float dpp_shr(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x110 + ROT, 0xf, 0xf, true));
 }
 __device__ __forceinline__ float lane_f32(float x, int lane) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
@@ -194,8 +200,42 @@ __global__ __launch_bounds__(256) void selective_token_kernel(GradArgs a) {
   }
 }
 
-// One wave a head and block: the step sizes' gradients from dc, du . x and the states' product,
-//   dl_t = sum_{s >= t} dc_s + end,  dd_t = A dl_t + du_t . x_t,  end = sum_j d_j t2_j + e^{c_L} <G, S>.
+// Sum over the later (earlier) lanes of this lane's group of W, W = 8 or 16: shifted first, so that nothing is taken off again.
+template <int W, int ROT>
+__device__ __forceinline__ float later_lane(float x) {
+  const float y = dpp_shl<ROT>(x);
+  return (lane_id() & (W - 1)) + ROT < W ? y : 0.f;
+}
+template <int W, int ROT>
+__device__ __forceinline__ float earlier_lane(float x) {
+  const float y = dpp_shr<ROT>(x);
+  return (lane_id() & (W - 1)) >= ROT ? y : 0.f;
+}
+template <int W>
+__device__ __forceinline__ float sum_later(float x) {
+  x = later_lane<W, 1>(x);
+  x += later_lane<W, 1>(x);
+  x += later_lane<W, 2>(x);
+  x += later_lane<W, 4>(x);
+  if constexpr (W > 8) x += later_lane<W, 8>(x);
+  return x;
+}
+template <int W>
+__device__ __forceinline__ float sum_earlier(float x) {
+  x = earlier_lane<W, 1>(x);
+  x += earlier_lane<W, 1>(x);
+  x += earlier_lane<W, 2>(x);
+  x += earlier_lane<W, 4>(x);
+  if constexpr (W > 8) x += earlier_lane<W, 8>(x);
+  return x;
+}
+
+// One wave a head and block: the step sizes' gradients, dd_t = A dl_t + du_t . x_t.  dl_t could be summed as rows less
+// columns of Q from t on, but where the decay is strong the pairs across t are few and small, and their sum would drown in
+// the rounding of all later pairs.  So they are taken by where they lie.  Of the pairs (i, j) across token t of tile I
+//   both in I:              rows less columns inside the tile, from t to its end;
+//   i in I, j before it:    rows in earlier tiles, from t to the tile's end;     i behind I, j in it: columns before t;
+//   i behind I, j before:   a difference again, but of the sums over whole tiles of pairs across tiles alone.
 template <class E, int LB, int CS>
 __global__ __launch_bounds__(256) void selective_steps_kernel(GradArgs a) {
   constexpr int PL = LB / 64;
@@ -211,62 +251,74 @@ __global__ __launch_bounds__(256) void selective_steps_kernel(GradArgs a) {
   for (int k = 0; k < PL; ++k) dz[k] = 0.f;
   if (t0 < len) {
     const float* tk = a.tokens + id * kPlanes * LB + lane * PL;
-    float dc[PL], direct[PL], d[PL], gdot = 0.f, tail = 0.f;
+    constexpr int W = 16 / PL, TOK = LB / 16;  // lanes of a tile, tiles
+    float sums[kSums][PL], d[PL], gdot = 0.f;
 #pragma unroll
     for (int k = 0; k < PL; ++k) {
       d[k] = tk[DD * LB + k];
-      dc[k] = direct[k] = 0.f;
+#pragma unroll
+      for (int n = 0; n < kSums; ++n) sums[n][k] = 0.f;
     }
     for (int pt = 0; pt < f.PT; ++pt) {
       const int64_t hp = id * f.PT + pt;
 #pragma unroll
       for (int c = 0; c < CS; ++c) {
 #pragma unroll
-        for (int k = 0; k < PL; ++k) {
-          const float2 v = *reinterpret_cast<const float2*>(a.diffs + ((hp * CS + c) * LB + lane * PL + k) * 2);
-          dc[k] += v.x;
-          direct[k] += v.y;
+        for (int n = 0; n < kSums; ++n) {
+#pragma unroll
+          for (int k = 0; k < PL; ++k) sums[n][k] += a.diffs[((hp * CS + c) * kSums + n) * LB + lane * PL + k];
         }
       }
       const float2 v = *reinterpret_cast<const float2*>(a.dots + (hp * 8 + (lane & 7)) * 2);
       gdot += lane < 8 ? v.x : 0.f;
       dskip += lane < 8 ? v.y : 0.f;
-      // d_j t2_j: the tokens' sums that the workgroups left beside.
-      const float* t2 = a.dots + static_cast<int64_t>(f.B) * f.nsave * f.H * f.PT * 16 + hp * 8;
-      tail += lane < 8 ? t2[lane] : 0.f;
     }
     const float total = lane_f32(tk[HI * LB + PL - 1], 63), rest = lane_f32(tk[LO * LB + PL - 1], 63);
     gdot = group_sum(row_sum(gdot));
     dskip = group_sum(row_sum(dskip));
-    tail = group_sum(row_sum(tail));
-    const float end = fmaf(exp2_f(total) * exp2_f(rest), gdot, tail);
-    float back = 0.f;
+    // From each token to its tile's end (t1 too), and before it in its tile; then a tile's own totals.
+    float rows = 0.f, both = 0.f, t1 = 0.f, cols = 0.f, t2 = 0.f, in_tile[PL];
+#pragma unroll
+    for (int k = 0; k < PL; ++k) {
+      cols += sums[COL][k];
+      t2 += sums[T2][k];
+    }
 #pragma unroll
     for (int k = PL - 1; k >= 0; --k) {
-      back += dc[k];
-      dc[k] = back;  // over this lane's tokens from k on
+      rows += sums[ROW][k];
+      both += sums[TILE][k];
+      t1 += sums[T1][k];
+      in_tile[k] = (rows + both) + t1;
     }
-    // Sums over the lanes behind: inside rows of 16, then the rows behind.
-    float behind = back;
-    behind += dpp_shl<1>(behind);
-    behind += dpp_shl<2>(behind);
-    behind += dpp_shl<4>(behind);
-    behind += dpp_shl<8>(behind);
-    const float r1 = lane_f32(behind, 16), r2 = lane_f32(behind, 32), r3 = lane_f32(behind, 48);
-    behind += lane < 16 ? (r1 + r2) + r3 : lane < 32 ? r2 + r3 : lane < 48 ? r3 : 0.f;
-    behind -= back;
+    const float rows_later = sum_later<W>(rows), both_later = sum_later<W>(both), t1_later = sum_later<W>(t1);
+    const float cols_before = sum_earlier<W>(cols), t2_before = sum_earlier<W>(t2);
+    const float rows_tile = rows + rows_later, t1_tile = t1 + t1_later;       // in a tile's first lane
+    const float cols_tile = cols + cols_before, t2_tile = t2 + t2_before;     // in its last
+    float across = 0.f, others = 0.f, crossing = 0.f;
+#pragma unroll
+    for (int i = 0; i < TOK; ++i) {
+      crossing -= lane_f32(rows_tile, i * W);
+      across = lane / W == i ? crossing : across;
+      crossing += lane_f32(cols_tile, i * W + W - 1);
+      const float behind = lane_f32(t1_tile, i * W), ahead = lane_f32(t2_tile, i * W + W - 1);
+      others += lane / W < i ? behind : lane / W > i ? ahead : 0.f;
+    }
+    const float end = exp2_f(total) * exp2_f(rest) * gdot;
+    const float all = ((rows_later + both_later) + (t1_later + others)) + (across + end);
+    float before = cols_before + t2_before;
     const float rate = f.rates[h];
 #pragma unroll
     for (int k = 0; k < PL; ++k) {
       const int64_t t = t0 + lane * PL + k;
-      const float dl = dc[k] + behind + end;
+      const float dl = in_tile[k] + before + all;
+      before += sums[COL][k] + sums[T2][k];
       if (t < len) {
         float slope = 1.f;
         if (f.softplus) {
           const float z = raw_step<E>(f, b, t, h);
           slope = z > 20.f ? 1.f : __builtin_amdgcn_rcpf(1.f + __expf(-z));
         }
-        dz[k] = fmaf(rate, dl, direct[k]) * slope;
+        dz[k] = fmaf(rate, dl, sums[DUX][k]) * slope;
         da = fmaf(d[k], dl, da);
         db += dz[k];
       }
@@ -386,14 +438,11 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       for (int p = 0; p < PW; ++p) dx[p] = f32x4{0.f, 0.f, 0.f, 0.f};
       Frag8<M> xf[2], yf[2], kf[NK];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        xf[k] = row_frag_t<XT, M>(xt, tile * 16, k * 32, lane);
-        yf[k] = row_frag_t<XT, M>(yt, tile * 16, k * 32, lane);
-      }
+      for (int k = 0; k < 2; ++k) xf[k] = row_frag_t<XT, M>(xt, tile * 16, k * 32, lane);
 #pragma unroll
       for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<KT, M>(kt, tile * 16, kk * 32, lane);
       const float hj = sc[HI * LB + tok], lj = sc[LO * LB + tok], dj = sc[DD * LB + tok];
-      float colsum = 0.f, w_diag = 0.f;
+      float near = 0.f, far = 0.f, kw_diag = 0.f, w_diag = 0.f;
       auto columns = [&](int dp, auto diag) {
         // The second tile past the block is the first again, with weights of zero.
         const int i0 = tile + dp, i1 = i0 + 1 < TOK ? i0 + 1 : i0;
@@ -413,12 +462,13 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
             const f32x4 hv = *reinterpret_cast<const f32x4*>(sc + HI * LB + ti), lv = *reinterpret_cast<const f32x4*>(sc + LO * LB + ti);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const bool in = ti + r >= tok;
+              const bool in = ti + r >= tok, own = ti + r == tok;
               const float e = exp2_f(in ? (hv[r] - hj) + (lv[r] - lj) : -INFINITY), wr = in ? w[u][r] : 0.f;
               ek[u][r] = e * (in ? k2[u][r] : 0.f);
               ew[u][r] = e * dj * wr;
-              colsum = fmaf(ek[u][r], wr, colsum);
-              w_diag += ti + r == tok ? wr : 0.f;
+              near = fmaf(ek[u][r], own ? 0.f : wr, near);
+              kw_diag = fmaf(ek[u][r], own ? wr : 0.f, kw_diag);
+              w_diag += own ? wr : 0.f;
             }
           } else {  // e^{c_i - c_j} through the end of the tile before i's: one exponential a lane, one product a pair
             const bool on = u == 0 || i1 != i0;
@@ -429,7 +479,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
             for (int r = 0; r < 4; ++r) {
               ek[u][r] = rv[r] * c * k2[u][r];
               ew[u][r] = rv[r] * cd * w[u][r];
-              colsum = fmaf(ek[u][r], w[u][r], colsum);
+              far = fmaf(ek[u][r], w[u][r], far);
             }
           }
         }
@@ -446,8 +496,10 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
 
       // Rows i of this wave's tile: dq from the columns j <= i, and the rows' sums.
       const float e_i = sc[EC * LB + tok];
-      float rowsum = 0.f;
+      float row_near = 0.f, row_far = 0.f;
       Frag8<M> qf[NK];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) yf[k] = row_frag_t<XT, M>(yt, tile * 16, k * 32, lane);
 #pragma unroll
       for (int kk = 0; kk < NK; ++kk) qf[kk] = row_frag<KT, M>(qt, tile * 16, kk * 32, lane);
       gr.load(a.adj + sat, pw, f.N, tid);
@@ -472,7 +524,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
             for (int r = 0; r < 4; ++r) {
               const bool in = tj + r <= tok;
               ew[u][r] = exp2_f(in ? (hj - hv[r]) + (lj - lv[r]) : -INFINITY) * (in ? dv[r] * w[u][r] : 0.f);
-              rowsum = fmaf(ew[u][r], in ? k2[u][r] : 0.f, rowsum);
+              row_near = fmaf(ew[u][r], tj + r < tok ? k2[u][r] : 0.f, row_near);
             }
           } else {  // through the end of j's tile
             const bool on = u == 0 || j0 > 0;
@@ -481,7 +533,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               ew[u][r] = c * dv[r] * w[u][r];
-              rowsum = fmaf(ew[u][r], k2[u][r], rowsum);
+              row_far = fmaf(ew[u][r], k2[u][r], row_far);
             }
           }
         }
@@ -494,6 +546,14 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll 1
       for (int dp = 2; dp <= tile; dp += 2) rows(dp, std::false_type{});
       sr.store(st, tid);
+      // What the step sizes' gradients want of this wave's tokens, as soon as it is there.
+      const __amdgpu_buffer_rsrc_t dfr = make_rsrc(a.diffs + (pair * CS + cs) * LB * kSums, LB * kSums * 4);
+      auto by_token = [&](int what, float x) { buf_store1<F32>(dfr, g == 0 ? (what * LB + tok) * 4 : kBufOOB, x); };
+      const bool one = cs == 0;
+      const float nr = group_sum(near), fr = group_sum(far), dux = one ? group_sum(kw_diag) + (nr + fr) : 0.f;
+      by_token(ROW, one ? group_sum(row_far) : 0.f);
+      by_token(TILE, one ? fmaf(-dj, nr, group_sum(row_near)) : 0.f);
+      by_token(COL, one ? dj * fr : 0.f);
       __syncthreads();
 
       // From the state: dq.
@@ -514,6 +574,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
         }
         if (nt & 1) hold_order();
       }
+      by_token(T1, e_i * group_sum(dot1));
       float dot = 0.f;
 #pragma unroll
       for (int i = 0; i < StateLoad<M, NP>::PER; ++i) {
@@ -528,7 +589,9 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       if (hp + 1 < h_hi) ask_rows(hn, pn, tid);
       __syncthreads();
 
-      // From the adjoint: dk and dx.
+      // From the adjoint: dk and dx.  (The values' fragments again: held through the rows they cost spills.)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) xf[k] = row_frag_t<XT, M>(xt, tile * 16, k * 32, lane);
       const float e_t = sc[EE * LB + tok];
       float dot2 = 0.f;
 #pragma unroll
@@ -567,18 +630,13 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
           out4<E>(dxr, dx_at + c, tok < in_block ? pw - c : 0, pvec, o);
         }
       }
-      // What the step sizes' gradients want of this wave's tokens.
-      const float s1 = e_i * group_sum(dot1), s2 = e_t * group_sum(dot2);
-      const float cols = cs == 0 ? group_sum(colsum) : 0.f, rws = cs == 0 ? group_sum(rowsum) : 0.f;
-      const __amdgpu_buffer_rsrc_t dfr = make_rsrc(a.diffs + (pair * CS + cs) * LB * 2, LB * 8);
-      buf_store1<F32>(dfr, g == 0 ? tok * 8 : kBufOOB, (rws - dj * cols) + (s1 - dj * s2));
-      buf_store1<F32>(dfr, g == 0 ? tok * 8 + 4 : kBufOOB, cols + s2);
-      const float tail = row_sum(dj * s2), wsum = group_sum(row_sum(w_diag));
-      const __amdgpu_buffer_rsrc_t dtr = make_rsrc(a.dots + (pair * 8 + wave) * 2, 8),
-                                   tlr = make_rsrc(a.dots + static_cast<int64_t>(f.B) * f.nsave * f.H * f.PT * 16 + pair * 8 + wave, 4);
+      const float s2 = e_t * group_sum(dot2);
+      by_token(T2, dj * s2);
+      by_token(DUX, dux + s2);
+      const float wsum = group_sum(row_sum(w_diag));
+      const __amdgpu_buffer_rsrc_t dtr = make_rsrc(a.dots + (pair * 8 + wave) * 2, 8);
       buf_store1<F32>(dtr, lane == 0 ? 0 : kBufOOB, dot);
       buf_store1<F32>(dtr, lane == 0 ? 4 : kBufOOB, cs == 0 ? wsum : 0.f);
-      buf_store1<F32>(tlr, lane == 0 ? 0 : kBufOOB, tail);
       __syncthreads();
       h = hn;
       pt = pn;
@@ -677,8 +735,8 @@ BwdPlan bwd_plan(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G, int64_t 
   p.part_state = at; at += p.parts > 1 ? up(p.parts * B * state) : 0;
   p.part_log = at; at += p.parts > 1 ? up(p.parts * B * H * 8) : 0;
   p.tokens = at; at += up(B * p.nsave * H * kPlanes * LB * 4);
-  p.diffs = at; at += up(pairs * CS * LB * 8);
-  p.dots = at; at += up(pairs * 24 * 4);
+  p.diffs = at; at += up(pairs * CS * LB * kSums * 4);
+  p.dots = at; at += up(pairs * 16 * 4);
   p.rows = at; at += p.splits > 1 ? up(p.splits * 2 * B * T * G * N * 4) : 0;
   p.heads = at; at += up(B * p.nsave * H * 12);
   p.bytes = at;

@@ -1061,7 +1061,8 @@ def cuda_selective_scan(keys: Tensor, values: Tensor, queries: Tensor, steps: Te
     batch (clamped to [0, T]; the tokens behind are not read, leave the state alone and come out as
     zeros).  The last two dimensions of keys, values and queries are packed; a slice of a wider row is read in
     place.  Returns (hidden [B, T, H, P], memory_out [B, H, P, N] float32).  Differentiable in all
-    but lengths.  Limits: N <= 128."""
+    but lengths.  An infinity or a NaN reaches no earlier token's row; in the backward it may reach any gradient of its
+    sequence.  Limits: N <= 128."""
     if values.is_cuda and _run_native("selective_scan", values.device, enabled=enabled,
                                       debug_fallback=debug_fallback):
         args = (keys, values, queries, steps, _f32(rates), _f32(memory), _f32(skip), _f32(step_bias), lengths,
