@@ -17,8 +17,9 @@
 // Where more than one workgroup shares a group, their sums are added in a fixed order by a last
 // kernel: no atomics, the same bits on every run.
 //
-// The step sizes' gradients stay float32: K and W are sums of exact products, and S and G enter t1 and t2 as two
-// bfloat16 parts (16 bits and more; 2^-17).  dl_t is summed without taking large sums off each other (see there).
+// The step sizes' gradients stay float32: K and W are sums of exact products, and S and G enter t1 and t2 as three
+// bfloat16 parts (24 bits; with two, 2^-17, the sums for the rates and the step bias, which cancel over the tokens, were
+// off by 1.3e-6 of their norm where they are now by 7e-7; forward and backward took 455 us for 480).  dl_t is summed without taking large sums off each other (see there).
 // dx, dk and dq are rounded to 16 bits in the end; their weights E K and E d W are rounded once to bfloat16,
 // as is G where it meets k.
 #include <stdint.h>
@@ -60,9 +61,11 @@ struct GradLds {
   using KT = SelTile<M, NP, true>;          // keys, queries, states: columns, and rows in 16-byte pieces
   using XT = SelTile<M, kSelRows, false>;   // values and their gradients: rows in 8-byte pieces
   static constexpr int LB = S::LB;
-  static constexpr int SPARTS = S::kHalf ? 2 : 1;             // parts of S and G in LDS
+  static constexpr int SPARTS = S::kHalf ? 3 : 1;             // parts of S and G in LDS: two of their own,
   static constexpr int STATE = kSelRows * KT::STRIDE;
-  static constexpr int TILES = LB * (2 * KT::STRIDE + 2 * XT::STRIDE) + SPARTS * STATE;
+  static constexpr int OWN = S::kHalf ? 2 : 1;                 // the third where the values lay
+  static_assert(SPARTS == OWN || STATE <= LB * XT::STRIDE, "the third part's room");
+  static constexpr int TILES = LB * (2 * KT::STRIDE + 2 * XT::STRIDE) + OWN * STATE;
   static constexpr int TOK = LB / 16;                          // token tiles
   static constexpr int CS = 8 / TOK;                           // waves that share one, a share of the columns each
   static constexpr size_t bytes = TILES * sizeof(typename ET<M>::raw) + kPlanes * LB * sizeof(float);
@@ -138,14 +141,16 @@ struct StateLoad {
       }
     }
   }
-  __device__ __forceinline__ void store(typename ET<M>::raw* tile, int tid) const {
-    typename ET<M>::raw* q = tile + KT::at(tid / (NP / 4), tid % (NP / 4) * 4);
+  // Parts FIRST to LAST - 1, part 2 into `third`.
+  template <int FIRST, int LAST>
+  __device__ __forceinline__ void store(typename ET<M>::raw* tile, typename ET<M>::raw* third, int tid) const {
+    const int at = KT::at(tid / (NP / 4), tid % (NP / 4) * 4);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       f32x4 rest = r[i];
 #pragma unroll
-      for (int s = 0; s < PARTS; ++s) {
-        store4_raw<M>(q + i * DROW * KT::STRIDE + s * GradLds<M, NP>::STATE, rest);
+      for (int s = 0; s < PARTS && s < LAST; ++s) {
+        if (s >= FIRST) store4_raw<M>((s == 2 ? third : tile + s * GradLds<M, NP>::STATE) + at + i * DROW * KT::STRIDE, rest);
         if (s + 1 < PARTS) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) rest[e] -= ET<M>::to_f(ET<M>::from_f(rest[e]));
@@ -351,7 +356,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
   raw* xt = qt + LB * KT::STRIDE;
   raw* yt = xt + LB * XT::STRIDE;
   raw* st = yt + LB * XT::STRIDE;
-  float* sc = reinterpret_cast<float*>(st + SP * Lds::STATE);
+  float* sc = reinterpret_cast<float*>(st + Lds::OWN * Lds::STATE);
 
   const SelArgs& f = a.s;
   uint32_t v = xcd_order(blockIdx.x, gridDim.x);
@@ -545,7 +550,9 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       rows(0, std::true_type{});
 #pragma unroll 1
       for (int dp = 2; dp <= tile; dp += 2) rows(dp, std::false_type{});
-      sr.store(st, tid);
+      sr.template store<0, 2>(st, xt, tid);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) xf[k] = row_frag_t<XT, M>(xt, tile * 16, k * 32, lane);
       // What the step sizes' gradients want of this wave's tokens, as soon as it is there.
       const __amdgpu_buffer_rsrc_t dfr = make_rsrc(a.diffs + (pair * CS + cs) * LB * kSums, LB * kSums * 4);
       auto by_token = [&](int what, float x) { buf_store1<F32>(dfr, g == 0 ? (what * LB + tok) * 4 : kBufOOB, x); };
@@ -555,6 +562,10 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       by_token(TILE, one ? fmaf(-dj, nr, group_sum(row_near)) : 0.f);
       by_token(COL, one ? dj * fr : 0.f);
       __syncthreads();
+      if constexpr (SP == 3) {  // the values' fragments are in registers: their room is free
+        sr.template store<2, 3>(st, xt, tid);
+        __syncthreads();
+      }
 
       // From the state: dq.
       float dot1 = 0.f;
@@ -564,7 +575,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
         for (int s = SP - 1; s >= 0; --s) {
 #pragma unroll
-          for (int k = 0; k < 2; ++k) r = mfma8(col_frag<KT, M>(st + s * Lds::STATE, k * 32, (cs * NT + nt) * 16, lane), yf[k], r);
+          for (int k = 0; k < 2; ++k) r = mfma8(col_frag<KT, M>(s == 2 ? xt : st + s * Lds::STATE, k * 32, (cs * NT + nt) * 16, lane), yf[k], r);
         }
         const f32x4 qv = lds_row4<M>(qt + KT::at(tok, (cs * NT + nt) * 16 + 4 * g));
 #pragma unroll
@@ -583,15 +594,13 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       }
       dot = group_sum(row_sum(dot));
       __syncthreads();
-      gr.store(st, tid);
+      gr.template store<0, 3>(st, xt, tid);
       const bool wrap = pt + 1 == f.PT;
       const int hn = h + (wrap ? 1 : 0), pn = wrap ? 0 : pt + 1;
       if (hp + 1 < h_hi) ask_rows(hn, pn, tid);
       __syncthreads();
 
-      // From the adjoint: dk and dx.  (The values' fragments again: held through the rows they cost spills.)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) xf[k] = row_frag_t<XT, M>(xt, tile * 16, k * 32, lane);
+      // From the adjoint: dk and dx.
       const float e_t = sc[EE * LB + tok];
       float dot2 = 0.f;
 #pragma unroll
@@ -600,7 +609,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
         for (int s = SP - 1; s >= 0; --s) {
 #pragma unroll
-          for (int k = 0; k < 2; ++k) r = mfma8(col_frag<KT, M>(st + s * Lds::STATE, k * 32, (cs * NT + nt) * 16, lane), xf[k], r);
+          for (int k = 0; k < 2; ++k) r = mfma8(col_frag<KT, M>(s == 2 ? xt : st + s * Lds::STATE, k * 32, (cs * NT + nt) * 16, lane), xf[k], r);
         }
         const f32x4 kv = lds_row4<M>(kt + KT::at(tok, (cs * NT + nt) * 16 + 4 * g));
 #pragma unroll
