@@ -362,27 +362,6 @@ __device__ __forceinline__ void state_add(f32x4 (&acc)[NT], const float* s, int 
   }
 }
 
-template <int NT>
-__device__ __forceinline__ void state_store(const f32x4 (&acc)[NT], float* s, int p0, int P, int N) {
-  const int lane = lane_id(), p = p0 + (lane & 15);
-  const bool whole = (N & 3) == 0;
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int n = nt * 16 + 4 * (lane >> 4);
-    if (p < P && n < N) {
-      float* q = s + static_cast<int64_t>(p) * N + n;
-      if (whole) {
-        *reinterpret_cast<float4*>(q) = make_float4(acc[nt][0], acc[nt][1], acc[nt][2], acc[nt][3]);
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (n + r < N) q[r] = acc[nt][r];
-        }
-      }
-    }
-  }
-}
-
 // The state's update acc = decay acc + sum_t weight_t x_t[p] k_t^T, 32 tokens at a time.  weight_t x_t is a float32
 // number, kept whole as three bfloat16 parts: the state is carried over thousands of tokens, where a
 // rounding to fewer bits would add up.
@@ -418,6 +397,48 @@ template <class T>
 __device__ __forceinline__ void store_as(T* p, T v, bool stream) {
   if (stream) __builtin_nontemporal_store(v, p);
   else *p = v;
+}
+
+// A lane's tiles hold four columns of one row, 64 bytes of each of 16 rows a store.  Two tiles' halves are exchanged
+// between lanes eight apart first, so that a store covers 128 bytes, a whole line, of each of eight rows (reverse walk of
+// 8 x 2048 tokens x 32 heads 97 -> 84 us, the forward with its states 137 -> 119).
+template <int NT>
+__device__ __forceinline__ void state_store(const f32x4 (&acc)[NT], float* s, int p0, int P, int N) {
+  static_assert(NT % 2 == 0, "tiles in pairs");
+  int lane = lane_id();
+  asm volatile("" : "+v"(lane));  // no address made from it is kept in registers between stores
+  const int p = lane & 15, low = p & 8;
+  if ((N & 3) == 0) {
+    const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(s, static_cast<uint32_t>(P * N * 4));
+#pragma unroll
+    for (int nt = 0; nt < NT; nt += 2) {
+      const int n = nt * 16 + 2 * low + 4 * (lane >> 4);
+      f32x4 v[2];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float give = low ? acc[nt][r] : acc[nt + 1][r];
+        const float take = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(give), 0x128, 0xf, 0xf, true));
+        v[0][r] = low ? take : acc[nt][r];
+        v[1][r] = low ? acc[nt + 1][r] : take;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+        const int row = p0 + 8 * u + (p & 7), at = row < P && n < N ? (row * N + n) * 4 : kBufOOB;
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[u]), rsrc, at, 0, 0);
+      }
+      hold_order();
+    }
+  } else if (p0 + p < P) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int n = nt * 16 + 4 * (lane >> 4) + r;
+        if (n < N) s[static_cast<int64_t>(p0 + p) * N + n] = acc[nt][r];
+      }
+    }
+  }
 }
 
 // Host side: f(E, M, NP, VEC) with one of the compiled forms.

@@ -378,7 +378,7 @@ __global__ __launch_bounds__(kWalkThreads) __attribute__((amdgpu_waves_per_eu(2,
 //   G_{before} = e^{c_L} G + sum_i e^{c_i} dy_i q_i^T,
 // from the gradient of the final state back to the first, G kept at the end of every backward chunk.
 // Waves 0-3 bring the chunks, one in LDS and one on its way; waves 4-7 hold 16 rows of the state each.  (One
-// role for all waves measured 120 us at 8 x 2048 tokens x 32 heads where this takes 96: a state's stores then stand between a load and its use.)
+// role for all waves measured 120 us at 8 x 2048 tokens x 32 heads where this took 96: a state's stores then stand between a load and its use.)
 template <class E, class M, int NP, bool VEC, bool REV, bool LOCAL>
 __global__ __launch_bounds__(kPassThreads) __attribute__((amdgpu_waves_per_eu(2, 4))) void selective_pass_kernel(SelArgs a) {
   using S = SelShape<M>;

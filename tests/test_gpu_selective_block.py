@@ -257,3 +257,30 @@ def test_past_32_bits(dev):
                                              skip=a.skip.abs(), step_bias=a.step_bias, softplus=True)
     assert ((memory - m1).abs() <= 2 * (16 + 160 + 4 * 256) * U * mmag).all()
     assert ((h[:, cut:].float() - h1.float()).abs() <= 2.1 * 2.0 ** -8 * (mag + h1.float().abs())).all()
+
+
+def test_empty_batches(dev):
+    """No sequences: empty results, and the parameters' gradients zeros."""
+    a = Layer(dev, torch.bfloat16, 0, 20, seed=11)
+    names = ("x", "steps", "weight", "bias", "state", "memory", "rates", "skip", "step_bias")
+    for k in names:
+        setattr(a, k, getattr(a, k).detach().requires_grad_())
+    h, state, memory = a(a.x, a.steps, a.state, a.memory)
+    assert h.shape == (0, 20, 4, 32) and state.shape == (0, 3, a.C) and memory.shape == (0, 4, 32, 32)
+    grads = torch.autograd.grad((h, state, memory), [getattr(a, k) for k in names],
+                                [torch.ones_like(t) for t in (h, state, memory)])
+    for k, g in zip(names, grads):
+        assert g.shape == getattr(a, k).shape and not g.any(), k
+    with torch.no_grad():
+        assert a.step(a.x[:, 0], a.steps[:, 0], a.state.clone(), a.memory.clone()).shape == (0, 4, 32)
+
+
+def test_the_torch_forms_on_the_gpu(dev):
+    """``enabled=False``: the PyTorch forms, float32 too, so both within the definition's bound."""
+    a = Layer(dev, torch.float32, 2, 70, seed=12)
+    off = dict(enabled=False, activation="silu")
+    y, s = cuda_ops.cuda_short_conv(a.x, a.weight, a.bias, a.state, **off)
+    h, m = cuda_ops.cuda_selective_scan(*a.split(y), a.steps, a.rates, a.memory, skip=a.skip, step_bias=a.step_bias,
+                                        softplus=True, enabled=False)
+    a.check(h, m)
+    a.check(*a(a.x, a.steps, a.state, a.memory)[::2])
