@@ -30,6 +30,7 @@ from typing import Any, Dict, Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 # The reference's five op schemas (bindings.cpp:6-10) and this library's additions.
 SCHEMA_OPS = (
@@ -901,6 +902,7 @@ class _ShortConvFn(torch.autograd.Function):
         return torch.ops.grm_cuda.short_conv_forward(x, weight, bias, state, lengths, silu)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_out, grad_state_out):
         x, weight, bias, state, lengths = ctx.saved_tensors
         dx, dw, db, ds = torch.ops.grm_cuda.short_conv_backward(grad_out, grad_state_out, x, weight, bias, state,
@@ -919,7 +921,7 @@ def cuda_short_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, st
     [B, width - 1, C] the rows before token 0 (None: zeros), lengths [B] the tokens of each sequence
     of a padded batch (clamped to [0, T]; the rows behind are not read and come out as zeros).
     Returns (out [B, T, C], state_out [B, width - 1, C]: the rows that the next call starts from).
-    Differentiable in x, weight, bias and state."""
+    Differentiable once in x, weight, bias and state."""
     silu = _silu_flag(activation)
     if x.is_cuda and _run_native("short_conv", x.device, enabled=enabled, debug_fallback=debug_fallback):
         if _wants_grad(x, weight, bias, state):
@@ -1033,6 +1035,7 @@ class _SelectiveScanFn(torch.autograd.Function):
         return hidden, memory_out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_hidden, grad_memory_out):
         keys, values, queries, steps, rates, memory, skip, step_bias, lengths, states = ctx.saved_tensors
         dk, dv, dq, ds, dr, dm, dskip, dbias = torch.ops.grm_cuda.selective_scan_backward(
@@ -1060,8 +1063,8 @@ def cuda_selective_scan(keys: Tensor, values: Tensor, queries: Tensor, steps: Te
     before token 0 (used in float32; None: zeros), lengths [B] the tokens of each sequence of a padded
     batch (clamped to [0, T]; the tokens behind are not read, leave the state alone and come out as
     zeros).  The last two dimensions of keys, values and queries are packed; a slice of a wider row is read in
-    place.  Returns (hidden [B, T, H, P], memory_out [B, H, P, N] float32).  Differentiable in all
-    but lengths.  An infinity or a NaN reaches no earlier token's row; in the backward it may reach any gradient of its
+    place.  Returns (hidden [B, T, H, P], memory_out [B, H, P, N] float32).  Differentiable once in
+    all but lengths.  An infinity or a NaN reaches no earlier token's row; in the backward it may reach any gradient of its
     sequence.  Limits: N <= 128."""
     if values.is_cuda and _run_native("selective_scan", values.device, enabled=enabled,
                                       debug_fallback=debug_fallback):

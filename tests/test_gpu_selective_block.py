@@ -284,3 +284,17 @@ def test_the_torch_forms_on_the_gpu(dev):
                                         softplus=True, enabled=False)
     a.check(h, m)
     a.check(*a(a.x, a.steps, a.state, a.memory)[::2])
+
+
+def test_no_second_derivatives(dev):
+    """A gradient of a gradient is refused, not taken as zero."""
+    a = Layer(dev, torch.float32, 1, 9, seed=13)
+    a.x, a.steps = a.x.detach().requires_grad_(), a.steps.detach().requires_grad_()
+    y, _ = cuda_ops.cuda_short_conv(a.x, a.weight, a.bias, a.state, activation="silu")
+    (dx,) = torch.autograd.grad(y.square().sum(), a.x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dx.square().sum(), a.x)
+    h, _ = cuda_ops.cuda_selective_scan(*a.split(y.detach()), a.steps, a.rates, a.memory)
+    (ds,) = torch.autograd.grad(h.square().sum(), a.steps, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(ds.square().sum(), a.steps)
