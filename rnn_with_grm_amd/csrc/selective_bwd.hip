@@ -18,8 +18,8 @@
 // kernel: no atomics, the same bits on every run.
 //
 // The step sizes' gradients stay float32: K and W are sums of exact products, and S and G enter t1 and t2 as three
-// bfloat16 parts (24 bits; with two, 2^-17, the sums for the rates and the step bias, which cancel over the tokens, were
-// off by 1.3e-6 of their norm where they are now by 7e-7, for 25 us of a forward and backward of 450).
+// bfloat16 parts (24 bits; with two, 2^-17, each token's gradient was off by 4.5e-7 where it is now by 1.7e-7, for 25 us of a
+// forward and backward of 455).
 // dl_t is summed without taking large sums off each other (at selective_steps_kernel).
 // dx, dk and dq are rounded to 16 bits in the end; their weights E K and E d W are rounded once to bfloat16,
 // as is G where it meets k.
@@ -37,8 +37,9 @@ constexpr int kGradThreads = 512;
 // through the token, and from the token through its tile's end times the step size.
 enum { HI, LO, DD, EC, EE, RB, TD, kPlanes };
 // A head's sums by token that the step sizes' gradients are made of: its row of Q in earlier 16-token tiles, its row less
-// its column inside its own tile, its column in later tiles, t1, d t2, and du . x.
-enum { ROW, TILE, COL, T1, T2, DUX, kSums };
+// its column inside its own tile, its column in later tiles, its row and its column in tiles that are not next to its
+// own, t1, d t2, and du . x.
+enum { ROW, TILE, COL, FAR_ROW, FAR_COL, T1, T2, DUX, kSums };
 
 struct GradArgs {
   SelArgs s;              // the forward's inputs; states: S before every block
@@ -241,7 +242,9 @@ __device__ __forceinline__ float sum_earlier(float x) {
 // the rounding of all later pairs.  So they are taken by where they lie.  Of the pairs (i, j) across token t of tile I
 //   both in I:              rows less columns inside the tile, from t to its end;
 //   i in I, j before it:    rows in earlier tiles, from t to the tile's end;     i behind I, j in it: columns before t;
-//   i behind I, j before:   a difference again, but of the sums over whole tiles of pairs across tiles alone.
+//   i behind I, j before:   a difference again, but of whole tiles' sums over pairs with a tile between them.
+// (As rows less columns throughout, the sums for the rates and the step bias, which cancel over the tokens, were off by
+// 3.5e-6 of their norm in bf16, 1.4e-6 in float32; now by 3e-7, as float32 operations one by one are.)
 template <class E, int LB, int CS>
 __global__ __launch_bounds__(256) void selective_steps_kernel(GradArgs a) {
   constexpr int PL = LB / 64;
@@ -283,9 +286,11 @@ __global__ __launch_bounds__(256) void selective_steps_kernel(GradArgs a) {
     gdot = group_sum(row_sum(gdot));
     dskip = group_sum(row_sum(dskip));
     // From each token to its tile's end (t1 too), and before it in its tile; then a tile's own totals.
-    float rows = 0.f, both = 0.f, t1 = 0.f, cols = 0.f, t2 = 0.f, in_tile[PL];
+    float rows = 0.f, both = 0.f, t1 = 0.f, cols = 0.f, t2 = 0.f, far_rows = 0.f, far_cols = 0.f, in_tile[PL];
 #pragma unroll
     for (int k = 0; k < PL; ++k) {
+      far_rows += sums[FAR_ROW][k];
+      far_cols += sums[FAR_COL][k];
       cols += sums[COL][k];
       t2 += sums[T2][k];
     }
@@ -298,14 +303,14 @@ __global__ __launch_bounds__(256) void selective_steps_kernel(GradArgs a) {
     }
     const float rows_later = sum_later<W>(rows), both_later = sum_later<W>(both), t1_later = sum_later<W>(t1);
     const float cols_before = sum_earlier<W>(cols), t2_before = sum_earlier<W>(t2);
-    const float rows_tile = rows + rows_later, t1_tile = t1 + t1_later;       // in a tile's first lane
-    const float cols_tile = cols + cols_before, t2_tile = t2 + t2_before;     // in its last
+    const float rows_tile = far_rows + sum_later<W>(far_rows), t1_tile = t1 + t1_later;        // in a tile's first lane
+    const float cols_tile = far_cols + sum_earlier<W>(far_cols), t2_tile = t2 + t2_before;     // in its last
     float across = 0.f, others = 0.f, crossing = 0.f;
 #pragma unroll
     for (int i = 0; i < TOK; ++i) {
-      crossing -= lane_f32(rows_tile, i * W);
+      // Pairs round tile i: those round i - 1, less the rows of i, and the columns of i - 1.
+      if (i > 0) crossing += lane_f32(cols_tile, i * W - 1) - lane_f32(rows_tile, i * W);
       across = lane / W == i ? crossing : across;
-      crossing += lane_f32(cols_tile, i * W + W - 1);
       const float behind = lane_f32(t1_tile, i * W), ahead = lane_f32(t2_tile, i * W + W - 1);
       others += lane / W < i ? behind : lane / W > i ? ahead : 0.f;
     }
@@ -448,7 +453,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
       for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<KT, M>(kt, tile * 16, kk * 32, lane);
       const float hj = sc[HI * LB + tok], lj = sc[LO * LB + tok], dj = sc[DD * LB + tok];
-      float near = 0.f, far = 0.f, kw_diag = 0.f, w_diag = 0.f;
+      float near = 0.f, next = 0.f, far = 0.f, kw_diag = 0.f, w_diag = 0.f;
       auto columns = [&](int dp, auto diag) {
         // The second tile past the block is the first again, with weights of zero.
         const int i0 = tile + dp, i1 = i0 + 1 < TOK ? i0 + 1 : i0;
@@ -485,7 +490,8 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
             for (int r = 0; r < 4; ++r) {
               ek[u][r] = rv[r] * c * k2[u][r];
               ew[u][r] = rv[r] * cd * w[u][r];
-              far = fmaf(ek[u][r], w[u][r], far);
+              float& to = decltype(diag)::value ? next : far;
+              to = fmaf(ek[u][r], w[u][r], to);
             }
           }
         }
@@ -500,9 +506,25 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll 1
       for (int dp = 2; dp < TOK - tile; dp += 2) columns(dp, std::false_type{});
 
+      // What the step sizes' gradients want of this wave's tokens, as soon as it is there: little is held meanwhile.
+      const __amdgpu_buffer_rsrc_t dfr = make_rsrc(a.diffs + (pair * CS + cs) * LB * kSums, LB * kSums * 4);
+      auto by_token = [&](int what, float x) { buf_store1<F32>(dfr, g == 0 ? (what * LB + tok) * 4 : kBufOOB, x); };
+      const __amdgpu_buffer_rsrc_t dtr = make_rsrc(a.dots + (pair * 8 + wave) * 2, 8);
+      const bool one = cs == 0;
+      float near_col, dux;
+      {
+        const float nr = group_sum(near), far_col = group_sum(far), fr = group_sum(next) + far_col;
+        const float wsum = group_sum(row_sum(w_diag));
+        near_col = dj * nr;
+        dux = one ? group_sum(kw_diag) + (nr + fr) : 0.f;
+        by_token(COL, one ? dj * fr : 0.f);
+        by_token(FAR_COL, one ? dj * far_col : 0.f);
+        buf_store1<F32>(dtr, lane == 0 ? 4 : kBufOOB, one ? wsum : 0.f);
+      }
+
       // Rows i of this wave's tile: dq from the columns j <= i, and the rows' sums.
       const float e_i = sc[EC * LB + tok];
-      float row_near = 0.f, row_far = 0.f;
+      float row_near = 0.f, row_next = 0.f, row_far = 0.f;
       Frag8<M> qf[NK];
 #pragma unroll
       for (int k = 0; k < 2; ++k) yf[k] = row_frag_t<XT, M>(yt, tile * 16, k * 32, lane);
@@ -539,7 +561,8 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               ew[u][r] = c * dv[r] * w[u][r];
-              row_far = fmaf(ew[u][r], k2[u][r], row_far);
+              float& to = decltype(diag)::value ? row_next : row_far;
+              to = fmaf(ew[u][r], k2[u][r], to);
             }
           }
         }
@@ -554,14 +577,10 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       sr.template store<0, 2>(st, xt, tid);
 #pragma unroll
       for (int k = 0; k < 2; ++k) xf[k] = row_frag_t<XT, M>(xt, tile * 16, k * 32, lane);
-      // What the step sizes' gradients want of this wave's tokens, as soon as it is there.
-      const __amdgpu_buffer_rsrc_t dfr = make_rsrc(a.diffs + (pair * CS + cs) * LB * kSums, LB * kSums * 4);
-      auto by_token = [&](int what, float x) { buf_store1<F32>(dfr, g == 0 ? (what * LB + tok) * 4 : kBufOOB, x); };
-      const bool one = cs == 0;
-      const float nr = group_sum(near), fr = group_sum(far), dux = one ? group_sum(kw_diag) + (nr + fr) : 0.f;
-      by_token(ROW, one ? group_sum(row_far) : 0.f);
-      by_token(TILE, one ? fmaf(-dj, nr, group_sum(row_near)) : 0.f);
-      by_token(COL, one ? dj * fr : 0.f);
+      const float far_row = group_sum(row_far);
+      by_token(ROW, one ? group_sum(row_next) + far_row : 0.f);
+      by_token(FAR_ROW, one ? far_row : 0.f);
+      by_token(TILE, one ? group_sum(row_near) - near_col : 0.f);
       __syncthreads();
       if constexpr (SP == 3) {  // the values' fragments are in registers: their room is free
         sr.template store<2, 3>(st, xt, tid);
@@ -643,10 +662,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       const float s2 = e_t * group_sum(dot2);
       by_token(T2, dj * s2);
       by_token(DUX, dux + s2);
-      const float wsum = group_sum(row_sum(w_diag));
-      const __amdgpu_buffer_rsrc_t dtr = make_rsrc(a.dots + (pair * 8 + wave) * 2, 8);
       buf_store1<F32>(dtr, lane == 0 ? 0 : kBufOOB, dot);
-      buf_store1<F32>(dtr, lane == 0 ? 4 : kBufOOB, cs == 0 ? wsum : 0.f);
       __syncthreads();
       h = hn;
       pt = pn;
