@@ -244,7 +244,7 @@ __device__ __forceinline__ float sum_earlier(float x) {
 //   i in I, j before it:    rows in earlier tiles, from t to the tile's end;     i behind I, j in it: columns before t;
 //   i behind I, j before:   a difference again, but of whole tiles' sums over pairs with a tile between them.
 // (As rows less columns throughout, the sums for the rates and the step bias, which cancel over the tokens, were off by
-// 3.5e-6 of their norm in bf16, 1.4e-6 in float32; now by 3e-7, as float32 operations one by one are.)
+// 3.5e-6 of their norm in bf16, 1.4e-6 in float32; now by 3e-7.)
 template <class E, int LB, int CS>
 __global__ __launch_bounds__(256) void selective_steps_kernel(GradArgs a) {
   constexpr int PL = LB / 64;
