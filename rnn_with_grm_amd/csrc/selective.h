@@ -253,7 +253,9 @@ struct TileLoad {
   static constexpr int DROW = THREADS / UPR;  // rows between a thread's units
   static_assert(THREADS % UPR == 0 && (UNITS % THREADS == 0 || PER == 1), "a thread's units share a column");
   u32x4 r[PER][W];
-  int off;          // byte offset of this thread's first unit, out of range where its column is
+  // Byte offset of this thread's first unit, out of range where its column is.  Rows past `rows` rely on the range check,
+  // so the rows' steps are added here and not left to the scalar offset, which the check need not see.
+  uint32_t off;
   int at;           // element in the LDS tile
   int step, width;  // bytes from row to row, columns
 
@@ -275,7 +277,7 @@ struct TileLoad {
       for (int i = 0; i < PER; ++i) {
 #pragma unroll
         for (int w = 0; w < W; ++w)
-          r[i][w] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + 16 * w, i * DROW * step, 0);
+          r[i][w] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + static_cast<uint32_t>(i * DROW * step + 16 * w), 0, 0);
       }
     } else {
       const int col = tid % UPR * 8;

@@ -130,10 +130,11 @@ struct StateLoad {
     const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(base, static_cast<uint32_t>((rows < kSelRows ? rows : kSelRows) * N * 4));
     const int row = tid / (NP / 4), n = tid % (NP / 4) * 4;
     if ((N & 3) == 0) {
-      const int off = n < N ? (row * N + n) * 4 : kBufOOB;
+      // (The whole offset in the vector register, where the range check sees it: rows past the state read zeros.)
+      const uint32_t off = n < N ? (row * N + n) * 4 : kBufOOB;
 #pragma unroll
       for (int i = 0; i < PER; ++i)
-        r[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, i * DROW * N * 4, 0));
+        r[i] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, off + static_cast<uint32_t>(i * DROW * N * 4), 0, 0));
     } else {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
