@@ -507,8 +507,9 @@ int grm_hip_short_conv_step(const void* x, const void* weight, const void* bias,
  * are not read, leave the state alone, and their rows of every output are zeros.
  * memory: float32 [batch, heads, value_dim, key_dim], 16-byte aligned, the state before token 0;
  * NULL: zeros.
- * bfloat16 inputs run bf16 MFMA (the float32 state kept whole in its updates, rounded once to bf16 where a
- * query reads it, as are the weights between tokens of a chunk); float16 and float32 inputs run float32 MFMA.
+ * bfloat16 inputs run bf16 MFMA (the float32 state kept whole in its updates; where a query reads it, it and the
+ * weights between tokens of a chunk are two bf16 parts, which lose 2^-16 of a term); float16 and float32 inputs run
+ * float32 MFMA.
  * Limits: key_dim <= 128, heads a multiple of groups, token strides and rows below 2^21 elements.
  */
 typedef struct grm_hip_selective_args {

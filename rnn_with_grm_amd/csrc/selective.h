@@ -226,6 +226,12 @@ __device__ __forceinline__ Frag8<M> pair_frag(f32x4 lo, f32x4 hi) {
   }
 }
 
+// What a rounded part leaves of v: of an infinity the same infinity, so that products with its parts have its sign.
+template <class M>
+__device__ __forceinline__ float part_rest(float v, typename ET<M>::raw part) {
+  return v - __builtin_amdgcn_fmed3f(ET<M>::to_f(part), -3.4028235e38f, 3.4028235e38f);
+}
+
 // Float32 values as PARTS fragments whose sum they are: each the rounded remainder of the ones before.
 template <class M, int PARTS>
 __device__ __forceinline__ void split_frag(const float (&v)[8], Frag8<M> (&out)[PARTS]) {
@@ -236,7 +242,7 @@ __device__ __forceinline__ void split_frag(const float (&v)[8], Frag8<M> (&out)[
   for (int p = 0; p < PARTS; ++p) {
     out[p] = pair_frag<M>(f32x4{rest[0], rest[1], rest[2], rest[3]}, f32x4{rest[4], rest[5], rest[6], rest[7]});
 #pragma unroll
-    for (int e = 0; e < 8; ++e) rest[e] -= ET<M>::to_f(out[p].e[e]);
+    for (int e = 0; e < 8; ++e) rest[e] = part_rest<M>(rest[e], out[p].e[e]);
   }
 }
 

@@ -12,8 +12,8 @@
 // per 128 tokens).  Eight waves in two roles with one barrier a chunk.  In the step of chunk c
 //   waves 0-3  bring chunk c + 2 from memory into the third of three LDS stages, and form the weights
 //              between the tokens of chunk c + 1, e^{c_i - c_j} d_j (q_i . k_j), into one of two LDS tiles;
-//   waves 4-7  hold the state in float32 accumulators, 16 value rows each, which are the operand of the
-//              queries' product as they stand; they write the chunk's outputs and move the state.
+//   waves 4-7  hold the state in float32 accumulators, 16 value rows each, which lie as the queries' product
+//              wants its operand; they write the chunk's outputs and move the state.
 // Where heads are too few to fill 256 CUs, sequences are cut in time: a first launch sums each part's own
 // writes, and each part of the second starts from the combination of the parts before it.
 #include <stdint.h>
@@ -27,16 +27,45 @@ constexpr int kWalkThreads = 512;
 constexpr int kPassThreads = 512;
 constexpr int kMaxParts = 32;
 
+// Weights between a chunk's tokens in LDS: the 16 x 16 tiles on and below the diagonal, each as its lanes hold it, four
+// columns a lane, which is how the product reads it again.  bfloat16 inputs: as two bfloat16 parts, as is the state where a
+// query reads it: 2^-16 of a term is lost, far below the rounding of the output that it is summed into.  (8 x 2048 tokens x
+// 32 heads take 101 us so; with one part, whose 2^-8 of every term is seen in the outputs, they took 90.)
+template <class M>
+struct WeightTile {
+  static constexpr int NIT = SelShape<M>::L / 16, TILES = NIT * (NIT + 1) / 2;
+  static constexpr int PARTS = SelShape<M>::kHalf ? 2 : 1, PART = TILES * 256;
+  using raw = typename ET<M>::raw;
+  __device__ __forceinline__ static int at(int it, int jt, int lane) { return (it * (it + 1) / 2 + jt) * 256 + 4 * lane; }
+  __device__ __forceinline__ static void put(raw* m, int it, int jt, int lane, f32x4 v) {
+#pragma unroll
+    for (int p = 0; p < PARTS; ++p) {
+      store4_raw<M>(m + p * PART + at(it, jt, lane), v);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = part_rest<M>(v[r], ET<M>::from_f(v[r]));
+    }
+  }
+  // Row tile `it`, columns 32 s to 32 s + 31: zeros where they lie in a tile above the diagonal.
+  __device__ __forceinline__ static Frag8<M> frag(const raw* m, int part, int it, int s, int lane) {
+    const raw* p = m + part * PART + at(it, 2 * s, lane);
+    if (2 * s + 1 <= it) return lds_frag_4x2<M>(p, p + 256);
+    Frag8<M> f = {};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f.e[e] = p[e];
+    return f;
+  }
+};
+
 template <class M, int NP>
 struct WalkLds {
   using S = SelShape<M>;
   using KT = SelTile<M, NP, true>;         // keys: columns
   using QT = SelTile<M, NP, false>;        // queries: rows in 8-byte pieces
   using XT = SelTile<M, kSelRows, true>;   // values: columns
-  using MT = SelTile<M, S::L, false>;      // weights between tokens: rows in 8-byte pieces
+  using W4 = WeightTile<M>;                // weights between tokens
   static constexpr int Q0 = S::L * KT::STRIDE, X0 = Q0 + S::L * QT::STRIDE;
   static constexpr int STAGES = 3, STAGE = X0 + S::L * XT::STRIDE;  // a chunk's tiles
-  static constexpr int MIX = S::L * MT::STRIDE;
+  static constexpr int MIX = W4::PARTS * W4::PART;  // a chunk's weights
   static constexpr int SCAL = 5 * S::L + 8;  // hi, lo, d, tail weight, decay; total; whether a value is infinite or NaN, by wave
   static constexpr size_t bytes =
       (STAGES * STAGE + 2 * MIX) * sizeof(typename ET<M>::raw) + STAGES * SCAL * sizeof(float);
@@ -73,6 +102,13 @@ __device__ __forceinline__ void part_start(f32x4 (&acc)[NT], const SelArgs& a, c
   if (a.memory != nullptr) state_add<NT>(acc, a.memory + head * one, p0, a.P, a.N, exp2_d(log));
 }
 
+// Two accumulators of the state as the operand of the queries' product, in the parts that sum up to it.
+template <class M, int PARTS>
+__device__ __forceinline__ void state_frag(f32x4 lo, f32x4 hi, Frag8<M> (&out)[PARTS]) {
+  const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  split_frag<M, PARTS>(v, out);
+}
+
 template <class E, class M, int NP, bool VEC>
 __global__ __launch_bounds__(kWalkThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void selective_walk_kernel(SelArgs a) {
   using S = SelShape<M>;
@@ -82,7 +118,7 @@ __global__ __launch_bounds__(kWalkThreads) __attribute__((amdgpu_waves_per_eu(2,
   using KT = typename Lds::KT;
   using QT = typename Lds::QT;
   using XT = typename Lds::XT;
-  using MT = typename Lds::MT;
+  using W4 = typename Lds::W4;
   constexpr int L = S::L, NT = NP / 16, NK = NP / 32, NIT = L / 16, NS32 = L / 32;
   extern __shared__ __align__(16) unsigned char smem[];
   raw* stage = reinterpret_cast<raw*>(smem);
@@ -182,14 +218,10 @@ __global__ __launch_bounds__(kWalkThreads) __attribute__((amdgpu_waves_per_eu(2,
             const float x = (hi_i - hj[r]) + (lo_i - lj[r]);
             d[r] = (in ? d[r] * dj[r] : 0.f) * exp2_f(in ? x : -INFINITY);
           }
-          // One rounding of the weights to 16 bits, as far from them as the output's own rounding is
-          // from it; the values they meet are exact.
-          store4_raw<M>(m + MT::at(i, j0), d);
+          W4::put(m, it, jt, lane, d);
         }
       }
     };
-    // The tiles behind the diagonal that share a 32-token step with it stay zero.
-    for (int u = tid; u < 2 * Lds::MIX; u += kWalkThreads / 2) mix[u] = 0;
     if (chunks > 0) {
       load();
       put(0);
@@ -240,7 +272,7 @@ __global__ __launch_bounds__(kWalkThreads) __attribute__((amdgpu_waves_per_eu(2,
       }
       // Reads are issued a phase ahead of the products that want them: the weights and the first keys with
       // the state's product, the next chunk's queries with the last of the update.
-      Frag8<M> xf[NS32], sf[NK], mf[NS32][NIT], kf[NT];
+      Frag8<M> xf[NS32], mf[NS32][NIT], kf[NT];
       f32x4 xv[NIT];
       float e[NIT];
 #pragma unroll
@@ -250,49 +282,33 @@ __global__ __launch_bounds__(kWalkThreads) __attribute__((amdgpu_waves_per_eu(2,
       for (int s = 0; s < NS32; ++s) {
         xf[s] = col_frag<XT, M>(xs, 32 * s, rw);
 #pragma unroll
-        for (int it = 2 * s; it < NIT; ++it) mf[s][it] = row_frag_t<MT, M>(m, it * 16, 32 * s);
+        for (int it = 2 * s; it < NIT; ++it) mf[s][it] = W4::frag(m, W4::PARTS - 1, it, s, lane);
       }
-#pragma unroll
-      for (int kk = 0; kk < NK; ++kk) sf[kk] = pair_frag<M>(acc[2 * kk], acc[2 * kk + 1]);
       hold_order();
       f32x4 y[NIT];
 #pragma unroll
       for (int it = 0; it < NIT; ++it) y[it] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int kk = 0; kk < NK; ++kk) {
+        Frag8<M> sf[W4::PARTS];
+        state_frag<M>(acc[2 * kk], acc[2 * kk + 1], sf);
 #pragma unroll
-        for (int it = 0; it < NIT; ++it) y[it] = mfma8(sf[kk], qf[kk][it], y[it]);
+        for (int p = W4::PARTS - 1; p >= 0; --p) {
+#pragma unroll
+          for (int it = 0; it < NIT; ++it) y[it] = mfma8(sf[p], qf[kk][it], y[it]);
+        }
       }
-      key_frags<KT, M, NT>(kf, ks, 0);
-#pragma unroll
-      for (int it = 0; it < NIT; ++it) xv[it] = lds_row4<M>(xs + XT::at(it * 16 + n16, col));
-      f32x4 w0 = *reinterpret_cast<const f32x4*>(sc + 3 * L + 4 * g), w1 = *reinterpret_cast<const f32x4*>(sc + 3 * L + 16 + 4 * g);
-      const float decay = sc[5 * L];
-      hold_order();
-#pragma unroll
-      for (int it = 0; it < NIT; ++it) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) y[it][r] *= e[it];
-      }
-#pragma unroll
-      for (int s = 0; s < NS32; ++s) {
-#pragma unroll
-        for (int it = 2 * s; it < NIT; ++it) y[it] = mfma8(xf[s], mf[s][it], y[it]);
-      }
-      if (__builtin_expect(__any(flags[0] + flags[1] + flags[2] + flags[3] != 0.f), 0)) {
-        // A weight of zero does not keep an infinity or a NaN out of a product: all outputs again, one token i at a
-        // time, with the values of the tokens behind it taken out.  (The lane's number anew: what is made of it here
+      const bool odd = __any(flags[0] + flags[1] + flags[2] + flags[3] != 0.f);
+      if (__builtin_expect(odd, 0)) {
+        // A weight of zero does not keep an infinity or a NaN out of a product: all outputs one token i at a time, with the values of the tokens behind it taken out.  (The lane's number anew: what is made of it here
         // is not to be kept in registers for the case.)
         int ln = lane_id();
         asm volatile("" : "+v"(ln));
 #pragma unroll
         for (int it = 0; it < NIT; ++it) {
-          f32x4 from = {0.f, 0.f, 0.f, 0.f};
+          f32x4 from;
 #pragma unroll
-          for (int kk = 0; kk < NK; ++kk)
-            from = mfma8(pair_frag<M>(acc[2 * kk], acc[2 * kk + 1]), row_frag_t<QT, M>(ks + Lds::Q0, it * 16, kk * 32, ln), from);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) from[r] *= e[it];
+          for (int r = 0; r < 4; ++r) from[r] = y[it][r] * e[it];
 #pragma unroll 1
           for (int k = 0; k < 16; ++k) {
             f32x4 one = from;
@@ -304,10 +320,48 @@ __global__ __launch_bounds__(kWalkThreads) __attribute__((amdgpu_waves_per_eu(2,
                 const int t = 32 * s + 4 * (ln >> 4) + (u < 4 ? u : 12 + u);
                 x.e[u] = t <= it * 16 + k ? x.e[u] : static_cast<raw>(0);
               }
-              one = mfma8(x, mf[s][it], one);
+              one = mfma8(x, W4::frag(m, 0, it, s, ln), one);
+              if constexpr (W4::PARTS == 2) {  // a weight's rest is of either sign or zero: not for an infinity
+#pragma unroll
+                for (int u = 0; u < 8; ++u) x.e[u] = isfinite(ET<M>::to_f(x.e[u])) ? x.e[u] : static_cast<raw>(0);
+                one = mfma8(x, W4::frag(m, 1, it, s, ln), one);
+              }
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) y[it][r] = (ln & 15) == k ? one[r] : y[it][r];
+          }
+        }
+      }
+      key_frags<KT, M, NT>(kf, ks, 0);
+#pragma unroll
+      for (int it = 0; it < NIT; ++it) xv[it] = lds_row4<M>(xs + XT::at(it * 16 + n16, col));
+      f32x4 w0 = *reinterpret_cast<const f32x4*>(sc + 3 * L + 4 * g), w1 = *reinterpret_cast<const f32x4*>(sc + 3 * L + 16 + 4 * g);
+      const float decay = sc[5 * L];
+      Frag8<M> mt[NS32][NIT];  // the weights' first part
+      if constexpr (W4::PARTS == 2) {
+#pragma unroll
+        for (int s = 0; s < NS32; ++s) {
+#pragma unroll
+          for (int it = 2 * s; it < NIT; ++it) mt[s][it] = W4::frag(m, 0, it, s, lane);
+        }
+      }
+      hold_order();
+      if (__builtin_expect(!odd, 1)) {
+#pragma unroll
+        for (int it = 0; it < NIT; ++it) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) y[it][r] *= e[it];
+        }
+#pragma unroll
+        for (int s = 0; s < NS32; ++s) {
+#pragma unroll
+          for (int it = 2 * s; it < NIT; ++it) y[it] = mfma8(xf[s], mf[s][it], y[it]);
+        }
+        if constexpr (W4::PARTS == 2) {
+#pragma unroll
+          for (int s = 0; s < NS32; ++s) {
+#pragma unroll
+            for (int it = 2 * s; it < NIT; ++it) y[it] = mfma8(xf[s], mt[s][it], y[it]);
           }
         }
       }

@@ -1,0 +1,45 @@
+"""How far the selective scan's results are from its float64 definition beyond the outputs' own rounding.
+
+``mag`` is the definition on magnitudes.  bfloat16 inputs: what a query reads of the state and the weights between
+tokens are held as two bfloat16 parts, the second the rounded rest of the first, so 2^-8 * 2^-8 of a term is lost; the
+float32 sums add the steps of the forward's own bound (N + 128 + T / 8 + 32) 2^-24."""
+
+import pytest
+import torch
+
+import selective_oracle as oracle
+from rnn_with_grm_amd import cuda_ops
+from test_gpu_selective_scan import DTYPES, NAMES, U, definition, half, inputs, near, run
+
+pytestmark = pytest.mark.gpu
+PARTS = 2.0 ** -16 * 1.01
+
+
+@pytest.mark.parametrize("B,T,H,P,G,N,lengths", [(2, 200, 4, 64, 2, 128, None), (2, 130, 3, 80, 1, 64, (130, 71)),
+                                                 (1, 70, 2, 5, 1, 7, None), (1, 1100, 1, 64, 1, 96, None)])
+def test_forward(dev, B, T, H, P, G, N, lengths):
+    x = inputs(dev, B, T, H, P, G, N, torch.bfloat16, seed=T)
+    n = None if lengths is None else torch.tensor(lengths, device=dev)
+    hidden, memory = run(x, n)
+    xr = dict(zip(NAMES, oracle.to64(*(x[k] for k in NAMES))))
+    ref, rmem = definition(xr, n, True)
+    mag, mmag = definition(xr, n, True, absolute=True)
+    steps = N + 128 + T / 8 + 32
+    near(hidden, ref, mag, torch.bfloat16, PARTS, steps)
+    near(memory, rmem, mmag, torch.float32, 0, steps)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_an_infinity_stays_one(dev, dtype):
+    """With positive keys and queries an infinite value, or element of the first state, is a sum that is infinite, with
+    its sign, for its row of the state from its token on."""
+    x = inputs(dev, 1, 150, 2, 32, 1, 32, dtype, seed=21)
+    x["keys"], x["queries"], x["values"] = x["keys"].abs() + 0.125, x["queries"].abs() + 0.125, x["values"].clone()
+    x["rates"] = x["rates"].clamp(min=-0.05)  # far from a decay of zero in float32
+    x["values"][0, 20, 1, 5] = float("inf")
+    x["memory"][0, 0, 9, 3] = float("-inf")
+    hidden, memory = run(x)
+    ref, rmem = definition(dict(zip(NAMES, oracle.to64(*(x[k] for k in NAMES)))), None, True)
+    assert int((~torch.isfinite(ref)).sum()) == 130 + 150 and int((~torch.isfinite(rmem)).sum()) == 33
+    for kind in (torch.isposinf, torch.isneginf, torch.isnan):  # (a NaN where a negative skip meets the infinite value)
+        assert torch.equal(kind(hidden).cpu(), kind(ref)) and torch.equal(kind(memory).cpu(), kind(rmem))
