@@ -246,6 +246,13 @@ __device__ __forceinline__ void split_frag(const float (&v)[8], Frag8<M> (&out)[
   }
 }
 
+// Two accumulators as pair_frag, in parts.
+template <class M, int PARTS>
+__device__ __forceinline__ void split_pair(f32x4 lo, f32x4 hi, Frag8<M> (&out)[PARTS]) {
+  const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  split_frag<M, PARTS>(v, out);
+}
+
 // Rows [0, ROWS) x [0, COLS) of a tile from global memory into registers (8 elements a unit, units dealt to
 // THREADS threads), then into LDS as M.  Rows from `rows` on and columns from `cols` on are zeros: they
 // lie outside the buffer resource or are sent there, so no load stands behind a branch and all stay in

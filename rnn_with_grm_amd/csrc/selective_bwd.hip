@@ -21,8 +21,9 @@
 // bfloat16 parts (24 bits; with two, 2^-17, each token's gradient was off by 4.5e-7 where it is now by 1.7e-7, for 25 us of a
 // forward and backward of 455).
 // dl_t is summed without taking large sums off each other (at selective_steps_kernel).
-// dx, dk and dq are rounded to 16 bits in the end; their weights E K and E d W are rounded once to bfloat16,
-// as is G where it meets k.
+// dx, dk and dq are rounded to 16 bits in the end; their weights E K and E d W, and G where it meets k, are two bfloat16
+// parts, which lose 2^-16 of a term (8 x 2048 tokens x 32 heads, forward and backward: 489 us; with one part, whose 2^-8 is
+// seen in the outputs, 458).
 #include <stdint.h>
 
 #include "selective.h"
@@ -356,6 +357,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
   using XT = typename Lds::XT;
   constexpr int LB = S::LB, TOK = Lds::TOK, CS = Lds::CS, SP = Lds::SPARTS;
   constexpr int NK = NP / 32, NT = NP / 16 / CS, PW = kSelRows / 16 / CS;
+  constexpr int WP = Lds::OWN;  // parts of the weights E K and E d W, and of G where it meets k
   constexpr int NPL = (kPlanes * LB + kGradThreads - 1) / kGradThreads;
   extern __shared__ __align__(16) unsigned char smem[];
   raw* kt = reinterpret_cast<raw*>(smem);
@@ -496,12 +498,23 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
             }
           }
         }
-        const Frag8<M> ekf = pair_frag<M>(ek[0], ek[1]), ewf = pair_frag<M>(ew[0], ew[1]);
+        Frag8<M> ekf[WP], ewf[WP];
+        split_pair<M>(ek[0], ek[1], ekf);
 #pragma unroll
-        for (int p = 0; p < PW; ++p) dx[p] = mfma8(col_frag2<XT, M>(yt, i0 * 16, i1 * 16, (cs * PW + p) * 16, lane), ekf, dx[p]);
+        for (int p = 0; p < PW; ++p) {
+          const Frag8<M> yc = col_frag2<XT, M>(yt, i0 * 16, i1 * 16, (cs * PW + p) * 16, lane);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          dk[nt] = mfma8(col_frag2<KT, M>(qt, i0 * 16, i1 * 16, (cs * NT + nt) * 16, lane), ewf, dk[nt]);
+          for (int s = WP - 1; s >= 0; --s) dx[p] = mfma8(yc, ekf[s], dx[p]);
+          if (p & 1) hold_order();
+        }
+        hold_order();
+        split_pair<M>(ew[0], ew[1], ewf);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const Frag8<M> qc = col_frag2<KT, M>(qt, i0 * 16, i1 * 16, (cs * NT + nt) * 16, lane);
+#pragma unroll
+          for (int s = WP - 1; s >= 0; --s) dk[nt] = mfma8(qc, ewf[s], dk[nt]);
+        }
       };
       columns(0, std::true_type{});
 #pragma unroll 1
@@ -567,10 +580,14 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
             }
           }
         }
-        const Frag8<M> ewf = pair_frag<M>(ew[0], ew[1]);
+        Frag8<M> ewf[WP];
+        split_pair<M>(ew[0], ew[1], ewf);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          dq[nt] = mfma8(col_frag2<KT, M>(kt, j0 * 16, j1 * 16, (cs * NT + nt) * 16, lane), ewf, dq[nt]);
+        for (int nt = 0; nt < NT; ++nt) {
+          const Frag8<M> kc = col_frag2<KT, M>(kt, j0 * 16, j1 * 16, (cs * NT + nt) * 16, lane);
+#pragma unroll
+          for (int s = WP - 1; s >= 0; --s) dq[nt] = mfma8(kc, ewf[s], dq[nt]);
+        }
       };
       rows(0, std::true_type{});
 #pragma unroll 1
@@ -651,7 +668,10 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
         for (int p = 0; p < PW; ++p) {
           f32x4 u = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int kk = 0; kk < NK; ++kk) u = mfma8(row_frag<KT, M>(st, (cs * PW + p) * 16, kk * 32, lane), kf[kk], u);
+          for (int s = WP - 1; s >= 0; --s) {
+#pragma unroll
+            for (int kk = 0; kk < NK; ++kk) u = mfma8(row_frag<KT, M>(st + s * Lds::STATE, (cs * PW + p) * 16, kk * 32, lane), kf[kk], u);
+          }
           const int c = (cs * PW + p) * 16 + 4 * g;
           const f32x4 yv = lds_row4<M>(yt + XT::at(tok, c));
           f32x4 o;

@@ -102,13 +102,6 @@ __device__ __forceinline__ void part_start(f32x4 (&acc)[NT], const SelArgs& a, c
   if (a.memory != nullptr) state_add<NT>(acc, a.memory + head * one, p0, a.P, a.N, exp2_d(log));
 }
 
-// Two accumulators of the state as the operand of the queries' product, in the parts that sum up to it.
-template <class M, int PARTS>
-__device__ __forceinline__ void state_frag(f32x4 lo, f32x4 hi, Frag8<M> (&out)[PARTS]) {
-  const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-  split_frag<M, PARTS>(v, out);
-}
-
 template <class E, class M, int NP, bool VEC>
 __global__ __launch_bounds__(kWalkThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void selective_walk_kernel(SelArgs a) {
   using S = SelShape<M>;
@@ -291,7 +284,7 @@ __global__ __launch_bounds__(kWalkThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
       for (int kk = 0; kk < NK; ++kk) {
         Frag8<M> sf[W4::PARTS];
-        state_frag<M>(acc[2 * kk], acc[2 * kk + 1], sf);
+        split_pair<M>(acc[2 * kk], acc[2 * kk + 1], sf);
 #pragma unroll
         for (int p = W4::PARTS - 1; p >= 0; --p) {
 #pragma unroll

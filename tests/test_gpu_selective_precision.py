@@ -9,6 +9,7 @@ import torch
 
 import selective_oracle as oracle
 from rnn_with_grm_amd import cuda_ops
+from test_gpu_selective_bwd import magnitudes
 from test_gpu_selective_scan import DTYPES, NAMES, U, definition, half, inputs, near, run
 
 pytestmark = pytest.mark.gpu
@@ -43,3 +44,28 @@ def test_an_infinity_stays_one(dev, dtype):
     assert int((~torch.isfinite(ref)).sum()) == 130 + 150 and int((~torch.isfinite(rmem)).sum()) == 33
     for kind in (torch.isposinf, torch.isneginf, torch.isnan):  # (a NaN where a negative skip meets the infinite value)
         assert torch.equal(kind(hidden).cpu(), kind(ref)) and torch.equal(kind(memory).cpu(), kind(rmem))
+
+
+@pytest.mark.parametrize("B,T,H,P,G,N,lengths", [(2, 200, 4, 64, 2, 128, None), (2, 130, 3, 80, 1, 64, (130, 71)),
+                                                 (1, 70, 2, 5, 1, 7, None), (1, 1100, 1, 64, 1, 96, None)])
+def test_gradients(dev, B, T, H, P, G, N, lengths):
+    """The weights between tokens and the adjoint are two bfloat16 parts where keys, values and queries get their
+    gradients from them; all else, the states in the step sizes' gradients among it, is float32 to its last bits: the
+    bounds of test_gpu_selective_bwd without a rounding to 16 bits inside."""
+    x = inputs(dev, B, T, H, P, G, N, torch.bfloat16, seed=T + 1)
+    n = None if lengths is None else torch.tensor(lengths, device=dev)
+    leaves = {k: x[k].detach().requires_grad_() for k in NAMES}
+    outs = run(leaves, n)
+    g = torch.Generator().manual_seed(T)
+    dy, dm = torch.randn(outs[0].shape, generator=g).to(torch.bfloat16), torch.randn(outs[1].shape, generator=g)
+    got = torch.autograd.grad(outs, [leaves[k] for k in NAMES], [dy.to(dev), dm.to(dev)])
+    x64 = dict(zip(NAMES, oracle.to64(*(x[k] for k in NAMES), grad=True)))
+    ref = oracle.selective_scan(*(x64[k] for k in NAMES), n, True)
+    want = torch.autograd.grad(ref, [x64[k] for k in NAMES], (dy.double(), dm.double()))
+    mags = magnitudes(x64, n, True, dy.double(), dm.double())
+    steps = N + P + 256 + T / 8 + 64
+    for k, a, b in zip(NAMES, got, want):
+        try:
+            near(a, b, mags[k], a.dtype, PARTS if k in ("keys", "values", "queries") else 0, steps)
+        except AssertionError as e:
+            raise AssertionError(f"gradient of {k}: {e}") from None
