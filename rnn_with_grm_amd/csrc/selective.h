@@ -333,14 +333,16 @@ struct TileLoad {
     }
     return (any & (std::is_same_v<E, F32> ? 0x80000000u : 0x80008000u)) != 0;
   }
-  __device__ __forceinline__ void store(typename ET<M>::raw* tile, int tid) const {
+  // negated: with the other sign (16-bit tiles).
+  __device__ __forceinline__ void store(typename ET<M>::raw* tile, int tid, bool negated = false) const {
     if (UNITS < THREADS && tid >= UNITS) return;
+    const uint32_t flip = sizeof(typename ET<M>::raw) == 2 && negated ? 0x80008000u : 0u;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       typename ET<M>::raw* p = tile + at + i * DROW * T::STRIDE;
       if constexpr (ES == sizeof(typename ET<M>::raw)) {
 #pragma unroll
-        for (int w = 0; w < W; ++w) reinterpret_cast<u32x4*>(p)[w] = r[i][w];
+        for (int w = 0; w < W; ++w) reinterpret_cast<u32x4*>(p)[w] = r[i][w] ^ flip;
       } else {
         const U8<E> e = __builtin_bit_cast(U8<E>, r[i][0]);
 #pragma unroll
@@ -416,9 +418,9 @@ __device__ __forceinline__ void store_as(T* p, T v, bool stream) {
 
 // A lane's tiles hold four columns of one row, 64 bytes of each of 16 rows a store.  Two tiles' halves are exchanged
 // between lanes eight apart first, so that a store covers 128 bytes, a whole line, of each of eight rows (reverse walk of
-// 8 x 2048 tokens x 32 heads 97 -> 84 us, the forward with its states 137 -> 119).
+// 8 x 2048 tokens x 32 heads 97 -> 84 us, the forward with its states 137 -> 119).  `sign`: 1 or -1, a factor.
 template <int NT>
-__device__ __forceinline__ void state_store(const f32x4 (&acc)[NT], float* s, int p0, int P, int N) {
+__device__ __forceinline__ void state_store(const f32x4 (&acc)[NT], float* s, int p0, int P, int N, float sign = 1.f) {
   static_assert(NT % 2 == 0, "tiles in pairs");
   int lane = lane_id();
   asm volatile("" : "+v"(lane));  // no address made from it is kept in registers between stores
@@ -440,7 +442,7 @@ __device__ __forceinline__ void state_store(const f32x4 (&acc)[NT], float* s, in
       for (int u = 0; u < 2; ++u) {
         typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
         const int row = p0 + 8 * u + (p & 7), at = row < P && n < N ? (row * N + n) * 4 : kBufOOB;
-        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[u]), rsrc, at, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[u] * sign), rsrc, at, 0, 0);
       }
       hold_order();
     }
@@ -450,7 +452,7 @@ __device__ __forceinline__ void state_store(const f32x4 (&acc)[NT], float* s, in
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int n = nt * 16 + 4 * (lane >> 4) + r;
-        if (n < N) s[static_cast<int64_t>(p0 + p) * N + n] = acc[nt][r];
+        if (n < N) s[static_cast<int64_t>(p0 + p) * N + n] = sign * acc[nt][r];
       }
     }
   }

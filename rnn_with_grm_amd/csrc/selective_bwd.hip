@@ -145,13 +145,13 @@ struct StateLoad {
       }
     }
   }
-  // Parts FIRST to LAST - 1, part 2 into `third`.
+  // Parts FIRST to LAST - 1 of `sign` (1 or -1) times the state, part 2 into `third`.
   template <int FIRST, int LAST>
-  __device__ __forceinline__ void store(typename ET<M>::raw* tile, typename ET<M>::raw* third, int tid) const {
+  __device__ __forceinline__ void store(typename ET<M>::raw* tile, typename ET<M>::raw* third, int tid, float sign) const {
     const int at = KT::at(tid / (NP / 4), tid % (NP / 4) * 4);
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      f32x4 rest = r[i];
+      f32x4 rest = r[i] * sign;
 #pragma unroll
       for (int s = 0; s < PARTS && s < LAST; ++s) {
         if (s >= FIRST) store4_raw<M>((s == 2 ? third : tile + s * GradLds<M, NP>::STATE) + at + i * DROW * KT::STRIDE, rest);
@@ -246,7 +246,7 @@ __device__ __forceinline__ float sum_earlier(float x) {
 //   i in I, j before it:    rows in earlier tiles, from t to the tile's end;     i behind I, j in it: columns before t;
 //   i behind I, j before:   a difference again, but of whole tiles' sums over pairs with a tile between them.
 // (As rows less columns throughout, the sums for the rates and the step bias, which cancel over the tokens, were off by
-// 3.5e-6 of their norm in bf16, 1.4e-6 in float32; now by 3e-7.)
+// 3.5e-6 of their norm in bf16, 1.4e-6 in float32; now by 1e-7 to 5e-7.)
 template <class E, int LB, int CS>
 __global__ __launch_bounds__(256) void selective_steps_kernel(GradArgs a) {
   constexpr int PL = LB / 64;
@@ -388,6 +388,12 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
   const int64_t blocks = static_cast<int64_t>(b) * f.nsave + blk;
   int h = gi * (f.H / f.G) + h_lo / f.PT, pt = h_lo % f.PT;  // the head and its value tile
 
+  // The bf16 matrix products round a sum down a little more often than up (by 0.3% of their error's spread; the float32 ones do
+  // not).  The step sizes' gradients add up thousands of W and S^T dy and G^T x times keys, queries and values that are mostly
+  // of one sign, and cancel, so that in the sums for `rates` this was what was seen of their error: 7e-7 to 1.6e-6 of their norm, now
+  // 1e-7 to 5e-7.  So in every other block x and S, and with them W, S^T dy and G^T x, carry the other sign.
+  const float sg = S::kHalf && ((b + blk) & 1) ? -1.f : 1.f;
+
   f32x4 dk[NT], dq[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i) dk[i] = dq[i] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -436,7 +442,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       const int64_t sat = ((blocks * f.H + h) * f.P + p0) * f.N;
       const int64_t pair = (blocks * f.H + h) * f.PT + pt;
       xr.at = yr.at = XT::at(tid / (kSelRows / 8), tid % (kSelRows / 8) * 8);
-      xr.store(xt, tid);
+      xr.store(xt, tid, sg < 0.f);
       yr.store(yt, tid);
 #pragma unroll
       for (int i = 0; i < NPL; ++i) {
@@ -455,7 +461,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       for (int k = 0; k < 2; ++k) xf[k] = row_frag_t<XT, M>(xt, tile * 16, k * 32, lane);
 #pragma unroll
       for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<KT, M>(kt, tile * 16, kk * 32, lane);
-      const float hj = sc[HI * LB + tok], lj = sc[LO * LB + tok], dj = sc[DD * LB + tok];
+      const float hj = sc[HI * LB + tok], lj = sc[LO * LB + tok], djs = sg * sc[DD * LB + tok];
       float near = 0.f, next = 0.f, far = 0.f, kw_diag = 0.f, w_diag = 0.f;
       auto columns = [&](int dp, auto diag) {
         // The second tile past the block is the first again, with weights of zero.
@@ -479,7 +485,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
               const bool in = ti + r >= tok, own = ti + r == tok;
               const float e = exp2_f(in ? (hv[r] - hj) + (lv[r] - lj) : -INFINITY), wr = in ? w[u][r] : 0.f;
               ek[u][r] = e * (in ? k2[u][r] : 0.f);
-              ew[u][r] = e * dj * wr;
+              ew[u][r] = e * djs * wr;
               near = fmaf(ek[u][r], own ? 0.f : wr, near);
               kw_diag = fmaf(ek[u][r], own ? wr : 0.f, kw_diag);
               w_diag += own ? wr : 0.f;
@@ -488,7 +494,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
             const bool on = u == 0 || i1 != i0;
             const f32x4 rv = *reinterpret_cast<const f32x4*>(sc + RB * LB + ti);
             const int before = on ? it * 16 - 1 : 0;
-            const float c = on ? exp2_f((sc[HI * LB + before] - hj) + (sc[LO * LB + before] - lj)) : 0.f, cd = c * dj;
+            const float c = on ? exp2_f((sc[HI * LB + before] - hj) + (sc[LO * LB + before] - lj)) : 0.f, cd = c * djs;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               ek[u][r] = rv[r] * c * k2[u][r];
@@ -528,16 +534,16 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       float near_col, dux;
       {
         const float nr = group_sum(near), far_col = group_sum(far), fr = group_sum(next) + far_col;
-        const float wsum = group_sum(row_sum(w_diag));
-        near_col = dj * nr;
-        dux = one ? group_sum(kw_diag) + (nr + fr) : 0.f;
-        by_token(COL, one ? dj * fr : 0.f);
-        by_token(FAR_COL, one ? dj * far_col : 0.f);
+        const float wsum = group_sum(row_sum(sg * w_diag));
+        near_col = djs * nr;
+        dux = one ? sg * (group_sum(kw_diag) + (nr + fr)) : 0.f;
+        by_token(COL, one ? djs * fr : 0.f);
+        by_token(FAR_COL, one ? djs * far_col : 0.f);
         buf_store1<F32>(dtr, lane == 0 ? 4 : kBufOOB, one ? wsum : 0.f);
       }
 
       // Rows i of this wave's tile: dq from the columns j <= i, and the rows' sums.
-      const float e_i = sc[EC * LB + tok];
+      const float e_i = sg * sc[EC * LB + tok];
       float row_near = 0.f, row_next = 0.f, row_far = 0.f;
       Frag8<M> qf[NK];
 #pragma unroll
@@ -565,13 +571,13 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const bool in = tj + r <= tok;
-              ew[u][r] = exp2_f(in ? (hj - hv[r]) + (lj - lv[r]) : -INFINITY) * (in ? dv[r] * w[u][r] : 0.f);
+              ew[u][r] = exp2_f(in ? (hj - hv[r]) + (lj - lv[r]) : -INFINITY) * (in ? sg * dv[r] * w[u][r] : 0.f);
               row_near = fmaf(ew[u][r], tj + r < tok ? k2[u][r] : 0.f, row_near);
             }
           } else {  // through the end of j's tile
             const bool on = u == 0 || j0 > 0;
             const f32x4 dv = *reinterpret_cast<const f32x4*>(sc + TD * LB + tj);
-            const float c = on ? exp2_f((hj - sc[HI * LB + jt * 16 + 15]) + (lj - sc[LO * LB + jt * 16 + 15])) : 0.f;
+            const float c = on ? sg * exp2_f((hj - sc[HI * LB + jt * 16 + 15]) + (lj - sc[LO * LB + jt * 16 + 15])) : 0.f;
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               ew[u][r] = c * dv[r] * w[u][r];
@@ -592,7 +598,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       rows(0, std::true_type{});
 #pragma unroll 1
       for (int dp = 2; dp <= tile; dp += 2) rows(dp, std::false_type{});
-      sr.template store<0, 2>(st, xt, tid);
+      sr.template store<0, 2>(st, xt, tid, sg);
 #pragma unroll
       for (int k = 0; k < 2; ++k) xf[k] = row_frag_t<XT, M>(xt, tile * 16, k * 32, lane);
       const float far_row = group_sum(row_far);
@@ -601,7 +607,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       by_token(TILE, one ? group_sum(row_near) - near_col : 0.f);
       __syncthreads();
       if constexpr (SP == 3) {  // the values' fragments are in registers: their room is free
-        sr.template store<2, 3>(st, xt, tid);
+        sr.template store<2, 3>(st, xt, tid, sg);
         __syncthreads();
       }
 
@@ -632,7 +638,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
       }
       dot = group_sum(row_sum(dot));
       __syncthreads();
-      gr.template store<0, 3>(st, xt, tid);
+      gr.template store<0, 3>(st, xt, tid, 1.f);
       const bool wrap = pt + 1 == f.PT;
       const int hn = h + (wrap ? 1 : 0), pn = wrap ? 0 : pt + 1;
       if (hp + 1 < h_hi) ask_rows(hn, pn, tid);
@@ -653,7 +659,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           dot2 = fmaf(kv[e], r[e], dot2);
-          dk[nt][e] = fmaf(dj * e_t, r[e], dk[nt][e]);
+          dk[nt][e] = fmaf(djs * e_t, r[e], dk[nt][e]);
         }
         if (nt & 1) hold_order();
       }
@@ -664,6 +670,7 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
         const int dx_at = tok * static_cast<int>(wide);
 #pragma unroll
         for (int kk = 0; kk < NK; ++kk) kf[kk] = row_frag<KT, M>(kt, tile * 16, kk * 32, lane);
+        const float dj = sg * djs;
 #pragma unroll
         for (int p = 0; p < PW; ++p) {
           f32x4 u = {0.f, 0.f, 0.f, 0.f};
@@ -680,8 +687,8 @@ __global__ __launch_bounds__(kGradThreads) __attribute__((amdgpu_waves_per_eu(2,
           out4<E>(dxr, dx_at + c, tok < in_block ? pw - c : 0, pvec, o);
         }
       }
-      const float s2 = e_t * group_sum(dot2);
-      by_token(T2, dj * s2);
+      const float s2 = sg * e_t * group_sum(dot2);
+      by_token(T2, sg * djs * s2);
       by_token(DUX, dux + s2);
       buf_store1<F32>(dtr, lane == 0 ? 0 : kBufOOB, dot);
       __syncthreads();

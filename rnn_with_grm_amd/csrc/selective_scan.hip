@@ -434,6 +434,9 @@ __global__ __launch_bounds__(kPassThreads) __attribute__((amdgpu_waves_per_eu(2,
   using KT = SelTile<M, NP, true>;
   using XT = SelTile<M, kSelRows, true>;
   constexpr int L = S::L, NT = NP / 16, X0 = L * KT::STRIDE, STAGE = X0 + L * XT::STRIDE, SCAL = L + 4;
+  // The adjoint of bfloat16 inputs changes its sign from chunk to chunk, against the bf16 products' leaning to one side (see
+  // selective_grad_kernel): it meets keys and values that are mostly of one sign in the step sizes' gradients.
+  constexpr bool TURN = REV && S::kHalf;
   extern __shared__ __align__(16) unsigned char smem[];
   raw* stage = reinterpret_cast<raw*>(smem);
   float* scal = reinterpret_cast<float*>(stage + 2 * STAGE);
@@ -474,8 +477,8 @@ __global__ __launch_bounds__(kPassThreads) __attribute__((amdgpu_waves_per_eu(2,
       if (wave == kStepWave) {
         const TokenScalars t = token_scalars<L>(a, step_value<E>(a, z) + bias, chunk_of(i) * L + lane < live, rate);
         float* o = scal + (i & 1) * SCAL;
-        if (lane < L) o[lane] = REV ? exp2_d(t.cum) : t.d * exp2_d(t.total - t.cum);
-        if (lane == 0) o[L] = exp2_d(t.total);
+        if (lane < L) o[lane] = REV ? (TURN && !(i & 1) ? -1.f : 1.f) * exp2_d(t.cum) : t.d * exp2_d(t.total - t.cum);
+        if (lane == 0) o[L] = (TURN ? -1.f : 1.f) * exp2_d(t.total);
         log += t.total;
       }
     };
@@ -508,7 +511,8 @@ __global__ __launch_bounds__(kPassThreads) __attribute__((amdgpu_waves_per_eu(2,
       if (REV && !LOCAL) {
         const int64_t t = t_first + static_cast<int64_t>(chunk_of(i)) * L;
         if (i == 0 || (t + L) % S::LB == 0)
-          state_store<NT>(acc, a.states + ((w.b * a.nsave + t / S::LB) * a.H + w.h) * a.P * a.N, sp, a.P, a.N);
+          state_store<NT>(acc, a.states + ((w.b * a.nsave + t / S::LB) * a.H + w.h) * a.P * a.N, sp, a.P, a.N,
+                          TURN && (i & 1) ? -1.f : 1.f);
       }
       const float decay = sc[L];
 #pragma unroll
@@ -525,8 +529,9 @@ __global__ __launch_bounds__(kPassThreads) __attribute__((amdgpu_waves_per_eu(2,
       }
       __syncthreads();
     }
-    if (LOCAL) state_store<NT>(acc, a.part_state + slot * one, sp, a.P, a.N);
-    else if (w.part == 0) state_store<NT>(acc, a.memory_out + head * one, sp, a.P, a.N);
+    const float sign = TURN && (chunks & 1) ? -1.f : 1.f;
+    if (LOCAL) state_store<NT>(acc, a.part_state + slot * one, sp, a.P, a.N, sign);
+    else if (w.part == 0) state_store<NT>(acc, a.memory_out + head * one, sp, a.P, a.N, sign);
   }
 }
 
