@@ -1029,19 +1029,20 @@ class _SelectiveScanFn(torch.autograd.Function):
     def forward(ctx, keys, values, queries, steps, rates, memory, skip, step_bias, lengths, softplus: bool):
         hidden, memory_out, states = torch.ops.grm_cuda.selective_scan_forward(
             keys, values, queries, steps, rates, memory, skip, step_bias, lengths, softplus, True)
-        ctx.softplus = softplus
-        ctx.save_for_backward(keys, values, queries, steps, rates, memory, skip, step_bias, lengths, states)
+        ctx.softplus, ctx.has_memory = softplus, memory is not None
+        # (Not the first state: the backward does not read it, and a caller may move it in place.)
+        ctx.save_for_backward(keys, values, queries, steps, rates, skip, step_bias, lengths, states)
         ctx.set_materialize_grads(False)
         return hidden, memory_out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_hidden, grad_memory_out):
-        keys, values, queries, steps, rates, memory, skip, step_bias, lengths, states = ctx.saved_tensors
+        keys, values, queries, steps, rates, skip, step_bias, lengths, states = ctx.saved_tensors
         dk, dv, dq, ds, dr, dm, dskip, dbias = torch.ops.grm_cuda.selective_scan_backward(
             grad_hidden, grad_memory_out, keys, values, queries, steps, rates, skip, step_bias, lengths, states,
             ctx.softplus)
-        return (dk, dv, dq, ds, dr, None if memory is None else dm, None if skip is None else dskip,
+        return (dk, dv, dq, ds, dr, dm if ctx.has_memory else None, None if skip is None else dskip,
                 None if step_bias is None else dbias, None, None)
 
 
