@@ -44,6 +44,9 @@ void check_device(const Tensor& t, const Tensor& like, const char* op, const cha
   TORCH_CHECK_VALUE(t.is_cuda() && t.device() == like.device(), op, ": ", name, " must be on ", like.device());
 }
 
+// Autograd's count of writes to an argument: a graph that saved it for its backward then refuses to use what it holds now.
+void written(Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
+
 // A contiguous optional tensor's pointer; `keep` holds what it points into.
 void* opt_ptr(const OptTensor& t, Tensor& keep) {
   if (!has(t)) return nullptr;
@@ -181,6 +184,7 @@ Tensor short_conv_step_out(const Tensor& x, const Tensor& state, const Tensor& w
                                    state_out.data_ptr(), c.B, c.C, c.W, stride_of(xr, 0, c.C), c.dtype, c.w_dtype,
                                    silu, stream_of(x)),
            op);
+  written(state_out);
   return out;
 }
 
@@ -355,6 +359,7 @@ Tensor selective_step_out(const Tensor& keys, const Tensor& values, const Tensor
                     op, ": memory_out must be contiguous, 16-byte aligned and match memory");
   Tensor hidden = at::empty({s.B, s.H, s.P}, values.options());
   check_rc(grm_hip_selective_step(&s.args, hidden.data_ptr(), memory_out.data_ptr<float>(), stream_of(values)), op);
+  written(memory_out);
   return hidden;
 }
 

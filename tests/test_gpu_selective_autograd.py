@@ -19,3 +19,36 @@ def test_the_first_state_may_be_moved_before_the_backward(dev):
     leaves["memory"].copy_(memory.detach())
     got = torch.autograd.grad(hidden.sum(), [leaves[k] for k in names])
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def step_args(x):
+    return [x[k][:, 0] for k in ("keys", "values", "queries", "steps")] + [x["rates"]]
+
+
+def test_steps_in_place_count_as_writes(dev):
+    """A state that a graph has saved for its backward and a single token has moved since: the backward is refused, as
+    after any write in place, and not computed from the moved state."""
+    g = torch.Generator().manual_seed(3)
+    x, w, state = (torch.randn(*s, generator=g).to(dev) for s in ((2, 9, 8), (8, 4), (2, 3, 8)))
+    w.requires_grad_()
+    out, _ = cuda_ops.cuda_short_conv(x, w, None, state)
+    with torch.no_grad():
+        cuda_ops.cuda_short_conv_step(x[:, 0], state, w, state_out=state)
+    assert state._version == 1
+    with pytest.raises(RuntimeError, match="inplace"):
+        out.sum().backward()
+    a = inputs(dev, 2, 1, 2, 16, 1, 16, torch.float32, seed=4)
+    leaf = torch.ones_like(a["memory"], requires_grad=True)
+    product = (leaf * a["memory"]).sum()  # saves the state
+    cuda_ops.cuda_selective_step(*step_args(a), a["memory"], memory_out=a["memory"])
+    assert a["memory"]._version == 1
+    with pytest.raises(RuntimeError, match="inplace"):
+        product.backward()
+
+
+def test_steps_in_place_in_inference_mode(dev):
+    with torch.inference_mode():
+        a = inputs(dev, 2, 1, 2, 16, 1, 16, torch.float32, seed=4)
+        want = cuda_ops.cuda_selective_step(*step_args(a), a["memory"])
+        got = cuda_ops.cuda_selective_step(*step_args(a), a["memory"], memory_out=a["memory"])
+    assert all(torch.equal(u, v) for u, v in zip(got, want)) and got[1] is a["memory"]
