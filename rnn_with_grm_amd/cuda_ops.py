@@ -30,6 +30,7 @@ from typing import Any, Dict, Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 # The reference's five op schemas (bindings.cpp:6-10) and this library's additions.
@@ -839,8 +840,16 @@ def cuda_linear_residual_layer_norm(x: Tensor, weight: Tensor, bias: Optional[Te
 # Selective state scan and its short causal convolution.  The reference has neither; the scan is the
 # linear memory above with a decay and a write strength that each token chooses per head.
 
+def _has_tangent(*tensors: Optional[Tensor]) -> bool:
+    """Whether a forward-mode derivative is asked for (torch.autograd.forward_ad, torch.func.jvp): the native ops
+    alone would drop it, while an autograd function without one refuses the call."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def _wants_grad(*tensors: Optional[Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors) or
+            _has_tangent(*tensors))
 
 
 def _live_tokens(lengths: Optional[Tensor], batch: int, seq_len: int, device) -> Optional[Tensor]:
@@ -921,7 +930,7 @@ def cuda_short_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, st
     [B, width - 1, C] the rows before token 0 (None: zeros), lengths [B] the tokens of each sequence
     of a padded batch (clamped to [0, T]; the rows behind are not read and come out as zeros).
     Returns (out [B, T, C], state_out [B, width - 1, C]: the rows that the next call starts from).
-    Differentiable once in x, weight, bias and state."""
+    Differentiable once, backwards, in x, weight, bias and state (forward-mode derivatives are refused on the GPU)."""
     silu = _silu_flag(activation)
     if x.is_cuda and _run_native("short_conv", x.device, enabled=enabled, debug_fallback=debug_fallback):
         if _wants_grad(x, weight, bias, state):
@@ -1064,8 +1073,8 @@ def cuda_selective_scan(keys: Tensor, values: Tensor, queries: Tensor, steps: Te
     before token 0 (used in float32; None: zeros), lengths [B] the tokens of each sequence of a padded
     batch (clamped to [0, T]; the tokens behind are not read, leave the state alone and come out as
     zeros).  The last two dimensions of keys, values and queries are packed; a slice of a wider row is read in
-    place.  Returns (hidden [B, T, H, P], memory_out [B, H, P, N] float32).  Differentiable once in
-    all but lengths.  An infinity or a NaN reaches no earlier token's row; in the backward it may reach any gradient of its
+    place.  Returns (hidden [B, T, H, P], memory_out [B, H, P, N] float32).  Differentiable once,
+    backwards, in all but lengths (forward-mode derivatives are refused on the GPU).  An infinity or a NaN reaches no earlier token's row; in the backward it may reach any gradient of its
     sequence.  Limits: N <= 128."""
     if values.is_cuda and _run_native("selective_scan", values.device, enabled=enabled,
                                       debug_fallback=debug_fallback):

@@ -52,3 +52,33 @@ def test_steps_in_place_in_inference_mode(dev):
         want = cuda_ops.cuda_selective_step(*step_args(a), a["memory"])
         got = cuda_ops.cuda_selective_step(*step_args(a), a["memory"], memory_out=a["memory"])
     assert all(torch.equal(u, v) for u, v in zip(got, want)) and got[1] is a["memory"]
+
+
+@pytest.mark.parametrize("grad_enabled", [True, False])
+def test_no_forward_derivatives(dev, grad_enabled):
+    """A tangent is refused, not dropped; the PyTorch forms carry it."""
+    x = inputs(dev, 2, 5, 2, 16, 1, 16, torch.float32, seed=5)
+    c, w, state = torch.randn(2, 5, 8, device=dev), torch.randn(8, 4, device=dev), torch.randn(2, 3, 8, device=dev)
+    calls = {
+        "conv": (lambda t, **k: cuda_ops.cuda_short_conv(t, w, None, state, **k)[0], c),
+        "conv_step": (lambda t, **k: cuda_ops.cuda_short_conv_step(c[:, 0], t, w, **k)[1], state),
+        "scan": (lambda t, **k: cuda_ops.cuda_selective_scan(x["keys"], x["values"], x["queries"], x["steps"], t, **k)[0],
+                 x["rates"]),
+        "step": (lambda t, **k: cuda_ops.cuda_selective_step(*step_args(x), t, **k)[0], x["memory"]),
+    }
+    with torch.set_grad_enabled(grad_enabled):
+        for name, (f, t) in calls.items():
+            tangent = torch.randn_like(t)
+            for mode in (lambda g: torch.func.jvp(g, (t,), (tangent,)), lambda g: forward(g, t, tangent)):
+                with pytest.raises((RuntimeError, NotImplementedError)):
+                    mode(f)
+            out, moved = torch.func.jvp(lambda v: f(v, enabled=False), (t,), (tangent,))
+            plain = (f(t + 0.01 * tangent, enabled=False) - f(t - 0.01 * tangent, enabled=False)) / 0.02
+            assert (moved - plain).norm() <= 0.02 * plain.norm(), name  # differences over 0.01 of a tangent of order 1
+            with torch.no_grad():
+                assert torch.isfinite(f(t)).all()  # and without one the kernels run
+
+
+def forward(g, t, tangent):
+    with torch.autograd.forward_ad.dual_level():
+        return g(torch.autograd.forward_ad.make_dual(t, tangent))
