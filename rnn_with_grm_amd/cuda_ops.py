@@ -443,6 +443,18 @@ class _RetrieveFuseFn(torch.autograd.Function):
         return None, None, dq, dg, dh, dw, db, None
 
 
+def _has_tangent(*tensors: Optional[Tensor]) -> bool:
+    """Whether a forward-mode derivative is asked for (torch.autograd.forward_ad, torch.func.jvp): the native ops
+    alone would drop it, while an autograd function without one refuses the call."""
+    return forward_ad._current_level >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def _wants_grad(*tensors: Optional[Tensor]) -> bool:
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors) or
+            _has_tangent(*tensors))
+
+
 # ---------------------------------------------------------------------------
 # Entry points (the reference's cuda_ops.py:347-402, then this library's own).
 
@@ -562,7 +574,7 @@ def cuda_gather_apply(memories_per_batch: Tensor, topk_indices: Tensor, queries:
     Under autograd, when only the queries need a gradient (a detached archive, as in the
     models) the native op runs with the transposed apply as its backward; when the memories
     need one too, the composition runs."""
-    needs_grad = torch.is_grad_enabled() and (memories_per_batch.requires_grad or queries.requires_grad)
+    needs_grad = _wants_grad(memories_per_batch, queries)
     native = _run_native("gather_apply", memories_per_batch.device, enabled=enabled, debug_fallback=debug_fallback)
     if native and not needs_grad:
         return torch.ops.grm_cuda.gather_apply(memories_per_batch, topk_indices, queries, dtype)
@@ -586,8 +598,7 @@ def cuda_retrieve_fuse(memories_per_batch: Tensor, topk_indices: Tensor, queries
     under autograd (queries, gates, h or the LayerNorm parameters; a detached archive) the
     native _RetrieveFuseFn runs with float32 rows and keeps only [B, Q, H] for its backward.
     Memories that need a gradient take the torch composition."""
-    needs_grad = torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in (memories_per_batch, queries, gates, h_online, weight, bias))
+    needs_grad = _wants_grad(memories_per_batch, queries, gates, h_online, weight, bias)
     native = _run_native("retrieve_fuse", h_online.device, enabled=enabled, debug_fallback=debug_fallback)
     if native and not needs_grad:
         return torch.ops.grm_cuda.retrieve_fuse(memories_per_batch, topk_indices, queries, gates, h_online, weight,
@@ -667,7 +678,7 @@ def cuda_project_split(proj: Tensor, key_dim: int, value_dim: int, extra_dim: in
     F.normalize'd (paper_grm.py:491-493; the extra part is the gating query projection,
     paper_grm.py:570-574).  Inference only: under autograd the split views and
     F.normalize run."""
-    if not (torch.is_grad_enabled() and proj.requires_grad) and _run_native(
+    if not _wants_grad(proj) and _run_native(
             "project_split", proj.device, enabled=enabled, debug_fallback=debug_fallback):
         k, v, q, e = torch.ops.grm_cuda.project_split(proj, int(key_dim), int(value_dim), int(extra_dim), float(eps))
         return (k, v, q) + ((e,) if extra_dim else ())
@@ -743,8 +754,7 @@ def cuda_project_gemm(x: Tensor, weight: Tensor, bias: Optional[Tensor], key_dim
     split and the keys' and queries' L2 normalisation as its epilogue (paper_grm.py:491-493,
     570-574).  Under autograd, 16-bit inputs take _ProjectGemmFn (the fused forward, a native
     backward on library GEMMs); other dtypes F.linear and cuda_project_split."""
-    needs_grad = torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in (x, weight, bias))
+    needs_grad = _wants_grad(x, weight, bias)
     if _run_native("project_gemm", x.device, enabled=enabled, debug_fallback=debug_fallback):
         if not needs_grad:
             k, v, q, e = torch.ops.grm_cuda.project_gemm(x, weight, bias, int(key_dim), int(value_dim),
@@ -763,8 +773,7 @@ def cuda_residual_layer_norm(x: Tensor, residual: Tensor, weight: Optional[Tenso
                              debug_fallback: bool = False) -> Tensor:
     """layer_norm(x + residual) (multilayer_grm.py:92-97).  Inference only: under autograd
     the add and torch's layer_norm run."""
-    needs_grad = torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in (x, residual, weight, bias))
+    needs_grad = _wants_grad(x, residual, weight, bias)
     if not needs_grad and _run_native("residual_layer_norm", x.device, enabled=enabled,
                                       debug_fallback=debug_fallback):
         return torch.ops.grm_cuda.residual_layer_norm(x, residual, weight, bias, float(eps))
@@ -824,8 +833,7 @@ def cuda_linear_residual_layer_norm(x: Tensor, weight: Tensor, bias: Optional[Te
     (paper_grm.py:709) and the block output (multilayer_grm.py:92-97) as one GEMM whose epilogue
     is the residual add and the LayerNorm.  Under autograd, 16-bit inputs take
     _LinearResidualLayerNormFn; other dtypes the torch composition."""
-    needs_grad = torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in (x, weight, bias, residual, ln_weight, ln_bias))
+    needs_grad = _wants_grad(x, weight, bias, residual, ln_weight, ln_bias)
     if _run_native("linear_residual_layer_norm", x.device, enabled=enabled, debug_fallback=debug_fallback):
         if not needs_grad:
             return torch.ops.grm_cuda.linear_residual_layer_norm(x, weight, bias, residual, ln_weight, ln_bias,
@@ -839,18 +847,6 @@ def cuda_linear_residual_layer_norm(x: Tensor, weight: Tensor, bias: Optional[Te
 # ---------------------------------------------------------------------------
 # Selective state scan and its short causal convolution.  The reference has neither; the scan is the
 # linear memory above with a decay and a write strength that each token chooses per head.
-
-def _has_tangent(*tensors: Optional[Tensor]) -> bool:
-    """Whether a forward-mode derivative is asked for (torch.autograd.forward_ad, torch.func.jvp): the native ops
-    alone would drop it, while an autograd function without one refuses the call."""
-    return forward_ad._current_level >= 0 and any(
-        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
-
-
-def _wants_grad(*tensors: Optional[Tensor]) -> bool:
-    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors) or
-            _has_tangent(*tensors))
-
 
 def _live_tokens(lengths: Optional[Tensor], batch: int, seq_len: int, device) -> Optional[Tensor]:
     """[B, T] bool, the tokens before each sequence's length; None without lengths."""
