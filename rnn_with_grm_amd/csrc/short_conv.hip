@@ -276,11 +276,13 @@ __global__ __launch_bounds__(kThreads) void conv_bwd_kernel(ConvArgs a) {
                 gv[i] *= sg * fmaf(p, 1.f - sg, 1.f);
               }
               if (!INNER && t >= n) gv[i] = 0.f;
-              const float gw = INNER || t < t1 ? gv[i] : 0.f;  // the rows past the run are another one's
-              db[i] += gw;
+              // The rows past the run are another one's, those past the length nobody's.  They are kept out of the
+              // products too: an infinity that the window still holds would make a NaN of a gradient of zero.
+              const bool own = INNER || (t < t1 && t < n);
+              db[i] += own ? gv[i] : 0.f;
 #pragma unroll
               for (int j = 0; j < W; ++j) {
-                dw[j][i] = fmaf(gw, win[(u + 1 + j) % W][i], dw[j][i]);
+                dw[j][i] = own ? fmaf(gv[i], win[(u + 1 + j) % W][i], dw[j][i]) : dw[j][i];
                 dx[i] = fmaf(w[j][i], g[(u + W - j) % W][i], dx[i]);
               }
               if (!INNER && s >= n) dx[i] = 0.f;

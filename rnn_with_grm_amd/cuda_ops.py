@@ -884,7 +884,10 @@ def _torch_short_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor], state: 
         xf = xf.masked_fill(~live[..., None], 0.0)
     before = xf.new_zeros(B, W - 1, C) if state is None else state.to(cdt)
     full = torch.cat([before, xf], 1)
-    pre = sum(full[:, w:w + T] * wf[:, w] for w in range(W))
+    rows = [full[:, w:w + T] for w in range(W)]
+    if live is not None:  # a dead token's window holds live rows, whose infinities times a gradient of zero would be NaN
+        rows = [r.masked_fill(~live[..., None], 0.0) for r in rows]
+    pre = sum(r * wf[:, w] for w, r in enumerate(rows))
     if bias is not None:
         pre = pre + bias.to(cdt)
     out = torch.nn.functional.silu(pre) if silu else pre
