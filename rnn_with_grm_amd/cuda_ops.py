@@ -989,6 +989,26 @@ def _check_selective(keys: Tensor, values: Tensor, queries: Tensor, steps: Tenso
         raise ValueError("selective_scan: memory must be [batch, heads, value_dim, key_dim]")
 
 
+def _lower_product(weights: Tensor, x: Tensor, lower: Tensor) -> Tensor:
+    """``weights @ x`` of a lower triangular matrix whose zeros above the diagonal keep infinities and NaN of x out,
+    as a sum over j <= i does: those are counted apart."""
+    odd = ~torch.isfinite(x)
+    try:
+        if not x.is_cuda and not odd.any():  # (on the GPU nothing waits for the answer)
+            return torch.matmul(weights, x)
+    except RuntimeError:  # torch.func.vmap: no answer for all of its rows
+        pass
+    out = torch.matmul(weights, x.masked_fill(odd, 0.0))
+    with torch.no_grad():
+        w, inf, nan = torch.sign(weights), torch.sign(x).masked_fill(~torch.isinf(x), 0.0), torch.isnan(x).to(x.dtype)
+        up = torch.matmul(w.clamp(min=0), inf.clamp(min=0)) + torch.matmul(w.clamp(max=0), inf.clamp(max=0))
+        down = torch.matmul(w.clamp(min=0), inf.clamp(max=0)) + torch.matmul(w.clamp(max=0), inf.clamp(min=0))
+        none = torch.matmul(lower.to(x.dtype), nan) + torch.matmul((lower & (weights == 0)).to(x.dtype), inf.abs())
+        odd_sum = (torch.zeros_like(out).masked_fill(up > 0, math.inf) + torch.zeros_like(out).masked_fill(down < 0, -math.inf)
+                   ).masked_fill(none > 0, math.nan)
+    return out + odd_sum
+
+
 def _torch_selective_scan(keys: Tensor, values: Tensor, queries: Tensor, steps: Tensor, rates: Tensor,
                           memory: Optional[Tensor], skip: Optional[Tensor], step_bias: Optional[Tensor],
                           lengths: Optional[Tensor], softplus: bool) -> Tuple[Tensor, Tensor]:
@@ -1018,8 +1038,8 @@ def _torch_selective_scan(keys: Tensor, values: Tensor, queries: Tensor, steps: 
         cum = (dc.double() * rates.double()[:, None]).cumsum(-1)
         lower = torch.ones(n, n, dtype=torch.bool, device=x.device).tril()
         decay = torch.exp((cum[..., :, None] - cum[..., None, :]).masked_fill(~lower, -math.inf)).to(cdt)
-        within = torch.matmul(torch.matmul(qc, kc.transpose(-1, -2)) * decay * dc[..., None, :], xc)
-        outs.append(within + torch.exp(cum).to(cdt)[..., None] * torch.matmul(qc, state.transpose(-1, -2)))
+        mix = (torch.matmul(qc, kc.transpose(-1, -2)) * decay * dc[..., None, :]).masked_fill(~lower, 0.0)
+        outs.append(_lower_product(mix, xc, lower) + torch.exp(cum).to(cdt)[..., None] * torch.matmul(qc, state.transpose(-1, -2)))
         tail = torch.exp(cum[..., -1:] - cum).to(cdt) * dc
         state = (torch.exp(cum[..., -1]).to(cdt)[..., None, None] * state +
                  torch.matmul((xc * tail[..., None]).transpose(-1, -2), kc))
