@@ -1046,7 +1046,7 @@ def _torch_selective_scan(keys: Tensor, values: Tensor, queries: Tensor, steps: 
     hidden = torch.cat(outs, 2).transpose(1, 2) if outs else x.new_zeros(B, 0, H, P)
     if skip is not None:
         hidden = hidden + skip.to(cdt)[:, None] * x
-    return hidden.to(values.dtype), state
+    return hidden.to(values.dtype), state if T else state.clone()  # (of no tokens: not the caller's own tensor)
 
 
 class _SelectiveScanFn(torch.autograd.Function):
