@@ -510,7 +510,8 @@ int grm_hip_short_conv_step(const void* x, const void* weight, const void* bias,
  * bfloat16 inputs run bf16 MFMA (the float32 state kept whole in its updates; where a query reads it, it and the
  * weights between tokens of a chunk are two bf16 parts, which lose 2^-16 of a term); float16 and float32 inputs run
  * float32 MFMA.
- * Limits: key_dim <= 128, heads a multiple of groups, token strides and rows below 2^21 elements.
+ * Limits: key_dim <= 128, heads a multiple of groups, token strides and rows of at most 2^21 elements, batch * heads *
+ * ceil(value_dim / 64) below 2^23 (single token: batch * heads below 2^24).
  */
 typedef struct grm_hip_selective_args {
   const void* keys;

@@ -478,7 +478,7 @@ inline int64_t sel_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // More than the eight 4 MB L2 caches hold is stored past them: what would be written back at the kernel's end leaves
 // during it: the step of 64 sequences x 32 heads 33.1 -> 30.7 us, the scan of 8 x 2048 tokens x 32 heads 90.5 -> 87.6.
 inline int sel_streams(int64_t bytes) { return bytes > (int64_t{32} << 20); }
-int sel_check(const struct grm_hip_selective_args* u, const char* what);
+int sel_check(const struct grm_hip_selective_args* u, const char* what, bool step = false);
 SelArgs sel_args(const struct grm_hip_selective_args* u);
 // Tokens of a backward chunk, and time parts of a walk: part_tokens set to a multiple of it.
 int64_t sel_block(int dtype);

@@ -830,7 +830,8 @@ extern "C" int grm_hip_selective_scan_bwd(const grm_hip_selective_args* u, const
     set_error("%s: workspace missing, misaligned or too small", what);
     return GRM_HIP_EINVAL;
   }
-  if (p.wgs * p.splits > INT32_MAX) {
+  const int64_t waves4 = sel_ceil(u->batch * p.nsave * u->heads, 4);
+  if (p.wgs * p.splits * kGradThreads > UINT32_MAX || waves4 * 256 > UINT32_MAX) {  // a grid dimension has fewer than 2^32 threads
     set_error("%s: too many blocks for one launch", what);
     return GRM_HIP_EUNSUPPORTED;
   }
@@ -868,7 +869,7 @@ extern "C" int grm_hip_selective_scan_bwd(const grm_hip_selective_args* u, const
     a.rows_part = p.splits > 1 ? reinterpret_cast<float*>(ws + p.rows) : nullptr;
     a.head_part = reinterpret_cast<float*>(ws + p.heads);
     a.splits = p.splits;
-    const dim3 waves(static_cast<uint32_t>(sel_ceil(u->batch * p.nsave * u->heads, 4)));
+    const dim3 waves(static_cast<uint32_t>(waves4));
     sel_with_form(u->dtype, u->key_dim, a.s.vec != 0, [&](auto e, auto m, auto np, auto vec) {
       using E = decltype(e);
       using M = decltype(m);

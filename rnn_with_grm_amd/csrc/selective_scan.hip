@@ -25,6 +25,7 @@ namespace {
 
 constexpr int kWalkThreads = 512;
 constexpr int kPassThreads = 512;
+constexpr int kStepThreads = 256;
 constexpr int kMaxParts = 32;
 
 // Weights between a chunk's tokens in LDS: the 16 x 16 tiles on and below the diagonal, each as its lanes hold it, four
@@ -538,7 +539,7 @@ __global__ __launch_bounds__(kPassThreads) __attribute__((amdgpu_waves_per_eu(2,
 // One token: a row of the state lies on LPR lanes (4 columns each), a wave moves 64 / LPR rows at a
 // time, each element read and written by one thread (so memory_out may be memory).
 template <class E, int LPR>
-__global__ __launch_bounds__(256) void selective_step_kernel(SelArgs a) {
+__global__ __launch_bounds__(kStepThreads) void selective_step_kernel(SelArgs a) {
   using raw = typename ET<E>::raw;
   constexpr int RPW = 64 / LPR, U = 4;  // rows a wave moves at once, and in how many loads
   const int lane = lane_id(), wave = static_cast<int>(threadIdx.x) >> 6;
@@ -639,7 +640,7 @@ int sel_parts(int64_t seqs, int64_t T, int dtype, int64_t* part_tokens) {
   return static_cast<int>(sel_ceil(blocks, per));
 }
 
-int sel_check(const grm_hip_selective_args* u, const char* what) {
+int sel_check(const grm_hip_selective_args* u, const char* what, bool step) {
   auto bad = [&](const char* why) {
     set_error("%s: %s", what, why);
     return GRM_HIP_EINVAL;
@@ -665,8 +666,15 @@ int sel_check(const grm_hip_selective_args* u, const char* what) {
   if (u->heads > most || u->value_dim > most || u->groups > most || u->batch > (1 << 24) || u->keys_token_stride < 0 ||
       u->keys_token_stride > most || u->values_token_stride < 0 || u->values_token_stride > most ||
       u->queries_token_stride < 0 || u->queries_token_stride > most || u->heads * u->value_dim > most ||
-      u->groups * u->key_dim > most || u->heads * sel_ceil(u->value_dim, kSelRows) * u->batch > (1 << 24)) {
-    set_error("%s: token strides and row widths must be below 2^21 elements and batch * heads * value tiles below 2^24", what);
+      u->groups * u->key_dim > most) {
+    set_error("%s: token strides and row widths must be at most 2^21 elements", what);
+    return GRM_HIP_EUNSUPPORTED;
+  }
+  // (A grid dimension has fewer than 2^32 threads.)
+  const int64_t wgs = u->heads * u->batch * (step ? 1 : sel_ceil(u->value_dim, kSelRows)), threads = step ? kStepThreads : kWalkThreads;
+  if (wgs * threads > UINT32_MAX) {
+    set_error("%s: batch * heads%s must be below %lld", what, step ? "" : " * ceil(value_dim / 64)",
+              static_cast<long long>((int64_t{UINT32_MAX} + 1) / threads));
     return GRM_HIP_EUNSUPPORTED;
   }
   if (u->seq_len > 1 && (u->keys_token_stride < u->groups * u->key_dim || u->queries_token_stride < u->groups * u->key_dim ||
@@ -783,7 +791,7 @@ extern "C" int grm_hip_selective_scan_fwd(const grm_hip_selective_args* u, void*
 
 extern "C" int grm_hip_selective_step(const grm_hip_selective_args* u, void* hidden, float* memory_out, void* stream) {
   const char* what = "selective_step";
-  if (int rc = sel_check(u, what)) return rc;
+  if (int rc = sel_check(u, what, true)) return rc;
   if (u->seq_len != 1 || u->lengths != nullptr) {
     set_error("%s: seq_len must be 1, without lengths", what);
     return GRM_HIP_EINVAL;
@@ -803,8 +811,9 @@ extern "C" int grm_hip_selective_step(const grm_hip_selective_args* u, void* hid
   a.stream = sel_streams(state_bytes);
   auto go = [&](auto e, auto lpr) {
     constexpr int LPR = decltype(lpr)::value, rows = 4 * (64 / LPR) * 4;  // of a workgroup at a time
+    const int64_t tiles = sel_ceil(a.P, rows), most = 65535;  // a grid's second dimension; the kernel goes round
     selective_step_kernel<decltype(e), LPR>
-        <<<dim3(static_cast<uint32_t>(a.B) * a.H, static_cast<uint32_t>(sel_ceil(a.P, rows))), dim3(256), 0,
+        <<<dim3(static_cast<uint32_t>(a.B) * a.H, static_cast<uint32_t>(tiles < most ? tiles : most)), dim3(kStepThreads), 0,
            static_cast<hipStream_t>(stream)>>>(a);
   };
   auto by_width = [&](auto e) {

@@ -515,7 +515,7 @@ extern "C" int grm_hip_short_conv_bwd(const void* x, const void* weight, const v
   a.runs = ceil_div(seq_len > 0 ? seq_len : 1, a.run);
   const int64_t parts = batch > 0 ? bwd_parts(batch, seq_len, a.run) : 0;
   const int64_t blocks = ceil_div(channels, 64 * v), weight_blocks = ceil_div(channels * (width + 1), 64);
-  if (weight_blocks > kMaxBlocks || blocks > kMaxBlocks) {
+  if (weight_blocks >= kMaxBlocks || blocks > kMaxBlocks) {  // (512 threads a block, fewer than 2^32 in all)
     set_error("short_conv backward: too many elements for one launch");
     return GRM_HIP_EUNSUPPORTED;
   }
