@@ -370,6 +370,12 @@ __global__ __launch_bounds__(kThreads) void conv_step_kernel(ConvArgs a) {
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+// More elements than any memory has.  (Below, no product of sizes passes 63 bits.)
+bool too_many(int64_t B, int64_t T, int64_t C) {
+  const int64_t most = int64_t{1} << 50;
+  return B > most || T > most || C > most || (B > 0 && T + 4 > most / B / C);
+}
+
 int check_conv(const ConvArgs& a, int64_t width, int dtype, int w_dtype, const char* what) {
   if (a.B < 0 || a.T < 0 || a.C < 1) {
     set_error("%s: batch and seq_len must be >= 0 and channels >= 1", what);
@@ -377,6 +383,10 @@ int check_conv(const ConvArgs& a, int64_t width, int dtype, int w_dtype, const c
   }
   if (width < 2 || width > 4) {
     set_error("%s: width must be 2, 3 or 4, got %lld", what, static_cast<long long>(width));
+    return GRM_HIP_EUNSUPPORTED;
+  }
+  if (too_many(a.B, a.T, a.C)) {
+    set_error("%s: too many elements", what);
     return GRM_HIP_EUNSUPPORTED;
   }
   if (dtype < 0 || dtype > 2 || (w_dtype != dtype && w_dtype != GRM_HIP_F32)) {
@@ -481,7 +491,9 @@ extern "C" int grm_hip_short_conv_fwd(const void* x, const void* weight, const v
 
 extern "C" int64_t grm_hip_short_conv_bwd_workspace(int64_t batch, int64_t seq_len, int64_t channels, int64_t width,
                                                     int dtype) {
-  if (batch <= 0 || seq_len < 0 || channels <= 0 || width < 2 || width > 4 || dtype < 0 || dtype > 2) return 0;
+  if (batch <= 0 || seq_len < 0 || channels <= 0 || width < 2 || width > 4 || dtype < 0 || dtype > 2 ||
+      too_many(batch, seq_len, channels))
+    return 0;
   const int64_t a = bwd_parts(batch, seq_len, bwd_run(batch, seq_len, channels, true)),
                 b = bwd_parts(batch, seq_len, bwd_run(batch, seq_len, channels, false));
   return (a > b ? a : b) * channels * (width + 1) * 4;

@@ -83,3 +83,16 @@ def test_convolution_weights_of_too_many_channels():
     back = capi.load().grm_hip_short_conv_bwd(FAKE, FAKE, None, None, None, FAKE, None, FAKE, FAKE, None, None, FAKE, 1 << 62, 1, 1, C,
                                               4, C, C, capi.BF16, capi.BF16, 0, None)
     assert back == capi.EUNSUPPORTED
+
+
+@pytest.mark.parametrize("B,T,C", [(1 << 62, 1, 4), (4, 1 << 62, 4), (4, 1, 1 << 62), (1 << 30, 1 << 30, 16), ((1 << 63) - 1, 8, 8),
+                                   (1 << 40, 1 << 12, 1), (2, (1 << 63) - 1, 2)])
+def test_convolutions_whose_sizes_pass_63_bits(B, T, C):
+    """Their products would wrap round to a small launch."""
+    lib = capi.load()
+    assert lib.grm_hip_short_conv_fwd(FAKE, FAKE, None, None, None, FAKE, 2 * FAKE, B, T, C, 4, T * C % (1 << 62), C, 0, 0, 0, None) == capi.EUNSUPPORTED
+    assert lib.grm_hip_short_conv_bwd_workspace(B, T, C, 4, 0) == 0
+    assert lib.grm_hip_short_conv_bwd(FAKE, FAKE, None, None, None, FAKE, None, FAKE, FAKE, None, None, FAKE, 1 << 62, B, T, C, 4,
+                                      T * C % (1 << 62), C, 0, 0, 0, None) == capi.EUNSUPPORTED
+    if T == 1:
+        assert lib.grm_hip_short_conv_step(FAKE, FAKE, None, FAKE, FAKE, FAKE, B, C, 4, C, 0, 0, 0, None) == capi.EUNSUPPORTED
