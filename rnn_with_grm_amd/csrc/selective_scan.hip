@@ -371,7 +371,8 @@ __global__ __launch_bounds__(kWalkThreads) __attribute__((amdgpu_waves_per_eu(2,
         const int t = c * L + it * 16 + n16;
         f32x4 v;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = t < live ? fmaf(skip, xv[it][r], y[it][r]) : 0.f;
+        for (int r = 0; r < 4; ++r)  // (without `skip` no product with zero: an infinite value would make a NaN of it)
+          v[r] = t < live ? (a.skip != nullptr ? fmaf(skip, xv[it][r], y[it][r]) : y[it][r]) : 0.f;
         if (t_first + t < t_last) {
           eraw* o = hid + t * hstride + col;
           if (hvec) {
@@ -406,6 +407,13 @@ __global__ __launch_bounds__(kWalkThreads) __attribute__((amdgpu_waves_per_eu(2,
           weigh_frag<M>(xf[s + 1 < NS32 ? s + 1 : 0], w0, w1, part);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) kf[nt] = kn[nt];
+        }
+      }
+      if (__builtin_expect(odd && a.N < NP, 0)) {  // an infinity times the zeros of the columns past the keys' width
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[nt][r] = nt * 16 + 4 * g + r < a.N ? acc[nt][r] : 0.f;
         }
       }
       __syncthreads();
@@ -604,7 +612,7 @@ __global__ __launch_bounds__(kStepThreads) void selective_step_kernel(SelArgs a)
           if (col + 3 < a.N) s[3] = m[u].w;
         }
       }
-      if (p < a.P && lane % LPR == 0) hp[p] = ET<E>::from_f(fmaf(skip, x[u], y));
+      if (p < a.P && lane % LPR == 0) hp[p] = ET<E>::from_f(a.skip != nullptr ? fmaf(skip, x[u], y) : y);
     }
   }
 }
