@@ -138,7 +138,7 @@ template <int L>
 __device__ __forceinline__ TokenScalars token_scalars(const SelArgs& a, float z, bool live, float rate) {
   TokenScalars s;
   s.d = lane_id() < L && live ? step_size(a, z) : 0.f;
-  double l = static_cast<double>(s.d) * static_cast<double>(rate);
+  double l = live ? static_cast<double>(s.d) * static_cast<double>(rate) : 0.0;  // (the rate may be infinite)
   l = l < -200.0 ? -200.0 : l;
   l *= 1.4426950408889634;  // log2(e)
   s.cum = wave_prefix(l);

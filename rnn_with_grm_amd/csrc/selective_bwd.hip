@@ -183,7 +183,7 @@ __global__ __launch_bounds__(256) void selective_token_kernel(GradArgs a) {
   for (int k = 0; k < PL; ++k) {
     const int64_t t = t0 + lane * PL + k;
     d[k] = t < len ? step_size(f, raw_step<E>(f, b, t, h)) : 0.f;
-    double l = static_cast<double>(d[k]) * static_cast<double>(rate);
+    double l = t < len ? static_cast<double>(d[k]) * static_cast<double>(rate) : 0.0;
     l = l < -200.0 ? -200.0 : l;
     sum += l * 1.4426950408889634;
     cum[k] = sum;

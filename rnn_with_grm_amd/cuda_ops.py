@@ -1035,7 +1035,10 @@ def _torch_selective_scan(keys: Tensor, values: Tensor, queries: Tensor, steps: 
         part = slice(t0, min(t0 + 64, T))
         xc, kc, qc, dc = xh[:, :, part], kh[:, :, part], qh[:, :, part], dh[:, :, part]
         n = xc.size(2)
-        cum = (dc.double() * rates.double()[:, None]).cumsum(-1)
+        log = (dc.double() * rates.double()[:, None]).clamp(min=-1000.0)  # a decay of zero, and sums that stay numbers
+        if live is not None:
+            log = log.masked_fill(~live[:, None, part], 0.0)
+        cum = log.cumsum(-1)
         lower = torch.ones(n, n, dtype=torch.bool, device=x.device).tril()
         decay = torch.exp((cum[..., :, None] - cum[..., None, :]).masked_fill(~lower, -math.inf)).to(cdt)
         mix = (torch.matmul(qc, kc.transpose(-1, -2)) * decay * dc[..., None, :]).masked_fill(~lower, 0.0)

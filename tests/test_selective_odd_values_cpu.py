@@ -77,3 +77,15 @@ def test_under_vmap():
         torch.testing.assert_close(o, scan({**x, "values": v})[0])
     jac = torch.func.jacfwd(lambda r: scan({**x, "rates": r})[0])(x["rates"])
     assert jac.shape == (1, 10, 2, 3, 2) and torch.isfinite(jac).all()
+
+
+@pytest.mark.parametrize("T,lengths", [(10, None), (70, None), (70, (41,))])
+def test_a_rate_of_minus_infinity(T, lengths):
+    """A head that forgets everything at every token."""
+    import selective_oracle as oracle
+    x = {k: v.double() for k, v in scan_inputs(T).items()}
+    x["rates"] = torch.tensor([-0.5, -INF], dtype=torch.float64)
+    n = None if lengths is None else torch.tensor(lengths)
+    got = scan(x, lengths=n)
+    for a, b in zip(got, oracle.selective_scan(*(x[k] for k in NAMES), n, True)):
+        torch.testing.assert_close(a, b, rtol=1e-10, atol=1e-10)
