@@ -941,7 +941,7 @@ def cuda_short_conv(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, st
 def _check_out(out: Optional[Tensor], like: Tensor, name: str, grad: bool) -> None:
     if out is None:
         return
-    if grad:
+    if grad or _wants_grad(out):
         raise ValueError(f"{name} cannot be given where gradients are wanted")
     if out.shape != like.shape or out.dtype != like.dtype or not out.is_contiguous():
         raise ValueError(f"{name} must be contiguous and match its input in shape and type")
