@@ -37,7 +37,9 @@ extern "C" {
 #define GRM_HIP_EINVAL (-1)      /* bad pointer, size or dtype */
 #define GRM_HIP_EUNSUPPORTED (-2) /* valid for the reference, not for this kernel (e.g. key_dim > 256) */
 
-/* Library ABI version (major * 100 + minor). */
+/* Library ABI version (major * 100 + minor).  The short convolution and the selective scan (grm_hip_short_conv_*,
+ * grm_hip_selective_*) came without a new number: 109 is a library with or without them, which the lookup of their
+ * symbols tells. */
 int grm_hip_abi_version(void);
 
 /* Thread-local text of the last error returned by any entry point. */

@@ -19,9 +19,10 @@ namespace grmhip {
 
 constexpr int kSelRows = 64;  // value rows of a state tile
 
-// Compute type M: BF16 inputs run bf16 MFMA; float32 and float16 inputs run float32 MFMA on float32 tiles (states
-// and decayed weights leave float16's range, and splitting both operands into bfloat16 parts would
-// cost as many products).
+// Compute type M: BF16 inputs run bf16 MFMA; float32 and float16 inputs run float32 MFMA on float32 tiles, which keeps
+// every bit in one product.  (bfloat16 parts would do too, a float16 number being two of them and a float32 one
+// three: four products for q . k of float16, six for a state's update, of a sixteenth of the cycles each.  That form is not
+// built; the float32 one is 7 to 14 times its floor in bytes at 5 x 777 float16 tokens x 12 heads.)
 template <class M>
 struct SelShape {
   static constexpr bool kHalf = sizeof(typename ET<M>::raw) == 2;
@@ -476,7 +477,8 @@ void sel_with_form(int dtype, int64_t N, bool vec, F f) {
 }
 inline int64_t sel_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 // More than the eight 4 MB L2 caches hold is stored past them: what would be written back at the kernel's end leaves
-// during it: the step of 64 sequences x 32 heads 33.1 -> 30.7 us, the scan of 8 x 2048 tokens x 32 heads 90.5 -> 87.6.
+// during it: the step of 64 sequences x 32 heads 33.8 -> 33.3 us, back to back; the scan of 8 x 2048 tokens x 32 heads the same
+// either way.
 inline int sel_streams(int64_t bytes) { return bytes > (int64_t{32} << 20); }
 int sel_check(const struct grm_hip_selective_args* u, const char* what, bool step = false);
 SelArgs sel_args(const struct grm_hip_selective_args* u);

@@ -18,12 +18,11 @@
 // kernel: no atomics, the same bits on every run.
 //
 // The step sizes' gradients stay float32: K and W are sums of exact products, and S and G enter t1 and t2 as three
-// bfloat16 parts (24 bits; with two, 2^-17, each token's gradient was off by 4.5e-7 where it is now by 1.7e-7, for 25 us of a
-// forward and backward of 455).
+// bfloat16 parts (24 bits; with two, 2^-17, each token's gradient was off by 4.5e-7 where it is now by 1.7e-7, for 25 us).
 // dl_t is summed without taking large sums off each other (at selective_steps_kernel).
 // dx, dk and dq are rounded to 16 bits in the end; their weights E K and E d W, and G where it meets k, are two bfloat16
-// parts, which lose 2^-16 of a term (8 x 2048 tokens x 32 heads, forward and backward: 489 us; with one part, whose 2^-8 is
-// seen in the outputs, 458).
+// parts, which lose 2^-16 of a term (8 x 2048 tokens x 32 heads, forward and backward: 489 us, 494 with the signs in turn below; with one part,
+// whose 2^-8 is seen in the outputs, 458).
 #include <stdint.h>
 
 #include "selective.h"
@@ -776,8 +775,8 @@ BwdPlan bwd_plan(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G, int64_t 
   p.nsave = sel_ceil(T, LB);
   p.parts = sel_parts(B * H * p.PT, T, dtype, &p.part_tokens);
   // A workgroup for each of 256 CUs; the heads of a group are shared no further, since every share reads
-  // the keys and queries and writes a float32 copy of dk and dq (4 x 1000 float32 tokens x 8 heads in 2 groups, forward
-  // and backward: 117 us in two shares, 142 us in one).
+  // the keys and queries and writes a float32 copy of dk and dq (selective_grad_kernel at 4 x 1000 float32 tokens x 8
+  // heads in 2 groups: 39 us in two shares, 66 us in one).
   p.wgs = B * p.nsave * G;
   const int64_t heads = H / G * p.PT;
   int64_t splits = p.wgs > 0 ? sel_ceil(256, p.wgs) : 1;

@@ -635,8 +635,8 @@ uint32_t walk_blocks(const SelArgs& a) { return static_cast<uint32_t>(a.B) * a.H
 int64_t sel_block(int dtype) { return dtype == GRM_HIP_BF16 ? SelShape<BF16>::LB : SelShape<F32>::LB; }
 
 // Enough parts for a workgroup on each of 256 CUs, of at least four backward chunks each: a part costs a
-// second reading of its keys and values (32768 bf16 tokens x 16 heads of one sequence: 154 us in 16 parts,
-// 1125 us in one).
+// second reading of its keys and values (32768 bf16 tokens x 16 heads of one sequence: 165 us in 16 parts,
+// 1400 us in one).
 int sel_parts(int64_t seqs, int64_t T, int dtype, int64_t* part_tokens) {
   const int64_t block = sel_block(dtype), blocks = T > 0 ? sel_ceil(T, block) : 1;
   int64_t parts = 256 / (seqs > 0 ? seqs : 1);
@@ -711,8 +711,8 @@ SelArgs sel_args(const grm_hip_selective_args* u) {
   a.parts = 1;
   a.steps_f32 = u->steps_dtype == GRM_HIP_F32;
   a.softplus = u->softplus;
-  // Whole 16-byte loads where every row of 8-element units allows them: 8 x 2048 bf16 tokens x 32 heads take 92 us so,
-  // and 218 us element by element.
+  // Whole 16-byte loads where every row of 8-element units allows them: 8 x 2048 bf16 tokens x 32 heads take half the
+  // time of element by element so (121 and 240 us, back to back).
   a.vec = u->value_dim % 8 == 0 && u->key_dim % 8 == 0 && aligned(u->keys) && aligned(u->values) &&
           aligned(u->queries) && (u->keys_batch_stride | u->keys_token_stride | u->values_batch_stride |
                                   u->values_token_stride | u->queries_batch_stride | u->queries_token_stride) % 8 == 0;

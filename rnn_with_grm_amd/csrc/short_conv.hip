@@ -14,8 +14,8 @@
 // workgroup's four waves in LDS, and over the workgroups by a second kernel in a fixed order (no
 // atomics: the same sums on every run).  All arithmetic is float32, rounded once on output.
 //
-// HBM bounds the prompts, the launch bounds single tokens: 8 x 2048 tokens x 2304 bf16 channels 33 us
-// (151 MB, 4.6 TB/s), with all gradients 104 us (forward 33, backward 66, its weights' sums 5), one
+// HBM bounds the prompts, the launch bounds single tokens: 8 x 2048 tokens x 2304 bf16 channels 36 us
+// (151 MB, 4.2 TB/s), with all gradients 104 us (by trace forward 31, backward 64, its weights' sums 4), one
 // token of 64 sequences 8 us.
 #include <stdint.h>
 
@@ -434,8 +434,8 @@ int streams(int64_t elements, int dtype) { return elements * (dtype == GRM_HIP_F
 
 // The backward's runs: about 3000, one and a half for each of the waves that fit the chip at once (8 x 2048 tokens of
 // 2304 bf16 channels, forward and backward: 104 us; 2000 runs: 115, 4000: 109), of 16 tokens at least (three rows of each
-// run's 19 or more are formed twice).  A thread has four channels: with eight, its sums and windows leave two waves a
-// SIMD (the backward kernel 96 us, with four 62).
+// run's 19 or more are formed twice).  A thread has four channels: with eight the backward kernel
+// measured 96 us, with four 64.  (Not for the waves a SIMD holds: two in both forms, at 256 and 178 registers.)
 int64_t bwd_run(int64_t B, int64_t T, int64_t C, bool vec) {
   const int64_t run = ceil_div(B * T * ceil_div(C, 64 * (vec ? 4 : 1)), 3000);
   return run < 16 ? 16 : run < T ? run : (T > 16 ? T : 16);
