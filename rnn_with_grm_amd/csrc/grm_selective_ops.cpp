@@ -45,7 +45,10 @@ void check_device(const Tensor& t, const Tensor& like, const char* op, const cha
 }
 
 // Autograd's count of writes to an argument: a graph that saved it for its backward then refuses to use what it holds now.
-void written(Tensor& t) { t.unsafeGetTensorImpl()->bump_version(); }
+// (No graph can save a tensor made in inference mode, and it has no count.)
+void written(Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 
 // A contiguous optional tensor's pointer; `keep` holds what it points into.
 void* opt_ptr(const OptTensor& t, Tensor& keep) {

@@ -82,3 +82,20 @@ def test_no_forward_derivatives(dev, grad_enabled):
 def forward(g, t, tangent):
     with torch.autograd.forward_ad.dual_level():
         return g(torch.autograd.forward_ad.make_dual(t, tangent))
+
+
+def test_steps_on_states_made_in_inference_mode(dev):
+    """A prompt in inference mode, its single tokens outside of it, in place."""
+    g = torch.Generator().manual_seed(6)
+    x, w = torch.randn(2, 9, 8, generator=g).to(dev), torch.randn(8, 4, generator=g).to(dev)
+    a = inputs(dev, 2, 1, 2, 16, 1, 16, torch.float32, seed=6)
+    with torch.inference_mode():
+        _, state = cuda_ops.cuda_short_conv(x, w)
+        _, memory = run(a)
+    kept = state.clone(), memory.clone()
+    with torch.no_grad():
+        want = cuda_ops.cuda_short_conv_step(x[:, 0], kept[0], w), cuda_ops.cuda_selective_step(*step_args(a), kept[1])
+        y, _ = cuda_ops.cuda_short_conv_step(x[:, 0], state, w, state_out=state)
+        h, _ = cuda_ops.cuda_selective_step(*step_args(a), memory, memory_out=memory)
+    assert torch.equal(y, want[0][0]) and torch.equal(state, want[0][1])
+    assert torch.equal(h, want[1][0]) and torch.equal(memory, want[1][1])
