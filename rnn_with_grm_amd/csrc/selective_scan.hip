@@ -294,8 +294,9 @@ __global__ __launch_bounds__(kWalkThreads) __attribute__((amdgpu_waves_per_eu(2,
       }
       const bool odd = __any(flags[0] + flags[1] + flags[2] + flags[3] != 0.f);
       if (__builtin_expect(odd, 0)) {
-        // A weight of zero does not keep an infinity or a NaN out of a product: all outputs one token i at a time, with the values of the tokens behind it taken out.  (The lane's number anew: what is made of it here
-        // is not to be kept in registers for the case.)
+        // A weight of zero does not keep an infinity or a NaN out of a product: all outputs one token i at a time, with
+        // the values of the tokens behind it taken out.  (The lane's number anew: what is made of it here is not to be
+        // kept in registers for the case.)
         int ln = lane_id();
         asm volatile("" : "+v"(ln));
 #pragma unroll
@@ -671,7 +672,7 @@ int sel_check(const grm_hip_selective_args* u, const char* what, bool step) {
     return GRM_HIP_EUNSUPPORTED;
   }
   // (One by one first: no product passes 63 bits.)
-  if (u->heads > most || u->value_dim > most || u->groups > most || u->batch > (1 << 24) || u->keys_token_stride < 0 ||
+  if (u->heads > most || u->value_dim > most || u->groups > most || u->keys_token_stride < 0 ||
       u->keys_token_stride > most || u->values_token_stride < 0 || u->values_token_stride > most ||
       u->queries_token_stride < 0 || u->queries_token_stride > most || u->heads * u->value_dim > most ||
       u->groups * u->key_dim > most) {
@@ -679,7 +680,8 @@ int sel_check(const grm_hip_selective_args* u, const char* what, bool step) {
     return GRM_HIP_EUNSUPPORTED;
   }
   // (A grid dimension has fewer than 2^32 threads.)
-  const int64_t wgs = u->heads * u->batch * (step ? 1 : sel_ceil(u->value_dim, kSelRows)), threads = step ? kStepThreads : kWalkThreads;
+  const int64_t batch = min_i64(u->batch, int64_t{1} << 32);
+  const int64_t wgs = u->heads * batch * (step ? 1 : sel_ceil(u->value_dim, kSelRows)), threads = step ? kStepThreads : kWalkThreads;
   if (wgs * threads > UINT32_MAX) {
     set_error("%s: batch * heads%s must be below %lld", what, step ? "" : " * ceil(value_dim / 64)",
               static_cast<long long>((int64_t{UINT32_MAX} + 1) / threads));

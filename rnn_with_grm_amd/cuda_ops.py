@@ -446,7 +446,7 @@ class _RetrieveFuseFn(torch.autograd.Function):
 def _has_tangent(*tensors: Optional[Tensor]) -> bool:
     """Whether a forward-mode derivative is asked for (torch.autograd.forward_ad, torch.func.jvp): the native ops
     alone would drop it, while an autograd function without one refuses the call."""
-    return forward_ad._current_level >= 0 and any(
+    return getattr(forward_ad, "_current_level", 0) >= 0 and any(
         t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
