@@ -573,6 +573,80 @@ int grm_hip_selective_scan_bwd(const grm_hip_selective_args* args, const float* 
  */
 int grm_hip_selective_step(const grm_hip_selective_args* args, void* hidden, float* memory_out, void* stream);
 
+/*
+ * Gated delta rule: linear memory whose tokens first take out what the memory holds under their
+ * key.  No counterpart in the reference.
+ *   u_t = b_t (v_t - a_t M_{t-1} k_t),  M_t = a_t M_{t-1} + u_t k_t^T,  h_t = M_t q_t,  a_t = exp(log_decays_t)
+ * keys, queries [batch, seq_len, groups, key_dim]: a group's row serves heads / groups heads;
+ * values [batch, seq_len, heads, value_dim]; strengths (b) and log_decays (NULL: zeros) [batch,
+ * seq_len, heads].  The last two dimensions (of the last two: the last) are packed, the strides are
+ * elements between sequences and between tokens.  dtype is that of keys, values, queries and
+ * hidden; strengths and log_decays have it or are float32, each for itself.
+ * lengths: NULL, or int64 [batch] (device), clamped to [0, seq_len]: the tokens from lengths[b] on
+ * are not read, leave the state alone, and their rows of every output are zeros.
+ * memory: float32 [batch, heads, value_dim, key_dim], 16-byte aligned, the state before token 0;
+ * NULL: zeros.
+ * Products run bf16 MFMA on bfloat16 parts of their operands (three of a float32 number); where only a 16-bit output
+ * is reached, two parts, which lose 2^-16 of a term.  From a token that holds an infinity or a NaN on, what depends on it is NaN
+ * (a value: its column; a query: its row of hidden; all else: the head); earlier tokens are untouched.
+ * Limits: key_dim <= 128, heads a multiple of groups, token strides and rows of at most 2^21 elements, batch * heads *
+ * ceil(value_dim / 64) and batch * heads * ceil(seq_len / 64) below 2^24 (single token: batch * heads).
+ */
+typedef struct grm_hip_delta_args {
+  const void* keys;
+  const void* values;
+  const void* queries;
+  const void* strengths;
+  const void* log_decays;
+  const int64_t* lengths;
+  const float* memory;
+  int64_t batch, seq_len, heads, value_dim, groups, key_dim;
+  int64_t keys_batch_stride, keys_token_stride;
+  int64_t values_batch_stride, values_token_stride;
+  int64_t queries_batch_stride, queries_token_stride;
+  int64_t strengths_batch_stride, strengths_token_stride;
+  int64_t decays_batch_stride, decays_token_stride;
+  int dtype, strengths_dtype, decays_dtype;
+} grm_hip_delta_args;
+
+/*
+ * hidden:     [batch, seq_len, heads, value_dim], contiguous.
+ * memory_out: float32 [batch, heads, value_dim, key_dim], the state after each sequence's last
+ *             token; may not overlap memory.
+ * states:     NULL, or float32 [batch, ceil(seq_len / 64), heads, value_dim, key_dim]: the state
+ *             before every 64 tokens, which the backward reads (those behind a length are left as
+ *             they were).
+ * miss:       NULL, or float32 [batch, seq_len, heads, value_dim]: v_t - a_t M_{t-1} k_t, which the
+ *             backward reads (rows behind a length are left as they were).
+ * workspace:  grm_hip_delta_scan_workspace() bytes, 16-byte aligned.
+ */
+int64_t grm_hip_delta_scan_workspace(int64_t batch, int64_t seq_len, int64_t heads, int dtype);
+int grm_hip_delta_scan_fwd(const grm_hip_delta_args* args, void* hidden, float* memory_out, float* states, float* miss,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Gradients of grm_hip_delta_scan_fwd.  states and miss are what the forward left for the same
+ * arguments; grad_hidden [batch, seq_len, heads, value_dim] is contiguous in dtype, grad_memory_out
+ * float32 or NULL (zeros).  grad_keys, grad_values, grad_queries (dtype), grad_strengths
+ * (strengths_dtype) and grad_log_decays (decays_dtype; may be NULL) are contiguous, grad_memory
+ * float32.  Rows behind a sequence's length get zeros.  All sums are taken in a fixed order (no atomics).
+ * An infinity or a NaN in the inputs or gradients may reach every gradient of its sequence.
+ * Workspace: grm_hip_delta_scan_bwd_workspace() bytes, 16-byte aligned.
+ */
+int64_t grm_hip_delta_scan_bwd_workspace(int64_t batch, int64_t seq_len, int64_t heads, int64_t value_dim,
+                                         int64_t groups, int64_t key_dim);
+int grm_hip_delta_scan_bwd(const grm_hip_delta_args* args, const float* states, const float* miss,
+                           const void* grad_hidden, const float* grad_memory_out, void* grad_keys, void* grad_values,
+                           void* grad_queries, void* grad_strengths, void* grad_log_decays, float* grad_memory,
+                           void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * One token of grm_hip_delta_scan_fwd (seq_len = 1, no lengths): hidden [batch, heads, value_dim],
+ * memory_out the state moved by the token.  memory_out may be memory itself (updated in place),
+ * but not overlap it otherwise.
+ */
+int grm_hip_delta_step(const grm_hip_delta_args* args, void* hidden, float* memory_out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,6 +14,8 @@ from .cuda_ops import (  # noqa: F401
     cuda_apply_query,
     cuda_batched_memory_gather,
     cuda_chunk_update,
+    cuda_delta_scan,
+    cuda_delta_step,
     cuda_fuse_residual,
     cuda_gather_apply,
     cuda_segment_scan,
@@ -35,6 +37,8 @@ __all__ = [
     "cuda_apply_query",
     "cuda_batched_memory_gather",
     "cuda_chunk_update",
+    "cuda_delta_scan",
+    "cuda_delta_step",
     "cuda_fuse_residual",
     "cuda_gather_apply",
     "cuda_segment_scan",

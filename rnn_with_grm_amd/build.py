@@ -31,8 +31,8 @@ OFFLOAD_ARCH = "gfx950"
 HIP_SOURCES = ["grm_capi.hip", "chunk_scan.hip", "chunk_scan_wide.hip", "chunk_scan_vsplit.hip", "chunk_scan_par.hip",
                "chunk_bwd.hip", "chunk_bwd_f32.hip", "gather_apply.hip", "retrieve.hip", "retrieve_window.hip",
                "route_fuse.hip", "route_select.hip", "layer_glue.hip", "short_conv.hip",
-               "selective_scan.hip", "selective_bwd.hip"]
-EXT_SOURCES = ["grm_torch_ops.cpp", "grm_selective_ops.cpp"]
+               "selective_scan.hip", "selective_bwd.hip", "delta_scan.hip", "delta_bwd.hip"]
+EXT_SOURCES = ["grm_torch_ops.cpp", "grm_selective_ops.cpp", "grm_delta_ops.cpp"]
 
 # Packed fp32 instructions are kept out of every kernel (the flag is for the
 # device pass; the host pass warns that it does not know it, harmlessly).
@@ -76,7 +76,8 @@ def _stale(target: Path, deps: List[Path]) -> bool:
 
 def _headers() -> List[Path]:
     return [INCLUDE / "grm_hip.h", CSRC / "grm_hip_common.h", CSRC / "chunk_scan.h", CSRC / "chunk_bwd.h",
-            CSRC / "f32_tiles.h", CSRC / "route_select.h", CSRC / "retrieve.h", CSRC / "selective.h"]
+            CSRC / "f32_tiles.h", CSRC / "route_select.h", CSRC / "retrieve.h", CSRC / "selective.h", CSRC / "delta.h",
+            CSRC / "op_checks.h"]
 
 
 def build_hip_library(force: bool = True, verbose: bool = False, jobs: Optional[int] = None) -> Path:

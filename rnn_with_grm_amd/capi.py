@@ -89,6 +89,27 @@ SIGNATURES.update({
     "grm_hip_selective_step": (_C, [ctypes.POINTER(SelectiveArgs), _P, _P, _P]),
 })
 
+
+class DeltaArgs(ctypes.Structure):
+    """grm_hip_delta_args of include/grm_hip.h."""
+
+    _fields_ = ([(n, _P) for n in ("keys", "values", "queries", "strengths", "log_decays", "lengths", "memory")] +
+                [(n, _I) for n in ("batch", "seq_len", "heads", "value_dim", "groups", "key_dim",
+                                   "keys_batch_stride", "keys_token_stride", "values_batch_stride",
+                                   "values_token_stride", "queries_batch_stride", "queries_token_stride",
+                                   "strengths_batch_stride", "strengths_token_stride", "decays_batch_stride",
+                                   "decays_token_stride")] +
+                [(n, _C) for n in ("dtype", "strengths_dtype", "decays_dtype")])
+
+
+SIGNATURES.update({
+    "grm_hip_delta_scan_workspace": (_I, [_I, _I, _I, _C]),
+    "grm_hip_delta_scan_fwd": (_C, [ctypes.POINTER(DeltaArgs), _P, _P, _P, _P, _P, _I, _P]),
+    "grm_hip_delta_scan_bwd_workspace": (_I, [_I, _I, _I, _I, _I, _I]),
+    "grm_hip_delta_scan_bwd": (_C, [ctypes.POINTER(DeltaArgs)] + [_P] * 11 + [_I, _P]),
+    "grm_hip_delta_step": (_C, [ctypes.POINTER(DeltaArgs), _P, _P, _P]),
+})
+
 _lib: Optional[ctypes.CDLL] = None
 
 

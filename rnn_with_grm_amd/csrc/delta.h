@@ -1,0 +1,151 @@
+// Pieces shared by the delta rule's kernels (delta_scan.hip, delta_bwd.hip).
+//
+//   u_t = b_t (v_t - a_t M_{t-1} k_t),  M_t = a_t M_{t-1} + u_t k_t^T,  h_t = M_t q_t,  a_t = exp(g_t)
+//
+// A chunk of 64 tokens from state S, with c the running sum of g, D_i = e^{c_i}, W_ij = e^{c_i - c_j} (j <= i),
+// E_j = e^{c_63 - c_j} and diag(b) written b:
+//   m = v - a M k solves (I + A b) m = V - D K S^T with A_ij = W_ij k_i.k_j (j < i); u = b m
+//   H = D Q S^T + (W * Q K^T) b m,   S' = e^{c_63} S + (E b m)^T K
+// The inverse of I + A b and the weights W * Q K^T hang on no state: a launch of their own forms them for all chunks side
+// by side (delta_prep_kernel) and leaves them in the order in which matrix products read them.
+//
+// Numbers.  States, m and everything that reaches them are float32.  Products run on the bf16 MFMA: a float32
+// number is the sum of three bfloat16 parts, a float16 one of two, a bfloat16 one is itself, and the pairs of parts whose
+// product reaches 2^-24 of the whole are multiplied (six of nine; three where one side is bfloat16).  That costs 3/16 to
+// 6/16 of the float32 MFMA's cycles.  What only reaches a 16-bit output takes two parts (2^-16 of a term lost).
+#pragma once
+
+#include "selective.h"
+
+namespace grmhip {
+
+constexpr int kDTokens = 64;   // tokens of a chunk
+constexpr int kDCols = 64;     // value columns of a walk's workgroup, 16 a wave
+constexpr int kDFrags = 6;     // 16 x 32 fragments of a triangular 64 x 64 matrix
+constexpr int kDFragElems = 512;
+constexpr int kDScal = 208;    // floats kept of a chunk: D, E (forward: E b), b, first odd token
+
+// Parts of an input, and of a float32 number that only reaches outputs of type E.
+template <class E> struct DParts;
+template <> struct DParts<BF16> { static constexpr int IN = 1, OUT = 2; };
+template <> struct DParts<F16> { static constexpr int IN = 2, OUT = 2; };
+template <> struct DParts<F32> { static constexpr int IN = 3, OUT = 3; };
+
+typedef Frag8<BF16> B8;
+
+struct DeltaArgs {
+  const void *keys, *values, *queries;  // [B, T, G, N], [B, T, H, P], [B, T, G, N]
+  const void *strengths, *decays;       // [B, T, H]; decays may be null
+  const int64_t* lengths;               // [B] or null
+  const float* memory;                  // [B, H, P, N] or null
+  void* hidden;                         // [B, T, H, P]
+  float* memory_out;                    // [B, H, P, N]
+  float* states;                        // [B, C, H, P, N] or null: the state before every chunk
+  float* miss;                          // [B, T, H, P] or null: m
+  char* work;                           // what delta_prep_kernel leaves, [B, H, C]
+  int64_t kb, kt, vb, vt, qb, qt, sb, st, db, dt;
+  int64_t T;
+  int B, H, P, G, N, C, PT;
+  int s_f32, d_f32, vec;
+};
+
+// Bytes of a chunk of a head in the workspace: the inverse in three parts, the weights in PP parts, scalars.
+constexpr int64_t delta_chunk_bytes(int pp) { return (3 + pp) * kDFrags * kDFragElems * 2 + kDScal * 4; }
+
+// Fragment of row tile `t` and reduction step `s` among the six of a lower triangular matrix (columns up to the
+// row), and of an upper triangular one (from the row on).
+__host__ __device__ constexpr int lower_frag(int t, int s) { return t == 0 ? 0 : t == 1 ? 1 : t == 2 ? 2 + s : 4 + s; }
+__host__ __device__ constexpr int upper_frag(int t, int s) { return t == 0 ? s : t == 1 ? 2 + s : t == 2 ? 4 : 5; }
+
+__device__ __forceinline__ int64_t delta_length(const DeltaArgs& a, int b) {
+  return a.lengths == nullptr ? a.T : max_i64(0, min_i64(a.lengths[b], a.T));
+}
+
+// acc += sum of a[i] b[j] over the pairs with i + j < LIM, the smaller products first.
+template <int LIM, int NA, int NB>
+__device__ __forceinline__ f32x4 mma_parts(const B8 (&a)[NA], const B8 (&b)[NB], f32x4 acc) {
+#pragma unroll
+  for (int d = LIM - 1; d >= 0; --d) {
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      const int j = d - i;
+      if (j >= 0 && j < NB) acc = mfma8(a[i], b[j], acc);
+    }
+  }
+  return acc;
+}
+
+// Eight elements of type E as their parts.
+template <class E, int NI>
+__device__ __forceinline__ void input_parts(const U8<E>& u, B8 (&f)[NI]) {
+  if constexpr (std::is_same_v<E, BF16>) {
+    f[0] = __builtin_bit_cast(B8, u);
+  } else {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = ET<E>::to_f(u.e[e]);
+    split_frag<BF16, NI>(v, f);
+  }
+}
+
+// A loaded tile into LDS as NI tiles of parts, `part` elements apart; rows from `rows` on become zeros.
+template <class T, int NI, class E, class L>
+__device__ __forceinline__ void store_parts(const L& l, uint16_t* tile, int part, int rows, int tid) {
+  constexpr int UPR = L::UPR, PER = L::PER, DROW = L::DROW;
+  if (L::UNITS < DROW * UPR && tid >= L::UNITS) return;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int row = tid / UPR + i * DROW;
+    U8<E> u;
+    __builtin_memcpy(&u, &l.r[i][0], sizeof(u));
+    if (row >= rows) zero_u8<E>(u);
+    B8 f[NI];
+    input_parts<E, NI>(u, f);
+#pragma unroll
+    for (int p = 0; p < NI; ++p)
+      *reinterpret_cast<uint4*>(tile + p * part + l.at + i * DROW * T::STRIDE) = __builtin_bit_cast(uint4, f[p]);
+  }
+}
+
+// The parts of a fragment from tiles `part` elements apart.
+template <class T, int NI>
+__device__ __forceinline__ void row_parts_t(const uint16_t* tile, int part, int row, int col, B8 (&f)[NI]) {
+#pragma unroll
+  for (int p = 0; p < NI; ++p) f[p] = row_frag_t<T, BF16>(tile + p * part, row, col);
+}
+template <class T, int NI>
+__device__ __forceinline__ void col_parts(const uint16_t* tile, int part, int t0, int col, B8 (&f)[NI]) {
+#pragma unroll
+  for (int p = 0; p < NI; ++p) f[p] = col_frag<T, BF16>(tile + p * part, t0, col);
+}
+
+// A fragment's parts as delta_prep_kernel leaves them.
+template <int NP>
+__device__ __forceinline__ void stored_parts(const uint16_t* m, int frag, B8 (&f)[NP], int lane) {
+#pragma unroll
+  for (int p = 0; p < NP; ++p)
+    f[p] = __builtin_bit_cast(B8, *reinterpret_cast<const uint4*>(m + (frag * NP + p) * kDFragElems + 8 * lane));
+}
+
+int delta_check(const struct grm_hip_delta_args* u, const char* what, bool step);
+DeltaArgs delta_args(const struct grm_hip_delta_args* u);
+// The chunks' inverses and weights into a.work; `back`: in the reverse walk's form.
+int launch_delta_prep(const DeltaArgs& a, int dtype, bool back, hipStream_t stream, const char* what);
+
+// Host side: f(E, NK, VEC) with one of the compiled forms.
+template <class F>
+void delta_with_form(int dtype, int64_t N, bool vec, F f) {
+  auto by_vec = [&](auto e, auto nk) {
+    if (vec) f(e, nk, std::true_type{});
+    else f(e, nk, std::false_type{});
+  };
+  auto by_width = [&](auto e) {
+    if (N <= 64) by_vec(e, std::integral_constant<int, 64>{});
+    else by_vec(e, std::integral_constant<int, 128>{});
+  };
+  if (dtype == GRM_HIP_BF16) by_width(BF16{});
+  else if (dtype == GRM_HIP_F16) by_width(F16{});
+  else by_width(F32{});
+}
+
+}  // namespace grmhip

@@ -1,0 +1,723 @@
+// The gated delta rule on MI355X: the chunks' inverses and weights, the walk over a sequence's chunks, and the single
+// token.  The mathematics is in delta.h.
+#include "delta.h"
+
+namespace grmhip {
+namespace {
+
+constexpr int kPrepThreads = 256;
+constexpr int kWalkThreads = 256;
+constexpr int kStepThreads = 256;
+constexpr int kTriStride = 68;  // floats of a row of a 64 x 64 float32 matrix in LDS
+
+// acc += X Y of two 16 x 16 float32 tiles in LDS, in float32.
+__device__ __forceinline__ f32x4 mm16(const float* x, const float* y, f32x4 acc) {
+  const int g = lane_id() >> 4, n = lane_id() & 15;
+#pragma unroll
+  for (int s = 0; s < 4; ++s)
+    acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[n * kTriStride + 4 * s + g], y[(4 * s + g) * kTriStride + n], acc, 0, 0, 0);
+  return acc;
+}
+__device__ __forceinline__ void put16(float* y, f32x4 v) {
+  const int g = lane_id() >> 4, n = lane_id() & 15;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) y[(4 * g + r) * kTriStride + n] = v[r];
+}
+
+// One workgroup a chunk of a head.  Forward: the inverse of I + A b and the weights (W * Q K^T) b, both lower
+// triangular, by rows.  BACK: the inverse of I + b A and W * Q K^T, transposed (the reverse walk multiplies by their transposes).
+// The inverse: forward substitution inside the four 16 x 16 blocks of the diagonal, then two rounds of
+// -T2 (A21 T1) in float32 products.  Substitution does not cancel where keys lie close to each other, as a product of
+// powers of A would.
+template <class E, int NK, bool BACK>
+__global__ __launch_bounds__(kPrepThreads) void delta_prep_kernel(DeltaArgs a) {
+  using raw = typename ET<E>::raw;
+  constexpr int NI = DParts<E>::IN, PP = BACK ? 3 : DParts<E>::OUT, S = NK / 32;
+  __shared__ double cum_s[64];
+  __shared__ float b_s[64];
+  __shared__ int odd_s[4];
+  __shared__ __attribute__((aligned(16))) float A[64 * kTriStride], M[64 * kTriStride];
+  const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, n = lane & 15;
+  const uint32_t at = xcd_order(blockIdx.x, gridDim.x);
+  const int h = static_cast<int>(at % a.H), c = static_cast<int>(at / a.H % a.C), b = static_cast<int>(at / a.H / a.C);
+  const int64_t len = delta_length(a, b), t0 = static_cast<int64_t>(c) * kDTokens;
+  if (t0 >= len) return;
+  const int rows = static_cast<int>(min_i64(kDTokens, len - t0)), gi = h / (a.H / a.G);
+
+  // Scalars, lane = token, in every wave.
+  float bt = 0.f, gt = 0.f;
+  if (lane < rows) {
+    const int64_t i = b * a.sb + (t0 + lane) * a.st + h, j = b * a.db + (t0 + lane) * a.dt + h;
+    bt = a.s_f32 ? static_cast<const float*>(a.strengths)[i] : ET<E>::to_f(static_cast<const raw*>(a.strengths)[i]);
+    if (a.decays != nullptr)
+      gt = a.d_f32 ? static_cast<const float*>(a.decays)[j] : ET<E>::to_f(static_cast<const raw*>(a.decays)[j]);
+  }
+  const raw* kp = static_cast<const raw*>(a.keys) + b * a.kb + t0 * a.kt + static_cast<int64_t>(gi) * a.N;
+  const raw* qp = static_cast<const raw*>(a.queries) + b * a.qb + t0 * a.qt + static_cast<int64_t>(gi) * a.N;
+  const bool vec = a.vec != 0;
+  auto load = [&](const raw* p, int64_t stride, int tile, int s, int limit) {
+    const int row = 16 * tile + n;
+    return load_u8<E>(p + row * stride, 32 * s + 8 * g, a.N, row < limit, vec);
+  };
+  U8<E> ku[S], qu[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    ku[s] = load(kp, a.kt, w, s, rows);
+    qu[s] = load(qp, a.qt, w, s, rows);
+  }
+  // The first token whose key, strength or decay is no number (the walk takes it from there).
+  const float inf = __builtin_inff();
+  int odd = 64;
+  if (!BACK) {
+    bool bad = false;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) bad |= !(fabsf(ET<E>::to_f(ku[s].e[e])) < inf);
+    }
+    const uint64_t mask = __ballot(bad);
+    const uint32_t m16 = static_cast<uint32_t>((mask | mask >> 16 | mask >> 32 | mask >> 48) & 0xffff);
+    const uint64_t scal = __ballot(!(fabsf(bt) < inf) || !(gt < inf));
+    if (m16 != 0) odd = 16 * w + __builtin_ctz(m16);
+    if (scal != 0 && __builtin_ctzll(scal) < odd) odd = __builtin_ctzll(scal);
+    if (lane == 0) odd_s[w] = odd;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) odd = odd_s[i] < odd ? odd_s[i] : odd;
+    if (lane >= odd) bt = gt = 0.f;
+  }
+  // Log decays in log2 units and float64, as differences of running sums stay exact; a token's is held to -200 (a
+  // factor of 1e-60, nothing beside the 2^-24 of a term), so that sums stay numbers.
+  double l = static_cast<double>(gt) * 1.4426950408889634;
+  l = l < -200.0 ? -200.0 : l;
+  const double cum = wave_prefix(l), total = lane_value(cum, 63);
+  char* out = a.work + ((static_cast<int64_t>(b) * a.H + h) * a.C + c) * delta_chunk_bytes(PP);
+  uint16_t* tf = reinterpret_cast<uint16_t*>(out);
+  uint16_t* pf = tf + 3 * kDFrags * kDFragElems;
+  float* sc = reinterpret_cast<float*>(pf + PP * kDFrags * kDFragElems);
+  if (w == 0) {
+    cum_s[lane] = cum;
+    b_s[lane] = bt;
+    sc[lane] = exp2_d(cum);
+    sc[64 + lane] = exp2_d(total - cum) * (BACK ? 1.f : bt);
+    sc[128 + lane] = bt;
+    if (lane == 0) reinterpret_cast<int*>(sc)[192] = odd;
+  }
+  __syncthreads();
+
+  const int limit = odd < rows ? odd : rows;
+  B8 ki[S][NI], qi[S][NI];
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    if (16 * w + n >= limit) zero_u8<E>(ku[s]);
+    input_parts<E, NI>(ku[s], ki[s]);
+    input_parts<E, NI>(qu[s], qi[s]);
+  }
+  const double ci = cum_s[16 * w + n];
+  const float bi = b_s[16 * w + n];
+  for (int tj = 0; tj <= w; ++tj) {
+    f32x4 kk = {0.f, 0.f, 0.f, 0.f}, qk = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      B8 kj[NI];
+      input_parts<E, NI>(load(kp, a.kt, tj, s, limit), kj);
+      kk = mma_parts<3>(kj, ki[s], kk);                  // column i = 16 w + n, rows j = 16 tj + 4 g + r
+      if (BACK) qk = mma_parts<3>(qi[s], kj, qk);        // column j = 16 tj + n, rows i = 16 w + 4 g + r
+      else qk = mma_parts<3>(kj, qi[s], qk);
+    }
+    float x[4], y[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = 16 * w + n, j = 16 * tj + 4 * g + r;
+      const float wt = j <= i ? exp2_d(ci - cum_s[j]) : 0.f;
+      x[r] = j < i ? wt * kk[r] * (BACK ? bi : b_s[j]) : 0.f;
+      if (BACK) {
+        const int i2 = 16 * w + 4 * g + r, j2 = 16 * tj + n;
+        y[r] = j2 <= i2 ? exp2_d(cum_s[i2] - cum_s[j2]) * qk[r] : 0.f;
+      } else {
+        y[r] = j <= i ? wt * qk[r] * b_s[j] : 0.f;
+      }
+    }
+    *reinterpret_cast<float4*>(&A[(16 * w + n) * kTriStride + 16 * tj + 4 * g]) = make_float4(x[0], x[1], x[2], x[3]);
+    // Half a fragment: slots 0-3 are the first tile of the reduction's step, 4-7 the second.
+    const int frag = BACK ? upper_frag(tj, w >> 1) : lower_frag(w, tj >> 1), half = (BACK ? w : tj) & 1;
+    float rest[4] = {y[0], y[1], y[2], y[3]};
+#pragma unroll
+    for (int p = 0; p < PP; ++p) {
+      const uint2 v = make_uint2(pack2<BF16>(rest[0], rest[1]), pack2<BF16>(rest[2], rest[3]));
+      uint16_t* to = pf + (frag * PP + p) * kDFragElems + 8 * lane;
+      *reinterpret_cast<uint2*>(to + 4 * half) = v;
+      // The half of a step that lies beyond the diagonal.
+      if (BACK ? tj == w && half == 1 && (tj & 1) == 1 : tj == w && half == 0)
+        *reinterpret_cast<uint2*>(to + 4 * (1 - half)) = make_uint2(0u, 0u);
+      const uint16_t q[4] = {static_cast<uint16_t>(v.x), static_cast<uint16_t>(v.x >> 16), static_cast<uint16_t>(v.y),
+                             static_cast<uint16_t>(v.y >> 16)};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) rest[r] = part_rest<BF16>(rest[r], q[r]);
+    }
+  }
+  __syncthreads();
+
+  // Diagonal blocks, column n of block w in the registers of lane n (four times over).
+  auto tile = [](float* m, int i, int j) { return m + 16 * i * kTriStride + 16 * j; };
+  {
+    const float* d = tile(A, w, w);
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = i == n ? 1.f : 0.f;
+#pragma unroll
+    for (int j = 0; j < 15; ++j) {
+#pragma unroll
+      for (int i = j + 1; i < 16; ++i) x[i] = fmaf(-d[i * kTriStride + j], x[j], x[i]);
+    }
+    float* m = tile(M, w, w);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if ((i >> 2) == g) m[i * kTriStride + n] = x[i];
+  }
+  __syncthreads();
+  // The products wait in the tiles of A above the diagonal.
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  if (w < 2) put16(tile(A, 2 * w, 2 * w + 1), mm16(tile(A, 2 * w + 1, 2 * w), tile(M, 2 * w, 2 * w), zero));
+  __syncthreads();
+  if (w < 2) put16(tile(M, 2 * w + 1, 2 * w), -mm16(tile(M, 2 * w + 1, 2 * w + 1), tile(A, 2 * w, 2 * w + 1), zero));
+  __syncthreads();
+  {
+    const int i = 2 + (w >> 1), j = w & 1;
+    f32x4 y = mm16(tile(A, i, 1), tile(M, 1, j), zero);
+    if (j == 0) y = mm16(tile(A, i, 0), tile(M, 0, 0), y);
+    put16(tile(A, j, i), y);
+    __syncthreads();
+    f32x4 z = mm16(tile(M, i, 2), tile(A, j, 2), zero);
+    if (i == 3) z = mm16(tile(M, 3, 3), tile(A, j, 3), z);
+    put16(tile(M, i, j), -z);
+  }
+  __syncthreads();
+  // Into fragments: forward rows i with slots over j, backward rows j with slots over i.
+  const int f0 = BACK ? (w < 2 ? 0 : 1) : 0, f1 = BACK ? 1 : (w < 2 ? 0 : 1);
+  for (int s = f0; s <= f1; ++s) {
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int row = 16 * w + n, k = 32 * s + (e < 4 ? 4 * g + e : 16 + 4 * g + e - 4);
+      if (BACK) v[e] = k >= row ? M[k * kTriStride + row] : 0.f;
+      else v[e] = k <= row ? M[row * kTriStride + k] : 0.f;
+    }
+    B8 f[3];
+    split_frag<BF16, 3>(v, f);
+    const int frag = BACK ? upper_frag(w, s) : lower_frag(w, s);
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+      *reinterpret_cast<uint4*>(tf + (frag * 3 + p) * kDFragElems + 8 * lane) = __builtin_bit_cast(uint4, f[p]);
+  }
+}
+
+// LDS of a walk: keys and queries as their parts, values, the chunk's scalars.
+template <class E, int NK>
+struct WalkLds {
+  using KT = SelTile<BF16, NK, true>;
+  using QT = SelTile<BF16, NK, false>;
+  using VT = SelTile<E, kDCols, true>;
+  static constexpr int NI = DParts<E>::IN;
+  static constexpr int kpart = kDTokens * KT::STRIDE, qpart = kDTokens * QT::STRIDE;
+  static constexpr size_t k = 0, q = k + NI * kpart * 2, v = q + NI * qpart * 2,
+                          s = v + kDTokens * VT::STRIDE * sizeof(typename ET<E>::raw), bytes = s + 128 * 4;
+};
+
+// One workgroup walks 64 value columns of a head over the whole sequence; a wave holds 16 of them, its state in
+// accumulators (the state's columns never meet: each wave's chain is its own).  Accumulators of K S^T, of m and of the state
+// lie as the next product's operand wants them, so nothing but the inputs passes through LDS.
+template <class E, int NK, bool VEC>
+__global__ __launch_bounds__(kWalkThreads) void delta_walk_kernel(DeltaArgs a) {
+  using raw = typename ET<E>::raw;
+  using L = WalkLds<E, NK>;
+  using KT = typename L::KT;
+  using QT = typename L::QT;
+  using VT = typename L::VT;
+  constexpr int NI = L::NI, NO = DParts<E>::OUT, S = NK / 32, NT = NK / 16;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  uint16_t* kt = reinterpret_cast<uint16_t*>(lds + L::k);
+  uint16_t* qt = reinterpret_cast<uint16_t*>(lds + L::q);
+  raw* vt = reinterpret_cast<raw*>(lds + L::v);
+  float* sc = reinterpret_cast<float*>(lds + L::s);
+  const int tid = threadIdx.x, lane = lane_id(), w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, n = lane & 15;
+  const uint32_t at = xcd_order(blockIdx.x, gridDim.x);
+  const int pt = static_cast<int>(at % a.PT), h = static_cast<int>(at / a.PT % a.H), b = static_cast<int>(at / a.PT / a.H);
+  const int64_t len = delta_length(a, b);
+  const int col0 = pt * kDCols, p0 = col0 + 16 * w, gi = h / (a.H / a.G);
+  const int chunks = static_cast<int>((len + kDTokens - 1) / kDTokens);
+  const float inf = __builtin_inff();
+
+  const raw* kp = static_cast<const raw*>(a.keys) + b * a.kb + static_cast<int64_t>(gi) * a.N;
+  const raw* qp = static_cast<const raw*>(a.queries) + b * a.qb + static_cast<int64_t>(gi) * a.N;
+  const raw* vp = static_cast<const raw*>(a.values) + b * a.vb + static_cast<int64_t>(h) * a.P + col0;
+  const char* work = a.work + (static_cast<int64_t>(b) * a.H + h) * a.C * delta_chunk_bytes(NO);
+  TileLoad<E, KT, BF16, VEC, kDTokens, NK, kWalkThreads> kl;
+  TileLoad<E, QT, BF16, VEC, kDTokens, NK, kWalkThreads> ql;
+  TileLoad<E, VT, E, VEC, kDTokens, kDCols, kWalkThreads> vl;
+  kl.init(a.kt, a.N, tid);
+  ql.init(a.qt, a.N, tid);
+  vl.init(a.vt, a.P - col0 < kDCols ? a.P - col0 : kDCols, tid);
+  float sreg = 0.f;
+  int odd_next = 64;
+  auto fetch = [&](int c) {
+    const int64_t t0 = static_cast<int64_t>(c) * kDTokens;
+    kl.load(kp + t0 * a.kt, len - t0, tid);
+    ql.load(qp + t0 * a.qt, len - t0, tid);
+    vl.load(vp + t0 * a.vt, len - t0, tid);
+    const float* s = reinterpret_cast<const float*>(work + c * delta_chunk_bytes(NO) + (3 + NO) * kDFrags * kDFragElems * 2);
+    if (tid < 128) sreg = s[tid];
+    odd_next = reinterpret_cast<const int*>(s)[192];
+  };
+
+  f32x4 st[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) st[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int64_t head = static_cast<int64_t>(b) * a.H + h, cells = static_cast<int64_t>(a.P) * a.N;
+  if (a.memory != nullptr) state_add<NT>(st, a.memory + head * cells, p0, a.P, a.N, 1.f);
+  if (chunks > 0) fetch(0);
+
+  for (int c = 0; c < chunks; ++c) {
+    const int64_t t0 = static_cast<int64_t>(c) * kDTokens;
+    const int odd_key = odd_next;
+    __syncthreads();
+    store_parts<KT, NI, E>(kl, kt, L::kpart, odd_key, tid);
+    store_parts<QT, NI, E>(ql, qt, L::qpart, kDTokens, tid);
+    vl.store(vt, tid);
+    if (tid < 128) sc[tid] = sreg;
+    __syncthreads();
+    if (c + 1 < chunks) fetch(c + 1);
+    const uint16_t* tf = reinterpret_cast<const uint16_t*>(work + c * delta_chunk_bytes(NO));
+    const uint16_t* pf = tf + 3 * kDFrags * kDFragElems;
+    if (a.states != nullptr)
+      state_store<NT>(st, a.states + ((static_cast<int64_t>(b) * a.C + c) * a.H + h) * cells, p0, a.P, a.N);
+
+    // K S^T (a token a row, a value a column) and Q S^T (transposed, as its rows are stored).
+    B8 sp[S][3];
+#pragma unroll
+    for (int s = 0; s < S; ++s) split_pair<BF16, 3>(st[2 * s], st[2 * s + 1], sp[s]);
+    f32x4 x[4], o[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      x[t] = o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        B8 kf[NI], qf[NI], so[NO];
+        row_parts_t<KT, NI>(kt, L::kpart, 16 * t, 32 * s, kf);
+        row_parts_t<QT, NI>(qt, L::qpart, 16 * t, 32 * s, qf);
+#pragma unroll
+        for (int p = 0; p < NO; ++p) so[p] = sp[s][p];
+        x[t] = mma_parts<3>(kf, sp[s], x[t]);
+        o[t] = mma_parts<NO>(so, qf, o[t]);
+      }
+    }
+    // V - D K S^T.
+    f32x4 rt[4];
+    bool any = false;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const Frag8<E> vf = col_frag<VT, E>(vt, 32 * s, 16 * w);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float4 d = *reinterpret_cast<const float4*>(sc + 32 * s + 16 * i + 4 * g);
+        const float dd[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float v = fmaf(-dd[r], x[2 * s + i][r], ET<E>::to_f(vf.e[4 * i + r]));
+          rt[2 * s + i][r] = v;
+          any |= !(fabsf(v) < inf);
+        }
+      }
+    }
+    // A value, key or state that is no number: from its token on the column is NaN.  Its rows stay out of the products,
+    // whose zeros would not keep them out of earlier tokens' sums.
+    int cut = 64;
+    if (__any(any) || odd_key < 64) {
+      auto first = [&](const f32x4 (&y)[4]) {
+        int f = 64;
+#pragma unroll
+        for (int t = 3; t >= 0; --t) {
+#pragma unroll
+          for (int r = 3; r >= 0; --r)
+            if (!(fabsf(y[t][r]) < inf)) f = 16 * t + 4 * g + r;
+        }
+        const int f1 = __shfl_xor(f, 16), f2 = f < f1 ? f : f1, f3 = __shfl_xor(f2, 32);
+        return f2 < f3 ? f2 : f3;
+      };
+      cut = first(rt);
+      cut = cut < odd_key ? cut : odd_key;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (16 * t + 4 * g + r >= cut) rt[t][r] = 0.f;
+      }
+    }
+    // m.
+    f32x4 m[4];
+    {
+      B8 rp[2][3];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) split_pair<BF16, 3>(rt[2 * s], rt[2 * s + 1], rp[s]);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        m[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s <= t / 2; ++s) {
+          B8 f[3];
+          stored_parts<3>(tf, lower_frag(t, s), f, lane);
+          m[t] = mma_parts<3>(f, rp[s], m[t]);
+        }
+      }
+    }
+    if (a.miss != nullptr && p0 + n < a.P) {
+      float* to = a.miss + ((static_cast<int64_t>(b) * a.T + t0) * a.H + h) * a.P + p0 + n;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int tok = 16 * t + 4 * g + r;
+          if (t0 + tok < len) to[static_cast<int64_t>(tok) * a.H * a.P] = m[t][r];
+        }
+      }
+    }
+    // H^T = S Q^T D + m^T P^T.
+    {
+      B8 mp[2][NO];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) split_pair<BF16, NO>(m[2 * s], m[2 * s + 1], mp[s]);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        o[t] *= sc[16 * t + n];
+#pragma unroll
+        for (int s = 0; s <= t / 2; ++s) {
+          B8 f[NO];
+          stored_parts<NO>(pf, lower_frag(t, s), f, lane);
+          o[t] = mma_parts<NO>(mp[s], f, o[t]);
+        }
+      }
+    }
+    if (__any(cut < 64)) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int f = __shfl(cut, 4 * g + r);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          if (16 * t + n >= f) o[t][r] = __builtin_nanf("");
+      }
+    }
+    {
+      const int p = p0 + 4 * g;
+      raw* to = static_cast<raw*>(a.hidden) + ((static_cast<int64_t>(b) * a.T + t0) * a.H + h) * a.P + p;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int tok = 16 * t + n;
+        if (t0 + tok < a.T) {
+          raw* row = to + static_cast<int64_t>(tok) * a.H * a.P;
+          if (VEC) {
+            if (p < a.P) store4_raw<E>(row, o[t]);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (p + r < a.P) row[r] = ET<E>::from_f(o[t][r]);
+          }
+        }
+      }
+    }
+    // S' = e^{c_63} S + (E b m)^T K.
+    {
+      const float keep = sc[63];
+#pragma unroll
+      for (int i = 0; i < NT; ++i) st[i] *= keep;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        f32x4 em[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float4 e = *reinterpret_cast<const float4*>(sc + 64 + 32 * s + 16 * i + 4 * g);
+          em[i] = f32x4{m[2 * s + i][0] * e.x, m[2 * s + i][1] * e.y, m[2 * s + i][2] * e.z, m[2 * s + i][3] * e.w};
+        }
+        B8 ep[3];
+        split_pair<BF16, 3>(em[0], em[1], ep);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          B8 kf[NI];
+          col_parts<KT, NI>(kt, L::kpart, 32 * s, 16 * i, kf);
+          st[i] = mma_parts<3>(kf, ep, st[i]);
+        }
+      }
+    }
+    if (cut < 64) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) st[i] = f32x4{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
+    }
+  }
+  state_store<NT>(st, a.memory_out + head * cells, p0, a.P, a.N);
+  // Rows behind the last chunk.
+  for (int64_t t = static_cast<int64_t>(chunks) * kDTokens + tid / 16; t < a.T; t += kWalkThreads / 16) {
+    raw* row = static_cast<raw*>(a.hidden) + ((b * a.T + t) * a.H + h) * a.P + col0;
+    for (int p = tid % 16; p < kDCols && col0 + p < a.P; p += 16) row[p] = 0;
+  }
+}
+
+// One token.  LPR lanes share a state row; both dot products with the row are taken from the state as it was, so
+// that it is read and written once: M q = a (M0 q) + u (k.q).
+template <class E, int LPR>
+__global__ __launch_bounds__(kStepThreads) void delta_step_kernel(DeltaArgs a) {
+  using raw = typename ET<E>::raw;
+  constexpr int RPW = 64 / LPR, U = 4;
+  const int lane = lane_id(), wave = static_cast<int>(threadIdx.x) >> 6;
+  const uint32_t head = blockIdx.x;
+  const int h = static_cast<int>(head % a.H), b = static_cast<int>(head / a.H), gi = h / (a.H / a.G);
+  const int col = 4 * (lane % LPR);
+  const bool whole = (a.N & 3) == 0;
+  float k[4], q[4];
+  const raw* kp = static_cast<const raw*>(a.keys) + b * a.kb + static_cast<int64_t>(gi) * a.N;
+  const raw* qp = static_cast<const raw*>(a.queries) + b * a.qb + static_cast<int64_t>(gi) * a.N;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const bool in = col + r < a.N;
+    k[r] = in ? ET<E>::to_f(kp[col + r]) : 0.f;
+    q[r] = in ? ET<E>::to_f(qp[col + r]) : 0.f;
+  }
+  const int64_t is = b * a.sb + h, id = b * a.db + h;
+  const float bt = a.s_f32 ? static_cast<const float*>(a.strengths)[is] : ET<E>::to_f(static_cast<const raw*>(a.strengths)[is]);
+  float keep = 1.f;
+  if (a.decays != nullptr)
+    keep = expf(a.d_f32 ? static_cast<const float*>(a.decays)[id] : ET<E>::to_f(static_cast<const raw*>(a.decays)[id]));
+  const raw* xp = static_cast<const raw*>(a.values) + b * a.vb + static_cast<int64_t>(h) * a.P;
+  const float* mp = a.memory + static_cast<int64_t>(head) * a.P * a.N;
+  float* op = a.memory_out + static_cast<int64_t>(head) * a.P * a.N;
+  raw* hp = static_cast<raw*>(a.hidden) + static_cast<int64_t>(head) * a.P;
+  const int stride = static_cast<int>(gridDim.y) * 4 * RPW * U;
+  for (int p0 = (static_cast<int>(blockIdx.y) * 4 + wave) * RPW * U; p0 < a.P; p0 += stride) {
+    f32x4 m[U];
+    float x[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int p = p0 + i * RPW + lane / LPR;
+      m[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      x[i] = p < a.P ? ET<E>::to_f(xp[p]) : 0.f;
+      if (p < a.P && col < a.N) {
+        const float* s = mp + static_cast<int64_t>(p) * a.N + col;
+        if (whole) {
+          m[i] = *reinterpret_cast<const f32x4*>(s);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) m[i][r] = col + r < a.N ? s[r] : 0.f;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int p = p0 + i * RPW + lane / LPR;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) m[i][r] *= keep;
+      float mk = fmaf(m[i][0], k[0], fmaf(m[i][1], k[1], fmaf(m[i][2], k[2], m[i][3] * k[3])));
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) mk += __shfl_xor(mk, o);
+      const float u = bt * (x[i] - mk);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) m[i][r] = fmaf(u, k[r], m[i][r]);
+      float y = fmaf(m[i][0], q[0], fmaf(m[i][1], q[1], fmaf(m[i][2], q[2], m[i][3] * q[3])));
+#pragma unroll
+      for (int o = LPR / 2; o > 0; o >>= 1) y += __shfl_xor(y, o);
+      if (p < a.P && col < a.N) {
+        float* s = op + static_cast<int64_t>(p) * a.N + col;
+        if (whole) {
+          *reinterpret_cast<f32x4*>(s) = m[i];
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (col + r < a.N) s[r] = m[i][r];
+        }
+      }
+      if (p < a.P && lane % LPR == 0) hp[p] = ET<E>::from_f(y);
+    }
+  }
+}
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int set_lds(const void* kernel, size_t bytes, const char* what) {
+  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (e != hipSuccess) {
+    set_error("%s: %s", what, hipGetErrorString(e));
+    return static_cast<int>(e);
+  }
+  return GRM_HIP_OK;
+}
+
+int out_parts(int dtype) { return dtype == GRM_HIP_F32 ? 3 : 2; }
+
+}  // namespace
+
+int delta_check(const grm_hip_delta_args* u, const char* what, bool step) {
+  auto bad = [&](const char* why) {
+    set_error("%s: %s", what, why);
+    return GRM_HIP_EINVAL;
+  };
+  if (u == nullptr) return bad("no arguments");
+  if (u->batch < 0 || u->seq_len < 0 || u->heads < 1 || u->value_dim < 1 || u->groups < 1 || u->key_dim < 1)
+    return bad("batch and seq_len must be >= 0, the other sizes >= 1");
+  if (u->heads % u->groups != 0) return bad("heads must be a multiple of groups");
+  if (u->dtype < 0 || u->dtype > 2 || (u->strengths_dtype != u->dtype && u->strengths_dtype != GRM_HIP_F32) ||
+      (u->decays_dtype != u->dtype && u->decays_dtype != GRM_HIP_F32)) {
+    set_error("%s: keys, values and queries must be float32, float16 or bfloat16, strengths and log_decays the same or float32", what);
+    return GRM_HIP_EUNSUPPORTED;
+  }
+  if (u->key_dim > 128) {
+    set_error("%s: key_dim must be <= 128, got %lld", what, static_cast<long long>(u->key_dim));
+    return GRM_HIP_EUNSUPPORTED;
+  }
+  const int64_t most = int64_t{1} << 21;
+  if (u->seq_len > (1 << 30)) {
+    set_error("%s: seq_len must be at most 2^30", what);
+    return GRM_HIP_EUNSUPPORTED;
+  }
+  // (One by one first: no product passes 63 bits.)
+  if (u->heads > most || u->value_dim > most || u->groups > most || u->keys_token_stride < 0 ||
+      u->keys_token_stride > most || u->values_token_stride < 0 || u->values_token_stride > most ||
+      u->queries_token_stride < 0 || u->queries_token_stride > most || u->heads * u->value_dim > most ||
+      u->groups * u->key_dim > most) {
+    set_error("%s: token strides and row widths must be at most 2^21 elements", what);
+    return GRM_HIP_EUNSUPPORTED;
+  }
+  // (A grid dimension has fewer than 2^32 threads; every kernel here has 256 a workgroup.)
+  const int64_t seqs = u->heads * min_i64(u->batch, int64_t{1} << 32), grid = int64_t{1} << 24;
+  const int64_t tiles = (u->value_dim + kDCols - 1) / kDCols, chunks = (u->seq_len + kDTokens - 1) / kDTokens;
+  if (seqs >= grid || (!step && (seqs * tiles >= grid || seqs * chunks >= grid))) {
+    set_error(step ? "%s: batch * heads must be below 2^24"
+                   : "%s: batch * heads * ceil(value_dim / 64) and batch * heads * ceil(seq_len / 64) must be below 2^24", what);
+    return GRM_HIP_EUNSUPPORTED;
+  }
+  if (u->seq_len > 1 && (u->keys_token_stride < u->groups * u->key_dim || u->queries_token_stride < u->groups * u->key_dim ||
+                         u->values_token_stride < u->heads * u->value_dim))
+    return bad("token strides must not be below a row's width");
+  if (u->batch > 0 && u->seq_len > 0 &&
+      (u->keys == nullptr || u->values == nullptr || u->queries == nullptr || u->strengths == nullptr))
+    return bad("keys, values, queries and strengths are required");
+  if (!aligned(u->memory)) return bad("memory must be 16-byte aligned");
+  return GRM_HIP_OK;
+}
+
+DeltaArgs delta_args(const grm_hip_delta_args* u) {
+  DeltaArgs a{};
+  a.keys = u->keys; a.values = u->values; a.queries = u->queries;
+  a.strengths = u->strengths; a.decays = u->log_decays; a.lengths = u->lengths; a.memory = u->memory;
+  a.kb = u->keys_batch_stride; a.kt = u->keys_token_stride;
+  a.vb = u->values_batch_stride; a.vt = u->values_token_stride;
+  a.qb = u->queries_batch_stride; a.qt = u->queries_token_stride;
+  a.sb = u->strengths_batch_stride; a.st = u->strengths_token_stride;
+  a.db = u->decays_batch_stride; a.dt = u->decays_token_stride;
+  a.T = u->seq_len;
+  a.B = static_cast<int>(u->batch); a.H = static_cast<int>(u->heads); a.P = static_cast<int>(u->value_dim);
+  a.G = static_cast<int>(u->groups); a.N = static_cast<int>(u->key_dim);
+  a.C = static_cast<int>((u->seq_len + kDTokens - 1) / kDTokens);
+  a.PT = static_cast<int>((u->value_dim + kDCols - 1) / kDCols);
+  a.s_f32 = u->strengths_dtype == GRM_HIP_F32;
+  a.d_f32 = u->decays_dtype == GRM_HIP_F32;
+  // Whole 16-byte loads where every row of 8-element units allows them.
+  a.vec = u->value_dim % 8 == 0 && u->key_dim % 8 == 0 && aligned(u->keys) && aligned(u->values) &&
+          aligned(u->queries) && (u->keys_batch_stride | u->keys_token_stride | u->values_batch_stride |
+                                  u->values_token_stride | u->queries_batch_stride | u->queries_token_stride) % 8 == 0;
+  return a;
+}
+
+int launch_delta_prep(const DeltaArgs& a, int dtype, bool back, hipStream_t stream, const char* what) {
+  int rc = GRM_HIP_OK;
+  delta_with_form(dtype, a.N, true, [&](auto e, auto nk, auto) {
+    using E = decltype(e);
+    constexpr int NK = decltype(nk)::value;
+    const dim3 grid(static_cast<uint32_t>(a.B) * a.H * a.C);
+    if (back) delta_prep_kernel<E, NK, true><<<grid, dim3(kPrepThreads), 0, stream>>>(a);
+    else delta_prep_kernel<E, NK, false><<<grid, dim3(kPrepThreads), 0, stream>>>(a);
+    rc = check_launch(what);
+  });
+  return rc;
+}
+
+}  // namespace grmhip
+
+using namespace grmhip;
+
+extern "C" int64_t grm_hip_delta_scan_workspace(int64_t batch, int64_t seq_len, int64_t heads, int dtype) {
+  if (batch <= 0 || seq_len <= 0 || heads <= 0 || dtype < 0 || dtype > 2) return 0;
+  return batch * heads * ((seq_len + kDTokens - 1) / kDTokens) * delta_chunk_bytes(out_parts(dtype));
+}
+
+extern "C" int grm_hip_delta_scan_fwd(const grm_hip_delta_args* u, void* hidden, float* memory_out, float* states,
+                                      float* miss, void* workspace, int64_t workspace_bytes, void* stream) {
+  const char* what = "delta_scan";
+  if (int rc = delta_check(u, what, false)) return rc;
+  if (u->batch == 0) return GRM_HIP_OK;
+  const int64_t state_bytes = u->batch * u->heads * u->value_dim * u->key_dim * 4;
+  if (memory_out == nullptr || (u->seq_len > 0 && hidden == nullptr) || !aligned(memory_out) || !aligned(states)) {
+    set_error("%s: hidden and memory_out are required, memory_out and states 16-byte aligned", what);
+    return GRM_HIP_EINVAL;
+  }
+  if (ranges_overlap(u->memory, state_bytes, memory_out, state_bytes)) {
+    set_error("%s: memory_out may not overlap memory", what);
+    return GRM_HIP_EINVAL;
+  }
+  DeltaArgs a = delta_args(u);
+  a.hidden = hidden; a.memory_out = memory_out; a.states = states; a.miss = miss;
+  a.work = static_cast<char*>(workspace);
+  if (a.C > 0) {
+    if (workspace == nullptr || !aligned(workspace) ||
+        workspace_bytes < grm_hip_delta_scan_workspace(u->batch, u->seq_len, u->heads, u->dtype)) {
+      set_error("%s: workspace missing, misaligned or too small", what);
+      return GRM_HIP_EINVAL;
+    }
+    if (int rc = launch_delta_prep(a, u->dtype, false, static_cast<hipStream_t>(stream), what)) return rc;
+  }
+  int rc = GRM_HIP_OK;
+  delta_with_form(u->dtype, a.N, a.vec != 0 && aligned(hidden), [&](auto e, auto nk, auto vec) {
+    using E = decltype(e);
+    constexpr int NK = decltype(nk)::value;
+    auto kernel = delta_walk_kernel<E, NK, decltype(vec)::value>;
+    constexpr size_t lds = WalkLds<E, NK>::bytes;
+    if ((rc = set_lds(reinterpret_cast<const void*>(kernel), lds, what)) != GRM_HIP_OK) return;
+    kernel<<<dim3(static_cast<uint32_t>(a.B) * a.H * a.PT), dim3(kWalkThreads), lds, static_cast<hipStream_t>(stream)>>>(a);
+    rc = check_launch(what);
+  });
+  return rc;
+}
+
+extern "C" int grm_hip_delta_step(const grm_hip_delta_args* u, void* hidden, float* memory_out, void* stream) {
+  const char* what = "delta_step";
+  if (int rc = delta_check(u, what, true)) return rc;
+  if (u->seq_len != 1 || u->lengths != nullptr) {
+    set_error("%s: seq_len must be 1, without lengths", what);
+    return GRM_HIP_EINVAL;
+  }
+  if (u->batch == 0) return GRM_HIP_OK;
+  if (u->memory == nullptr || hidden == nullptr || memory_out == nullptr || !aligned(memory_out)) {
+    set_error("%s: memory, hidden and memory_out are required, memory_out 16-byte aligned", what);
+    return GRM_HIP_EINVAL;
+  }
+  const int64_t state_bytes = u->batch * u->heads * u->value_dim * u->key_dim * 4;
+  if (memory_out != u->memory && ranges_overlap(u->memory, state_bytes, memory_out, state_bytes)) {
+    set_error("%s: memory_out must be memory itself or not overlap it", what);
+    return GRM_HIP_EINVAL;
+  }
+  DeltaArgs a = delta_args(u);
+  a.hidden = hidden; a.memory_out = memory_out;
+  auto go = [&](auto e, auto lpr) {
+    constexpr int LPR = decltype(lpr)::value, rows = 4 * (64 / LPR) * 4;  // of a workgroup at a time
+    const int64_t tiles = (a.P + rows - 1) / rows, most = 65535;  // a grid's second dimension; the kernel goes round
+    delta_step_kernel<decltype(e), LPR>
+        <<<dim3(static_cast<uint32_t>(a.B) * a.H, static_cast<uint32_t>(tiles < most ? tiles : most)), dim3(kStepThreads), 0,
+           static_cast<hipStream_t>(stream)>>>(a);
+  };
+  auto by_width = [&](auto e) {
+    if (a.N <= 16) go(e, std::integral_constant<int, 4>{});
+    else if (a.N <= 32) go(e, std::integral_constant<int, 8>{});
+    else if (a.N <= 64) go(e, std::integral_constant<int, 16>{});
+    else go(e, std::integral_constant<int, 32>{});
+  };
+  if (u->dtype == GRM_HIP_F32) by_width(F32{});
+  else if (u->dtype == GRM_HIP_F16) by_width(F16{});
+  else by_width(BF16{});
+  return check_launch(what);
+}

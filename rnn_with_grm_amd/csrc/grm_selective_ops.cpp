@@ -3,85 +3,14 @@
 // outputs and workspace with ATen on the inputs' device and calls the C ABI of libgrm_hip.so on
 // that device's current stream.  Inputs the kernels do not cover raise; CPU tensors take
 // cuda_ops' PyTorch forms and never reach these ops.
-#include <torch/extension.h>
-
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPStream.h>
-
-#include <initializer_list>
 #include <tuple>
 
-#include "grm_hip.h"
+#include "op_checks.h"
 
 namespace grm_selective {
 namespace {
 
-using at::Tensor;
-using OptTensor = c10::optional<Tensor>;
-
-int dtype_code(const Tensor& t, const char* op, const char* name) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return GRM_HIP_F32;
-    case at::kHalf: return GRM_HIP_F16;
-    case at::kBFloat16: return GRM_HIP_BF16;
-    default: break;
-  }
-  TORCH_CHECK_VALUE(false, op, ": ", name, " must be float32, float16 or bfloat16, got ", t.scalar_type());
-  return -1;
-}
-
-bool has(const OptTensor& t) { return t.has_value() && t->defined(); }
-
-void* stream_of(const Tensor& t) {
-  return static_cast<void*>(c10::hip::getCurrentHIPStream(t.device().index()).stream());
-}
-
-void check_rc(int rc, const char* op) {
-  TORCH_CHECK(rc == GRM_HIP_OK, op, " failed (", rc, "): ", grm_hip_last_error());
-}
-
-void check_device(const Tensor& t, const Tensor& like, const char* op, const char* name) {
-  TORCH_CHECK_VALUE(t.is_cuda() && t.device() == like.device(), op, ": ", name, " must be on ", like.device());
-}
-
-// Autograd's count of writes to an argument: a graph that saved it for its backward then refuses to use what it holds now.
-// (No graph can save a tensor made in inference mode, and it has no count.)
-void written(Tensor& t) {
-  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-}
-
-// A contiguous optional tensor's pointer; `keep` holds what it points into.
-void* opt_ptr(const OptTensor& t, Tensor& keep) {
-  if (!has(t)) return nullptr;
-  keep = t->contiguous();
-  return keep.data_ptr();
-}
-
-// Rows of the last `inner` dimensions packed, any stride between tokens and sequences: a slice of a
-// wider projection is read where it lies.
-Tensor packed_rows(const Tensor& t, int64_t inner) {
-  int64_t want = 1;
-  for (int64_t d = t.dim() - 1; d >= t.dim() - inner; --d) {
-    if (t.size(d) != 1 && t.stride(d) != want) return t.contiguous();
-    want *= t.size(d);
-  }
-  // Rows of a sequence lie one behind the other, near enough for 32-bit offsets inside a tile of tokens.
-  const int64_t d = t.dim() - inner - 1;
-  if (d > 0 && t.size(d) != 1 && (t.stride(d) < want || t.stride(d) > (int64_t{1} << 21))) return t.contiguous();
-  return t;
-}
-
-int64_t stride_of(const Tensor& t, int64_t dim, int64_t packed) { return t.size(dim) > 1 ? t.stride(dim) : packed; }
-
-const int64_t* lengths_ptr(const OptTensor& lengths, int64_t B, const Tensor& like, const char* op, Tensor& keep) {
-  if (!has(lengths)) return nullptr;
-  check_device(*lengths, like, op, "lengths");
-  TORCH_CHECK_VALUE(lengths->dim() == 1 && lengths->size(0) == B &&
-                  (lengths->scalar_type() == at::kLong || lengths->scalar_type() == at::kInt),
-              op, ": lengths must be int32 or int64 [batch]");
-  keep = lengths->to(at::kLong).contiguous();
-  return keep.data_ptr<int64_t>();
-}
+using namespace grm_ops;
 
 // ---------------------------------------------------------------------------
 // Short convolution.
@@ -200,19 +129,12 @@ std::tuple<Tensor, Tensor> short_conv_step(const Tensor& x, const Tensor& state,
 // ---------------------------------------------------------------------------
 // Selective scan.
 
-bool aligned16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
-
 // The checked inputs of a call and what keeps their memory alive.
 struct Scan {
   int64_t B, T, H, P, G, N;
   grm_hip_selective_args args;
   Tensor keys, values, queries, steps, rates, skip, bias, lengths, memory;
 };
-
-Tensor f32_state(const Tensor& t) {
-  Tensor m = t.contiguous();
-  return aligned16(m) ? m : m.clone();
-}
 
 // `step`: one token, without the length's dimension.
 Scan check_scan(const Tensor& keys, const Tensor& values, const Tensor& queries, const Tensor& steps,
@@ -278,10 +200,6 @@ Scan check_scan(const Tensor& keys, const Tensor& values, const Tensor& queries,
   strides(s.steps, s.H, &a.steps_batch_stride, &a.steps_token_stride);
   a.dtype = dt; a.steps_dtype = sdt; a.softplus = softplus;
   return s;
-}
-
-Tensor bytes(int64_t n, const Tensor& like) {
-  return at::empty({std::max<int64_t>(n, 16)}, like.options().dtype(at::kByte));
 }
 
 std::tuple<Tensor, Tensor, Tensor> selective_scan_forward(const Tensor& keys, const Tensor& values,

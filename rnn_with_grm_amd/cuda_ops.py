@@ -18,7 +18,8 @@ Deliberate differences:
   * New entry points: ``cuda_segment_scan``, ``cuda_topk_route``,
     ``cuda_segment_route``, ``cuda_gather_apply`` and ``cuda_fuse_residual``; the
     selective state scan and its short convolution (``cuda_selective_scan``,
-    ``cuda_selective_step``, ``cuda_short_conv``, ``cuda_short_conv_step``).
+    ``cuda_selective_step``, ``cuda_short_conv``, ``cuda_short_conv_step``); the gated
+    delta rule (``cuda_delta_scan``, ``cuda_delta_step``).
 """
 
 from __future__ import annotations
@@ -46,7 +47,7 @@ EXTRA_OPS = ("segment_scan_forward", "topk_route", "fuse_residual", "gather_appl
              "gather_apply_backward_tokens", "apply_query_backward_queries", "archive_cast", "project_gemm",
              "linear_residual_layer_norm", "segment_retrieve_fuse", "selective_scan_forward", "selective_scan_backward",
              "selective_step", "selective_step_out", "short_conv_forward", "short_conv_backward", "short_conv_step",
-             "short_conv_step_out")
+             "short_conv_step_out", "delta_scan_forward", "delta_scan_backward", "delta_step", "delta_step_out")
 
 # Environment variables of the reference (cuda_ops.py:26-32): one per op and a global one.
 GLOBAL_POLICY_ENV = "GRM_CUDA_KERNEL_POLICY"
@@ -1134,11 +1135,140 @@ def cuda_selective_step(keys: Tensor, values: Tensor, queries: Tensor, steps: Te
     return hidden[:, 0], moved if memory_out is None else memory_out.copy_(moved)
 
 
+# ---------------------------------------------------------------------------
+# Gated delta rule.  The reference has no counterpart; it is the linear memory above whose tokens first take out
+# what the memory holds under their key.
+
+def _check_delta(keys: Tensor, values: Tensor, queries: Tensor, strengths: Tensor, log_decays: Optional[Tensor],
+                 memory: Optional[Tensor]) -> None:
+    if keys.ndim != 4 or values.ndim != 4 or strengths.ndim != 3:
+        raise ValueError("delta_scan: keys and queries must be [batch, seq_len, groups, key_dim], values [batch, "
+                         "seq_len, heads, value_dim], strengths and log_decays [batch, seq_len, heads]")
+    B, T, H, P = values.shape
+    G, N = keys.shape[2:]
+    if (queries.shape != keys.shape or keys.shape[:2] != (B, T) or strengths.shape != (B, T, H) or
+            (log_decays is not None and log_decays.shape != (B, T, H))):
+        raise ValueError("delta_scan: keys, queries, values, strengths and log_decays must agree in batch, length and "
+                         "heads")
+    if G < 1 or H < 1 or P < 1 or H % G != 0 or not 1 <= N <= 128:
+        raise ValueError("delta_scan: heads must be a multiple of groups and key_dim in [1, 128]")
+    if not keys.dtype == values.dtype == queries.dtype or any(
+            t is not None and t.dtype not in (values.dtype, torch.float32) for t in (strengths, log_decays)):
+        raise ValueError("delta_scan: keys, values and queries must share a type, strengths and log_decays have it or "
+                         "float32")
+    if memory is not None and memory.shape != (B, H, P, N):
+        raise ValueError("delta_scan: memory must be [batch, heads, value_dim, key_dim]")
+
+
+def _torch_delta_scan(keys: Tensor, values: Tensor, queries: Tensor, strengths: Tensor, log_decays: Optional[Tensor],
+                      memory: Optional[Tensor], lengths: Optional[Tensor]) -> Tuple[Tensor, Tensor]:
+    """Token by token in float32 (float64 for float64 inputs)."""
+    _check_delta(keys, values, queries, strengths, log_decays, memory)
+    B, T, H, P = values.shape
+    G, N = keys.shape[2:]
+    cdt = torch.float64 if values.dtype == torch.float64 else torch.float32
+    state = values.new_zeros(B, H, P, N, dtype=cdt) if memory is None else memory.to(cdt)
+    v, k, q, b = values.to(cdt), keys.to(cdt), queries.to(cdt), strengths.to(cdt)
+    g = torch.zeros_like(b) if log_decays is None else log_decays.to(cdt)
+    live = _live_tokens(lengths, B, T, values.device)
+    if live is not None:
+        b, g = b.masked_fill(~live[..., None], 0.0), g.masked_fill(~live[..., None], 0.0)
+        v, k, q = (t.masked_fill(~live[..., None, None], 0.0) for t in (v, k, q))
+    outs = []
+    for t in range(T):
+        kt, qt = (x[:, t].repeat_interleave(H // G, 1)[..., None, :] for x in (k, q))
+        moved = torch.exp(g[:, t])[..., None, None] * state
+        moved = moved + (b[:, t, :, None] * (v[:, t] - (moved * kt).sum(-1)))[..., None] * kt
+        if live is not None:  # a state that is no number stays as it is behind the length
+            moved = torch.where(live[:, t, None, None, None], moved, state)
+        state, h = moved, (moved * qt).sum(-1)
+        outs.append(h if live is None else h.masked_fill(~live[:, t, None, None], 0.0))
+    hidden = torch.stack(outs, 1) if outs else v.new_zeros(B, 0, H, P)
+    return hidden.to(values.dtype), state if T else state.clone()  # (of no tokens: not the caller's own tensor)
+
+
+class _DeltaScanFn(torch.autograd.Function):
+    """The delta rule; where gradients are wanted the forward also keeps the float32 state before every
+    64 tokens and what each token's value missed, from which the backward forms all gradients."""
+
+    @staticmethod
+    def forward(ctx, keys, values, queries, strengths, log_decays, memory, lengths):
+        hidden, memory_out, states, miss = torch.ops.grm_cuda.delta_scan_forward(
+            keys, values, queries, strengths, log_decays, memory, lengths, True)
+        ctx.has_memory = memory is not None
+        # (Not the first state: the backward does not read it, and a caller may move it in place.)
+        ctx.save_for_backward(keys, values, queries, strengths, log_decays, lengths, states, miss)
+        ctx.set_materialize_grads(False)
+        return hidden, memory_out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_hidden, grad_memory_out):
+        keys, values, queries, strengths, log_decays, lengths, states, miss = ctx.saved_tensors
+        dk, dv, dq, db, dg, dm = torch.ops.grm_cuda.delta_scan_backward(
+            grad_hidden, grad_memory_out, keys, values, queries, strengths, log_decays, lengths, states, miss)
+        return dk, dv, dq, db, None if log_decays is None else dg, dm if ctx.has_memory else None, None
+
+
+def cuda_delta_scan(keys: Tensor, values: Tensor, queries: Tensor, strengths: Tensor,
+                    log_decays: Optional[Tensor] = None, memory: Optional[Tensor] = None, *,
+                    lengths: Optional[Tensor] = None, enabled: bool = True,
+                    debug_fallback: bool = False) -> Tuple[Tensor, Tensor]:
+    """Linear memory whose tokens replace what it holds under their key (the gated delta rule).  With
+    ``a_t = exp(log_decays_t)`` (None: 1) and ``u_t = strengths_t (v_t - a_t M_{t-1} k_t)``,
+    ``M_t = a_t M_{t-1} + u_t k_t^T`` and ``h_t = M_t q_t``.
+
+    keys, queries [B, T, G, N] (a group's row is shared by H / G heads; keys of about unit length keep the
+    state bounded for strengths in [0, 1]), values [B, T, H, P] in one type (float32, float16 or bfloat16),
+    strengths and log_decays [B, T, H] in that type or float32, memory [B, H, P, N] the state before token 0
+    (used in float32; None: zeros), lengths [B] the tokens of each sequence of a padded batch (clamped to
+    [0, T]; the tokens behind are not read, leave the state alone and come out as zeros).  The last two
+    dimensions of keys, values and queries are packed; a slice of a wider row is read in place.  Returns
+    (hidden [B, T, H, P], memory_out [B, H, P, N] float32).  Differentiable once, backwards, in all but
+    lengths (forward-mode derivatives are refused on the GPU).  An infinity or a NaN reaches no earlier
+    token's row (on the GPU what depends on it is NaN from its token on: of a value its column, of a query its
+    row, else the head); in the backward it may reach any gradient of its sequence.  Limits: N <= 128."""
+    if values.is_cuda and _run_native("delta_scan", values.device, enabled=enabled, debug_fallback=debug_fallback):
+        args = (keys, values, queries, strengths, log_decays, _f32(memory), lengths)
+        if _wants_grad(keys, values, queries, strengths, log_decays, memory):
+            return _DeltaScanFn.apply(*args)
+        return torch.ops.grm_cuda.delta_scan_forward(*args, False)[:2]
+    return _torch_delta_scan(keys, values, queries, strengths, log_decays, memory, lengths)
+
+
+def cuda_delta_step(keys: Tensor, values: Tensor, queries: Tensor, strengths: Tensor, log_decays: Optional[Tensor],
+                    memory: Tensor, *, memory_out: Optional[Tensor] = None, enabled: bool = True,
+                    debug_fallback: bool = False) -> Tuple[Tensor, Tensor]:
+    """One token of ``cuda_delta_scan``: keys, queries [B, G, N], values [B, H, P], strengths and log_decays
+    [B, H], memory [B, H, P, N] float32.  Returns (hidden [B, H, P], the state moved by this token).
+    ``memory_out`` takes that state; with ``memory_out=memory`` it is updated in place, as a serving loop or
+    a captured graph keeps it."""
+    grad = _wants_grad(keys, values, queries, strengths, log_decays, memory)
+    if memory_out is not None:
+        _check_out(memory_out, memory, "memory_out", grad)
+    if not grad and values.is_cuda and _run_native("delta_scan", values.device, enabled=enabled,
+                                                   debug_fallback=debug_fallback):
+        args = (keys, values, queries, strengths, log_decays, memory)
+        if memory_out is None:
+            return torch.ops.grm_cuda.delta_step(*args)
+        return torch.ops.grm_cuda.delta_step_out(*args, memory_out), memory_out
+    if values.ndim != 3 or keys.ndim != 3 or queries.ndim != 3 or strengths.ndim != 2 or (
+            log_decays is not None and log_decays.ndim != 2):
+        raise ValueError("delta_step: keys and queries must be [batch, groups, key_dim], values [batch, heads, "
+                         "value_dim], strengths and log_decays [batch, heads]")
+    hidden, moved = cuda_delta_scan(keys[:, None], values[:, None], queries[:, None], strengths[:, None],
+                                    None if log_decays is None else log_decays[:, None], memory, enabled=enabled,
+                                    debug_fallback=debug_fallback)
+    return hidden[:, 0], moved if memory_out is None else memory_out.copy_(moved)
+
+
 __all__ = [
     "GrmExtensionUnavailable",
     "cuda_apply_query",
     "cuda_batched_memory_gather",
     "cuda_chunk_update",
+    "cuda_delta_scan",
+    "cuda_delta_step",
     "cuda_fuse_residual",
     "cuda_gather_apply",
     "cuda_linear_residual_layer_norm",
