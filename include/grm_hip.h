@@ -647,6 +647,31 @@ int grm_hip_delta_scan_bwd(const grm_hip_delta_args* args, const float* states, 
  */
 int grm_hip_delta_step(const grm_hip_delta_args* args, void* hidden, float* memory_out, void* stream);
 
+/*
+ * Group norm of rows with their channels last, and its activation or gate.  No counterpart in the reference.
+ *   n = (x - mean) / sqrt(var + eps) over each of `groups` equal groups of a row's channels
+ *       (center = 0: x / sqrt(mean(x^2) + eps)),  y = n weight + bias
+ *   out = y act(gate), without a gate act(y);  act = silu ? silu : identity
+ * x, gate (or NULL): [rows, channels], rows x_stride and gate_stride elements apart; out contiguous, all in dtype.
+ * weight, bias (or NULL): [channels] in weight_dtype: dtype or float32.  Float32 arithmetic.  Limits: at most 4096
+ * channels a group and 2^21 in all, 2^31 rows, strides up to 2^31.
+ */
+int grm_hip_group_norm_fwd(const void* x, const void* weight, const void* bias, const void* gate, void* out,
+                           int64_t rows, int64_t channels, int64_t groups, int64_t x_stride, int64_t gate_stride,
+                           int dtype, int weight_dtype, int silu, int center, float eps, void* stream);
+
+/*
+ * Gradients of grm_hip_group_norm_fwd: grad_out, grad_x and grad_gate (required with a gate) are contiguous;
+ * grad_weight and grad_bias may be NULL.  The weights' sums are taken in a fixed order (no atomics).
+ * Workspace: grm_hip_group_norm_bwd_workspace() bytes, 16-byte aligned.
+ */
+int64_t grm_hip_group_norm_bwd_workspace(int64_t rows, int64_t channels, int64_t groups);
+int grm_hip_group_norm_bwd(const void* x, const void* weight, const void* bias, const void* gate, const void* grad_out,
+                           void* grad_x, void* grad_weight, void* grad_bias, void* grad_gate, void* workspace,
+                           int64_t workspace_bytes, int64_t rows, int64_t channels, int64_t groups, int64_t x_stride,
+                           int64_t gate_stride, int dtype, int weight_dtype, int silu, int center, float eps,
+                           void* stream);
+
 #ifdef __cplusplus
 }
 #endif

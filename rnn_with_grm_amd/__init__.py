@@ -18,6 +18,7 @@ from .cuda_ops import (  # noqa: F401
     cuda_delta_step,
     cuda_fuse_residual,
     cuda_gather_apply,
+    cuda_group_norm,
     cuda_segment_scan,
     cuda_selective_scan,
     cuda_selective_step,
@@ -41,6 +42,7 @@ __all__ = [
     "cuda_delta_step",
     "cuda_fuse_residual",
     "cuda_gather_apply",
+    "cuda_group_norm",
     "cuda_segment_scan",
     "cuda_selective_scan",
     "cuda_selective_step",

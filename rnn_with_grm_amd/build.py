@@ -31,7 +31,7 @@ OFFLOAD_ARCH = "gfx950"
 HIP_SOURCES = ["grm_capi.hip", "chunk_scan.hip", "chunk_scan_wide.hip", "chunk_scan_vsplit.hip", "chunk_scan_par.hip",
                "chunk_bwd.hip", "chunk_bwd_f32.hip", "gather_apply.hip", "retrieve.hip", "retrieve_window.hip",
                "route_fuse.hip", "route_select.hip", "layer_glue.hip", "short_conv.hip",
-               "selective_scan.hip", "selective_bwd.hip", "delta_scan.hip", "delta_bwd.hip"]
+               "selective_scan.hip", "selective_bwd.hip", "delta_scan.hip", "delta_bwd.hip", "group_norm.hip"]
 EXT_SOURCES = ["grm_torch_ops.cpp", "grm_selective_ops.cpp", "grm_delta_ops.cpp"]
 
 # Packed fp32 instructions are kept out of every kernel (the flag is for the

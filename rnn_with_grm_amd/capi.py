@@ -108,6 +108,9 @@ SIGNATURES.update({
     "grm_hip_delta_scan_bwd_workspace": (_I, [_I, _I, _I, _I, _I, _I]),
     "grm_hip_delta_scan_bwd": (_C, [ctypes.POINTER(DeltaArgs)] + [_P] * 11 + [_I, _P]),
     "grm_hip_delta_step": (_C, [ctypes.POINTER(DeltaArgs), _P, _P, _P]),
+    "grm_hip_group_norm_fwd": (_C, [_P] * 5 + [_I] * 5 + [_C] * 4 + [ctypes.c_float, _P]),
+    "grm_hip_group_norm_bwd_workspace": (_I, [_I, _I, _I]),
+    "grm_hip_group_norm_bwd": (_C, [_P] * 10 + [_I] * 6 + [_C] * 4 + [ctypes.c_float, _P]),
 })
 
 _lib: Optional[ctypes.CDLL] = None

@@ -1,4 +1,4 @@
-// torch.ops.grm_cuda: the gated delta rule, on the CUDA key (HIP devices dispatch there in PyTorch-ROCm).  Each op
+// torch.ops.grm_cuda: the gated delta rule and the group norm behind it, on the CUDA key (HIP devices dispatch there in PyTorch-ROCm).  Each op
 // checks its inputs, allocates its outputs and workspace with ATen on the inputs' device and calls the C ABI of libgrm_hip.so
 // on that device's current stream.  Inputs the kernels do not cover raise; CPU tensors take cuda_ops' PyTorch forms.
 #include <tuple>
@@ -164,12 +164,94 @@ std::tuple<Tensor, Tensor> delta_step(const Tensor& keys, const Tensor& values, 
   return {delta_step_out(keys, values, queries, strengths, log_decays, memory, moved), moved};
 }
 
+// ---------------------------------------------------------------------------
+// Group norm.
+
+// Rows of packed channels, any stride between them.
+struct Norm {
+  int64_t rows, C;
+  int dtype, w_dtype;
+};
+
+Norm check_norm(const Tensor& x, int64_t groups, const OptTensor& weight, const OptTensor& bias, const OptTensor& gate,
+                const char* op) {
+  TORCH_CHECK_VALUE(x.dim() == 2, op, ": x must be [rows, channels]");
+  Norm n{x.size(0), x.size(1), dtype_code(x, op, "x"), 0};
+  TORCH_CHECK_VALUE(n.C >= 1 && groups >= 1 && n.C % groups == 0, op, ": channels must be a multiple of groups");
+  TORCH_CHECK_VALUE(n.C / groups <= 4096, op, ": at most 4096 channels a group");
+  n.w_dtype = n.dtype;
+  auto param = [&](const OptTensor& t, const char* name) {
+    if (!has(t)) return;
+    check_device(*t, x, op, name);
+    TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == n.C && (t->scalar_type() == x.scalar_type() || t->scalar_type() == at::kFloat),
+                      op, ": ", name, " must be [channels] in x's type or float32");
+    n.w_dtype = dtype_code(*t, op, name);
+  };
+  param(weight, "weight");
+  param(bias, "bias");
+  TORCH_CHECK_VALUE(!has(weight) || !has(bias) || weight->scalar_type() == bias->scalar_type(), op,
+                    ": weight and bias must share a type");
+  if (has(gate)) {
+    check_device(*gate, x, op, "gate");
+    TORCH_CHECK_VALUE(gate->sizes() == x.sizes() && gate->scalar_type() == x.scalar_type(), op, ": gate must match x");
+  }
+  return n;
+}
+
+Tensor packed_channels(const Tensor& t) {
+  if ((t.size(1) != 1 && t.stride(1) != 1) || (t.size(0) > 1 && (t.stride(0) < t.size(1) || t.stride(0) > (int64_t{1} << 31))))
+    return t.contiguous();
+  return t;
+}
+
+Tensor group_norm_forward(const Tensor& x, int64_t groups, const OptTensor& weight, const OptTensor& bias,
+                          const OptTensor& gate, bool silu, bool center, double eps) {
+  const char* op = "group_norm";
+  const Norm n = check_norm(x, groups, weight, bias, gate, op);
+  c10::OptionalDeviceGuard guard(x.device());
+  Tensor xr = packed_channels(x), gr = has(gate) ? packed_channels(*gate) : Tensor(), kw, kb;
+  Tensor out = at::empty({n.rows, n.C}, x.options());
+  const void *wp = opt_ptr(weight, kw), *bp = opt_ptr(bias, kb);
+  check_rc(grm_hip_group_norm_fwd(xr.data_ptr(), wp, bp, gr.defined() ? gr.data_ptr() : nullptr, out.data_ptr(), n.rows, n.C,
+                                  groups, stride_of(xr, 0, n.C), gr.defined() ? stride_of(gr, 0, n.C) : n.C, n.dtype, n.w_dtype,
+                                  silu, center, static_cast<float>(eps), stream_of(x)),
+           op);
+  return out;
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> group_norm_backward(const Tensor& grad_out, const Tensor& x, int64_t groups,
+                                                               const OptTensor& weight, const OptTensor& bias,
+                                                               const OptTensor& gate, bool silu, bool center, double eps) {
+  const char* op = "group_norm backward";
+  const Norm n = check_norm(x, groups, weight, bias, gate, op);
+  check_device(grad_out, x, op, "grad_out");
+  TORCH_CHECK_VALUE(grad_out.sizes() == x.sizes() && grad_out.scalar_type() == x.scalar_type(), op, ": grad_out must match x");
+  c10::OptionalDeviceGuard guard(x.device());
+  Tensor xr = packed_channels(x), gr = has(gate) ? packed_channels(*gate) : Tensor(), go = grad_out.contiguous(), kw, kb;
+  Tensor dx = at::empty({n.rows, n.C}, x.options());
+  Tensor dw = has(weight) ? at::empty({n.C}, weight->options()) : Tensor(), db = has(bias) ? at::empty({n.C}, bias->options()) : Tensor();
+  Tensor dg = has(gate) ? at::empty({n.rows, n.C}, x.options()) : Tensor();
+  const void *wp = opt_ptr(weight, kw), *bp = opt_ptr(bias, kb);
+  const int64_t wsb = grm_hip_group_norm_bwd_workspace(n.rows, n.C, groups);
+  Tensor ws = bytes(wsb, x);
+  check_rc(grm_hip_group_norm_bwd(xr.data_ptr(), wp, bp, gr.defined() ? gr.data_ptr() : nullptr, go.data_ptr(), dx.data_ptr(),
+                                  dw.defined() ? dw.data_ptr() : nullptr, db.defined() ? db.data_ptr() : nullptr,
+                                  dg.defined() ? dg.data_ptr() : nullptr, ws.data_ptr(), wsb, n.rows, n.C, groups,
+                                  stride_of(xr, 0, n.C), gr.defined() ? stride_of(gr, 0, n.C) : n.C, n.dtype, n.w_dtype, silu,
+                                  center, static_cast<float>(eps), stream_of(x)),
+           op);
+  auto given = [&](const Tensor& t) { return t.defined() ? t : at::empty({0}, x.options()); };
+  return {dx, given(dw), given(db), given(dg)};
+}
+
 }  // namespace
 }  // namespace grm_delta
 
 TORCH_LIBRARY_FRAGMENT(grm_cuda, m) {
   m.def("delta_scan_forward(Tensor keys, Tensor values, Tensor queries, Tensor strengths, Tensor? log_decays, Tensor? memory, Tensor? lengths, bool save) -> (Tensor hidden, Tensor memory_out, Tensor states, Tensor miss)");
   m.def("delta_scan_backward(Tensor? grad_hidden, Tensor? grad_memory_out, Tensor keys, Tensor values, Tensor queries, Tensor strengths, Tensor? log_decays, Tensor? lengths, Tensor states, Tensor miss) -> (Tensor grad_keys, Tensor grad_values, Tensor grad_queries, Tensor grad_strengths, Tensor grad_log_decays, Tensor grad_memory)");
+  m.def("group_norm_forward(Tensor x, int groups, Tensor? weight, Tensor? bias, Tensor? gate, bool silu, bool center, float eps) -> Tensor");
+  m.def("group_norm_backward(Tensor grad_out, Tensor x, int groups, Tensor? weight, Tensor? bias, Tensor? gate, bool silu, bool center, float eps) -> (Tensor grad_x, Tensor grad_weight, Tensor grad_bias, Tensor grad_gate)");
   m.def("delta_step(Tensor keys, Tensor values, Tensor queries, Tensor strengths, Tensor? log_decays, Tensor memory) -> (Tensor hidden, Tensor memory_out)");
   m.def("delta_step_out(Tensor keys, Tensor values, Tensor queries, Tensor strengths, Tensor? log_decays, Tensor memory, Tensor(a!) memory_out) -> Tensor");
 }
@@ -177,6 +259,8 @@ TORCH_LIBRARY_FRAGMENT(grm_cuda, m) {
 TORCH_LIBRARY_IMPL(grm_cuda, CUDA, m) {
   m.impl("delta_scan_forward", grm_delta::delta_scan_forward);
   m.impl("delta_scan_backward", grm_delta::delta_scan_backward);
+  m.impl("group_norm_forward", grm_delta::group_norm_forward);
+  m.impl("group_norm_backward", grm_delta::group_norm_backward);
   m.impl("delta_step", grm_delta::delta_step);
   m.impl("delta_step_out", grm_delta::delta_step_out);
 }

@@ -19,7 +19,8 @@ Deliberate differences:
     ``cuda_segment_route``, ``cuda_gather_apply`` and ``cuda_fuse_residual``; the
     selective state scan and its short convolution (``cuda_selective_scan``,
     ``cuda_selective_step``, ``cuda_short_conv``, ``cuda_short_conv_step``); the gated
-    delta rule (``cuda_delta_scan``, ``cuda_delta_step``).
+    delta rule (``cuda_delta_scan``, ``cuda_delta_step``) and the group norm behind a linear
+    memory (``cuda_group_norm``).
 """
 
 from __future__ import annotations
@@ -47,7 +48,8 @@ EXTRA_OPS = ("segment_scan_forward", "topk_route", "fuse_residual", "gather_appl
              "gather_apply_backward_tokens", "apply_query_backward_queries", "archive_cast", "project_gemm",
              "linear_residual_layer_norm", "segment_retrieve_fuse", "selective_scan_forward", "selective_scan_backward",
              "selective_step", "selective_step_out", "short_conv_forward", "short_conv_backward", "short_conv_step",
-             "short_conv_step_out", "delta_scan_forward", "delta_scan_backward", "delta_step", "delta_step_out")
+             "short_conv_step_out", "delta_scan_forward", "delta_scan_backward", "delta_step", "delta_step_out",
+             "group_norm_forward", "group_norm_backward")
 
 # Environment variables of the reference (cuda_ops.py:26-32): one per op and a global one.
 GLOBAL_POLICY_ENV = "GRM_CUDA_KERNEL_POLICY"
@@ -1262,6 +1264,84 @@ def cuda_delta_step(keys: Tensor, values: Tensor, queries: Tensor, strengths: Te
     return hidden[:, 0], moved if memory_out is None else memory_out.copy_(moved)
 
 
+# ---------------------------------------------------------------------------
+# Group norm of rows.
+
+def _torch_group_norm(x: Tensor, groups: int, weight: Optional[Tensor], bias: Optional[Tensor], gate: Optional[Tensor],
+                      silu: bool, center: bool, eps: float) -> Tensor:
+    C = x.size(-1)
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and (t.shape != (C,) or t.dtype not in (x.dtype, torch.float32)):
+            raise ValueError(f"group_norm: {name} must be [channels] in x's type or float32")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError("group_norm: weight and bias must share a type")
+    if gate is not None and (gate.shape != x.shape or gate.dtype != x.dtype):
+        raise ValueError("group_norm: gate must match x")
+    cdt = torch.float64 if x.dtype == torch.float64 else torch.float32
+    n = x.to(cdt).unflatten(-1, (groups, C // groups))
+    if center:
+        n = n - n.mean(-1, keepdim=True)
+    y = (n * torch.rsqrt(n.square().mean(-1, keepdim=True) + eps)).flatten(-2)
+    if weight is not None:
+        y = y * weight.to(cdt)
+    if bias is not None:
+        y = y + bias.to(cdt)
+    z = y if gate is None else gate.to(cdt)
+    z = torch.nn.functional.silu(z) if silu else z
+    return (z if gate is None else y * z).to(x.dtype)
+
+
+class _GroupNormFn(torch.autograd.Function):
+    """The norm's inputs are all that its backward needs: a row's mean and variance come from
+    the registers that hold it anyway."""
+
+    @staticmethod
+    def forward(ctx, x, groups, weight, bias, gate, silu: bool, center: bool, eps: float):
+        ctx.form = (silu, center, eps)
+        ctx.groups = groups
+        ctx.save_for_backward(x, weight, bias, gate)
+        return torch.ops.grm_cuda.group_norm_forward(x, groups, weight, bias, gate, silu, center, eps)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        x, weight, bias, gate = ctx.saved_tensors
+        dx, dw, db, dg = torch.ops.grm_cuda.group_norm_backward(grad_out, x, ctx.groups, weight, bias, gate, *ctx.form)
+        return (dx, None, None if weight is None else dw, None if bias is None else db, None if gate is None else dg,
+                None, None, None)
+
+
+def cuda_group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None,
+                    gate: Optional[Tensor] = None, *, activation: Optional[str] = None, center: bool = True,
+                    eps: float = 1e-5, enabled: bool = True, debug_fallback: bool = False) -> Tensor:
+    """Group norm of every row (token) on its own, channels last: ``n = (x - mean) / sqrt(var + eps)`` over each of
+    ``groups`` equal groups of a row's channels (``center=False``: ``x / sqrt(mean(x^2) + eps)``),
+    ``y = n weight + bias``, then ``act(y)``, or with a gate ``y act(gate)``; ``activation`` None or "silu".
+    Behind a linear memory a group is a head's values: ``cuda_group_norm(hidden.flatten(-2), heads, ...)``.
+
+    x and gate [..., C] in one type (float32, float16 or bfloat16; rows of packed channels, e.g. a slice of a wider
+    projection, are read in place), weight and bias [C] in x's type or float32.  Returns x's shape and type.
+    Differentiable once, backwards, in x, weight, bias and gate (forward-mode derivatives are refused on
+    the GPU).  Limits: at most 4096 channels a group."""
+    silu = _silu_flag(activation)
+    groups = int(groups)
+    if x.ndim < 1 or groups < 1 or x.size(-1) < 1 or x.size(-1) % groups != 0:
+        raise ValueError("group_norm: x must be [..., channels] and channels a multiple of groups")
+    if x.size(-1) // groups > 4096:
+        raise ValueError("group_norm: at most 4096 channels a group")
+    if not 0.0 <= eps < math.inf:
+        raise ValueError(f"group_norm: eps must be a number >= 0, got {eps}")
+    if x.is_cuda and _run_native("group_norm", x.device, enabled=enabled, debug_fallback=debug_fallback):
+        if gate is not None and gate.shape != x.shape:
+            raise ValueError("group_norm: gate must match x")
+        rows = (x.reshape(-1, x.size(-1)), groups, weight, bias, None if gate is None else gate.reshape(-1, x.size(-1)), silu,
+                bool(center), float(eps))
+        if _wants_grad(x, weight, bias, gate):
+            return _GroupNormFn.apply(*rows).view(x.shape)
+        return torch.ops.grm_cuda.group_norm_forward(*rows).view(x.shape)
+    return _torch_group_norm(x, groups, weight, bias, gate, silu, center, eps)
+
+
 __all__ = [
     "GrmExtensionUnavailable",
     "cuda_apply_query",
@@ -1271,6 +1351,7 @@ __all__ = [
     "cuda_delta_step",
     "cuda_fuse_residual",
     "cuda_gather_apply",
+    "cuda_group_norm",
     "cuda_linear_residual_layer_norm",
     "cuda_project_gemm",
     "cuda_project_split",
