@@ -61,6 +61,34 @@ __device__ __forceinline__ int64_t delta_length(const DeltaArgs& a, int b) {
   return a.lengths == nullptr ? a.T : max_i64(0, min_i64(a.lengths[b], a.T));
 }
 
+// Float32 values as parts whose sum they are: each the rounded remainder of the ones before.  (An infinity's further
+// parts are NaN, and so is what it reaches.)
+template <int PARTS>
+__device__ __forceinline__ void split8(const float (&v)[8], B8 (&out)[PARTS]) {
+  float rest[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) rest[e] = v[e];
+#pragma unroll
+  for (int p = 0; p < PARTS; ++p) {
+    uint32_t u[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      u[e] = pack2<BF16>(rest[2 * e], rest[2 * e + 1]);
+      if (p + 1 < PARTS) {
+        rest[2 * e] -= __uint_as_float(u[e] << 16);
+        rest[2 * e + 1] -= __uint_as_float(u[e] & 0xffff0000u);
+      }
+    }
+    out[p] = __builtin_bit_cast(B8, make_uint4(u[0], u[1], u[2], u[3]));
+  }
+}
+// Two accumulators (tokens 0-15 and 16-31 of a step) as one fragment's parts.
+template <int PARTS>
+__device__ __forceinline__ void split2(f32x4 lo, f32x4 hi, B8 (&out)[PARTS]) {
+  const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  split8<PARTS>(v, out);
+}
+
 // acc += sum of a[i] b[j] over the pairs with i + j < LIM, the smaller products first.
 template <int LIM, int NA, int NB>
 __device__ __forceinline__ f32x4 mma_parts(const B8 (&a)[NA], const B8 (&b)[NB], f32x4 acc) {
@@ -75,6 +103,45 @@ __device__ __forceinline__ f32x4 mma_parts(const B8 (&a)[NA], const B8 (&b)[NB],
   return acc;
 }
 
+// The same for several accumulators that share b (ROWS: a[t] is the left operand; else the right one): consecutive
+// products hang on different accumulators.
+template <int LIM, bool ROWS, int C, int NA, int NB>
+__device__ __forceinline__ void mma_many(const B8 (&a)[C][NA], const B8 (&b)[NB], f32x4 (&acc)[C]) {
+#pragma unroll
+  for (int d = LIM - 1; d >= 0; --d) {
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      const int j = d - i;
+      if (j < 0 || j >= NB) continue;
+#pragma unroll
+      for (int t = 0; t < C; ++t) acc[t] = ROWS ? mfma8(a[t][i], b[j], acc[t]) : mfma8(b[j], a[t][i], acc[t]);
+    }
+  }
+}
+
+// Products of a triangular 64 x 64 matrix, whose six fragments are f, with b's two steps of tokens: acc[t] += rows of tile t.
+// LOWER: tile t meets steps up to its own, else from its own on.  ROWS as above.
+template <int LIM, bool LOWER, bool ROWS, int NA, int NB>
+__device__ __forceinline__ void mma_triangle(const B8 (&f)[kDFrags][NA], const B8 (&b)[2][NB], f32x4 (&acc)[4]) {
+#pragma unroll
+  for (int d = LIM - 1; d >= 0; --d) {
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      const int j = d - i;
+      if (j < 0 || j >= NB) continue;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          if (LOWER ? s > t / 2 : s < t / 2) continue;
+          const B8& x = f[LOWER ? lower_frag(t, s) : upper_frag(t, s)][i];
+          acc[t] = ROWS ? mfma8(x, b[s][j], acc[t]) : mfma8(b[s][j], x, acc[t]);
+        }
+      }
+    }
+  }
+}
+
 // Eight elements of type E as their parts.
 template <class E, int NI>
 __device__ __forceinline__ void input_parts(const U8<E>& u, B8 (&f)[NI]) {
@@ -84,7 +151,7 @@ __device__ __forceinline__ void input_parts(const U8<E>& u, B8 (&f)[NI]) {
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = ET<E>::to_f(u.e[e]);
-    split_frag<BF16, NI>(v, f);
+    split8<NI>(v, f);
   }
 }
 
@@ -125,6 +192,12 @@ __device__ __forceinline__ void stored_parts(const uint16_t* m, int frag, B8 (&f
 #pragma unroll
   for (int p = 0; p < NP; ++p)
     f[p] = __builtin_bit_cast(B8, *reinterpret_cast<const uint4*>(m + (frag * NP + p) * kDFragElems + 8 * lane));
+}
+
+template <int NP>
+__device__ __forceinline__ void stored_triangle(const uint16_t* m, B8 (&f)[kDFrags][NP], int lane) {
+#pragma unroll
+  for (int i = 0; i < kDFrags; ++i) stored_parts<NP>(m, i, f[i], lane);
 }
 
 int delta_check(const struct grm_hip_delta_args* u, const char* what, bool step);

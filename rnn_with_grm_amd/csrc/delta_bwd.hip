@@ -39,7 +39,7 @@ struct ReverseLds {
 // Two accumulators scaled by what sc holds for their tokens (row tiles t0 and t0 + 1 of 16), in three parts.
 __device__ __forceinline__ void scaled_pair(const f32x4& lo, const f32x4& hi, const float* sc, int g, B8 (&out)[3]) {
   const float4 a = *reinterpret_cast<const float4*>(sc + 4 * g), b = *reinterpret_cast<const float4*>(sc + 16 + 4 * g);
-  split_pair<BF16, 3>(f32x4{lo[0] * a.x, lo[1] * a.y, lo[2] * a.z, lo[3] * a.w},
+  split2<3>(f32x4{lo[0] * a.x, lo[1] * a.y, lo[2] * a.z, lo[3] * a.w},
                       f32x4{hi[0] * b.x, hi[1] * b.y, hi[2] * b.z, hi[3] * b.w}, out);
 }
 
@@ -108,7 +108,7 @@ __global__ __launch_bounds__(kThreads) void delta_reverse_kernel(DeltaBwdArgs ba
     {
       B8 gp[S][3];
 #pragma unroll
-      for (int s = 0; s < S; ++s) split_pair<BF16, 3>(st[2 * s], st[2 * s + 1], gp[s]);
+      for (int s = 0; s < S; ++s) split2<3>(st[2 * s], st[2 * s + 1], gp[s]);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         z[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -148,7 +148,7 @@ __global__ __launch_bounds__(kThreads) void delta_reverse_kernel(DeltaBwdArgs ba
     {
       B8 zp[2][3];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) split_pair<BF16, 3>(z[2 * s], z[2 * s + 1], zp[s]);
+      for (int s = 0; s < 2; ++s) split2<3>(z[2 * s], z[2 * s + 1], zp[s]);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         du[t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -308,8 +308,8 @@ __global__ __launch_bounds__(kThreads) void delta_grad_kernel(DeltaBwdArgs ba) {
         hv.e[e] = ok ? static_cast<const raw*>(ba.dhidden)[my + p] : raw(0);
       }
       B8 mp[3], up[3], hp[NI];
-      split_frag<BF16, 3>(mv, mp);
-      split_frag<BF16, 3>(uv, up);
+      split8<3>(mv, mp);
+      split8<3>(uv, up);
       input_parts<E, NI>(hv, hp);
       __syncthreads();
       store_parts<ST, 3, F32>(sl, stile, L::spart, 32, tid);
@@ -483,9 +483,9 @@ __global__ __launch_bounds__(kThreads) void delta_grad_kernel(DeltaBwdArgs ba) {
         xr[e] = xm[tok * L::XS + k];
       }
       B8 yp[NO], xp[NO], cp[NO];
-      split_frag<BF16, NO>(yr, yp);
-      split_frag<BF16, NO>(xr, xp);
-      split_frag<BF16, NO>(yc, cp);
+      split8<NO>(yr, yp);
+      split8<NO>(xr, xp);
+      split8<NO>(yc, cp);
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         B8 kf[NI], qf[NI];

@@ -204,7 +204,7 @@ __global__ __launch_bounds__(kPrepThreads) void delta_prep_kernel(DeltaArgs a) {
       else v[e] = k <= row ? M[row * kTriStride + k] : 0.f;
     }
     B8 f[3];
-    split_frag<BF16, 3>(v, f);
+    split8<3>(v, f);
     const int frag = BACK ? upper_frag(w, s) : lower_frag(w, s);
 #pragma unroll
     for (int p = 0; p < 3; ++p)
@@ -228,7 +228,7 @@ struct WalkLds {
 // accumulators (the state's columns never meet: each wave's chain is its own).  Accumulators of K S^T, of m and of the state
 // lie as the next product's operand wants them, so nothing but the inputs passes through LDS.
 template <class E, int NK, bool VEC>
-__global__ __launch_bounds__(kWalkThreads) void delta_walk_kernel(DeltaArgs a) {
+__global__ __launch_bounds__(kWalkThreads, 1) void delta_walk_kernel(DeltaArgs a) {
   using raw = typename ET<E>::raw;
   using L = WalkLds<E, NK>;
   using KT = typename L::KT;
@@ -266,7 +266,7 @@ __global__ __launch_bounds__(kWalkThreads) void delta_walk_kernel(DeltaArgs a) {
     ql.load(qp + t0 * a.qt, len - t0, tid);
     vl.load(vp + t0 * a.vt, len - t0, tid);
     const float* s = reinterpret_cast<const float*>(work + c * delta_chunk_bytes(NO) + (3 + NO) * kDFrags * kDFragElems * 2);
-    if (tid < 128) sreg = s[tid];
+    sreg = s[tid & 127];
     odd_next = reinterpret_cast<const int*>(s)[192];
   };
 
@@ -275,7 +275,13 @@ __global__ __launch_bounds__(kWalkThreads) void delta_walk_kernel(DeltaArgs a) {
   for (int i = 0; i < NT; ++i) st[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int64_t head = static_cast<int64_t>(b) * a.H + h, cells = static_cast<int64_t>(a.P) * a.N;
   if (a.memory != nullptr) state_add<NT>(st, a.memory + head * cells, p0, a.P, a.N, 1.f);
-  if (chunks > 0) fetch(0);
+  // The triangular matrices' fragments, loaded a chunk ahead as soon as the last ones are done with.
+  B8 tf[kDFrags][3], pf[kDFrags][NO];
+  if (chunks > 0) {
+    fetch(0);
+    stored_triangle<3>(reinterpret_cast<const uint16_t*>(work), tf, lane);
+    stored_triangle<NO>(reinterpret_cast<const uint16_t*>(work) + 3 * kDFrags * kDFragElems, pf, lane);
+  }
 
   for (int c = 0; c < chunks; ++c) {
     const int64_t t0 = static_cast<int64_t>(c) * kDTokens;
@@ -286,30 +292,31 @@ __global__ __launch_bounds__(kWalkThreads) void delta_walk_kernel(DeltaArgs a) {
     vl.store(vt, tid);
     if (tid < 128) sc[tid] = sreg;
     __syncthreads();
-    if (c + 1 < chunks) fetch(c + 1);
-    const uint16_t* tf = reinterpret_cast<const uint16_t*>(work + c * delta_chunk_bytes(NO));
-    const uint16_t* pf = tf + 3 * kDFrags * kDFragElems;
+    // Loads ahead stand behind no branch (behind the last chunk it is loaded again): a wait then counts them exactly.
+    const int next = c + 1 < chunks ? c + 1 : c;
+    fetch(next);
     if (a.states != nullptr)
       state_store<NT>(st, a.states + ((static_cast<int64_t>(b) * a.C + c) * a.H + h) * cells, p0, a.P, a.N);
 
     // K S^T (a token a row, a value a column) and Q S^T (transposed, as its rows are stored).
     B8 sp[S][3];
 #pragma unroll
-    for (int s = 0; s < S; ++s) split_pair<BF16, 3>(st[2 * s], st[2 * s + 1], sp[s]);
+    for (int s = 0; s < S; ++s) split2<3>(st[2 * s], st[2 * s + 1], sp[s]);
     f32x4 x[4], o[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      x[t] = o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < 4; ++t) x[t] = o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        B8 kf[NI], qf[NI], so[NO];
-        row_parts_t<KT, NI>(kt, L::kpart, 16 * t, 32 * s, kf);
-        row_parts_t<QT, NI>(qt, L::qpart, 16 * t, 32 * s, qf);
+    for (int s = 0; s < S; ++s) {
+      B8 kf[4][NI], qf[4][NI], so[NO];
 #pragma unroll
-        for (int p = 0; p < NO; ++p) so[p] = sp[s][p];
-        x[t] = mma_parts<3>(kf, sp[s], x[t]);
-        o[t] = mma_parts<NO>(so, qf, o[t]);
+      for (int t = 0; t < 4; ++t) {
+        row_parts_t<KT, NI>(kt, L::kpart, 16 * t, 32 * s, kf[t]);
+        row_parts_t<QT, NI>(qt, L::qpart, 16 * t, 32 * s, qf[t]);
       }
+#pragma unroll
+      for (int p = 0; p < NO; ++p) so[p] = sp[s][p];
+      mma_many<3, true>(kf, sp[s], x);
+      mma_many<NO, false>(qf, so, o);
     }
     // V - D K S^T.
     f32x4 rt[4];
@@ -358,18 +365,12 @@ __global__ __launch_bounds__(kWalkThreads) void delta_walk_kernel(DeltaArgs a) {
     {
       B8 rp[2][3];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) split_pair<BF16, 3>(rt[2 * s], rt[2 * s + 1], rp[s]);
+      for (int s = 0; s < 2; ++s) split2<3>(rt[2 * s], rt[2 * s + 1], rp[s]);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        m[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s <= t / 2; ++s) {
-          B8 f[3];
-          stored_parts<3>(tf, lower_frag(t, s), f, lane);
-          m[t] = mma_parts<3>(f, rp[s], m[t]);
-        }
-      }
+      for (int t = 0; t < 4; ++t) m[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      mma_triangle<3, true, true>(tf, rp, m);
     }
+    stored_triangle<3>(reinterpret_cast<const uint16_t*>(work + next * delta_chunk_bytes(NO)), tf, lane);
     if (a.miss != nullptr && p0 + n < a.P) {
       float* to = a.miss + ((static_cast<int64_t>(b) * a.T + t0) * a.H + h) * a.P + p0 + n;
 #pragma unroll
@@ -385,18 +386,12 @@ __global__ __launch_bounds__(kWalkThreads) void delta_walk_kernel(DeltaArgs a) {
     {
       B8 mp[2][NO];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) split_pair<BF16, NO>(m[2 * s], m[2 * s + 1], mp[s]);
+      for (int s = 0; s < 2; ++s) split2<NO>(m[2 * s], m[2 * s + 1], mp[s]);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        o[t] *= sc[16 * t + n];
-#pragma unroll
-        for (int s = 0; s <= t / 2; ++s) {
-          B8 f[NO];
-          stored_parts<NO>(pf, lower_frag(t, s), f, lane);
-          o[t] = mma_parts<NO>(mp[s], f, o[t]);
-        }
-      }
+      for (int t = 0; t < 4; ++t) o[t] *= sc[16 * t + n];
+      mma_triangle<NO, true, false>(pf, mp, o);
     }
+    stored_triangle<NO>(reinterpret_cast<const uint16_t*>(work + next * delta_chunk_bytes(NO)) + 3 * kDFrags * kDFragElems, pf, lane);
     if (__any(cut < 64)) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -407,20 +402,19 @@ __global__ __launch_bounds__(kWalkThreads) void delta_walk_kernel(DeltaArgs a) {
       }
     }
     {
-      const int p = p0 + 4 * g;
-      raw* to = static_cast<raw*>(a.hidden) + ((static_cast<int64_t>(b) * a.T + t0) * a.H + h) * a.P + p;
+      const int p = p0 + 4 * g, row = a.H * a.P * static_cast<int>(sizeof(raw));
+      const int64_t left = a.T - t0;
+      const __amdgpu_buffer_rsrc_t to =
+          make_rsrc(static_cast<raw*>(a.hidden) + ((static_cast<int64_t>(b) * a.T + t0) * a.H + h) * a.P, 0x7ffffff0u);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const int tok = 16 * t + n;
-        if (t0 + tok < a.T) {
-          raw* row = to + static_cast<int64_t>(tok) * a.H * a.P;
-          if (VEC) {
-            if (p < a.P) store4_raw<E>(row, o[t]);
-          } else {
+        if (VEC) {
+          buf_store4<E>(to, tok < left && p < a.P ? tok * row + p * static_cast<int>(sizeof(raw)) : kBufOOB, o[t]);
+        } else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (p + r < a.P) row[r] = ET<E>::from_f(o[t][r]);
-          }
+          for (int r = 0; r < 4; ++r)
+            buf_store1<E>(to, tok < left && p + r < a.P ? tok * row + (p + r) * static_cast<int>(sizeof(raw)) : kBufOOB, o[t][r]);
         }
       }
     }
@@ -438,13 +432,11 @@ __global__ __launch_bounds__(kWalkThreads) void delta_walk_kernel(DeltaArgs a) {
           em[i] = f32x4{m[2 * s + i][0] * e.x, m[2 * s + i][1] * e.y, m[2 * s + i][2] * e.z, m[2 * s + i][3] * e.w};
         }
         B8 ep[3];
-        split_pair<BF16, 3>(em[0], em[1], ep);
+        split2<3>(em[0], em[1], ep);
+        B8 kf[NT][NI];
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          B8 kf[NI];
-          col_parts<KT, NI>(kt, L::kpart, 32 * s, 16 * i, kf);
-          st[i] = mma_parts<3>(kf, ep, st[i]);
-        }
+        for (int i = 0; i < NT; ++i) col_parts<KT, NI>(kt, L::kpart, 32 * s, 16 * i, kf[i]);
+        mma_many<3, true>(kf, ep, st);
       }
     }
     if (cut < 64) {
@@ -457,6 +449,352 @@ __global__ __launch_bounds__(kWalkThreads) void delta_walk_kernel(DeltaArgs a) {
   for (int64_t t = static_cast<int64_t>(chunks) * kDTokens + tid / 16; t < a.T; t += kWalkThreads / 16) {
     raw* row = static_cast<raw*>(a.hidden) + ((b * a.T + t) * a.H + h) * a.P + col0;
     for (int p = tid % 16; p < kDCols && col0 + p < a.P; p += 16) row[p] = 0;
+  }
+}
+
+// LDS of the walk in two halves: two stages of a chunk, where they fit, else of its keys alone.
+template <class E, int NK>
+struct PairLds {
+  using KT = SelTile<BF16, NK, true>;
+  using QT = SelTile<BF16, NK, false>;
+  using VT = SelTile<E, kDCols, true>;
+  static constexpr int NI = DParts<E>::IN, NO = DParts<E>::OUT, SCAL = 132;
+  static constexpr int kpart = kDTokens * KT::STRIDE, qpart = kDTokens * QT::STRIDE;
+  static constexpr int state = NK / 32 * NO * kDFragElems;  // a wave's state as fragments
+  static constexpr int qstage = NI * qpart, vstage = kDTokens * VT::STRIDE;
+  static constexpr size_t kbytes = 2 * NI * kpart * 2, qvbytes = qstage * 2 + vstage * sizeof(typename ET<E>::raw),
+                          other = 4 * state * 2 + 4 * 4 * 64 * 16 + 2 * SCAL * 4 + 64 * 4;
+  static constexpr int QV = kbytes + 2 * qvbytes + other <= 160 * 1024 ? 2 : 1;  // stages of queries and values
+  static constexpr size_t k = 0, q = kbytes, v = q + QV * qstage * 2, s = v + QV * vstage * sizeof(typename ET<E>::raw),
+                          m = s + 4 * state * 2, sc = m + 4 * 4 * 64 * 16, cut = sc + 2 * SCAL * 4, bytes = cut + 64 * 4;
+  static constexpr bool fits = bytes <= 160 * 1024;
+};
+
+// The walk over a sequence's chunks, 64 value columns of a head a workgroup.  Four state waves hold 16 columns each, in
+// accumulators, and run the chain that a chunk hangs on: K S^T, m, the next state.  Four output waves, one beside each
+// on its SIMD, load the chunks ahead into LDS and form what hangs on no later chunk: Q S^T while m is formed, then
+// the weights' product with m, and the stores.  A state's columns never meet, so a state wave's chain is its own;
+// accumulators of K S^T, of m and of the state lie as the next product's operand wants them.  Two barriers a chunk:
+// m is there, the next state is there.
+template <class E, int NK, bool VEC>
+__global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaArgs a) {
+  using raw = typename ET<E>::raw;
+  using L = PairLds<E, NK>;
+  using KT = typename L::KT;
+  using QT = typename L::QT;
+  using VT = typename L::VT;
+  constexpr int NI = L::NI, NO = L::NO, S = NK / 32, NT = NK / 16, QV = L::QV;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  uint16_t* kt = reinterpret_cast<uint16_t*>(lds + L::k);
+  uint16_t* qt = reinterpret_cast<uint16_t*>(lds + L::q);
+  raw* vt = reinterpret_cast<raw*>(lds + L::v);
+  float* sc = reinterpret_cast<float*>(lds + L::sc);
+  int* cuts = reinterpret_cast<int*>(lds + L::cut);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
+  const int lane = lane_id(), g = lane >> 4, n = lane & 15;
+  const uint32_t at = xcd_order(blockIdx.x, gridDim.x);
+  const int pt = static_cast<int>(at % a.PT), h = static_cast<int>(at / a.PT % a.H), b = static_cast<int>(at / a.PT / a.H);
+  const int64_t len = delta_length(a, b);
+  const int col0 = pt * kDCols, p0 = col0 + 16 * w, gi = h / (a.H / a.G);
+  const int chunks = static_cast<int>((len + kDTokens - 1) / kDTokens);
+  const int64_t head = static_cast<int64_t>(b) * a.H + h, cells = static_cast<int64_t>(a.P) * a.N;
+  const char* work = a.work + head * a.C * delta_chunk_bytes(NO);
+  uint16_t* sf = reinterpret_cast<uint16_t*>(lds + L::s) + w * L::state + 8 * lane;
+  f32x4* mf = reinterpret_cast<f32x4*>(lds + L::m) + w * 256 + lane;
+
+  if (wave < 4) {
+    __builtin_amdgcn_s_setprio(2);
+    const float inf = __builtin_inff();
+    f32x4 st[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) st[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (a.memory != nullptr) state_add<NT>(st, a.memory + head * cells, p0, a.P, a.N, 1.f);
+    // The triangular matrix's fragments, loaded a chunk ahead as soon as the last ones are done with.
+    B8 tf[kDFrags][3], sp[S][3];
+    if (chunks > 0) stored_triangle<3>(reinterpret_cast<const uint16_t*>(work), tf, lane);
+    auto publish = [&](int s) {
+      split2<3>(st[2 * s], st[2 * s + 1], sp[s]);
+#pragma unroll
+      for (int p = 0; p < NO; ++p)
+        *reinterpret_cast<uint4*>(sf + (s * NO + p) * kDFragElems) = __builtin_bit_cast(uint4, sp[s][p]);
+    };
+    auto keep_state = [&](int c) {
+      if (a.states != nullptr && c < chunks)
+        state_store<NT>(st, a.states + ((static_cast<int64_t>(b) * a.C + c) * a.H + h) * cells, p0, a.P, a.N);
+    };
+    B8 kr[2][4][NI];  // keys by rows, [step & 1][tile]
+    auto row_keys = [&](const uint16_t* from, int s) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) row_parts_t<KT, NI>(from, L::kpart, 16 * t, 32 * s, kr[s & 1][t]);
+    };
+    keep_state(0);
+#pragma unroll
+    for (int s = 0; s < S; ++s) publish(s);
+    __syncthreads();
+    if (chunks > 0) row_keys(kt, 0);
+    for (int c = 0; c < chunks; ++c) {
+      const uint16_t* kc = kt + (c & 1) * NI * L::kpart;
+      const float* scc = sc + (c & 1) * L::SCAL;
+      const int next = c + 1 < chunks ? c + 1 : c;
+      const raw* vc = vt + (c & (QV - 1)) * L::vstage;
+      // (Read ahead of the products, which they wait for.)
+      Frag8<E> vf[2];
+      float4 dd[4];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) vf[s] = col_frag<VT, E>(vc, 32 * s, 16 * w);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) dd[t] = *reinterpret_cast<const float4*>(scc + 16 * t + 4 * g);
+      const int odd_key = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(scc)[128]);
+      hold_order();
+      // K S^T: a token a row, a value a column.
+      f32x4 x[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) x[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        if (s + 1 < S) row_keys(kc, s + 1);
+        mma_many<3, true>(kr[s & 1], sp[s], x);
+        hold_order();
+      }
+      // V - D K S^T.
+      float odd = 0.f;  // (a product with zero is zero or NaN)
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const float d[4] = {dd[t].x, dd[t].y, dd[t].z, dd[t].w};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          x[t][r] = fmaf(-d[r], x[t][r], ET<E>::to_f(vf[t / 2].e[4 * (t & 1) + r]));
+          odd = fmaf(x[t][r], 0.f, odd);
+        }
+      }
+      // A value, key or state that is no number: from its token on the column is NaN.  Its rows stay out of the products,
+      // whose zeros would not keep them out of earlier tokens' sums.
+      int cut = 64;
+      if (__any(odd != 0.f) || odd_key < 64) {
+        int f = odd_key;
+#pragma unroll
+        for (int t = 3; t >= 0; --t) {
+#pragma unroll
+          for (int r = 3; r >= 0; --r) {
+            const int tok = 16 * t + 4 * g + r;
+            if (!(fabsf(x[t][r]) < inf) && tok < f) f = tok;
+          }
+        }
+        const int f1 = __shfl_xor(f, 16), f2 = f < f1 ? f : f1, f3 = __shfl_xor(f2, 32);
+        cut = f2 < f3 ? f2 : f3;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (16 * t + 4 * g + r >= cut) x[t][r] = 0.f;
+        }
+      }
+      f32x4 m[4];
+      {
+        B8 rp[2][3];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) split2<3>(x[2 * s], x[2 * s + 1], rp[s]);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) m[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        mma_triangle<3, true, true>(tf, rp, m);
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) mf[64 * t] = m[t];
+      if (g == 0) cuts[16 * w + n] = cut;
+      B8 kf[2][2][2][NI];  // [pair & 1][step][tile of the pair]
+      auto pair_keys = [&](int j) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) col_parts<KT, NI>(kc, L::kpart, 32 * s, 16 * (2 * j + i), kf[j & 1][s][i]);
+        }
+      };
+      pair_keys(0);
+      __syncthreads();
+      // S' = e^{c_63} S + (E b m)^T K, two tiles of keys at a time: while one pair's products run, the last pair's sums
+      // are split for the next chunk and a share of its triangular matrix is called for (all at once the loads would wait for
+      // each other).  Loads ahead stand behind no branch (behind the last chunk it is loaded again): a wait then counts
+      // them exactly.
+      const float keep = scc[63];
+      const uint16_t* tn = reinterpret_cast<const uint16_t*>(work + next * delta_chunk_bytes(NO));
+      B8 ep[2][3];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        f32x4 em[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float4 e = *reinterpret_cast<const float4*>(scc + 64 + 32 * s + 16 * i + 4 * g);
+          em[i] = f32x4{m[2 * s + i][0] * e.x, m[2 * s + i][1] * e.y, m[2 * s + i][2] * e.z, m[2 * s + i][3] * e.w};
+        }
+        split2<3>(em[0], em[1], ep[s]);
+      }
+#pragma unroll
+      for (int j = 0; j < S; ++j) {
+        if (j + 1 < S) pair_keys(j + 1);
+        f32x4 y[2] = {st[2 * j] * keep, st[2 * j + 1] * keep};
+#pragma unroll
+        for (int s = 0; s < 2; ++s) mma_many<3, true>(kf[j & 1][s], ep[s], y);
+        st[2 * j] = y[0];
+        st[2 * j + 1] = y[1];
+        constexpr int per = (kDFrags + S - 1) / S;
+#pragma unroll
+        for (int f = j * per; f < (j + 1) * per; ++f)
+          if (f < kDFrags) stored_parts<3>(tn, f, tf[f], lane);
+        if (j > 0) publish(j - 1);
+        hold_order();
+      }
+      if (cut < 64) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) st[i] = f32x4{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
+      }
+      if (__any(cut < 64)) {
+#pragma unroll
+        for (int s = 0; s + 1 < S; ++s) publish(s);
+      }
+      publish(S - 1);
+      keep_state(c + 1);
+      row_keys(kt + ((c + 1) & 1) * NI * L::kpart, 0);  // (there since the chunk's first barrier)
+      __syncthreads();
+    }
+    state_store<NT>(st, a.memory_out + head * cells, p0, a.P, a.N);
+  } else {
+    const int tid = static_cast<int>(threadIdx.x) - kWalkThreads;
+    const raw* kp = static_cast<const raw*>(a.keys) + b * a.kb + static_cast<int64_t>(gi) * a.N;
+    const raw* qp = static_cast<const raw*>(a.queries) + b * a.qb + static_cast<int64_t>(gi) * a.N;
+    const raw* vp = static_cast<const raw*>(a.values) + b * a.vb + static_cast<int64_t>(h) * a.P + col0;
+    TileLoad<E, KT, BF16, VEC, kDTokens, NK, kWalkThreads> kl;
+    TileLoad<E, QT, BF16, VEC, kDTokens, NK, kWalkThreads> ql;
+    TileLoad<E, VT, E, VEC, kDTokens, kDCols, kWalkThreads> vl;
+    kl.init(a.kt, a.N, tid);
+    ql.init(a.qt, a.N, tid);
+    vl.init(a.vt, a.P - col0 < kDCols ? a.P - col0 : kDCols, tid);
+    float sreg = 0.f, warm = 0.f;
+    int oreg = 64;
+    B8 pf[kDFrags][NO];
+    auto fetch = [&](int want) {
+      const int c = want < chunks ? want : chunks - 1;
+      const int64_t t0 = static_cast<int64_t>(c) * kDTokens;
+      const float* s = reinterpret_cast<const float*>(work + c * delta_chunk_bytes(NO) + (3 + NO) * kDFrags * kDFragElems * 2);
+      sreg = s[tid & 127];
+      oreg = reinterpret_cast<const int*>(s)[192];
+      kl.load(kp + t0 * a.kt, len - t0, tid);
+      ql.load(qp + t0 * a.qt, len - t0, tid);
+      vl.load(vp + t0 * a.vt, len - t0, tid);
+    };
+    auto place_qv = [&](int c) {
+      store_parts<QT, NI, E>(ql, qt + (c & (QV - 1)) * L::qstage, L::qpart, kDTokens, tid);
+      vl.store(vt + (c & (QV - 1)) * L::vstage, tid);
+    };
+    auto place_k = [&](int c) {
+      store_parts<KT, NI, E>(kl, kt + (c & 1) * NI * L::kpart, L::kpart, oreg, tid);
+      float* to = sc + (c & 1) * L::SCAL;
+      if (tid < 128) to[tid] = sreg;
+      if (tid == 128) reinterpret_cast<int*>(to)[128] = oreg;
+    };
+    // One word of every line of a later chunk's matrices, so that they lie in the L2 when they are called for.
+    auto warm_up = [&](int want) {
+      const int c = want < chunks ? want : chunks - 1;
+      asm volatile("" ::"v"(warm));
+      constexpr int lines = static_cast<int>(delta_chunk_bytes(NO) / 128);
+      for (int i = tid; i < lines; i += kWalkThreads) warm = *reinterpret_cast<const float*>(work + c * delta_chunk_bytes(NO) + 128 * i);
+    };
+    auto weights = [&](int want) {
+      const int c = want < chunks ? want : chunks - 1;
+      stored_triangle<NO>(reinterpret_cast<const uint16_t*>(work + c * delta_chunk_bytes(NO)) + 3 * kDFrags * kDFragElems, pf, lane);
+    };
+    if (chunks > 0) {
+      fetch(0);
+      place_k(0);
+      place_qv(0);
+      weights(0);
+      fetch(1);
+    }
+    __syncthreads();
+    const int p = p0 + 4 * g, row = a.H * a.P * static_cast<int>(sizeof(raw));
+    for (int c = 0; c < chunks; ++c) {
+      const int64_t t0 = static_cast<int64_t>(c) * kDTokens;
+      place_k(c + 1);
+      if constexpr (QV == 2) {
+        place_qv(c + 1);
+        fetch(c + 2);
+      }
+      warm_up(c + 3);
+      const uint16_t* qc = qt + (c & (QV - 1)) * L::qstage;
+      // S Q^T: a value a row, a token a column, as rows are stored.
+      f32x4 o[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        B8 qf[4][NI], so[NO];
+#pragma unroll
+        for (int i = 0; i < NO; ++i) so[i] = __builtin_bit_cast(B8, *reinterpret_cast<const uint4*>(sf + (s * NO + i) * kDFragElems));
+#pragma unroll
+        for (int t = 0; t < 4; ++t) row_parts_t<QT, NI>(qc, L::qpart, 16 * t, 32 * s, qf[t]);
+        mma_many<NO, false>(qf, so, o);
+      }
+      const float* scc = sc + (c & 1) * L::SCAL;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) o[t] *= scc[16 * t + n];
+      __syncthreads();
+      f32x4 m[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) m[t] = mf[64 * t];
+      const int cut = cuts[16 * w + n];
+      {
+        B8 mp[2][NO];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) split2<NO>(m[2 * s], m[2 * s + 1], mp[s]);
+        mma_triangle<NO, true, false>(pf, mp, o);
+      }
+      weights(c + 1);
+      if constexpr (QV == 1) {
+        place_qv(c + 1);
+        fetch(c + 2);
+      }
+      if (__any(cut < 64)) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int f = __shfl(cut, 4 * g + r);
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            if (16 * t + n >= f) o[t][r] = __builtin_nanf("");
+        }
+      }
+      const int64_t left = a.T - t0;
+      const __amdgpu_buffer_rsrc_t to =
+          make_rsrc(static_cast<raw*>(a.hidden) + ((static_cast<int64_t>(b) * a.T + t0) * a.H + h) * a.P, 0x7ffffff0u);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int tok = 16 * t + n;
+        if (VEC) {
+          buf_store4<E>(to, tok < left && p < a.P ? tok * row + p * static_cast<int>(sizeof(raw)) : kBufOOB, o[t]);
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            buf_store1<E>(to, tok < left && p + r < a.P ? tok * row + (p + r) * static_cast<int>(sizeof(raw)) : kBufOOB, o[t][r]);
+        }
+      }
+      if (a.miss != nullptr) {
+        const int mrow = a.H * a.P * 4, col = p0 + n;
+        const __amdgpu_buffer_rsrc_t ms =
+            make_rsrc(a.miss + ((static_cast<int64_t>(b) * a.T + t0) * a.H + h) * a.P, 0x7ffffff0u);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int tok = 16 * t + 4 * g + r;
+            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(m[t][r]), ms, t0 + tok < len && col < a.P ? tok * mrow + col * 4 : kBufOOB, 0, 0);
+          }
+        }
+      }
+      __syncthreads();
+    }
+    // Rows behind the last chunk.
+    for (int64_t t = static_cast<int64_t>(chunks) * kDTokens + tid / 16; t < a.T; t += kWalkThreads / 16) {
+      raw* to = static_cast<raw*>(a.hidden) + ((b * a.T + t) * a.H + h) * a.P + col0;
+      for (int i = tid % 16; i < kDCols && col0 + i < a.P; i += 16) to[i] = 0;
+    }
   }
 }
 
@@ -583,12 +921,12 @@ int delta_check(const grm_hip_delta_args* u, const char* what, bool step) {
     set_error("%s: token strides and row widths must be at most 2^21 elements", what);
     return GRM_HIP_EUNSUPPORTED;
   }
-  // (A grid dimension has fewer than 2^32 threads; every kernel here has 256 a workgroup.)
+  // (A grid dimension has fewer than 2^32 threads, of which a walk's workgroup has 512 and the others' 256.)
   const int64_t seqs = u->heads * min_i64(u->batch, int64_t{1} << 32), grid = int64_t{1} << 24;
   const int64_t tiles = (u->value_dim + kDCols - 1) / kDCols, chunks = (u->seq_len + kDTokens - 1) / kDTokens;
-  if (seqs >= grid || (!step && (seqs * tiles >= grid || seqs * chunks >= grid))) {
+  if (seqs >= grid || (!step && (seqs * tiles >= grid / 2 || seqs * chunks >= grid))) {
     set_error(step ? "%s: batch * heads must be below 2^24"
-                   : "%s: batch * heads * ceil(value_dim / 64) and batch * heads * ceil(seq_len / 64) must be below 2^24", what);
+                   : "%s: batch * heads * ceil(value_dim / 64) must be below 2^23 and batch * heads * ceil(seq_len / 64) below 2^24", what);
     return GRM_HIP_EUNSUPPORTED;
   }
   if (u->seq_len > 1 && (u->keys_token_stride < u->groups * u->key_dim || u->queries_token_stride < u->groups * u->key_dim ||
@@ -675,10 +1013,18 @@ extern "C" int grm_hip_delta_scan_fwd(const grm_hip_delta_args* u, void* hidden,
   delta_with_form(u->dtype, a.N, a.vec != 0 && aligned(hidden), [&](auto e, auto nk, auto vec) {
     using E = decltype(e);
     constexpr int NK = decltype(nk)::value;
-    auto kernel = delta_walk_kernel<E, NK, decltype(vec)::value>;
-    constexpr size_t lds = WalkLds<E, NK>::bytes;
-    if ((rc = set_lds(reinterpret_cast<const void*>(kernel), lds, what)) != GRM_HIP_OK) return;
-    kernel<<<dim3(static_cast<uint32_t>(a.B) * a.H * a.PT), dim3(kWalkThreads), lds, static_cast<hipStream_t>(stream)>>>(a);
+    const dim3 grid(static_cast<uint32_t>(a.B) * a.H * a.PT);
+    if constexpr (PairLds<E, NK>::fits) {
+      auto kernel = delta_pair_kernel<E, NK, decltype(vec)::value>;
+      constexpr size_t lds = PairLds<E, NK>::bytes;
+      if ((rc = set_lds(reinterpret_cast<const void*>(kernel), lds, what)) != GRM_HIP_OK) return;
+      kernel<<<grid, dim3(2 * kWalkThreads), lds, static_cast<hipStream_t>(stream)>>>(a);
+    } else {
+      auto kernel = delta_walk_kernel<E, NK, decltype(vec)::value>;
+      constexpr size_t lds = WalkLds<E, NK>::bytes;
+      if ((rc = set_lds(reinterpret_cast<const void*>(kernel), lds, what)) != GRM_HIP_OK) return;
+      kernel<<<grid, dim3(kWalkThreads), lds, static_cast<hipStream_t>(stream)>>>(a);
+    }
     rc = check_launch(what);
   });
   return rc;
