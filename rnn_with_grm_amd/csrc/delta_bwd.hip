@@ -4,8 +4,10 @@
 //   G0 = e^{c_63} G + (D dH)^T Q - (D b du)^T K,  dV = b du,  db = sum_p du m
 //   Y  = W b_j (dH m^T)  (j <= i),  X = -W b_i b_j (du m^T)  (j < i)
 //   dQ = D dH S + Y K,  dK = -D b du S + E b m G + Y^T Q + (X + X^T) K
-// and for the log decays, dc_i = row sums less column sums of T = X * K K^T + Y * Q K^T, + q.(D dH S) - k.(D b du S) - e_i
-// with e = k.(E b m G); dg_t = sum_{i >= t} dc_i + sum e + e^{c_63} <G, S>.
+// and for the log decays, with T = X * K K^T + Y * Q K^T and e_j = k_j.(E b m G)_j, dc_i = row sums less column sums of T (j < i)
+// + q_i.(D dH S)_i - k_i.(D b du S)_i - e_i; dg_t = sum_{i >= t} dc_i + sum_j e_j + e^{c_63} <G, S>.  (The column sums are
+// b m.du less e, and the rows' dh.h - dv.(v - m) in all, without a sum over pairs; but those are rounded apart from each other and
+// leave 8e-7 to 2e-6 of dg's norm where decays are weak, the sums over pairs 1e-7 to 4e-7.)
 // The walk over the chunks from the last to the first leaves du and G (delta_reverse_kernel); all else is done for all chunks
 // side by side (delta_grad_kernel).  No atomics: sums are taken in a fixed order.
 #include "delta.h"
@@ -14,6 +16,8 @@ namespace grmhip {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kGradThreads = 512;
+constexpr int kGradWaves = 2;  // a SIMD
 
 struct DeltaBwdArgs {
   DeltaArgs f;
@@ -204,46 +208,101 @@ struct GradLds {
   using ST = SelTile<BF16, NK, true>;
   static constexpr int NI = DParts<E>::IN, XS = 68;
   static constexpr int spart = 32 * ST::STRIDE, kpart = kDTokens * ST::STRIDE;
-  static constexpr size_t s = 0, gs = s + 3 * spart * 2, mf = gs + 3 * spart * 2, end1 = mf + 4 * 3 * kDFragElems * 2;
+  static constexpr size_t gs = 3 * spart * 2, mf = gs + 3 * spart * 2, stage = mf + 4 * 3 * kDFragElems * 2, end1 = 2 * stage;
   static constexpr size_t k = 0, q = k + NI * kpart * 2, x = q + NI * kpart * 2, y = x + 64 * XS * 4, end2 = y + 64 * XS * 4;
-  static constexpr size_t cum = end1 > end2 ? end1 : end2, dc = cum + 64 * 8, b = dc + 64 * 8, red = b + 64 * 4,
+  static constexpr size_t cum = end1 > end2 ? end1 : end2, dc = cum + 64 * 8, b = dc + 12 * 64 * 8, red = b + 64 * 4,
                           bytes = red + 16 * 8;
 };
 
-// Sum over the 16 lanes of a row, in every lane of it; and over the four rows.
-__device__ __forceinline__ double row_sum(double x) {
-#pragma unroll
-  for (int o = 1; o < 16; o <<= 1) x += __shfl_xor(x, o);
-  return x;
+// Sum over the 16 lanes of a row, in every lane of it (rotations by 8, 4, 2, 1), and over the four rows (rows' exchanges): no
+// trip through LDS.
+template <int CTRL>
+__device__ __forceinline__ float rotated(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+template <int CTRL>
+__device__ __forceinline__ double rotated(double x) {
+  return dpp_f64<CTRL, 0xf>(x);
 }
 template <class T>
-__device__ __forceinline__ T quad_sum(T x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
+__device__ __forceinline__ T row_sum(T x) {
+  x += rotated<0x128>(x);
+  x += rotated<0x124>(x);
+  x += rotated<0x122>(x);
+  return x + rotated<0x121>(x);
+}
+__device__ __forceinline__ float quad_sum(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+__device__ __forceinline__ double quad_sum(double x) {
+  auto both = [](auto lo, auto hi) {
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi[0]) << 32 | lo[0]) +
+           __builtin_bit_cast(double, static_cast<uint64_t>(hi[1]) << 32 | lo[1]);
+  };
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t l = static_cast<uint32_t>(u), h = static_cast<uint32_t>(u >> 32);
+  x = both(__builtin_amdgcn_permlane16_swap(l, l, false, false), __builtin_amdgcn_permlane16_swap(h, h, false, false));
+  const uint64_t v = __builtin_bit_cast(uint64_t, x);
+  const uint32_t m = static_cast<uint32_t>(v), k = static_cast<uint32_t>(v >> 32);
+  return both(__builtin_amdgcn_permlane32_swap(m, m, false, false), __builtin_amdgcn_permlane32_swap(k, k, false, false));
 }
 
-// One workgroup a chunk of a share of a group's heads; wave w holds token tile w, its gradients of keys and queries (transposed: a
-// lane has four keys of one token) summed over the heads in registers.
+// x, from here on: addresses made from it are made anew instead of being held (and spilled) since before a loop.
+__device__ __forceinline__ int anew(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
+// Values p + 0..3 and p + 16..19 of a row at byte offset `off`, as they lie in memory; zeros where not `ok` or from P on.
+template <class E, bool VEC>
+__device__ __forceinline__ U8<E> load_slots(__amdgpu_buffer_rsrc_t r, int off, int p, int P, bool ok) {
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  constexpr int ES = static_cast<int>(sizeof(typename ET<E>::raw));
+  if constexpr (VEC) {
+    const int a = ok && p < P ? off + p * ES : kBufOOB, b = ok && p + 16 < P ? off + (p + 16) * ES : kBufOOB;
+    if constexpr (ES == 2) {
+      const u32x2 lo = __builtin_amdgcn_raw_buffer_load_b64(r, a, 0, 0), hi = __builtin_amdgcn_raw_buffer_load_b64(r, b, 0, 0);
+      return __builtin_bit_cast(U8<E>, make_uint4(lo[0], lo[1], hi[0], hi[1]));
+    } else {
+      struct { u32x4 lo, hi; } v = {__builtin_amdgcn_raw_buffer_load_b128(r, a, 0, 0), __builtin_amdgcn_raw_buffer_load_b128(r, b, 0, 0)};
+      return __builtin_bit_cast(U8<E>, v);
+    }
+  } else {
+    U8<E> v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const int c = p + (e < 4 ? e : 12 + e);
+      v.e[e] = buf_load1<E>(r, ok && c < P ? off + c * ES : kBufOOB);
+    }
+    return v;
+  }
+}
+
+// One workgroup a chunk of a share of a group's heads.  Two waves a tile of 16 tokens, each with half of the keys: gradients
+// of keys and queries (transposed: a lane has four keys of one token) are summed over the heads in registers.
+// Tiles of the states lie in two stages: while one is worked on the next is split into its parts and the one behind it loaded.
 template <class E, int NK, bool VEC>
-__global__ __launch_bounds__(kThreads) void delta_grad_kernel(DeltaBwdArgs ba) {
+__global__ __launch_bounds__(kGradThreads, kGradWaves) void delta_grad_kernel(DeltaBwdArgs ba) {
   using raw = typename ET<E>::raw;
   using L = GradLds<E, NK>;
   using ST = typename L::ST;
-  constexpr int NI = L::NI, NO = DParts<E>::OUT, S = NK / 32, NT = NK / 16;
+  constexpr int NI = L::NI, NO = DParts<E>::OUT, S = NK / 32, NT = NK / 32, ES = static_cast<int>(sizeof(raw));
   const DeltaArgs& a = ba.f;
   extern __shared__ __attribute__((aligned(16))) char lds[];
-  uint16_t* stile = reinterpret_cast<uint16_t*>(lds + L::s);
-  uint16_t* gtile = reinterpret_cast<uint16_t*>(lds + L::gs);
-  uint16_t* mfrag = reinterpret_cast<uint16_t*>(lds + L::mf);
   uint16_t* kt = reinterpret_cast<uint16_t*>(lds + L::k);
   uint16_t* qt = reinterpret_cast<uint16_t*>(lds + L::q);
   float* xm = reinterpret_cast<float*>(lds + L::x);
   float* ym = reinterpret_cast<float*>(lds + L::y);
   double* cum_s = reinterpret_cast<double*>(lds + L::cum);
-  double* dc_s = reinterpret_cast<double*>(lds + L::dc);
+  double* dc_s = reinterpret_cast<double*>(lds + L::dc);  // [12][64]: own and row sums of both halves, column sums of every wave
   float* b_s = reinterpret_cast<float*>(lds + L::b);
   double* red = reinterpret_cast<double*>(lds + L::red);
-  const int tid = threadIdx.x, lane = lane_id(), w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, n = lane & 15;
+  const int tid = threadIdx.x, lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = wave & 3, half = wave >> 2;
+  const int g = lane >> 4, n = lane & 15, key0 = half * (NK / 2);
   const uint32_t at = xcd_order(blockIdx.x, gridDim.x);
   const int share = static_cast<int>(at % ba.shares), gi = static_cast<int>(at / ba.shares % a.G);
   const int c = static_cast<int>(at / ba.shares / a.G % a.C), b = static_cast<int>(at / ba.shares / a.G / a.C);
@@ -253,6 +312,7 @@ __global__ __launch_bounds__(kThreads) void delta_grad_kernel(DeltaBwdArgs ba) {
   const int hpg = a.H / a.G, h0 = gi * hpg + share * ba.per, h1 = min(h0 + ba.per, (gi + 1) * hpg);
   const int64_t row = static_cast<int64_t>(a.H) * a.P;
   const int tok = 16 * w + n;
+  const bool in = tok < rows;
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 
   f32x4 dk[NT], dq[NT];
@@ -260,6 +320,8 @@ __global__ __launch_bounds__(kThreads) void delta_grad_kernel(DeltaBwdArgs ba) {
   for (int i = 0; i < NT; ++i) dk[i] = dq[i] = zero;
 
   for (int h = h0; h < h1 && rows > 0; ++h) {
+    const int lane = anew(lane_id()), tid = wave * 64 + lane, g = lane >> 4, n = lane & 15, tok = 16 * w + n;
+    const bool in = tok < rows;
     // Scalars, lane = token, in every wave.
     float bt = 0.f, gt = 0.f;
     if (lane < rows) {
@@ -268,78 +330,110 @@ __global__ __launch_bounds__(kThreads) void delta_grad_kernel(DeltaBwdArgs ba) {
       if (a.decays != nullptr)
         gt = a.d_f32 ? static_cast<const float*>(a.decays)[j] : ET<E>::to_f(static_cast<const raw*>(a.decays)[j]);
     }
+    // Products over the values, 32 at a time; a tile's loads are under way while the one before is worked on.
+    const int64_t cells = static_cast<int64_t>(a.P) * a.N, slab = ((static_cast<int64_t>(b) * a.C + c) * a.H + h) * cells;
+    const int64_t first = (b * a.T + t0) * row + static_cast<int64_t>(h) * a.P;
+    const __amdgpu_buffer_rsrc_t mr = make_rsrc(a.miss + first, 0x7ffffff0u), ur = make_rsrc(ba.du + first, 0x7ffffff0u),
+                                 hr = make_rsrc(static_cast<const raw*>(ba.dhidden) + first, 0x7ffffff0u),
+                                 dr = make_rsrc(static_cast<raw*>(ba.dv) + first, 0x7ffffff0u);
+    const int off = tok * static_cast<int>(row);
+    TileLoad<F32, ST, BF16, VEC, 32, NK, kGradThreads> sl, gl;
+    sl.init(a.N, a.N, tid);
+    gl.init(a.N, a.N, tid);
+    U8<F32> mv, uv;
+    U8<E> hv;
+    float dots = 0.f, mu = 0.f;
+    const int tiles = (a.P + 31) / 32;
+    auto fetch = [&](int want) {  // (behind the last tile it is loaded again)
+      const int p0 = 32 * (want < tiles ? want : tiles - 1);
+      sl.load(a.states + slab + static_cast<int64_t>(p0) * a.N, a.P - p0, tid);
+      gl.load(ba.gstates + slab + static_cast<int64_t>(p0) * a.N, a.P - p0, tid);
+      mv = load_slots<F32, VEC>(mr, off * 4, p0 + 4 * g, a.P, in);
+      uv = load_slots<F32, VEC>(ur, off * 4, p0 + 4 * g, a.P, in);
+      hv = load_slots<E, VEC>(hr, off * ES, p0 + 4 * g, a.P, in);
+    };
+    auto place = [&](int tile) {
+      char* to = lds + (tile & 1) * L::stage;
+      store_parts<ST, 3, F32>(sl, reinterpret_cast<uint16_t*>(to), L::spart, 32, tid);
+      store_parts<ST, 3, F32>(gl, reinterpret_cast<uint16_t*>(to + L::gs), L::spart, 32, tid);
+      if (half == 0) {  // this wave's rows of m for the others
+        B8 mo[3];
+        split8<3>(mv.e, mo);
+        uint16_t* mf = reinterpret_cast<uint16_t*>(to + L::mf) + w * 3 * kDFragElems + 8 * lane;
+#pragma unroll
+        for (int p = 0; p < 3; ++p) *reinterpret_cast<uint4*>(mf + p * kDFragElems) = __builtin_bit_cast(uint4, mo[p]);
+      }
+      if (tile < tiles && (sl.UNITS >= kGradThreads || tid < sl.UNITS)) {
+#pragma unroll
+        for (int i = 0; i < sl.PER; ++i) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            dots = fmaf(__uint_as_float(sl.r[i][e >> 2][e & 3]), __uint_as_float(gl.r[i][e >> 2][e & 3]), dots);
+        }
+      }
+    };
+    fetch(0);
     double l = static_cast<double>(gt) * 1.4426950408889634;
     l = l < -200.0 ? -200.0 : l;
     const double cum = wave_prefix(l), total = lane_value(cum, 63);
-    __syncthreads();  // (the last head's readers are done)
-    if (w == 0) {
-      cum_s[lane] = cum;
-      b_s[lane] = bt;
-      dc_s[lane] = 0.0;
-    }
     const double mycum = __shfl(cum, tok);
     const float myb = __shfl(bt, tok), myd = exp2_d(mycum), mye = exp2_d(total - mycum);
+    const float eb = mye * myb, db = -myd * myb;
+    __syncthreads();  // (the last head's readers are done)
+    if (wave == 0) {
+      cum_s[lane] = cum;
+      b_s[lane] = bt;
+    }
 
-    // Products over the values, 32 at a time.
-    f32x4 yq[NT], yk[NT], yg[NT], wt[4], zt[4];
+    f32x4 yq[NT], yk[NT], yg[NT], wz[4];
 #pragma unroll
     for (int i = 0; i < NT; ++i) yq[i] = yk[i] = yg[i] = zero;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) wt[i] = zt[i] = zero;
-    const int64_t cells = static_cast<int64_t>(a.P) * a.N, slab = ((static_cast<int64_t>(b) * a.C + c) * a.H + h) * cells;
-    const int64_t my = (b * a.T + t0 + tok) * row + static_cast<int64_t>(h) * a.P;
-    const bool in = tok < rows;
-    TileLoad<F32, ST, BF16, VEC, 32, NK, kThreads> sl, gl;
-    sl.init(a.N, a.N, tid);
-    gl.init(a.N, a.N, tid);
-    float dots = 0.f, dbs = 0.f;
-    for (int p0 = 0; p0 < a.P; p0 += 32) {
-      sl.load(a.states + slab + static_cast<int64_t>(p0) * a.N, a.P - p0, tid);
-      gl.load(ba.gstates + slab + static_cast<int64_t>(p0) * a.N, a.P - p0, tid);
-      // This wave's rows: slots 0-3 are values 4 g + e, 4-7 are 16 + 4 g + e.
-      float mv[8], uv[8];
-      U8<E> hv;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int p = p0 + (e < 4 ? 4 * g + e : 12 + 4 * g + e);
-        const bool ok = in && p < a.P;
-        mv[e] = ok ? a.miss[my + p] : 0.f;
-        uv[e] = ok ? ba.du[my + p] : 0.f;
-        hv.e[e] = ok ? static_cast<const raw*>(ba.dhidden)[my + p] : raw(0);
-      }
-      B8 mp[3], up[3], hp[NI];
-      split8<3>(mv, mp);
-      split8<3>(uv, up);
+    for (int i = 0; i < 4; ++i) wz[i] = zero;
+    place(0);
+    for (int tile = 0; tile < tiles; ++tile) {
+      const int p0 = 32 * tile;
+      B8 up[3], hp[NI];
+      split8<3>(uv.e, up);
       input_parts<E, NI>(hv, hp);
-      __syncthreads();
-      store_parts<ST, 3, F32>(sl, stile, L::spart, 32, tid);
-      store_parts<ST, 3, F32>(gl, gtile, L::spart, 32, tid);
+      if (half == 1) {  // dV, and the strengths' sums
+        float dv[8];
 #pragma unroll
-      for (int i = 0; i < sl.PER; ++i) {
+        for (int e = 0; e < 8; ++e) {
+          dv[e] = myb * uv.e[e];
+          mu = fmaf(uv.e[e], mv.e[e], mu);
+        }
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          dots = fmaf(__uint_as_float(sl.r[i][e >> 2][e & 3]), __uint_as_float(gl.r[i][e >> 2][e & 3]), dots);
+        for (int u = 0; u < 2; ++u) {
+          const int p = p0 + 4 * g + 16 * u;
+          if (VEC) {
+            buf_store4<E>(dr, in && p < a.P ? (off + p) * ES : kBufOOB, f32x4{dv[4 * u], dv[4 * u + 1], dv[4 * u + 2], dv[4 * u + 3]});
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) buf_store1<E>(dr, in && p + r < a.P ? (off + p + r) * ES : kBufOOB, dv[4 * u + r]);
+          }
+        }
       }
-#pragma unroll
-      for (int p = 0; p < 3; ++p)
-        *reinterpret_cast<uint4*>(mfrag + (w * 3 + p) * kDFragElems + 8 * lane) = __builtin_bit_cast(uint4, mp[p]);
-      // dV and the strengths' sums.
-      raw* dv = static_cast<raw*>(ba.dv) + my + p0;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int p = e < 4 ? 4 * g + e : 12 + 4 * g + e;
-        dbs = fmaf(uv[e], mv[e], dbs);
-        if (in && p0 + p < a.P) dv[p] = ET<E>::from_f(myb * uv[e]);
-      }
+      fetch(tile + 1);
       __syncthreads();
+      const char* from = lds + (tile & 1) * L::stage;
+      const uint16_t* stile = reinterpret_cast<const uint16_t*>(from);
+      const uint16_t* gtile = reinterpret_cast<const uint16_t*>(from + L::gs);
+      const uint16_t* mfrag = reinterpret_cast<const uint16_t*>(from + L::mf);
+      {
+        B8 mp[3];
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        B8 sf[3], gf[3];
-        col_parts<ST, 3>(stile, L::spart, 0, 16 * i, sf);
-        col_parts<ST, 3>(gtile, L::spart, 0, 16 * i, gf);
-        yq[i] = mma_parts<3>(sf, hp, yq[i]);
-        yk[i] = mma_parts<3>(sf, up, yk[i]);
-        yg[i] = mma_parts<3>(gf, mp, yg[i]);
+        for (int p = 0; p < 3; ++p)
+          mp[p] = __builtin_bit_cast(B8, *reinterpret_cast<const uint4*>(mfrag + (w * 3 + p) * kDFragElems + 8 * lane));
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          B8 sf[3], gf[3];
+          col_parts<ST, 3>(stile, L::spart, 0, key0 + 16 * i, sf);
+          col_parts<ST, 3>(gtile, L::spart, 0, key0 + 16 * i, gf);
+          yq[i] = mma_parts<3>(sf, hp, yq[i]);
+          yk[i] = mma_parts<3>(sf, up, yk[i]);
+          yg[i] = mma_parts<3>(gf, mp, yg[i]);
+        }
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -348,35 +442,33 @@ __global__ __launch_bounds__(kThreads) void delta_grad_kernel(DeltaBwdArgs ba) {
 #pragma unroll
           for (int p = 0; p < 3; ++p)
             f[p] = __builtin_bit_cast(B8, *reinterpret_cast<const uint4*>(mfrag + (j * 3 + p) * kDFragElems + 8 * lane));
-          wt[j] = mma_parts<3>(up, f, wt[j]);  // rows i = 16 w + 4 g + r, column j = 16 j + n
-          zt[j] = mma_parts<3>(hp, f, zt[j]);
+          // Rows i = 16 w + 4 g + r, column j = 16 j + n: half 0 du m^T, half 1 dH m^T.
+          if (half == 0) wz[j] = mma_parts<3>(up, f, wz[j]);
+          else wz[j] = mma_parts<3>(hp, f, wz[j]);
         }
       }
+      place(tile + 1);
     }
-    // <G, S> over the workgroup.
-    double dot = static_cast<double>(dots);
-    dot = quad_sum(row_sum(dot));
-    if (lane == 0) red[w] = dot;
     __syncthreads();  // (the tiles make room)
     {
-      TileLoad<E, ST, BF16, VEC, kDTokens, NK, kThreads> kl;
+      TileLoad<E, ST, BF16, VEC, kDTokens, NK, kGradThreads> kl, ql;
       kl.init(a.kt, a.N, tid);
+      ql.init(a.qt, a.N, tid);
       kl.load(static_cast<const raw*>(a.keys) + b * a.kb + t0 * a.kt + static_cast<int64_t>(gi) * a.N, rows, tid);
+      ql.load(static_cast<const raw*>(a.queries) + b * a.qb + t0 * a.qt + static_cast<int64_t>(gi) * a.N, rows, tid);
       store_parts<ST, NI, E>(kl, kt, L::kpart, kDTokens, tid);
-      kl.init(a.qt, a.N, tid);
-      kl.load(static_cast<const raw*>(a.queries) + b * a.qb + t0 * a.qt + static_cast<int64_t>(gi) * a.N, rows, tid);
-      store_parts<ST, NI, E>(kl, qt, L::kpart, kDTokens, tid);
+      store_parts<ST, NI, E>(ql, qt, L::kpart, kDTokens, tid);
     }
     __syncthreads();
-    // q.(D dH S), k.(D b du S), k.(E b m G): a lane's four keys of every tile, then over the four rows of lanes.
+    // q.(dH S), k.(du S), k.(m G): a lane's four keys of every tile.
     float al = 0.f, be = 0.f, ep = 0.f;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       f32x4 kv = zero, qv = zero;
 #pragma unroll
       for (int p = NI - 1; p >= 0; --p) {
-        const uint2 ku = *reinterpret_cast<const uint2*>(kt + p * L::kpart + ST::at(tok, 16 * i + 4 * g));
-        const uint2 qu = *reinterpret_cast<const uint2*>(qt + p * L::kpart + ST::at(tok, 16 * i + 4 * g));
+        const uint2 ku = *reinterpret_cast<const uint2*>(kt + p * L::kpart + ST::at(tok, key0 + 16 * i + 4 * g));
+        const uint2 qu = *reinterpret_cast<const uint2*>(qt + p * L::kpart + ST::at(tok, key0 + 16 * i + 4 * g));
         kv += f32x4{__uint_as_float(ku.x << 16), __uint_as_float(ku.x & 0xffff0000u), __uint_as_float(ku.y << 16),
                     __uint_as_float(ku.y & 0xffff0000u)};
         qv += f32x4{__uint_as_float(qu.x << 16), __uint_as_float(qu.x & 0xffff0000u), __uint_as_float(qu.y << 16),
@@ -389,98 +481,110 @@ __global__ __launch_bounds__(kThreads) void delta_grad_kernel(DeltaBwdArgs ba) {
         ep = fmaf(kv[r], yg[i][r], ep);
       }
       dq[i] += yq[i] * myd;
-      dk[i] += yg[i] * (mye * myb) - yk[i] * (myd * myb);
+      dk[i] += yg[i] * eb + yk[i] * db;
     }
-    const double eps = quad_sum(static_cast<double>(ep) * static_cast<double>(mye * myb));
-    const double own = quad_sum(static_cast<double>(al) * static_cast<double>(myd) -
-                                static_cast<double>(be) * static_cast<double>(myd * myb)) - eps;
-    dbs = quad_sum(dbs);
-    const double esum = row_sum(eps);  // of this wave's 16 tokens
-    if (lane == 0) red[4 + w] = esum;
+    // <G, S>, and the sum of k.(E b m G), over the workgroup.
+    const double eps = static_cast<double>(ep) * static_cast<double>(eb);
+    {
+      double e = eps + static_cast<double>(dots) * static_cast<double>(exp2_d(total));
+      e = quad_sum(row_sum(e));
+      if (lane == 0) red[wave] = e;
+    }
+    const double own = quad_sum(static_cast<double>(al) * static_cast<double>(myd) + static_cast<double>(be) * static_cast<double>(db) - eps);
+    mu = quad_sum(mu);
+    if (g == 0) {
+      dc_s[half * 64 + tok] = own;
+      if (half == 1 && tok < all) {
+        const int64_t i = (b * a.T + t0 + tok) * a.H + h;
+        const float v = in ? mu : 0.f;
+        if (a.s_f32) static_cast<float*>(ba.ds)[i] = v;
+        else static_cast<raw*>(ba.ds)[i] = ET<E>::from_f(v);
+      }
+    }
 
-    // The matrices between tokens, and what they give the decays.
-    double rsum[4] = {0.0, 0.0, 0.0, 0.0}, csum[4] = {0.0, 0.0, 0.0, 0.0};
+    // The matrices between tokens, half 0 X and half 1 Y, and their shares of T's row and column sums.
+    f32x4 dot[4];
+    const int lane2 = anew(lane), g2 = lane2 >> 4, n2 = lane2 & 15;
+    {
+      const uint16_t* left = half == 0 ? kt : qt;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) dot[j] = zero;
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        B8 li[NI], kj[4][NI];
+        row_parts_t<ST, NI>(left, L::kpart, 16 * w, 32 * s, li);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) row_parts_t<ST, NI>(kt, L::kpart, 16 * j, 32 * s, kj[j]);
+        mma_many<3, false>(kj, li, dot);  // (tiles above the diagonal are not used)
+      }
+    }
+    double rsum[4] = {0.0, 0.0, 0.0, 0.0}, ci[4];
+    float bi[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      ci[r] = cum_s[16 * w + 4 * g2 + r];
+      bi[r] = half == 0 ? -b_s[16 * w + 4 * g2 + r] : 1.f;
+    }
+    float* mat = half == 0 ? xm : ym;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
+      double csum = 0.0;
       if (j <= w) {
-        f32x4 kk = zero, qk = zero;
-#pragma unroll
-        for (int s = 0; s < S; ++s) {
-          B8 ki[NI], qi[NI], kj[NI];
-          row_parts_t<ST, NI>(kt, L::kpart, 16 * w, 32 * s, ki);
-          row_parts_t<ST, NI>(qt, L::kpart, 16 * w, 32 * s, qi);
-          row_parts_t<ST, NI>(kt, L::kpart, 16 * j, 32 * s, kj);
-          kk = mma_parts<3>(ki, kj, kk);
-          qk = mma_parts<3>(qi, kj, qk);
-        }
-        const int tj = 16 * j + n;
+        const int tj = 16 * j + n2;
         const double cj = cum_s[tj];
         const float bj = b_s[tj];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const int ti = 16 * w + 4 * g + r;
-          const float decay = tj <= ti ? exp2_d(cum_s[ti] - cj) : 0.f;
-          const float y = decay * bj * zt[j][r];
-          const float x = tj < ti ? -decay * b_s[ti] * bj * wt[j][r] : 0.f;
-          ym[ti * L::XS + tj] = y;
-          if (tj <= ti) xm[ti * L::XS + tj] = xm[tj * L::XS + ti] = x;
-          if (tj < ti) {  // (a token's weight of itself does not decay)
-            const double tau = static_cast<double>(x) * static_cast<double>(kk[r]) + static_cast<double>(y) * static_cast<double>(qk[r]);
-            rsum[r] += tau;
-            csum[j] += tau;
-          }
+          const int ti = 16 * w + 4 * g2 + r;
+          const bool below = tj < ti, seen = half == 0 ? below : tj <= ti;
+          const float x = (seen ? exp2_f(static_cast<float>(ci[r] - cj)) * (bi[r] * bj) : 0.f) * wz[j][r];
+          // (What lies above the diagonal goes to the row's padding.)
+          mat[ti * L::XS + (tj <= ti ? tj : 64)] = x;
+          if (half == 0) mat[tj <= ti ? tj * L::XS + ti : ti * L::XS + 64] = x;
+          // (A token's weight of itself does not decay.  Row and column sums take the same rounded product, so that what
+          // cancels between them does so whole.)
+          const double tau = below ? static_cast<double>(x * dot[j][r]) : 0.0;
+          rsum[r] += tau;
+          csum += tau;
         }
       }
+      csum = quad_sum(csum);
+      if (g2 == 0) dc_s[(4 + wave) * 64 + 16 * j + n2] = csum;
     }
 #pragma unroll
-    for (int r = 0; r < 4; ++r) rsum[r] = row_sum(rsum[r]);
-    // One wave at a time adds its column sums: a fixed order.
-    for (int v = 0; v < 4; ++v) {
-      if (v == w) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const double cs = quad_sum(csum[j]);
-          if (j <= w && g == 0) dc_s[16 * j + n] -= cs;
-        }
-      }
-      __syncthreads();
+    for (int r = 0; r < 4; ++r) {
+      rsum[r] = row_sum(rsum[r]);
+      if (n2 == 0) dc_s[(2 + half) * 64 + 16 * w + 4 * g2 + r] = rsum[r];
     }
-    // (A wave's own rows from here on.)
+    __syncthreads();
+    if (wave == 0 && ba.dd != nullptr) {
+      double d = 0.0;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (n == 0) dc_s[16 * w + 4 * g + r] += rsum[r];
-    __syncthreads();
-    if (g == 0) dc_s[tok] += own;
-    __syncthreads();
-    if (w == 0) {
-      // dg_t = sum_{i >= t} dc_i + sum e + e^{c_63} <G, S>.
-      const double d = dc_s[lane], pre = wave_prefix(d), whole = lane_value(pre, 63);
-      const double dg = whole - pre + d + (red[4] + red[5] + red[6] + red[7]) +
-                        static_cast<double>(exp2_d(total)) * (red[0] + red[1] + red[2] + red[3]);
-      if (ba.dd != nullptr && lane < all) {
+      for (int i = 0; i < 12; ++i) d += i < 4 ? dc_s[64 * i + lane] : -dc_s[64 * i + lane];
+      const double pre = wave_prefix(d), whole = lane_value(pre, 63);
+      double dg = whole - pre + d;
+#pragma unroll
+      for (int i = 0; i < kGradThreads / 64; ++i) dg += red[i];
+      if (lane < all) {
         const int64_t i = (b * a.T + t0 + lane) * a.H + h;
         const float v = lane < rows ? static_cast<float>(dg) : 0.f;
         if (a.d_f32) static_cast<float*>(ba.dd)[i] = v;
         else static_cast<raw*>(ba.dd)[i] = ET<E>::from_f(v);
       }
     }
-    if (g == 0 && tok < all) {
-      const int64_t i = (b * a.T + t0 + tok) * a.H + h;
-      const float v = in ? dbs : 0.f;
-      if (a.s_f32) static_cast<float*>(ba.ds)[i] = v;
-      else static_cast<raw*>(ba.ds)[i] = ET<E>::from_f(v);
-    }
     // dQ^T += K^T Y^T, dK^T += K^T (X + X^T) + Q^T Y.
+    const int lane3 = anew(lane), g3 = lane3 >> 4, tok3 = 16 * w + (lane3 & 15);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       float yr[8], xr[8], yc[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int k = 32 * s + (e < 4 ? 4 * g + e : 12 + 4 * g + e);
-        // (16 x 16 tiles above the diagonal of Y are not written.)
-        yr[e] = (k >> 4) <= w ? ym[tok * L::XS + k] : 0.f;
-        yc[e] = (k >> 4) >= w ? ym[k * L::XS + tok] : 0.f;
-        xr[e] = xm[tok * L::XS + k];
+        const int k = 32 * s + (e < 4 ? 4 * g3 + e : 12 + 4 * g3 + e);
+        // (Y is not written above the diagonal.)
+        const float up = ym[tok3 * L::XS + k], down = ym[k * L::XS + tok3];
+        yr[e] = k <= tok3 ? up : 0.f;
+        yc[e] = k >= tok3 ? down : 0.f;
+        xr[e] = xm[tok3 * L::XS + k];
       }
       B8 yp[NO], xp[NO], cp[NO];
       split8<NO>(yr, yp);
@@ -489,8 +593,8 @@ __global__ __launch_bounds__(kThreads) void delta_grad_kernel(DeltaBwdArgs ba) {
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         B8 kf[NI], qf[NI];
-        col_parts<ST, NI>(kt, L::kpart, 32 * s, 16 * i, kf);
-        col_parts<ST, NI>(qt, L::kpart, 32 * s, 16 * i, qf);
+        col_parts<ST, NI>(kt, L::kpart, 32 * s, key0 + 16 * i, kf);
+        col_parts<ST, NI>(qt, L::kpart, 32 * s, key0 + 16 * i, qf);
         dq[i] = mma_parts<NO>(kf, yp, dq[i]);
         dk[i] = mma_parts<NO>(kf, xp, dk[i]);
         dk[i] = mma_parts<NO>(qf, cp, dk[i]);
@@ -500,7 +604,7 @@ __global__ __launch_bounds__(kThreads) void delta_grad_kernel(DeltaBwdArgs ba) {
   // Rows behind the length.
   if (rows < all) {
     for (int h = h0; h < h1; ++h) {
-      for (int i = tid; i < (all - rows) * a.P; i += kThreads) {
+      for (int i = tid; i < (all - rows) * a.P; i += kGradThreads) {
         const int r = rows + i / a.P;
         static_cast<raw*>(ba.dv)[(b * a.T + t0 + r) * row + static_cast<int64_t>(h) * a.P + i % a.P] = 0;
       }
@@ -521,7 +625,7 @@ __global__ __launch_bounds__(kThreads) void delta_grad_kernel(DeltaBwdArgs ba) {
     const bool whole = (a.N & 3) == 0;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const int k = 16 * i + 4 * g;
+      const int k = key0 + 16 * i + 4 * g;
       if (k >= a.N) continue;
       if (ba.part != nullptr) {
         float* pk = ba.part + share * plane + to + k;
@@ -659,7 +763,7 @@ extern "C" int grm_hip_delta_scan_bwd(const grm_hip_delta_args* u, const float* 
     auto kernel = delta_grad_kernel<E, NK, VEC>;
     constexpr size_t lds = GradLds<E, NK>::bytes;
     if ((rc = set_lds(reinterpret_cast<const void*>(kernel), lds)) != GRM_HIP_OK) return;
-    kernel<<<dim3(static_cast<uint32_t>(a.f.B) * a.f.C * a.f.G * a.shares), dim3(kThreads), lds, hs>>>(a);
+    kernel<<<dim3(static_cast<uint32_t>(a.f.B) * a.f.C * a.f.G * a.shares), dim3(kGradThreads), lds, hs>>>(a);
     if ((rc = check_launch(what)) != GRM_HIP_OK || a.part == nullptr) return;
     const int64_t plane = static_cast<int64_t>(a.f.B) * a.f.T * a.f.G * a.f.N, blocks = (2 * plane + kThreads - 1) / kThreads;
     delta_share_sum_kernel<E><<<dim3(static_cast<uint32_t>(blocks < 4096 ? blocks : 4096)), dim3(kThreads), 0, hs>>>(
