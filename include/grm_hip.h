@@ -617,7 +617,7 @@ typedef struct grm_hip_delta_args {
  *             before every 64 tokens, which the backward reads (those behind a length are left as
  *             they were).
  * miss:       NULL, or float32 [batch, seq_len, heads, value_dim]: v_t - a_t M_{t-1} k_t, which the
- *             backward reads (rows behind a length are left as they were).
+ *             backward reads (rows behind a length are left as they were).  Given with states or not at all.
  * workspace:  grm_hip_delta_scan_workspace() bytes, 16-byte aligned.
  */
 int64_t grm_hip_delta_scan_workspace(int64_t batch, int64_t seq_len, int64_t heads, int dtype);

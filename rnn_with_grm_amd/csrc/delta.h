@@ -142,6 +142,38 @@ __device__ __forceinline__ void mma_triangle(const B8 (&f)[kDFrags][NA], const B
   }
 }
 
+// A wave's 16 value rows of a state to memory, as state_store does; WHOLE: rows of whole 16-byte units, and no branch
+// around the stores, so that waits for loads before them are counted past them.
+template <bool WHOLE, int NT>
+__device__ __forceinline__ void state_out(const f32x4 (&acc)[NT], float* s, int p0, int P, int N) {
+  if constexpr (!WHOLE) {
+    state_store<NT>(acc, s, p0, P, N);
+  } else {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    int lane = lane_id();
+    asm volatile("" : "+v"(lane));  // no address made from it is kept in registers between stores
+    const int low = lane & 8;
+    const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(s, static_cast<uint32_t>(P * N * 4));
+#pragma unroll
+    for (int nt = 0; nt < NT; nt += 2) {  // (halves exchanged between lanes eight apart: whole 128-byte lines)
+      const int n = nt * 16 + 2 * low + 4 * (lane >> 4);
+      f32x4 v[2];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float give = low ? acc[nt][r] : acc[nt + 1][r];
+        const float take = __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(give), 0x128, 0xf, 0xf, true));
+        v[0][r] = low ? take : acc[nt][r];
+        v[1][r] = low ? acc[nt + 1][r] : take;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int row = p0 + 8 * u + (lane & 7);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[u]), rsrc, row < P && n < N ? (row * N + n) * 4 : kBufOOB, 0, 0);
+      }
+    }
+  }
+}
+
 // Eight elements of type E as their parts.
 template <class E, int NI>
 __device__ __forceinline__ void input_parts(const U8<E>& u, B8 (&f)[NI]) {

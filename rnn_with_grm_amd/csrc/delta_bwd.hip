@@ -47,7 +47,7 @@ __device__ __forceinline__ void scaled_pair(const f32x4& lo, const f32x4& hi, co
                       f32x4{hi[0] * b.x, hi[1] * b.y, hi[2] * b.z, hi[3] * b.w}, out);
 }
 
-// The walk's mirror: 16 value columns of the gradient's state a wave, chunks from the last to the first.
+// The same where two stages of keys do not fit into LDS (float16 and float32 keys wider than 64): four waves that do all of it.
 template <class E, int NK, bool VEC>
 __global__ __launch_bounds__(kThreads) void delta_reverse_kernel(DeltaBwdArgs ba) {
   using raw = typename ET<E>::raw;
@@ -199,6 +199,253 @@ __global__ __launch_bounds__(kThreads) void delta_reverse_kernel(DeltaBwdArgs ba
     }
   }
   state_store<NT>(st, ba.dm + head * cells, p0, a.P, a.N);
+}
+
+// LDS of the mirror walk in two halves.
+template <class E, int NK>
+struct MirrorLds {
+  using KT = SelTile<BF16, NK, true>;
+  using VT = SelTile<E, kDCols, true>;
+  static constexpr int NI = DParts<E>::IN, kpart = kDTokens * KT::STRIDE, SCAL = 192, NT = NK / 16;
+  static constexpr size_t k = 0, q = k + 2 * NI * kpart * 2, v = q + NI * kpart * 2,
+                          z = v + kDTokens * VT::STRIDE * sizeof(typename ET<E>::raw), u = z + 4 * 4 * 64 * 16,
+                          c = u + 4 * 4 * 64 * 16, s = c + 4 * NT * 64 * 16, bytes = s + 2 * SCAL * 4;
+  static constexpr bool fits = bytes <= 160 * 1024;
+};
+
+// The walk's mirror: 64 value columns of the gradient's state a workgroup, chunks from the last to the first.  Four state
+// waves run the chain that the next chunk hangs on (K G^T, du, the state's update by the keys); four output waves, one beside
+// each on its SIMD, load the chunks ahead, form what hangs on no state, (W * Q K^T)^T dH and (D dH)^T Q, one chunk ahead, and
+// store du.  Two barriers a chunk: du is there, the next state is there.
+template <class E, int NK, bool VEC>
+__global__ __launch_bounds__(2 * kThreads, 2) void delta_mirror_kernel(DeltaBwdArgs ba) {
+  using raw = typename ET<E>::raw;
+  using L = MirrorLds<E, NK>;
+  using KT = typename L::KT;
+  using VT = typename L::VT;
+  constexpr int NI = L::NI, S = NK / 32, NT = NK / 16;
+  const DeltaArgs& a = ba.f;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  uint16_t* kt = reinterpret_cast<uint16_t*>(lds + L::k);
+  uint16_t* qt = reinterpret_cast<uint16_t*>(lds + L::q);
+  raw* vt = reinterpret_cast<raw*>(lds + L::v);
+  float* sc = reinterpret_cast<float*>(lds + L::s);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
+  const int lane = lane_id(), g = lane >> 4, n = lane & 15;
+  const uint32_t at = xcd_order(blockIdx.x, gridDim.x);
+  const int pt = static_cast<int>(at % a.PT), h = static_cast<int>(at / a.PT % a.H), b = static_cast<int>(at / a.PT / a.H);
+  const int64_t len = delta_length(a, b);
+  const int col0 = pt * kDCols, p0 = col0 + 16 * w, gi = h / (a.H / a.G);
+  const int chunks = static_cast<int>((len + kDTokens - 1) / kDTokens);
+  const int64_t head = static_cast<int64_t>(b) * a.H + h, cells = static_cast<int64_t>(a.P) * a.N, row = static_cast<int64_t>(a.H) * a.P;
+  const char* work = a.work + head * a.C * delta_chunk_bytes(3);
+  f32x4* zf = reinterpret_cast<f32x4*>(lds + L::z) + w * 256 + lane;
+  f32x4* uf = reinterpret_cast<f32x4*>(lds + L::u) + w * 256 + lane;
+  f32x4* cf = reinterpret_cast<f32x4*>(lds + L::c) + w * NT * 64 + lane;
+
+  if (wave < 4) {
+    __builtin_amdgcn_s_setprio(2);
+    f32x4 st[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) st[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (ba.dmemory != nullptr) state_add<NT>(st, ba.dmemory + head * cells, p0, a.P, a.N, 1.f);
+    B8 tf[kDFrags][3], gp[S][3], kr[2][4][NI];
+    auto row_keys = [&](const uint16_t* from, int s) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) row_parts_t<KT, NI>(from, L::kpart, 16 * t, 32 * s, kr[s & 1][t]);
+    };
+    auto keep_state = [&](int c) {  // (before the first chunk: behind the last value row, where nothing is stored)
+      state_out<VEC>(st, ba.gstates + ((static_cast<int64_t>(b) * a.C + (c < 0 ? 0 : c)) * a.H + h) * cells, c < 0 ? a.P : p0, a.P, a.N);
+    };
+#pragma unroll
+    for (int s = 0; s < S; ++s) split2<3>(st[2 * s], st[2 * s + 1], gp[s]);
+    if (chunks > 0) {
+      stored_triangle<3>(reinterpret_cast<const uint16_t*>(work + (chunks - 1) * delta_chunk_bytes(3)), tf, lane);
+      keep_state(chunks - 1);
+    }
+    __syncthreads();
+    __syncthreads();
+    if (chunks > 0) row_keys(kt + ((chunks - 1) & 1) * NI * L::kpart, 0);
+    for (int c = chunks - 1; c >= 0; --c) {
+      const uint16_t* kc = kt + (c & 1) * NI * L::kpart;
+      const float* scc = sc + (c & 1) * L::SCAL;
+      const int next = c > 0 ? c - 1 : 0;
+      f32x4 z[4], z0[4];
+      float4 e[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        z[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        z0[t] = zf[64 * t];
+        e[t] = *reinterpret_cast<const float4*>(scc + 64 + 16 * t + 4 * g);
+      }
+      hold_order();
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        if (s + 1 < S) row_keys(kc, s + 1);
+        mma_many<3, true>(kr[s & 1], gp[s], z);
+        hold_order();
+      }
+      f32x4 du[4];
+      {
+        B8 zp[2][3];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          z[t] = f32x4{fmaf(z[t][0], e[t].x, z0[t][0]), fmaf(z[t][1], e[t].y, z0[t][1]), fmaf(z[t][2], e[t].z, z0[t][2]),
+                       fmaf(z[t][3], e[t].w, z0[t][3])};
+          du[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+#pragma unroll
+        for (int s = 0; s < 2; ++s) split2<3>(z[2 * s], z[2 * s + 1], zp[s]);
+        mma_triangle<3, false, true>(tf, zp, du);
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) uf[64 * t] = du[t];
+      B8 kf[2][2][2][NI];  // [pair & 1][step][tile of the pair]
+      auto pair_keys = [&](int j) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) col_parts<KT, NI>(kc, L::kpart, 32 * s, 16 * (2 * j + i), kf[j & 1][s][i]);
+        }
+      };
+      pair_keys(0);
+      __syncthreads();
+      // G0 = e^{c_63} G + (D dH)^T Q - (D b du)^T K, two tiles of keys at a time.
+      const float keep = scc[63];
+      const uint16_t* tn = reinterpret_cast<const uint16_t*>(work + next * delta_chunk_bytes(3));
+      B8 ep[2][3];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        f32x4 em[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float4 d = *reinterpret_cast<const float4*>(scc + 32 * s + 16 * i + 4 * g),
+                       bb = *reinterpret_cast<const float4*>(scc + 128 + 32 * s + 16 * i + 4 * g);
+          const f32x4 v = du[2 * s + i];
+          em[i] = f32x4{-v[0] * (d.x * bb.x), -v[1] * (d.y * bb.y), -v[2] * (d.z * bb.z), -v[3] * (d.w * bb.w)};
+        }
+        split2<3>(em[0], em[1], ep[s]);
+      }
+#pragma unroll
+      for (int j = 0; j < S; ++j) {
+        if (j + 1 < S) pair_keys(j + 1);
+        f32x4 y[2] = {st[2 * j] * keep + cf[64 * (2 * j)], st[2 * j + 1] * keep + cf[64 * (2 * j + 1)]};
+#pragma unroll
+        for (int s = 0; s < 2; ++s) mma_many<3, true>(kf[j & 1][s], ep[s], y);
+        st[2 * j] = y[0];
+        st[2 * j + 1] = y[1];
+        constexpr int per = (kDFrags + S - 1) / S;
+#pragma unroll
+        for (int f = j * per; f < (j + 1) * per; ++f)
+          if (f < kDFrags) stored_parts<3>(tn, f, tf[f], lane);
+        if (j > 0) split2<3>(st[2 * j - 2], st[2 * j - 1], gp[j - 1]);
+        hold_order();
+      }
+      split2<3>(st[NT - 2], st[NT - 1], gp[S - 1]);
+      keep_state(c - 1);
+      row_keys(kt + (next & 1) * NI * L::kpart, 0);  // (there since the chunk's first barrier)
+      __syncthreads();
+    }
+    state_store<NT>(st, ba.dm + head * cells, p0, a.P, a.N);
+  } else {
+    const int tid = static_cast<int>(threadIdx.x) - kThreads;
+    const raw* kp = static_cast<const raw*>(a.keys) + b * a.kb + static_cast<int64_t>(gi) * a.N;
+    const raw* qp = static_cast<const raw*>(a.queries) + b * a.qb + static_cast<int64_t>(gi) * a.N;
+    const raw* vp = static_cast<const raw*>(ba.dhidden) + b * a.T * row + static_cast<int64_t>(h) * a.P + col0;
+    TileLoad<E, KT, BF16, VEC, kDTokens, NK, kThreads> kl, ql;
+    TileLoad<E, VT, E, VEC, kDTokens, kDCols, kThreads> vl;
+    kl.init(a.kt, a.N, tid);
+    ql.init(a.qt, a.N, tid);
+    vl.init(row, a.P - col0 < kDCols ? a.P - col0 : kDCols, tid);
+    float sreg = 0.f, warm = 0.f;
+    B8 pf[kDFrags][3];
+    auto fetch = [&](int want) {  // (before the first chunk it is loaded again)
+      const int c = want > 0 ? want : 0;
+      const int64_t t0 = static_cast<int64_t>(c) * kDTokens;
+      sreg = reinterpret_cast<const float*>(work + c * delta_chunk_bytes(3) + 6 * kDFrags * kDFragElems * 2)[tid < 192 ? tid : 0];
+      kl.load(kp + t0 * a.kt, len - t0, tid);
+      ql.load(qp + t0 * a.qt, len - t0, tid);
+      vl.load(vp + t0 * row, len - t0, tid);
+    };
+    auto place = [&](int c) {
+      store_parts<KT, NI, E>(kl, kt + (c & 1) * NI * L::kpart, L::kpart, kDTokens, tid);
+      store_parts<KT, NI, E>(ql, qt, L::kpart, kDTokens, tid);
+      vl.store(vt, tid);
+      if (tid < 192) sc[(c & 1) * L::SCAL + tid] = sreg;
+    };
+    auto weights = [&](int want) {
+      stored_triangle<3>(reinterpret_cast<const uint16_t*>(work + (want > 0 ? want : 0) * delta_chunk_bytes(3)) + 3 * kDFrags * kDFragElems, pf, lane);
+    };
+    // One word of every line of a later chunk's matrices, so that they lie in the L2 when they are called for.
+    auto warm_up = [&](int want) {
+      asm volatile("" ::"v"(warm));
+      constexpr int lines = static_cast<int>(delta_chunk_bytes(3) / 128);
+      for (int i = tid; i < lines; i += kThreads) warm = *reinterpret_cast<const float*>(work + (want > 0 ? want : 0) * delta_chunk_bytes(3) + 128 * i);
+    };
+    f32x4 cc[NT];
+    // What hangs on no state: (W * Q K^T)^T dH for the state waves, (D dH)^T Q into cc.
+    auto ahead = [&](int c) {
+      B8 hp[2][NI];
+      f32x4 dh[4], z[4];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const Frag8<E> f = col_frag<VT, E>(vt, 32 * s, 16 * w);
+        input_parts<E, NI>(__builtin_bit_cast(U8<E>, f), hp[s]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          dh[2 * s][r] = ET<E>::to_f(f.e[r]);
+          dh[2 * s + 1][r] = ET<E>::to_f(f.e[4 + r]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) z[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      mma_triangle<3, false, true>(pf, hp, z);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) zf[64 * t] = z[t];
+      weights(c - 1);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) cc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        B8 dp[3], qf[NT][NI];
+        scaled_pair(dh[2 * s], dh[2 * s + 1], sc + (c & 1) * L::SCAL + 32 * s, g, dp);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) col_parts<KT, NI>(qt, L::kpart, 32 * s, 16 * i, qf[i]);
+        mma_many<3, true>(qf, dp, cc);
+      }
+    };
+    if (chunks > 0) {
+      fetch(chunks - 1);
+      weights(chunks - 1);
+      place(chunks - 1);
+      fetch(chunks - 2);
+    }
+    __syncthreads();
+    if (chunks > 0) ahead(chunks - 1);
+    __syncthreads();
+    for (int c = chunks - 1; c >= 0; --c) {
+      const int64_t t0 = static_cast<int64_t>(c) * kDTokens;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) cf[64 * i] = cc[i];
+      if (c > 0) place(c - 1);
+      fetch(c - 2);
+      warm_up(c - 3);
+      __syncthreads();
+      const __amdgpu_buffer_rsrc_t to = make_rsrc(ba.du + (b * a.T + t0) * row + static_cast<int64_t>(h) * a.P, 0x7ffffff0u);
+      const int step = static_cast<int>(row) * 4, col = p0 + n;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const f32x4 du = uf[64 * t];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int tok = 16 * t + 4 * g + r;
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(du[r]), to, t0 + tok < len && col < a.P ? tok * step + col * 4 : kBufOOB, 0, 0);
+        }
+      }
+      if (c > 0) ahead(c - 1);
+      __syncthreads();
+    }
+  }
 }
 
 // LDS of the gradients: two state tiles of 32 value rows and the fragments of m while products over values run, then keys,
@@ -754,10 +1001,13 @@ extern "C" int grm_hip_delta_scan_bwd(const grm_hip_delta_args* u, const float* 
     constexpr int NK = decltype(nk)::value;
     constexpr bool VEC = decltype(vec)::value;
     {
-      auto kernel = delta_reverse_kernel<E, NK, VEC>;
-      constexpr size_t lds = ReverseLds<E, NK>::bytes;
-      if ((rc = set_lds(reinterpret_cast<const void*>(kernel), lds)) != GRM_HIP_OK) return;
-      kernel<<<dim3(static_cast<uint32_t>(a.f.B) * a.f.H * a.f.PT), dim3(kThreads), lds, hs>>>(a);
+      auto go = [&](auto kernel, int threads, size_t lds) {
+        if ((rc = set_lds(reinterpret_cast<const void*>(kernel), lds)) != GRM_HIP_OK) return;
+        kernel<<<dim3(static_cast<uint32_t>(a.f.B) * a.f.H * a.f.PT), dim3(threads), lds, hs>>>(a);
+      };
+      if constexpr (MirrorLds<E, NK>::fits) go(delta_mirror_kernel<E, NK, VEC>, 2 * kThreads, MirrorLds<E, NK>::bytes);
+      else go(delta_reverse_kernel<E, NK, VEC>, kThreads, ReverseLds<E, NK>::bytes);
+      if (rc != GRM_HIP_OK) return;
       if ((rc = check_launch(what)) != GRM_HIP_OK || a.f.C == 0) return;
     }
     auto kernel = delta_grad_kernel<E, NK, VEC>;

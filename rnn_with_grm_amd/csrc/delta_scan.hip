@@ -476,7 +476,8 @@ struct PairLds {
 // the weights' product with m, and the stores.  A state's columns never meet, so a state wave's chain is its own;
 // accumulators of K S^T, of m and of the state lie as the next product's operand wants them.  Two barriers a chunk:
 // m is there, the next state is there.
-template <class E, int NK, bool VEC>
+// SAVE: the states before every chunk and m are kept for the backward.
+template <class E, int NK, bool VEC, bool SAVE>
 __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaArgs a) {
   using raw = typename ET<E>::raw;
   using L = PairLds<E, NK>;
@@ -519,15 +520,16 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
         *reinterpret_cast<uint4*>(sf + (s * NO + p) * kDFragElems) = __builtin_bit_cast(uint4, sp[s][p]);
     };
     auto keep_state = [&](int c) {
-      if (a.states != nullptr && c < chunks)
-        state_store<NT>(st, a.states + ((static_cast<int64_t>(b) * a.C + c) * a.H + h) * cells, p0, a.P, a.N);
+      // (Behind the last chunk its state is not kept: the stores fall behind the last value row.)
+      if constexpr (SAVE)
+        state_out<VEC>(st, a.states + ((static_cast<int64_t>(b) * a.C + (c < chunks ? c : c - 1)) * a.H + h) * cells, c < chunks ? p0 : a.P, a.P, a.N);
     };
     B8 kr[2][4][NI];  // keys by rows, [step & 1][tile]
     auto row_keys = [&](const uint16_t* from, int s) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) row_parts_t<KT, NI>(from, L::kpart, 16 * t, 32 * s, kr[s & 1][t]);
     };
-    keep_state(0);
+    if (chunks > 0) keep_state(0);
 #pragma unroll
     for (int s = 0; s < S; ++s) publish(s);
     __syncthreads();
@@ -775,7 +777,7 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
             buf_store1<E>(to, tok < left && p + r < a.P ? tok * row + (p + r) * static_cast<int>(sizeof(raw)) : kBufOOB, o[t][r]);
         }
       }
-      if (a.miss != nullptr) {
+      if constexpr (SAVE) {
         const int mrow = a.H * a.P * 4, col = p0 + n;
         const __amdgpu_buffer_rsrc_t ms =
             make_rsrc(a.miss + ((static_cast<int64_t>(b) * a.T + t0) * a.H + h) * a.P, 0x7ffffff0u);
@@ -994,6 +996,10 @@ extern "C" int grm_hip_delta_scan_fwd(const grm_hip_delta_args* u, void* hidden,
     set_error("%s: hidden and memory_out are required, memory_out and states 16-byte aligned", what);
     return GRM_HIP_EINVAL;
   }
+  if ((states == nullptr) != (miss == nullptr)) {
+    set_error("%s: states and miss are given both or neither", what);
+    return GRM_HIP_EINVAL;
+  }
   if (ranges_overlap(u->memory, state_bytes, memory_out, state_bytes)) {
     set_error("%s: memory_out may not overlap memory", what);
     return GRM_HIP_EINVAL;
@@ -1015,17 +1021,21 @@ extern "C" int grm_hip_delta_scan_fwd(const grm_hip_delta_args* u, void* hidden,
     constexpr int NK = decltype(nk)::value;
     const dim3 grid(static_cast<uint32_t>(a.B) * a.H * a.PT);
     if constexpr (PairLds<E, NK>::fits) {
-      auto kernel = delta_pair_kernel<E, NK, decltype(vec)::value>;
-      constexpr size_t lds = PairLds<E, NK>::bytes;
-      if ((rc = set_lds(reinterpret_cast<const void*>(kernel), lds, what)) != GRM_HIP_OK) return;
-      kernel<<<grid, dim3(2 * kWalkThreads), lds, static_cast<hipStream_t>(stream)>>>(a);
+      auto go = [&](auto kernel) {
+        constexpr size_t lds = PairLds<E, NK>::bytes;
+        if ((rc = set_lds(reinterpret_cast<const void*>(kernel), lds, what)) != GRM_HIP_OK) return;
+        kernel<<<grid, dim3(2 * kWalkThreads), lds, static_cast<hipStream_t>(stream)>>>(a);
+        rc = check_launch(what);
+      };
+      if (states != nullptr) go(delta_pair_kernel<E, NK, decltype(vec)::value, true>);
+      else go(delta_pair_kernel<E, NK, decltype(vec)::value, false>);
     } else {
       auto kernel = delta_walk_kernel<E, NK, decltype(vec)::value>;
       constexpr size_t lds = WalkLds<E, NK>::bytes;
       if ((rc = set_lds(reinterpret_cast<const void*>(kernel), lds, what)) != GRM_HIP_OK) return;
       kernel<<<grid, dim3(kWalkThreads), lds, static_cast<hipStream_t>(stream)>>>(a);
+      rc = check_launch(what);
     }
-    rc = check_launch(what);
   });
   return rc;
 }
