@@ -24,19 +24,32 @@ __device__ __forceinline__ void put16(float* y, f32x4 v) {
   for (int r = 0; r < 4; ++r) y[(4 * g + r) * kTriStride + n] = v[r];
 }
 
+// LDS of a chunk's preparation: A, and in one place the keys' fragments and then the inverse.
+template <class E, int NK>
+struct PrepLds {
+  static constexpr int NI = DParts<E>::IN, S = NK / 32, frags = 4 * S * NI;
+  static constexpr size_t a = 0, m = 64 * kTriStride * 4, keys = frags * kDFragElems * 2,
+                          cum = m + (keys > 64 * kTriStride * 4 ? keys : 64 * kTriStride * 4), b = cum + 64 * 8, odd = b + 64 * 4,
+                          bytes = odd + 4 * 4;
+};
+
 // One workgroup a chunk of a head.  Forward: the inverse of I + A b and the weights (W * Q K^T) b, both lower
 // triangular, by rows.  BACK: the inverse of I + b A and W * Q K^T, transposed (the reverse walk multiplies by their transposes).
 // The inverse: forward substitution inside the four 16 x 16 blocks of the diagonal, then two rounds of
 // -T2 (A21 T1) in float32 products.  Substitution does not cancel where keys lie close to each other, as a product of
-// powers of A would.
-template <class E, int NK, bool BACK>
+// powers of A would.  Wave w holds token tile w; the other tiles' keys come as fragments through LDS.
+template <class E, int NK, bool VEC, bool BACK>
 __global__ __launch_bounds__(kPrepThreads) void delta_prep_kernel(DeltaArgs a) {
   using raw = typename ET<E>::raw;
-  constexpr int NI = DParts<E>::IN, PP = BACK ? 3 : DParts<E>::OUT, S = NK / 32;
-  __shared__ double cum_s[64];
-  __shared__ float b_s[64];
-  __shared__ int odd_s[4];
-  __shared__ __attribute__((aligned(16))) float A[64 * kTriStride], M[64 * kTriStride];
+  using L = PrepLds<E, NK>;
+  constexpr int NI = DParts<E>::IN, PP = BACK ? 3 : DParts<E>::OUT, S = NK / 32, ES = static_cast<int>(sizeof(raw));
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  float* A = reinterpret_cast<float*>(lds + L::a);
+  float* M = reinterpret_cast<float*>(lds + L::m);
+  uint16_t* keys = reinterpret_cast<uint16_t*>(lds + L::m);
+  double* cum_s = reinterpret_cast<double*>(lds + L::cum);
+  float* b_s = reinterpret_cast<float*>(lds + L::b);
+  int* odd_s = reinterpret_cast<int*>(lds + L::odd);
   const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, n = lane & 15;
   const uint32_t at = xcd_order(blockIdx.x, gridDim.x);
   const int h = static_cast<int>(at % a.H), c = static_cast<int>(at / a.H % a.C), b = static_cast<int>(at / a.H / a.C);
@@ -44,6 +57,29 @@ __global__ __launch_bounds__(kPrepThreads) void delta_prep_kernel(DeltaArgs a) {
   if (t0 >= len) return;
   const int rows = static_cast<int>(min_i64(kDTokens, len - t0)), gi = h / (a.H / a.G);
 
+  // Keys and queries of this wave's tile, with no load behind a branch.
+  U8<E> ku[S], qu[S];
+  {
+    const __amdgpu_buffer_rsrc_t kr = make_rsrc(static_cast<const raw*>(a.keys) + b * a.kb + t0 * a.kt + static_cast<int64_t>(gi) * a.N, 0x7ffffff0u),
+                                 qr = make_rsrc(static_cast<const raw*>(a.queries) + b * a.qb + t0 * a.qt + static_cast<int64_t>(gi) * a.N, 0x7ffffff0u);
+    const int tok = 16 * w + n, ko = tok * static_cast<int>(a.kt), qo = tok * static_cast<int>(a.qt);
+    auto load = [&](__amdgpu_buffer_rsrc_t r, int off, int s) {
+      const int col = 32 * s + 8 * g;
+      if constexpr (VEC) {
+        return buf_load8<E>(r, tok < rows && col < a.N ? (off + col) * ES : kBufOOB);
+      } else {
+        U8<E> u;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) u.e[e] = buf_load1<E>(r, tok < rows && col + e < a.N ? (off + col + e) * ES : kBufOOB);
+        return u;
+      }
+    };
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      ku[s] = load(kr, ko, s);
+      qu[s] = load(qr, qo, s);
+    }
+  }
   // Scalars, lane = token, in every wave.
   float bt = 0.f, gt = 0.f;
   if (lane < rows) {
@@ -52,30 +88,17 @@ __global__ __launch_bounds__(kPrepThreads) void delta_prep_kernel(DeltaArgs a) {
     if (a.decays != nullptr)
       gt = a.d_f32 ? static_cast<const float*>(a.decays)[j] : ET<E>::to_f(static_cast<const raw*>(a.decays)[j]);
   }
-  const raw* kp = static_cast<const raw*>(a.keys) + b * a.kb + t0 * a.kt + static_cast<int64_t>(gi) * a.N;
-  const raw* qp = static_cast<const raw*>(a.queries) + b * a.qb + t0 * a.qt + static_cast<int64_t>(gi) * a.N;
-  const bool vec = a.vec != 0;
-  auto load = [&](const raw* p, int64_t stride, int tile, int s, int limit) {
-    const int row = 16 * tile + n;
-    return load_u8<E>(p + row * stride, 32 * s + 8 * g, a.N, row < limit, vec);
-  };
-  U8<E> ku[S], qu[S];
-#pragma unroll
-  for (int s = 0; s < S; ++s) {
-    ku[s] = load(kp, a.kt, w, s, rows);
-    qu[s] = load(qp, a.qt, w, s, rows);
-  }
   // The first token whose key, strength or decay is no number (the walk takes it from there).
   const float inf = __builtin_inff();
   int odd = 64;
   if (!BACK) {
-    bool bad = false;
+    float zero = 0.f;  // (a product with zero is zero or NaN)
 #pragma unroll
     for (int s = 0; s < S; ++s) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) bad |= !(fabsf(ET<E>::to_f(ku[s].e[e])) < inf);
+      for (int e = 0; e < 8; ++e) zero = fmaf(ET<E>::to_f(ku[s].e[e]), 0.f, zero);
     }
-    const uint64_t mask = __ballot(bad);
+    const uint64_t mask = __ballot(zero != 0.f);
     const uint32_t m16 = static_cast<uint32_t>((mask | mask >> 16 | mask >> 32 | mask >> 48) & 0xffff);
     const uint64_t scal = __ballot(!(fabsf(bt) < inf) || !(gt < inf));
     if (m16 != 0) odd = 16 * w + __builtin_ctz(m16);
@@ -103,77 +126,108 @@ __global__ __launch_bounds__(kPrepThreads) void delta_prep_kernel(DeltaArgs a) {
     sc[128 + lane] = bt;
     if (lane == 0) reinterpret_cast<int*>(sc)[192] = odd;
   }
-  __syncthreads();
-
-  const int limit = odd < rows ? odd : rows;
   B8 ki[S][NI], qi[S][NI];
 #pragma unroll
   for (int s = 0; s < S; ++s) {
-    if (16 * w + n >= limit) zero_u8<E>(ku[s]);
+    if (!BACK && 16 * w + n >= odd) zero_u8<E>(ku[s]);
     input_parts<E, NI>(ku[s], ki[s]);
     input_parts<E, NI>(qu[s], qi[s]);
+#pragma unroll
+    for (int p = 0; p < NI; ++p)
+      *reinterpret_cast<uint4*>(keys + ((w * S + s) * NI + p) * kDFragElems + 8 * lane) = __builtin_bit_cast(uint4, ki[s][p]);
   }
-  const double ci = cum_s[16 * w + n];
-  const float bi = b_s[16 * w + n];
-  for (int tj = 0; tj <= w; ++tj) {
+  __syncthreads();
+
+  const int i = 16 * w + n;
+  const double ci = cum_s[i];
+  const float bi = b_s[i];
+  float y[4][4];
+#pragma unroll
+  for (int tj = 0; tj < 4; ++tj) {
     f32x4 kk = {0.f, 0.f, 0.f, 0.f}, qk = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[tj][r] = 0.f;
+    if (tj > w) continue;
 #pragma unroll
     for (int s = 0; s < S; ++s) {
       B8 kj[NI];
-      input_parts<E, NI>(load(kp, a.kt, tj, s, limit), kj);
+#pragma unroll
+      for (int p = 0; p < NI; ++p)
+        kj[p] = __builtin_bit_cast(B8, *reinterpret_cast<const uint4*>(keys + ((tj * S + s) * NI + p) * kDFragElems + 8 * lane));
       kk = mma_parts<3>(kj, ki[s], kk);                  // column i = 16 w + n, rows j = 16 tj + 4 g + r
       if (BACK) qk = mma_parts<3>(qi[s], kj, qk);        // column j = 16 tj + n, rows i = 16 w + 4 g + r
       else qk = mma_parts<3>(kj, qi[s], qk);
     }
-    float x[4], y[4];
+    float x[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      const int i = 16 * w + n, j = 16 * tj + 4 * g + r;
-      const float wt = j <= i ? exp2_d(ci - cum_s[j]) : 0.f;
-      x[r] = j < i ? wt * kk[r] * (BACK ? bi : b_s[j]) : 0.f;
+      const int j = 16 * tj + 4 * g + r;
+      const float bj = b_s[j], wt = j <= i ? exp2_f(static_cast<float>(ci - cum_s[j])) : 0.f;
+      x[r] = j < i ? wt * kk[r] * (BACK ? bi : bj) : 0.f;
       if (BACK) {
         const int i2 = 16 * w + 4 * g + r, j2 = 16 * tj + n;
-        y[r] = j2 <= i2 ? exp2_d(cum_s[i2] - cum_s[j2]) * qk[r] : 0.f;
+        y[tj][r] = j2 <= i2 ? exp2_f(static_cast<float>(cum_s[i2] - cum_s[j2])) * qk[r] : 0.f;
       } else {
-        y[r] = j <= i ? wt * qk[r] * b_s[j] : 0.f;
+        y[tj][r] = j <= i ? wt * qk[r] * bj : 0.f;
       }
     }
-    *reinterpret_cast<float4*>(&A[(16 * w + n) * kTriStride + 16 * tj + 4 * g]) = make_float4(x[0], x[1], x[2], x[3]);
-    // Half a fragment: slots 0-3 are the first tile of the reduction's step, 4-7 the second.
-    const int frag = BACK ? upper_frag(tj, w >> 1) : lower_frag(w, tj >> 1), half = (BACK ? w : tj) & 1;
-    float rest[4] = {y[0], y[1], y[2], y[3]};
+    *reinterpret_cast<float4*>(&A[i * kTriStride + 16 * tj + 4 * g]) = make_float4(x[0], x[1], x[2], x[3]);
+  }
+  // The weights: forward a step of a fragment is two tiles of this wave; backward its halves come from two waves.
+  if constexpr (!BACK) {
 #pragma unroll
-    for (int p = 0; p < PP; ++p) {
-      const uint2 v = make_uint2(pack2<BF16>(rest[0], rest[1]), pack2<BF16>(rest[2], rest[3]));
-      uint16_t* to = pf + (frag * PP + p) * kDFragElems + 8 * lane;
-      *reinterpret_cast<uint2*>(to + 4 * half) = v;
-      // The half of a step that lies beyond the diagonal.
-      if (BACK ? tj == w && half == 1 && (tj & 1) == 1 : tj == w && half == 0)
-        *reinterpret_cast<uint2*>(to + 4 * (1 - half)) = make_uint2(0u, 0u);
-      const uint16_t q[4] = {static_cast<uint16_t>(v.x), static_cast<uint16_t>(v.x >> 16), static_cast<uint16_t>(v.y),
-                             static_cast<uint16_t>(v.y >> 16)};
+    for (int s = 0; s < 2; ++s) {
+      if (s > w / 2) continue;
+      const float v[8] = {y[2 * s][0], y[2 * s][1], y[2 * s][2], y[2 * s][3], y[2 * s + 1][0], y[2 * s + 1][1], y[2 * s + 1][2], y[2 * s + 1][3]};
+      B8 f[PP];
+      split8<PP>(v, f);
+      const int frag = w < 2 ? w : 2 * w - 2 + s;  // lower_frag(w, s)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) rest[r] = part_rest<BF16>(rest[r], q[r]);
+      for (int p = 0; p < PP; ++p)
+        *reinterpret_cast<uint4*>(pf + (frag * PP + p) * kDFragElems + 8 * lane) = __builtin_bit_cast(uint4, f[p]);
+    }
+  } else {
+#pragma unroll
+    for (int tj = 0; tj < 4; ++tj) {
+      if (tj > w) continue;
+      const int frag = tj < 2 ? 2 * tj + (w >> 1) : tj + 2, half = w & 1;  // upper_frag(tj, w / 2)
+      float v[8] = {y[tj][0], y[tj][1], y[tj][2], y[tj][3], 0.f, 0.f, 0.f, 0.f};
+      B8 f[PP];
+      split8<PP>(v, f);
+#pragma unroll
+      for (int p = 0; p < PP; ++p) {
+        const uint4 u = __builtin_bit_cast(uint4, f[p]);
+        uint16_t* to = pf + (frag * PP + p) * kDFragElems + 8 * lane;
+        *reinterpret_cast<uint2*>(to + 4 * half) = make_uint2(u.x, u.y);
+        if (tj == w && half == 1) *reinterpret_cast<uint2*>(to) = make_uint2(0u, 0u);  // (beyond the diagonal)
+      }
     }
   }
   __syncthreads();
 
-  // Diagonal blocks, column n of block w in the registers of lane n (four times over).
+  // Diagonal blocks, column n of block w in the registers of lane n (four times over); A's rows in whole reads.
   auto tile = [](float* m, int i, int j) { return m + 16 * i * kTriStride + 16 * j; };
   {
     const float* d = tile(A, w, w);
     float x[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = i == n ? 1.f : 0.f;
+    for (int r = 0; r < 16; ++r) {
+      float v = r == n ? 1.f : 0.f, u = 0.f;
 #pragma unroll
-    for (int j = 0; j < 15; ++j) {
+      for (int q = 0; q < 4; ++q) {
+        if (4 * q >= r) continue;
+        const float4 e = *reinterpret_cast<const float4*>(d + r * kTriStride + 4 * q);
+        const float ee[4] = {e.x, e.y, e.z, e.w};
 #pragma unroll
-      for (int i = j + 1; i < 16; ++i) x[i] = fmaf(-d[i * kTriStride + j], x[j], x[i]);
+        for (int k = 0; k < 4; ++k)
+          if (4 * q + k < r) (k & 1 ? u : v) = fmaf(-ee[k], x[4 * q + k], k & 1 ? u : v);
+      }
+      x[r] = v + u;
     }
     float* m = tile(M, w, w);
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      if ((i >> 2) == g) m[i * kTriStride + n] = x[i];
+    for (int r = 0; r < 16; ++r)
+      if ((r >> 2) == g) m[r * kTriStride + n] = x[r];
   }
   __syncthreads();
   // The products wait in the tiles of A above the diagonal.
@@ -183,29 +237,30 @@ __global__ __launch_bounds__(kPrepThreads) void delta_prep_kernel(DeltaArgs a) {
   if (w < 2) put16(tile(M, 2 * w + 1, 2 * w), -mm16(tile(M, 2 * w + 1, 2 * w + 1), tile(A, 2 * w, 2 * w + 1), zero));
   __syncthreads();
   {
-    const int i = 2 + (w >> 1), j = w & 1;
-    f32x4 y = mm16(tile(A, i, 1), tile(M, 1, j), zero);
-    if (j == 0) y = mm16(tile(A, i, 0), tile(M, 0, 0), y);
-    put16(tile(A, j, i), y);
+    const int ti = 2 + (w >> 1), tj = w & 1;
+    f32x4 v = mm16(tile(A, ti, 1), tile(M, 1, tj), zero);
+    if (tj == 0) v = mm16(tile(A, ti, 0), tile(M, 0, 0), v);
+    put16(tile(A, tj, ti), v);
     __syncthreads();
-    f32x4 z = mm16(tile(M, i, 2), tile(A, j, 2), zero);
-    if (i == 3) z = mm16(tile(M, 3, 3), tile(A, j, 3), z);
-    put16(tile(M, i, j), -z);
+    f32x4 z = mm16(tile(M, ti, 2), tile(A, tj, 2), zero);
+    if (ti == 3) z = mm16(tile(M, 3, 3), tile(A, tj, 3), z);
+    put16(tile(M, ti, tj), -z);
   }
   __syncthreads();
   // Into fragments: forward rows i with slots over j, backward rows j with slots over i.
-  const int f0 = BACK ? (w < 2 ? 0 : 1) : 0, f1 = BACK ? 1 : (w < 2 ? 0 : 1);
-  for (int s = f0; s <= f1; ++s) {
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    if (BACK ? s < w / 2 : s > w / 2) continue;
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const int row = 16 * w + n, k = 32 * s + (e < 4 ? 4 * g + e : 16 + 4 * g + e - 4);
-      if (BACK) v[e] = k >= row ? M[k * kTriStride + row] : 0.f;
-      else v[e] = k <= row ? M[row * kTriStride + k] : 0.f;
+      const int k = 32 * s + (e < 4 ? 4 * g + e : 16 + 4 * g + e - 4);
+      const float u = BACK ? M[k * kTriStride + i] : M[i * kTriStride + k];
+      v[e] = (BACK ? k >= i : k <= i) ? u : 0.f;
     }
     B8 f[3];
     split8<3>(v, f);
-    const int frag = BACK ? upper_frag(w, s) : lower_frag(w, s);
+    const int frag = BACK ? (w < 2 ? 2 * w + s : w + 2) : (w < 2 ? w : 2 * w - 2 + s);
 #pragma unroll
     for (int p = 0; p < 3; ++p)
       *reinterpret_cast<uint4*>(tf + (frag * 3 + p) * kDFragElems + 8 * lane) = __builtin_bit_cast(uint4, f[p]);
@@ -966,13 +1021,18 @@ DeltaArgs delta_args(const grm_hip_delta_args* u) {
 
 int launch_delta_prep(const DeltaArgs& a, int dtype, bool back, hipStream_t stream, const char* what) {
   int rc = GRM_HIP_OK;
-  delta_with_form(dtype, a.N, true, [&](auto e, auto nk, auto) {
+  delta_with_form(dtype, a.N, a.vec != 0, [&](auto e, auto nk, auto vec) {
     using E = decltype(e);
     constexpr int NK = decltype(nk)::value;
-    const dim3 grid(static_cast<uint32_t>(a.B) * a.H * a.C);
-    if (back) delta_prep_kernel<E, NK, true><<<grid, dim3(kPrepThreads), 0, stream>>>(a);
-    else delta_prep_kernel<E, NK, false><<<grid, dim3(kPrepThreads), 0, stream>>>(a);
-    rc = check_launch(what);
+    constexpr bool VEC = decltype(vec)::value;
+    auto go = [&](auto kernel) {
+      constexpr size_t lds = PrepLds<E, NK>::bytes;
+      if ((rc = set_lds(reinterpret_cast<const void*>(kernel), lds, what)) != GRM_HIP_OK) return;
+      kernel<<<dim3(static_cast<uint32_t>(a.B) * a.H * a.C), dim3(kPrepThreads), lds, stream>>>(a);
+      rc = check_launch(what);
+    };
+    if (back) go(delta_prep_kernel<E, NK, VEC, true>);
+    else go(delta_prep_kernel<E, NK, VEC, false>);
   });
   return rc;
 }
