@@ -39,7 +39,7 @@ struct PrepLds {
 // -T2 (A21 T1) in float32 products.  Substitution does not cancel where keys lie close to each other, as a product of
 // powers of A would.  Wave w holds token tile w; the other tiles' keys come as fragments through LDS.
 template <class E, int NK, bool VEC, bool BACK>
-__global__ __launch_bounds__(kPrepThreads) void delta_prep_kernel(DeltaArgs a) {
+__global__ __launch_bounds__(kPrepThreads, 4) void delta_prep_kernel(DeltaArgs a) {
   using raw = typename ET<E>::raw;
   using L = PrepLds<E, NK>;
   constexpr int NI = DParts<E>::IN, PP = BACK ? 3 : DParts<E>::OUT, S = NK / 32, ES = static_cast<int>(sizeof(raw));
