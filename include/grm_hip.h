@@ -620,7 +620,8 @@ typedef struct grm_hip_delta_args {
  *             backward reads (rows behind a length are left as they were).  Given with states or not at all.
  * workspace:  grm_hip_delta_scan_workspace() bytes, 16-byte aligned.
  */
-int64_t grm_hip_delta_scan_workspace(int64_t batch, int64_t seq_len, int64_t heads, int dtype);
+int64_t grm_hip_delta_scan_workspace(int64_t batch, int64_t seq_len, int64_t heads, int64_t value_dim, int64_t key_dim,
+                                     int dtype);
 int grm_hip_delta_scan_fwd(const grm_hip_delta_args* args, void* hidden, float* memory_out, float* states, float* miss,
                            void* workspace, int64_t workspace_bytes, void* stream);
 

@@ -103,7 +103,7 @@ class DeltaArgs(ctypes.Structure):
 
 
 SIGNATURES.update({
-    "grm_hip_delta_scan_workspace": (_I, [_I, _I, _I, _C]),
+    "grm_hip_delta_scan_workspace": (_I, [_I, _I, _I, _I, _I, _C]),
     "grm_hip_delta_scan_fwd": (_C, [ctypes.POINTER(DeltaArgs), _P, _P, _P, _P, _P, _I, _P]),
     "grm_hip_delta_scan_bwd_workspace": (_I, [_I, _I, _I, _I, _I, _I]),
     "grm_hip_delta_scan_bwd": (_C, [ctypes.POINTER(DeltaArgs)] + [_P] * 11 + [_I, _P]),

@@ -43,9 +43,12 @@ struct DeltaArgs {
   float* states;                        // [B, C, H, P, N] or null: the state before every chunk
   float* miss;                          // [B, T, H, P] or null: m
   char* work;                           // what delta_prep_kernel leaves, [B, H, C]
+  float* part_state;                    // [parts - 1, B, H, P, N]: what a part leaves of a zero state, then the state behind it
+  float* part_map;                      // [parts - 1, B, H, N, N]: what a part makes of the identity, without values
   int64_t kb, kt, vb, vt, qb, qt, sb, st, db, dt;
   int64_t T;
   int B, H, P, G, N, C, PT;
+  int parts, part_chunks, NT;           // time parts, their chunks, tiles of 64 rows of a part's map
   int s_f32, d_f32, vec;
 };
 

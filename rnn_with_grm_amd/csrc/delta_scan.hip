@@ -532,7 +532,11 @@ struct PairLds {
 // accumulators of K S^T, of m and of the state lie as the next product's operand wants them.  Two barriers a chunk:
 // m is there, the next state is there.
 // SAVE: the states before every chunk and m are kept for the backward.
-template <class E, int NK, bool VEC, bool SAVE>
+// Sequences in time parts: a first launch (LOCAL) walks all parts but the last side by side and without outputs.  Rows of a
+// state never meet, and without values each passes through a part as a row of a matrix product; so beside the value rows of a
+// part, from a zero state, go the N rows of the identity without values, whose end is the part's map.  delta_join_kernel makes
+// the parts' first states of both, and the second launch walks every part from its own.
+template <class E, int NK, bool VEC, bool SAVE, bool LOCAL>
 __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaArgs a) {
   using raw = typename ET<E>::raw;
   using L = PairLds<E, NK>;
@@ -549,11 +553,16 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
   const int lane = lane_id(), g = lane >> 4, n = lane & 15;
   const uint32_t at = xcd_order(blockIdx.x, gridDim.x);
-  const int pt = static_cast<int>(at % a.PT), h = static_cast<int>(at / a.PT % a.H), b = static_cast<int>(at / a.PT / a.H);
+  const int tiles = LOCAL ? a.PT + a.NT : a.PT, parts = LOCAL ? a.parts - 1 : a.parts;
+  const int pt = static_cast<int>(at % tiles), part = static_cast<int>(at / tiles % parts);
+  const int h = static_cast<int>(at / tiles / parts % a.H), b = static_cast<int>(at / tiles / parts / a.H);
+  const bool map = LOCAL && pt >= a.PT;  // rows of the identity
+  if (map && part == 0) return;          // (the first part starts from the sequence's own state)
   const int64_t len = delta_length(a, b);
-  const int col0 = pt * kDCols, p0 = col0 + 16 * w, gi = h / (a.H / a.G);
-  const int chunks = static_cast<int>((len + kDTokens - 1) / kDTokens);
-  const int64_t head = static_cast<int64_t>(b) * a.H + h, cells = static_cast<int64_t>(a.P) * a.N;
+  const int col0 = (map ? pt - a.PT : pt) * kDCols, p0 = col0 + 16 * w, gi = h / (a.H / a.G), prows = map ? a.N : a.P;
+  const int first = part * a.part_chunks, have = static_cast<int>((len + kDTokens - 1) / kDTokens);
+  const int chunks = have < first + a.part_chunks ? (have > first ? have : first) : first + a.part_chunks;  // this part's end
+  const int64_t head = static_cast<int64_t>(b) * a.H + h, cells = static_cast<int64_t>(a.P) * a.N, all = static_cast<int64_t>(a.B) * a.H;
   const char* work = a.work + head * a.C * delta_chunk_bytes(NO);
   uint16_t* sf = reinterpret_cast<uint16_t*>(lds + L::s) + w * L::state + 8 * lane;
   f32x4* mf = reinterpret_cast<f32x4*>(lds + L::m) + w * 256 + lane;
@@ -564,12 +573,23 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
     f32x4 st[NT];
 #pragma unroll
     for (int i = 0; i < NT; ++i) st[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (a.memory != nullptr) state_add<NT>(st, a.memory + head * cells, p0, a.P, a.N, 1.f);
+    if (map) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st[i][r] = p0 + n == 16 * i + 4 * g + r && p0 + n < a.N ? 1.f : 0.f;
+      }
+    } else if (part > 0 && !LOCAL) {
+      state_add<NT>(st, a.part_state + ((part - 1) * all + head) * cells, p0, a.P, a.N, 1.f);
+    } else if (part == 0 && a.memory != nullptr) {
+      state_add<NT>(st, a.memory + head * cells, p0, a.P, a.N, 1.f);
+    }
     // The triangular matrix's fragments, loaded a chunk ahead as soon as the last ones are done with.
     B8 tf[kDFrags][3], sp[S][3];
-    if (chunks > 0) stored_triangle<3>(reinterpret_cast<const uint16_t*>(work), tf, lane);
+    if (chunks > first) stored_triangle<3>(reinterpret_cast<const uint16_t*>(work + first * delta_chunk_bytes(NO)), tf, lane);
     auto publish = [&](int s) {
       split2<3>(st[2 * s], st[2 * s + 1], sp[s]);
+      if constexpr (LOCAL) return;
 #pragma unroll
       for (int p = 0; p < NO; ++p)
         *reinterpret_cast<uint4*>(sf + (s * NO + p) * kDFragElems) = __builtin_bit_cast(uint4, sp[s][p]);
@@ -584,12 +604,12 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
 #pragma unroll
       for (int t = 0; t < 4; ++t) row_parts_t<KT, NI>(from, L::kpart, 16 * t, 32 * s, kr[s & 1][t]);
     };
-    if (chunks > 0) keep_state(0);
+    if (chunks > first) keep_state(first);
 #pragma unroll
     for (int s = 0; s < S; ++s) publish(s);
     __syncthreads();
-    if (chunks > 0) row_keys(kt, 0);
-    for (int c = 0; c < chunks; ++c) {
+    if (chunks > first) row_keys(kt + (first & 1) * NI * L::kpart, 0);
+    for (int c = first; c < chunks; ++c) {
       const uint16_t* kc = kt + (c & 1) * NI * L::kpart;
       const float* scc = sc + (c & 1) * L::SCAL;
       const int next = c + 1 < chunks ? c + 1 : c;
@@ -655,8 +675,10 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
         for (int t = 0; t < 4; ++t) m[t] = f32x4{0.f, 0.f, 0.f, 0.f};
         mma_triangle<3, true, true>(tf, rp, m);
       }
+      if constexpr (!LOCAL) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) mf[64 * t] = m[t];
+        for (int t = 0; t < 4; ++t) mf[64 * t] = m[t];
+      }
       if (g == 0) cuts[16 * w + n] = cut;
       B8 kf[2][2][2][NI];  // [pair & 1][step][tile of the pair]
       auto pair_keys = [&](int j) {
@@ -713,18 +735,20 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
       row_keys(kt + ((c + 1) & 1) * NI * L::kpart, 0);  // (there since the chunk's first barrier)
       __syncthreads();
     }
-    state_store<NT>(st, a.memory_out + head * cells, p0, a.P, a.N);
+    if (map) state_store<NT>(st, a.part_map + (part * all + head) * a.N * a.N, p0, a.N, a.N);
+    else if (LOCAL) state_store<NT>(st, a.part_state + (part * all + head) * cells, p0, a.P, a.N);
+    else if (part == a.parts - 1) state_store<NT>(st, a.memory_out + head * cells, p0, a.P, a.N);
   } else {
     const int tid = static_cast<int>(threadIdx.x) - kWalkThreads;
     const raw* kp = static_cast<const raw*>(a.keys) + b * a.kb + static_cast<int64_t>(gi) * a.N;
     const raw* qp = static_cast<const raw*>(a.queries) + b * a.qb + static_cast<int64_t>(gi) * a.N;
-    const raw* vp = static_cast<const raw*>(a.values) + b * a.vb + static_cast<int64_t>(h) * a.P + col0;
+    const raw* vp = static_cast<const raw*>(a.values) + b * a.vb + static_cast<int64_t>(h) * a.P + (map ? 0 : col0);
     TileLoad<E, KT, BF16, VEC, kDTokens, NK, kWalkThreads> kl;
     TileLoad<E, QT, BF16, VEC, kDTokens, NK, kWalkThreads> ql;
     TileLoad<E, VT, E, VEC, kDTokens, kDCols, kWalkThreads> vl;
     kl.init(a.kt, a.N, tid);
     ql.init(a.qt, a.N, tid);
-    vl.init(a.vt, a.P - col0 < kDCols ? a.P - col0 : kDCols, tid);
+    vl.init(a.vt, prows - col0 < kDCols ? prows - col0 : kDCols, tid);
     float sreg = 0.f, warm = 0.f;
     int oreg = 64;
     B8 pf[kDFrags][NO];
@@ -735,11 +759,11 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
       sreg = s[tid & 127];
       oreg = reinterpret_cast<const int*>(s)[192];
       kl.load(kp + t0 * a.kt, len - t0, tid);
-      ql.load(qp + t0 * a.qt, len - t0, tid);
-      vl.load(vp + t0 * a.vt, len - t0, tid);
+      if constexpr (!LOCAL) ql.load(qp + t0 * a.qt, len - t0, tid);
+      vl.load(vp + t0 * a.vt, map ? 0 : len - t0, tid);  // (a map's rows have no values)
     };
     auto place_qv = [&](int c) {
-      store_parts<QT, NI, E>(ql, qt + (c & (QV - 1)) * L::qstage, L::qpart, kDTokens, tid);
+      if constexpr (!LOCAL) store_parts<QT, NI, E>(ql, qt + (c & (QV - 1)) * L::qstage, L::qpart, kDTokens, tid);
       vl.store(vt + (c & (QV - 1)) * L::vstage, tid);
     };
     auto place_k = [&](int c) {
@@ -752,23 +776,24 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
     auto warm_up = [&](int want) {
       const int c = want < chunks ? want : chunks - 1;
       asm volatile("" ::"v"(warm));
-      constexpr int lines = static_cast<int>(delta_chunk_bytes(NO) / 128);
+      constexpr int lines = static_cast<int>((LOCAL ? 3 * kDFrags * kDFragElems * 2 : delta_chunk_bytes(NO)) / 128);
       for (int i = tid; i < lines; i += kWalkThreads) warm = *reinterpret_cast<const float*>(work + c * delta_chunk_bytes(NO) + 128 * i);
     };
     auto weights = [&](int want) {
+      if constexpr (LOCAL) return;
       const int c = want < chunks ? want : chunks - 1;
       stored_triangle<NO>(reinterpret_cast<const uint16_t*>(work + c * delta_chunk_bytes(NO)) + 3 * kDFrags * kDFragElems, pf, lane);
     };
-    if (chunks > 0) {
-      fetch(0);
-      place_k(0);
-      place_qv(0);
-      weights(0);
-      fetch(1);
+    if (chunks > first) {
+      fetch(first);
+      place_k(first);
+      place_qv(first);
+      weights(first);
+      fetch(first + 1);
     }
     __syncthreads();
     const int p = p0 + 4 * g, row = a.H * a.P * static_cast<int>(sizeof(raw));
-    for (int c = 0; c < chunks; ++c) {
+    for (int c = first; c < chunks; ++c) {
       const int64_t t0 = static_cast<int64_t>(c) * kDTokens;
       place_k(c + 1);
       if constexpr (QV == 2) {
@@ -776,6 +801,15 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
         fetch(c + 2);
       }
       warm_up(c + 3);
+      if constexpr (LOCAL) {
+        __syncthreads();
+        if constexpr (QV == 1) {
+          place_qv(c + 1);
+          fetch(c + 2);
+        }
+        __syncthreads();
+        continue;
+      }
       const uint16_t* qc = qt + (c & (QV - 1)) * L::qstage;
       // S Q^T: a value a row, a token a column, as rows are stored.
       f32x4 o[4];
@@ -847,10 +881,86 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
       }
       __syncthreads();
     }
-    // Rows behind the last chunk.
-    for (int64_t t = static_cast<int64_t>(chunks) * kDTokens + tid / 16; t < a.T; t += kWalkThreads / 16) {
+    // Rows of this part behind the last chunk.
+    if constexpr (LOCAL) return;
+    const int64_t end = min_i64(a.T, (static_cast<int64_t>(first) + a.part_chunks) * kDTokens);
+    for (int64_t t = static_cast<int64_t>(chunks) * kDTokens + tid / 16; t < end; t += kWalkThreads / 16) {
       raw* to = static_cast<raw*>(a.hidden) + ((b * a.T + t) * a.H + h) * a.P + col0;
       for (int i = tid % 16; i < kDCols && col0 + i < a.P; i += 16) to[i] = 0;
+    }
+  }
+}
+
+// The state before every part but the first: M_{p+1} = M_p F_p + D_p with the parts' maps F and what they leave of a zero
+// state D (of the first, of the sequence's own state: M_1).  A workgroup takes 16 value rows through all parts; each wave
+// holds 32 of the keys, and they hand each other the state's fragments.  The map hangs on no state and is loaded a part
+// ahead (7 parts of 16 heads of 128 x 128: 155 us with a wave for all keys and no loads ahead).
+template <int NK>
+__global__ __launch_bounds__(2 * NK) void delta_join_kernel(DeltaArgs a) {
+  constexpr int S = NK / 32;
+  __shared__ __attribute__((aligned(16))) uint16_t frags[S * 3 * kDFragElems];
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = lane_id(), g = lane >> 4, n = lane & 15;
+  const int tiles = (a.P + 15) / 16, p0 = static_cast<int>(blockIdx.x % tiles) * 16;
+  const int64_t head = blockIdx.x / tiles, cells = static_cast<int64_t>(a.P) * a.N, all = static_cast<int64_t>(a.B) * a.H;
+  float map[2][S][8];
+  auto fetch = [&](int want) {
+    const int p = want < a.parts - 1 ? want : a.parts - 2;
+    const __amdgpu_buffer_rsrc_t r = make_rsrc(a.part_map + (p * all + head) * a.N * a.N, static_cast<uint32_t>(a.N * a.N * 4));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int from = 32 * s + (e < 4 ? 4 * g + e : 12 + 4 * g + e), to = 32 * w + 16 * i + n;
+          map[i][s][e] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, from < a.N && to < a.N ? (from * a.N + to) * 4 : kBufOOB, 0, 0));
+        }
+      }
+    }
+  };
+  // This wave's tiles of a state: value row p0 + n, keys 32 w + 16 i + 4 g + r.
+  auto where = [&](int i, int r) {
+    const int key = 32 * w + 16 * i + 4 * g + r;
+    return p0 + n < a.P && key < a.N ? ((p0 + n) * a.N + key) * 4 : kBufOOB;
+  };
+  auto rsrc = [&](int p) { return make_rsrc(a.part_state + (p * all + head) * cells, static_cast<uint32_t>(cells * 4)); };
+  f32x4 st[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) st[i][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc(0), where(i, r), 0, 0));
+  }
+  fetch(1);
+  for (int p = 1; p < a.parts - 1; ++p) {
+    B8 sp[3], f[2][S][3];
+    split2<3>(st[0], st[1], sp);
+#pragma unroll
+    for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(frags + (w * 3 + q) * kDFragElems + 8 * lane) = __builtin_bit_cast(uint4, sp[q]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) st[i][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc(p), where(i, r), 0, 0));
+#pragma unroll
+      for (int s = 0; s < S; ++s) split8<3>(map[i][s], f[i][s]);
+    }
+    fetch(p + 1);
+    __syncthreads();
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      B8 m[3], fs[2][3];
+#pragma unroll
+      for (int q = 0; q < 3; ++q) {
+        m[q] = __builtin_bit_cast(B8, *reinterpret_cast<const uint4*>(frags + (s * 3 + q) * kDFragElems + 8 * lane));
+        fs[0][q] = f[0][s][q];
+        fs[1][q] = f[1][s][q];
+      }
+      mma_many<3, true>(fs, m, st);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(st[i][r]), rsrc(p), where(i, r), 0, 0);
     }
   }
 }
@@ -944,6 +1054,37 @@ int set_lds(const void* kernel, size_t bytes, const char* what) {
 }
 
 int out_parts(int dtype) { return dtype == GRM_HIP_F32 ? 3 : 2; }
+int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
+
+// Time parts of a sequence.  256 CUs hold a workgroup each; a part costs its chunks once more, for the value rows and for
+// the N rows of its map, so parts are taken where they shorten the longest line of chunks behind each other (in units of
+// a chunk; a launch and a join count as a few).  32768 bf16 tokens x 16 heads of 128 x 128: 1900 us in one part.
+int time_parts(int64_t seqs, int64_t P, int64_t N, int64_t C, int dtype, int64_t* part_chunks) {
+  *part_chunks = C;
+  if ((dtype != GRM_HIP_BF16 && N > 64) || seqs > 4096) return 1;  // (delta_walk_kernel takes whole sequences)
+  const int64_t PT = (P + kDCols - 1) / kDCols, NT = (N + kDCols - 1) / kDCols;
+  auto rounds = [](int64_t wgs) { return (wgs + 255) / 256; };
+  int64_t best = C * rounds(seqs * PT), parts = 1;
+  for (int64_t r = 2; r <= 64 && r <= C / 4; ++r) {
+    const int64_t per = (C + r - 1) / r, n = (C + per - 1) / per;
+    const int64_t cost = per * (rounds(seqs * PT * n) + rounds(seqs * (PT + NT) * (n - 1))) + 2 * n + 6;
+    if (cost < best) best = cost, parts = n, *part_chunks = per;
+  }
+  return static_cast<int>(parts);
+}
+
+struct Work {
+  int64_t states, maps, bytes;
+};
+Work work_of(int64_t B, int64_t T, int64_t H, int64_t P, int64_t N, int dtype, int* parts, int64_t* part_chunks) {
+  const int64_t C = (T + kDTokens - 1) / kDTokens;
+  *parts = time_parts(B * H, P, N, C, dtype, part_chunks);
+  Work w{};
+  w.states = up16(B * H * C * delta_chunk_bytes(out_parts(dtype)));
+  w.maps = w.states + up16((*parts - 1) * B * H * P * N * 4);
+  w.bytes = w.maps + (*parts - 1) * B * H * N * N * 4;
+  return w;
+}
 
 }  // namespace
 
@@ -1010,6 +1151,9 @@ DeltaArgs delta_args(const grm_hip_delta_args* u) {
   a.G = static_cast<int>(u->groups); a.N = static_cast<int>(u->key_dim);
   a.C = static_cast<int>((u->seq_len + kDTokens - 1) / kDTokens);
   a.PT = static_cast<int>((u->value_dim + kDCols - 1) / kDCols);
+  a.NT = static_cast<int>((u->key_dim + kDCols - 1) / kDCols);
+  a.parts = 1;
+  a.part_chunks = a.C;
   a.s_f32 = u->strengths_dtype == GRM_HIP_F32;
   a.d_f32 = u->decays_dtype == GRM_HIP_F32;
   // Whole 16-byte loads where every row of 8-element units allows them.
@@ -1041,9 +1185,12 @@ int launch_delta_prep(const DeltaArgs& a, int dtype, bool back, hipStream_t stre
 
 using namespace grmhip;
 
-extern "C" int64_t grm_hip_delta_scan_workspace(int64_t batch, int64_t seq_len, int64_t heads, int dtype) {
-  if (batch <= 0 || seq_len <= 0 || heads <= 0 || dtype < 0 || dtype > 2) return 0;
-  return batch * heads * ((seq_len + kDTokens - 1) / kDTokens) * delta_chunk_bytes(out_parts(dtype));
+extern "C" int64_t grm_hip_delta_scan_workspace(int64_t batch, int64_t seq_len, int64_t heads, int64_t value_dim, int64_t key_dim,
+                                                int dtype) {
+  if (batch <= 0 || seq_len <= 0 || heads <= 0 || value_dim <= 0 || key_dim <= 0 || dtype < 0 || dtype > 2) return 0;
+  int parts = 1;
+  int64_t part_chunks = 0;
+  return work_of(batch, seq_len, heads, value_dim, key_dim, dtype, &parts, &part_chunks).bytes;
 }
 
 extern "C" int grm_hip_delta_scan_fwd(const grm_hip_delta_args* u, void* hidden, float* memory_out, float* states,
@@ -1068,8 +1215,12 @@ extern "C" int grm_hip_delta_scan_fwd(const grm_hip_delta_args* u, void* hidden,
   a.hidden = hidden; a.memory_out = memory_out; a.states = states; a.miss = miss;
   a.work = static_cast<char*>(workspace);
   if (a.C > 0) {
-    if (workspace == nullptr || !aligned(workspace) ||
-        workspace_bytes < grm_hip_delta_scan_workspace(u->batch, u->seq_len, u->heads, u->dtype)) {
+    int64_t part_chunks = 0;
+    const Work wk = work_of(u->batch, u->seq_len, u->heads, u->value_dim, u->key_dim, u->dtype, &a.parts, &part_chunks);
+    a.part_chunks = static_cast<int>(part_chunks);
+    a.part_state = reinterpret_cast<float*>(a.work + wk.states);
+    a.part_map = reinterpret_cast<float*>(a.work + wk.maps);
+    if (workspace == nullptr || !aligned(workspace) || workspace_bytes < wk.bytes) {
       set_error("%s: workspace missing, misaligned or too small", what);
       return GRM_HIP_EINVAL;
     }
@@ -1079,21 +1230,30 @@ extern "C" int grm_hip_delta_scan_fwd(const grm_hip_delta_args* u, void* hidden,
   delta_with_form(u->dtype, a.N, a.vec != 0 && aligned(hidden), [&](auto e, auto nk, auto vec) {
     using E = decltype(e);
     constexpr int NK = decltype(nk)::value;
-    const dim3 grid(static_cast<uint32_t>(a.B) * a.H * a.PT);
+    const uint32_t heads = static_cast<uint32_t>(a.B) * a.H;
     if constexpr (PairLds<E, NK>::fits) {
-      auto go = [&](auto kernel) {
+      constexpr bool V = decltype(vec)::value;
+      auto go = [&](auto kernel, uint32_t grid) {
         constexpr size_t lds = PairLds<E, NK>::bytes;
         if ((rc = set_lds(reinterpret_cast<const void*>(kernel), lds, what)) != GRM_HIP_OK) return;
-        kernel<<<grid, dim3(2 * kWalkThreads), lds, static_cast<hipStream_t>(stream)>>>(a);
+        kernel<<<dim3(grid), dim3(2 * kWalkThreads), lds, static_cast<hipStream_t>(stream)>>>(a);
         rc = check_launch(what);
       };
-      if (states != nullptr) go(delta_pair_kernel<E, NK, decltype(vec)::value, true>);
-      else go(delta_pair_kernel<E, NK, decltype(vec)::value, false>);
+      if (a.parts > 1) {
+        go(delta_pair_kernel<E, NK, V, false, true>, heads * (a.PT + a.NT) * (a.parts - 1));
+        if (rc != GRM_HIP_OK) return;
+        if (a.parts > 2) {
+          delta_join_kernel<NK><<<dim3(heads * ((a.P + 15) / 16)), dim3(2 * NK), 0, static_cast<hipStream_t>(stream)>>>(a);
+          if ((rc = check_launch(what)) != GRM_HIP_OK) return;
+        }
+      }
+      if (states != nullptr) go(delta_pair_kernel<E, NK, V, true, false>, heads * a.PT * a.parts);
+      else go(delta_pair_kernel<E, NK, V, false, false>, heads * a.PT * a.parts);
     } else {
       auto kernel = delta_walk_kernel<E, NK, decltype(vec)::value>;
       constexpr size_t lds = WalkLds<E, NK>::bytes;
       if ((rc = set_lds(reinterpret_cast<const void*>(kernel), lds, what)) != GRM_HIP_OK) return;
-      kernel<<<grid, dim3(kWalkThreads), lds, static_cast<hipStream_t>(stream)>>>(a);
+      kernel<<<dim3(heads * a.PT), dim3(kWalkThreads), lds, static_cast<hipStream_t>(stream)>>>(a);
       rc = check_launch(what);
     }
   });

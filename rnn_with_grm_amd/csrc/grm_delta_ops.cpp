@@ -90,7 +90,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> delta_scan_forward(const Tensor& keys
   Tensor memory_out = at::empty({s.B, s.H, s.P, s.N}, f32);
   Tensor states = save ? at::empty({s.B, (s.T + kTokens - 1) / kTokens, s.H, s.P, s.N}, f32) : at::empty({0}, f32);
   Tensor miss = save ? at::empty({s.B, s.T, s.H, s.P}, f32) : at::empty({0}, f32);
-  const int64_t wsb = grm_hip_delta_scan_workspace(s.B, s.T, s.H, s.args.dtype);
+  const int64_t wsb = grm_hip_delta_scan_workspace(s.B, s.T, s.H, s.P, s.N, s.args.dtype);
   Tensor ws = bytes(wsb, values);
   check_rc(grm_hip_delta_scan_fwd(&s.args, hidden.data_ptr(), memory_out.data_ptr<float>(),
                                   save ? states.data_ptr<float>() : nullptr, save ? miss.data_ptr<float>() : nullptr,
