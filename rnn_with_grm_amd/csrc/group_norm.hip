@@ -100,7 +100,7 @@ __device__ __forceinline__ float normalise(const NormArgs& a, int l, float (&x)[
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < EPL; ++j) s += x[j];
-    const float mean = group_sum<LG>(s) * inv;
+    const float mean = group_sum<LG>(s) / static_cast<float>(a.width);  // (rounded once: equal values leave nothing)
 #pragma unroll
     for (int j = 0; j < EPL; ++j) x[j] = channel<LG, VEC>(l, j) < a.width ? x[j] - mean : 0.f;
   }
