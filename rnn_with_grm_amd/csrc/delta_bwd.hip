@@ -204,10 +204,11 @@ __global__ __launch_bounds__(kThreads) void delta_reverse_kernel(DeltaBwdArgs ba
 // LDS of the mirror walk in two halves.
 template <class E, int NK>
 struct MirrorLds {
-  using KT = SelTile<BF16, NK, true>;
+  using KT = SelTile<BF16, NK, false>;  // read by rows and by columns
+  using QT = SelTile<BF16, NK, true>;   // read by columns
   using VT = SelTile<E, kDCols, true>;
-  static constexpr int NI = DParts<E>::IN, kpart = kDTokens * KT::STRIDE, SCAL = 192, NT = NK / 16;
-  static constexpr size_t k = 0, q = k + 2 * NI * kpart * 2, v = q + NI * kpart * 2,
+  static constexpr int NI = DParts<E>::IN, kpart = kDTokens * KT::STRIDE, qpart = kDTokens * QT::STRIDE, SCAL = 192, NT = NK / 16;
+  static constexpr size_t k = 0, q = k + 2 * NI * kpart * 2, v = q + NI * qpart * 2,
                           z = v + kDTokens * VT::STRIDE * sizeof(typename ET<E>::raw), u = z + 4 * 4 * 64 * 16,
                           c = u + 4 * 4 * 64 * 16, s = c + 4 * NT * 64 * 16, bytes = s + 2 * SCAL * 4;
   static constexpr bool fits = bytes <= 160 * 1024;
@@ -222,6 +223,7 @@ __global__ __launch_bounds__(2 * kThreads, 2) void delta_mirror_kernel(DeltaBwdA
   using raw = typename ET<E>::raw;
   using L = MirrorLds<E, NK>;
   using KT = typename L::KT;
+  using QT = typename L::QT;
   using VT = typename L::VT;
   constexpr int NI = L::NI, S = NK / 32, NT = NK / 16;
   const DeltaArgs& a = ba.f;
@@ -352,7 +354,8 @@ __global__ __launch_bounds__(2 * kThreads, 2) void delta_mirror_kernel(DeltaBwdA
     const raw* kp = static_cast<const raw*>(a.keys) + b * a.kb + static_cast<int64_t>(gi) * a.N;
     const raw* qp = static_cast<const raw*>(a.queries) + b * a.qb + static_cast<int64_t>(gi) * a.N;
     const raw* vp = static_cast<const raw*>(ba.dhidden) + b * a.T * row + static_cast<int64_t>(h) * a.P + col0;
-    TileLoad<E, KT, BF16, VEC, kDTokens, NK, kThreads> kl, ql;
+    TileLoad<E, KT, BF16, VEC, kDTokens, NK, kThreads> kl;
+    TileLoad<E, QT, BF16, VEC, kDTokens, NK, kThreads> ql;
     TileLoad<E, VT, E, VEC, kDTokens, kDCols, kThreads> vl;
     kl.init(a.kt, a.N, tid);
     ql.init(a.qt, a.N, tid);
@@ -369,7 +372,7 @@ __global__ __launch_bounds__(2 * kThreads, 2) void delta_mirror_kernel(DeltaBwdA
     };
     auto place = [&](int c) {
       store_parts<KT, NI, E>(kl, kt + (c & 1) * NI * L::kpart, L::kpart, kDTokens, tid);
-      store_parts<KT, NI, E>(ql, qt, L::kpart, kDTokens, tid);
+      store_parts<QT, NI, E>(ql, qt, L::qpart, kDTokens, tid);
       vl.store(vt, tid);
       if (tid < 192) sc[(c & 1) * L::SCAL + tid] = sreg;
     };
@@ -402,7 +405,6 @@ __global__ __launch_bounds__(2 * kThreads, 2) void delta_mirror_kernel(DeltaBwdA
       mma_triangle<3, false, true>(pf, hp, z);
 #pragma unroll
       for (int t = 0; t < 4; ++t) zf[64 * t] = z[t];
-      weights(c - 1);
 #pragma unroll
       for (int i = 0; i < NT; ++i) cc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -410,7 +412,7 @@ __global__ __launch_bounds__(2 * kThreads, 2) void delta_mirror_kernel(DeltaBwdA
         B8 dp[3], qf[NT][NI];
         scaled_pair(dh[2 * s], dh[2 * s + 1], sc + (c & 1) * L::SCAL + 32 * s, g, dp);
 #pragma unroll
-        for (int i = 0; i < NT; ++i) col_parts<KT, NI>(qt, L::kpart, 32 * s, 16 * i, qf[i]);
+        for (int i = 0; i < NT; ++i) col_parts<QT, NI>(qt, L::qpart, 32 * s, 16 * i, qf[i]);
         mma_many<3, true>(qf, dp, cc);
       }
     };
@@ -427,8 +429,8 @@ __global__ __launch_bounds__(2 * kThreads, 2) void delta_mirror_kernel(DeltaBwdA
       const int64_t t0 = static_cast<int64_t>(c) * kDTokens;
 #pragma unroll
       for (int i = 0; i < NT; ++i) cf[64 * i] = cc[i];
+      weights(c - 1);  // (loads are dealt to both halves of a chunk)
       if (c > 0) place(c - 1);
-      fetch(c - 2);
       warm_up(c - 3);
       __syncthreads();
       const __amdgpu_buffer_rsrc_t to = make_rsrc(ba.du + (b * a.T + t0) * row + static_cast<int64_t>(h) * a.P, 0x7ffffff0u);
@@ -443,6 +445,7 @@ __global__ __launch_bounds__(2 * kThreads, 2) void delta_mirror_kernel(DeltaBwdA
         }
       }
       if (c > 0) ahead(c - 1);
+      fetch(c - 2);
       __syncthreads();
     }
   }
@@ -453,8 +456,9 @@ __global__ __launch_bounds__(2 * kThreads, 2) void delta_mirror_kernel(DeltaBwdA
 template <class E, int NK>
 struct GradLds {
   using ST = SelTile<BF16, NK, true>;
+  using KT = SelTile<BF16, NK, false>;  // keys and queries: read by rows, by columns and in 8 bytes
   static constexpr int NI = DParts<E>::IN, XS = 68;
-  static constexpr int spart = 32 * ST::STRIDE, kpart = kDTokens * ST::STRIDE;
+  static constexpr int spart = 32 * ST::STRIDE, kpart = kDTokens * KT::STRIDE;
   static constexpr size_t gs = 3 * spart * 2, mf = gs + 3 * spart * 2, stage = mf + 4 * 3 * kDFragElems * 2, end1 = 2 * stage;
   static constexpr size_t k = 0, q = k + NI * kpart * 2, x = q + NI * kpart * 2, y = x + 64 * XS * 4, end2 = y + 64 * XS * 4;
   static constexpr size_t cum = end1 > end2 ? end1 : end2, dc = cum + 64 * 8, b = dc + 12 * 64 * 8, red = b + 64 * 4,
@@ -537,6 +541,7 @@ __global__ __launch_bounds__(kGradThreads, kGradWaves) void delta_grad_kernel(De
   using raw = typename ET<E>::raw;
   using L = GradLds<E, NK>;
   using ST = typename L::ST;
+  using KT = typename L::KT;
   constexpr int NI = L::NI, NO = DParts<E>::OUT, S = NK / 32, NT = NK / 32, ES = static_cast<int>(sizeof(raw));
   const DeltaArgs& a = ba.f;
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -698,13 +703,13 @@ __global__ __launch_bounds__(kGradThreads, kGradWaves) void delta_grad_kernel(De
     }
     __syncthreads();  // (the tiles make room)
     {
-      TileLoad<E, ST, BF16, VEC, kDTokens, NK, kGradThreads> kl, ql;
+      TileLoad<E, KT, BF16, VEC, kDTokens, NK, kGradThreads> kl, ql;
       kl.init(a.kt, a.N, tid);
       ql.init(a.qt, a.N, tid);
       kl.load(static_cast<const raw*>(a.keys) + b * a.kb + t0 * a.kt + static_cast<int64_t>(gi) * a.N, rows, tid);
       ql.load(static_cast<const raw*>(a.queries) + b * a.qb + t0 * a.qt + static_cast<int64_t>(gi) * a.N, rows, tid);
-      store_parts<ST, NI, E>(kl, kt, L::kpart, kDTokens, tid);
-      store_parts<ST, NI, E>(ql, qt, L::kpart, kDTokens, tid);
+      store_parts<KT, NI, E>(kl, kt, L::kpart, kDTokens, tid);
+      store_parts<KT, NI, E>(ql, qt, L::kpart, kDTokens, tid);
     }
     __syncthreads();
     // q.(dH S), k.(du S), k.(m G): a lane's four keys of every tile.
@@ -714,8 +719,8 @@ __global__ __launch_bounds__(kGradThreads, kGradWaves) void delta_grad_kernel(De
       f32x4 kv = zero, qv = zero;
 #pragma unroll
       for (int p = NI - 1; p >= 0; --p) {
-        const uint2 ku = *reinterpret_cast<const uint2*>(kt + p * L::kpart + ST::at(tok, key0 + 16 * i + 4 * g));
-        const uint2 qu = *reinterpret_cast<const uint2*>(qt + p * L::kpart + ST::at(tok, key0 + 16 * i + 4 * g));
+        const uint2 ku = *reinterpret_cast<const uint2*>(kt + p * L::kpart + KT::at(tok, key0 + 16 * i + 4 * g));
+        const uint2 qu = *reinterpret_cast<const uint2*>(qt + p * L::kpart + KT::at(tok, key0 + 16 * i + 4 * g));
         kv += f32x4{__uint_as_float(ku.x << 16), __uint_as_float(ku.x & 0xffff0000u), __uint_as_float(ku.y << 16),
                     __uint_as_float(ku.y & 0xffff0000u)};
         qv += f32x4{__uint_as_float(qu.x << 16), __uint_as_float(qu.x & 0xffff0000u), __uint_as_float(qu.y << 16),
@@ -759,9 +764,9 @@ __global__ __launch_bounds__(kGradThreads, kGradWaves) void delta_grad_kernel(De
 #pragma unroll
       for (int s = 0; s < S; ++s) {
         B8 li[NI], kj[4][NI];
-        row_parts_t<ST, NI>(left, L::kpart, 16 * w, 32 * s, li);
+        row_parts_t<KT, NI>(left, L::kpart, 16 * w, 32 * s, li);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) row_parts_t<ST, NI>(kt, L::kpart, 16 * j, 32 * s, kj[j]);
+        for (int j = 0; j < 4; ++j) row_parts_t<KT, NI>(kt, L::kpart, 16 * j, 32 * s, kj[j]);
         mma_many<3, false>(kj, li, dot);  // (tiles above the diagonal are not used)
       }
     }
@@ -840,8 +845,8 @@ __global__ __launch_bounds__(kGradThreads, kGradWaves) void delta_grad_kernel(De
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         B8 kf[NI], qf[NI];
-        col_parts<ST, NI>(kt, L::kpart, 32 * s, key0 + 16 * i, kf);
-        col_parts<ST, NI>(qt, L::kpart, 32 * s, key0 + 16 * i, qf);
+        col_parts<KT, NI>(kt, L::kpart, 32 * s, key0 + 16 * i, kf);
+        col_parts<KT, NI>(qt, L::kpart, 32 * s, key0 + 16 * i, qf);
         dq[i] = mma_parts<NO>(kf, yp, dq[i]);
         dk[i] = mma_parts<NO>(kf, xp, dk[i]);
         dk[i] = mma_parts<NO>(qf, cp, dk[i]);

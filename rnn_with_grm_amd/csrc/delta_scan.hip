@@ -510,7 +510,9 @@ __global__ __launch_bounds__(kWalkThreads, 1) void delta_walk_kernel(DeltaArgs a
 // LDS of the walk in two halves: two stages of a chunk, where they fit, else of its keys alone.
 template <class E, int NK>
 struct PairLds {
-  using KT = SelTile<BF16, NK, true>;
+  // Keys are read by rows and by columns; rows 4 banks apart (2 clocks a row read, 4 a column read) take 148 us for 8 x 2048
+  // tokens x 16 heads where rows 8 banks apart (4 and 2) took 166: the row reads stand in the chain.
+  using KT = SelTile<BF16, NK, false>;
   using QT = SelTile<BF16, NK, false>;
   using VT = SelTile<E, kDCols, true>;
   static constexpr int NI = DParts<E>::IN, NO = DParts<E>::OUT, SCAL = 132;
@@ -788,25 +790,21 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
       fetch(first);
       place_k(first);
       place_qv(first);
-      weights(first);
       fetch(first + 1);
     }
     __syncthreads();
     const int p = p0 + 4 * g, row = a.H * a.P * static_cast<int>(sizeof(raw));
     for (int c = first; c < chunks; ++c) {
       const int64_t t0 = static_cast<int64_t>(c) * kDTokens;
+      // (Loads are dealt to both halves of a chunk: the state waves call for their matrix in the second one.)
+      weights(c);
       place_k(c + 1);
-      if constexpr (QV == 2) {
-        place_qv(c + 1);
-        fetch(c + 2);
-      }
+      if constexpr (QV == 2) place_qv(c + 1);
       warm_up(c + 3);
       if constexpr (LOCAL) {
         __syncthreads();
-        if constexpr (QV == 1) {
-          place_qv(c + 1);
-          fetch(c + 2);
-        }
+        if constexpr (QV == 1) place_qv(c + 1);
+        fetch(c + 2);
         __syncthreads();
         continue;
       }
@@ -838,11 +836,8 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
         for (int s = 0; s < 2; ++s) split2<NO>(m[2 * s], m[2 * s + 1], mp[s]);
         mma_triangle<NO, true, false>(pf, mp, o);
       }
-      weights(c + 1);
-      if constexpr (QV == 1) {
-        place_qv(c + 1);
-        fetch(c + 2);
-      }
+      if constexpr (QV == 1) place_qv(c + 1);
+      fetch(c + 2);
       if (__any(cut < 64)) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
