@@ -225,24 +225,27 @@ __global__ __launch_bounds__(kThreads) void group_norm_bwd_kernel(NormArgs a) {
   }
 }
 
-// The workgroups' sums: 32 channels a workgroup, eight threads a channel.
+// The workgroups' sums: 32 channels a workgroup, 32 threads a channel (of 1024 rows of sums in 2048 channels 12 us with eight).
+constexpr int kSumThreads = 1024;
 template <class W>
-__global__ __launch_bounds__(kThreads) void group_norm_sum_kernel(const float* part, void* dw, void* db, int C, int blocks) {
-  __shared__ float s[8][32];
-  const int c = static_cast<int>(blockIdx.x) * 32 + static_cast<int>(threadIdx.x) % 32, k = static_cast<int>(threadIdx.x) / 32;
+__global__ __launch_bounds__(kSumThreads) void group_norm_sum_kernel(const float* part, void* dw, void* db, int C, int blocks) {
+  __shared__ float s[32][33];
+  const int l = static_cast<int>(threadIdx.x) % 32, k = static_cast<int>(threadIdx.x) / 32, c = static_cast<int>(blockIdx.x) * 32 + l;
   const float* p = part + static_cast<int64_t>(blockIdx.y) * blocks * C;
   float v = 0.f;
   if (c < C) {
 #pragma unroll 4
-    for (int i = k; i < blocks; i += 8) v += p[static_cast<int64_t>(i) * C + c];
+    for (int i = k; i < blocks; i += 32) v += p[static_cast<int64_t>(i) * C + c];
   }
-  s[k][threadIdx.x % 32] = v;
+  s[k][l] = v;
   __syncthreads();
+  // A half wave adds up a channel's 32 sums.
+  float t = s[l][k];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) t += __shfl_xor(t, o);
+  const int to_c = static_cast<int>(blockIdx.x) * 32 + k;
   void* to = blockIdx.y ? db : dw;
-  if (k == 0 && c < C && to != nullptr) {
-    for (int i = 1; i < 8; ++i) v += s[i][threadIdx.x];
-    static_cast<typename ET<W>::raw*>(to)[c] = ET<W>::from_f(v);
-  }
+  if (l == 0 && to_c < C && to != nullptr) static_cast<typename ET<W>::raw*>(to)[to_c] = ET<W>::from_f(t);
 }
 
 struct Form {
@@ -403,8 +406,8 @@ extern "C" int grm_hip_group_norm_bwd(const void* x, const void* weight, const v
   if (grad_weight == nullptr && grad_bias == nullptr) return GRM_HIP_OK;
   const dim3 grid(static_cast<uint32_t>((channels + 31) / 32), 2);
   const int blocks = rows > 0 ? static_cast<int>(f.row_blocks) : 0;  // of no rows: zeros
-  if (weight_dtype == GRM_HIP_F32) group_norm_sum_kernel<F32><<<grid, dim3(kThreads), 0, hs>>>(a.part, grad_weight, grad_bias, a.C, blocks);
-  else if (weight_dtype == GRM_HIP_F16) group_norm_sum_kernel<F16><<<grid, dim3(kThreads), 0, hs>>>(a.part, grad_weight, grad_bias, a.C, blocks);
-  else group_norm_sum_kernel<BF16><<<grid, dim3(kThreads), 0, hs>>>(a.part, grad_weight, grad_bias, a.C, blocks);
+  if (weight_dtype == GRM_HIP_F32) group_norm_sum_kernel<F32><<<grid, dim3(kSumThreads), 0, hs>>>(a.part, grad_weight, grad_bias, a.C, blocks);
+  else if (weight_dtype == GRM_HIP_F16) group_norm_sum_kernel<F16><<<grid, dim3(kSumThreads), 0, hs>>>(a.part, grad_weight, grad_bias, a.C, blocks);
+  else group_norm_sum_kernel<BF16><<<grid, dim3(kSumThreads), 0, hs>>>(a.part, grad_weight, grad_bias, a.C, blocks);
   return check_launch(what);
 }

@@ -1334,11 +1334,13 @@ def cuda_group_norm(x: Tensor, groups: int, weight: Optional[Tensor] = None, bia
     if x.is_cuda and _run_native("group_norm", x.device, enabled=enabled, debug_fallback=debug_fallback):
         if gate is not None and gate.shape != x.shape:
             raise ValueError("group_norm: gate must match x")
-        rows = (x.reshape(-1, x.size(-1)), groups, weight, bias, None if gate is None else gate.reshape(-1, x.size(-1)), silu,
-                bool(center), float(eps))
+        flat = (lambda t: t) if x.ndim == 2 else lambda t: None if t is None else t.reshape(-1, x.size(-1))
+        rows = (flat(x), groups, weight, bias, flat(gate), silu, bool(center), float(eps))
         if _wants_grad(x, weight, bias, gate):
-            return _GroupNormFn.apply(*rows).view(x.shape)
-        return torch.ops.grm_cuda.group_norm_forward(*rows).view(x.shape)
+            out = _GroupNormFn.apply(*rows)
+        else:
+            out = torch.ops.grm_cuda.group_norm_forward(*rows)
+        return out if x.ndim == 2 else out.view(x.shape)
     return _torch_group_norm(x, groups, weight, bias, gate, silu, center, eps)
 
 
