@@ -682,9 +682,15 @@ __global__ __launch_bounds__(kGradThreads, kGradWaves) void delta_grad_kernel(De
           B8 sf[3], gf[3];
           col_parts<ST, 3>(stile, L::spart, 0, key0 + 16 * i, sf);
           col_parts<ST, 3>(gtile, L::spart, 0, key0 + 16 * i, gf);
-          yq[i] = mma_parts<3>(sf, hp, yq[i]);
-          yk[i] = mma_parts<3>(sf, up, yk[i]);
-          yg[i] = mma_parts<3>(gf, mp, yg[i]);
+#pragma unroll
+          for (int o = 2; o >= 0; --o) {  // (three sums in turn: a product waits for none of the two before it)
+#pragma unroll
+            for (int k = 0; k <= o; ++k) {
+              yk[i] = mfma8(sf[k], up[o - k], yk[i]);
+              yg[i] = mfma8(gf[k], mp[o - k], yg[i]);
+              if (o - k < NI) yq[i] = mfma8(sf[k], hp[o - k], yq[i]);
+            }
+          }
         }
       }
 #pragma unroll
