@@ -590,7 +590,7 @@ int grm_hip_selective_step(const grm_hip_selective_args* args, void* hidden, flo
  * is reached, two parts, which lose 2^-16 of a term.  From a token that holds an infinity or a NaN on, what depends on it is NaN
  * (a value: its column; a query: its row of hidden; all else: the head); earlier tokens are untouched.
  * Limits: key_dim <= 128, heads a multiple of groups, token strides and rows of at most 2^21 elements, batch * heads *
- * ceil(value_dim / 64) below 2^23 and batch * heads * ceil(seq_len / 64) below 2^24 (single token: batch * heads).
+ * ceil(value_dim / 64) and batch * heads * ceil(seq_len / 64) below 2^23 (single token: batch * heads below 2^24).
  */
 typedef struct grm_hip_delta_args {
   const void* keys;

@@ -510,8 +510,8 @@ __global__ __launch_bounds__(kWalkThreads, 1) void delta_walk_kernel(DeltaArgs a
 // LDS of the walk in two halves: two stages of a chunk, where they fit, else of its keys alone.
 template <class E, int NK>
 struct PairLds {
-  // Keys are read by rows and by columns; rows 4 banks apart (2 clocks a row read, 4 a column read) take 148 us for 8 x 2048
-  // tokens x 16 heads where rows 8 banks apart (4 and 2) took 166: the row reads stand in the chain.
+  // Keys are read by rows and by columns; rows 4 banks apart (2 clocks a row read, 4 a column read) take 140 us for 8 x 2048
+  // tokens x 16 heads where rows 8 banks apart (4 and 2) took 148: the row reads stand in the chain.
   using KT = SelTile<BF16, NK, false>;
   using QT = SelTile<BF16, NK, false>;
   using VT = SelTile<E, kDCols, true>;
@@ -1114,12 +1114,12 @@ int delta_check(const grm_hip_delta_args* u, const char* what, bool step) {
     set_error("%s: token strides and row widths must be at most 2^21 elements", what);
     return GRM_HIP_EUNSUPPORTED;
   }
-  // (A grid dimension has fewer than 2^32 threads, of which a walk's workgroup has 512 and the others' 256.)
+  // (A grid dimension has fewer than 2^32 threads, of which a workgroup of a walk and of the gradients has 512, of a token 256.)
   const int64_t seqs = u->heads * min_i64(u->batch, int64_t{1} << 32), grid = int64_t{1} << 24;
   const int64_t tiles = (u->value_dim + kDCols - 1) / kDCols, chunks = (u->seq_len + kDTokens - 1) / kDTokens;
-  if (seqs >= grid || (!step && (seqs * tiles >= grid / 2 || seqs * chunks >= grid))) {
+  if (seqs >= grid || (!step && (seqs * tiles >= grid / 2 || seqs * chunks >= grid / 2))) {
     set_error(step ? "%s: batch * heads must be below 2^24"
-                   : "%s: batch * heads * ceil(value_dim / 64) must be below 2^23 and batch * heads * ceil(seq_len / 64) below 2^24", what);
+                   : "%s: batch * heads * ceil(value_dim / 64) and batch * heads * ceil(seq_len / 64) must be below 2^23", what);
     return GRM_HIP_EUNSUPPORTED;
   }
   if (u->seq_len > 1 && (u->keys_token_stride < u->groups * u->key_dim || u->queries_token_stride < u->groups * u->key_dim ||

@@ -130,7 +130,7 @@ BAD = [
     (dict(dtype=7), capi.EUNSUPPORTED), (dict(strengths_dtype=capi.F16), capi.EUNSUPPORTED), (dict(decays_dtype=5), capi.EUNSUPPORTED),
     (dict(seq_len=2 ** 31), capi.EUNSUPPORTED), (dict(heads=2 ** 22, groups=2 ** 22), capi.EUNSUPPORTED),
     (dict(value_dim=2 ** 62), capi.EUNSUPPORTED), (dict(batch=2 ** 62), capi.EUNSUPPORTED), (dict(keys_token_stride=15), capi.EINVAL),
-    (dict(values_token_stride=2 ** 22), capi.EUNSUPPORTED), (dict(batch=2 ** 21, heads=4), capi.EUNSUPPORTED),
+    (dict(values_token_stride=2 ** 22), capi.EUNSUPPORTED), (dict(batch=2 ** 21, heads=4), capi.EUNSUPPORTED), (dict(seq_len=2 ** 27 + 1, batch=1), capi.EUNSUPPORTED),
     (dict(keys=None), capi.EINVAL), (dict(strengths=None), capi.EINVAL), (dict(memory=20), capi.EINVAL),
 ]
 
