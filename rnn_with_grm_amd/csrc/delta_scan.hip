@@ -526,6 +526,14 @@ struct PairLds {
                           m = s + 4 * state * 2, sc = m + 4 * 4 * 64 * 16, cut = sc + 2 * SCAL * 4, bytes = cut + 64 * 4;
   static constexpr bool fits = bytes <= 160 * 1024;
 };
+// Of the parts' walk without outputs: three stages of keys and two of both halves' values.
+template <class E, int NK>
+struct LocalLds : PairLds<E, NK> {
+  using L = PairLds<E, NK>;
+  static constexpr size_t k = 0, v = 3 * L::NI * L::kpart * 2, sc = v + 4 * L::vstage * sizeof(typename ET<E>::raw),
+                          bytes = sc + 3 * L::SCAL * 4;
+  static_assert(!L::fits || bytes <= 160 * 1024, "three stages");
+};
 
 // The walk over a sequence's chunks, 64 value columns of a head a workgroup.  Four state waves hold 16 columns each, in
 // accumulators, and run the chain that a chunk hangs on: K S^T, m, the next state.  Four output waves, one beside each
@@ -537,15 +545,18 @@ struct PairLds {
 // Sequences in time parts: a first launch (LOCAL) walks all parts but the last side by side and without outputs.  Rows of a
 // state never meet, and without values each passes through a part as a row of a matrix product; so beside the value rows of a
 // part, from a zero state, go the N rows of the identity without values, whose end is the part's map.  delta_join_kernel makes
-// the parts' first states of both, and the second launch walks every part from its own.
+// the parts' first states of both, and the second launch walks every part from its own.  Without outputs all eight waves hold
+// states, 128 columns of value rows and then identity a workgroup, so that two chains share a SIMD; they load the keys
+// together, three stages, one barrier a chunk (7 parts of 64 chunks x 16 heads of 128 x 128: 340 us; 446 with a chain a SIMD).
 template <class E, int NK, bool VEC, bool SAVE, bool LOCAL>
 __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaArgs a) {
   using raw = typename ET<E>::raw;
-  using L = PairLds<E, NK>;
+  using L = std::conditional_t<LOCAL, LocalLds<E, NK>, PairLds<E, NK>>;
   using KT = typename L::KT;
   using QT = typename L::QT;
   using VT = typename L::VT;
-  constexpr int NI = L::NI, NO = L::NO, S = NK / 32, NT = NK / 16, QV = L::QV;
+  constexpr int NI = L::NI, NO = L::NO, S = NK / 32, NT = NK / 16, QV = LOCAL ? 2 : L::QV;
+  constexpr int KLOADERS = (LOCAL ? 2 : 1) * kWalkThreads;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   uint16_t* kt = reinterpret_cast<uint16_t*>(lds + L::k);
   uint16_t* qt = reinterpret_cast<uint16_t*>(lds + L::q);
@@ -555,11 +566,12 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
   const int lane = lane_id(), g = lane >> 4, n = lane & 15;
   const uint32_t at = xcd_order(blockIdx.x, gridDim.x);
-  const int tiles = LOCAL ? a.PT + a.NT : a.PT, parts = LOCAL ? a.parts - 1 : a.parts;
-  const int pt = static_cast<int>(at % tiles), part = static_cast<int>(at / tiles % parts);
+  const int tiles = LOCAL ? (a.PT + a.NT + 1) / 2 : a.PT, parts = LOCAL ? a.parts - 1 : a.parts;
+  const int half = LOCAL ? wave >> 2 : 0;
+  const int pt = static_cast<int>(at % tiles) * (LOCAL ? 2 : 1) + half, part = static_cast<int>(at / tiles % parts);
   const int h = static_cast<int>(at / tiles / parts % a.H), b = static_cast<int>(at / tiles / parts / a.H);
   const bool map = LOCAL && pt >= a.PT;  // rows of the identity
-  if (map && part == 0) return;          // (the first part starts from the sequence's own state)
+  if (LOCAL && pt - half >= a.PT && part == 0) return;  // (the first part starts from the sequence's own state)
   const int64_t len = delta_length(a, b);
   const int col0 = (map ? pt - a.PT : pt) * kDCols, p0 = col0 + 16 * w, gi = h / (a.H / a.G), prows = map ? a.N : a.P;
   const int first = part * a.part_chunks, have = static_cast<int>((len + kDTokens - 1) / kDTokens);
@@ -569,8 +581,59 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
   uint16_t* sf = reinterpret_cast<uint16_t*>(lds + L::s) + w * L::state + 8 * lane;
   f32x4* mf = reinterpret_cast<f32x4*>(lds + L::m) + w * 256 + lane;
 
-  if (wave < 4) {
-    __builtin_amdgcn_s_setprio(2);
+  const int tid = static_cast<int>(threadIdx.x) - (LOCAL ? 0 : kWalkThreads), vtid = tid % kWalkThreads;  // of the loading waves
+  const raw* kp = static_cast<const raw*>(a.keys) + b * a.kb + static_cast<int64_t>(gi) * a.N;
+  const raw* qp = static_cast<const raw*>(a.queries) + b * a.qb + static_cast<int64_t>(gi) * a.N;
+  const raw* vp = static_cast<const raw*>(a.values) + b * a.vb + static_cast<int64_t>(h) * a.P + (map ? 0 : col0);
+  TileLoad<E, KT, BF16, VEC, kDTokens, NK, KLOADERS> kl;
+  TileLoad<E, QT, BF16, VEC, kDTokens, NK, kWalkThreads> ql;
+  TileLoad<E, VT, E, VEC, kDTokens, kDCols, kWalkThreads> vl;
+  float sreg = 0.f, warm = 0.f;
+  int oreg = 64;
+  auto fetch = [&](int want) {
+    const int c = want < chunks ? want : chunks - 1;
+    const int64_t t0 = static_cast<int64_t>(c) * kDTokens;
+    const float* s = reinterpret_cast<const float*>(work + c * delta_chunk_bytes(NO) + (3 + NO) * kDFrags * kDFragElems * 2);
+    sreg = s[tid & 127];
+    oreg = reinterpret_cast<const int*>(s)[192];
+    kl.load(kp + t0 * a.kt, len - t0, tid);
+    if constexpr (!LOCAL) ql.load(qp + t0 * a.qt, len - t0, tid);
+    vl.load(vp + t0 * a.vt, map ? 0 : len - t0, vtid);  // (a map's rows have no values)
+  };
+  auto place_qv = [&](int c) {
+    if constexpr (!LOCAL) store_parts<QT, NI, E>(ql, qt + (c & (QV - 1)) * L::qstage, L::qpart, kDTokens, tid);
+    vl.store(vt + (2 * half + (c & (QV - 1))) * L::vstage, vtid);
+  };
+  auto stage = [](int c) { return LOCAL ? c % 3 : c & 1; };
+  auto place_k = [&](int c) {
+    store_parts<KT, NI, E>(kl, kt + stage(c) * NI * L::kpart, L::kpart, oreg, tid);
+    float* to = sc + stage(c) * L::SCAL;
+    if (tid < 128) to[tid] = sreg;
+    if (tid == 128) reinterpret_cast<int*>(to)[128] = oreg;
+  };
+  // One word of every line of a later chunk's matrices, so that they lie in the L2 when they are called for.
+  auto warm_up = [&](int want) {
+    const int c = want < chunks ? want : chunks - 1;
+    asm volatile("" ::"v"(warm));
+    constexpr int lines = static_cast<int>((LOCAL ? 3 * kDFrags * kDFragElems * 2 : delta_chunk_bytes(NO)) / 128);
+    for (int i = tid; i < lines; i += KLOADERS) warm = *reinterpret_cast<const float*>(work + c * delta_chunk_bytes(NO) + 128 * i);
+  };
+  auto begin = [&] {
+    kl.init(a.kt, a.N, tid);
+    if constexpr (!LOCAL) ql.init(a.qt, a.N, tid);
+    const int cols = prows - col0;
+    vl.init(a.vt, cols > kDCols ? kDCols : cols > 0 ? cols : 0, vtid);
+    if (chunks > first) {
+      fetch(first);
+      place_k(first);
+      place_qv(first);
+      fetch(first + 1);
+    }
+  };
+
+  if (LOCAL || wave < 4) {
+    if constexpr (LOCAL) begin();
+    else __builtin_amdgcn_s_setprio(2);
     const float inf = __builtin_inff();
     f32x4 st[NT];
 #pragma unroll
@@ -610,12 +673,12 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
 #pragma unroll
     for (int s = 0; s < S; ++s) publish(s);
     __syncthreads();
-    if (chunks > first) row_keys(kt + (first & 1) * NI * L::kpart, 0);
+    if (chunks > first) row_keys(kt + stage(first) * NI * L::kpart, 0);
     for (int c = first; c < chunks; ++c) {
-      const uint16_t* kc = kt + (c & 1) * NI * L::kpart;
-      const float* scc = sc + (c & 1) * L::SCAL;
+      const uint16_t* kc = kt + stage(c) * NI * L::kpart;
+      const float* scc = sc + stage(c) * L::SCAL;
       const int next = c + 1 < chunks ? c + 1 : c;
-      const raw* vc = vt + (c & (QV - 1)) * L::vstage;
+      const raw* vc = vt + (2 * half + (c & (QV - 1))) * L::vstage;
       // (Read ahead of the products, which they wait for.)
       Frag8<E> vf[2];
       float4 dd[4];
@@ -624,6 +687,12 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
 #pragma unroll
       for (int t = 0; t < 4; ++t) dd[t] = *reinterpret_cast<const float4*>(scc + 16 * t + 4 * g);
       const int odd_key = __builtin_amdgcn_readfirstlane(reinterpret_cast<const int*>(scc)[128]);
+      if constexpr (LOCAL) {  // (the stages of the keys two chunks ago and of the last chunk's values)
+        place_k(c + 1);
+        place_qv(c + 1);
+        warm_up(c + 3);
+        fetch(c + 2);
+      }
       hold_order();
       // K S^T: a token a row, a value a column.
       f32x4 x[4];
@@ -680,8 +749,8 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
       if constexpr (!LOCAL) {
 #pragma unroll
         for (int t = 0; t < 4; ++t) mf[64 * t] = m[t];
+        if (g == 0) cuts[16 * w + n] = cut;
       }
-      if (g == 0) cuts[16 * w + n] = cut;
       B8 kf[2][2][2][NI];  // [pair & 1][step][tile of the pair]
       auto pair_keys = [&](int j) {
 #pragma unroll
@@ -734,64 +803,19 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
       }
       publish(S - 1);
       keep_state(c + 1);
-      row_keys(kt + ((c + 1) & 1) * NI * L::kpart, 0);  // (there since the chunk's first barrier)
-      __syncthreads();
+      row_keys(kt + stage(c + 1) * NI * L::kpart, 0);  // (there since the chunk's first barrier)
+      if constexpr (!LOCAL) __syncthreads();
     }
     if (map) state_store<NT>(st, a.part_map + (part * all + head) * a.N * a.N, p0, a.N, a.N);
     else if (LOCAL) state_store<NT>(st, a.part_state + (part * all + head) * cells, p0, a.P, a.N);
     else if (part == a.parts - 1) state_store<NT>(st, a.memory_out + head * cells, p0, a.P, a.N);
   } else {
-    const int tid = static_cast<int>(threadIdx.x) - kWalkThreads;
-    const raw* kp = static_cast<const raw*>(a.keys) + b * a.kb + static_cast<int64_t>(gi) * a.N;
-    const raw* qp = static_cast<const raw*>(a.queries) + b * a.qb + static_cast<int64_t>(gi) * a.N;
-    const raw* vp = static_cast<const raw*>(a.values) + b * a.vb + static_cast<int64_t>(h) * a.P + (map ? 0 : col0);
-    TileLoad<E, KT, BF16, VEC, kDTokens, NK, kWalkThreads> kl;
-    TileLoad<E, QT, BF16, VEC, kDTokens, NK, kWalkThreads> ql;
-    TileLoad<E, VT, E, VEC, kDTokens, kDCols, kWalkThreads> vl;
-    kl.init(a.kt, a.N, tid);
-    ql.init(a.qt, a.N, tid);
-    vl.init(a.vt, prows - col0 < kDCols ? prows - col0 : kDCols, tid);
-    float sreg = 0.f, warm = 0.f;
-    int oreg = 64;
     B8 pf[kDFrags][NO];
-    auto fetch = [&](int want) {
-      const int c = want < chunks ? want : chunks - 1;
-      const int64_t t0 = static_cast<int64_t>(c) * kDTokens;
-      const float* s = reinterpret_cast<const float*>(work + c * delta_chunk_bytes(NO) + (3 + NO) * kDFrags * kDFragElems * 2);
-      sreg = s[tid & 127];
-      oreg = reinterpret_cast<const int*>(s)[192];
-      kl.load(kp + t0 * a.kt, len - t0, tid);
-      if constexpr (!LOCAL) ql.load(qp + t0 * a.qt, len - t0, tid);
-      vl.load(vp + t0 * a.vt, map ? 0 : len - t0, tid);  // (a map's rows have no values)
-    };
-    auto place_qv = [&](int c) {
-      if constexpr (!LOCAL) store_parts<QT, NI, E>(ql, qt + (c & (QV - 1)) * L::qstage, L::qpart, kDTokens, tid);
-      vl.store(vt + (c & (QV - 1)) * L::vstage, tid);
-    };
-    auto place_k = [&](int c) {
-      store_parts<KT, NI, E>(kl, kt + (c & 1) * NI * L::kpart, L::kpart, oreg, tid);
-      float* to = sc + (c & 1) * L::SCAL;
-      if (tid < 128) to[tid] = sreg;
-      if (tid == 128) reinterpret_cast<int*>(to)[128] = oreg;
-    };
-    // One word of every line of a later chunk's matrices, so that they lie in the L2 when they are called for.
-    auto warm_up = [&](int want) {
-      const int c = want < chunks ? want : chunks - 1;
-      asm volatile("" ::"v"(warm));
-      constexpr int lines = static_cast<int>((LOCAL ? 3 * kDFrags * kDFragElems * 2 : delta_chunk_bytes(NO)) / 128);
-      for (int i = tid; i < lines; i += kWalkThreads) warm = *reinterpret_cast<const float*>(work + c * delta_chunk_bytes(NO) + 128 * i);
-    };
     auto weights = [&](int want) {
-      if constexpr (LOCAL) return;
       const int c = want < chunks ? want : chunks - 1;
       stored_triangle<NO>(reinterpret_cast<const uint16_t*>(work + c * delta_chunk_bytes(NO)) + 3 * kDFrags * kDFragElems, pf, lane);
     };
-    if (chunks > first) {
-      fetch(first);
-      place_k(first);
-      place_qv(first);
-      fetch(first + 1);
-    }
+    begin();
     __syncthreads();
     const int p = p0 + 4 * g, row = a.H * a.P * static_cast<int>(sizeof(raw));
     for (int c = first; c < chunks; ++c) {
@@ -801,13 +825,6 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
       place_k(c + 1);
       if constexpr (QV == 2) place_qv(c + 1);
       warm_up(c + 3);
-      if constexpr (LOCAL) {
-        __syncthreads();
-        if constexpr (QV == 1) place_qv(c + 1);
-        fetch(c + 2);
-        __syncthreads();
-        continue;
-      }
       const uint16_t* qc = qt + (c & (QV - 1)) * L::qstage;
       // S Q^T: a value a row, a token a column, as rows are stored.
       f32x4 o[4];
@@ -877,7 +894,6 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
       __syncthreads();
     }
     // Rows of this part behind the last chunk.
-    if constexpr (LOCAL) return;
     const int64_t end = min_i64(a.T, (static_cast<int64_t>(first) + a.part_chunks) * kDTokens);
     for (int64_t t = static_cast<int64_t>(chunks) * kDTokens + tid / 16; t < end; t += kWalkThreads / 16) {
       raw* to = static_cast<raw*>(a.hidden) + ((b * a.T + t) * a.H + h) * a.P + col0;
@@ -1052,17 +1068,18 @@ int out_parts(int dtype) { return dtype == GRM_HIP_F32 ? 3 : 2; }
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 
 // Time parts of a sequence.  256 CUs hold a workgroup each; a part costs its chunks once more, for the value rows and for
-// the N rows of its map, so parts are taken where they shorten the longest line of chunks behind each other (in units of
-// a chunk; a launch and a join count as a few).  32768 bf16 tokens x 16 heads of 128 x 128: 1900 us in one part.
+// the N rows of its map, so parts are taken where they shorten the longest line of chunks behind each other (in quarters of
+// a chunk's time; one of the first walk, with two chains a SIMD, takes five, a launch and a join a few chunks).  32768 bf16
+// tokens x 16 heads of 128 x 128: 1900 us in one part, 650 in eight.
 int time_parts(int64_t seqs, int64_t P, int64_t N, int64_t C, int dtype, int64_t* part_chunks) {
   *part_chunks = C;
   if ((dtype != GRM_HIP_BF16 && N > 64) || seqs > 4096) return 1;  // (delta_walk_kernel takes whole sequences)
   const int64_t PT = (P + kDCols - 1) / kDCols, NT = (N + kDCols - 1) / kDCols;
   auto rounds = [](int64_t wgs) { return (wgs + 255) / 256; };
-  int64_t best = C * rounds(seqs * PT), parts = 1;
+  int64_t best = 4 * C * rounds(seqs * PT), parts = 1;
   for (int64_t r = 2; r <= 64 && r <= C / 4; ++r) {
     const int64_t per = (C + r - 1) / r, n = (C + per - 1) / per;
-    const int64_t cost = per * (rounds(seqs * PT * n) + rounds(seqs * (PT + NT) * (n - 1))) + 2 * n + 6;
+    const int64_t cost = per * (4 * rounds(seqs * PT * n) + 5 * rounds(seqs * ((PT + NT + 1) / 2) * (n - 1))) + 8 * n + 24;
     if (cost < best) best = cost, parts = n, *part_chunks = per;
   }
   return static_cast<int>(parts);
@@ -1228,22 +1245,21 @@ extern "C" int grm_hip_delta_scan_fwd(const grm_hip_delta_args* u, void* hidden,
     const uint32_t heads = static_cast<uint32_t>(a.B) * a.H;
     if constexpr (PairLds<E, NK>::fits) {
       constexpr bool V = decltype(vec)::value;
-      auto go = [&](auto kernel, uint32_t grid) {
-        constexpr size_t lds = PairLds<E, NK>::bytes;
+      auto go = [&](auto kernel, uint32_t grid, size_t lds) {
         if ((rc = set_lds(reinterpret_cast<const void*>(kernel), lds, what)) != GRM_HIP_OK) return;
         kernel<<<dim3(grid), dim3(2 * kWalkThreads), lds, static_cast<hipStream_t>(stream)>>>(a);
         rc = check_launch(what);
       };
       if (a.parts > 1) {
-        go(delta_pair_kernel<E, NK, V, false, true>, heads * (a.PT + a.NT) * (a.parts - 1));
+        go(delta_pair_kernel<E, NK, V, false, true>, heads * ((a.PT + a.NT + 1) / 2) * (a.parts - 1), LocalLds<E, NK>::bytes);
         if (rc != GRM_HIP_OK) return;
         if (a.parts > 2) {
           delta_join_kernel<NK><<<dim3(heads * ((a.P + 15) / 16)), dim3(2 * NK), 0, static_cast<hipStream_t>(stream)>>>(a);
           if ((rc = check_launch(what)) != GRM_HIP_OK) return;
         }
       }
-      if (states != nullptr) go(delta_pair_kernel<E, NK, V, true, false>, heads * a.PT * a.parts);
-      else go(delta_pair_kernel<E, NK, V, false, false>, heads * a.PT * a.parts);
+      if (states != nullptr) go(delta_pair_kernel<E, NK, V, true, false>, heads * a.PT * a.parts, PairLds<E, NK>::bytes);
+      else go(delta_pair_kernel<E, NK, V, false, false>, heads * a.PT * a.parts, PairLds<E, NK>::bytes);
     } else {
       auto kernel = delta_walk_kernel<E, NK, decltype(vec)::value>;
       constexpr size_t lds = WalkLds<E, NK>::bytes;
