@@ -145,20 +145,21 @@ __device__ __forceinline__ void mma_triangle(const B8 (&f)[kDFrags][NA], const B
   }
 }
 
-// A wave's 16 value rows of a state to memory, as state_store does; WHOLE: rows of whole 16-byte units, and no branch
-// around the stores, so that waits for loads before them are counted past them.
+// Tiles nt and nt + 1 of a wave's 16 value rows of a state to memory, as state_store does (which takes all at once where rows
+// are not of whole 16-byte units).  The walk stores them between the products that read them (8 x 2048 bf16 tokens x 16 heads of
+// 128 x 128: 216 us behind the chunk's last product, 207 here); its mirror, whose output waves load and store more in
+// that half, behind the last one (207-211 us; 220 between the products).
 template <bool WHOLE, int NT>
-__device__ __forceinline__ void state_out(const f32x4 (&acc)[NT], float* s, int p0, int P, int N) {
+__device__ __forceinline__ void state_out(const f32x4 (&acc)[NT], int nt, float* s, int p0, int P, int N) {
   if constexpr (!WHOLE) {
-    state_store<NT>(acc, s, p0, P, N);
+    if (nt == 0) state_store<NT>(acc, s, p0, P, N);
   } else {
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     int lane = lane_id();
     asm volatile("" : "+v"(lane));  // no address made from it is kept in registers between stores
     const int low = lane & 8;
     const __amdgpu_buffer_rsrc_t rsrc = make_rsrc(s, static_cast<uint32_t>(P * N * 4));
-#pragma unroll
-    for (int nt = 0; nt < NT; nt += 2) {  // (halves exchanged between lanes eight apart: whole 128-byte lines)
+    {  // (halves exchanged between lanes eight apart: whole 128-byte lines)
       const int n = nt * 16 + 2 * low + 4 * (lane >> 4);
       f32x4 v[2];
 #pragma unroll
@@ -172,6 +173,51 @@ __device__ __forceinline__ void state_out(const f32x4 (&acc)[NT], float* s, int 
       for (int u = 0; u < 2; ++u) {
         const int row = p0 + 8 * u + (lane & 7);
         __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v[u]), rsrc, row < P && n < N ? (row * N + n) * 4 : kBufOOB, 0, 0);
+      }
+    }
+  }
+}
+
+// Four rows of a lane's column as a row's four columns, among the four lanes of a quad: rows leave in 16 bytes.
+__device__ __forceinline__ f32x4 quad_turn(f32x4 v) {
+  const int lane = lane_id();
+  auto swap = [](float mine, float other, bool second, auto ctrl) {  // (second: `mine` is handed over, else `other`)
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(second ? mine : other), decltype(ctrl)::value, 0xf, 0xf, true));
+  };
+  const bool odd = lane & 1, high = lane & 2;
+  constexpr std::integral_constant<int, 0xb1> by1{};  // lanes 1 0 3 2
+  constexpr std::integral_constant<int, 0x4e> by2{};  // lanes 2 3 0 1
+#pragma unroll
+  for (int i = 0; i < 4; i += 2) {
+    const float t = swap(v[i], v[i + 1], odd, by1);
+    v[i] = odd ? t : v[i];
+    v[i + 1] = odd ? v[i + 1] : t;
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float t = swap(v[i], v[i + 2], high, by2);
+    v[i] = high ? t : v[i];
+    v[i + 2] = high ? v[i + 2] : t;
+  }
+  return v;
+}
+
+// A column of 16 x 4 float32 accumulators (tokens 16 t + 4 g + r, value p0 + n) to rows of `step` bytes; WHOLE: in 16 bytes
+// (a quarter of the stores).
+template <bool WHOLE>
+__device__ __forceinline__ void rows_out(const f32x4 (&acc)[4], __amdgpu_buffer_rsrc_t to, int step, int64_t rows, int p0, int P) {
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  const int g = lane_id() >> 4, n = lane_id() & 15;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    if constexpr (WHOLE) {
+      const int tok = 16 * t + 4 * g + (n & 3), col = p0 + (n & 12);
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, quad_turn(acc[t])), to, tok < rows && col < P ? tok * step + col * 4 : kBufOOB, 0, 0);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int tok = 16 * t + 4 * g + r;
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(acc[t][r]), to, tok < rows && p0 + n < P ? tok * step + (p0 + n) * 4 : kBufOOB, 0, 0);
       }
     }
   }

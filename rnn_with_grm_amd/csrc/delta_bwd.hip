@@ -258,7 +258,9 @@ __global__ __launch_bounds__(2 * kThreads, 2) void delta_mirror_kernel(DeltaBwdA
       for (int t = 0; t < 4; ++t) row_parts_t<KT, NI>(from, L::kpart, 16 * t, 32 * s, kr[s & 1][t]);
     };
     auto keep_state = [&](int c) {  // (before the first chunk: behind the last value row, where nothing is stored)
-      state_out<VEC>(st, ba.gstates + ((static_cast<int64_t>(b) * a.C + (c < 0 ? 0 : c)) * a.H + h) * cells, c < 0 ? a.P : p0, a.P, a.N);
+#pragma unroll
+      for (int s = 0; s < S; ++s)
+        state_out<VEC>(st, 2 * s, ba.gstates + ((static_cast<int64_t>(b) * a.C + (c < 0 ? 0 : c)) * a.H + h) * cells, c < 0 ? a.P : p0, a.P, a.N);
     };
 #pragma unroll
     for (int s = 0; s < S; ++s) split2<3>(st[2 * s], st[2 * s + 1], gp[s]);
@@ -435,16 +437,10 @@ __global__ __launch_bounds__(2 * kThreads, 2) void delta_mirror_kernel(DeltaBwdA
       warm_up(c - 3);
       __syncthreads();
       const __amdgpu_buffer_rsrc_t to = make_rsrc(ba.du + (b * a.T + t0) * row + static_cast<int64_t>(h) * a.P, 0x7ffffff0u);
-      const int step = static_cast<int>(row) * 4, col = p0 + n;
+      f32x4 du[4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const f32x4 du = uf[64 * t];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int tok = 16 * t + 4 * g + r;
-          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(du[r]), to, t0 + tok < len && col < a.P ? tok * step + col * 4 : kBufOOB, 0, 0);
-        }
-      }
+      for (int t = 0; t < 4; ++t) du[t] = uf[64 * t];
+      rows_out<VEC>(du, to, static_cast<int>(row) * 4, len - t0, p0, a.P);
       if (c > 0) ahead(c - 1);
       fetch(c - 2);
       __syncthreads();

@@ -664,17 +664,14 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
       for (int p = 0; p < NO; ++p)
         *reinterpret_cast<uint4*>(sf + (s * NO + p) * kDFragElems) = __builtin_bit_cast(uint4, sp[s][p]);
     };
-    auto keep_state = [&](int c) {
-      // (Behind the last chunk its state is not kept: the stores fall behind the last value row.)
-      if constexpr (SAVE)
-        state_out<VEC>(st, a.states + ((static_cast<int64_t>(b) * a.C + (c < chunks ? c : c - 1)) * a.H + h) * cells, c < chunks ? p0 : a.P, a.P, a.N);
+    auto keep_state = [&](int c, int s) {
+      if constexpr (SAVE) state_out<VEC>(st, 2 * s, a.states + ((static_cast<int64_t>(b) * a.C + c) * a.H + h) * cells, p0, a.P, a.N);
     };
     B8 kr[2][4][NI];  // keys by rows, [step & 1][tile]
     auto row_keys = [&](const uint16_t* from, int s) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) row_parts_t<KT, NI>(from, L::kpart, 16 * t, 32 * s, kr[s & 1][t]);
     };
-    if (chunks > first) keep_state(first);
 #pragma unroll
     for (int s = 0; s < S; ++s) publish(s);
     __syncthreads();
@@ -707,6 +704,7 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
       for (int s = 0; s < S; ++s) {
         if (s + 1 < S) row_keys(kc, s + 1);
         mma_many<3, true>(kr[s & 1], sp[s], x);
+        keep_state(c, s);
         hold_order();
       }
       // V - D K S^T.
@@ -807,7 +805,6 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
         for (int s = 0; s + 1 < S; ++s) publish(s);
       }
       publish(S - 1);
-      keep_state(c + 1);
       row_keys(kt + stage(c + 1) * NI * L::kpart, 0);  // (there since the chunk's first barrier)
       if constexpr (!LOCAL) __syncthreads();
     }
@@ -884,17 +881,9 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
         }
       }
       if constexpr (SAVE) {
-        const int mrow = a.H * a.P * 4, col = p0 + n;
         const __amdgpu_buffer_rsrc_t ms =
             make_rsrc(a.miss + ((static_cast<int64_t>(b) * a.T + t0) * a.H + h) * a.P, 0x7ffffff0u);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int tok = 16 * t + 4 * g + r;
-            __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(m[t][r]), ms, t0 + tok < len && col < a.P ? tok * mrow + col * 4 : kBufOOB, 0, 0);
-          }
-        }
+        rows_out<VEC>(m, ms, a.H * a.P * 4, len - t0, p0, a.P);
       }
       __syncthreads();
     }

@@ -94,11 +94,12 @@ def test_gradients_through_the_block(dev):
         assert (a.double().cpu() - b).norm() <= 4 * 8 * math.sqrt(154) * 16 * 2.0 ** -24 * b.norm()
 
 
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-def test_long_sequences_of_few_heads(dev, dtype):
-    """In time parts, whole key widths, with gradients."""
+@pytest.mark.parametrize("dtype,P1,N1", [(torch.bfloat16, 40, 128), (torch.float32, 40, 64), (torch.bfloat16, 70, 90),
+                                         (torch.float16, 130, 30), (torch.float32, 5, 7)])
+def test_long_sequences_of_few_heads(dev, dtype, P1, N1):
+    """In time parts, with gradients: whole and odd widths, odd numbers of column tiles."""
     g = torch.Generator().manual_seed(4)
-    T, P1, N1 = 3000, 40, 128 if dtype == torch.bfloat16 else 64
+    T = 3000
     unit = lambda: 0.99 * torch.nn.functional.normalize(torch.randn(1, T, 1, N1, generator=g), dim=-1)  # noqa: E731
     x = [unit().to(dtype).to(dev), torch.randn(1, T, 1, P1, generator=g).to(dtype).to(dev), unit().to(dtype).to(dev),
          torch.rand(1, T, 1, generator=g).to(dtype).to(dev), (-0.02 * torch.rand(1, T, 1, generator=g)).to(dev),
