@@ -285,6 +285,10 @@ int delta_check(const struct grm_hip_delta_args* u, const char* what, bool step)
 DeltaArgs delta_args(const struct grm_hip_delta_args* u);
 // The chunks' inverses and weights into a.work; `back`: in the reverse walk's form.
 int launch_delta_prep(const DeltaArgs& a, int dtype, bool back, hipStream_t stream, const char* what);
+// The parts' first states of part_state and part_map, for parts above two.
+int launch_delta_join(const DeltaArgs& a, hipStream_t stream, const char* what);
+// Time parts of the walk over C chunks and of its mirror, and a part's chunks.
+int delta_time_parts(int64_t seqs, int64_t P, int64_t N, int64_t C, int dtype, bool mirror, int64_t* part_chunks);
 
 // Host side: f(E, NK, VEC) with one of the compiled forms.
 template <class F>

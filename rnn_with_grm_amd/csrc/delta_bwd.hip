@@ -218,8 +218,11 @@ struct MirrorLds {
 // waves run the chain that the next chunk hangs on (K G^T, du, the state's update by the keys); four output waves, one beside
 // each on its SIMD, load the chunks ahead, form what hangs on no state, (W * Q K^T)^T dH and (D dH)^T Q, one chunk ahead, and
 // store du.  Two barriers a chunk: du is there, the next state is there.
+// Time parts as the walk's: a first launch (LOCAL) takes all parts but a sequence's first one from their ends to their
+// beginnings, from a zero state and, without rows of values, from the identity's rows; the second each from its own
+// (16384 bf16 tokens x 8 heads of 128 x 128: 1046 us in one part, in nine 127 and 164 with a join of 26-49 between).
 // Bound by the chain, like the walk: 206-224 us for 8 x 2048 bf16 tokens x 16 heads of 128 x 128, 400 MB of states and du written.
-template <class E, int NK, bool VEC>
+template <class E, int NK, bool VEC, bool LOCAL>
 __global__ __launch_bounds__(2 * kThreads, 2) void delta_mirror_kernel(DeltaBwdArgs ba) {
   using raw = typename ET<E>::raw;
   using L = MirrorLds<E, NK>;
@@ -236,10 +239,16 @@ __global__ __launch_bounds__(2 * kThreads, 2) void delta_mirror_kernel(DeltaBwdA
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
   const int lane = lane_id(), g = lane >> 4, n = lane & 15;
   const uint32_t at = xcd_order(blockIdx.x, gridDim.x);
-  const int pt = static_cast<int>(at % a.PT), h = static_cast<int>(at / a.PT % a.H), b = static_cast<int>(at / a.PT / a.H);
+  const int tiles = LOCAL ? a.PT + a.NT : a.PT, parts = LOCAL ? a.parts - 1 : a.parts;
+  const int pt = static_cast<int>(at % tiles), turn = static_cast<int>(at / tiles % parts);  // (the last part is the first in turn)
+  const int h = static_cast<int>(at / tiles / parts % a.H), b = static_cast<int>(at / tiles / parts / a.H);
+  const bool map = LOCAL && pt >= a.PT;  // rows of the identity
+  if (map && turn == 0) return;
   const int64_t len = delta_length(a, b);
-  const int col0 = pt * kDCols, p0 = col0 + 16 * w, gi = h / (a.H / a.G);
-  const int chunks = static_cast<int>((len + kDTokens - 1) / kDTokens);
+  const int col0 = (map ? pt - a.PT : pt) * kDCols, p0 = col0 + 16 * w, gi = h / (a.H / a.G), prows = map ? a.N : a.P;
+  const int part = a.parts - 1 - turn, first = part * a.part_chunks, have = static_cast<int>((len + kDTokens - 1) / kDTokens);
+  const int chunks = have < first + a.part_chunks ? (have > first ? have : first) : first + a.part_chunks;  // this part's end
+  const int64_t all = static_cast<int64_t>(a.B) * a.H;
   const int64_t head = static_cast<int64_t>(b) * a.H + h, cells = static_cast<int64_t>(a.P) * a.N, row = static_cast<int64_t>(a.H) * a.P;
   const char* work = a.work + head * a.C * delta_chunk_bytes(3);
   f32x4* zf = reinterpret_cast<f32x4*>(lds + L::z) + w * 256 + lane;
@@ -251,30 +260,42 @@ __global__ __launch_bounds__(2 * kThreads, 2) void delta_mirror_kernel(DeltaBwdA
     f32x4 st[NT];
 #pragma unroll
     for (int i = 0; i < NT; ++i) st[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (ba.dmemory != nullptr) state_add<NT>(st, ba.dmemory + head * cells, p0, a.P, a.N, 1.f);
+    if (map) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) st[i][r] = p0 + n == 16 * i + 4 * g + r && p0 + n < a.N ? 1.f : 0.f;
+      }
+    } else if (turn > 0 && !LOCAL) {
+      state_add<NT>(st, a.part_state + ((turn - 1) * all + head) * cells, p0, a.P, a.N, 1.f);
+    } else if (turn == 0 && ba.dmemory != nullptr) {
+      state_add<NT>(st, ba.dmemory + head * cells, p0, a.P, a.N, 1.f);
+    }
     B8 tf[kDFrags][3], gp[S][3], kr[2][4][NI];
     auto row_keys = [&](const uint16_t* from, int s) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) row_parts_t<KT, NI>(from, L::kpart, 16 * t, 32 * s, kr[s & 1][t]);
     };
     auto keep_state = [&](int c) {  // (before the first chunk: behind the last value row, where nothing is stored)
+      if constexpr (LOCAL) return;
 #pragma unroll
       for (int s = 0; s < S; ++s)
-        state_out<VEC>(st, 2 * s, ba.gstates + ((static_cast<int64_t>(b) * a.C + (c < 0 ? 0 : c)) * a.H + h) * cells, c < 0 ? a.P : p0, a.P, a.N);
+        state_out<VEC>(st, 2 * s, ba.gstates + ((static_cast<int64_t>(b) * a.C + (c < first ? first : c)) * a.H + h) * cells,
+                       c < first ? a.P : p0, a.P, a.N);
     };
 #pragma unroll
     for (int s = 0; s < S; ++s) split2<3>(st[2 * s], st[2 * s + 1], gp[s]);
-    if (chunks > 0) {
+    if (chunks > first) {
       stored_triangle<3>(reinterpret_cast<const uint16_t*>(work + (chunks - 1) * delta_chunk_bytes(3)), tf, lane);
       keep_state(chunks - 1);
     }
     __syncthreads();
     __syncthreads();
-    if (chunks > 0) row_keys(kt + ((chunks - 1) & 1) * NI * L::kpart, 0);
-    for (int c = chunks - 1; c >= 0; --c) {
+    if (chunks > first) row_keys(kt + ((chunks - 1) & 1) * NI * L::kpart, 0);
+    for (int c = chunks - 1; c >= first; --c) {
       const uint16_t* kc = kt + (c & 1) * NI * L::kpart;
       const float* scc = sc + (c & 1) * L::SCAL;
-      const int next = c > 0 ? c - 1 : 0;
+      const int next = c > first ? c - 1 : first;
       f32x4 z[4], z0[4];
       float4 e[4];
 #pragma unroll
@@ -303,8 +324,10 @@ __global__ __launch_bounds__(2 * kThreads, 2) void delta_mirror_kernel(DeltaBwdA
         for (int s = 0; s < 2; ++s) split2<3>(z[2 * s], z[2 * s + 1], zp[s]);
         mma_triangle<3, false, true>(tf, zp, du);
       }
+      if constexpr (!LOCAL) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) uf[64 * t] = du[t];
+        for (int t = 0; t < 4; ++t) uf[64 * t] = du[t];
+      }
       B8 kf[2][2][2][NI];  // [pair & 1][step][tile of the pair]
       auto pair_keys = [&](int j) {
 #pragma unroll
@@ -351,27 +374,29 @@ __global__ __launch_bounds__(2 * kThreads, 2) void delta_mirror_kernel(DeltaBwdA
       row_keys(kt + (next & 1) * NI * L::kpart, 0);  // (there since the chunk's first barrier)
       __syncthreads();
     }
-    state_store<NT>(st, ba.dm + head * cells, p0, a.P, a.N);
+    if (map) state_store<NT>(st, a.part_map + (turn * all + head) * a.N * a.N, p0, a.N, a.N);
+    else if (LOCAL) state_store<NT>(st, a.part_state + (turn * all + head) * cells, p0, a.P, a.N);
+    else if (part == 0) state_store<NT>(st, ba.dm + head * cells, p0, a.P, a.N);
   } else {
     const int tid = static_cast<int>(threadIdx.x) - kThreads;
     const raw* kp = static_cast<const raw*>(a.keys) + b * a.kb + static_cast<int64_t>(gi) * a.N;
     const raw* qp = static_cast<const raw*>(a.queries) + b * a.qb + static_cast<int64_t>(gi) * a.N;
-    const raw* vp = static_cast<const raw*>(ba.dhidden) + b * a.T * row + static_cast<int64_t>(h) * a.P + col0;
+    const raw* vp = static_cast<const raw*>(ba.dhidden) + b * a.T * row + static_cast<int64_t>(h) * a.P + (map ? 0 : col0);
     TileLoad<E, KT, BF16, VEC, kDTokens, NK, kThreads> kl;
     TileLoad<E, QT, BF16, VEC, kDTokens, NK, kThreads> ql;
     TileLoad<E, VT, E, VEC, kDTokens, kDCols, kThreads> vl;
     kl.init(a.kt, a.N, tid);
     ql.init(a.qt, a.N, tid);
-    vl.init(row, a.P - col0 < kDCols ? a.P - col0 : kDCols, tid);
+    vl.init(row, prows - col0 < kDCols ? prows - col0 : kDCols, tid);
     float sreg = 0.f, warm = 0.f;
     B8 pf[kDFrags][3];
     auto fetch = [&](int want) {  // (before the first chunk it is loaded again)
-      const int c = want > 0 ? want : 0;
+      const int c = want > first ? want : first;
       const int64_t t0 = static_cast<int64_t>(c) * kDTokens;
       sreg = reinterpret_cast<const float*>(work + c * delta_chunk_bytes(3) + 6 * kDFrags * kDFragElems * 2)[tid < 192 ? tid : 0];
       kl.load(kp + t0 * a.kt, len - t0, tid);
       ql.load(qp + t0 * a.qt, len - t0, tid);
-      vl.load(vp + t0 * row, len - t0, tid);
+      vl.load(vp + t0 * row, map ? 0 : len - t0, tid);  // (a map's rows have no values)
     };
     auto place = [&](int c) {
       store_parts<KT, NI, E>(kl, kt + (c & 1) * NI * L::kpart, L::kpart, kDTokens, tid);
@@ -380,13 +405,13 @@ __global__ __launch_bounds__(2 * kThreads, 2) void delta_mirror_kernel(DeltaBwdA
       if (tid < 192) sc[(c & 1) * L::SCAL + tid] = sreg;
     };
     auto weights = [&](int want) {
-      stored_triangle<3>(reinterpret_cast<const uint16_t*>(work + (want > 0 ? want : 0) * delta_chunk_bytes(3)) + 3 * kDFrags * kDFragElems, pf, lane);
+      stored_triangle<3>(reinterpret_cast<const uint16_t*>(work + (want > first ? want : first) * delta_chunk_bytes(3)) + 3 * kDFrags * kDFragElems, pf, lane);
     };
     // One word of every line of a later chunk's matrices, so that they lie in the L2 when they are called for.
     auto warm_up = [&](int want) {
       asm volatile("" ::"v"(warm));
       constexpr int lines = static_cast<int>(delta_chunk_bytes(3) / 128);
-      for (int i = tid; i < lines; i += kThreads) warm = *reinterpret_cast<const float*>(work + (want > 0 ? want : 0) * delta_chunk_bytes(3) + 128 * i);
+      for (int i = tid; i < lines; i += kThreads) warm = *reinterpret_cast<const float*>(work + (want > first ? want : first) * delta_chunk_bytes(3) + 128 * i);
     };
     f32x4 cc[NT];
     // What hangs on no state: (W * Q K^T)^T dH for the state waves, (D dH)^T Q into cc.
@@ -419,29 +444,31 @@ __global__ __launch_bounds__(2 * kThreads, 2) void delta_mirror_kernel(DeltaBwdA
         mma_many<3, true>(qf, dp, cc);
       }
     };
-    if (chunks > 0) {
+    if (chunks > first) {
       fetch(chunks - 1);
       weights(chunks - 1);
       place(chunks - 1);
       fetch(chunks - 2);
     }
     __syncthreads();
-    if (chunks > 0) ahead(chunks - 1);
+    if (chunks > first) ahead(chunks - 1);
     __syncthreads();
-    for (int c = chunks - 1; c >= 0; --c) {
+    for (int c = chunks - 1; c >= first; --c) {
       const int64_t t0 = static_cast<int64_t>(c) * kDTokens;
 #pragma unroll
       for (int i = 0; i < NT; ++i) cf[64 * i] = cc[i];
       weights(c - 1);  // (loads are dealt to both halves of a chunk)
-      if (c > 0) place(c - 1);
+      if (c > first) place(c - 1);
       warm_up(c - 3);
       __syncthreads();
-      const __amdgpu_buffer_rsrc_t to = make_rsrc(ba.du + (b * a.T + t0) * row + static_cast<int64_t>(h) * a.P, 0x7ffffff0u);
-      f32x4 du[4];
+      if constexpr (!LOCAL) {
+        const __amdgpu_buffer_rsrc_t to = make_rsrc(ba.du + (b * a.T + t0) * row + static_cast<int64_t>(h) * a.P, 0x7ffffff0u);
+        f32x4 du[4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) du[t] = uf[64 * t];
-      rows_out<VEC>(du, to, static_cast<int>(row) * 4, len - t0, p0, a.P);
-      if (c > 0) ahead(c - 1);
+        for (int t = 0; t < 4; ++t) du[t] = uf[64 * t];
+        rows_out<VEC>(du, to, static_cast<int>(row) * 4, len - t0, p0, a.P);
+      }
+      if (c > first) ahead(c - 1);
       fetch(c - 2);
       __syncthreads();
     }
@@ -941,7 +968,8 @@ int share_count(int64_t B, int64_t C, int64_t H, int64_t G) {
 }
 
 struct Work {
-  int64_t chunks, states, du, part, bytes;
+  int64_t chunks, states, du, part, part_state, part_map, part_chunks, bytes;
+  int parts;
 };
 Work work_of(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G, int64_t N) {
   const int64_t C = (T + kDTokens - 1) / kDTokens, shares = share_count(B, C, H, G);
@@ -950,7 +978,11 @@ Work work_of(int64_t B, int64_t T, int64_t H, int64_t P, int64_t G, int64_t N) {
   w.states = up16(B * H * C * delta_chunk_bytes(3));
   w.du = w.states + up16(B * C * H * P * N * 4);
   w.part = w.du + up16(B * T * H * P * 4);
-  w.bytes = w.part + (shares > 1 ? 2 * shares * B * T * G * N * 4 : 0);
+  w.part_state = w.part + up16(shares > 1 ? 2 * shares * B * T * G * N * 4 : 0);
+  // (Of any type: what takes no parts needs less.)
+  w.parts = delta_time_parts(B * H, P, N, C, GRM_HIP_BF16, true, &w.part_chunks);
+  w.part_map = w.part_state + up16((w.parts - 1) * B * H * P * N * 4);
+  w.bytes = w.part_map + (w.parts - 1) * B * H * N * N * 4;
   return w;
 }
 
@@ -993,12 +1025,17 @@ extern "C" int grm_hip_delta_scan_bwd(const grm_hip_delta_args* u, const float* 
   a.f.memory = nullptr;
   a.dhidden = grad_hidden; a.dmemory = grad_memory_out;
   a.dk = grad_keys; a.dv = grad_values; a.dq = grad_queries; a.ds = grad_strengths; a.dd = grad_log_decays; a.dm = grad_memory;
+  int64_t part_chunks = 0;
   if (u->seq_len > 0) {
     a.gstates = reinterpret_cast<float*>(a.f.work + wk.states);
     a.du = reinterpret_cast<float*>(a.f.work + wk.du);
     a.shares = share_count(u->batch, a.f.C, u->heads, u->groups);
     a.per = static_cast<int>((u->heads / u->groups + a.shares - 1) / a.shares);
     a.part = a.shares > 1 ? reinterpret_cast<float*>(a.f.work + wk.part) : nullptr;
+    a.f.parts = delta_time_parts(u->batch * u->heads, u->value_dim, u->key_dim, a.f.C, u->dtype, true, &part_chunks);
+    a.f.part_chunks = static_cast<int>(part_chunks);
+    a.f.part_state = reinterpret_cast<float*>(a.f.work + wk.part_state);
+    a.f.part_map = reinterpret_cast<float*>(a.f.work + wk.part_map);
     if (int rc = launch_delta_prep(a.f, u->dtype, true, hs, what)) return rc;
   }
   auto set_lds = [&](const void* kernel, size_t bytes) {
@@ -1013,14 +1050,22 @@ extern "C" int grm_hip_delta_scan_bwd(const grm_hip_delta_args* u, const float* 
     constexpr int NK = decltype(nk)::value;
     constexpr bool VEC = decltype(vec)::value;
     {
-      auto go = [&](auto kernel, int threads, size_t lds) {
-        if ((rc = set_lds(reinterpret_cast<const void*>(kernel), lds)) != GRM_HIP_OK) return;
-        kernel<<<dim3(static_cast<uint32_t>(a.f.B) * a.f.H * a.f.PT), dim3(threads), lds, hs>>>(a);
+      auto go = [&](auto kernel, int64_t tiles, int threads, size_t lds) {
+        if (rc != GRM_HIP_OK || (rc = set_lds(reinterpret_cast<const void*>(kernel), lds)) != GRM_HIP_OK) return;
+        kernel<<<dim3(static_cast<uint32_t>(a.f.B) * a.f.H * static_cast<uint32_t>(tiles)), dim3(threads), lds, hs>>>(a);
+        rc = check_launch(what);
       };
-      if constexpr (MirrorLds<E, NK>::fits) go(delta_mirror_kernel<E, NK, VEC>, 2 * kThreads, MirrorLds<E, NK>::bytes);
-      else go(delta_reverse_kernel<E, NK, VEC>, kThreads, ReverseLds<E, NK>::bytes);
-      if (rc != GRM_HIP_OK) return;
-      if ((rc = check_launch(what)) != GRM_HIP_OK || a.f.C == 0) return;
+      if constexpr (MirrorLds<E, NK>::fits) {
+        constexpr size_t lds = MirrorLds<E, NK>::bytes;
+        if (a.f.parts > 1) {
+          go(delta_mirror_kernel<E, NK, VEC, true>, (a.f.PT + a.f.NT) * (a.f.parts - 1), 2 * kThreads, lds);
+          if (rc == GRM_HIP_OK) rc = launch_delta_join(a.f, hs, what);
+        }
+        go(delta_mirror_kernel<E, NK, VEC, false>, a.f.PT * a.f.parts, 2 * kThreads, lds);
+      } else {
+        go(delta_reverse_kernel<E, NK, VEC>, a.f.PT, kThreads, ReverseLds<E, NK>::bytes);
+      }
+      if (rc != GRM_HIP_OK || a.f.C == 0) return;
     }
     auto kernel = delta_grad_kernel<E, NK, VEC>;
     constexpr size_t lds = GradLds<E, NK>::bytes;

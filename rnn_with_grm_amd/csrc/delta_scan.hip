@@ -1062,30 +1062,12 @@ int set_lds(const void* kernel, size_t bytes, const char* what) {
 int out_parts(int dtype) { return dtype == GRM_HIP_F32 ? 3 : 2; }
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 
-// Time parts of a sequence.  256 CUs hold a workgroup each; a part costs its chunks once more, for the value rows and for
-// the N rows of its map, so parts are taken where they shorten the longest line of chunks behind each other (in quarters of
-// a chunk's time; one of the first walk, with two chains a SIMD, takes five, a launch and a join a few chunks).  32768 bf16
-// tokens x 16 heads of 128 x 128: 1900 us in one part, 650 in eight.
-int time_parts(int64_t seqs, int64_t P, int64_t N, int64_t C, int dtype, int64_t* part_chunks) {
-  *part_chunks = C;
-  if ((dtype != GRM_HIP_BF16 && N > 64) || seqs > 4096) return 1;  // (delta_walk_kernel takes whole sequences)
-  const int64_t PT = (P + kDCols - 1) / kDCols, NT = (N + kDCols - 1) / kDCols;
-  auto rounds = [](int64_t wgs) { return (wgs + 255) / 256; };
-  int64_t best = 4 * C * rounds(seqs * PT), parts = 1;
-  for (int64_t r = 2; r <= 64 && r <= C / 4; ++r) {
-    const int64_t per = (C + r - 1) / r, n = (C + per - 1) / per;
-    const int64_t cost = per * (4 * rounds(seqs * PT * n) + 5 * rounds(seqs * ((PT + NT + 1) / 2) * (n - 1))) + 8 * n + 24;
-    if (cost < best) best = cost, parts = n, *part_chunks = per;
-  }
-  return static_cast<int>(parts);
-}
-
 struct Work {
   int64_t states, maps, bytes;
 };
 Work work_of(int64_t B, int64_t T, int64_t H, int64_t P, int64_t N, int dtype, int* parts, int64_t* part_chunks) {
   const int64_t C = (T + kDTokens - 1) / kDTokens;
-  *parts = time_parts(B * H, P, N, C, dtype, part_chunks);
+  *parts = delta_time_parts(B * H, P, N, C, dtype, false, part_chunks);
   Work w{};
   w.states = up16(B * H * C * delta_chunk_bytes(out_parts(dtype)));
   w.maps = w.states + up16((*parts - 1) * B * H * P * N * 4);
@@ -1094,6 +1076,25 @@ Work work_of(int64_t B, int64_t T, int64_t H, int64_t P, int64_t N, int dtype, i
 }
 
 }  // namespace
+
+// Time parts of a sequence.  256 CUs hold a workgroup each; a part costs its chunks once more, for the value rows and for
+// the N rows of its map, so parts are taken where they shorten the longest line of chunks behind each other (in quarters of
+// a chunk's time; one of the first walk, with two chains a SIMD, takes five, of the mirror's four, a launch and a join a
+// few chunks).  32768 bf16 tokens x 16 heads of 128 x 128: 1900 us in one part, 650 in eight.
+int delta_time_parts(int64_t seqs, int64_t P, int64_t N, int64_t C, int dtype, bool mirror, int64_t* part_chunks) {
+  *part_chunks = C;
+  if ((dtype != GRM_HIP_BF16 && N > 64) || seqs > 4096) return 1;  // (delta_walk_kernel and delta_reverse_kernel take whole sequences)
+  const int64_t PT = (P + kDCols - 1) / kDCols, NT = (N + kDCols - 1) / kDCols;
+  auto rounds = [](int64_t wgs) { return (wgs + 255) / 256; };
+  int64_t best = 4 * C * rounds(seqs * PT), parts = 1;
+  for (int64_t r = 2; r <= 64 && r <= C / 4; ++r) {
+    const int64_t per = (C + r - 1) / r, n = (C + per - 1) / per;
+    const int64_t first = mirror ? 4 * rounds(seqs * (PT + NT) * (n - 1)) : 5 * rounds(seqs * ((PT + NT + 1) / 2) * (n - 1));
+    const int64_t cost = per * (4 * rounds(seqs * PT * n) + first) + 8 * n + 24;
+    if (cost < best) best = cost, parts = n, *part_chunks = per;
+  }
+  return static_cast<int>(parts);
+}
 
 int delta_check(const grm_hip_delta_args* u, const char* what, bool step) {
   auto bad = [&](const char* why) {
@@ -1188,6 +1189,14 @@ int launch_delta_prep(const DeltaArgs& a, int dtype, bool back, hipStream_t stre
   return rc;
 }
 
+int launch_delta_join(const DeltaArgs& a, hipStream_t stream, const char* what) {
+  if (a.parts <= 2) return GRM_HIP_OK;  // (the first part's end is the second one's start)
+  const dim3 grid(static_cast<uint32_t>(a.B) * a.H * ((a.P + 15) / 16));
+  if (a.N <= 64) delta_join_kernel<64><<<grid, dim3(128), 0, stream>>>(a);
+  else delta_join_kernel<128><<<grid, dim3(256), 0, stream>>>(a);
+  return check_launch(what);
+}
+
 }  // namespace grmhip
 
 using namespace grmhip;
@@ -1248,10 +1257,7 @@ extern "C" int grm_hip_delta_scan_fwd(const grm_hip_delta_args* u, void* hidden,
       if (a.parts > 1) {
         go(delta_pair_kernel<E, NK, V, false, true>, heads * ((a.PT + a.NT + 1) / 2) * (a.parts - 1), LocalLds<E, NK>::bytes);
         if (rc != GRM_HIP_OK) return;
-        if (a.parts > 2) {
-          delta_join_kernel<NK><<<dim3(heads * ((a.P + 15) / 16)), dim3(2 * NK), 0, static_cast<hipStream_t>(stream)>>>(a);
-          if ((rc = check_launch(what)) != GRM_HIP_OK) return;
-        }
+        if ((rc = launch_delta_join(a, static_cast<hipStream_t>(stream), what)) != GRM_HIP_OK) return;
       }
       if (states != nullptr) go(delta_pair_kernel<E, NK, V, true, false>, heads * a.PT * a.parts, PairLds<E, NK>::bytes);
       else go(delta_pair_kernel<E, NK, V, false, false>, heads * a.PT * a.parts, PairLds<E, NK>::bytes);

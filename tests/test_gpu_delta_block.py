@@ -121,11 +121,12 @@ def test_long_sequences_of_few_heads(dev, dtype, P1, N1):
         assert (a - b).norm() <= bound * b.norm()
 
 
-def test_captured_gradients(dev):
-    """Forward and backward of the delta rule in a graph, with leaves of its own, replayed between eager work."""
-    x, beta, decay, _ = inputs(dev, 2, 200, torch.bfloat16)
+@pytest.mark.parametrize("T", [200, 3000])
+def test_captured_gradients(dev, T):
+    """Forward and backward of the delta rule in a graph, with leaves of its own, replayed between eager work; in time parts too."""
+    x, beta, decay, _ = inputs(dev, 2, T, torch.bfloat16)
     rows = x.clone()
-    seed = torch.randn(2, 200, H, P, device=dev).bfloat16()
+    seed = torch.randn(2, T, H, P, device=dev).bfloat16()
 
     def work():
         v, k, q = rows.split((H * P, G * N, G * N), -1)
