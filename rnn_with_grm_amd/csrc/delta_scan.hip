@@ -269,6 +269,14 @@ __global__ __launch_bounds__(kPrepThreads, 4) void delta_prep_kernel(DeltaArgs a
   }
 }
 
+// Zeros for the tokens (columns) from `rows` on: a query of zeros alone gives NaN of a state that is no number, and what is
+// NaN from a live token on stays so to the chunk's end.
+__device__ __forceinline__ void clear_rows(f32x4 (&o)[4], int64_t rows) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+    if (16 * t + (lane_id() & 15) >= rows) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+}
+
 // LDS of a walk: keys and queries as their parts, values, the chunk's scalars.
 template <class E, int NK>
 struct WalkLds {
@@ -459,6 +467,7 @@ __global__ __launch_bounds__(kWalkThreads, 1) void delta_walk_kernel(DeltaArgs a
           if (16 * t + n >= f) o[t][r] = __builtin_nanf("");
       }
     }
+    if (t0 + kDTokens > len) clear_rows(o, len - t0);
     {
       const int p = p0 + 4 * g, row = a.H * a.P * static_cast<int>(sizeof(raw));
       const int64_t left = a.T - t0;
@@ -866,6 +875,7 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
             if (16 * t + n >= f) o[t][r] = __builtin_nanf("");
         }
       }
+      if (t0 + kDTokens > len) clear_rows(o, len - t0);
       const int64_t left = a.T - t0;
       const __amdgpu_buffer_rsrc_t to =
           make_rsrc(static_cast<raw*>(a.hidden) + ((static_cast<int64_t>(b) * a.T + t0) * a.H + h) * a.P, 0x7ffffff0u);

@@ -1,0 +1,59 @@
+"""The delta rule behind the lengths of a padded batch, also where live tokens, states or gradients hold values that are no
+numbers.  What is compared here has to be equal: zeros, states that nothing moves, and rows that nothing reaches."""
+
+import pytest
+import torch
+
+from rnn_with_grm_amd import cuda_ops
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+NAMES = ("keys", "values", "queries", "strengths", "log_decays", "memory")
+
+
+def inputs(dev, B, T, H, P, G, N, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    unit = lambda *s: 0.99 * torch.nn.functional.normalize(r(*s), dim=-1)  # noqa: E731
+    x = [unit(B, T, G, N).to(dtype), r(B, T, H, P).to(dtype), unit(B, T, G, N).to(dtype), torch.rand(B, T, H, generator=g).to(dtype),
+         -0.05 * torch.rand(B, T, H, generator=g), r(B, H, P, N)]
+    return dict(zip(NAMES, (t.to(dev) for t in x)))
+
+
+def run(x, n):
+    return cuda_ops.cuda_delta_scan(*(x[k] for k in NAMES), lengths=n)
+
+
+# Where a bad value of sequence 0 goes, and what is NaN of it from its token on: a column of head 1, a row, head 1, or the group.
+PLACES = [("values", (1, 5), "column"), ("queries", (0, 3), "row"), ("keys", (0, 3), "group"), ("strengths", (1,), "head"),
+          ("log_decays", (1,), "head"), ("memory", (1, 5, 3), "column")]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,P,N,lengths,at", [(20, 40, 32, (10, 20), 5), (150, 40, 128, (100, 7), 77), (150, 37, 65, (100, 0), 70),
+                                              (70, 64, 64, (65, 64), 64), (3000, 24, 48, (1500, 2990), 1400)])
+def test_rows_behind_a_length_are_zeros(dev, T, P, N, lengths, at, dtype):
+    x = inputs(dev, 2, T, 2, P, 1, N, dtype, seed=T)
+    n = torch.tensor(lengths, device=dev)
+    hidden, memory = run(x, n)
+    live = torch.arange(T, device=dev) < n[:, None]
+    assert not hidden[~live].any()
+    for bad in (float("inf"), float("nan")):
+        for name, where, what in PLACES:
+            y = dict(x, **{name: x[name].clone()})
+            y[name][(0, *where) if name == "memory" else (0, at, *where)] = bad
+            h, m = run(y, n)
+            assert torch.equal(h[~live], torch.zeros_like(h[~live])), (name, bad)
+            odd, gone = torch.zeros_like(h, dtype=torch.bool), torch.zeros_like(m, dtype=torch.bool)
+            start = 0 if name == "memory" else at
+            if what == "column":
+                odd[0, start:, 1, 5], gone[0, 1, 5] = True, True
+            elif what == "row":
+                odd[0, at] = True
+            elif what == "head":
+                odd[0, start:, 1], gone[0, 1] = True, True
+            else:
+                odd[0, start:], gone[0] = True, True
+            odd &= live[..., None, None]
+            assert torch.equal(torch.isnan(h), odd) and torch.equal(torch.isnan(m), gone), (name, bad)
+            assert torch.equal(h[~odd], hidden[~odd]) and torch.equal(m[~gone], memory[~gone]), (name, bad)
