@@ -906,6 +906,10 @@ __global__ __launch_bounds__(kGradThreads, kGradWaves) void delta_grad_kernel(De
     }
   }
   if (tok < all) {
+    if (!in) {  // (a state that is no number makes NaN of the zeros that stand for these rows)
+#pragma unroll
+      for (int i = 0; i < NT; ++i) dk[i] = dq[i] = zero;
+    }
     const int64_t to = ((b * a.T + t0 + tok) * a.G + gi) * a.N;
     const int64_t plane = static_cast<int64_t>(a.B) * a.T * a.G * a.N;
     const bool whole = (a.N & 3) == 0;

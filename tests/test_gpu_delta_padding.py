@@ -57,3 +57,34 @@ def test_rows_behind_a_length_are_zeros(dev, T, P, N, lengths, at, dtype):
             odd &= live[..., None, None]
             assert torch.equal(torch.isnan(h), odd) and torch.equal(torch.isnan(m), gone), (name, bad)
             assert torch.equal(h[~odd], hidden[~odd]) and torch.equal(m[~gone], memory[~gone]), (name, bad)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,P,N,lengths,at", [(20, 40, 32, (10, 20), 5), (150, 40, 128, (100, 7), 77), (150, 37, 65, (100, 0), 70),
+                                              (3000, 24, 48, (1500, 2990), 1400)])
+def test_gradients_behind_a_length_are_zeros(dev, T, P, N, lengths, at, dtype):
+    """Also where a live value, state or gradient is no number; the other sequence's gradients are what they were."""
+    x = inputs(dev, 2, T, 2, P, 1, N, dtype, seed=T)
+    n = torch.tensor(lengths, device=dev)
+    live = torch.arange(T, device=dev) < n[:, None]
+    g = torch.Generator().manual_seed(1)
+    seeds = [torch.randn(2, T, 2, P, generator=g).to(dtype).to(dev), torch.randn(2, 2, P, N, generator=g).to(dev)]
+
+    def gradients(x, seeds):
+        leaves = [x[k].detach().requires_grad_() for k in NAMES]
+        return torch.autograd.grad(cuda_ops.cuda_delta_scan(*leaves, lengths=n), leaves, seeds)
+
+    want = gradients(x, seeds)
+    for bad in (float("inf"), float("nan")):
+        for name, where, _ in PLACES + [("hidden", (1, 5), ""), ("memory_out", (1, 5, 3), "")]:
+            y, s = dict(x), list(seeds)
+            if name in y:
+                to = y[name] = y[name].clone()
+            else:
+                i = ("hidden", "memory_out").index(name)
+                to = s[i] = s[i].clone()
+            to[(0, *where) if to.shape == x["memory"].shape else (0, at, *where)] = bad
+            for k, a, b in zip(NAMES, gradients(y, s), want):
+                if k != "memory":
+                    assert torch.equal(a[~live], torch.zeros_like(a[~live])), (name, bad, k)
+                assert torch.equal(a[1], b[1]), (name, bad, k)
