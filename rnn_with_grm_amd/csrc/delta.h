@@ -49,6 +49,7 @@ struct DeltaArgs {
   int64_t T;
   int B, H, P, G, N, C, PT;
   int parts, part_chunks, NT;           // time parts, their chunks, tiles of 64 rows of a part's map
+  int mirror;                           // parts are numbered from the last one
   int s_f32, d_f32, vec;
 };
 

@@ -1038,6 +1038,7 @@ extern "C" int grm_hip_delta_scan_bwd(const grm_hip_delta_args* u, const float* 
     a.part = a.shares > 1 ? reinterpret_cast<float*>(a.f.work + wk.part) : nullptr;
     a.f.parts = delta_time_parts(u->batch * u->heads, u->value_dim, u->key_dim, a.f.C, u->dtype, true, &part_chunks);
     a.f.part_chunks = static_cast<int>(part_chunks);
+    a.f.mirror = 1;
     a.f.part_state = reinterpret_cast<float*>(a.f.work + wk.part_state);
     a.f.part_map = reinterpret_cast<float*>(a.f.work + wk.part_map);
     if (int rc = launch_delta_prep(a.f, u->dtype, true, hs, what)) return rc;

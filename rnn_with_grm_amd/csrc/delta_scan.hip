@@ -910,6 +910,8 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
 // state D (of the first, of the sequence's own state: M_1).  A workgroup takes 16 value rows through all parts; each wave
 // holds 32 of the keys, and they hand each other the state's fragments.  The map hangs on no state and is loaded a part
 // ahead.  A chain of loads: 26 us for 7 parts of 16 heads of 128 x 128 (155 with a wave for all keys and no loads ahead).
+// A part behind a sequence's length hands its state on as it is: the product with the identity would make NaN of a row with
+// an infinity, and of numbers that round to one in 16 bits.
 template <int NK>
 __global__ __launch_bounds__(2 * NK) void delta_join_kernel(DeltaArgs a) {
   constexpr int S = NK / 32;
@@ -946,7 +948,17 @@ __global__ __launch_bounds__(2 * NK) void delta_join_kernel(DeltaArgs a) {
     for (int r = 0; r < 4; ++r) st[i][r] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rsrc(0), where(i, r), 0, 0));
   }
   fetch(1);
+  const int have = static_cast<int>((delta_length(a, static_cast<int>(head / a.H)) + kDTokens - 1) / kDTokens);
   for (int p = 1; p < a.parts - 1; ++p) {
+    if ((a.mirror ? a.parts - 1 - p : p) * a.part_chunks >= have) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(st[i][r]), rsrc(p), where(i, r), 0, 0);
+      }
+      fetch(p + 1);
+      continue;
+    }
     B8 sp[3], f[2][S][3];
     split2<3>(st[0], st[1], sp);
 #pragma unroll

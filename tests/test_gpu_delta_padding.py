@@ -88,3 +88,26 @@ def test_gradients_behind_a_length_are_zeros(dev, T, P, N, lengths, at, dtype):
                 if k != "memory":
                     assert torch.equal(a[~live], torch.zeros_like(a[~live])), (name, bad, k)
                 assert torch.equal(a[1], b[1]), (name, bad, k)
+
+
+@pytest.mark.parametrize("T", [100, 3000])
+def test_a_state_that_no_token_moves(dev, T):
+    """An empty sequence hands its state on as it is, in time parts too: infinities, NaN, the largest and the smallest numbers."""
+    x = inputs(dev, 3, T, 1, 40, 1, 48, torch.bfloat16, seed=3)
+    odd = torch.tensor([float("inf"), float("-inf"), float("nan"), 3.4028235e38, 1e-38, 1e-45, 1.0000001], device=dev)
+    x["memory"][0, 0, ::6, 3] = odd
+    x["memory"][2, 0, 3] = odd[3]
+    n = torch.tensor([0, T // 2, -4], device=dev)
+    hidden, memory = run(x, n)
+    assert not hidden[0].any() and not hidden[2].any()
+    for b in (0, 2):
+        assert torch.equal(memory[b].view(torch.int32), x["memory"][b].view(torch.int32))
+    assert torch.isfinite(memory[1]).all()
+    # its gradient likewise
+    leaves = [x[k].detach().requires_grad_() for k in NAMES]
+    seed = torch.ones_like(memory)
+    seed[0, 0, ::6, 3] = odd
+    grads = torch.autograd.grad(cuda_ops.cuda_delta_scan(*leaves, lengths=n)[1], leaves, seed)
+    for b in (0, 2):
+        assert torch.equal(grads[5][b].view(torch.int32), seed[b].view(torch.int32))
+        assert not any(t[b].any() for t in grads[:5])
