@@ -77,7 +77,7 @@ def _stale(target: Path, deps: List[Path]) -> bool:
 def _headers() -> List[Path]:
     return [INCLUDE / "grm_hip.h", CSRC / "grm_hip_common.h", CSRC / "chunk_scan.h", CSRC / "chunk_bwd.h",
             CSRC / "f32_tiles.h", CSRC / "route_select.h", CSRC / "retrieve.h", CSRC / "selective.h", CSRC / "delta.h",
-            CSRC / "op_checks.h"]
+            CSRC / "delta_limits.h", CSRC / "op_checks.h"]
 
 
 def build_hip_library(force: bool = True, verbose: bool = False, jobs: Optional[int] = None) -> Path:

@@ -1,6 +1,7 @@
 // The gated delta rule on MI355X: the chunks' inverses and weights, the walk over a sequence's chunks, and the single
 // token.  The mathematics is in delta.h.
 #include "delta.h"
+#include "delta_limits.h"
 
 namespace grmhip {
 namespace {
@@ -1136,25 +1137,14 @@ int delta_check(const grm_hip_delta_args* u, const char* what, bool step) {
     set_error("%s: key_dim must be <= 128, got %lld", what, static_cast<long long>(u->key_dim));
     return GRM_HIP_EUNSUPPORTED;
   }
+  if (const char* limit = delta_limit(u->batch, u->seq_len, u->heads, u->value_dim, u->groups, u->key_dim, step)) {
+    set_error("%s: %s", what, limit);
+    return GRM_HIP_EUNSUPPORTED;
+  }
   const int64_t most = int64_t{1} << 21;
-  if (u->seq_len > (1 << 30)) {
-    set_error("%s: seq_len must be at most 2^30", what);
-    return GRM_HIP_EUNSUPPORTED;
-  }
-  // (One by one first: no product passes 63 bits.)
-  if (u->heads > most || u->value_dim > most || u->groups > most || u->keys_token_stride < 0 ||
-      u->keys_token_stride > most || u->values_token_stride < 0 || u->values_token_stride > most ||
-      u->queries_token_stride < 0 || u->queries_token_stride > most || u->heads * u->value_dim > most ||
-      u->groups * u->key_dim > most) {
+  if (u->keys_token_stride < 0 || u->keys_token_stride > most || u->values_token_stride < 0 || u->values_token_stride > most ||
+      u->queries_token_stride < 0 || u->queries_token_stride > most) {
     set_error("%s: token strides and row widths must be at most 2^21 elements", what);
-    return GRM_HIP_EUNSUPPORTED;
-  }
-  // (A grid dimension has fewer than 2^32 threads, of which a workgroup of a walk and of the gradients has 512, of a token 256.)
-  const int64_t seqs = u->heads * min_i64(u->batch, int64_t{1} << 32), grid = int64_t{1} << 24;
-  const int64_t tiles = (u->value_dim + kDCols - 1) / kDCols, chunks = (u->seq_len + kDTokens - 1) / kDTokens;
-  if (seqs >= grid || (!step && (seqs * tiles >= grid / 2 || seqs * chunks >= grid / 2))) {
-    set_error(step ? "%s: batch * heads must be below 2^24"
-                   : "%s: batch * heads * ceil(value_dim / 64) and batch * heads * ceil(seq_len / 64) must be below 2^23", what);
     return GRM_HIP_EUNSUPPORTED;
   }
   if (u->seq_len > 1 && (u->keys_token_stride < u->groups * u->key_dim || u->queries_token_stride < u->groups * u->key_dim ||

@@ -3,6 +3,7 @@
 // on that device's current stream.  Inputs the kernels do not cover raise; CPU tensors take cuda_ops' PyTorch forms.
 #include <tuple>
 
+#include "delta_limits.h"
 #include "op_checks.h"
 
 namespace grm_delta {
@@ -43,6 +44,8 @@ Delta check_delta(const Tensor& keys, const Tensor& values, const Tensor& querie
   TORCH_CHECK_VALUE(keys.scalar_type() == values.scalar_type() && queries.scalar_type() == values.scalar_type() &&
                         (sdt == dt || sdt == GRM_HIP_F32) && (ddt == dt || ddt == GRM_HIP_F32),
                     op, ": keys, values and queries must share a type, strengths and log_decays have it or float32");
+  const char* limit = grmhip::delta_limit(s.B, s.T, s.H, s.P, s.G, s.N, step);
+  TORCH_CHECK(limit == nullptr, op, ": ", limit == nullptr ? "" : limit);
   check_device(keys, values, op, "keys");
   check_device(queries, values, op, "queries");
   check_device(strengths, values, op, "strengths");
@@ -143,6 +146,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> delta_scan_backward(
   return {gk, gv, gq, gb, gd, gm};
 }
 
+Tensor step(const Delta& s, const Tensor& values, Tensor& memory_out, const char* op) {
+  Tensor hidden = at::empty({s.B, s.H, s.P}, values.options());
+  check_rc(grm_hip_delta_step(&s.args, hidden.data_ptr(), memory_out.data_ptr<float>(), stream_of(values)), op);
+  return hidden;
+}
+
 Tensor delta_step_out(const Tensor& keys, const Tensor& values, const Tensor& queries, const Tensor& strengths,
                       const OptTensor& log_decays, const Tensor& memory, Tensor& memory_out) {
   const char* op = "delta_step";
@@ -152,16 +161,18 @@ Tensor delta_step_out(const Tensor& keys, const Tensor& values, const Tensor& qu
   TORCH_CHECK_VALUE(memory_out.sizes() == memory.sizes() && memory_out.scalar_type() == at::kFloat &&
                         memory_out.is_contiguous() && aligned16(memory_out),
                     op, ": memory_out must be contiguous, 16-byte aligned and match memory");
-  Tensor hidden = at::empty({s.B, s.H, s.P}, values.options());
-  check_rc(grm_hip_delta_step(&s.args, hidden.data_ptr(), memory_out.data_ptr<float>(), stream_of(values)), op);
+  Tensor hidden = step(s, values, memory_out, op);
   written(memory_out);
   return hidden;
 }
 
 std::tuple<Tensor, Tensor> delta_step(const Tensor& keys, const Tensor& values, const Tensor& queries,
                                       const Tensor& strengths, const OptTensor& log_decays, const Tensor& memory) {
+  const char* op = "delta_step";
+  c10::OptionalDeviceGuard guard(values.device());
+  const Delta s = check_delta(keys, values, queries, strengths, log_decays, memory, c10::nullopt, true, op);
   Tensor moved = at::empty(memory.sizes(), memory.options());
-  return {delta_step_out(keys, values, queries, strengths, log_decays, memory, moved), moved};
+  return {step(s, values, moved, op), moved};
 }
 
 // ---------------------------------------------------------------------------
