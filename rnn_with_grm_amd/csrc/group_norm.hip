@@ -1,8 +1,8 @@
 // Group norm of rows (tokens) with their channels last, its activation or activated gate, and the gradients.
 //   n = (x - mean) / sqrt(var + eps) over each group of a row (without centre: x / sqrt(mean x^2 + eps))
 //   y = n w + b;  out = y act(gate), without a gate act(y)
-// Bound by the rows' bytes.  LG lanes hold a group in registers (EPL channels each), so that a row is read once; mean and
-// variance are two sums over registers, float32.  A thread keeps its channels over all rows that its workgroup
+// Bound by the rows' bytes.  LG lanes hold a group in registers (EPL channels each), so that a row is read once; mean
+// (in two steps) and variance are sums over registers, float32.  A thread keeps its channels over all rows that its workgroup
 // walks: weights are loaded once, and their gradients are summed in registers, then over the workgroup in LDS, then over the
 // workgroups by a second launch, always in the same order.  16384 bf16 rows of 16 groups of 128 with a gate: 37 us
 // (201 MB, 5.4 TB/s); gradients 61 (336 MB, 5.5 TB/s) and 4.6 for the sums.
@@ -98,12 +98,17 @@ template <int LG, int EPL, bool VEC>
 __device__ __forceinline__ float normalise(const NormArgs& a, int l, float (&x)[EPL]) {
   const float inv = 1.f / static_cast<float>(a.width);
   if (a.center) {
-    float s = 0.f;
+    // Twice: the first mean is off by a few steps of the values, the second takes out what that left in every difference.  Of
+    // equal values nothing is left: the first differences are a few steps of x each, whose sums are exact.
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) s += x[j];
-    const float mean = group_sum<LG>(s) / static_cast<float>(a.width);  // (rounded once: equal values leave nothing)
+    for (int pass = 0; pass < 2; ++pass) {
+      float s = 0.f;
 #pragma unroll
-    for (int j = 0; j < EPL; ++j) x[j] = channel<LG, VEC>(l, j) < a.width ? x[j] - mean : 0.f;
+      for (int j = 0; j < EPL; ++j) s += x[j];
+      const float mean = group_sum<LG>(s) / static_cast<float>(a.width);
+#pragma unroll
+      for (int j = 0; j < EPL; ++j) x[j] = channel<LG, VEC>(l, j) < a.width ? x[j] - mean : 0.f;
+    }
   }
   float s = 0.f;
 #pragma unroll
