@@ -29,6 +29,7 @@ struct DeltaBwdArgs {
   float* dm;              // [B, H, P, N]
   float* part;            // [2, shares, B, T, G, N] or null: dk and dq of a share of a group's heads
   int shares, per;        // shares of a group's heads, heads of a share
+  int whole;              // four keys' gradients leave in one store
 };
 
 template <class E, int NK>
@@ -912,7 +913,6 @@ __global__ __launch_bounds__(kGradThreads, kGradWaves) void delta_grad_kernel(De
     }
     const int64_t to = ((b * a.T + t0 + tok) * a.G + gi) * a.N;
     const int64_t plane = static_cast<int64_t>(a.B) * a.T * a.G * a.N;
-    const bool whole = (a.N & 3) == 0;
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       const int k = key0 + 16 * i + 4 * g;
@@ -930,7 +930,7 @@ __global__ __launch_bounds__(kGradThreads, kGradWaves) void delta_grad_kernel(De
       } else {
         raw* pk = static_cast<raw*>(ba.dk) + to + k;
         raw* pq = static_cast<raw*>(ba.dq) + to + k;
-        if (whole) {
+        if (ba.whole) {
           store4_raw<E>(pk, dk[i]);
           store4_raw<E>(pq, dq[i]);
         } else {
@@ -1029,6 +1029,7 @@ extern "C" int grm_hip_delta_scan_bwd(const grm_hip_delta_args* u, const float* 
   a.f.memory = nullptr;
   a.dhidden = grad_hidden; a.dmemory = grad_memory_out;
   a.dk = grad_keys; a.dv = grad_values; a.dq = grad_queries; a.ds = grad_strengths; a.dd = grad_log_decays; a.dm = grad_memory;
+  a.whole = (u->key_dim & 3) == 0 && aligned(grad_keys) && aligned(grad_queries);
   int64_t part_chunks = 0;
   if (u->seq_len > 0) {
     a.gstates = reinterpret_cast<float*>(a.f.work + wk.states);
@@ -1050,7 +1051,7 @@ extern "C" int grm_hip_delta_scan_bwd(const grm_hip_delta_args* u, const float* 
     return static_cast<int>(e);
   };
   int rc = GRM_HIP_OK;
-  delta_with_form(u->dtype, a.f.N, a.f.vec != 0 && aligned(grad_hidden), [&](auto e, auto nk, auto vec) {
+  delta_with_form(u->dtype, a.f.N, a.f.vec != 0 && aligned(grad_hidden) && aligned(grad_values), [&](auto e, auto nk, auto vec) {
     using E = decltype(e);
     constexpr int NK = decltype(nk)::value;
     constexpr bool VEC = decltype(vec)::value;
