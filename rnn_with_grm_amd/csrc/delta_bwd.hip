@@ -682,6 +682,8 @@ __global__ __launch_bounds__(kGradThreads, kGradWaves) void delta_grad_kernel(De
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           dv[e] = myb * uv.e[e];
+          // (A float32 product, so that every form rounds it alike: one value's conversion to float16 would take the product in.)
+          if constexpr (!VEC) asm volatile("" : "+v"(dv[e]));
           mu = fmaf(uv.e[e], mv.e[e], mu);
         }
 #pragma unroll
