@@ -31,7 +31,8 @@ PLACES = [("values", (1, 5), "column"), ("queries", (0, 3), "row"), ("keys", (0,
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,P,N,lengths,at", [(20, 40, 32, (10, 20), 5), (150, 40, 128, (100, 7), 77), (150, 37, 65, (100, 0), 70),
-                                              (70, 64, 64, (65, 64), 64), (3000, 24, 48, (1500, 2990), 1400)])
+                                              (70, 64, 64, (65, 64), 64), (3000, 24, 48, (1500, 2990), 1400),
+                                              (3000, 70, 48, (3000, 2990), 700)])
 def test_rows_behind_a_length_are_zeros(dev, T, P, N, lengths, at, dtype):
     x = inputs(dev, 2, T, 2, P, 1, N, dtype, seed=T)
     n = torch.tensor(lengths, device=dev)
@@ -61,7 +62,7 @@ def test_rows_behind_a_length_are_zeros(dev, T, P, N, lengths, at, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,P,N,lengths,at", [(20, 40, 32, (10, 20), 5), (150, 40, 128, (100, 7), 77), (150, 37, 65, (100, 0), 70),
-                                              (3000, 24, 48, (1500, 2990), 1400)])
+                                              (3000, 24, 48, (1500, 2990), 1400), (3000, 70, 48, (2999, 2990), 700)])
 def test_gradients_behind_a_length_are_zeros(dev, T, P, N, lengths, at, dtype):
     """Also where a live value, state or gradient is no number; the other sequence's gradients are what they were."""
     x = inputs(dev, 2, T, 2, P, 1, N, dtype, seed=T)
