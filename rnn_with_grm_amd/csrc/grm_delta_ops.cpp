@@ -190,6 +190,7 @@ Norm check_norm(const Tensor& x, int64_t groups, const OptTensor& weight, const 
   Norm n{x.size(0), x.size(1), dtype_code(x, op, "x"), 0};
   TORCH_CHECK_VALUE(n.C >= 1 && groups >= 1 && n.C % groups == 0, op, ": channels must be a multiple of groups");
   TORCH_CHECK_VALUE(n.C / groups <= 4096, op, ": at most 4096 channels a group");
+  TORCH_CHECK(n.C <= (int64_t{1} << 21) && n.rows <= (int64_t{1} << 31), op, ": at most 2^21 channels and 2^31 rows");
   n.w_dtype = n.dtype;
   auto param = [&](const OptTensor& t, const char* name) {
     if (!has(t)) return;
