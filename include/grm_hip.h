@@ -583,12 +583,15 @@ int grm_hip_selective_step(const grm_hip_selective_args* args, void* hidden, flo
  * elements between sequences and between tokens.  dtype is that of keys, values, queries and
  * hidden; strengths and log_decays have it or are float32, each for itself.
  * lengths: NULL, or int64 [batch] (device), clamped to [0, seq_len]: the tokens from lengths[b] on
- * are not read, leave the state alone, and their rows of every output are zeros.
+ * are not read, leave the state alone, and their rows of every output are zeros, whatever the
+ * tokens before them hold.
  * memory: float32 [batch, heads, value_dim, key_dim], 16-byte aligned, the state before token 0;
  * NULL: zeros.
  * Products run bf16 MFMA on bfloat16 parts of their operands (three of a float32 number); where only a 16-bit output
  * is reached, two parts, which lose 2^-16 of a term.  From a token that holds an infinity or a NaN on, what depends on it is NaN
- * (a value: its column; a query: its row of hidden; all else: the head); earlier tokens are untouched.
+ * (a value: its column; a query: its row of hidden; all else: the head); earlier tokens are untouched.  Numbers of 3.39e38 and
+ * more, which round to an infinity in a bfloat16 part, and finite ones whose products pass float32 may make NaN of all rows of
+ * their 64 tokens too.
  * Limits: key_dim <= 128, heads a multiple of groups, token strides and rows of at most 2^21 elements, batch * heads *
  * ceil(value_dim / 64) and batch * heads * ceil(seq_len / 64) below 2^23 (single token: batch * heads below 2^24).
  */
@@ -631,7 +634,8 @@ int grm_hip_delta_scan_fwd(const grm_hip_delta_args* args, void* hidden, float* 
  * float32 or NULL (zeros).  grad_keys, grad_values, grad_queries (dtype), grad_strengths
  * (strengths_dtype) and grad_log_decays (decays_dtype; may be NULL) are contiguous, grad_memory
  * float32.  Rows behind a sequence's length get zeros.  All sums are taken in a fixed order (no atomics).
- * An infinity or a NaN in the inputs or gradients may reach every gradient of its sequence.
+ * An infinity or a NaN in the inputs or gradients may reach every gradient of its sequence's tokens.
+ * states, grad_memory_out and grad_memory are 16-byte aligned, all else begins at any element.
  * Workspace: grm_hip_delta_scan_bwd_workspace() bytes, 16-byte aligned.
  */
 int64_t grm_hip_delta_scan_bwd_workspace(int64_t batch, int64_t seq_len, int64_t heads, int64_t value_dim,
@@ -644,7 +648,7 @@ int grm_hip_delta_scan_bwd(const grm_hip_delta_args* args, const float* states, 
 /*
  * One token of grm_hip_delta_scan_fwd (seq_len = 1, no lengths): hidden [batch, heads, value_dim],
  * memory_out the state moved by the token.  memory_out may be memory itself (updated in place),
- * but not overlap it otherwise.
+ * but not overlap it otherwise.  Float32 arithmetic, as written: an infinity stays one where it does there.
  */
 int grm_hip_delta_step(const grm_hip_delta_args* args, void* hidden, float* memory_out, void* stream);
 

@@ -12,7 +12,13 @@
 // Numbers.  States, m and everything that reaches them are float32.  Products run on the bf16 MFMA: a float32
 // number is the sum of three bfloat16 parts, a float16 one of two, a bfloat16 one is itself, and the pairs of parts whose
 // product reaches 2^-24 of the whole are multiplied (six of nine; three where one side is bfloat16).  That costs 3/16 to
-// 6/16 of the float32 MFMA's cycles.  What only reaches a 16-bit output takes two parts (2^-16 of a term lost).
+// 6/16 of the float32 MFMA's cycles.
+// What only reaches a 16-bit output takes two parts, and their three larger products: 2^-16 of a term is lost where the output's
+// rounding loses 2^-9 or 2^-12.  These are the state and m as queries read them, W * Q K^T, and X, Y of the keys' and queries'
+// gradients; the state itself and all that a later token reads keep their 24 bits.  With three parts there, bfloat16 outputs differ
+// from a float32 form's by 3.7e-5 of their norm instead of 1.2e-4 (neighbours in the last rounding), the error against float64
+// is the same (1.7e-3; float16 2.1e-4), and calls take longer: 8 x 2048 bf16 tokens x 16 heads of 128 x 128 180 -> 199 us, with
+// gradients 953 -> 988, 32768 tokens 638 -> 681, 5 x 777 x 12 heads float16 63 -> 66.
 #pragma once
 
 #include "selective.h"

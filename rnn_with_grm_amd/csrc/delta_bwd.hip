@@ -48,7 +48,9 @@ __device__ __forceinline__ void scaled_pair(const f32x4& lo, const f32x4& hi, co
                       f32x4{hi[0] * b.x, hi[1] * b.y, hi[2] * b.z, hi[3] * b.w}, out);
 }
 
-// The same where two stages of keys do not fit into LDS (float16 and float32 keys wider than 64): four waves that do all of it.
+// The same where two stages of keys do not fit into LDS (float16 and float32 keys wider than 64): four waves that do all of it, in
+// one time part.  8 x 2048 tokens x 16 heads of 128 x 128 with gradients, whole calls: 1.38 ms in float16, 1.90 in float32 (bfloat16
+// by the other kernel 0.95-0.98); 16384 tokens x 16 heads 5.7 and 8.3 (1.36).
 template <class E, int NK, bool VEC>
 __global__ __launch_bounds__(kThreads) void delta_reverse_kernel(DeltaBwdArgs ba) {
   using raw = typename ET<E>::raw;
@@ -221,8 +223,8 @@ struct MirrorLds {
 // store du.  Two barriers a chunk: du is there, the next state is there.
 // Time parts as the walk's: a first launch (LOCAL) takes all parts but a sequence's first one from their ends to their
 // beginnings, from a zero state and, without rows of values, from the identity's rows; the second each from its own
-// (16384 bf16 tokens x 8 heads of 128 x 128: 1046 us in one part, in nine 127 and 164 with a join of 26-49 between).
-// Bound by the chain, like the walk: 206-224 us for 8 x 2048 bf16 tokens x 16 heads of 128 x 128, 400 MB of states and du written.
+// (16384 bf16 tokens x 8 heads of 128 x 128: 1046 us in one part, in nine 129 and 163 with a join of 29 between).
+// Bound by the chain, like the walk: 207-234 us for 8 x 2048 bf16 tokens x 16 heads of 128 x 128, 400 MB of states and du written.
 template <class E, int NK, bool VEC, bool LOCAL>
 __global__ __launch_bounds__(2 * kThreads, 2) void delta_mirror_kernel(DeltaBwdArgs ba) {
   using raw = typename ET<E>::raw;
@@ -561,7 +563,7 @@ __device__ __forceinline__ U8<E> load_slots(__amdgpu_buffer_rsrc_t r, int off, i
 // One workgroup a chunk of a share of a group's heads.  Two waves a tile of 16 tokens, each with half of the keys: gradients
 // of keys and queries (transposed: a lane has four keys of one token) are summed over the heads in registers.
 // Tiles of the states lie in two stages: while one is worked on the next is split into its parts and the one behind it loaded.
-// 464-518 us for 8 x 2048 bf16 tokens x 16 heads of 128 x 128 (640 MB): one workgroup of two waves a SIMD fits the registers (256
+// 461-521 us for 8 x 2048 bf16 tokens x 16 heads of 128 x 128 (656 MB): one workgroup of two waves a SIMD fits the registers (256
 // each; a third wave spills), so loads, splits and products, 18% of a SIMD's time, take turns at the barriers.  A wave a token
 // tile with all keys took 720; halves that do their products in different order, or keys called for behind the last state
 // tile, gave nothing (543 and 471-554).

@@ -293,7 +293,9 @@ struct WalkLds {
 // One workgroup walks 64 value columns of a head over the whole sequence; a wave holds 16 of them, its state in
 // accumulators (the state's columns never meet: each wave's chain is its own).  Accumulators of K S^T, of m and of the state
 // lie as the next product's operand wants them, so nothing but the inputs passes through LDS.
-// For float16 and float32 keys wider than 64 only, whose stages for delta_pair_kernel do not fit.
+// For float16 and float32 keys wider than 64 only, whose stages for delta_pair_kernel do not fit, and in one time part.  8 x 2048
+// tokens x 16 heads of 128 x 128, whole calls: 316 us in float16, 529 in float32 (bfloat16 by the other kernel 180-230); a
+// sequence of 32768 tokens x 16 heads, which its 32 workgroups walk alone, 3.7 and 5.7 ms (0.66).
 template <class E, int NK, bool VEC>
 __global__ __launch_bounds__(kWalkThreads, 1) void delta_walk_kernel(DeltaArgs a) {
   using raw = typename ET<E>::raw;
@@ -554,8 +556,8 @@ struct LocalLds : PairLds<E, NK> {
 // the weights' product with m, and the stores.  A state's columns never meet, so a state wave's chain is its own;
 // accumulators of K S^T, of m and of the state lie as the next product's operand wants them.  Two barriers a chunk:
 // m is there, the next state is there.
-// Bound by the chain: 8 x 2048 bf16 tokens x 16 heads of 128 x 128 take 140 us, some 7500 cycles a chunk, of which a SIMD's matrix
-// products are 35% and a CU's LDS accesses 45% (four waves that did all of it took 130 us more).
+// Bound by the chain: 8 x 2048 bf16 tokens x 16 heads of 128 x 128 take 140 us, 4.4 a chunk.  Of the busy cycles a SIMD's matrix
+// products are 35% and a CU's LDS accesses 44% (four waves that did all of it took 130 us more).
 // SAVE: the states before every chunk and m are kept for the backward.
 // Sequences in time parts: a first launch (LOCAL) walks all parts but the last side by side and without outputs.  Rows of a
 // state never meet, and without values each passes through a part as a row of a matrix product; so beside the value rows of a
@@ -910,7 +912,7 @@ __global__ __launch_bounds__(2 * kWalkThreads, 2) void delta_pair_kernel(DeltaAr
 // The state before every part but the first: M_{p+1} = M_p F_p + D_p with the parts' maps F and what they leave of a zero
 // state D (of the first, of the sequence's own state: M_1).  A workgroup takes 16 value rows through all parts; each wave
 // holds 32 of the keys, and they hand each other the state's fragments.  The map hangs on no state and is loaded a part
-// ahead.  A chain of loads: 26 us for 7 parts of 16 heads of 128 x 128 (155 with a wave for all keys and no loads ahead).
+// ahead.  A chain of loads: 26-29 us for 7 parts of 16 heads of 128 x 128 (155 with a wave for all keys and no loads ahead).
 // A part behind a sequence's length hands its state on as it is: the product with the identity would make NaN of a row with
 // an infinity, and of numbers that round to one in 16 bits.
 template <int NK>
@@ -993,8 +995,8 @@ __global__ __launch_bounds__(2 * NK) void delta_join_kernel(DeltaArgs a) {
   }
 }
 
-// One token.  LPR lanes share a state row; both dot products with the row are taken from the state as it was, so
-// that it is read and written once: M q = a (M0 q) + u (k.q).  Bound by those bytes: 27.4 us for 64 sequences x 16 heads of
+// One token.  LPR lanes share a state row, which is read and written once: its product with k is summed over them, the row moves
+// by u k in their registers, and its product with q is summed.  Bound by those bytes: 27.7 us for 64 sequences x 16 heads of
 // 128 x 128 (134 MB, 4.9 TB/s, what a large copy reaches).
 template <class E, int LPR>
 __global__ __launch_bounds__(kStepThreads) void delta_step_kernel(DeltaArgs a) {
@@ -1103,7 +1105,9 @@ Work work_of(int64_t B, int64_t T, int64_t H, int64_t P, int64_t N, int dtype, i
 // Time parts of a sequence.  256 CUs hold a workgroup each; a part costs its chunks once more, for the value rows and for
 // the N rows of its map, so parts are taken where they shorten the longest line of chunks behind each other (in quarters of
 // a chunk's time; one of the first walk, with two chains a SIMD, takes five, of the mirror's four, a launch and a join a
-// few chunks).  32768 bf16 tokens x 16 heads of 128 x 128: 1900 us in one part, 650 in eight.
+// few chunks).  32768 bf16 tokens x 16 heads of 128 x 128: 1900 us in one part, 640 in eight.  The prices are those of bfloat16
+// keys of 128, and are taken for every form; where sequences have 13 to 30 chunks (4 x 1000 float32 tokens x 8 heads of 64 x 64 take
+// one part) they have not been set against times of parts.
 int delta_time_parts(int64_t seqs, int64_t P, int64_t N, int64_t C, int dtype, bool mirror, int64_t* part_chunks) {
   *part_chunks = C;
   if ((dtype != GRM_HIP_BF16 && N > 64) || seqs > 4096) return 1;  // (delta_walk_kernel and delta_reverse_kernel take whole sequences)

@@ -1229,7 +1229,9 @@ def cuda_delta_scan(keys: Tensor, values: Tensor, queries: Tensor, strengths: Te
     (hidden [B, T, H, P], memory_out [B, H, P, N] float32).  Differentiable once, backwards, in all but
     lengths (forward-mode derivatives are refused on the GPU).  An infinity or a NaN reaches no earlier
     token's row (on the GPU what depends on it is NaN from its token on: of a value its column, of a query its
-    row, else the head); in the backward it may reach any gradient of its sequence.  Limits: N <= 128."""
+    row, else the head); in the backward it may reach any gradient of its sequence's tokens.  States, and all that a
+    later token reads, are float32; on the GPU operands that only reach a 16-bit result are held to 2^-16
+    (a float32 call takes 24 bits everywhere).  Limits: N <= 128."""
     if values.is_cuda and _run_native("delta_scan", values.device, enabled=enabled, debug_fallback=debug_fallback):
         args = (keys, values, queries, strengths, log_decays, _f32(memory), lengths)
         if _wants_grad(keys, values, queries, strengths, log_decays, memory):
