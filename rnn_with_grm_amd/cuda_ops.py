@@ -1282,6 +1282,8 @@ def _torch_group_norm(x: Tensor, groups: int, weight: Optional[Tensor], bias: Op
     cdt = torch.float64 if x.dtype == torch.float64 else torch.float32
     n = x.to(cdt).unflatten(-1, (groups, C // groups))
     if center:
+        # Twice, as the kernel: the second mean takes out what the first was off by (of equal values nothing is left).
+        n = n - n.mean(-1, keepdim=True)
         n = n - n.mean(-1, keepdim=True)
     y = (n * torch.rsqrt(n.square().mean(-1, keepdim=True) + eps)).flatten(-2)
     if weight is not None:
